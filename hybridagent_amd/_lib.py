@@ -94,6 +94,23 @@ SIGNATURES = {
                                                    _I64, _I64, _I64, _I64, _I64, _I64, _VP, _SZ, _VP]),
     "moe_ffn_block_routing_offsets": (ctypes.c_int, [_I64, _I64, _I64, _I64, _I64, _I64,
                                                      ctypes.POINTER(_SZ), ctypes.POINTER(_SZ)]),
+    "w4a16_layer_norm": (ctypes.c_int, [_VP, _VP, _VP, _VP, _VP, _VP, ctypes.c_int, _I64, _I64, _F32, _VP]),
+    "w4a16_layer_norm_backward_workspace_bytes": (_SZ, [_I64, _I64]),
+    "w4a16_layer_norm_backward": (ctypes.c_int, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, ctypes.c_int, _I64, _I64,
+                                                 _VP, _SZ, _VP]),
+    "w4a16_gated_mlp_workspace_bytes": (_SZ, [_I64, _I64, _I64]),
+    "w4a16_gated_mlp_saved_bytes": (_SZ, [_I64, _I64]),
+    "w4a16_gated_mlp": (ctypes.c_int, [_VP, _VP, _VP, _VP, _VP, _VP, _SZ, _I64, _I64, _I64, _VP, _SZ, _VP]),
+    "w4a16_gated_mlp_backward_workspace_bytes": (_SZ, [_I64, _I64, _I64]),
+    "w4a16_gated_mlp_backward": (ctypes.c_int, [_VP, _VP, _VP, _VP, _VP, _VP, _SZ, _VP, _VP, _VP, _VP, _I64, _I64,
+                                                _I64, _VP, _SZ, _VP]),
+    "w4a16_hybridlink_saved_bytes": (_SZ, [_I64, _I64]),
+    "w4a16_hybridlink_train_workspace_bytes": (_SZ, [_I64, _I64]),
+    "w4a16_hybridlink_train": (ctypes.c_int, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _SZ, _I64, _I64,
+                                              _F32, _VP, _SZ, _VP]),
+    "w4a16_hybridlink_backward_workspace_bytes": (_SZ, [_I64, _I64]),
+    "w4a16_hybridlink_backward": (ctypes.c_int, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _SZ, _VP, _VP, _VP, _VP, _VP, _VP,
+                                                 _VP, _VP, _VP, _I64, _I64, _VP, _SZ, _VP]),
 }
 
 _lib = None
@@ -798,6 +815,206 @@ def ffn_block(residual: torch.Tensor, attn_out: torch.Tensor, post_attn_ln_w: to
     idx = ws[io.value:io.value + 8 * n].view(torch.int64).reshape(M, top_k).clone()
     w = ws[wo.value:wo.value + 4 * n].view(torch.float32).reshape(M, top_k).clone()
     return out, idx, w
+
+
+# ------------------------------------------------------------------ training forms
+
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}  # enum w4a16_dtype
+
+
+def _rows_like(t: torch.Tensor, name: str, like: torch.Tensor) -> torch.Tensor:
+    """t of the shape and type of ``like`` (a gradient of it), as contiguous rows."""
+    if t.shape != like.shape or t.dtype != like.dtype:
+        raise ValueError(f"{name} must be {like.dtype} {list(like.shape)}, got {t.dtype} {list(t.shape)}")
+    return _rows(t.contiguous(), t.shape[-1])
+
+
+def _saved(t: torch.Tensor, nbytes: int) -> torch.Tensor:
+    if t.dtype != torch.uint8 or t.dim() != 1 or not t.is_contiguous() or t.numel() != nbytes:
+        raise ValueError(f"saved must be the uint8 [{nbytes}] that the forward call of this shape returned")
+    return t
+
+
+def _ln_params(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None):
+    dt = _DTYPES.get(x.dtype)
+    if dt is None:
+        raise ValueError(f"x must be bfloat16, float16 or float32, got {x.dtype}")
+    if x.dim() == 0:
+        raise ValueError("x must have a last dimension")
+    H = x.shape[-1]
+    for t, n in ((weight, "weight"), (bias, "bias")):
+        if t is not None and (t.shape != (H,) or t.dtype != x.dtype):
+            raise ValueError(f"{n} must be {x.dtype} [{H}], got {t.dtype} {list(t.shape)}")
+    return dt, H
+
+
+def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, eps: float = 1e-5,
+               return_stats: bool = False):
+    """nn.LayerNorm over the last dimension (hybridlink.py:20,23) of bf16, fp16 or fp32 rows,
+    weight and bias [H] of the same type; statistics in fp32.  With ``return_stats``
+    (y, mean, rstd), float32 of x's leading shape, for ``layer_norm_backward``."""
+    dev = _require_gpu(x, weight, bias)
+    dt, H = _ln_params(x, weight, bias)
+    x2 = _rows(x.contiguous(), H)
+    M = x2.shape[0]
+    y = torch.empty_like(x2)
+    mean = rstd = None
+    if return_stats:
+        mean, rstd = (torch.empty(x.shape[:-1], dtype=torch.float32, device=dev) for _ in range(2))
+    weight = weight.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    _call("w4a16_layer_norm", dev, load().w4a16_layer_norm, _ptr(x2), _ptr(weight), _ptr(bias), _ptr(y), _ptr(mean),
+          _ptr(rstd), dt, M, H, float(eps))
+    y = _like(y, x.shape)
+    return (y, mean, rstd) if return_stats else y
+
+
+def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, mean: torch.Tensor,
+                        rstd: torch.Tensor, bias: bool = True):
+    """(dx, dweight, dbias) of ``layer_norm`` for the gradient ``dy`` of its output; ``mean`` and
+    ``rstd`` are what the forward returned.  dbias is None where ``bias`` is False.  The sums
+    over the rows are taken in fp32 in an order set by the shape."""
+    dev = _require_gpu(dy, x, weight, mean, rstd)
+    dt, H = _ln_params(x, weight, None)
+    dy2 = _rows_like(dy, "dy", x)
+    for t, n in ((mean, "mean"), (rstd, "rstd")):
+        if t.shape != x.shape[:-1] or t.dtype != torch.float32:
+            raise ValueError(f"{n} must be float32 {list(x.shape[:-1])}, got {t.dtype} {list(t.shape)}")
+    x2 = _rows(x.contiguous(), H)
+    weight, mean, rstd = weight.contiguous(), mean.contiguous(), rstd.contiguous()
+    M = x2.shape[0]
+    dx = torch.empty_like(x2)
+    dw = torch.empty_like(weight)
+    db = torch.empty_like(weight) if bias else None
+    lib = load()
+    nbytes = lib.w4a16_layer_norm_backward_workspace_bytes(M, H)
+    ws = _workspace(nbytes, dev)
+    _call("w4a16_layer_norm_backward", dev, lib.w4a16_layer_norm_backward, _ptr(dy2), _ptr(x2), _ptr(weight),
+          _ptr(mean), _ptr(rstd), _ptr(dx), _ptr(dw), _ptr(db), dt, M, H, _ptr(ws), nbytes)
+    return _like(dx, x.shape), dw, db
+
+
+def _mlp_weights(x: torch.Tensor, gate_w: torch.Tensor, up_w: torch.Tensor, down_w: torch.Tensor):
+    if x.dim() == 0:
+        raise ValueError("x must have a last dimension")
+    H = x.shape[-1]
+    gate_w, up_w, down_w = _bf16(gate_w, "gate_w"), _bf16(up_w, "up_w"), _bf16(down_w, "down_w")
+    I = gate_w.shape[0]
+    if gate_w.shape != (I, H) or up_w.shape != (I, H) or down_w.shape != (H, I):
+        raise ValueError(f"the weights must be gate/up [I, {H}] and down [{H}, I], got {list(gate_w.shape)}, "
+                         f"{list(up_w.shape)}, {list(down_w.shape)}")
+    return gate_w, up_w, down_w, H, I
+
+
+def gated_mlp(x: torch.Tensor, gate_w: torch.Tensor, up_w: torch.Tensor, down_w: torch.Tensor,
+              return_saved: bool = False):
+    """The gated feed-forward block (the shared MLP of backends.py:105-108):
+    y = (gelu_tanh(x gate_w^T) * (x up_w^T)) down_w^T on bf16 [..., H], weights in the nn.Linear
+    layout.  With ``return_saved`` (y, saved): what ``gated_mlp_backward`` needs, one uint8 tensor
+    of about 6 bytes per row and column of I."""
+    dev = _require_gpu(x, gate_w, up_w, down_w)
+    x = _bf16(x, "x")
+    gate_w, up_w, down_w, H, I = _mlp_weights(x, gate_w, up_w, down_w)
+    x2 = _rows(x, H)
+    M = x2.shape[0]
+    y = torch.empty_like(x2)
+    lib = load()
+    nbytes = lib.w4a16_gated_mlp_workspace_bytes(M, H, I)
+    ws = _workspace(nbytes, dev)
+    saved, nsaved = None, 0
+    if return_saved:
+        nsaved = lib.w4a16_gated_mlp_saved_bytes(M, I)
+        saved = torch.empty((nsaved,), dtype=torch.uint8, device=dev)
+    _call("w4a16_gated_mlp", dev, lib.w4a16_gated_mlp, _ptr(x2), _ptr(gate_w), _ptr(up_w), _ptr(down_w), _ptr(y),
+          _ptr(saved) if nsaved else None, nsaved, M, H, I, _ptr(ws), nbytes)
+    y = _like(y, x.shape)
+    return (y, saved) if return_saved else y
+
+
+def gated_mlp_backward(dy: torch.Tensor, x: torch.Tensor, gate_w: torch.Tensor, up_w: torch.Tensor,
+                       down_w: torch.Tensor, saved: torch.Tensor, needs=(True, True, True, True)):
+    """(dx, dgate_w, dup_w, ddown_w) of ``gated_mlp`` for the gradient ``dy`` of its output and the
+    ``saved`` of that forward call.  ``needs``: which of the four are wanted; the others are None
+    and not computed (a frozen weight's)."""
+    dev = _require_gpu(dy, x, gate_w, up_w, down_w, saved)
+    x = _bf16(x, "x")
+    gate_w, up_w, down_w, H, I = _mlp_weights(x, gate_w, up_w, down_w)
+    dy2 = _rows_like(dy, "dy", x)
+    x2 = _rows(x, H)
+    M = x2.shape[0]
+    lib = load()
+    nsaved = lib.w4a16_gated_mlp_saved_bytes(M, I)
+    saved = _saved(saved, nsaved)
+    if len(needs) != 4:
+        raise ValueError("needs must say for each of dx, dgate_w, dup_w and ddown_w whether it is wanted")
+    dx, dg, du, dd = (torch.empty_like(t) if n else None for t, n in zip((x2, gate_w, up_w, down_w), needs))
+    nbytes = lib.w4a16_gated_mlp_backward_workspace_bytes(M, H, I)
+    ws = _workspace(nbytes, dev)
+    _call("w4a16_gated_mlp_backward", dev, lib.w4a16_gated_mlp_backward, _ptr(dy2), _ptr(x2), _ptr(gate_w),
+          _ptr(up_w), _ptr(down_w), _ptr(saved), nsaved, _ptr(dx), _ptr(dg), _ptr(du), _ptr(dd), M, H, I, _ptr(ws),
+          nbytes)
+    return None if dx is None else _like(dx, x.shape), dg, du, dd
+
+
+def _link_params(h: torch.Tensor, params):
+    names = ("pre_ln weight", "pre_ln bias", "proj1 weight", "proj1 bias", "proj2 weight", "proj2 bias",
+             "post_ln weight", "post_ln bias")
+    if h.dim() == 0:
+        raise ValueError("h must have a last dimension")
+    H = h.shape[-1]
+    params = tuple(_bf16(p, n) for p, n in zip(params, names))
+    for i, p in enumerate(params):
+        want = (H, H) if i in (2, 4) else (H,)
+        if p.shape != want:
+            raise ValueError(f"{names[i]} must be {list(want)}, got {list(p.shape)}")
+    return params, H
+
+
+def hybridlink_train(h: torch.Tensor, ln1_w: torch.Tensor, ln1_b: torch.Tensor, p1_w: torch.Tensor,
+                     p1_b: torch.Tensor, p2_w: torch.Tensor, p2_b: torch.Tensor, ln2_w: torch.Tensor,
+                     ln2_b: torch.Tensor, eps: float = 1e-5):
+    """``hybridlink`` (hybridlink.py:17-28) for training -> (out, saved): ``saved`` is what
+    ``hybridlink_backward`` needs, one uint8 tensor of about 8 bytes per element of h.  Each
+    intermediate is rounded to bf16 once, from fp32 (``hybridlink`` rounds where the torch
+    modules do)."""
+    dev = _require_gpu(h, ln1_w, ln1_b, p1_w, p1_b, p2_w, p2_b, ln2_w, ln2_b)
+    h = _bf16(h, "h")
+    params, H = _link_params(h, (ln1_w, ln1_b, p1_w, p1_b, p2_w, p2_b, ln2_w, ln2_b))
+    h2 = _rows(h, H)
+    B = h2.shape[0]
+    out = torch.empty_like(h2)
+    lib = load()
+    nsaved = lib.w4a16_hybridlink_saved_bytes(B, H)
+    saved = torch.empty((nsaved,), dtype=torch.uint8, device=dev)
+    nbytes = lib.w4a16_hybridlink_train_workspace_bytes(B, H)
+    ws = _workspace(nbytes, dev)
+    _call("w4a16_hybridlink_train", dev, lib.w4a16_hybridlink_train, _ptr(h2), *[_ptr(p) for p in params], _ptr(out),
+          _ptr(saved), nsaved, B, H, float(eps), _ptr(ws), nbytes)
+    return _like(out, h.shape), saved
+
+
+def hybridlink_backward(dout: torch.Tensor, h: torch.Tensor, ln1_w: torch.Tensor, ln1_b: torch.Tensor,
+                        p1_w: torch.Tensor, p1_b: torch.Tensor, p2_w: torch.Tensor, p2_b: torch.Tensor,
+                        ln2_w: torch.Tensor, ln2_b: torch.Tensor, saved: torch.Tensor):
+    """(dh, then the gradients of the eight parameters in their order) of ``hybridlink_train`` for
+    the gradient ``dout`` of its output and the ``saved`` of that forward call."""
+    dev = _require_gpu(dout, h, ln1_w, ln1_b, p1_w, p1_b, p2_w, p2_b, ln2_w, ln2_b, saved)
+    h = _bf16(h, "h")
+    params, H = _link_params(h, (ln1_w, ln1_b, p1_w, p1_b, p2_w, p2_b, ln2_w, ln2_b))
+    d2 = _rows_like(dout, "dout", h)
+    h2 = _rows(h, H)
+    B = h2.shape[0]
+    lib = load()
+    nsaved = lib.w4a16_hybridlink_saved_bytes(B, H)
+    saved = _saved(saved, nsaved)
+    dh = torch.empty_like(h2)
+    grads = tuple(torch.empty_like(p) for p in params)
+    nbytes = lib.w4a16_hybridlink_backward_workspace_bytes(B, H)
+    ws = _workspace(nbytes, dev)
+    _call("w4a16_hybridlink_backward", dev, lib.w4a16_hybridlink_backward, _ptr(d2), _ptr(h2), _ptr(params[0]),
+          _ptr(params[2]), _ptr(params[4]), _ptr(params[6]), _ptr(saved), nsaved, _ptr(dh),
+          *[_ptr(g) for g in grads], B, H, _ptr(ws), nbytes)
+    return (_like(dh, h.shape), *grads)
 
 
 class MoEStages:

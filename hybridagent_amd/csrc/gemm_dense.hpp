@@ -1,0 +1,432 @@
+// Dense bf16 GEMM of the training forms (gated_mlp, HybridLink): one kernel
+// template for the three products that a linear y = x W^T takes part in,
+//
+//   kDgNT  y  = x W^T    both operands with k contiguous
+//   kDgNN  dx = dy W     the rows with k contiguous, the weights [k][n]
+//   kDgTN  dW = dy^T x   both operands [k][.], k the tokens
+//
+// as C[m][n] = sum_k A(m, k) B(n, k) with fp32 accumulation on
+// v_mfma_f32_16x16x32_bf16, B the first operand, so that a lane ends with
+// four consecutive n of one row m.
+//
+// A workgroup of four wavefronts (2 x 2) owns a tile of 32 MI rows x 32 NI
+// columns, a wavefront 16 MI x 16 NI of it.  k advances in stages of 32
+// through a ring of dg_stages LDS slots filled by direct 16-byte global -> LDS
+// loads; the fragments of stage t + 1 are read while stage t is multiplied,
+// so that a stage has one barrier and its loads have two to three stages to
+// land.  Stages past the end are issued with an empty buffer descriptor, which
+// reads nothing, so that every wait counts the same loads.
+//
+// LDS formats of a stage's operand tile, both free of bank conflicts:
+//   rows  (k contiguous)  [rows][32 k], 64 bytes a row, the 16-byte chunks
+//         XOR-swizzled by (row / 4) % 4: a fragment is 16 rows x 64 bytes, one
+//         ds_read_b128 per lane;
+//   cols  ([k][.])        [32 k][cols], the 32-byte units of a row
+//         XOR-swizzled by bits of k (dg_swz): a fragment of 16 columns x 32 k
+//         is two transposing reads (ds_read_b64_tr_b16), which take 4 k x 16
+//         columns per 16 lanes and give each lane the 4 k of its column.
+// The swizzle is applied to the load's source address (a direct load's LDS
+// addresses are consecutive).
+#pragma once
+#include <algorithm>
+#include <type_traits>
+
+#include "common.hpp"
+#include "launch.hpp"
+#include "lds_pipe.hpp"
+#include "rules.hpp"
+
+namespace w4a16 {
+
+constexpr int kDgThreads = 256;
+constexpr int kDgKT = 32;     // k per stage
+
+// LDS slots of a tile: four, or three where two workgroups then share a CU
+constexpr int dg_stages(int mi, int ni) { return mi * ni >= 24 && mi * ni <= 36 ? 3 : 4; }
+constexpr int kDgGroupM = 4;  // row tiles that run with a column tile
+constexpr int dg_bm(int mi) { return 32 * mi; }
+constexpr int dg_bn(int epi, int ni) { return epi == kDgGateUp ? 16 * ni : 32 * ni; }
+
+typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4_t;
+
+// s_waitcnt vmcnt(N), nothing else
+template <int N>
+__device__ __forceinline__ void dg_wait_vm() {
+  __builtin_amdgcn_s_waitcnt(px_vm_wait(N));
+}
+
+// A transposing LDS read: of 4 k x 16 columns per 16 lanes (lane i's address:
+// row i / 4, columns 4 (i % 4) .. + 3) each lane gets the 4 k of column i.  The
+// restrict argument gives the read alias information: without any the compiler
+// waits for every direct LDS load in flight before it.
+typedef __attribute__((address_space(3))) bf16x4_t lds_bf16x4_t;
+__device__ __forceinline__ bf16x4_t dg_tr_read(lds_bf16x4_t* __restrict__ p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4bf16(p);
+}
+
+// the swizzle of row k of a cols tile of W columns: which 32-byte unit of an
+// aligned group goes where.  A transposing read's first 32 lanes take rows 0 ..
+// 3 and 8 .. 11 (+ 4): eight different units of the 256-byte bank window.
+template <int W>
+__device__ __forceinline__ int dg_swz(int k) {
+  if constexpr (W % 128 == 0)
+    return (k & 3) | ((k >> 1) & 4);
+  else  // rows are 128 bytes apart modulo the window
+    return ((k >> 1) & 1) | ((k >> 2) & 2);
+}
+
+// One operand's side of a tile: W rows (or columns), F fragments of 16 per
+// wavefront.  COLS: the cols format.  GU (rows format): the first half of a
+// wavefront's fragments come from p, the second half, same rows, from p2.
+template <bool COLS, bool GU, int F>
+struct DgOperand {
+  static constexpr int W = 32 * F;
+  static constexpr int kBytes = W * kDgKT * 2;
+  static constexpr int kLoads = F / 2;  // per wavefront and stage
+  int voff[kLoads];                     // a lane's source bytes, per load
+  int foff[COLS ? F : 1];               // its fragment bytes in a stage
+
+  // first: the tile's first row, n: rows there are (rows past it repeat the last)
+  __device__ __forceinline__ void init(int first, int n, int64_t ld) {
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+      const int ins = wave + 4 * j;
+      if constexpr (COLS) {
+        const int pos = 1024 * ins + 16 * lane;
+        const int k = pos / (2 * W), s = (pos - k * 2 * W) >> 4;
+        const int unit = (s >> 1) ^ dg_swz<W>(k);
+        const int col = min(16 * unit + 8 * (s & 1), n - first - 8);
+        voff[j] = k * (int)ld * 2 + 2 * col;
+      } else {
+        int r = 16 * ins + (lane >> 2);
+        const int chunk = (lane & 3) ^ ((lane >> 4) & 3);
+        if constexpr (GU) {
+          // tile rows 16 F w + [0, 8 F): rows 8 F w + .. of p, [8 F, 16 F): of p2
+          const int w = r / (16 * F), in = r - 16 * F * w;
+          r = 8 * F * w + (in >= 8 * F ? in - 8 * F : in);
+        }
+        voff[j] = min(r, n - first - 1) * (int)ld * 2 + 16 * chunk;
+      }
+    }
+  }
+  // w: the wavefront's half of the tile
+  __device__ __forceinline__ void init_frag(int w) {
+    const int lane = threadIdx.x & 63;
+    if constexpr (COLS) {
+      const int k = 8 * (lane >> 4) + ((lane & 15) >> 2);
+#pragma unroll
+      for (int f = 0; f < F; ++f) foff[f] = k * 2 * W + 32 * ((w * F + f) ^ dg_swz<W>(k)) + 8 * (lane & 3);
+    } else {
+      foff[0] = 1024 * F * w + (lane & 15) * 64 + 16 * ((lane >> 4) ^ ((lane >> 2) & 3));
+    }
+  }
+  static __device__ __forceinline__ bool second(int j) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    return (wave + 4 * j) % F >= F / 2;
+  }
+  __device__ __forceinline__ u32x4_t frag(const unsigned char* st, int f) const {
+    if constexpr (COLS) {
+      const unsigned char* p = st + foff[f];
+      const bf16x4_t lo = dg_tr_read((lds_bf16x4_t*)p);
+      const bf16x4_t hi = dg_tr_read((lds_bf16x4_t*)(p + 8 * W));
+      const bf16x8_t v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+      return __builtin_bit_cast(u32x4_t, v);
+    } else {
+      return *reinterpret_cast<const u32x4_t*>(st + foff[0] + 1024 * f);
+    }
+  }
+};
+
+// ---- epilogues on four consecutive columns n .. n + 3 of row m
+
+__device__ __forceinline__ void dg_ld4(const uint16_t* p, float v[4]) {
+  const uint2 u = *reinterpret_cast<const uint2*>(p);
+  v[0] = bf16_bits_to_f32(u.x & 0xFFFFu);
+  v[1] = bf16_bits_to_f32(u.x >> 16);
+  v[2] = bf16_bits_to_f32(u.y & 0xFFFFu);
+  v[3] = bf16_bits_to_f32(u.y >> 16);
+}
+__device__ __forceinline__ void dg_st4(uint16_t* p, const float v[4]) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+}
+
+// d/dx gelu_tanh = s + x s (1 - s) 2 u', s = 1 / (1 + exp(-2 u)),
+// u' = sqrt(2/pi) (1 + 3 0.044715 x^2); beyond |x| = 12 it is 0 or 1 (the
+// comparisons leave a NaN as it is).
+__device__ __forceinline__ void gelu_tanh_and_slope(float x, float* act, float* slope) {
+  const float xc = x < -12.f ? -12.f : (x > 12.f ? 12.f : x);
+  const float x2 = xc * xc;
+  const float u = 0.7978845608028654f * xc * (1.0f + 0.044715f * x2);
+  const float s = __fdividef(1.0f, 1.0f + __expf(-2.0f * u));
+  *act = x * s;
+  *slope = s + xc * s * (1.0f - s) * 1.5957691216057308f * (1.0f + 0.134145f * x2);
+}
+__device__ __forceinline__ float gelu_erf_f32(float x) { return 0.5f * x * (1.0f + erff(x * 0.70710678118654752f)); }
+// d/dx gelu_erf = Phi(x) + x phi(x)
+__device__ __forceinline__ float gelu_erf_slope(float x) {
+  return 0.5f * (1.0f + erff(x * 0.70710678118654752f)) + x * (0.3989422804014327f * __expf(-0.5f * x * x));
+}
+
+// v: the sums (v2: kDgGateUp's up sums); o: the element's offset in row-major [M, N]
+template <int EPI>
+__device__ __forceinline__ void dg_finish(const DgEpilogue& e, int64_t o, int n, const float v[4], const float v2[4]) {
+  float r[4], s[4];
+  if constexpr (EPI == kDgPlain) {
+    dg_st4(e.out + o, v);
+  } else if constexpr (EPI == kDgGateUp) {
+    // h = gelu_tanh(a) b from the sums themselves, rounded once; a and b are
+    // rounded for the backward pass alone
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = gelu_tanh_f32(v[i]) * v2[i];
+    dg_st4(e.out + o, r);
+    if (e.out2 != nullptr) {
+      dg_st4(e.out2 + o, v);
+      dg_st4(e.out3 + o, v2);
+    }
+  } else if constexpr (EPI == kDgGateUpBack) {
+    float a[4], b[4];
+    dg_ld4(e.in + o, a);
+    dg_ld4(e.in2 + o, b);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float act, slope;
+      gelu_tanh_and_slope(a[i], &act, &slope);
+      r[i] = v[i] * b[i] * slope;
+      s[i] = v[i] * act;
+    }
+    dg_st4(e.out + o, r);
+    dg_st4(e.out2 + o, s);
+  } else if constexpr (EPI == kDgBiasGelu) {
+    dg_ld4(e.bias + n, s);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s[i] += v[i];
+      r[i] = gelu_erf_f32(s[i]);
+    }
+    dg_st4(e.out + o, r);
+    dg_st4(e.out2 + o, s);
+  } else if constexpr (EPI == kDgBiasResidual) {
+    float b[4];
+    dg_ld4(e.bias + n, b);
+    dg_ld4(e.in + o, s);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = s[i] + (v[i] + b[i]);
+    dg_st4(e.out + o, r);
+  } else if constexpr (EPI == kDgGeluBack) {
+    dg_ld4(e.in + o, s);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = v[i] * gelu_erf_slope(s[i]);
+    dg_st4(e.out + o, r);
+  }
+}
+
+// the workgroup's item: every XCD (workgroups go round robin) has a run of
+// consecutive ones; -1 past them
+__device__ __forceinline__ int dg_item(int total) {
+  const int per = (total + 7) >> 3, x = (int)(blockIdx.x & 7), i = (int)(blockIdx.x >> 3);
+  return i < per && x * per + i < total ? x * per + i : -1;
+}
+
+template <int LAYOUT, int EPI, int MI, int NI>
+__global__ __launch_bounds__(kDgThreads, MI * NI > 36 ? 1 : 2) void k_gemm_dense(DgArgs a) {
+  constexpr bool AC = LAYOUT == kDgTN, BC = LAYOUT != kDgNT;
+  constexpr bool GU = EPI == kDgGateUp;
+  using OA = DgOperand<AC, false, MI>;
+  using OB = DgOperand<BC, GU, NI>;
+  constexpr int kStage = OA::kBytes + OB::kBytes;
+  constexpr int kStages = dg_stages(MI, NI);
+  constexpr int kLoads = OA::kLoads + OB::kLoads;
+  constexpr int BM = dg_bm(MI), BN = dg_bn(EPI, NI);
+  extern __shared__ __align__(16) unsigned char smem[];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+
+  // the tile: kDgGroupM row tiles run with each column tile
+  int item = dg_item(a.tiles * a.ksplit);
+  if (item < 0) return;
+  const int split = item / a.tiles;
+  item -= split * a.tiles;
+  int pi = 0;
+  while (pi + 1 < a.nprob && item >= a.prob[pi + 1].tile0) ++pi;
+  const DgProblem p = a.prob[pi];
+  item -= p.tile0;
+  const int n_mt = (p.M + BM - 1) / BM, n_nt = (p.N + BN - 1) / BN;
+  const int grp = item / (kDgGroupM * n_nt);
+  const int rem = item - grp * kDgGroupM * n_nt;
+  const int gm = min(kDgGroupM, n_mt - grp * kDgGroupM);
+  const int nt = rem / gm;
+  const int m0 = (grp * kDgGroupM + rem - nt * gm) * BM, n0 = nt * BN;
+  const int per = (a.nk + a.ksplit - 1) / a.ksplit;
+  const int t0 = split * per, t1 = min(a.nk, t0 + per);
+
+  OA oa;
+  OB ob;
+  oa.init(m0, p.M, p.lda);
+  ob.init(n0, p.N, p.ldb);
+  oa.init_frag(wave >> 1);
+  ob.init_frag(wave & 1);
+
+  // load j (of the wavefront's kLoads) of stage t into a slot.  The descriptor
+  // is empty past the range; cols: it starts at the stage's first k and ends
+  // with row K - 1, so that rows past K read as zero.  Rows: stages of the
+  // second pair (t >= nk1) follow the first's.
+  auto issue = [&](int t, unsigned char* slot, int j) {
+    const bool two = LAYOUT == kDgNN && t >= a.nk1;
+    const int tt = two ? t - a.nk1 : t;
+    const bool any = t < t1;
+    const int left = min(kDgKT, a.K - tt * kDgKT);
+    if (j < OA::kLoads) {
+      const uint16_t* b = two ? p.A2 : p.A;
+      const auto r = AC ? make_rsrc(b + (int64_t)tt * kDgKT * p.lda + m0, any ? (uint32_t)(left * p.lda - m0) * 2u : 0u)
+                        : make_rsrc(b + (int64_t)m0 * p.lda, any ? (uint32_t)(min(p.M - m0, BM) * p.lda) * 2u : 0u);
+      px_dma16(r, oa.voff[j], AC ? 0 : tt * (kDgKT * 2), slot + (wave + 4 * j) * 1024);
+    } else {
+      const int i = j - OA::kLoads;
+      const uint16_t* b = two || (GU && OB::second(i)) ? p.B2 : p.B;
+      const auto r = BC ? make_rsrc(b + (int64_t)tt * kDgKT * p.ldb + n0, any ? (uint32_t)(left * p.ldb - n0) * 2u : 0u)
+                        : make_rsrc(b + (int64_t)n0 * p.ldb, any ? (uint32_t)(min(p.N - n0, BN) * p.ldb) * 2u : 0u);
+      px_dma16(r, ob.voff[i], BC ? 0 : tt * (kDgKT * 2), slot + OA::kBytes + (wave + 4 * i) * 1024);
+    }
+  };
+
+  f32x4_t acc[MI][NI];
+#pragma unroll
+  for (int m = 0; m < MI; ++m)
+#pragma unroll
+    for (int n = 0; n < NI; ++n) acc[m][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  u32x4_t fa[MI], fb[NI];
+
+#pragma unroll
+  for (int s = 0; s < kStages; ++s)
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) issue(t0 + s, smem + s * kStage, j);
+  dg_wait_vm<(kStages - 1) * kLoads>();
+  px_barrier();
+#pragma unroll
+  for (int n = 0; n < NI; ++n) fb[n] = ob.frag(smem + OA::kBytes, n);
+#pragma unroll
+  for (int m = 0; m < MI; ++m) fa[m] = oa.frag(smem, m);
+
+  // Stage t, its fragments at hand: after the first row of fragments' MFMAs
+  // the wavefronts meet (stage t + 1 has landed, slot t is read), then slot t
+  // is refilled with stage t + kStages and every fragment register takes its
+  // fragment of stage t + 1 right after its last MFMA.  The last two rows go
+  // column by column, so that a column's fragment has 2 (NI - 1) MFMAs to
+  // arrive.
+  int slot = 0;
+  for (int t = t0; t < t1; ++t) {
+    const int ns = slot == kStages - 1 ? 0 : slot + 1;
+    unsigned char* refill = smem + slot * kStage;
+    const unsigned char* st = smem + ns * kStage;
+#pragma unroll
+    for (int n = 0; n < NI; ++n) acc[0][n] = mfma16(fb[n], fa[0], acc[0][n]);
+    __builtin_amdgcn_sched_barrier(0);
+    dg_wait_vm<(kStages - 2) * kLoads>();
+    px_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    if (MI > 2) fa[0] = oa.frag(st, 0);
+#pragma unroll
+    for (int m = 1; m < MI - 2; ++m) {
+#pragma unroll
+      for (int n = 0; n < NI; ++n) acc[m][n] = mfma16(fb[n], fa[m], acc[m][n]);
+      fa[m] = oa.frag(st, m);
+#pragma unroll
+      for (int j = (m - 1) * kLoads / (MI > 3 ? MI - 3 : 1); j < m * kLoads / (MI > 3 ? MI - 3 : 1); ++j)
+        issue(t + kStages, refill, j);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (MI <= 3) {
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) issue(t + kStages, refill, j);
+    }
+#pragma unroll
+    for (int n = 0; n < NI; ++n) {
+      if (MI > 2) acc[MI - 2][n] = mfma16(fb[n], fa[MI - 2], acc[MI - 2][n]);
+      acc[MI - 1][n] = mfma16(fb[n], fa[MI - 1], acc[MI - 1][n]);
+      fb[n] = ob.frag(st + OA::kBytes, n);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    fa[MI - 2] = oa.frag(st, MI - 2);
+    fa[MI - 1] = oa.frag(st, MI - 1);
+    slot = ns;
+  }
+  dg_wait_vm<0>();  // no load may land in another workgroup's LDS
+
+  // epilogue: lane l holds columns 4 (l / 16) .. + 3 of row l % 16 of each 16 x 16 tile
+  constexpr int NO = GU ? NI / 2 : NI;
+#pragma unroll
+  for (int m = 0; m < MI; ++m) {
+    const int row = m0 + 16 * (MI * (wave >> 1) + m) + (lane & 15);
+    if (row >= p.M) continue;
+#pragma unroll
+    for (int n = 0; n < NO; ++n) {
+      const int col = n0 + 16 * (NO * (wave & 1) + n) + 4 * (lane >> 4);
+      if (col >= p.N) continue;
+      const int64_t o = (int64_t)row * p.N + col;
+      float v[4], v2[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] = acc[m][n][i];
+        v2[i] = acc[m][GU ? n + NO : n][i];
+      }
+      if (a.ksplit > 1) {
+        float* q = a.part + split * a.plane + p.part0 + o;
+        *reinterpret_cast<float4*>(q) = make_float4(v[0], v[1], v[2], v[3]);
+        if (GU) *reinterpret_cast<float4*>(q + (int64_t)p.M * p.N) = make_float4(v2[0], v2[1], v2[2], v2[3]);
+      } else {
+        dg_finish<EPI>(p.e, o, col, v, v2);
+      }
+    }
+  }
+}
+
+// The sums of a split launch: the splits' partial sums in order, then the
+// epilogue; a thread has four columns of one row.
+template <int EPI>
+__global__ __launch_bounds__(256) void k_gemm_dense_join(DgArgs a) {
+  const DgProblem p = a.prob[blockIdx.y];
+  const int64_t n4 = (int64_t)p.M * p.N / 4;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n4) return;
+  const int64_t o = 4 * i;
+  const float* q = a.part + p.part0 + o;
+  float v[4] = {0.f, 0.f, 0.f, 0.f}, v2[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < a.ksplit; ++s) {
+    const float4 t = *reinterpret_cast<const float4*>(q + s * a.plane);
+    v[0] += t.x; v[1] += t.y; v[2] += t.z; v[3] += t.w;
+    if (EPI == kDgGateUp) {
+      const float4 u = *reinterpret_cast<const float4*>(q + s * a.plane + (int64_t)p.M * p.N);
+      v2[0] += u.x; v2[1] += u.y; v2[2] += u.z; v2[3] += u.w;
+    }
+  }
+  dg_finish<EPI>(p.e, o, (int)(o % p.N), v, v2);
+}
+
+template <int LAYOUT, int EPI, int MI, int NI>
+hipError_t dg_launch(const DgArgs& a, hipStream_t s) {
+  constexpr int lds = dg_stages(MI, NI) * (32 * MI + 32 * NI) * kDgKT * 2;
+  static_assert(lds <= 160 * 1024, "LDS of a CU");
+  const int64_t total = (int64_t)a.tiles * a.ksplit;
+  const int grid = (int)(8 * ((total + 7) / 8));
+  hipLaunchKernelGGL((k_gemm_dense<LAYOUT, EPI, MI, NI>), dim3(grid), dim3(kDgThreads), lds, s, a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || a.ksplit == 1) return e;
+  int64_t most = 0;
+  for (int i = 0; i < a.nprob; ++i) most = std::max(most, (int64_t)a.prob[i].M * a.prob[i].N / 4);
+  hipLaunchKernelGGL(k_gemm_dense_join<EPI>, dim3((unsigned)((most + 255) / 256), a.nprob), dim3(256), 0, s, a);
+  return hipGetLastError();
+}
+
+// the launch with the tile that `a` was planned for
+template <int LAYOUT, int EPI>
+hipError_t dg_launch_tile(const DgArgs& a, hipStream_t s) {
+#define W4A16_DG(MI_, NI_) \
+  if (a.mi == MI_ && a.ni == NI_) return dg_launch<LAYOUT, EPI, MI_, NI_>(a, s);
+  W4A16_DG_TILES(W4A16_DG)
+#undef W4A16_DG
+  return hipErrorInvalidValue;
+}
+
+}  // namespace w4a16

@@ -1,0 +1,465 @@
+// Layer norm and its backward pass for rows of bf16, fp16 or fp32 (weights in
+// the rows' type, everything computed in fp32):
+//   mean = sum x / H, rstd = 1 / sqrt(sum (x - mean)^2 / H + eps)
+//   y = (x - mean) rstd w + b
+//   xh = (x - mean) rstd, g = dy w
+//   dx = rstd (g - sum g / H - xh sum(g xh) / H) (+ add)
+//   dw = sum over rows of dy xh, db = sum over rows of dy
+// The variance is of the deviations from the mean (a second pass over the row
+// in registers), not a difference of squares.
+//
+// A row is held in registers by TPR threads, EPT elements each: a wavefront
+// (no LDS, no barrier) or a workgroup.  Loads are 16 bytes per lane where
+// rows and pointers allow it (VEC elements), else one element.  The weights
+// are loaded once per thread and kept across its rows.
+//
+// Bound: HBM.  The column sums of the backward pass are kept in registers
+// across the rows of a thread, added over a workgroup's wavefronts in LDS and
+// written once per workgroup (kLnPartials at most); a second launch adds those
+// in order, so that a result depends on the shape alone.
+#include <algorithm>
+#include <type_traits>
+
+#include "common.hpp"
+#include "launch.hpp"
+
+namespace w4a16 {
+
+namespace {
+
+template <typename T>
+struct LnType;
+template <>
+struct LnType<__bf16> {
+  static __device__ __forceinline__ float load(uint32_t bits) { return bf16_bits_to_f32(bits); }
+};
+template <>
+struct LnType<_Float16> {
+  static __device__ __forceinline__ float load(uint32_t bits) {
+    return (float)__builtin_bit_cast(_Float16, (uint16_t)bits);
+  }
+};
+
+// a thread's EPT elements of a row as they lie in memory: chunk q of thread t
+// of TPR is elements (t + TPR q) VEC ..; those past the row read as zero and
+// are not stored (the row's buffer descriptor ends with it)
+template <typename T, int VEC, int EPT, int TPR>
+struct LnRaw {
+  static constexpr int NQ = EPT / VEC;
+  static constexpr int kChunk = VEC * (int)sizeof(T);
+  static constexpr int kWords = kChunk / 4 > 0 ? kChunk / 4 : 1;
+  uint32_t w[NQ][kWords];
+
+  __device__ __forceinline__ void load(const void* row, int t, int H) {
+    const auto r = make_rsrc(row, (uint32_t)(H * (int)sizeof(T)));
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      const int o = t * kChunk + TPR * q * kChunk;
+      if constexpr (VEC > 1) {
+        const u32x4_t v = buf_ld16(r, o, 0);
+        w[q][0] = v.x;
+        w[q][1] = v.y;
+        w[q][2] = v.z;
+        w[q][3] = v.w;
+      } else if constexpr (sizeof(T) == 4) {
+        w[q][0] = __builtin_amdgcn_raw_buffer_load_b32(r, o, 0, 0);
+      } else {
+        w[q][0] = buf_ld_u16(r, o);
+      }
+    }
+  }
+  __device__ __forceinline__ float get(int q, int e) const {
+    if constexpr (sizeof(T) == 4)
+      return __uint_as_float(w[q][e]);
+    else
+      return LnType<T>::load((e & 1) ? w[q][e >> 1] >> 16 : w[q][e >> 1] & 0xFFFFu);
+  }
+  // what is computed from the values is computed again after this, not kept
+  __device__ __forceinline__ void forget() {
+#pragma unroll
+    for (int q = 0; q < NQ; ++q)
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) w[q][i] = opaque(w[q][i]);
+  }
+};
+
+// chunk q of a row from VEC values, rounded to T
+template <typename T, int VEC, int TPR>
+__device__ __forceinline__ void ln_store(__amdgpu_buffer_rsrc_t r, int t, int q, const float* v) {
+  constexpr int kChunk = VEC * (int)sizeof(T);
+  const int o = t * kChunk + TPR * q * kChunk;
+  if constexpr (VEC > 1) {
+    typedef T vec_t __attribute__((ext_vector_type(VEC)));
+    vec_t u;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) u[i] = (T)v[i];
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, u), r, o, 0, 0);
+  } else if constexpr (sizeof(T) == 4) {
+    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v[0]), r, o, 0, 0);
+  } else {
+    __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, (T)v[0]), r, o, 0, 0);
+  }
+}
+
+// sums of N values over the TPR threads of a row, in a fixed order
+template <int TPR, int N>
+__device__ __forceinline__ void ln_sum(float (&v)[N], float* part) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = wave_sum_f32(v[i]);
+  if constexpr (TPR > 64) {
+    constexpr int W = TPR / 64;
+    const int w = threadIdx.x >> 6;
+    __syncthreads();  // the last sums have been read
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) part[i * W + w] = v[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float t = part[i * W];
+#pragma unroll
+      for (int j = 1; j < W; ++j) t += part[i * W + j];
+      v[i] = t;
+    }
+  }
+}
+
+constexpr int ln_threads(int tpr) { return 256; }
+// backward: a wavefront's rows in workgroups of eight of them
+constexpr int ln_back_threads(int tpr) { return tpr > 64 ? tpr : 512; }
+// the thread's row of the workgroup's (wavefront-uniform)
+template <int TPR>
+__device__ __forceinline__ int ln_row_of() {
+  return TPR > 64 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+}
+
+}  // namespace
+
+template <typename T, int VEC, int EPT, int TPR>
+__global__ __launch_bounds__(ln_threads(TPR)) void k_ln_forward(LnArgs a) {
+  using Raw = LnRaw<T, VEC, EPT, TPR>;
+  __shared__ float part[TPR > 64 ? TPR / 64 : 1];
+  constexpr int RPB = ln_threads(TPR) / TPR;  // rows per workgroup
+  const int t = threadIdx.x % TPR;
+  const int H = a.H, nchunks = H / VEC;
+  const float fh = (float)H;
+  int64_t row = (int64_t)blockIdx.x * RPB + ln_row_of<TPR>();
+  if (row >= a.M) return;  // (a workgroup per row: all of it)
+  Raw x, w, b;
+  // the row first: its statistics wait for nothing else
+  x.load(static_cast<const T*>(a.x) + row * H, t, H);
+  w.load(a.w, t, H);
+  b.load(a.b != nullptr ? a.b : a.w, t, a.b != nullptr ? H : 0);
+  for (;;) {
+    float s[1] = {0.f};
+#pragma unroll
+    for (int q = 0; q < Raw::NQ; ++q)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) s[0] += x.get(q, e);
+    ln_sum<TPR>(s, part);
+    const float mean = s[0] / fh;
+    float d2[1] = {0.f};
+    x.forget();
+#pragma unroll
+    for (int q = 0; q < Raw::NQ; ++q) {
+      const bool in = t + TPR * q < nchunks;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float d = in ? x.get(q, e) - mean : 0.f;
+        d2[0] = __builtin_fmaf(d, d, d2[0]);
+      }
+    }
+    ln_sum<TPR>(d2, part);
+    const float rstd = 1.0f / sqrtf(d2[0] / fh + a.eps);
+    x.forget();
+    const auto yr = make_rsrc(static_cast<T*>(a.y) + row * H, (uint32_t)(H * (int)sizeof(T)));
+#pragma unroll
+    for (int q = 0; q < Raw::NQ; ++q) {
+      float o[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) o[e] = __builtin_fmaf((x.get(q, e) - mean) * rstd, w.get(q, e), b.get(q, e));
+      ln_store<T, VEC, TPR>(yr, t, q, o);
+    }
+    if (a.mean != nullptr && t == 0) {
+      a.mean[row] = mean;
+      a.rstd[row] = rstd;
+    }
+    row += (int64_t)gridDim.x * RPB;
+    if (row >= a.M) break;
+    x.load(static_cast<const T*>(a.x) + row * H, t, H);
+    w.forget();
+    b.forget();
+  }
+}
+
+template <typename T, int VEC, int EPT, int TPR, bool ADD>
+__global__ __launch_bounds__(ln_back_threads(TPR)) void k_ln_backward(LnArgs a) {
+  using Raw = LnRaw<T, VEC, EPT, TPR>;
+  constexpr int RPB = ln_back_threads(TPR) / TPR;
+  extern __shared__ float smem[];  // TPR > 64: the rows' sums; else [2][H] of the column sums
+  const int t = threadIdx.x % TPR;
+  const int H = a.H;
+  const float fh = (float)H;
+  Raw w;
+  w.load(a.w, t, H);
+  float dw[EPT], db[EPT];
+#pragma unroll
+  for (int i = 0; i < EPT; ++i) dw[i] = db[i] = 0.f;
+  for (int64_t row = (int64_t)blockIdx.x * RPB + ln_row_of<TPR>(); row < a.M; row += (int64_t)gridDim.x * RPB) {
+    Raw x, dy, add;
+    x.load(static_cast<const T*>(a.x) + row * H, t, H);
+    dy.load(static_cast<const T*>(a.dy) + row * H, t, H);
+    if (ADD) add.load(static_cast<const T*>(a.add) + row * H, t, H);
+    w.forget();
+    const float mean = a.mean[row], rstd = a.rstd[row];
+    float s[2] = {0.f, 0.f};  // sum g, sum g xh
+#pragma unroll
+    for (int q = 0; q < Raw::NQ; ++q)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        // elements past the row: dy is zero there
+        const float xh = (x.get(q, e) - mean) * rstd, d = dy.get(q, e), g = d * w.get(q, e);
+        s[0] += g;
+        s[1] = __builtin_fmaf(g, xh, s[1]);
+        dw[q * VEC + e] = __builtin_fmaf(d, xh, dw[q * VEC + e]);
+        db[q * VEC + e] += d;
+      }
+    ln_sum<TPR>(s, smem);
+    const float m0 = s[0] / fh, m1 = s[1] / fh;
+    x.forget();
+    dy.forget();
+    w.forget();
+    const auto dxr = make_rsrc(static_cast<T*>(a.y) + row * H, (uint32_t)(H * (int)sizeof(T)));
+#pragma unroll
+    for (int q = 0; q < Raw::NQ; ++q) {
+      float o[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float xh = (x.get(q, e) - mean) * rstd, g = dy.get(q, e) * w.get(q, e);
+        o[e] = rstd * (g - m0 - xh * m1);
+        if (ADD) o[e] += add.get(q, e);
+      }
+      ln_store<T, VEC, TPR>(dxr, t, q, o);
+    }
+  }
+  // the workgroup's column sums, [2][H]
+  float* out = a.part + (int64_t)blockIdx.x * 2 * H;
+  if constexpr (TPR > 64) {
+#pragma unroll
+    for (int q = 0; q < Raw::NQ; ++q)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const int c = (t + TPR * q) * VEC + e;
+        if (c < H) {
+          out[c] = dw[q * VEC + e];
+          out[H + c] = db[q * VEC + e];
+        }
+      }
+  } else {
+    const int wave = threadIdx.x >> 6;
+    for (int v = 0; v < RPB; ++v) {
+      if (wave == v) {
+#pragma unroll
+        for (int q = 0; q < Raw::NQ; ++q)
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            const int c = (t + TPR * q) * VEC + e;
+            if (c < H) {
+              smem[c] = v == 0 ? dw[q * VEC + e] : smem[c] + dw[q * VEC + e];
+              smem[H + c] = v == 0 ? db[q * VEC + e] : smem[H + c] + db[q * VEC + e];
+            }
+          }
+      }
+      __syncthreads();
+    }
+    for (int c = threadIdx.x; c < 2 * H; c += ln_back_threads(TPR)) out[c] = smem[c];
+  }
+}
+
+// Column sums of nb partial rows of `cols` floats, each plane of `plane`
+// columns rounded to T into its own tensor (null: not wanted).  A workgroup
+// has 32 columns, eight threads a column, each the partials i, i + 8, ...; the
+// eight sums are added in order.
+template <typename T>
+__global__ __launch_bounds__(256) void k_column_join(const float* __restrict__ part, int nb, int cols, int plane,
+                                                     T* out0, T* out1) {
+  __shared__ float s[8][32];
+  const int c = blockIdx.x * 32 + (threadIdx.x & 31), r = threadIdx.x >> 5;
+  float v = 0.f;
+  if (c < cols) {
+#pragma unroll 8
+    for (int i = r; i < nb; i += 8) v += part[(int64_t)i * cols + c];
+  }
+  s[r][threadIdx.x & 31] = v;
+  __syncthreads();
+  if (threadIdx.x >= 32 || c >= cols) return;
+  float t = s[0][threadIdx.x];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) t += s[i][threadIdx.x];
+  T* o = c < plane ? out0 : out1;
+  if (o != nullptr) o[c < plane ? c : c - plane] = (T)t;
+}
+
+// Column sums of bf16 rows (the linears' bias gradients): workgroup (x, y) has
+// columns 64 x 8 .. of the y-th run of rows, a wavefront every fourth row.
+__global__ __launch_bounds__(256) void k_column_sum(const uint16_t* __restrict__ x, int64_t M, int H, int rows,
+                                                    float* __restrict__ part) {
+  __shared__ float s[4][512];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int c8 = blockIdx.x * 64 + lane, n8 = H >> 3;
+  const int64_t r0 = (int64_t)blockIdx.y * rows, r1 = min(M, r0 + rows);
+  float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (c8 < n8) {
+#pragma unroll 4
+    for (int64_t r = r0 + wave; r < r1; r += 4) {
+      const u32x4_t u = ld16(x + r * H + 8 * c8);
+      const uint32_t w4[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[2 * i] += bf16_bits_to_f32(w4[i] & 0xFFFFu);
+        v[2 * i + 1] += bf16_bits_to_f32(w4[i] >> 16);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) s[wave][8 * lane + i] = v[i];
+  __syncthreads();
+  for (int i = threadIdx.x; i < 512; i += 256) {
+    const int c = blockIdx.x * 512 + i;
+    if (c < H) part[(int64_t)blockIdx.y * H + c] = ((s[0][i] + s[1][i]) + s[2][i]) + s[3][i];
+  }
+}
+
+namespace {
+
+inline bool ln_vector(const LnArgs& a, int size) {
+  const int vec = 16 / size;
+  if (a.H % vec != 0) return false;
+  const void* p[] = {a.x, a.w, a.b, a.y, a.dy, a.add};
+  for (const void* q : p)
+    if (reinterpret_cast<uintptr_t>(q) & 15u) return false;
+  return true;
+}
+
+// elements of a row that a wavefront keeps in the backward pass without
+// spilling: per lane 48 of 16 bits in pairs, 32 otherwise
+template <typename T, int VEC>
+constexpr int ln_back_wave_h() {
+  return sizeof(T) == 4 || VEC == 1 ? 64 * 32 : 64 * 48;
+}
+
+template <typename T, int VEC>
+hipError_t ln_forward(const LnArgs& a, hipStream_t s) {
+  // few rows: a workgroup each, so that a row's arithmetic is spread out; many:
+  // a wavefront each
+  const bool wave = a.H <= 64 * 48 && a.M > kLnWaveRows;
+  const int per = wave ? 64 : 256;
+  const int ept = (a.H + per * VEC - 1) / (per * VEC) * VEC;
+  const int64_t groups = wave ? (a.M + 3) / 4 : a.M;
+  const dim3 grid((unsigned)std::min<int64_t>(groups, kLnMaxGrid));
+#define W4A16_LN(EPT_, TPR_) hipLaunchKernelGGL((k_ln_forward<T, VEC, EPT_, TPR_>), grid, dim3(ln_threads(TPR_)), 0, s, a)
+  if (per == 64) {
+    if (ept <= 16) W4A16_LN(16, 64);
+    else if (ept <= 32) W4A16_LN(32, 64);
+    else W4A16_LN(48, 64);
+  } else {
+    if (ept <= 8) W4A16_LN(8, 256);
+    else if (ept <= 16) W4A16_LN(16, 256);
+    else W4A16_LN(32, 256);
+  }
+#undef W4A16_LN
+  return hipGetLastError();
+}
+
+template <typename T, int VEC>
+hipError_t ln_backward(const LnArgs& a, T* dw, T* db, hipStream_t s) {
+  int nb = 0;
+  if (a.M > 0) {
+    const bool wave = a.H <= ln_back_wave_h<T, VEC>();
+    const int per = wave ? 64 : 256;
+    const int ept = (a.H + per * VEC - 1) / (per * VEC) * VEC;
+    nb = (int)std::min<int64_t>(wave ? (a.M + 7) / 8 : a.M, kLnPartials);
+    const size_t lds = wave ? 2 * (size_t)a.H * 4 : 2 * 4 * 4;
+#define W4A16_LN1(EPT_, TPR_, ADD_) \
+  hipLaunchKernelGGL((k_ln_backward<T, VEC, EPT_, TPR_, ADD_>), dim3(nb), dim3(ln_back_threads(TPR_)), lds, s, a)
+#define W4A16_LN(EPT_, TPR_)                                                  \
+  do {                                                                        \
+    if (a.add != nullptr) {                                                   \
+      /* (HybridLink's rows alone) */                                         \
+      if constexpr (std::is_same<T, __bf16>::value) W4A16_LN1(EPT_, TPR_, true); \
+      else return hipErrorInvalidValue;                                       \
+    } else {                                                                  \
+      W4A16_LN1(EPT_, TPR_, false);                                           \
+    }                                                                         \
+  } while (0)
+    if (per == 64) {
+      if (ept <= 16) W4A16_LN(16, 64);
+      else if (ept <= 32) W4A16_LN(32, 64);
+      else if constexpr (ln_back_wave_h<T, VEC>() > 64 * 32) W4A16_LN(48, 64);
+    } else {
+      if (ept <= 16) W4A16_LN(16, 256);
+      else W4A16_LN(32, 256);
+    }
+#undef W4A16_LN
+#undef W4A16_LN1
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  hipLaunchKernelGGL(k_column_join<T>, dim3((2 * a.H + 31) / 32), dim3(256), 0, s, a.part, nb, 2 * a.H, a.H, dw, db);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+int ln_partials(int64_t M) { return (int)std::min<int64_t>(M, kLnPartials); }
+
+hipError_t launch_ln_forward(int dtype, const LnArgs& a, hipStream_t s) {
+  if (a.M == 0) return hipSuccess;
+  if (a.H <= 0 || a.H > kLnMaxH) return hipErrorInvalidValue;
+  const bool v = ln_vector(a, dtype == 2 ? 4 : 2);
+  switch (dtype) {
+    case 0: return v ? ln_forward<__bf16, 8>(a, s) : ln_forward<__bf16, 1>(a, s);
+    case 1: return v ? ln_forward<_Float16, 8>(a, s) : ln_forward<_Float16, 1>(a, s);
+    case 2: return v ? ln_forward<float, 4>(a, s) : ln_forward<float, 1>(a, s);
+    default: return hipErrorInvalidValue;
+  }
+}
+
+hipError_t launch_ln_backward(int dtype, const LnArgs& a, void* dw, void* db, hipStream_t s) {
+  if (a.H <= 0 || a.H > kLnMaxH || a.M < 0) return hipErrorInvalidValue;
+  const bool v = ln_vector(a, dtype == 2 ? 4 : 2);
+  switch (dtype) {
+    case 0:
+      return v ? ln_backward<__bf16, 8>(a, static_cast<__bf16*>(dw), static_cast<__bf16*>(db), s)
+               : ln_backward<__bf16, 1>(a, static_cast<__bf16*>(dw), static_cast<__bf16*>(db), s);
+    case 1:
+      return v ? ln_backward<_Float16, 8>(a, static_cast<_Float16*>(dw), static_cast<_Float16*>(db), s)
+               : ln_backward<_Float16, 1>(a, static_cast<_Float16*>(dw), static_cast<_Float16*>(db), s);
+    case 2:
+      return v ? ln_backward<float, 4>(a, static_cast<float*>(dw), static_cast<float*>(db), s)
+               : ln_backward<float, 1>(a, static_cast<float*>(dw), static_cast<float*>(db), s);
+    default: return hipErrorInvalidValue;
+  }
+}
+
+int column_sum_partials(int64_t M) { return (int)std::min<int64_t>((M + 15) / 16, kColSumPartials); }
+
+hipError_t launch_column_sum(const uint16_t* x, int64_t M, int H, float* part, uint16_t* out, hipStream_t s) {
+  if (H <= 0 || H % 8 != 0 || M < 0) return hipErrorInvalidValue;
+  int nb = 0;
+  if (M > 0) {
+    const int want = column_sum_partials(M);
+    const int64_t rows = ((M + want - 1) / want + 3) / 4 * 4;
+    if (rows > (1 << 30)) return hipErrorInvalidValue;
+    nb = (int)((M + rows - 1) / rows);
+    hipLaunchKernelGGL(k_column_sum, dim3((H + 511) / 512, nb), dim3(256), 0, s, x, M, H, (int)rows, part);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  hipLaunchKernelGGL(k_column_join<__bf16>, dim3((H + 31) / 32), dim3(256), 0, s, part, nb, H, H,
+                     reinterpret_cast<__bf16*>(out), static_cast<__bf16*>(nullptr));
+  return hipGetLastError();
+}
+
+}  // namespace w4a16

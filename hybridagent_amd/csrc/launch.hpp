@@ -337,6 +337,63 @@ struct GemmBf16Args {
 bool gemm_bf16_supported(int64_t K, int64_t cols);
 // max_items: grouped, most m-tiles
 hipError_t launch_gemm_bf16(int epi, GemmBf16Args a, int max_items, hipStream_t s);
+// Layer norm (kernels_layer_norm.hip); dtype: 0 bf16, 1 fp16, 2 fp32
+struct LnArgs {
+  const void *x, *w, *b;    // b nullable
+  void* y;                  // backward: dx
+  float *mean, *rstd;       // forward: nullable together
+  const void *dy, *add;     // backward; add nullable, [M, H]: added to dx
+  float* part;              // backward: ln_partials(M) * 2 H floats
+  int64_t M;
+  int H;
+  float eps;
+};
+constexpr int kLnMaxH = 8192;
+constexpr int kLnPartials = 256;   // one workgroup per CU
+constexpr int kLnMaxGrid = 4096;
+constexpr int64_t kLnWaveRows = 512;
+int ln_partials(int64_t M);
+hipError_t launch_ln_forward(int dtype, const LnArgs& a, hipStream_t s);
+hipError_t launch_ln_backward(int dtype, const LnArgs& a, void* dw, void* db, hipStream_t s);
+// out = the column sums of bf16 rows; part: column_sum_partials(M) * H floats
+constexpr int kColSumPartials = 128;
+int column_sum_partials(int64_t M);
+hipError_t launch_column_sum(const uint16_t* x, int64_t M, int H, float* part, uint16_t* out, hipStream_t s);
+// Dense bf16 GEMMs of the training forms (gemm_dense.hpp).
+enum DenseLayout { kDgNT = 0, kDgNN = 1, kDgTN = 2 };
+enum DenseEpilogue {
+  kDgPlain = 0,        // out = C
+  kDgGateUp = 1,       // NT, B gate rows, B2 up rows: out = gelu_tanh(C) C2; out2, out3 (nullable) = C, C2
+  kDgGateUpBack = 2,   // NN, in = a, in2 = b: out = C b gelu_tanh'(a), out2 = C gelu_tanh(a)
+  kDgBiasGelu = 3,     // NT: out2 = z = C + bias, out = gelu_erf(z)
+  kDgBiasResidual = 4, // NT: out = in + C + bias
+  kDgGeluBack = 5      // NN: out = C gelu_erf'(in)
+};
+struct DgEpilogue {
+  uint16_t *out, *out2, *out3;
+  const uint16_t *in, *in2, *bias;
+};
+struct DgProblem {
+  const uint16_t *A, *A2, *B, *B2;  // NN: C = A B + A2 B2 (A2 null: A B alone)
+  int M, N;                         // of C, row-major, N a multiple of 8
+  int lda, ldb;                     // elements between rows of the operands
+  DgEpilogue e;
+  int tile0;                        // set by dense_gemm_args: first tile,
+  int64_t part0;                    // first element in a plane of partial sums
+};
+constexpr int kDgMaxProblems = 3;
+struct DgArgs {
+  DgProblem prob[kDgMaxProblems];
+  int nprob;
+  int K;        // of one pair; a multiple of 32 (TN: any)
+  int mi, ni, ksplit;  // the plan
+  float* part;  // ksplit > 1: planes of partial sums
+  int64_t plane;
+  int tiles, nk, nk1;
+};
+// a launch of up to three products of one layout and epilogue; a.part holds
+// dense_gemm_part_floats(plane) floats (null: no split)
+hipError_t launch_gemm_dense(int layout, int epi, DgArgs a, hipStream_t s);
 // prefill grouped GEMM: one launch per stage, items = (m-tile, n-tile)
 hipError_t launch_prefill(int mode, PrefillArgs a, int max_mtiles, hipStream_t s);
 // the exact-form prefill GEMM (kernels_prefill_x.hip): H and I multiples of

@@ -97,4 +97,43 @@ inline int linear_w4_blocks(int64_t M, int64_t N, int cus, int max_blocks) {
   return cheapest_blocks(M, N, cus, max_blocks, cost);
 }
 
+// Dense GEMMs (gemm_dense.hpp): the tiles that are built, 32 mi rows x 32 ni
+// operand columns each.
+#define W4A16_DG_TILES(X) X(8, 8) X(6, 6) X(8, 4) X(4, 8) X(4, 4) X(2, 4) X(2, 2)
+struct DenseShape {
+  int64_t rows, cols;  // of the product (gate/up: both halves' columns)
+};
+struct DensePlan {
+  int mi, ni, ksplit;
+};
+// planes of fp32 partial sums that a split product may take: at most 8, at
+// most 32 MB
+constexpr int kDgMaxSplit = 8;
+constexpr int64_t kDgPartFloats = int64_t(8) << 20;
+inline int dense_part_planes(int64_t plane) {
+  const int64_t n = plane > 0 ? kDgPartFloats / plane : 0;
+  return n >= kDgMaxSplit ? kDgMaxSplit : n >= 2 ? (int)n : 1;
+}
+inline DensePlan dense_plan(const DenseShape* sh, int nprob, int nk, int max_split, int cus) {
+  DensePlan best{0, 0, 1};
+  int64_t least = 0;
+#define W4A16_DG(MI_, NI_)                                                                             \
+  {                                                                                                    \
+    int64_t tiles = 0;                                                                                 \
+    for (int i = 0; i < nprob; ++i)                                                                    \
+      tiles += (sh[i].rows + 32 * MI_ - 1) / (32 * MI_) * ((sh[i].cols + 32 * NI_ - 1) / (32 * NI_));  \
+    for (int ks = 1; ks <= max_split && (ks == 1 || nk >= 4 * ks); ++ks) {                             \
+      const int64_t rounds = (tiles * ks + cus - 1) / cus;                                             \
+      const int64_t c = rounds * ((nk + ks - 1) / ks + 8) * (MI_ * NI_ + 8) + (ks > 1 ? 400 : 0);      \
+      if (best.mi == 0 || c < least) {                                                                 \
+        best = DensePlan{MI_, NI_, ks};                                                                \
+        least = c;                                                                                     \
+      }                                                                                                \
+    }                                                                                                  \
+  }
+  W4A16_DG_TILES(W4A16_DG)
+#undef W4A16_DG
+  return best;
+}
+
 }  // namespace w4a16

@@ -1,0 +1,122 @@
+"""Differentiable forms of the framework's dense maps, on the HIP library.
+
+The reference trains HybridLink and the dense weights around the experts
+through torch's autograd (hybrid_sft/train.py, hybrid_agent/hybridlink.py);
+these are the same maps with hand-written backward passes:
+
+* ``layer_norm``  nn.LayerNorm (hybridlink.py:20,23)
+* ``gated_mlp``   the shared MLP of a decoder layer (backends.py:105-108)
+* ``hybridlink``  HybridLink.forward (hybridlink.py:17-28), and ``HybridLink``,
+  the module with the reference's parameter names
+
+Each is one pair of library calls (``_lib.layer_norm`` and
+``_lib.layer_norm_backward``, ...), differentiable once.  Code that captures
+a training step into a graph calls those pairs itself: the functions here
+refuse to record a backward pass while the stream is capturing, because a
+gradient accumulated on another stream's graph would end the capture.
+"""
+from __future__ import annotations
+
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+
+
+def _wants_grad(*tensors) -> bool:
+    """Whether the call records a backward pass; refuses where it cannot."""
+    if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in tensors):
+        return False
+    if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("a differentiable call cannot be captured into a graph: call the forward and backward "
+                           "functions of hybridagent_amd._lib in the captured code instead")
+    return True
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, mean, rstd = _lib.layer_norm(x, weight, bias, eps, return_stats=True)
+        ctx.save_for_backward(x, weight, mean, rstd)
+        ctx.bias = bias is not None
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, mean, rstd = ctx.saved_tensors
+        dx, dw, db = _lib.layer_norm_backward(dy, x, weight, mean, rstd, bias=ctx.bias)
+        return dx, dw, db, None
+
+
+def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
+               eps: float = 1e-5) -> torch.Tensor:
+    """Layer norm over the last dimension of bf16, fp16 or fp32 rows."""
+    if _wants_grad(x, weight, bias):
+        return _LayerNorm.apply(x, weight, bias, eps)
+    return _lib.layer_norm(x, weight, bias, eps)
+
+
+class _GatedMLP(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate_w, up_w, down_w):
+        y, saved = _lib.gated_mlp(x, gate_w, up_w, down_w, return_saved=True)
+        ctx.save_for_backward(x, gate_w, up_w, down_w, saved)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        return _lib.gated_mlp_backward(dy, *ctx.saved_tensors, needs=ctx.needs_input_grad)
+
+
+def gated_mlp(x: torch.Tensor, gate_w: torch.Tensor, up_w: torch.Tensor, down_w: torch.Tensor) -> torch.Tensor:
+    """(gelu_tanh(x gate_w^T) * (x up_w^T)) down_w^T on bf16 [..., H]."""
+    if _wants_grad(x, gate_w, up_w, down_w):
+        return _GatedMLP.apply(x, gate_w, up_w, down_w)
+    return _lib.gated_mlp(x, gate_w, up_w, down_w)
+
+
+class _HybridLink(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, h, eps, *params):
+        out, saved = _lib.hybridlink_train(h, *params, eps)
+        ctx.save_for_backward(h, *params, saved)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        h, *params, saved = ctx.saved_tensors
+        dh, *grads = _lib.hybridlink_backward(dout, h, *params, saved)
+        return (dh, None, *grads)
+
+
+def hybridlink(h: torch.Tensor, ln1_w: torch.Tensor, ln1_b: torch.Tensor, p1_w: torch.Tensor, p1_b: torch.Tensor,
+               p2_w: torch.Tensor, p2_b: torch.Tensor, ln2_w: torch.Tensor, ln2_b: torch.Tensor,
+               eps: float = 1e-5) -> torch.Tensor:
+    """HybridLink of bf16 [..., H]: with a backward pass where an argument wants a gradient, else
+    the inference call (``_lib.hybridlink``; the two round their intermediates at different points)."""
+    params = (ln1_w, ln1_b, p1_w, p1_b, p2_w, p2_b, ln2_w, ln2_b)
+    if _wants_grad(h, *params):
+        return _HybridLink.apply(h, eps, *params)
+    return _lib.hybridlink(h, *params, eps)
+
+
+class HybridLink(nn.Module):
+    """R(h) = post_ln(h + proj2(GELU(proj1(pre_ln(h))))) with the reference module's parameter names
+    (hybridlink.py:17-28), so its state dict loads as it is."""
+
+    def __init__(self, hidden_size: int, eps: float = 1e-5, dtype: torch.dtype = torch.bfloat16,
+                 device: torch.device | str | None = None) -> None:
+        super().__init__()
+        kw = {"dtype": dtype, "device": device}
+        self.pre_ln = nn.LayerNorm(hidden_size, eps=eps, **kw)
+        self.proj1 = nn.Linear(hidden_size, hidden_size, **kw)
+        self.proj2 = nn.Linear(hidden_size, hidden_size, **kw)
+        self.post_ln = nn.LayerNorm(hidden_size, eps=eps, **kw)
+
+    def forward(self, h: torch.Tensor) -> torch.Tensor:
+        return hybridlink(h, self.pre_ln.weight, self.pre_ln.bias, self.proj1.weight, self.proj1.bias,
+                          self.proj2.weight, self.proj2.bias, self.post_ln.weight, self.post_ln.bias, self.pre_ln.eps)

@@ -373,6 +373,84 @@ W4A16_API int moe_ffn_block_forward_tiled(
 W4A16_API int moe_ffn_block_routing_offsets(int64_t M, int64_t top_k, int64_t E, int64_t H, int64_t I,
                                             int64_t Im, size_t* idx_offset, size_t* w_offset);
 
+/* ---- Training forms of the dense maps: forward passes that keep what the
+ * backward needs, and the backward passes.  No kernel of the reference
+ * matches them (it trains through torch's autograd); the maps are those of
+ * the entry points above.  Gradients are sums in fp32, rounded once to the
+ * tensor's type; every sum's order depends on the shapes alone, so a call
+ * repeated on the same inputs gives the same bits.  Gradients of weights are
+ * written, not accumulated, also for zero rows (as zeros).                  */
+
+/* The type of a tensor whose entry point takes several. */
+enum w4a16_dtype { W4A16_BF16 = 0, W4A16_F16 = 1, W4A16_F32 = 2 };
+
+/* nn.LayerNorm over rows of H (hybridlink.py:20,23: pre_ln, post_ln):
+ *   mean = sum x / H, rstd = 1 / sqrt(sum (x - mean)^2 / H + eps)
+ *   y = (x - mean) * rstd * weight + bias
+ * x, y [M, H], weight, bias (NULL: none) [H], all of `dtype`; mean, rstd
+ * float32 [M], written where non-NULL (both or neither).  H <= 8192, any
+ * alignment of the type (16-byte loads where H and the pointers allow them).
+ * backward, with g = dy * weight and xh = (x - mean) * rstd:
+ *   dx = rstd * (g - sum g / H - xh * (sum g xh) / H)
+ *   dweight = sum over rows of dy xh, dbias = sum over rows of dy
+ * (dbias NULL: not wanted), all of `dtype`.                                 */
+W4A16_API int w4a16_layer_norm(const void* x, const void* weight, const void* bias, void* y, float* mean, float* rstd,
+                               int dtype, int64_t M, int64_t H, float eps, void* stream);
+W4A16_API size_t w4a16_layer_norm_backward_workspace_bytes(int64_t M, int64_t H);
+W4A16_API int w4a16_layer_norm_backward(const void* dy, const void* x, const void* weight, const float* mean,
+                                        const float* rstd, void* dx, void* dweight, void* dbias, int dtype, int64_t M,
+                                        int64_t H, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The gated feed-forward block (the shared MLP, backends.py:105-108):
+ *   a = x gate_w^T, b = x up_w^T, h = gelu_tanh(a) * b, y = h down_w^T
+ * x, y [M, H]; gate_w, up_w [I, H]; down_w [H, I]; bf16.  h is rounded to bf16
+ * once, from the fp32 sums (moe_ffn_block_forward rounds where the
+ * reference's torch ops do: a, b, gelu(a) and h).  `saved` (NULL: a call
+ * without a backward pass): w4a16_gated_mlp_saved_bytes(M, I) bytes that the
+ * forward fills (a, b and h in bf16) and the backward of the same M, H, I reads.
+ * backward, with dh = dy down_w:
+ *   da = dh * b * gelu_tanh'(a), db = dh * gelu_tanh(a)   (rounded to bf16)
+ *   dx = da gate_w + db up_w
+ *   dgate_w = da^T x, dup_w = db^T x, ddown_w = dy^T h
+ * (each of the four nullable: not wanted, and not computed).
+ * H, I multiples of 32, at most 32768; 16-byte aligned pointers.            */
+W4A16_API size_t w4a16_gated_mlp_workspace_bytes(int64_t M, int64_t H, int64_t I);
+W4A16_API size_t w4a16_gated_mlp_saved_bytes(int64_t M, int64_t I);
+W4A16_API int w4a16_gated_mlp(const uint16_t* x, const uint16_t* gate_w, const uint16_t* up_w, const uint16_t* down_w,
+                              uint16_t* y, void* saved, size_t saved_bytes, int64_t M, int64_t H, int64_t I,
+                              void* workspace, size_t workspace_bytes, void* stream);
+W4A16_API size_t w4a16_gated_mlp_backward_workspace_bytes(int64_t M, int64_t H, int64_t I);
+W4A16_API int w4a16_gated_mlp_backward(const uint16_t* dy, const uint16_t* x, const uint16_t* gate_w,
+                                       const uint16_t* up_w, const uint16_t* down_w, const void* saved,
+                                       size_t saved_bytes, uint16_t* dx, uint16_t* dgate_w, uint16_t* dup_w,
+                                       uint16_t* ddown_w, int64_t M, int64_t H, int64_t I, void* workspace,
+                                       size_t workspace_bytes, void* stream);
+
+/* HybridLink with a backward pass (hybridlink.py:17-28; parameters as for
+ * w4a16_hybridlink):
+ *   a = LN(h; ln1), z = a p1_w^T + p1_b, g = gelu_erf(z),
+ *   r = h + (g p2_w^T + p2_b), out = LN(r; ln2)
+ * a, z, g, r and out are rounded to bf16 once each, from fp32
+ * (w4a16_hybridlink rounds where the torch modules do, so the two differ by
+ * roundings).  `saved`: w4a16_hybridlink_saved_bytes(B, H) bytes that the
+ * forward fills and the backward of the same B, H reads.  The backward gives
+ * dh and the gradients of the eight parameters.  H a multiple of 32, at most
+ * 8192; every pointer 16-byte aligned.                                      */
+W4A16_API size_t w4a16_hybridlink_saved_bytes(int64_t B, int64_t H);
+W4A16_API size_t w4a16_hybridlink_train_workspace_bytes(int64_t B, int64_t H);
+W4A16_API int w4a16_hybridlink_train(const uint16_t* h, const uint16_t* ln1_w, const uint16_t* ln1_b,
+                                     const uint16_t* p1_w, const uint16_t* p1_b, const uint16_t* p2_w,
+                                     const uint16_t* p2_b, const uint16_t* ln2_w, const uint16_t* ln2_b, uint16_t* out,
+                                     void* saved, size_t saved_bytes, int64_t B, int64_t H, float eps, void* workspace,
+                                     size_t workspace_bytes, void* stream);
+W4A16_API size_t w4a16_hybridlink_backward_workspace_bytes(int64_t B, int64_t H);
+W4A16_API int w4a16_hybridlink_backward(const uint16_t* dout, const uint16_t* h, const uint16_t* ln1_w,
+                                        const uint16_t* p1_w, const uint16_t* p2_w, const uint16_t* ln2_w,
+                                        const void* saved, size_t saved_bytes, uint16_t* dh, uint16_t* dln1_w,
+                                        uint16_t* dln1_b, uint16_t* dp1_w, uint16_t* dp1_b, uint16_t* dp2_w,
+                                        uint16_t* dp2_b, uint16_t* dln2_w, uint16_t* dln2_b, int64_t B, int64_t H,
+                                        void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
