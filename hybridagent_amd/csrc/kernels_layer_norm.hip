@@ -197,7 +197,7 @@ template <typename T, int VEC, int EPT, int TPR, bool ADD>
 __global__ __launch_bounds__(ln_back_threads(TPR)) void k_ln_backward(LnArgs a) {
   using Raw = LnRaw<T, VEC, EPT, TPR>;
   constexpr int RPB = ln_back_threads(TPR) / TPR;
-  extern __shared__ float smem[];  // TPR > 64: the rows' sums; else [2][H] of the column sums
+  extern __shared__ float smem[];  // TPR > 64: a row's sums; else column sums, [4][2][EPT][64]
   const int t = threadIdx.x % TPR;
   const int H = a.H;
   const float fh = (float)H;
@@ -243,38 +243,53 @@ __global__ __launch_bounds__(ln_back_threads(TPR)) void k_ln_backward(LnArgs a) 
       ln_store<T, VEC, TPR>(dxr, t, q, o);
     }
   }
-  // the workgroup's column sums, [2][H]
-  float* out = a.part + (int64_t)blockIdx.x * 2 * H;
-  if constexpr (TPR > 64) {
+  // the wavefronts' column sums: the upper half hand theirs to the lower half,
+  // until the first has them all (a value at its lane's place in a row of 64:
+  // no bank conflicts)
+  if constexpr (TPR == 64) {
+    const int wave = threadIdx.x >> 6;
 #pragma unroll
-    for (int q = 0; q < Raw::NQ; ++q)
+    for (int half = RPB / 2; half >= 1; half /= 2) {
+      float* mine = smem + (wave & (half - 1)) * 2 * EPT * 64 + t;
+      if (wave >= half && wave < 2 * half) {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const int c = (t + TPR * q) * VEC + e;
-        if (c < H) {
-          out[c] = dw[q * VEC + e];
-          out[H + c] = db[q * VEC + e];
+        for (int i = 0; i < EPT; ++i) {
+          mine[64 * i] = dw[i];
+          mine[64 * (EPT + i)] = db[i];
         }
       }
-  } else {
-    const int wave = threadIdx.x >> 6;
-    for (int v = 0; v < RPB; ++v) {
-      if (wave == v) {
+      __syncthreads();
+      if (wave < half) {
 #pragma unroll
-        for (int q = 0; q < Raw::NQ; ++q)
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            const int c = (t + TPR * q) * VEC + e;
-            if (c < H) {
-              smem[c] = v == 0 ? dw[q * VEC + e] : smem[c] + dw[q * VEC + e];
-              smem[H + c] = v == 0 ? db[q * VEC + e] : smem[H + c] + db[q * VEC + e];
-            }
-          }
+        for (int i = 0; i < EPT; ++i) {
+          dw[i] += mine[64 * i];
+          db[i] += mine[64 * (EPT + i)];
+        }
       }
       __syncthreads();
     }
-    for (int c = threadIdx.x; c < 2 * H; c += ln_back_threads(TPR)) out[c] = smem[c];
+    if (wave != 0) return;
   }
+  // the workgroup's, [2][H]
+  const auto wr = make_rsrc(a.part + (int64_t)blockIdx.x * 2 * H, (uint32_t)(H * 4));
+  const auto br = make_rsrc(a.part + (int64_t)blockIdx.x * 2 * H + H, (uint32_t)(H * 4));
+#pragma unroll
+  for (int q = 0; q < Raw::NQ; ++q)
+#pragma unroll
+    for (int e = 0; e < VEC; e += VEC < 4 ? 1 : 4) {
+      const int o = ((t + TPR * q) * VEC + e) * 4, i = q * VEC + e;
+      if constexpr (VEC < 4) {
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(dw[i]), wr, o, 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(db[i]), br, o, 0, 0);
+      } else {
+        __builtin_amdgcn_raw_buffer_store_b128(
+            u32x4_t{__float_as_uint(dw[i]), __float_as_uint(dw[i + 1]), __float_as_uint(dw[i + 2]),
+                    __float_as_uint(dw[i + 3])}, wr, o, 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b128(
+            u32x4_t{__float_as_uint(db[i]), __float_as_uint(db[i + 1]), __float_as_uint(db[i + 2]),
+                    __float_as_uint(db[i + 3])}, br, o, 0, 0);
+      }
+    }
 }
 
 // Column sums of nb partial rows of `cols` floats, each plane of `plane`
@@ -380,9 +395,9 @@ hipError_t ln_backward(const LnArgs& a, T* dw, T* db, hipStream_t s) {
     const int per = wave ? 64 : 256;
     const int ept = (a.H + per * VEC - 1) / (per * VEC) * VEC;
     nb = (int)std::min<int64_t>(wave ? (a.M + 7) / 8 : a.M, kLnPartials);
-    const size_t lds = wave ? 2 * (size_t)a.H * 4 : 2 * 4 * 4;
-#define W4A16_LN1(EPT_, TPR_, ADD_) \
-  hipLaunchKernelGGL((k_ln_backward<T, VEC, EPT_, TPR_, ADD_>), dim3(nb), dim3(ln_back_threads(TPR_)), lds, s, a)
+#define W4A16_LN1(EPT_, TPR_, ADD_)                                                                             \
+  hipLaunchKernelGGL((k_ln_backward<T, VEC, EPT_, TPR_, ADD_>), dim3(nb), dim3(ln_back_threads(TPR_)),            \
+                     TPR_ == 64 ? 4 * 2 * EPT_ * 64 * 4 : 2 * 4 * 4, s, a)
 #define W4A16_LN(EPT_, TPR_)                                                  \
   do {                                                                        \
     if (a.add != nullptr) {                                                   \
