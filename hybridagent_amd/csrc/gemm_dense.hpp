@@ -19,7 +19,7 @@
 //
 // LDS formats of a stage's operand tile, both free of bank conflicts:
 //   rows  (k contiguous)  [rows][32 k], 64 bytes a row, the 16-byte chunks
-//         XOR-swizzled by (row / 4) % 4: a fragment is 16 rows x 64 bytes, one
+//         XOR-swizzled by dg_row_swz(row): a fragment is 16 rows x 64 bytes, one
 //         ds_read_b128 per lane;
 //   cols  ([k][.])        [32 k][cols], the 32-byte units of a row
 //         XOR-swizzled by bits of k (dg_swz): a fragment of 16 columns x 32 k
@@ -75,6 +75,12 @@ __device__ __forceinline__ int dg_swz(int k) {
     return ((k >> 1) & 1) | ((k >> 2) & 2);
 }
 
+// the swizzle of the 16-byte chunks of a rows tile, by the row's group of four.
+// A 16-byte read goes in groups of 16 lanes, 0..3, 12..15, 20..27 and 4..11,
+// 16..19, 28..31 of each 32: with lane l on row l % 16, chunk l / 16, each such
+// group covers the 256-byte bank window once.
+__device__ __forceinline__ int dg_row_swz(int quad) { return (((quad ^ (quad >> 1)) & 1) << 1) | ((quad >> 1) & 1); }
+
 // One operand's side of a tile: W rows (or columns), F fragments of 16 per
 // wavefront.  COLS: the cols format.  GU (rows format): the first half of a
 // wavefront's fragments come from p, the second half, same rows, from p2.
@@ -101,7 +107,7 @@ struct DgOperand {
         voff[j] = k * (int)ld * 2 + 2 * col;
       } else {
         int r = 16 * ins + (lane >> 2);
-        const int chunk = (lane & 3) ^ ((lane >> 4) & 3);
+        const int chunk = (lane & 3) ^ dg_row_swz((lane >> 4) & 3);
         if constexpr (GU) {
           // tile rows 16 F w + [0, 8 F): rows 8 F w + .. of p, [8 F, 16 F): of p2
           const int w = r / (16 * F), in = r - 16 * F * w;
@@ -119,7 +125,7 @@ struct DgOperand {
 #pragma unroll
       for (int f = 0; f < F; ++f) foff[f] = k * 2 * W + 32 * ((w * F + f) ^ dg_swz<W>(k)) + 8 * (lane & 3);
     } else {
-      foff[0] = 1024 * F * w + (lane & 15) * 64 + 16 * ((lane >> 4) ^ ((lane >> 2) & 3));
+      foff[0] = 1024 * F * w + (lane & 15) * 64 + 16 * ((lane >> 4) ^ dg_row_swz((lane >> 2) & 3));
     }
   }
   static __device__ __forceinline__ bool second(int j) {
@@ -268,89 +274,171 @@ __global__ __launch_bounds__(kDgThreads, MI * NI > 36 ? 1 : 2) void k_gemm_dense
   oa.init_frag(wave >> 1);
   ob.init_frag(wave & 1);
 
-  // load j (of the wavefront's kLoads) of stage t into a slot.  The descriptor
-  // is empty past the range; cols: it starts at the stage's first k and ends
-  // with row K - 1, so that rows past K read as zero.  Rows: stages of the
-  // second pair (t >= nk1) follow the first's.
-  auto issue = [&](int t, unsigned char* slot, int j) {
+  // Where stage t's loads come from.  The descriptors are empty past the
+  // range; cols: they start at the stage's first k and end with row K - 1, so
+  // that rows past K read as zero.  Rows: stages of the second pair (t >= nk1)
+  // follow the first's.
+  struct Src {
+    __amdgpu_buffer_rsrc_t a, b, b2;
+    int off;
+  };
+  auto source = [&](int t) {
     const bool two = LAYOUT == kDgNN && t >= a.nk1;
     const int tt = two ? t - a.nk1 : t;
     const bool any = t < t1;
     const int left = min(kDgKT, a.K - tt * kDgKT);
+    const uint16_t* pa = two ? p.A2 : p.A;
+    const uint16_t* pb = two ? p.B2 : p.B;
+    Src r;
+    r.a = AC ? make_rsrc(pa + (int64_t)tt * kDgKT * p.lda + m0, any ? (uint32_t)(left * p.lda - m0) * 2u : 0u)
+             : make_rsrc(pa + (int64_t)m0 * p.lda, any ? (uint32_t)(min(p.M - m0, BM) * p.lda) * 2u : 0u);
+    const uint32_t bbytes = (uint32_t)(min(p.N - n0, BN) * p.ldb) * 2u;
+    r.b = BC ? make_rsrc(pb + (int64_t)tt * kDgKT * p.ldb + n0, any ? (uint32_t)(left * p.ldb - n0) * 2u : 0u)
+             : make_rsrc(pb + (int64_t)n0 * p.ldb, any ? bbytes : 0u);
+    r.b2 = GU ? make_rsrc(p.B2 + (int64_t)n0 * p.ldb, any ? bbytes : 0u) : r.b;
+    r.off = tt * (kDgKT * 2);
+    return r;
+  };
+  // load j of the wavefront's kLoads into a slot
+  auto issue = [&](const Src& r, unsigned char* slot, int j) {
     if (j < OA::kLoads) {
-      const uint16_t* b = two ? p.A2 : p.A;
-      const auto r = AC ? make_rsrc(b + (int64_t)tt * kDgKT * p.lda + m0, any ? (uint32_t)(left * p.lda - m0) * 2u : 0u)
-                        : make_rsrc(b + (int64_t)m0 * p.lda, any ? (uint32_t)(min(p.M - m0, BM) * p.lda) * 2u : 0u);
-      px_dma16(r, oa.voff[j], AC ? 0 : tt * (kDgKT * 2), slot + (wave + 4 * j) * 1024);
+      px_dma16(r.a, oa.voff[j], AC ? 0 : r.off, slot + (wave + 4 * j) * 1024);
     } else {
       const int i = j - OA::kLoads;
-      const uint16_t* b = two || (GU && OB::second(i)) ? p.B2 : p.B;
-      const auto r = BC ? make_rsrc(b + (int64_t)tt * kDgKT * p.ldb + n0, any ? (uint32_t)(left * p.ldb - n0) * 2u : 0u)
-                        : make_rsrc(b + (int64_t)n0 * p.ldb, any ? (uint32_t)(min(p.N - n0, BN) * p.ldb) * 2u : 0u);
-      px_dma16(r, ob.voff[i], BC ? 0 : tt * (kDgKT * 2), slot + OA::kBytes + (wave + 4 * i) * 1024);
+      if (GU && OB::second(i))
+        px_dma16(r.b2, ob.voff[i], r.off, slot + OA::kBytes + (wave + 4 * i) * 1024);
+      else
+        px_dma16(r.b, ob.voff[i], BC ? 0 : r.off, slot + OA::kBytes + (wave + 4 * i) * 1024);
     }
   };
 
+  // Accumulators past what the vector registers hold live in the accumulation
+  // registers.  Named so before and after the loop, each keeps one place in
+  // it; otherwise the compiler moves up to 200 of them around per stage.
   f32x4_t acc[MI][NI];
+  constexpr bool kAccRegs = MI * NI > 36;
 #pragma unroll
   for (int m = 0; m < MI; ++m)
 #pragma unroll
-    for (int n = 0; n < NI; ++n) acc[m][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  u32x4_t fa[MI], fb[NI];
+    for (int n = 0; n < NI; ++n) {
+      acc[m][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      if (kAccRegs) asm volatile("" : "+a"(acc[m][n]));
+    }
+  // column fragments twice where there is room: those of the next stage are
+  // then read all along a stage
+  constexpr int kB = kAccRegs ? 2 : 1;
+  u32x4_t fa[MI], fb[kB][NI];
 
 #pragma unroll
-  for (int s = 0; s < kStages; ++s)
+  for (int s = 0; s < kStages; ++s) {
+    const Src r = source(t0 + s);
 #pragma unroll
-    for (int j = 0; j < kLoads; ++j) issue(t0 + s, smem + s * kStage, j);
+    for (int j = 0; j < kLoads; ++j) issue(r, smem + s * kStage, j);
+  }
   dg_wait_vm<(kStages - 1) * kLoads>();
   px_barrier();
 #pragma unroll
-  for (int n = 0; n < NI; ++n) fb[n] = ob.frag(smem + OA::kBytes, n);
+  for (int n = 0; n < NI; ++n) fb[0][n] = ob.frag(smem + OA::kBytes, n);
 #pragma unroll
   for (int m = 0; m < MI; ++m) fa[m] = oa.frag(smem, m);
 
   // Stage t, its fragments at hand: after the first row of fragments' MFMAs
   // the wavefronts meet (stage t + 1 has landed, slot t is read), then slot t
   // is refilled with stage t + kStages and every fragment register takes its
-  // fragment of stage t + 1 right after its last MFMA.  The last two rows go
-  // column by column, so that a column's fragment has 2 (NI - 1) MFMAs to
-  // arrive.
+  // fragment of stage t + 1 after its last MFMA.  Reads and loads go one by one
+  // between the MFMAs: one after every second keeps the matrix unit fed.
   int slot = 0;
-  for (int t = t0; t < t1; ++t) {
+  auto stage = [&](int t, auto cur_) {
+    constexpr int cur = kB == 2 ? decltype(cur_)::value : 0, nxt = kB == 2 ? cur ^ 1 : 0;
     const int ns = slot == kStages - 1 ? 0 : slot + 1;
     unsigned char* refill = smem + slot * kStage;
     const unsigned char* st = smem + ns * kStage;
+    const Src src = source(t + kStages);
 #pragma unroll
-    for (int n = 0; n < NI; ++n) acc[0][n] = mfma16(fb[n], fa[0], acc[0][n]);
+    for (int n = 0; n < NI; ++n) acc[0][n] = mfma16(fb[cur][n], fa[0], acc[0][n]);
     __builtin_amdgcn_sched_barrier(0);
     dg_wait_vm<(kStages - 2) * kLoads>();
     px_barrier();
     __builtin_amdgcn_sched_barrier(0);
-    if (MI > 2) fa[0] = oa.frag(st, 0);
+    if constexpr (kB == 2) {
+      // operation o of the row m: its MFMAs are done one ahead
+      constexpr int R = MI - 1;
 #pragma unroll
-    for (int m = 1; m < MI - 2; ++m) {
+      for (int m = 1; m < MI; ++m) {
+        // this row's: fa[m - 1], then column fragments and loads by turns
+        const int b0 = (m - 1) * NI / R, b1 = m * NI / R, l0 = (m - 1) * kLoads / R, l1 = m * kLoads / R;
+        int done = 0;
 #pragma unroll
-      for (int n = 0; n < NI; ++n) acc[m][n] = mfma16(fb[n], fa[m], acc[m][n]);
-      fa[m] = oa.frag(st, m);
+        for (int n = 0; n < NI; ++n) {
+          acc[m][n] = mfma16(fb[cur][n], fa[m], acc[m][n]);
+          if (n % 2 == 0 || NI < 6) {
+            if (done == 0) {
+              fa[m - 1] = oa.frag(st, m - 1);
+            } else {
+              const int k = done - 1;
+              if (k < b1 - b0)
+                fb[nxt][b0 + k] = ob.frag(st + OA::kBytes, b0 + k);
+              else if (k - (b1 - b0) < l1 - l0)
+                issue(src, refill, l0 + k - (b1 - b0));
+            }
+            ++done;
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+        // what did not fit
 #pragma unroll
-      for (int j = (m - 1) * kLoads / (MI > 3 ? MI - 3 : 1); j < m * kLoads / (MI > 3 ? MI - 3 : 1); ++j)
-        issue(t + kStages, refill, j);
-      __builtin_amdgcn_sched_barrier(0);
+        for (int k = done - 1; k < (b1 - b0) + (l1 - l0); ++k) {
+          if (k < b1 - b0)
+            fb[nxt][b0 + k] = ob.frag(st + OA::kBytes, b0 + k);
+          else
+            issue(src, refill, l0 + k - (b1 - b0));
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      fa[MI - 1] = oa.frag(st, MI - 1);
+    } else {
+      if (MI > 2) fa[0] = oa.frag(st, 0);
+#pragma unroll
+      for (int m = 1; m < MI - 2; ++m) {
+#pragma unroll
+        for (int n = 0; n < NI; ++n) acc[m][n] = mfma16(fb[0][n], fa[m], acc[m][n]);
+        fa[m] = oa.frag(st, m);
+#pragma unroll
+        for (int j = (m - 1) * kLoads / (MI > 3 ? MI - 3 : 1); j < m * kLoads / (MI > 3 ? MI - 3 : 1); ++j)
+          issue(src, refill, j);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if constexpr (MI <= 3) {
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) issue(src, refill, j);
+      }
+      // the last two rows column by column, so that a column's fragment has
+      // 2 (NI - 1) MFMAs to arrive
+#pragma unroll
+      for (int n = 0; n < NI; ++n) {
+        if (MI > 2) acc[MI - 2][n] = mfma16(fb[0][n], fa[MI - 2], acc[MI - 2][n]);
+        acc[MI - 1][n] = mfma16(fb[0][n], fa[MI - 1], acc[MI - 1][n]);
+        fb[0][n] = ob.frag(st + OA::kBytes, n);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      fa[MI - 2] = oa.frag(st, MI - 2);
+      fa[MI - 1] = oa.frag(st, MI - 1);
     }
-    if constexpr (MI <= 3) {
-#pragma unroll
-      for (int j = 0; j < kLoads; ++j) issue(t + kStages, refill, j);
-    }
-#pragma unroll
-    for (int n = 0; n < NI; ++n) {
-      if (MI > 2) acc[MI - 2][n] = mfma16(fb[n], fa[MI - 2], acc[MI - 2][n]);
-      acc[MI - 1][n] = mfma16(fb[n], fa[MI - 1], acc[MI - 1][n]);
-      fb[n] = ob.frag(st + OA::kBytes, n);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    fa[MI - 2] = oa.frag(st, MI - 2);
-    fa[MI - 1] = oa.frag(st, MI - 1);
     slot = ns;
+  };
+  if constexpr (kB == 2) {
+    for (int t = t0; t < t1; t += 2) {
+      stage(t, std::integral_constant<int, 0>{});
+      if (t + 1 < t1) stage(t + 1, std::integral_constant<int, 1>{});
+    }
+  } else {
+    for (int t = t0; t < t1; ++t) stage(t, std::integral_constant<int, 0>{});
+  }
+  if constexpr (kAccRegs) {
+#pragma unroll
+    for (int m = 0; m < MI; ++m)
+#pragma unroll
+      for (int n = 0; n < NI; ++n) asm volatile("" : "+a"(acc[m][n]));
   }
   dg_wait_vm<0>();  // no load may land in another workgroup's LDS
 
@@ -422,7 +510,7 @@ hipError_t dg_launch(const DgArgs& a, hipStream_t s) {
 // the launch with the tile that `a` was planned for
 template <int LAYOUT, int EPI>
 hipError_t dg_launch_tile(const DgArgs& a, hipStream_t s) {
-#define W4A16_DG(MI_, NI_) \
+#define W4A16_DG(MI_, NI_, OCC_, ALONE_, EACH_) \
   if (a.mi == MI_ && a.ni == NI_) return dg_launch<LAYOUT, EPI, MI_, NI_>(a, s);
   W4A16_DG_TILES(W4A16_DG)
 #undef W4A16_DG
