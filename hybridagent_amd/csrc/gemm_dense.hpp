@@ -145,17 +145,18 @@ struct DgOperand {
   }
 };
 
-// ---- epilogues on four consecutive columns n .. n + 3 of row m
+// ---- epilogues on eight consecutive columns n .. n + 7 of row m
 
-__device__ __forceinline__ void dg_ld4(const uint16_t* p, float v[4]) {
-  const uint2 u = *reinterpret_cast<const uint2*>(p);
-  v[0] = bf16_bits_to_f32(u.x & 0xFFFFu);
-  v[1] = bf16_bits_to_f32(u.x >> 16);
-  v[2] = bf16_bits_to_f32(u.y & 0xFFFFu);
-  v[3] = bf16_bits_to_f32(u.y >> 16);
+__device__ __forceinline__ void dg_unpack8(u32x4_t u, float v[8]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = bf16_bits_to_f32(w[i] & 0xFFFFu);
+    v[2 * i + 1] = bf16_bits_to_f32(w[i] >> 16);
+  }
 }
-__device__ __forceinline__ void dg_st4(uint16_t* p, const float v[4]) {
-  *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+__device__ __forceinline__ void dg_st8(uint16_t* p, const float v[8]) {
+  st16(p, u32x4_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])});
 }
 
 // d/dx gelu_tanh = s + x s (1 - s) 2 u', s = 1 / (1 + exp(-2 u)),
@@ -169,62 +170,91 @@ __device__ __forceinline__ void gelu_tanh_and_slope(float x, float* act, float* 
   *act = x * s;
   *slope = s + xc * s * (1.0f - s) * 1.5957691216057308f * (1.0f + 0.134145f * x2);
 }
-__device__ __forceinline__ float gelu_erf_f32(float x) { return 0.5f * x * (1.0f + erff(x * 0.70710678118654752f)); }
-// d/dx gelu_erf = Phi(x) + x phi(x)
-__device__ __forceinline__ float gelu_erf_slope(float x) {
-  return 0.5f * (1.0f + erff(x * 0.70710678118654752f)) + x * (0.3989422804014327f * __expf(-0.5f * x * x));
+// gelu_erf = x Phi(x) and its slope Phi(x) + x phi(x), with the normal tail
+// Q(|x|) = exp(-x^2 / 2) P(t) / 2, t = 1 / (1 + 0.3275911 |x| / sqrt(2)), P the
+// fifth-degree polynomial of Abramowitz and Stegun 7.1.26: Phi is off by 7e-8
+// at most, the tail by 2^-9 of itself down to Q = 3e-7 and by 1 % at 6e-16;
+// erff and an exponential of their own took three times the instructions
+// (2049 rows of 2816: 65 us against 49 without the activation).
+__device__ __forceinline__ void gelu_erf_and_slope(float x, float* act, float* slope) {
+  const float e = __expf(-0.5f * x * x);
+  const float t = __fdividef(1.0f, 1.0f + 0.2316418882f * fabsf(x));
+  const float P = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+  const float q = 0.5f * P * e;
+  const float cdf = x < 0.f ? q : 1.0f - q;
+  *act = x * cdf;
+  *slope = cdf + x * (0.3989422804014327f * e);
+}
+
+// what the epilogue reads of e.in and e.in2 at element o
+struct DgIn {
+  u32x4_t a, b;
+};
+template <int EPI>
+__device__ __forceinline__ DgIn dg_fetch(const DgEpilogue& e, int64_t o) {
+  DgIn r;
+  r.a = r.b = u32x4_t{0u, 0u, 0u, 0u};
+  if (EPI == kDgGateUpBack || EPI == kDgBiasResidual || EPI == kDgGeluBack) r.a = ld16(e.in + o);
+  if (EPI == kDgGateUpBack) r.b = ld16(e.in2 + o);
+  return r;
 }
 
 // v: the sums (v2: kDgGateUp's up sums); o: the element's offset in row-major [M, N]
 template <int EPI>
-__device__ __forceinline__ void dg_finish(const DgEpilogue& e, int64_t o, int n, const float v[4], const float v2[4]) {
-  float r[4], s[4];
+__device__ __forceinline__ void dg_finish(const DgEpilogue& e, int64_t o, int n, const float v[8], const float v2[8],
+                                          const DgIn& in) {
+  float r[8], s[8];
   if constexpr (EPI == kDgPlain) {
-    dg_st4(e.out + o, v);
+    dg_st8(e.out + o, v);
   } else if constexpr (EPI == kDgGateUp) {
     // h = gelu_tanh(a) b from the sums themselves, rounded once; a and b are
     // rounded for the backward pass alone
 #pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = gelu_tanh_f32(v[i]) * v2[i];
-    dg_st4(e.out + o, r);
+    for (int i = 0; i < 8; ++i) r[i] = gelu_tanh_f32(v[i]) * v2[i];
+    dg_st8(e.out + o, r);
     if (e.out2 != nullptr) {
-      dg_st4(e.out2 + o, v);
-      dg_st4(e.out3 + o, v2);
+      dg_st8(e.out2 + o, v);
+      dg_st8(e.out3 + o, v2);
     }
   } else if constexpr (EPI == kDgGateUpBack) {
-    float a[4], b[4];
-    dg_ld4(e.in + o, a);
-    dg_ld4(e.in2 + o, b);
+    float a[8], b[8];
+    dg_unpack8(in.a, a);
+    dg_unpack8(in.b, b);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 8; ++i) {
       float act, slope;
       gelu_tanh_and_slope(a[i], &act, &slope);
       r[i] = v[i] * b[i] * slope;
       s[i] = v[i] * act;
     }
-    dg_st4(e.out + o, r);
-    dg_st4(e.out2 + o, s);
+    dg_st8(e.out + o, r);
+    dg_st8(e.out2 + o, s);
   } else if constexpr (EPI == kDgBiasGelu) {
-    dg_ld4(e.bias + n, s);
+    dg_unpack8(ld16(e.bias + n), s);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 8; ++i) {
+      float slope;
       s[i] += v[i];
-      r[i] = gelu_erf_f32(s[i]);
+      gelu_erf_and_slope(s[i], &r[i], &slope);
     }
-    dg_st4(e.out + o, r);
-    dg_st4(e.out2 + o, s);
+    dg_st8(e.out + o, r);
+    dg_st8(e.out2 + o, s);
   } else if constexpr (EPI == kDgBiasResidual) {
-    float b[4];
-    dg_ld4(e.bias + n, b);
-    dg_ld4(e.in + o, s);
+    float b[8];
+    dg_unpack8(ld16(e.bias + n), b);
+    dg_unpack8(in.a, s);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = s[i] + (v[i] + b[i]);
-    dg_st4(e.out + o, r);
+    for (int i = 0; i < 8; ++i) r[i] = s[i] + (v[i] + b[i]);
+    dg_st8(e.out + o, r);
   } else if constexpr (EPI == kDgGeluBack) {
-    dg_ld4(e.in + o, s);
+    dg_unpack8(in.a, s);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = v[i] * gelu_erf_slope(s[i]);
-    dg_st4(e.out + o, r);
+    for (int i = 0; i < 8; ++i) {
+      float act, slope;
+      gelu_erf_and_slope(s[i], &act, &slope);
+      r[i] = v[i] * slope;
+    }
+    dg_st8(e.out + o, r);
   }
 }
 
@@ -442,54 +472,87 @@ __global__ __launch_bounds__(kDgThreads, MI * NI > 36 ? 1 : 2) void k_gemm_dense
   }
   dg_wait_vm<0>();  // no load may land in another workgroup's LDS
 
-  // epilogue: lane l holds columns 4 (l / 16) .. + 3 of row l % 16 of each 16 x 16 tile
+  // Epilogue, 16 rows of the wavefront at a time: lane l holds columns
+  // 4 (l / 16) .. + 3 of row l % 16 of each 16 x 16 tile; through the
+  // wavefront's own part of the LDS it gets eight consecutive columns of a row,
+  // so that every load and store is 16 bytes per lane and whole rows of the
+  // wavefront's columns (8 bytes in 32-byte pieces took half as long again).
+  px_barrier();  // every wavefront is past its reads of the ring
   constexpr int NO = GU ? NI / 2 : NI;
+  // floats; 4 modulo the 64 banks where that is not twice the row
+  constexpr int kPitch = NO > 4 ? 132 : NO > 2 ? 68 : 16 * NO + 4;
+  constexpr int kPlanes = GU ? 2 : 1;
+  static_assert(4 * kPlanes * 16 * kPitch * 4 <= kStages * kStage, "the epilogue's rows fit in the ring");
+  float* const rows = reinterpret_cast<float*>(smem) + wave * kPlanes * 16 * kPitch;
+  constexpr int kIter = (2 * NO * 16 + 63) / 64;
+  const int r0 = m0 + 16 * MI * (wave >> 1), c0 = n0 + 16 * NO * (wave & 1);
 #pragma unroll
   for (int m = 0; m < MI; ++m) {
-    const int row = m0 + 16 * (MI * (wave >> 1) + m) + (lane & 15);
-    if (row >= p.M) continue;
+    DgIn in[kIter];
+    int64_t o[kIter];
+    bool ok[kIter];
+#pragma unroll
+    for (int i = 0; i < kIter; ++i) {
+      const int idx = lane + 64 * i, row = r0 + 16 * m + idx / (2 * NO), col = c0 + 8 * (idx % (2 * NO));
+      ok[i] = idx < 32 * NO && row < p.M && col < p.N;
+      o[i] = (int64_t)row * p.N + col;
+      if (ok[i] && a.ksplit == 1) in[i] = dg_fetch<EPI>(p.e, o[i]);
+    }
 #pragma unroll
     for (int n = 0; n < NO; ++n) {
-      const int col = n0 + 16 * (NO * (wave & 1) + n) + 4 * (lane >> 4);
-      if (col >= p.N) continue;
-      const int64_t o = (int64_t)row * p.N + col;
-      float v[4], v2[4];
+      float* q = rows + (lane & 15) * kPitch + 16 * n + 4 * (lane >> 4);
+      *reinterpret_cast<f32x4_t*>(q) = acc[m][n];
+      if (GU) *reinterpret_cast<f32x4_t*>(q + 16 * kPitch) = acc[m][GU ? n + NO : n];
+    }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        v[i] = acc[m][n][i];
-        v2[i] = acc[m][GU ? n + NO : n][i];
+    for (int i = 0; i < kIter; ++i) {
+      const int idx = lane + 64 * i;
+      if (!ok[i]) continue;
+      const float* q = rows + idx / (2 * NO) * kPitch + 8 * (idx % (2 * NO));
+      float v[8], v2[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        v[k] = q[k];
+        v2[k] = GU ? q[16 * kPitch + k] : 0.f;
       }
       if (a.ksplit > 1) {
-        float* q = a.part + split * a.plane + p.part0 + o;
-        *reinterpret_cast<float4*>(q) = make_float4(v[0], v[1], v[2], v[3]);
-        if (GU) *reinterpret_cast<float4*>(q + (int64_t)p.M * p.N) = make_float4(v2[0], v2[1], v2[2], v2[3]);
+        float* d = a.part + split * a.plane + p.part0 + o[i];
+#pragma unroll
+        for (int k = 0; k < 8; k += 4) {
+          *reinterpret_cast<float4*>(d + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+          if (GU)
+            *reinterpret_cast<float4*>(d + (int64_t)p.M * p.N + k) = make_float4(v2[k], v2[k + 1], v2[k + 2], v2[k + 3]);
+        }
       } else {
-        dg_finish<EPI>(p.e, o, col, v, v2);
+        dg_finish<EPI>(p.e, o[i], c0 + 8 * (idx % (2 * NO)), v, v2, in[i]);
       }
     }
   }
 }
 
 // The sums of a split launch: the splits' partial sums in order, then the
-// epilogue; a thread has four columns of one row.
+// epilogue; a thread has eight columns of one row.
 template <int EPI>
 __global__ __launch_bounds__(256) void k_gemm_dense_join(DgArgs a) {
   const DgProblem p = a.prob[blockIdx.y];
-  const int64_t n4 = (int64_t)p.M * p.N / 4;
+  const int64_t n8 = (int64_t)p.M * p.N / 8;
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n4) return;
-  const int64_t o = 4 * i;
+  if (i >= n8) return;
+  const int64_t o = 8 * i;
+  const DgIn in = dg_fetch<EPI>(p.e, o);
   const float* q = a.part + p.part0 + o;
-  float v[4] = {0.f, 0.f, 0.f, 0.f}, v2[4] = {0.f, 0.f, 0.f, 0.f};
+  float v[8], v2[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = v2[k] = 0.f;
+#pragma unroll 4
   for (int s = 0; s < a.ksplit; ++s) {
-    const float4 t = *reinterpret_cast<const float4*>(q + s * a.plane);
-    v[0] += t.x; v[1] += t.y; v[2] += t.z; v[3] += t.w;
-    if (EPI == kDgGateUp) {
-      const float4 u = *reinterpret_cast<const float4*>(q + s * a.plane + (int64_t)p.M * p.N);
-      v2[0] += u.x; v2[1] += u.y; v2[2] += u.z; v2[3] += u.w;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      v[k] += q[s * a.plane + k];
+      if (EPI == kDgGateUp) v2[k] += q[s * a.plane + (int64_t)p.M * p.N + k];
     }
   }
-  dg_finish<EPI>(p.e, o, (int)(o % p.N), v, v2);
+  dg_finish<EPI>(p.e, o, (int)(o % p.N), v, v2, in);
 }
 
 template <int LAYOUT, int EPI, int MI, int NI>
@@ -502,7 +565,7 @@ hipError_t dg_launch(const DgArgs& a, hipStream_t s) {
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.ksplit == 1) return e;
   int64_t most = 0;
-  for (int i = 0; i < a.nprob; ++i) most = std::max(most, (int64_t)a.prob[i].M * a.prob[i].N / 4);
+  for (int i = 0; i < a.nprob; ++i) most = std::max(most, (int64_t)a.prob[i].M * a.prob[i].N / 8);
   hipLaunchKernelGGL(k_gemm_dense_join<EPI>, dim3((unsigned)((most + 255) / 256), a.nprob), dim3(256), 0, s, a);
   return hipGetLastError();
 }
