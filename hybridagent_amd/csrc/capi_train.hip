@@ -139,7 +139,7 @@ LinkBackWs link_back_ws(void* p, int64_t B, int64_t H) {
   w.dz = c.take<uint16_t>(B * H);
   w.da = c.take<uint16_t>(B * H);
   w.part = c.take<float>(std::max({part_floats(B * H), part_floats(2 * H * H), (size_t)ln_partials(B) * 2 * H,
-                                   (size_t)column_sum_partials(B) * H}));
+                                   (size_t)column_sum_partials(B) * 2 * H}));
   w.bytes = c.used;
   return w;
 }
@@ -358,8 +358,7 @@ int w4a16_hybridlink_backward(const uint16_t* dout, const uint16_t* h, const uin
     a.part = B > 0 && part_floats(2 * H * H) > 0 ? gemm_part : nullptr;
     e = launch_gemm_dense(kDgTN, kDgPlain, a, s);
   }
-  if (e == hipSuccess) e = launch_column_sum(ws.dr, B, (int)H, ws.part, dp2_b, s);
-  if (e == hipSuccess) e = launch_column_sum(ws.dz, B, (int)H, ws.part, dp1_b, s);
+  if (e == hipSuccess) e = launch_column_sums(ws.dr, ws.dz, B, (int)H, ws.part, dp2_b, dp1_b, s);
   // pre_ln, and the residual's dr
   LnArgs n1 = ln_args(h, ln1_w, nullptr, dh, sv.mean1, sv.rstd1, B, H, 0.f);
   n1.dy = ws.da;

@@ -27,14 +27,17 @@ hipError_t launch_gemm_dense(int layout, int epi, DgArgs a, hipStream_t s) {
     a.plane += (int64_t)p.M * p.N * (gu ? 2 : 1);
     sh[i] = DenseShape{p.M, gu ? 2 * (int64_t)p.N : p.N};
   }
-  if (a.mi == 0) {
+  const bool thin = a.mi == 0 && layout != kDgTN && a.nprob == 1 &&
+                    a.prob[0].M <= dense_thin_rows(layout == kDgNN);
+  if (thin) a.ksplit = 1;
+  if (a.mi == 0 && !thin) {
     const DensePlan pl = dense_plan(sh, a.nprob, a.nk, a.part != nullptr ? dense_part_planes(a.plane) : 1, device_cus());
     a.mi = pl.mi;
     a.ni = pl.ni;
     a.ksplit = pl.ksplit;
   }
   a.tiles = 0;
-  for (int i = 0; i < a.nprob; ++i) {
+  for (int i = 0; i < a.nprob && !thin; ++i) {
     DgProblem& p = a.prob[i];
     const int bm = dg_bm(a.mi), bn = dg_bn(epi, a.ni);
     const int64_t t = (int64_t)((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn);

@@ -316,34 +316,43 @@ __global__ __launch_bounds__(256) void k_column_join(const float* __restrict__ p
   if (o != nullptr) o[c < plane ? c : c - plane] = (T)t;
 }
 
-// Column sums of bf16 rows (the linears' bias gradients): workgroup (x, y) has
-// columns 64 x 8 .. of the y-th run of rows, a wavefront every fourth row.
-__global__ __launch_bounds__(256) void k_column_sum(const uint16_t* __restrict__ x, int64_t M, int H, int rows,
-                                                    float* __restrict__ part) {
-  __shared__ float s[4][512];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int c8 = blockIdx.x * 64 + lane, n8 = H >> 3;
+// Column sums of two bf16 matrices (the linears' bias gradients): workgroup
+// (x, y, z) has columns 64 x .. 64 x + 63 of the y-th run of rows of matrix z,
+// thread t the columns 8 (t % 8) .. of every 32nd row; the 32 sums are added in
+// order.  One run: the results; else a row of partial sums for k_column_join.
+__global__ __launch_bounds__(256) void k_column_sum(const uint16_t* __restrict__ x0, const uint16_t* __restrict__ x1,
+                                                    int64_t M, int H, int64_t rows, float* __restrict__ part,
+                                                    __bf16* out0, __bf16* out1) {
+  __shared__ float s[32][64 + 4];
+  const uint16_t* x = blockIdx.z == 0 ? x0 : x1;
+  const int c = threadIdx.x & 7, r = threadIdx.x >> 3;
+  const int col = blockIdx.x * 64 + 8 * c;
   const int64_t r0 = (int64_t)blockIdx.y * rows, r1 = min(M, r0 + rows);
   float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (c8 < n8) {
+  if (col < H) {
 #pragma unroll 4
-    for (int64_t r = r0 + wave; r < r1; r += 4) {
-      const u32x4_t u = ld16(x + r * H + 8 * c8);
+    for (int64_t i = r0 + r; i < r1; i += 32) {
+      const u32x4_t u = ld16(x + i * H + col);
       const uint32_t w4[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        v[2 * i] += bf16_bits_to_f32(w4[i] & 0xFFFFu);
-        v[2 * i + 1] += bf16_bits_to_f32(w4[i] >> 16);
+      for (int k = 0; k < 4; ++k) {
+        v[2 * k] += bf16_bits_to_f32(w4[k] & 0xFFFFu);
+        v[2 * k + 1] += bf16_bits_to_f32(w4[k] >> 16);
       }
     }
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) s[wave][8 * lane + i] = v[i];
+  for (int k = 0; k < 8; ++k) s[r][8 * c + k] = v[k];
   __syncthreads();
-  for (int i = threadIdx.x; i < 512; i += 256) {
-    const int c = blockIdx.x * 512 + i;
-    if (c < H) part[(int64_t)blockIdx.y * H + c] = ((s[0][i] + s[1][i]) + s[2][i]) + s[3][i];
-  }
+  const int o = blockIdx.x * 64 + (int)threadIdx.x;
+  if (threadIdx.x >= 64 || o >= H) return;
+  float t = s[0][threadIdx.x];
+#pragma unroll
+  for (int i = 1; i < 32; ++i) t += s[i][threadIdx.x];
+  if (gridDim.y > 1)
+    part[((int64_t)blockIdx.y * 2 + blockIdx.z) * H + o] = t;
+  else
+    (blockIdx.z == 0 ? out0 : out1)[o] = (__bf16)t;
 }
 
 namespace {
@@ -391,7 +400,8 @@ template <typename T, int VEC>
 hipError_t ln_backward(const LnArgs& a, T* dw, T* db, hipStream_t s) {
   int nb = 0;
   if (a.M > 0) {
-    const bool wave = a.H <= ln_back_wave_h<T, VEC>();
+    // few rows: a workgroup each (32 rows of 2816: 8.6 us by wavefronts, which are few then)
+    const bool wave = a.H <= ln_back_wave_h<T, VEC>() && a.M > kLnPartials;
     const int per = wave ? 64 : 256;
     const int ept = (a.H + per * VEC - 1) / (per * VEC) * VEC;
     nb = (int)std::min<int64_t>(wave ? (a.M + 7) / 8 : a.M, kLnPartials);
@@ -458,22 +468,20 @@ hipError_t launch_ln_backward(int dtype, const LnArgs& a, void* dw, void* db, hi
   }
 }
 
-int column_sum_partials(int64_t M) { return (int)std::min<int64_t>((M + 15) / 16, kColSumPartials); }
+int column_sum_partials(int64_t M) {
+  return M <= kColSumRows ? 0 : (int)std::min<int64_t>((M + kColSumRows - 1) / kColSumRows, kColSumPartials);
+}
 
-hipError_t launch_column_sum(const uint16_t* x, int64_t M, int H, float* part, uint16_t* out, hipStream_t s) {
+hipError_t launch_column_sums(const uint16_t* x0, const uint16_t* x1, int64_t M, int H, float* part, uint16_t* out0,
+                              uint16_t* out1, hipStream_t s) {
   if (H <= 0 || H % 8 != 0 || M < 0) return hipErrorInvalidValue;
-  int nb = 0;
-  if (M > 0) {
-    const int want = column_sum_partials(M);
-    const int64_t rows = ((M + want - 1) / want + 3) / 4 * 4;
-    if (rows > (1 << 30)) return hipErrorInvalidValue;
-    nb = (int)((M + rows - 1) / rows);
-    hipLaunchKernelGGL(k_column_sum, dim3((H + 511) / 512, nb), dim3(256), 0, s, x, M, H, (int)rows, part);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-  }
-  hipLaunchKernelGGL(k_column_join<__bf16>, dim3((H + 31) / 32), dim3(256), 0, s, part, nb, H, H,
-                     reinterpret_cast<__bf16*>(out), static_cast<__bf16*>(nullptr));
+  const int n = std::max(1, column_sum_partials(M));
+  const int64_t rows = (M + n - 1) / n;
+  __bf16 *o0 = reinterpret_cast<__bf16*>(out0), *o1 = reinterpret_cast<__bf16*>(out1);
+  hipLaunchKernelGGL(k_column_sum, dim3((H + 63) / 64, n, 2), dim3(256), 0, s, x0, x1, M, H, rows, part, o0, o1);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || n == 1) return e;
+  hipLaunchKernelGGL(k_column_join<__bf16>, dim3((2 * H + 31) / 32), dim3(256), 0, s, part, n, 2 * H, H, o0, o1);
   return hipGetLastError();
 }
 

@@ -355,10 +355,13 @@ constexpr int64_t kLnWaveRows = 512;
 int ln_partials(int64_t M);
 hipError_t launch_ln_forward(int dtype, const LnArgs& a, hipStream_t s);
 hipError_t launch_ln_backward(int dtype, const LnArgs& a, void* dw, void* db, hipStream_t s);
-// out = the column sums of bf16 rows; part: column_sum_partials(M) * H floats
+// out0, out1 = the column sums of two bf16 matrices of M rows; part:
+// column_sum_partials(M) * 2 H floats
 constexpr int kColSumPartials = 128;
+constexpr int64_t kColSumRows = 512;
 int column_sum_partials(int64_t M);
-hipError_t launch_column_sum(const uint16_t* x, int64_t M, int H, float* part, uint16_t* out, hipStream_t s);
+hipError_t launch_column_sums(const uint16_t* x0, const uint16_t* x1, int64_t M, int H, float* part, uint16_t* out0,
+                              uint16_t* out1, hipStream_t s);
 // Dense bf16 GEMMs of the training forms (gemm_dense.hpp).
 enum DenseLayout { kDgNT = 0, kDgNN = 1, kDgTN = 2 };
 enum DenseEpilogue {

@@ -114,6 +114,12 @@ inline int linear_w4_blocks(int64_t M, int64_t N, int cus, int max_blocks) {
   X(4, 2, 3, 215, 190)    \
   X(2, 4, 3, 215, 185)    \
   X(2, 2, 4, 155, 125)
+// Products of few rows run as the weights' stream (gemm_thin.hpp): x W^T up to
+// 64 rows (2816 x 2816, split over workgroups / streamed: 1 row 9.0/5.1 us, 32
+// 10.0/6.1, 64 9.5/8.2), dy W up to 32 (32 rows 9.8/8.3 us, 64 10.9/10.6; two
+// pairs of 2112: 7 rows 10.6/10.6, 64 12.8/17.6, where a workgroup's 64-byte
+// pieces of rows cost more than the second launch).
+constexpr int dense_thin_rows(bool nn) { return nn ? 32 : 64; }
 struct DenseShape {
   int64_t rows, cols;  // of the product (gate/up: both halves' columns)
 };
