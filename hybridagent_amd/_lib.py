@@ -860,7 +860,9 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     y = torch.empty_like(x2)
     mean = rstd = None
     if return_stats:
-        mean, rstd = (torch.empty(x.shape[:-1], dtype=torch.float32, device=dev) for _ in range(2))
+        lead = x.shape[:-1]
+        mean = torch.empty(lead, dtype=torch.float32, device=dev)
+        rstd = torch.empty(lead, dtype=torch.float32, device=dev)
     weight = weight.contiguous()
     bias = None if bias is None else bias.contiguous()
     _call("w4a16_layer_norm", dev, load().w4a16_layer_norm, _ptr(x2), _ptr(weight), _ptr(bias), _ptr(y), _ptr(mean),

@@ -129,7 +129,7 @@ LinkSaved link_saved(void* p, int64_t B, int64_t H) {
 
 struct LinkBackWs {
   uint16_t *dr, *dz, *da;
-  float* part;
+  float *part, *ln2, *ln1, *cols;
   size_t bytes;
 };
 LinkBackWs link_back_ws(void* p, int64_t B, int64_t H) {
@@ -138,8 +138,11 @@ LinkBackWs link_back_ws(void* p, int64_t B, int64_t H) {
   w.dr = c.take<uint16_t>(B * H);
   w.dz = c.take<uint16_t>(B * H);
   w.da = c.take<uint16_t>(B * H);
-  w.part = c.take<float>(std::max({part_floats(B * H), part_floats(2 * H * H), (size_t)ln_partials(B) * 2 * H,
-                                   (size_t)column_sum_partials(B) * 2 * H}));
+  w.part = c.take<float>(std::max(part_floats(B * H), part_floats(2 * H * H)));
+  // partial rows of the column sums, added in one launch at the end
+  w.ln2 = c.take<float>((size_t)ln_partials(B) * 2 * H);
+  w.ln1 = c.take<float>((size_t)ln_partials(B) * 2 * H);
+  w.cols = c.take<float>((size_t)column_sum_partials(B) * 2 * H);
   w.bytes = c.used;
   return w;
 }
@@ -190,7 +193,14 @@ int w4a16_layer_norm_backward(const void* dy, const void* x, const void* weight,
   LnArgs a = ln_args(x, weight, nullptr, dx, const_cast<float*>(mean), const_cast<float*>(rstd), M, H, 0.f);
   a.dy = dy;
   a.part = static_cast<float*>(workspace);
-  return launch_status(launch_ln_backward(dtype, a, dweight, dbias, static_cast<hipStream_t>(stream)));
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  LnJoin j{};
+  j.seg[0] = {a.part, ln_partials(M), dweight, dbias};
+  j.n = 1;
+  j.H = (int)H;
+  hipError_t e = launch_ln_backward(dtype, a, s);
+  if (e == hipSuccess) e = launch_column_join(dtype, j, s);
+  return launch_status(e);
 }
 
 size_t w4a16_gated_mlp_workspace_bytes(int64_t M, int64_t H, int64_t I) {
@@ -336,35 +346,41 @@ int w4a16_hybridlink_backward(const uint16_t* dout, const uint16_t* h, const uin
   hipStream_t s = static_cast<hipStream_t>(stream);
   const LinkSaved sv = link_saved(const_cast<void*>(saved), B, H);
   const LinkBackWs ws = link_back_ws(B > 0 ? workspace : nullptr, B, H);
-  float* const gemm_part = ws.part;
   // post_ln: dr, the gradient of r = h + proj2(g)
   LnArgs n2 = ln_args(sv.r, ln2_w, nullptr, ws.dr, sv.mean2, sv.rstd2, B, H, 0.f);
   n2.dy = dout;
-  n2.part = ws.part;
-  hipError_t e = launch_ln_backward(W4A16_BF16, n2, dln2_w, dln2_b, s);
+  n2.part = ws.ln2;
+  hipError_t e = launch_ln_backward(W4A16_BF16, n2, s);
   // dz = (dr W2) gelu'(z), da = dz W1
   if (e == hipSuccess && B > 0)
     e = product(kDgNN, kDgGeluBack,
                 problem(ws.dr, H, p2_w, H, B, H, DgEpilogue{ws.dz, nullptr, nullptr, sv.z, nullptr, nullptr}), H,
-                gemm_part, s);
+                ws.part, s);
   if (e == hipSuccess && B > 0)
-    e = product(kDgNN, kDgPlain, problem(ws.dz, H, p1_w, H, B, H, to(ws.da)), H, gemm_part, s);
+    e = product(kDgNN, kDgPlain, problem(ws.dz, H, p1_w, H, B, H, to(ws.da)), H, ws.part, s);
   if (e == hipSuccess) {
     DgArgs a{};
     a.prob[0] = problem(ws.dr, H, sv.g, H, H, H, to(dp2_w));
     a.prob[1] = problem(ws.dz, H, sv.a, H, H, H, to(dp1_w));
     a.nprob = 2;
     a.K = (int)B;
-    a.part = B > 0 && part_floats(2 * H * H) > 0 ? gemm_part : nullptr;
+    a.part = B > 0 && part_floats(2 * H * H) > 0 ? ws.part : nullptr;
     e = launch_gemm_dense(kDgTN, kDgPlain, a, s);
   }
-  if (e == hipSuccess) e = launch_column_sums(ws.dr, ws.dz, B, (int)H, ws.part, dp2_b, dp1_b, s);
+  if (e == hipSuccess) e = launch_column_sums(ws.dr, ws.dz, B, (int)H, ws.cols, dp2_b, dp1_b, s);
   // pre_ln, and the residual's dr
   LnArgs n1 = ln_args(h, ln1_w, nullptr, dh, sv.mean1, sv.rstd1, B, H, 0.f);
   n1.dy = ws.da;
   n1.add = ws.dr;
-  n1.part = ws.part;
-  if (e == hipSuccess) e = launch_ln_backward(W4A16_BF16, n1, dln1_w, dln1_b, s);
+  n1.part = ws.ln1;
+  if (e == hipSuccess) e = launch_ln_backward(W4A16_BF16, n1, s);
+  LnJoin j{};
+  j.seg[0] = {ws.ln1, ln_partials(B), dln1_w, dln1_b};
+  j.seg[1] = {ws.ln2, ln_partials(B), dln2_w, dln2_b};
+  j.seg[2] = {ws.cols, column_sum_partials(B), dp2_b, dp1_b};
+  j.n = column_sum_partials(B) > 0 ? 3 : 2;
+  j.H = (int)H;
+  if (e == hipSuccess) e = launch_column_join(W4A16_BF16, j, s);
   return launch_status(e);
 }
 

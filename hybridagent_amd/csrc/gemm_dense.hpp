@@ -10,7 +10,9 @@
 // four consecutive n of one row m.
 //
 // A workgroup of four wavefronts (2 x 2) owns a tile of 32 MI rows x 32 NI
-// columns, a wavefront 16 MI x 16 NI of it.  k advances in stages of 32
+// columns, a wavefront 16 MI x 16 NI of it; with KG > 1 there are KG such
+// groups, each with a part of K and a ring of its own, whose sums are added in
+// LDS (a few hundred rows: a wavefront's chain of stages is what takes the time).  k advances in stages of 32
 // through a ring of dg_stages LDS slots filled by direct 16-byte global -> LDS
 // loads; the fragments of stage t + 1 are read while stage t is multiplied,
 // so that a stage has one barrier and its loads have two to three stages to
@@ -93,9 +95,8 @@ struct DgOperand {
   int foff[COLS ? F : 1];               // its fragment bytes in a stage
 
   // first: the tile's first row, n: rows there are (rows past it repeat the last)
-  __device__ __forceinline__ void init(int first, int n, int64_t ld) {
+  __device__ __forceinline__ void init(int first, int n, int64_t ld, int wave) {
     const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) {
       const int ins = wave + 4 * j;
@@ -128,10 +129,7 @@ struct DgOperand {
       foff[0] = 1024 * F * w + (lane & 15) * 64 + 16 * ((lane >> 4) ^ dg_row_swz((lane >> 2) & 3));
     }
   }
-  static __device__ __forceinline__ bool second(int j) {
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    return (wave + 4 * j) % F >= F / 2;
-  }
+  static __device__ __forceinline__ bool second(int j, int wave) { return (wave + 4 * j) % F >= F / 2; }
   __device__ __forceinline__ u32x4_t frag(const unsigned char* st, int f) const {
     if constexpr (COLS) {
       const unsigned char* p = st + foff[f];
@@ -265,8 +263,8 @@ __device__ __forceinline__ int dg_item(int total) {
   return i < per && x * per + i < total ? x * per + i : -1;
 }
 
-template <int LAYOUT, int EPI, int MI, int NI>
-__global__ __launch_bounds__(kDgThreads, MI * NI > 36 ? 1 : 2) void k_gemm_dense(DgArgs a) {
+template <int LAYOUT, int EPI, int MI, int NI, int KG>
+__global__ __launch_bounds__(KG * kDgThreads, MI * NI > 36 ? 1 : KG > 2 ? KG : 2) void k_gemm_dense(DgArgs a) {
   constexpr bool AC = LAYOUT == kDgTN, BC = LAYOUT != kDgNT;
   constexpr bool GU = EPI == kDgGateUp;
   using OA = DgOperand<AC, false, MI>;
@@ -277,7 +275,9 @@ __global__ __launch_bounds__(kDgThreads, MI * NI > 36 ? 1 : 2) void k_gemm_dense
   constexpr int BM = dg_bm(MI), BN = dg_bn(EPI, NI);
   extern __shared__ __align__(16) unsigned char smem[];
   const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
+  const int group = KG > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 8) : 0;
+  unsigned char* const ring = smem + group * kStages * kStage;
 
   // the tile: kDgGroupM row tiles run with each column tile
   int item = dg_item(a.tiles * a.ksplit);
@@ -294,13 +294,15 @@ __global__ __launch_bounds__(kDgThreads, MI * NI > 36 ? 1 : 2) void k_gemm_dense
   const int gm = min(kDgGroupM, n_mt - grp * kDgGroupM);
   const int nt = rem / gm;
   const int m0 = (grp * kDgGroupM + rem - nt * gm) * BM, n0 = nt * BN;
-  const int per = (a.nk + a.ksplit - 1) / a.ksplit;
-  const int t0 = split * per, t1 = min(a.nk, t0 + per);
+  // the group's stages; every group runs as many (those past its range multiply
+  // the zeros that empty descriptors give)
+  const int per = (a.nk + a.ksplit * KG - 1) / (a.ksplit * KG);
+  const int t0 = (split * KG + group) * per, t1 = min(a.nk, t0 + per), tend = t0 + per;
 
   OA oa;
   OB ob;
-  oa.init(m0, p.M, p.lda);
-  ob.init(n0, p.N, p.ldb);
+  oa.init(m0, p.M, p.lda, wave);
+  ob.init(n0, p.N, p.ldb, wave);
   oa.init_frag(wave >> 1);
   ob.init_frag(wave & 1);
 
@@ -335,7 +337,7 @@ __global__ __launch_bounds__(kDgThreads, MI * NI > 36 ? 1 : 2) void k_gemm_dense
       px_dma16(r.a, oa.voff[j], AC ? 0 : r.off, slot + (wave + 4 * j) * 1024);
     } else {
       const int i = j - OA::kLoads;
-      if (GU && OB::second(i))
+      if (GU && OB::second(i, wave))
         px_dma16(r.b2, ob.voff[i], r.off, slot + OA::kBytes + (wave + 4 * i) * 1024);
       else
         px_dma16(r.b, ob.voff[i], BC ? 0 : r.off, slot + OA::kBytes + (wave + 4 * i) * 1024);
@@ -363,14 +365,14 @@ __global__ __launch_bounds__(kDgThreads, MI * NI > 36 ? 1 : 2) void k_gemm_dense
   for (int s = 0; s < kStages; ++s) {
     const Src r = source(t0 + s);
 #pragma unroll
-    for (int j = 0; j < kLoads; ++j) issue(r, smem + s * kStage, j);
+    for (int j = 0; j < kLoads; ++j) issue(r, ring + s * kStage, j);
   }
   dg_wait_vm<(kStages - 1) * kLoads>();
   px_barrier();
 #pragma unroll
-  for (int n = 0; n < NI; ++n) fb[0][n] = ob.frag(smem + OA::kBytes, n);
+  for (int n = 0; n < NI; ++n) fb[0][n] = ob.frag(ring + OA::kBytes, n);
 #pragma unroll
-  for (int m = 0; m < MI; ++m) fa[m] = oa.frag(smem, m);
+  for (int m = 0; m < MI; ++m) fa[m] = oa.frag(ring, m);
 
   // Stage t, its fragments at hand: after the first row of fragments' MFMAs
   // the wavefronts meet (stage t + 1 has landed, slot t is read), then slot t
@@ -381,8 +383,8 @@ __global__ __launch_bounds__(kDgThreads, MI * NI > 36 ? 1 : 2) void k_gemm_dense
   auto stage = [&](int t, auto cur_) {
     constexpr int cur = kB == 2 ? decltype(cur_)::value : 0, nxt = kB == 2 ? cur ^ 1 : 0;
     const int ns = slot == kStages - 1 ? 0 : slot + 1;
-    unsigned char* refill = smem + slot * kStage;
-    const unsigned char* st = smem + ns * kStage;
+    unsigned char* refill = ring + slot * kStage;
+    const unsigned char* st = ring + ns * kStage;
     const Src src = source(t + kStages);
 #pragma unroll
     for (int n = 0; n < NI; ++n) acc[0][n] = mfma16(fb[cur][n], fa[0], acc[0][n]);
@@ -457,12 +459,12 @@ __global__ __launch_bounds__(kDgThreads, MI * NI > 36 ? 1 : 2) void k_gemm_dense
     slot = ns;
   };
   if constexpr (kB == 2) {
-    for (int t = t0; t < t1; t += 2) {
+    for (int t = t0; t < tend; t += 2) {
       stage(t, std::integral_constant<int, 0>{});
-      if (t + 1 < t1) stage(t + 1, std::integral_constant<int, 1>{});
+      if (t + 1 < tend) stage(t + 1, std::integral_constant<int, 1>{});
     }
   } else {
-    for (int t = t0; t < t1; ++t) stage(t, std::integral_constant<int, 0>{});
+    for (int t = t0; t < tend; ++t) stage(t, std::integral_constant<int, 0>{});
   }
   if constexpr (kAccRegs) {
 #pragma unroll
@@ -478,12 +480,31 @@ __global__ __launch_bounds__(kDgThreads, MI * NI > 36 ? 1 : 2) void k_gemm_dense
   // so that every load and store is 16 bytes per lane and whole rows of the
   // wavefront's columns (8 bytes in 32-byte pieces took half as long again).
   px_barrier();  // every wavefront is past its reads of the ring
+  if constexpr (KG > 1) {
+    // the groups' sums, added in order
+    f32x4_t* const sums = reinterpret_cast<f32x4_t*>(smem) + wave * MI * NI * 64 + lane;
+    if (group > 0) {
+#pragma unroll
+      for (int m = 0; m < MI; ++m)
+#pragma unroll
+        for (int n = 0; n < NI; ++n) sums[((group - 1) * 4 * MI * NI + m * NI + n) * 64] = acc[m][n];
+    }
+    __syncthreads();
+    if (group > 0) return;
+#pragma unroll
+    for (int g = 1; g < KG; ++g)
+#pragma unroll
+      for (int m = 0; m < MI; ++m)
+#pragma unroll
+        for (int n = 0; n < NI; ++n) acc[m][n] += sums[((g - 1) * 4 * MI * NI + m * NI + n) * 64];
+  }
   constexpr int NO = GU ? NI / 2 : NI;
   // floats; 4 modulo the 64 banks where that is not twice the row
   constexpr int kPitch = NO > 4 ? 132 : NO > 2 ? 68 : 16 * NO + 4;
   constexpr int kPlanes = GU ? 2 : 1;
-  static_assert(4 * kPlanes * 16 * kPitch * 4 <= kStages * kStage, "the epilogue's rows fit in the ring");
-  float* const rows = reinterpret_cast<float*>(smem) + wave * kPlanes * 16 * kPitch;
+  constexpr int kSums = (KG - 1) * 4 * MI * NI * 1024;  // (what the groups left)
+  static_assert(kSums + 4 * kPlanes * 16 * kPitch * 4 <= KG * kStages * kStage, "the epilogue's rows fit in the ring");
+  float* const rows = reinterpret_cast<float*>(smem + kSums) + wave * kPlanes * 16 * kPitch;
   constexpr int kIter = (2 * NO * 16 + 63) / 64;
   const int r0 = m0 + 16 * MI * (wave >> 1), c0 = n0 + 16 * NO * (wave & 1);
 #pragma unroll
@@ -555,13 +576,13 @@ __global__ __launch_bounds__(256) void k_gemm_dense_join(DgArgs a) {
   dg_finish<EPI>(p.e, o, (int)(o % p.N), v, v2, in);
 }
 
-template <int LAYOUT, int EPI, int MI, int NI>
+template <int LAYOUT, int EPI, int MI, int NI, int KG>
 hipError_t dg_launch(const DgArgs& a, hipStream_t s) {
-  constexpr int lds = dg_stages(MI, NI) * (32 * MI + 32 * NI) * kDgKT * 2;
+  constexpr int lds = KG * dg_stages(MI, NI) * (32 * MI + 32 * NI) * kDgKT * 2;
   static_assert(lds <= 160 * 1024, "LDS of a CU");
   const int64_t total = (int64_t)a.tiles * a.ksplit;
   const int grid = (int)(8 * ((total + 7) / 8));
-  hipLaunchKernelGGL((k_gemm_dense<LAYOUT, EPI, MI, NI>), dim3(grid), dim3(kDgThreads), lds, s, a);
+  hipLaunchKernelGGL((k_gemm_dense<LAYOUT, EPI, MI, NI, KG>), dim3(grid), dim3(KG * kDgThreads), lds, s, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.ksplit == 1) return e;
   int64_t most = 0;
@@ -573,8 +594,8 @@ hipError_t dg_launch(const DgArgs& a, hipStream_t s) {
 // the launch with the tile that `a` was planned for
 template <int LAYOUT, int EPI>
 hipError_t dg_launch_tile(const DgArgs& a, hipStream_t s) {
-#define W4A16_DG(MI_, NI_, OCC_, ALONE_, EACH_) \
-  if (a.mi == MI_ && a.ni == NI_) return dg_launch<LAYOUT, EPI, MI_, NI_>(a, s);
+#define W4A16_DG(MI_, NI_, KG_, OCC_, ALONE_, EACH_) \
+  if (a.mi == MI_ && a.ni == NI_ && a.kg == KG_) return dg_launch<LAYOUT, EPI, MI_, NI_, KG_>(a, s);
   W4A16_DG_TILES(W4A16_DG)
 #undef W4A16_DG
   return hipErrorInvalidValue;

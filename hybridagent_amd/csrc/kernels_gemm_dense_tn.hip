@@ -34,6 +34,7 @@ hipError_t launch_gemm_dense(int layout, int epi, DgArgs a, hipStream_t s) {
     const DensePlan pl = dense_plan(sh, a.nprob, a.nk, a.part != nullptr ? dense_part_planes(a.plane) : 1, device_cus());
     a.mi = pl.mi;
     a.ni = pl.ni;
+    a.kg = pl.kg;
     a.ksplit = pl.ksplit;
   }
   a.tiles = 0;

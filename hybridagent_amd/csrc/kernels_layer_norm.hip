@@ -15,8 +15,9 @@
 //
 // Bound: HBM.  The column sums of the backward pass are kept in registers
 // across the rows of a thread, added over a workgroup's wavefronts in LDS and
-// written once per workgroup (kLnPartials at most); a second launch adds those
-// in order, so that a result depends on the shape alone.
+// written once per workgroup (kLnPartials at most); a second launch
+// (k_column_join) adds those in order, so that a result depends on the shape
+// alone.
 #include <algorithm>
 #include <type_traits>
 
@@ -292,19 +293,19 @@ __global__ __launch_bounds__(ln_back_threads(TPR)) void k_ln_backward(LnArgs a) 
     }
 }
 
-// Column sums of nb partial rows of `cols` floats, each plane of `plane`
-// columns rounded to T into its own tensor (null: not wanted).  A workgroup
-// has 32 columns, eight threads a column, each the partials i, i + 8, ...; the
-// eight sums are added in order.
+// Column sums of partial rows: segment blockIdx.y has nb rows of 2 H floats,
+// whose halves, rounded to T, are two gradients (null: not wanted).  A
+// workgroup has 32 columns, eight threads a column, each the partials i,
+// i + 8, ...; the eight sums are added in order.
 template <typename T>
-__global__ __launch_bounds__(256) void k_column_join(const float* __restrict__ part, int nb, int cols, int plane,
-                                                     T* out0, T* out1) {
+__global__ __launch_bounds__(256) void k_column_join(LnJoin a) {
   __shared__ float s[8][32];
-  const int c = blockIdx.x * 32 + (threadIdx.x & 31), r = threadIdx.x >> 5;
+  const auto& g = a.seg[blockIdx.y];
+  const int c = blockIdx.x * 32 + (threadIdx.x & 31), r = threadIdx.x >> 5, cols = 2 * a.H;
   float v = 0.f;
   if (c < cols) {
 #pragma unroll 8
-    for (int i = r; i < nb; i += 8) v += part[(int64_t)i * cols + c];
+    for (int i = r; i < g.nb; i += 8) v += g.part[(int64_t)i * cols + c];
   }
   s[r][threadIdx.x & 31] = v;
   __syncthreads();
@@ -312,14 +313,14 @@ __global__ __launch_bounds__(256) void k_column_join(const float* __restrict__ p
   float t = s[0][threadIdx.x];
 #pragma unroll
   for (int i = 1; i < 8; ++i) t += s[i][threadIdx.x];
-  T* o = c < plane ? out0 : out1;
-  if (o != nullptr) o[c < plane ? c : c - plane] = (T)t;
+  T* o = static_cast<T*>(c < a.H ? g.out0 : g.out1);
+  if (o != nullptr) o[c < a.H ? c : c - a.H] = (T)t;
 }
 
 // Column sums of two bf16 matrices (the linears' bias gradients): workgroup
 // (x, y, z) has columns 64 x .. 64 x + 63 of the y-th run of rows of matrix z,
 // thread t the columns 8 (t % 8) .. of every 32nd row; the 32 sums are added in
-// order.  One run: the results; else a row of partial sums for k_column_join.
+// order.  One run: the results; else rows of partial sums for k_column_join.
 __global__ __launch_bounds__(256) void k_column_sum(const uint16_t* __restrict__ x0, const uint16_t* __restrict__ x1,
                                                     int64_t M, int H, int64_t rows, float* __restrict__ part,
                                                     __bf16* out0, __bf16* out1) {
@@ -397,14 +398,13 @@ hipError_t ln_forward(const LnArgs& a, hipStream_t s) {
 }
 
 template <typename T, int VEC>
-hipError_t ln_backward(const LnArgs& a, T* dw, T* db, hipStream_t s) {
-  int nb = 0;
+hipError_t ln_backward(const LnArgs& a, hipStream_t s) {
   if (a.M > 0) {
     // few rows: a workgroup each (32 rows of 2816: 8.6 us by wavefronts, which are few then)
     const bool wave = a.H <= ln_back_wave_h<T, VEC>() && a.M > kLnPartials;
     const int per = wave ? 64 : 256;
     const int ept = (a.H + per * VEC - 1) / (per * VEC) * VEC;
-    nb = (int)std::min<int64_t>(wave ? (a.M + 7) / 8 : a.M, kLnPartials);
+    const int nb = ln_partials(a.M);
 #define W4A16_LN1(EPT_, TPR_, ADD_)                                                                             \
   hipLaunchKernelGGL((k_ln_backward<T, VEC, EPT_, TPR_, ADD_>), dim3(nb), dim3(ln_back_threads(TPR_)),            \
                      TPR_ == 64 ? 4 * 2 * EPT_ * 64 * 4 : 2 * 4 * 4, s, a)
@@ -428,16 +428,16 @@ hipError_t ln_backward(const LnArgs& a, T* dw, T* db, hipStream_t s) {
     }
 #undef W4A16_LN
 #undef W4A16_LN1
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL(k_column_join<T>, dim3((2 * a.H + 31) / 32), dim3(256), 0, s, a.part, nb, 2 * a.H, a.H, dw, db);
   return hipGetLastError();
 }
 
 }  // namespace
 
-int ln_partials(int64_t M) { return (int)std::min<int64_t>(M, kLnPartials); }
+int ln_partials(int64_t M) {
+  // a workgroup per row, or per eight rows at a time
+  return (int)(M <= kLnPartials ? M : std::min<int64_t>((M + 7) / 8, kLnPartials));
+}
 
 hipError_t launch_ln_forward(int dtype, const LnArgs& a, hipStream_t s) {
   if (a.M == 0) return hipSuccess;
@@ -451,21 +451,27 @@ hipError_t launch_ln_forward(int dtype, const LnArgs& a, hipStream_t s) {
   }
 }
 
-hipError_t launch_ln_backward(int dtype, const LnArgs& a, void* dw, void* db, hipStream_t s) {
+hipError_t launch_ln_backward(int dtype, const LnArgs& a, hipStream_t s) {
   if (a.H <= 0 || a.H > kLnMaxH || a.M < 0) return hipErrorInvalidValue;
   const bool v = ln_vector(a, dtype == 2 ? 4 : 2);
   switch (dtype) {
-    case 0:
-      return v ? ln_backward<__bf16, 8>(a, static_cast<__bf16*>(dw), static_cast<__bf16*>(db), s)
-               : ln_backward<__bf16, 1>(a, static_cast<__bf16*>(dw), static_cast<__bf16*>(db), s);
-    case 1:
-      return v ? ln_backward<_Float16, 8>(a, static_cast<_Float16*>(dw), static_cast<_Float16*>(db), s)
-               : ln_backward<_Float16, 1>(a, static_cast<_Float16*>(dw), static_cast<_Float16*>(db), s);
-    case 2:
-      return v ? ln_backward<float, 4>(a, static_cast<float*>(dw), static_cast<float*>(db), s)
-               : ln_backward<float, 1>(a, static_cast<float*>(dw), static_cast<float*>(db), s);
+    case 0: return v ? ln_backward<__bf16, 8>(a, s) : ln_backward<__bf16, 1>(a, s);
+    case 1: return v ? ln_backward<_Float16, 8>(a, s) : ln_backward<_Float16, 1>(a, s);
+    case 2: return v ? ln_backward<float, 4>(a, s) : ln_backward<float, 1>(a, s);
     default: return hipErrorInvalidValue;
   }
+}
+
+hipError_t launch_column_join(int dtype, const LnJoin& a, hipStream_t s) {
+  if (a.n == 0) return hipSuccess;
+  const dim3 grid((2 * a.H + 31) / 32, a.n);
+  switch (dtype) {
+    case 0: hipLaunchKernelGGL(k_column_join<__bf16>, grid, dim3(256), 0, s, a); break;
+    case 1: hipLaunchKernelGGL(k_column_join<_Float16>, grid, dim3(256), 0, s, a); break;
+    case 2: hipLaunchKernelGGL(k_column_join<float>, grid, dim3(256), 0, s, a); break;
+    default: return hipErrorInvalidValue;
+  }
+  return hipGetLastError();
 }
 
 int column_sum_partials(int64_t M) {
@@ -476,12 +482,8 @@ hipError_t launch_column_sums(const uint16_t* x0, const uint16_t* x1, int64_t M,
                               uint16_t* out1, hipStream_t s) {
   if (H <= 0 || H % 8 != 0 || M < 0) return hipErrorInvalidValue;
   const int n = std::max(1, column_sum_partials(M));
-  const int64_t rows = (M + n - 1) / n;
-  __bf16 *o0 = reinterpret_cast<__bf16*>(out0), *o1 = reinterpret_cast<__bf16*>(out1);
-  hipLaunchKernelGGL(k_column_sum, dim3((H + 63) / 64, n, 2), dim3(256), 0, s, x0, x1, M, H, rows, part, o0, o1);
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess || n == 1) return e;
-  hipLaunchKernelGGL(k_column_join<__bf16>, dim3((2 * H + 31) / 32), dim3(256), 0, s, part, n, 2 * H, H, o0, o1);
+  hipLaunchKernelGGL(k_column_sum, dim3((H + 63) / 64, n, 2), dim3(256), 0, s, x0, x1, M, H, (M + n - 1) / n, part,
+                     reinterpret_cast<__bf16*>(out0), reinterpret_cast<__bf16*>(out1));
   return hipGetLastError();
 }
 

@@ -354,9 +354,23 @@ constexpr int kLnMaxGrid = 4096;
 constexpr int64_t kLnWaveRows = 512;
 int ln_partials(int64_t M);
 hipError_t launch_ln_forward(int dtype, const LnArgs& a, hipStream_t s);
-hipError_t launch_ln_backward(int dtype, const LnArgs& a, void* dw, void* db, hipStream_t s);
-// out0, out1 = the column sums of two bf16 matrices of M rows; part:
-// column_sum_partials(M) * 2 H floats
+// dx, and the column sums' partial rows (a.part: ln_partials(M) rows of 2 H
+// floats, dw then db), which launch_column_join adds
+hipError_t launch_ln_backward(int dtype, const LnArgs& a, hipStream_t s);
+// up to three sets of nb partial rows of 2 H floats and the tensors that their
+// halves' sums go to
+struct LnJoin {
+  struct {
+    const float* part;
+    int nb;
+    void *out0, *out1;
+  } seg[3];
+  int n, H;
+};
+hipError_t launch_column_join(int dtype, const LnJoin& a, hipStream_t s);
+// out0, out1 = the column sums of two bf16 matrices of M rows; where
+// column_sum_partials(M) is not 0 that many partial rows of 2 H floats in part
+// instead, for launch_column_join
 constexpr int kColSumPartials = 128;
 constexpr int64_t kColSumRows = 512;
 int column_sum_partials(int64_t M);
@@ -389,7 +403,7 @@ struct DgArgs {
   DgProblem prob[kDgMaxProblems];
   int nprob;
   int K;        // of one pair; a multiple of 32 (TN: any)
-  int mi, ni, ksplit;  // the plan
+  int mi, ni, kg, ksplit;  // the plan
   float* part;  // ksplit > 1: planes of partial sums
   int64_t plane;
   int tiles, nk, nk1;

@@ -98,22 +98,27 @@ inline int linear_w4_blocks(int64_t M, int64_t N, int cus, int max_blocks) {
 }
 
 // Dense GEMMs (gemm_dense.hpp): the tiles that are built, 32 mi rows x 32 ni
-// operand columns each, with the workgroups that share a CU and what a stage
-// of 32 k takes, in ns, for a workgroup alone on a CU and for each of several
-// (256 .. 1024 tiles of K = 512 and 2816, the three layouts' mean).
-#define W4A16_DG_TILES(X) \
-  X(8, 8, 1, 670, 670)    \
-  X(8, 6, 1, 560, 560)    \
-  X(6, 8, 1, 560, 560)    \
-  X(6, 6, 2, 485, 430)    \
-  X(8, 4, 2, 460, 420)    \
-  X(4, 8, 2, 490, 415)    \
-  X(6, 4, 2, 370, 325)    \
-  X(4, 6, 2, 380, 315)    \
-  X(4, 4, 2, 300, 250)    \
-  X(4, 2, 3, 215, 190)    \
-  X(2, 4, 3, 215, 185)    \
-  X(2, 2, 4, 155, 125)
+// operand columns by kg groups of wavefronts, with the workgroups that share a
+// CU and what a stage of 32 k takes, in ns, for a group alone on a CU and for
+// each of several (256 .. 1024 tiles of K = 512 and 2816, the three layouts'
+// mean).
+#define W4A16_DG_TILES(X)    \
+  X(8, 8, 1, 1, 670, 670)    \
+  X(8, 6, 1, 1, 560, 560)    \
+  X(6, 8, 1, 1, 560, 560)    \
+  X(6, 6, 1, 2, 485, 430)    \
+  X(8, 4, 1, 2, 460, 420)    \
+  X(4, 8, 1, 2, 490, 415)    \
+  X(6, 4, 1, 2, 370, 325)    \
+  X(4, 6, 1, 2, 380, 315)    \
+  X(4, 4, 1, 2, 300, 250)    \
+  X(4, 4, 2, 1, 300, 250)    \
+  X(4, 2, 1, 3, 215, 190)    \
+  X(4, 2, 2, 1, 215, 190)    \
+  X(2, 4, 1, 3, 215, 185)    \
+  X(2, 4, 2, 1, 215, 185)    \
+  X(2, 2, 1, 4, 155, 125)    \
+  X(2, 2, 4, 1, 155, 125)
 // Products of few rows run as the weights' stream (gemm_thin.hpp): x W^T up to
 // 64 rows (2816 x 2816, split over workgroups / streamed: 1 row 9.0/5.1 us, 32
 // 10.0/6.1, 64 9.5/8.2), dy W up to 32 (32 rows 9.8/8.3 us, 64 10.9/10.6; two
@@ -124,7 +129,7 @@ struct DenseShape {
   int64_t rows, cols;  // of the product (gate/up: both halves' columns)
 };
 struct DensePlan {
-  int mi, ni, ksplit;
+  int mi, ni, kg, ksplit;
 };
 // planes of fp32 partial sums that a split product may take: at most 8, at
 // most 32 MB
@@ -136,33 +141,34 @@ inline int dense_part_planes(int64_t plane) {
 }
 // The tile and split whose time comes out least: rounds of the workgroups that
 // fit at once, each nk stages and an epilogue of some 210 ns per 16 x 16 tiles
-// of a wavefront; a split's launch that adds its planes takes 3 us and their
+// of a wavefront; joining groups takes 2 us more, a split's launch that adds its planes takes 3 us and their
 // bytes at 4 TB/s.
 inline DensePlan dense_plan(const DenseShape* sh, int nprob, int nk, int max_split, int cus) {
-  DensePlan best{0, 0, 1};
+  DensePlan best{0, 0, 1, 1};
   int64_t least = 0, plane = 0;
   for (int i = 0; i < nprob; ++i) plane += sh[i].rows * sh[i].cols;
-  auto consider = [&](int mi, int ni, int occ, int64_t alone, int64_t each) {
+  auto consider = [&](int mi, int ni, int kg, int occ, int64_t alone, int64_t each) {
     int64_t tiles = 0;
     for (int i = 0; i < nprob; ++i)
       tiles += (sh[i].rows + 32 * mi - 1) / (32 * mi) * ((sh[i].cols + 32 * ni - 1) / (32 * ni));
-    for (int ks = 1; ks <= max_split && (ks == 1 || nk >= 2 * ks); ++ks) {
+    for (int ks = 1; ks <= max_split && (ks == 1 || nk >= 2 * ks * kg); ++ks) {
       const int64_t n = (tiles * ks + cus - 1) / cus;  // workgroups a CU gets
-      const int64_t stages = (nk + ks - 1) / ks;
+      const int64_t stages = (nk + ks * kg - 1) / (ks * kg);
       auto round = [&](int64_t w) {
-        const int64_t step = w * each > alone ? w * each : alone;
-        return (stages + 2) * step + w * (ks > 1 ? 300 : 210) * mi * ni;
+        const int64_t step = w * kg * each > alone ? w * kg * each : alone;
+        return (stages + 2) * step + w * ((ks > 1 ? 300 : 210) + 50 * (kg - 1)) * mi * ni;
       };
       int64_t c = n / occ * round(occ);
       if (n % occ != 0) c += round(n % occ);
       if (ks > 1) c += 3000 + (2 * ks + 1) * plane / 1000;
+      if (kg > 1) c += 2000;
       if (best.mi == 0 || c < least) {
-        best = DensePlan{mi, ni, ks};
+        best = DensePlan{mi, ni, kg, ks};
         least = c;
       }
     }
   };
-#define W4A16_DG(MI_, NI_, OCC_, ALONE_, EACH_) consider(MI_, NI_, OCC_, ALONE_, EACH_);
+#define W4A16_DG(MI_, NI_, KG_, OCC_, ALONE_, EACH_) consider(MI_, NI_, KG_, OCC_, ALONE_, EACH_);
   W4A16_DG_TILES(W4A16_DG)
 #undef W4A16_DG
   return best;
