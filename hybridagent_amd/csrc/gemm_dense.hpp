@@ -49,6 +49,10 @@ constexpr int kDgGroupM = 4;  // row tiles that run with a column tile
 constexpr int dg_bm(int mi) { return 32 * mi; }
 constexpr int dg_bn(int epi, int ni) { return epi == kDgGateUp ? 16 * ni : 32 * ni; }
 
+// the epilogue's LDS rows (in the ring's place, behind what the groups left):
+// floats between them, 4 modulo the 64 banks where that is not twice the row
+constexpr int dg_epi_pitch(int no) { return no > 4 ? 132 : no > 2 ? 68 : 16 * no + 4; }
+
 typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4_t;
 
 // s_waitcnt vmcnt(N), nothing else
@@ -153,8 +157,54 @@ __device__ __forceinline__ void dg_unpack8(u32x4_t u, float v[8]) {
     v[2 * i + 1] = bf16_bits_to_f32(w[i] >> 16);
   }
 }
-__device__ __forceinline__ void dg_st8(uint16_t* p, const float v[8]) {
-  st16(p, u32x4_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])});
+__device__ __forceinline__ u32x4_t dg_pack8(const float v[8]) {
+  return u32x4_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
+}
+
+// What an epilogue reads and writes, from a row on: buffers that end with the
+// problem's last row, so that elements past it (and kDgOut) read as zero and
+// are not written.  Element offsets o of a row-major [rows][N] (at most 256
+// rows of 32768: byte offsets below 2^25).
+struct DgTarget {
+  __amdgpu_buffer_rsrc_t out, out2, out3, in, in2, part, part2;
+  const uint16_t* bias;
+  bool keep;  // kDgGateUp: out2, out3 wanted
+};
+constexpr int kDgOut = 1 << 28;
+__device__ __forceinline__ DgTarget dg_target(const DgArgs& a, const DgProblem& p, int split, int row, int rows,
+                                              bool two) {
+  const int left = max(min(p.M - row, rows), 0);
+  const int64_t at = (int64_t)row * p.N;
+  const uint32_t bytes = (uint32_t)(left * p.N) * 2u;
+  auto at16 = [&](const uint16_t* q) { return make_rsrc(q + at, q != nullptr ? bytes : 0u); };
+  DgTarget g;
+  g.out = at16(p.e.out);
+  g.out2 = at16(p.e.out2);
+  g.out3 = at16(p.e.out3);
+  g.in = at16(p.e.in);
+  g.in2 = at16(p.e.in2);
+  const float* part = a.part + split * a.plane + p.part0 + at;
+  g.part = make_rsrc(part, a.ksplit > 1 ? 2u * bytes : 0u);
+  g.part2 = make_rsrc(part + (int64_t)p.M * p.N, a.ksplit > 1 && two ? 2u * bytes : 0u);
+  g.bias = p.e.bias;
+  g.keep = p.e.out2 != nullptr;
+  return g;
+}
+__device__ __forceinline__ void dg_st8(__amdgpu_buffer_rsrc_t r, int o, const float v[8]) {
+  __builtin_amdgcn_raw_buffer_store_b128(dg_pack8(v), r, 2 * o, 0, 0);
+}
+template <bool TWO>
+__device__ __forceinline__ void dg_partial(const DgTarget& g, int o, const float v[8], const float v2[8]) {
+#pragma unroll
+  for (int k = 0; k < 8; k += 4) {
+    __builtin_amdgcn_raw_buffer_store_b128(u32x4_t{__float_as_uint(v[k]), __float_as_uint(v[k + 1]),
+                                                   __float_as_uint(v[k + 2]), __float_as_uint(v[k + 3])},
+                                           g.part, 4 * (o + k), 0, 0);
+    if (TWO)
+      __builtin_amdgcn_raw_buffer_store_b128(u32x4_t{__float_as_uint(v2[k]), __float_as_uint(v2[k + 1]),
+                                                     __float_as_uint(v2[k + 2]), __float_as_uint(v2[k + 3])},
+                                             g.part2, 4 * (o + k), 0, 0);
+  }
 }
 
 // d/dx gelu_tanh = s + x s (1 - s) 2 u', s = 1 / (1 + exp(-2 u)),
@@ -184,35 +234,40 @@ __device__ __forceinline__ void gelu_erf_and_slope(float x, float* act, float* s
   *slope = cdf + x * (0.3989422804014327f * e);
 }
 
-// what the epilogue reads of e.in and e.in2 at element o
+// what the epilogue reads of in and in2 at element o
 struct DgIn {
   u32x4_t a, b;
 };
 template <int EPI>
-__device__ __forceinline__ DgIn dg_fetch(const DgEpilogue& e, int64_t o) {
+__device__ __forceinline__ DgIn dg_fetch(const DgTarget& g, int o) {
   DgIn r;
   r.a = r.b = u32x4_t{0u, 0u, 0u, 0u};
-  if (EPI == kDgGateUpBack || EPI == kDgBiasResidual || EPI == kDgGeluBack) r.a = ld16(e.in + o);
-  if (EPI == kDgGateUpBack) r.b = ld16(e.in2 + o);
+  if (EPI == kDgGateUpBack || EPI == kDgBiasResidual || EPI == kDgGeluBack) r.a = buf_ld16(g.in, 2 * o, 0);
+  if (EPI == kDgGateUpBack) r.b = buf_ld16(g.in2, 2 * o, 0);
   return r;
 }
 
-// v: the sums (v2: kDgGateUp's up sums); o: the element's offset in row-major [M, N]
+// the bias of columns n .. n + 7 (element o: past the problem none)
+__device__ __forceinline__ u32x4_t dg_bias(const DgTarget& g, int o, int n) {
+  return o == kDgOut ? u32x4_t{0u, 0u, 0u, 0u} : ld16(g.bias + n);
+}
+
+// v: the sums (v2: kDgGateUp's up sums) of the target's elements o .. o + 7, column n on
 template <int EPI>
-__device__ __forceinline__ void dg_finish(const DgEpilogue& e, int64_t o, int n, const float v[8], const float v2[8],
+__device__ __forceinline__ void dg_finish(const DgTarget& g, int o, int n, const float v[8], const float v2[8],
                                           const DgIn& in) {
   float r[8], s[8];
   if constexpr (EPI == kDgPlain) {
-    dg_st8(e.out + o, v);
+    dg_st8(g.out, o, v);
   } else if constexpr (EPI == kDgGateUp) {
     // h = gelu_tanh(a) b from the sums themselves, rounded once; a and b are
     // rounded for the backward pass alone
 #pragma unroll
     for (int i = 0; i < 8; ++i) r[i] = gelu_tanh_f32(v[i]) * v2[i];
-    dg_st8(e.out + o, r);
-    if (e.out2 != nullptr) {
-      dg_st8(e.out2 + o, v);
-      dg_st8(e.out3 + o, v2);
+    dg_st8(g.out, o, r);
+    if (g.keep) {
+      dg_st8(g.out2, o, v);
+      dg_st8(g.out3, o, v2);
     }
   } else if constexpr (EPI == kDgGateUpBack) {
     float a[8], b[8];
@@ -225,25 +280,25 @@ __device__ __forceinline__ void dg_finish(const DgEpilogue& e, int64_t o, int n,
       r[i] = v[i] * b[i] * slope;
       s[i] = v[i] * act;
     }
-    dg_st8(e.out + o, r);
-    dg_st8(e.out2 + o, s);
+    dg_st8(g.out, o, r);
+    dg_st8(g.out2, o, s);
   } else if constexpr (EPI == kDgBiasGelu) {
-    dg_unpack8(ld16(e.bias + n), s);
+    dg_unpack8(dg_bias(g, o, n), s);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       float slope;
       s[i] += v[i];
       gelu_erf_and_slope(s[i], &r[i], &slope);
     }
-    dg_st8(e.out + o, r);
-    dg_st8(e.out2 + o, s);
+    dg_st8(g.out, o, r);
+    dg_st8(g.out2, o, s);
   } else if constexpr (EPI == kDgBiasResidual) {
     float b[8];
-    dg_unpack8(ld16(e.bias + n), b);
+    dg_unpack8(dg_bias(g, o, n), b);
     dg_unpack8(in.a, s);
 #pragma unroll
     for (int i = 0; i < 8; ++i) r[i] = s[i] + (v[i] + b[i]);
-    dg_st8(e.out + o, r);
+    dg_st8(g.out, o, r);
   } else if constexpr (EPI == kDgGeluBack) {
     dg_unpack8(in.a, s);
 #pragma unroll
@@ -252,7 +307,7 @@ __device__ __forceinline__ void dg_finish(const DgEpilogue& e, int64_t o, int n,
       gelu_erf_and_slope(s[i], &act, &slope);
       r[i] = v[i] * slope;
     }
-    dg_st8(e.out + o, r);
+    dg_st8(g.out, o, r);
   }
 }
 
@@ -286,7 +341,7 @@ __global__ __launch_bounds__(KG * kDgThreads, MI * NI > 36 ? 1 : KG > 2 ? KG : 2
   item -= split * a.tiles;
   int pi = 0;
   while (pi + 1 < a.nprob && item >= a.prob[pi + 1].tile0) ++pi;
-  const DgProblem p = a.prob[pi];
+  const DgProblem& p = a.prob[pi];
   item -= p.tile0;
   const int n_mt = (p.M + BM - 1) / BM, n_nt = (p.N + BN - 1) / BN;
   const int grp = item / (kDgGroupM * n_nt);
@@ -297,16 +352,22 @@ __global__ __launch_bounds__(KG * kDgThreads, MI * NI > 36 ? 1 : KG > 2 ? KG : 2
   // the group's stages; every group runs as many (those past its range multiply
   // the zeros that empty descriptors give)
   const int per = (a.nk + a.ksplit * KG - 1) / (a.ksplit * KG);
-  const int t0 = (split * KG + group) * per, t1 = min(a.nk, t0 + per), tend = t0 + per;
-
+  // what is loaded next, kStages ahead of the multiplication: stage t of the
+  // operands (their values here: the loop reads no arguments)
+  struct Feed {
+    const uint16_t *A, *A2, *B, *B2;
+    int M, N, lda, ldb, t, end;
+  };
+  Feed f{p.A, p.A2, p.B, p.B2, p.M, p.N, p.lda, p.ldb, (split * KG + group) * per, 0};
+  f.end = min(a.nk, f.t + per);
   OA oa;
   OB ob;
-  oa.init(m0, p.M, p.lda, wave);
-  ob.init(n0, p.N, p.ldb, wave);
+  oa.init(m0, f.M, f.lda, wave);
+  ob.init(n0, f.N, f.ldb, wave);
   oa.init_frag(wave >> 1);
   ob.init_frag(wave & 1);
 
-  // Where stage t's loads come from.  The descriptors are empty past the
+  // Where the next stage's loads come from.  The descriptors are empty past the
   // range; cols: they start at the stage's first k and end with row K - 1, so
   // that rows past K read as zero.  Rows: stages of the second pair (t >= nk1)
   // follow the first's.
@@ -314,20 +375,20 @@ __global__ __launch_bounds__(KG * kDgThreads, MI * NI > 36 ? 1 : KG > 2 ? KG : 2
     __amdgpu_buffer_rsrc_t a, b, b2;
     int off;
   };
-  auto source = [&](int t) {
-    const bool two = LAYOUT == kDgNN && t >= a.nk1;
-    const int tt = two ? t - a.nk1 : t;
-    const bool any = t < t1;
+  auto source = [&] {
+    const bool two = LAYOUT == kDgNN && f.t >= a.nk1;
+    const int tt = two ? f.t - a.nk1 : f.t;
+    const bool any = f.t < f.end;
     const int left = min(kDgKT, a.K - tt * kDgKT);
-    const uint16_t* pa = two ? p.A2 : p.A;
-    const uint16_t* pb = two ? p.B2 : p.B;
+    const uint16_t* pa = two ? f.A2 : f.A;
+    const uint16_t* pb = two ? f.B2 : f.B;
     Src r;
-    r.a = AC ? make_rsrc(pa + (int64_t)tt * kDgKT * p.lda + m0, any ? (uint32_t)(left * p.lda - m0) * 2u : 0u)
-             : make_rsrc(pa + (int64_t)m0 * p.lda, any ? (uint32_t)(min(p.M - m0, BM) * p.lda) * 2u : 0u);
-    const uint32_t bbytes = (uint32_t)(min(p.N - n0, BN) * p.ldb) * 2u;
-    r.b = BC ? make_rsrc(pb + (int64_t)tt * kDgKT * p.ldb + n0, any ? (uint32_t)(left * p.ldb - n0) * 2u : 0u)
-             : make_rsrc(pb + (int64_t)n0 * p.ldb, any ? bbytes : 0u);
-    r.b2 = GU ? make_rsrc(p.B2 + (int64_t)n0 * p.ldb, any ? bbytes : 0u) : r.b;
+    r.a = AC ? make_rsrc(pa + (int64_t)tt * kDgKT * f.lda + m0, any ? (uint32_t)(left * f.lda - m0) * 2u : 0u)
+             : make_rsrc(pa + (int64_t)m0 * f.lda, any ? (uint32_t)(min(f.M - m0, BM) * f.lda) * 2u : 0u);
+    const uint32_t bbytes = (uint32_t)(min(f.N - n0, BN) * f.ldb) * 2u;
+    r.b = BC ? make_rsrc(pb + (int64_t)tt * kDgKT * f.ldb + n0, any ? (uint32_t)(left * f.ldb - n0) * 2u : 0u)
+             : make_rsrc(pb + (int64_t)n0 * f.ldb, any ? bbytes : 0u);
+    r.b2 = GU ? make_rsrc(f.B2 + (int64_t)n0 * f.ldb, any ? bbytes : 0u) : r.b;
     r.off = tt * (kDgKT * 2);
     return r;
   };
@@ -349,13 +410,17 @@ __global__ __launch_bounds__(KG * kDgThreads, MI * NI > 36 ? 1 : KG > 2 ? KG : 2
   // it; otherwise the compiler moves up to 200 of them around per stage.
   f32x4_t acc[MI][NI];
   constexpr bool kAccRegs = MI * NI > 36;
+  auto pin = [&] {
+    if constexpr (kAccRegs) {
 #pragma unroll
-  for (int m = 0; m < MI; ++m)
+      for (int m = 0; m < MI; ++m)
 #pragma unroll
-    for (int n = 0; n < NI; ++n) {
-      acc[m][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-      if (kAccRegs) asm volatile("" : "+a"(acc[m][n]));
+        for (int n = 0; n < NI; ++n) asm volatile("" : "+a"(acc[m][n]));
     }
+  };
+  constexpr int NO = GU ? NI / 2 : NI;  // 16-column tiles of results per wavefront
+  constexpr int kPlanes = GU ? 2 : 1;
+  constexpr int kIter = (2 * 16 * NO + 63) / 64;
   // column fragments twice where there is room: those of the next stage are
   // then read all along a stage
   constexpr int kB = kAccRegs ? 2 : 1;
@@ -363,9 +428,10 @@ __global__ __launch_bounds__(KG * kDgThreads, MI * NI > 36 ? 1 : KG > 2 ? KG : 2
 
 #pragma unroll
   for (int s = 0; s < kStages; ++s) {
-    const Src r = source(t0 + s);
+    const Src r = source();
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) issue(r, ring + s * kStage, j);
+    ++f.t;
   }
   dg_wait_vm<(kStages - 1) * kLoads>();
   px_barrier();
@@ -380,12 +446,12 @@ __global__ __launch_bounds__(KG * kDgThreads, MI * NI > 36 ? 1 : KG > 2 ? KG : 2
   // fragment of stage t + 1 after its last MFMA.  Reads and loads go one by one
   // between the MFMAs: one after every second keeps the matrix unit fed.
   int slot = 0;
-  auto stage = [&](int t, auto cur_) {
+  auto stage = [&](auto cur_) {
     constexpr int cur = kB == 2 ? decltype(cur_)::value : 0, nxt = kB == 2 ? cur ^ 1 : 0;
     const int ns = slot == kStages - 1 ? 0 : slot + 1;
     unsigned char* refill = ring + slot * kStage;
     const unsigned char* st = ring + ns * kStage;
-    const Src src = source(t + kStages);
+    const Src src = source();
 #pragma unroll
     for (int n = 0; n < NI; ++n) acc[0][n] = mfma16(fb[cur][n], fa[0], acc[0][n]);
     __builtin_amdgcn_sched_barrier(0);
@@ -457,29 +523,25 @@ __global__ __launch_bounds__(KG * kDgThreads, MI * NI > 36 ? 1 : KG > 2 ? KG : 2
       fa[MI - 1] = oa.frag(st, MI - 1);
     }
     slot = ns;
+    ++f.t;
   };
+
+#pragma unroll
+  for (int m = 0; m < MI; ++m)
+#pragma unroll
+    for (int n = 0; n < NI; ++n) acc[m][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  pin();
   if constexpr (kB == 2) {
-    for (int t = t0; t < tend; t += 2) {
-      stage(t, std::integral_constant<int, 0>{});
-      if (t + 1 < tend) stage(t + 1, std::integral_constant<int, 1>{});
+    for (int t = 0; t < per; t += 2) {
+      stage(std::integral_constant<int, 0>{});
+      if (t + 1 < per) stage(std::integral_constant<int, 1>{});
     }
   } else {
-    for (int t = t0; t < tend; ++t) stage(t, std::integral_constant<int, 0>{});
+    for (int t = 0; t < per; ++t) stage(std::integral_constant<int, 0>{});
   }
-  if constexpr (kAccRegs) {
-#pragma unroll
-    for (int m = 0; m < MI; ++m)
-#pragma unroll
-      for (int n = 0; n < NI; ++n) asm volatile("" : "+a"(acc[m][n]));
-  }
-  dg_wait_vm<0>();  // no load may land in another workgroup's LDS
-
-  // Epilogue, 16 rows of the wavefront at a time: lane l holds columns
-  // 4 (l / 16) .. + 3 of row l % 16 of each 16 x 16 tile; through the
-  // wavefront's own part of the LDS it gets eight consecutive columns of a row,
-  // so that every load and store is 16 bytes per lane and whole rows of the
-  // wavefront's columns (8 bytes in 32-byte pieces took half as long again).
-  px_barrier();  // every wavefront is past its reads of the ring
+  pin();
+  dg_wait_vm<0>();  // no load may land in what the ring's place holds next,
+  px_barrier();     // and every wavefront is past its reads of the ring
   if constexpr (KG > 1) {
     // the groups' sums, added in order
     f32x4_t* const sums = reinterpret_cast<f32x4_t*>(smem) + wave * MI * NI * 64 + lane;
@@ -498,26 +560,28 @@ __global__ __launch_bounds__(KG * kDgThreads, MI * NI > 36 ? 1 : KG > 2 ? KG : 2
 #pragma unroll
         for (int n = 0; n < NI; ++n) acc[m][n] += sums[((g - 1) * 4 * MI * NI + m * NI + n) * 64];
   }
-  constexpr int NO = GU ? NI / 2 : NI;
-  // floats; 4 modulo the 64 banks where that is not twice the row
-  constexpr int kPitch = NO > 4 ? 132 : NO > 2 ? 68 : 16 * NO + 4;
-  constexpr int kPlanes = GU ? 2 : 1;
-  constexpr int kSums = (KG - 1) * 4 * MI * NI * 1024;  // (what the groups left)
+
+  // Epilogue, 16 rows of the wavefront at a time: lane l holds columns
+  // 4 (l / 16) .. + 3 of row l % 16 of each 16 x 16 tile; through the
+  // wavefront's own part of the LDS it gets eight consecutive columns of a row,
+  // so that every load and store is 16 bytes per lane and whole rows of the
+  // wavefront's columns (8 bytes in 32-byte pieces took half as long again).
+  constexpr int kPitch = dg_epi_pitch(NO);
+  constexpr int kSums = (KG - 1) * 4 * MI * NI * 1024;
   static_assert(kSums + 4 * kPlanes * 16 * kPitch * 4 <= KG * kStages * kStage, "the epilogue's rows fit in the ring");
   float* const rows = reinterpret_cast<float*>(smem + kSums) + wave * kPlanes * 16 * kPitch;
-  constexpr int kIter = (2 * NO * 16 + 63) / 64;
   const int r0 = m0 + 16 * MI * (wave >> 1), c0 = n0 + 16 * NO * (wave & 1);
+  const DgTarget g = dg_target(a, p, split, r0, 16 * MI, GU);
 #pragma unroll
   for (int m = 0; m < MI; ++m) {
     DgIn in[kIter];
-    int64_t o[kIter];
-    bool ok[kIter];
+    int o[kIter];
 #pragma unroll
     for (int i = 0; i < kIter; ++i) {
-      const int idx = lane + 64 * i, row = r0 + 16 * m + idx / (2 * NO), col = c0 + 8 * (idx % (2 * NO));
-      ok[i] = idx < 32 * NO && row < p.M && col < p.N;
-      o[i] = (int64_t)row * p.N + col;
-      if (ok[i] && a.ksplit == 1) in[i] = dg_fetch<EPI>(p.e, o[i]);
+      const int idx = lane + 64 * i, col = c0 + 8 * (idx % (2 * NO));
+      // element of the target; past it for lanes past the tile and columns past the problem
+      o[i] = idx < 32 * NO && col < p.N ? (16 * m + idx / (2 * NO)) * p.N + col : kDgOut;
+      in[i] = dg_fetch<EPI>(g, o[i]);
     }
 #pragma unroll
     for (int n = 0; n < NO; ++n) {
@@ -527,8 +591,7 @@ __global__ __launch_bounds__(KG * kDgThreads, MI * NI > 36 ? 1 : KG > 2 ? KG : 2
     }
 #pragma unroll
     for (int i = 0; i < kIter; ++i) {
-      const int idx = lane + 64 * i;
-      if (!ok[i]) continue;
+      const int idx = min(lane + 64 * i, 32 * NO - 1);
       const float* q = rows + idx / (2 * NO) * kPitch + 8 * (idx % (2 * NO));
       float v[8], v2[8];
 #pragma unroll
@@ -536,17 +599,10 @@ __global__ __launch_bounds__(KG * kDgThreads, MI * NI > 36 ? 1 : KG > 2 ? KG : 2
         v[k] = q[k];
         v2[k] = GU ? q[16 * kPitch + k] : 0.f;
       }
-      if (a.ksplit > 1) {
-        float* d = a.part + split * a.plane + p.part0 + o[i];
-#pragma unroll
-        for (int k = 0; k < 8; k += 4) {
-          *reinterpret_cast<float4*>(d + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
-          if (GU)
-            *reinterpret_cast<float4*>(d + (int64_t)p.M * p.N + k) = make_float4(v2[k], v2[k + 1], v2[k + 2], v2[k + 3]);
-        }
-      } else {
-        dg_finish<EPI>(p.e, o[i], c0 + 8 * (idx % (2 * NO)), v, v2, in[i]);
-      }
+      if (a.ksplit > 1)
+        dg_partial<GU>(g, o[i], v, v2);
+      else
+        dg_finish<EPI>(g, o[i], c0 + 8 * (idx % (2 * NO)), v, v2, in[i]);
     }
   }
 }
@@ -555,13 +611,16 @@ __global__ __launch_bounds__(KG * kDgThreads, MI * NI > 36 ? 1 : KG > 2 ? KG : 2
 // epilogue; a thread has eight columns of one row.
 template <int EPI>
 __global__ __launch_bounds__(256) void k_gemm_dense_join(DgArgs a) {
-  const DgProblem p = a.prob[blockIdx.y];
-  const int64_t n8 = (int64_t)p.M * p.N / 8;
+  const DgProblem& p = a.prob[blockIdx.y];
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n8) return;
-  const int64_t o = 8 * i;
-  const DgIn in = dg_fetch<EPI>(p.e, o);
-  const float* q = a.part + p.part0 + o;
+  if (i >= (int64_t)p.M * p.N / 8) return;
+  const int row = (int)(8 * i / p.N), n = (int)(8 * i - (int64_t)row * p.N);
+  // from the workgroup's first row on: some 2048 elements of few rows, or of one
+  const int row0 = (int)((int64_t)blockIdx.x * 2048 / p.N);
+  const DgTarget g = dg_target(a, p, 0, row0, 256, false);
+  const int o = (row - row0) * p.N + n;
+  const DgIn in = dg_fetch<EPI>(g, o);
+  const float* q = a.part + p.part0 + 8 * i;
   float v[8], v2[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) v[k] = v2[k] = 0.f;
@@ -573,16 +632,16 @@ __global__ __launch_bounds__(256) void k_gemm_dense_join(DgArgs a) {
       if (EPI == kDgGateUp) v2[k] += q[s * a.plane + (int64_t)p.M * p.N + k];
     }
   }
-  dg_finish<EPI>(p.e, o, (int)(o % p.N), v, v2, in);
+  dg_finish<EPI>(g, o, n, v, v2, in);
 }
 
 template <int LAYOUT, int EPI, int MI, int NI, int KG>
 hipError_t dg_launch(const DgArgs& a, hipStream_t s) {
-  constexpr int lds = KG * dg_stages(MI, NI) * (32 * MI + 32 * NI) * kDgKT * 2;
+  constexpr int lds = KG * dg_stages(MI, NI) * 32 * (MI + NI) * kDgKT * 2;
   static_assert(lds <= 160 * 1024, "LDS of a CU");
-  const int64_t total = (int64_t)a.tiles * a.ksplit;
-  const int grid = (int)(8 * ((total + 7) / 8));
-  hipLaunchKernelGGL((k_gemm_dense<LAYOUT, EPI, MI, NI, KG>), dim3(grid), dim3(KG * kDgThreads), lds, s, a);
+  const int64_t groups = ((int64_t)a.tiles * a.ksplit + 7) / 8;  // of eight workgroups, one per XCD
+  hipLaunchKernelGGL((k_gemm_dense<LAYOUT, EPI, MI, NI, KG>), dim3((unsigned)(8 * groups)), dim3(KG * kDgThreads), lds,
+                     s, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.ksplit == 1) return e;
   int64_t most = 0;

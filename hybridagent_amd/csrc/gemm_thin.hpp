@@ -138,8 +138,9 @@ __global__ __launch_bounds__(kThinThreads) void k_gemm_thin(DgArgs a) {
   constexpr int NC = GU ? 2 : 4;  // 8-column pieces of a row
   const int row = threadIdx.x / NC, c = threadIdx.x % NC;
   if (row >= 16 * MT || m0 + row >= M || n0 + 8 * c >= N) return;
-  const int64_t o = (int64_t)(m0 + row) * N + n0 + 8 * c;
-  const DgIn in = dg_fetch<EPI>(p.e, o);
+  const DgTarget g = dg_target(a, p, 0, m0, 16 * MT, false);
+  const int o = row * N + n0 + 8 * c;
+  const DgIn in = dg_fetch<EPI>(g, o);
   float v[8], v2[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) v[k] = v2[k] = 0.f;
@@ -152,7 +153,7 @@ __global__ __launch_bounds__(kThinThreads) void k_gemm_thin(DgArgs a) {
       if (GU) v2[k] += q[16 + k];
     }
   }
-  dg_finish<EPI>(p.e, o, n0 + 8 * c, v, v2, in);
+  dg_finish<EPI>(g, o, n0 + 8 * c, v, v2, in);
 }
 
 template <int LAYOUT, int EPI>
