@@ -198,7 +198,7 @@ template <typename T, int VEC, int EPT, int TPR, bool ADD>
 __global__ __launch_bounds__(ln_back_threads(TPR)) void k_ln_backward(LnArgs a) {
   using Raw = LnRaw<T, VEC, EPT, TPR>;
   constexpr int RPB = ln_back_threads(TPR) / TPR;
-  extern __shared__ float smem[];  // TPR > 64: a row's sums; else column sums, [4][2][EPT][64]
+  extern __shared__ __align__(16) float smem[];  // TPR > 64: a row's sums; else column sums, [4][2][EPT][64]
   const int t = threadIdx.x % TPR;
   const int H = a.H;
   const float fh = (float)H;
@@ -245,26 +245,29 @@ __global__ __launch_bounds__(ln_back_threads(TPR)) void k_ln_backward(LnArgs a) 
     }
   }
   // the wavefronts' column sums: the upper half hand theirs to the lower half,
-  // until the first has them all (a value at its lane's place in a row of 64:
-  // no bank conflicts)
+  // until the first has them all (16 bytes per lane, a KiB per instruction)
   if constexpr (TPR == 64) {
     const int wave = threadIdx.x >> 6;
 #pragma unroll
     for (int half = RPB / 2; half >= 1; half /= 2) {
-      float* mine = smem + (wave & (half - 1)) * 2 * EPT * 64 + t;
+      f32x4_t* mine = reinterpret_cast<f32x4_t*>(smem) + (wave & (half - 1)) * (EPT / 2) * 64 + t;
       if (wave >= half && wave < 2 * half) {
 #pragma unroll
-        for (int i = 0; i < EPT; ++i) {
-          mine[64 * i] = dw[i];
-          mine[64 * (EPT + i)] = db[i];
+        for (int i = 0; i < EPT; i += 4) {
+          mine[16 * i] = f32x4_t{dw[i], dw[i + 1], dw[i + 2], dw[i + 3]};
+          mine[16 * (EPT + i)] = f32x4_t{db[i], db[i + 1], db[i + 2], db[i + 3]};
         }
       }
       __syncthreads();
       if (wave < half) {
 #pragma unroll
-        for (int i = 0; i < EPT; ++i) {
-          dw[i] += mine[64 * i];
-          db[i] += mine[64 * (EPT + i)];
+        for (int i = 0; i < EPT; i += 4) {
+          const f32x4_t u = mine[16 * i], v = mine[16 * (EPT + i)];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            dw[i + k] += u[k];
+            db[i + k] += v[k];
+          }
         }
       }
       __syncthreads();
