@@ -913,7 +913,7 @@ def gated_mlp(x: torch.Tensor, gate_w: torch.Tensor, up_w: torch.Tensor, down_w:
     """The gated feed-forward block (the shared MLP of backends.py:105-108):
     y = (gelu_tanh(x gate_w^T) * (x up_w^T)) down_w^T on bf16 [..., H], weights in the nn.Linear
     layout.  With ``return_saved`` (y, saved): what ``gated_mlp_backward`` needs, one uint8 tensor
-    of about 6 bytes per row and column of I."""
+    of about 10 bytes per row and column of I."""
     dev = _require_gpu(x, gate_w, up_w, down_w)
     x = _bf16(x, "x")
     gate_w, up_w, down_w, H, I = _mlp_weights(x, gate_w, up_w, down_w)

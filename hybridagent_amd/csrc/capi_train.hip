@@ -64,14 +64,15 @@ inline hipError_t product(int layout, int epi, const DgProblem& p, int64_t K, fl
 }
 
 struct MlpSaved {
-  uint16_t *gate, *up, *inter;
+  float *gate, *up;
+  uint16_t* inter;
   size_t bytes;
 };
 MlpSaved mlp_saved(void* p, int64_t M, int64_t I) {
   Carve c(p);
   MlpSaved s;
-  s.gate = c.take<uint16_t>(M * I);
-  s.up = c.take<uint16_t>(M * I);
+  s.gate = c.take<float>(M * I);
+  s.up = c.take<float>(M * I);
   s.inter = c.take<uint16_t>(M * I);
   s.bytes = c.used;
   return s;
@@ -230,7 +231,7 @@ int w4a16_gated_mlp(const uint16_t* x, const uint16_t* gate_w, const uint16_t* u
   DgEpilogue e = to(ws.inter);
   if (saved != nullptr) {
     const MlpSaved sv = mlp_saved(saved, M, I);
-    e = DgEpilogue{sv.inter, sv.gate, sv.up, nullptr, nullptr, nullptr};
+    e = DgEpilogue{sv.inter, nullptr, sv.gate, sv.up, nullptr, nullptr};
   }
   DgProblem p = problem(x, H, gate_w, H, M, I, e);
   p.B2 = up_w;
@@ -263,7 +264,7 @@ int w4a16_gated_mlp_backward(const uint16_t* dy, const uint16_t* x, const uint16
   // dh = dy Wd; da, db
   if (M > 0 && (dx || dgate_w || dup_w))
     st = product(kDgNN, kDgGateUpBack,
-                 problem(dy, H, down_w, I, M, I, DgEpilogue{ws.da, ws.db, nullptr, sv.gate, sv.up, nullptr}), H,
+                 problem(dy, H, down_w, I, M, I, DgEpilogue{ws.da, ws.db, sv.gate, sv.up, nullptr, nullptr}), H,
                  ws.part, s);
   if (st == hipSuccess && M > 0 && dx) {
     // dx = da Wg + db Wu
@@ -317,7 +318,7 @@ int w4a16_hybridlink_train(const uint16_t* h, const uint16_t* ln1_w, const uint1
                 problem(sv.a, H, p1_w, H, B, H, DgEpilogue{sv.g, sv.z, nullptr, nullptr, nullptr, p1_b}), H, part, s);
   if (e == hipSuccess)
     e = product(kDgNT, kDgBiasResidual,
-                problem(sv.g, H, p2_w, H, B, H, DgEpilogue{sv.r, nullptr, nullptr, h, nullptr, p2_b}), H, part, s);
+                problem(sv.g, H, p2_w, H, B, H, DgEpilogue{sv.r, nullptr, nullptr, nullptr, h, p2_b}), H, part, s);
   if (e == hipSuccess)
     e = launch_ln_forward(W4A16_BF16, ln_args(sv.r, ln2_w, ln2_b, out, sv.mean2, sv.rstd2, B, H, eps), s);
   return launch_status(e);
@@ -354,7 +355,7 @@ int w4a16_hybridlink_backward(const uint16_t* dout, const uint16_t* h, const uin
   // dz = (dr W2) gelu'(z), da = dz W1
   if (e == hipSuccess && B > 0)
     e = product(kDgNN, kDgGeluBack,
-                problem(ws.dr, H, p2_w, H, B, H, DgEpilogue{ws.dz, nullptr, nullptr, sv.z, nullptr, nullptr}), H,
+                problem(ws.dr, H, p2_w, H, B, H, DgEpilogue{ws.dz, nullptr, nullptr, nullptr, sv.z, nullptr}), H,
                 ws.part, s);
   if (e == hipSuccess && B > 0)
     e = product(kDgNN, kDgPlain, problem(ws.dz, H, p1_w, H, B, H, to(ws.da)), H, ws.part, s);

@@ -166,9 +166,9 @@ __device__ __forceinline__ u32x4_t dg_pack8(const float v[8]) {
 // are not written.  Element offsets o of a row-major [rows][N] (at most 256
 // rows of 32768: byte offsets below 2^25).
 struct DgTarget {
-  __amdgpu_buffer_rsrc_t out, out2, out3, in, in2, part, part2;
+  __amdgpu_buffer_rsrc_t out, out2, sum, sum2, in, part, part2;
   const uint16_t* bias;
-  bool keep;  // kDgGateUp: out2, out3 wanted
+  bool keep;  // kDgGateUp: sum, sum2 wanted
 };
 constexpr int kDgOut = 1 << 28;
 __device__ __forceinline__ DgTarget dg_target(const DgArgs& a, const DgProblem& p, int split, int row, int rows,
@@ -177,34 +177,29 @@ __device__ __forceinline__ DgTarget dg_target(const DgArgs& a, const DgProblem& 
   const int64_t at = (int64_t)row * p.N;
   const uint32_t bytes = (uint32_t)(left * p.N) * 2u;
   auto at16 = [&](const uint16_t* q) { return make_rsrc(q + at, q != nullptr ? bytes : 0u); };
+  auto at32 = [&](const float* q) { return make_rsrc(q + at, q != nullptr ? 2u * bytes : 0u); };
   DgTarget g;
   g.out = at16(p.e.out);
   g.out2 = at16(p.e.out2);
-  g.out3 = at16(p.e.out3);
+  g.sum = at32(p.e.sum);
+  g.sum2 = at32(p.e.sum2);
   g.in = at16(p.e.in);
-  g.in2 = at16(p.e.in2);
   const float* part = a.part + split * a.plane + p.part0 + at;
   g.part = make_rsrc(part, a.ksplit > 1 ? 2u * bytes : 0u);
   g.part2 = make_rsrc(part + (int64_t)p.M * p.N, a.ksplit > 1 && two ? 2u * bytes : 0u);
   g.bias = p.e.bias;
-  g.keep = p.e.out2 != nullptr;
+  g.keep = p.e.sum != nullptr;
   return g;
 }
 __device__ __forceinline__ void dg_st8(__amdgpu_buffer_rsrc_t r, int o, const float v[8]) {
   __builtin_amdgcn_raw_buffer_store_b128(dg_pack8(v), r, 2 * o, 0, 0);
 }
-template <bool TWO>
-__device__ __forceinline__ void dg_partial(const DgTarget& g, int o, const float v[8], const float v2[8]) {
+__device__ __forceinline__ void dg_st8_f32(__amdgpu_buffer_rsrc_t r, int o, const float v[8]) {
 #pragma unroll
-  for (int k = 0; k < 8; k += 4) {
+  for (int k = 0; k < 8; k += 4)
     __builtin_amdgcn_raw_buffer_store_b128(u32x4_t{__float_as_uint(v[k]), __float_as_uint(v[k + 1]),
                                                    __float_as_uint(v[k + 2]), __float_as_uint(v[k + 3])},
-                                           g.part, 4 * (o + k), 0, 0);
-    if (TWO)
-      __builtin_amdgcn_raw_buffer_store_b128(u32x4_t{__float_as_uint(v2[k]), __float_as_uint(v2[k + 1]),
-                                                     __float_as_uint(v2[k + 2]), __float_as_uint(v2[k + 3])},
-                                             g.part2, 4 * (o + k), 0, 0);
-  }
+                                           r, 4 * (o + k), 0, 0);
 }
 
 // d/dx gelu_tanh = s + x s (1 - s) 2 u', s = 1 / (1 + exp(-2 u)),
@@ -234,16 +229,22 @@ __device__ __forceinline__ void gelu_erf_and_slope(float x, float* act, float* s
   *slope = cdf + x * (0.3989422804014327f * e);
 }
 
-// what the epilogue reads of in and in2 at element o
+// what the epilogue reads at element o: in, or sum and sum2
 struct DgIn {
-  u32x4_t a, b;
+  u32x4_t v[4];
 };
 template <int EPI>
 __device__ __forceinline__ DgIn dg_fetch(const DgTarget& g, int o) {
   DgIn r;
-  r.a = r.b = u32x4_t{0u, 0u, 0u, 0u};
-  if (EPI == kDgGateUpBack || EPI == kDgBiasResidual || EPI == kDgGeluBack) r.a = buf_ld16(g.in, 2 * o, 0);
-  if (EPI == kDgGateUpBack) r.b = buf_ld16(g.in2, 2 * o, 0);
+  if (EPI == kDgGateUpBack) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      r.v[k] = buf_ld16(g.sum, 4 * o, 16 * k);
+      r.v[2 + k] = buf_ld16(g.sum2, 4 * o, 16 * k);
+    }
+  } else if (EPI == kDgBiasResidual || EPI == kDgGeluBack) {
+    r.v[0] = buf_ld16(g.in, 2 * o, 0);
+  }
   return r;
 }
 
@@ -260,24 +261,25 @@ __device__ __forceinline__ void dg_finish(const DgTarget& g, int o, int n, const
   if constexpr (EPI == kDgPlain) {
     dg_st8(g.out, o, v);
   } else if constexpr (EPI == kDgGateUp) {
-    // h = gelu_tanh(a) b from the sums themselves, rounded once; a and b are
-    // rounded for the backward pass alone
+    // h = gelu_tanh(a) b from the sums themselves, rounded once.  The backward
+    // pass gets them as they are: rounded, they would cost its gradients as
+    // much as da's and db's own rounding (relative error against 64 bits of dx,
+    // dgate and dup 3.0e-3 instead of 2.4e-3).
 #pragma unroll
     for (int i = 0; i < 8; ++i) r[i] = gelu_tanh_f32(v[i]) * v2[i];
     dg_st8(g.out, o, r);
     if (g.keep) {
-      dg_st8(g.out2, o, v);
-      dg_st8(g.out3, o, v2);
+      dg_st8_f32(g.sum, o, v);
+      dg_st8_f32(g.sum2, o, v2);
     }
   } else if constexpr (EPI == kDgGateUpBack) {
-    float a[8], b[8];
-    dg_unpack8(in.a, a);
-    dg_unpack8(in.b, b);
+    const uint32_t a[8] = {in.v[0].x, in.v[0].y, in.v[0].z, in.v[0].w, in.v[1].x, in.v[1].y, in.v[1].z, in.v[1].w};
+    const uint32_t b[8] = {in.v[2].x, in.v[2].y, in.v[2].z, in.v[2].w, in.v[3].x, in.v[3].y, in.v[3].z, in.v[3].w};
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       float act, slope;
-      gelu_tanh_and_slope(a[i], &act, &slope);
-      r[i] = v[i] * b[i] * slope;
+      gelu_tanh_and_slope(__uint_as_float(a[i]), &act, &slope);
+      r[i] = v[i] * __uint_as_float(b[i]) * slope;
       s[i] = v[i] * act;
     }
     dg_st8(g.out, o, r);
@@ -295,12 +297,12 @@ __device__ __forceinline__ void dg_finish(const DgTarget& g, int o, int n, const
   } else if constexpr (EPI == kDgBiasResidual) {
     float b[8];
     dg_unpack8(dg_bias(g, o, n), b);
-    dg_unpack8(in.a, s);
+    dg_unpack8(in.v[0], s);
 #pragma unroll
     for (int i = 0; i < 8; ++i) r[i] = s[i] + (v[i] + b[i]);
     dg_st8(g.out, o, r);
   } else if constexpr (EPI == kDgGeluBack) {
-    dg_unpack8(in.a, s);
+    dg_unpack8(in.v[0], s);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       float act, slope;
@@ -599,10 +601,12 @@ __global__ __launch_bounds__(KG * kDgThreads, MI * NI > 36 ? 1 : KG > 2 ? KG : 2
         v[k] = q[k];
         v2[k] = GU ? q[16 * kPitch + k] : 0.f;
       }
-      if (a.ksplit > 1)
-        dg_partial<GU>(g, o[i], v, v2);
-      else
+      if (a.ksplit > 1) {
+        dg_st8_f32(g.part, o[i], v);
+        if (GU) dg_st8_f32(g.part2, o[i], v2);
+      } else {
         dg_finish<EPI>(g, o[i], c0 + 8 * (idx % (2 * NO)), v, v2, in[i]);
+      }
     }
   }
 }

@@ -380,15 +380,16 @@ hipError_t launch_column_sums(const uint16_t* x0, const uint16_t* x1, int64_t M,
 enum DenseLayout { kDgNT = 0, kDgNN = 1, kDgTN = 2 };
 enum DenseEpilogue {
   kDgPlain = 0,        // out = C
-  kDgGateUp = 1,       // NT, B gate rows, B2 up rows: out = gelu_tanh(C) C2; out2, out3 (nullable) = C, C2
-  kDgGateUpBack = 2,   // NN, in = a, in2 = b: out = C b gelu_tanh'(a), out2 = C gelu_tanh(a)
+  kDgGateUp = 1,       // NT, B gate rows, B2 up rows: out = gelu_tanh(C) C2; sum, sum2 (nullable) = C, C2
+  kDgGateUpBack = 2,   // NN, sum = a, sum2 = b: out = C b gelu_tanh'(a), out2 = C gelu_tanh(a)
   kDgBiasGelu = 3,     // NT: out2 = z = C + bias, out = gelu_erf(z)
   kDgBiasResidual = 4, // NT: out = in + C + bias
   kDgGeluBack = 5      // NN: out = C gelu_erf'(in)
 };
 struct DgEpilogue {
-  uint16_t *out, *out2, *out3;
-  const uint16_t *in, *in2, *bias;
+  uint16_t *out, *out2;
+  float *sum, *sum2;  // fp32, written or read
+  const uint16_t *in, *bias;
 };
 struct DgProblem {
   const uint16_t *A, *A2, *B, *B2;  // NN: C = A B + A2 B2 (A2 null: A B alone)

@@ -407,7 +407,7 @@ W4A16_API int w4a16_layer_norm_backward(const void* dy, const void* x, const voi
  * once, from the fp32 sums (moe_ffn_block_forward rounds where the
  * reference's torch ops do: a, b, gelu(a) and h).  `saved` (NULL: a call
  * without a backward pass): w4a16_gated_mlp_saved_bytes(M, I) bytes that the
- * forward fills (a, b and h in bf16) and the backward of the same M, H, I reads.
+ * forward fills (a, b in fp32, h in bf16) and the backward of the same M, H, I reads.
  * backward, with dh = dy down_w:
  *   da = dh * b * gelu_tanh'(a), db = dh * gelu_tanh(a)   (rounded to bf16)
  *   dx = da gate_w + db up_w
