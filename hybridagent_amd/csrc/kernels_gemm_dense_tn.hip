@@ -31,7 +31,8 @@ hipError_t launch_gemm_dense(int layout, int epi, DgArgs a, hipStream_t s) {
                     a.prob[0].M <= dense_thin_rows(layout == kDgNN);
   if (thin) a.ksplit = 1;
   if (a.mi == 0 && !thin) {
-    const DensePlan pl = dense_plan(sh, a.nprob, a.nk, a.part != nullptr ? dense_part_planes(a.plane) : 1, device_cus());
+    const DensePlan pl = dense_plan(sh, a.nprob, a.nk, a.part != nullptr ? dense_part_planes(a.plane) : 1, device_cus(),
+                                    layout == kDgNT);
     a.mi = pl.mi;
     a.ni = pl.ni;
     a.kg = pl.kg;

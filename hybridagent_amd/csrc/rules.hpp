@@ -114,11 +114,11 @@ inline int linear_w4_blocks(int64_t M, int64_t N, int cus, int max_blocks) {
   X(4, 4, 1, 2, 300, 250)    \
   X(4, 4, 2, 1, 300, 250)    \
   X(4, 2, 1, 3, 215, 190)    \
-  X(4, 2, 2, 1, 215, 190)    \
   X(2, 4, 1, 3, 215, 185)    \
   X(2, 4, 2, 1, 215, 185)    \
   X(2, 2, 1, 4, 155, 125)    \
   X(2, 2, 4, 1, 155, 125)
+
 // Products of few rows run as the weights' stream (gemm_thin.hpp): x W^T up to
 // 64 rows (2816 x 2816, split over workgroups / streamed: 1 row 9.0/5.1 us, 32
 // 10.0/6.1, 64 9.5/8.2), dy W up to 32 (32 rows 9.8/8.3 us, 64 10.9/10.6; two
@@ -141,9 +141,12 @@ inline int dense_part_planes(int64_t plane) {
 }
 // The tile and split whose time comes out least: rounds of the workgroups that
 // fit at once, each nk stages and an epilogue of some 210 ns per 16 x 16 tiles
-// of a wavefront; joining groups takes 2 us more, a split's launch that adds its planes takes 3 us and their
-// bytes at 4 TB/s.
-inline DensePlan dense_plan(const DenseShape* sh, int nprob, int nk, int max_split, int cus) {
+// of a wavefront; a split's launch that adds its planes takes 3 us and their
+// bytes at 4 TB/s.  Two groups to a tile gain less in x W^T (`rows`: both
+// operands come in 64-byte pieces of rows): 517 rows, 2 x 4 tiles in two groups
+// / 4 x 2 in one, 2112 -> 2816 17.7 / 15.0 us there, dy W 2816 -> 2112 18.7 /
+// 22.2.  Over 27 products of 32 .. 2049 rows the plan is 2 % off the fastest.
+inline DensePlan dense_plan(const DenseShape* sh, int nprob, int nk, int max_split, int cus, bool rows) {
   DensePlan best{0, 0, 1, 1};
   int64_t least = 0, plane = 0;
   for (int i = 0; i < nprob; ++i) plane += sh[i].rows * sh[i].cols;
@@ -161,7 +164,7 @@ inline DensePlan dense_plan(const DenseShape* sh, int nprob, int nk, int max_spl
       int64_t c = n / occ * round(occ);
       if (n % occ != 0) c += round(n % occ);
       if (ks > 1) c += 3000 + (2 * ks + 1) * plane / 1000;
-      if (kg > 1) c += 2000;
+      if (rows && kg == 2) c += 2500;
       if (best.mi == 0 || c < least) {
         best = DensePlan{mi, ni, kg, ks};
         least = c;
