@@ -368,7 +368,8 @@ int w4a16_hybridlink_backward(const uint16_t* dout, const uint16_t* h, const uin
     a.part = B > 0 && part_floats(2 * H * H) > 0 ? ws.part : nullptr;
     e = launch_gemm_dense(kDgTN, kDgPlain, a, s);
   }
-  if (e == hipSuccess) e = launch_column_sums(ws.dr, ws.dz, B, (int)H, ws.cols, dp2_b, dp1_b, s);
+  const int sums = column_sum_partials(B);
+  if (e == hipSuccess && sums > 0) e = launch_column_sums(ws.dr, ws.dz, B, (int)H, ws.cols, s);
   // pre_ln, and the residual's dr
   LnArgs n1 = ln_args(h, ln1_w, nullptr, dh, sv.mean1, sv.rstd1, B, H, 0.f);
   n1.dy = ws.da;
@@ -376,10 +377,13 @@ int w4a16_hybridlink_backward(const uint16_t* dout, const uint16_t* h, const uin
   n1.part = ws.ln1;
   if (e == hipSuccess) e = launch_ln_backward(W4A16_BF16, n1, s);
   LnJoin j{};
-  j.seg[0] = {ws.ln1, ln_partials(B), dln1_w, dln1_b};
-  j.seg[1] = {ws.ln2, ln_partials(B), dln2_w, dln2_b};
-  j.seg[2] = {ws.cols, column_sum_partials(B), dp2_b, dp1_b};
-  j.n = column_sum_partials(B) > 0 ? 3 : 2;
+  j.seg[0] = {ws.ln1, ln_partials(B), dln1_w, dln1_b, nullptr, nullptr};
+  j.seg[1] = {ws.ln2, ln_partials(B), dln2_w, dln2_b, nullptr, nullptr};
+  if (sums > 0 || B == 0)
+    j.seg[2] = {ws.cols, sums, dp2_b, dp1_b, nullptr, nullptr};
+  else
+    j.seg[2] = {nullptr, (int)B, dp2_b, dp1_b, ws.dr, ws.dz};
+  j.n = 3;
   j.H = (int)H;
   if (e == hipSuccess) e = launch_column_join(W4A16_BF16, j, s);
   return launch_status(e);

@@ -296,42 +296,15 @@ __global__ __launch_bounds__(ln_back_threads(TPR)) void k_ln_backward(LnArgs a) 
     }
 }
 
-// Column sums of partial rows: segment blockIdx.y has nb rows of 2 H floats,
-// whose halves, rounded to T, are two gradients (null: not wanted).  A
-// workgroup has 32 columns, eight threads a column, each the partials i,
-// i + 8, ...; the eight sums are added in order.
-template <typename T>
-__global__ __launch_bounds__(256) void k_column_join(LnJoin a) {
-  __shared__ float s[8][32];
-  const auto& g = a.seg[blockIdx.y];
-  const int c = blockIdx.x * 32 + (threadIdx.x & 31), r = threadIdx.x >> 5, cols = 2 * a.H;
-  float v = 0.f;
-  if (c < cols) {
-#pragma unroll 8
-    for (int i = r; i < g.nb; i += 8) v += g.part[(int64_t)i * cols + c];
-  }
-  s[r][threadIdx.x & 31] = v;
-  __syncthreads();
-  if (threadIdx.x >= 32 || c >= cols) return;
-  float t = s[0][threadIdx.x];
-#pragma unroll
-  for (int i = 1; i < 8; ++i) t += s[i][threadIdx.x];
-  T* o = static_cast<T*>(c < a.H ? g.out0 : g.out1);
-  if (o != nullptr) o[c < a.H ? c : c - a.H] = (T)t;
-}
+constexpr int kSumPitch = 64 + 4;
 
-// Column sums of two bf16 matrices (the linears' bias gradients): workgroup
-// (x, y, z) has columns 64 x .. 64 x + 63 of the y-th run of rows of matrix z,
-// thread t the columns 8 (t % 8) .. of every 32nd row; the 32 sums are added in
-// order.  One run: the results; else rows of partial sums for k_column_join.
-__global__ __launch_bounds__(256) void k_column_sum(const uint16_t* __restrict__ x0, const uint16_t* __restrict__ x1,
-                                                    int64_t M, int H, int64_t rows, float* __restrict__ part,
-                                                    __bf16* out0, __bf16* out1) {
-  __shared__ float s[32][64 + 4];
-  const uint16_t* x = blockIdx.z == 0 ? x0 : x1;
+// Column sums of rows r0 .. r1 of a bf16 matrix, columns 64 block ..: thread t
+// has columns 8 (t % 8) .. of every 32nd row; the 32 sums are added in order.
+// The result is that of threads t < 64, for column 64 block + t.
+__device__ __forceinline__ float column_sum(const uint16_t* __restrict__ x, int64_t r0, int64_t r1, int H, int block,
+                                            float* s) {
   const int c = threadIdx.x & 7, r = threadIdx.x >> 3;
-  const int col = blockIdx.x * 64 + 8 * c;
-  const int64_t r0 = (int64_t)blockIdx.y * rows, r1 = min(M, r0 + rows);
+  const int col = block * 64 + 8 * c;
   float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   if (col < H) {
 #pragma unroll 4
@@ -346,17 +319,59 @@ __global__ __launch_bounds__(256) void k_column_sum(const uint16_t* __restrict__
     }
   }
 #pragma unroll
-  for (int k = 0; k < 8; ++k) s[r][8 * c + k] = v[k];
+  for (int k = 0; k < 8; ++k) s[r * kSumPitch + 8 * c + k] = v[k];
   __syncthreads();
-  const int o = blockIdx.x * 64 + (int)threadIdx.x;
-  if (threadIdx.x >= 64 || o >= H) return;
-  float t = s[0][threadIdx.x];
+  if (threadIdx.x >= 64) return 0.f;
+  float t = s[threadIdx.x];
 #pragma unroll
-  for (int i = 1; i < 32; ++i) t += s[i][threadIdx.x];
-  if (gridDim.y > 1)
-    part[((int64_t)blockIdx.y * 2 + blockIdx.z) * H + o] = t;
-  else
-    (blockIdx.z == 0 ? out0 : out1)[o] = (__bf16)t;
+  for (int i = 1; i < 32; ++i) t += s[i * kSumPitch + threadIdx.x];
+  return t;
+}
+
+// Partial column sums of two bf16 matrices of many rows (the linears' bias
+// gradients): workgroup (x, y, z) has 64 columns of the y-th run of rows of
+// matrix z.
+__global__ __launch_bounds__(256) void k_column_sum(const uint16_t* __restrict__ x0, const uint16_t* __restrict__ x1,
+                                                    int64_t M, int H, int64_t rows, float* __restrict__ part) {
+  __shared__ float s[32 * kSumPitch];
+  const int64_t r0 = (int64_t)blockIdx.y * rows;
+  const float t = column_sum(blockIdx.z == 0 ? x0 : x1, r0, min(M, r0 + rows), H, blockIdx.x, s);
+  const int o = blockIdx.x * 64 + (int)threadIdx.x;
+  if (threadIdx.x < 64 && o < H) part[((int64_t)blockIdx.y * 2 + blockIdx.z) * H + o] = t;
+}
+
+// Column sums of partial rows: segment blockIdx.y has nb rows of 2 H floats,
+// whose halves, rounded to T, are two gradients (null: not wanted).  A
+// workgroup has 32 columns, eight threads a column, each the partials i,
+// i + 8, ...; the eight sums are added in order.  A segment with x0 has no
+// partials: its gradients are the sums of two bf16 matrices of nb rows (32 rows
+// of 2816: 4 us less than with a launch of their own).
+template <typename T>
+__global__ __launch_bounds__(256) void k_column_join(LnJoin a) {
+  __shared__ float s[32 * kSumPitch];
+  const auto& g = a.seg[blockIdx.y];
+  if (std::is_same_v<T, __bf16> && g.x0 != nullptr) {
+    const int blocks = (a.H + 63) / 64, z = (int)blockIdx.x >= blocks, block = blockIdx.x - z * blocks;
+    if (block >= blocks) return;
+    const float t = column_sum(z ? g.x1 : g.x0, 0, g.nb, a.H, block, s);
+    const int o = block * 64 + (int)threadIdx.x;
+    if (threadIdx.x < 64 && o < a.H) static_cast<T*>(z ? g.out1 : g.out0)[o] = (T)t;
+    return;
+  }
+  const int c = blockIdx.x * 32 + (threadIdx.x & 31), r = threadIdx.x >> 5, cols = 2 * a.H;
+  float v = 0.f;
+  if (c < cols) {
+#pragma unroll 8
+    for (int i = r; i < g.nb; i += 8) v += g.part[(int64_t)i * cols + c];
+  }
+  s[threadIdx.x] = v;
+  __syncthreads();
+  if (threadIdx.x >= 32 || c >= cols) return;
+  float t = s[threadIdx.x];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) t += s[32 * i + threadIdx.x];
+  T* o = static_cast<T*>(c < a.H ? g.out0 : g.out1);
+  if (o != nullptr) o[c < a.H ? c : c - a.H] = (T)t;
 }
 
 namespace {
@@ -481,12 +496,10 @@ int column_sum_partials(int64_t M) {
   return M <= kColSumRows ? 0 : (int)std::min<int64_t>((M + kColSumRows - 1) / kColSumRows, kColSumPartials);
 }
 
-hipError_t launch_column_sums(const uint16_t* x0, const uint16_t* x1, int64_t M, int H, float* part, uint16_t* out0,
-                              uint16_t* out1, hipStream_t s) {
-  if (H <= 0 || H % 8 != 0 || M < 0) return hipErrorInvalidValue;
-  const int n = std::max(1, column_sum_partials(M));
-  hipLaunchKernelGGL(k_column_sum, dim3((H + 63) / 64, n, 2), dim3(256), 0, s, x0, x1, M, H, (M + n - 1) / n, part,
-                     reinterpret_cast<__bf16*>(out0), reinterpret_cast<__bf16*>(out1));
+hipError_t launch_column_sums(const uint16_t* x0, const uint16_t* x1, int64_t M, int H, float* part, hipStream_t s) {
+  const int n = column_sum_partials(M);
+  if (H <= 0 || H % 8 != 0 || n <= 0) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(k_column_sum, dim3((H + 63) / 64, n, 2), dim3(256), 0, s, x0, x1, M, H, (M + n - 1) / n, part);
   return hipGetLastError();
 }
 

@@ -364,18 +364,18 @@ struct LnJoin {
     const float* part;
     int nb;
     void *out0, *out1;
+    const uint16_t *x0, *x1;  // bf16 rows to sum in place of partials (nb of them, H wide; bf16 only)
   } seg[3];
   int n, H;
 };
 hipError_t launch_column_join(int dtype, const LnJoin& a, hipStream_t s);
-// out0, out1 = the column sums of two bf16 matrices of M rows; where
-// column_sum_partials(M) is not 0 that many partial rows of 2 H floats in part
-// instead, for launch_column_join
+// The column sums of two bf16 matrices of M rows as column_sum_partials(M)
+// partial rows of 2 H floats, for launch_column_join; up to kColSumRows rows
+// there are none: the join sums them itself
 constexpr int kColSumPartials = 128;
 constexpr int64_t kColSumRows = 512;
 int column_sum_partials(int64_t M);
-hipError_t launch_column_sums(const uint16_t* x0, const uint16_t* x1, int64_t M, int H, float* part, uint16_t* out0,
-                              uint16_t* out1, hipStream_t s);
+hipError_t launch_column_sums(const uint16_t* x0, const uint16_t* x1, int64_t M, int H, float* part, hipStream_t s);
 // Dense bf16 GEMMs of the training forms (gemm_dense.hpp).
 enum DenseLayout { kDgNT = 0, kDgNN = 1, kDgTN = 2 };
 enum DenseEpilogue {
