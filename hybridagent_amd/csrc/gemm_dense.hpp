@@ -166,8 +166,7 @@ __device__ __forceinline__ u32x4_t dg_pack8(const float v[8]) {
 // are not written.  Element offsets o of a row-major [rows][N] (at most 256
 // rows of 32768: byte offsets below 2^25).
 struct DgTarget {
-  __amdgpu_buffer_rsrc_t out, out2, sum, sum2, in, part, part2;
-  const uint16_t* bias;
+  __amdgpu_buffer_rsrc_t out, out2, sum, sum2, in, bias, part, part2;
   bool keep;  // kDgGateUp: sum, sum2 wanted
 };
 constexpr int kDgOut = 1 << 28;
@@ -187,7 +186,7 @@ __device__ __forceinline__ DgTarget dg_target(const DgArgs& a, const DgProblem& 
   const float* part = a.part + split * a.plane + p.part0 + at;
   g.part = make_rsrc(part, a.ksplit > 1 ? 2u * bytes : 0u);
   g.part2 = make_rsrc(part + (int64_t)p.M * p.N, a.ksplit > 1 && two ? 2u * bytes : 0u);
-  g.bias = p.e.bias;
+  g.bias = make_rsrc(p.e.bias, p.e.bias != nullptr ? (uint32_t)p.N * 2u : 0u);
   g.keep = p.e.sum != nullptr;
   return g;
 }
@@ -229,9 +228,9 @@ __device__ __forceinline__ void gelu_erf_and_slope(float x, float* act, float* s
   *slope = cdf + x * (0.3989422804014327f * e);
 }
 
-// what the epilogue reads at element o: in, or sum and sum2
+// what the epilogue reads at element o, column n: in, or sum and sum2; the bias
 struct DgIn {
-  u32x4_t v[4];
+  u32x4_t v[4], bias;
 };
 template <int EPI>
 __device__ __forceinline__ DgIn dg_fetch(const DgTarget& g, int o) {
@@ -247,15 +246,15 @@ __device__ __forceinline__ DgIn dg_fetch(const DgTarget& g, int o) {
   }
   return r;
 }
-
-// the bias of columns n .. n + 7 (element o: past the problem none)
-__device__ __forceinline__ u32x4_t dg_bias(const DgTarget& g, int o, int n) {
-  return o == kDgOut ? u32x4_t{0u, 0u, 0u, 0u} : ld16(g.bias + n);
+// the bias of columns n .. n + 7 (zeros past the problem)
+template <int EPI>
+__device__ __forceinline__ u32x4_t dg_bias(const DgTarget& g, int n) {
+  return EPI == kDgBiasGelu || EPI == kDgBiasResidual ? buf_ld16(g.bias, 2 * n, 0) : u32x4_t{0u, 0u, 0u, 0u};
 }
 
-// v: the sums (v2: kDgGateUp's up sums) of the target's elements o .. o + 7, column n on
+// v: the sums (v2: kDgGateUp's up sums) of the target's elements o .. o + 7
 template <int EPI>
-__device__ __forceinline__ void dg_finish(const DgTarget& g, int o, int n, const float v[8], const float v2[8],
+__device__ __forceinline__ void dg_finish(const DgTarget& g, int o, const float v[8], const float v2[8],
                                           const DgIn& in) {
   float r[8], s[8];
   if constexpr (EPI == kDgPlain) {
@@ -285,7 +284,7 @@ __device__ __forceinline__ void dg_finish(const DgTarget& g, int o, int n, const
     dg_st8(g.out, o, r);
     dg_st8(g.out2, o, s);
   } else if constexpr (EPI == kDgBiasGelu) {
-    dg_unpack8(dg_bias(g, o, n), s);
+    dg_unpack8(in.bias, s);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       float slope;
@@ -296,7 +295,7 @@ __device__ __forceinline__ void dg_finish(const DgTarget& g, int o, int n, const
     dg_st8(g.out2, o, s);
   } else if constexpr (EPI == kDgBiasResidual) {
     float b[8];
-    dg_unpack8(dg_bias(g, o, n), b);
+    dg_unpack8(in.bias, b);
     dg_unpack8(in.v[0], s);
 #pragma unroll
     for (int i = 0; i < 8; ++i) r[i] = s[i] + (v[i] + b[i]);
@@ -574,17 +573,28 @@ __global__ __launch_bounds__(KG * kDgThreads, MI * NI > 36 ? 1 : KG > 2 ? KG : 2
   float* const rows = reinterpret_cast<float*>(smem + kSums) + wave * kPlanes * 16 * kPitch;
   const int r0 = m0 + 16 * MI * (wave >> 1), c0 = n0 + 16 * NO * (wave & 1);
   const DgTarget g = dg_target(a, p, split, r0, 16 * MI, GU);
-#pragma unroll
-  for (int m = 0; m < MI; ++m) {
-    DgIn in[kIter];
-    int o[kIter];
+  // What it reads is asked for kAhead steps of 16 rows before it is needed: a
+  // step by itself would wait for memory.
+  constexpr int kAhead = EPI != kDgGateUpBack ? 3 : MI * NI > 24 && !kAccRegs ? 0 : 1;
+  DgIn in[MI][kIter];
+  int o[MI][kIter];
+  u32x4_t bias[kIter];
+  auto fetch = [&](int m) {
 #pragma unroll
     for (int i = 0; i < kIter; ++i) {
       const int idx = lane + 64 * i, col = c0 + 8 * (idx % (2 * NO));
       // element of the target; past it for lanes past the tile and columns past the problem
-      o[i] = idx < 32 * NO && col < p.N ? (16 * m + idx / (2 * NO)) * p.N + col : kDgOut;
-      in[i] = dg_fetch<EPI>(g, o[i]);
+      o[m][i] = idx < 32 * NO && col < p.N ? (16 * m + idx / (2 * NO)) * p.N + col : kDgOut;
+      in[m][i] = dg_fetch<EPI>(g, o[m][i]);
     }
+  };
+#pragma unroll
+  for (int i = 0; i < kIter; ++i) bias[i] = dg_bias<EPI>(g, c0 + 8 * ((lane + 64 * i) % (2 * NO)));
+#pragma unroll
+  for (int m = 0; m < kAhead && m < MI; ++m) fetch(m);
+#pragma unroll
+  for (int m = 0; m < MI; ++m) {
+        if (m + kAhead < MI) fetch(m + kAhead);
 #pragma unroll
     for (int n = 0; n < NO; ++n) {
       float* q = rows + (lane & 15) * kPitch + 16 * n + 4 * (lane >> 4);
@@ -602,10 +612,11 @@ __global__ __launch_bounds__(KG * kDgThreads, MI * NI > 36 ? 1 : KG > 2 ? KG : 2
         v2[k] = GU ? q[16 * kPitch + k] : 0.f;
       }
       if (a.ksplit > 1) {
-        dg_st8_f32(g.part, o[i], v);
-        if (GU) dg_st8_f32(g.part2, o[i], v2);
+        dg_st8_f32(g.part, o[m][i], v);
+        if (GU) dg_st8_f32(g.part2, o[m][i], v2);
       } else {
-        dg_finish<EPI>(g, o[i], c0 + 8 * (idx % (2 * NO)), v, v2, in[i]);
+        in[m][i].bias = bias[i];
+        dg_finish<EPI>(g, o[m][i], v, v2, in[m][i]);
       }
     }
   }
@@ -623,7 +634,8 @@ __global__ __launch_bounds__(256) void k_gemm_dense_join(DgArgs a) {
   const int row0 = (int)((int64_t)blockIdx.x * 2048 / p.N);
   const DgTarget g = dg_target(a, p, 0, row0, 256, false);
   const int o = (row - row0) * p.N + n;
-  const DgIn in = dg_fetch<EPI>(g, o);
+  DgIn in = dg_fetch<EPI>(g, o);
+  in.bias = dg_bias<EPI>(g, n);
   const float* q = a.part + p.part0 + 8 * i;
   float v[8], v2[8];
 #pragma unroll
@@ -636,7 +648,7 @@ __global__ __launch_bounds__(256) void k_gemm_dense_join(DgArgs a) {
       if (EPI == kDgGateUp) v2[k] += q[s * a.plane + (int64_t)p.M * p.N + k];
     }
   }
-  dg_finish<EPI>(g, o, n, v, v2, in);
+  dg_finish<EPI>(g, o, v, v2, in);
 }
 
 template <int LAYOUT, int EPI, int MI, int NI, int KG>

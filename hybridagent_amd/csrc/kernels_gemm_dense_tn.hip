@@ -28,7 +28,7 @@ hipError_t launch_gemm_dense(int layout, int epi, DgArgs a, hipStream_t s) {
     sh[i] = DenseShape{p.M, gu ? 2 * (int64_t)p.N : p.N};
   }
   const bool thin = a.mi == 0 && layout != kDgTN && a.nprob == 1 &&
-                    a.prob[0].M <= dense_thin_rows(layout == kDgNN);
+                    dense_thin(a.prob[0].M, a.prob[0].N, gu ? 16 : 32, device_cus());
   if (thin) a.ksplit = 1;
   if (a.mi == 0 && !thin) {
     const DensePlan pl = dense_plan(sh, a.nprob, a.nk, a.part != nullptr ? dense_part_planes(a.plane) : 1, device_cus(),

@@ -119,12 +119,17 @@ inline int linear_w4_blocks(int64_t M, int64_t N, int cus, int max_blocks) {
   X(2, 2, 1, 4, 155, 125)    \
   X(2, 2, 4, 1, 155, 125)
 
-// Products of few rows run as the weights' stream (gemm_thin.hpp): x W^T up to
-// 64 rows (2816 x 2816, split over workgroups / streamed: 1 row 9.0/5.1 us, 32
-// 10.0/6.1, 64 9.5/8.2), dy W up to 32 (32 rows 9.8/8.3 us, 64 10.9/10.6; two
-// pairs of 2112: 7 rows 10.6/10.6, 64 12.8/17.6, where a workgroup's 64-byte
-// pieces of rows cost more than the second launch).
-constexpr int dense_thin_rows(bool nn) { return nn ? 32 : 64; }
+// Products of few rows run as the weights' stream (gemm_thin.hpp), 32 rows x
+// `cols` columns a workgroup: up to 64 rows, and up to 512 while the workgroups
+// are one round of the CUs (tiles of any shape, split as is best for them / streamed,
+// 2816 -> 2816: x W^T 96 rows 12.2/11.7 us; dy W 32 rows 11.5/9.9, 64 12.1/9.3,
+// 128 14.2/15.2; 2816 -> 2112, 96 rows 10.9/7.2, 12.3/8.5, 128 11.6/11.6,
+// 12.8/13.0; two pairs of 2112, 64 rows 14.3/12.2; 2816 -> 512, 512 rows
+// 10.8/7.1, 11.9/8.2; but 512 -> 128, 2048 rows 5.0/6.8, 5.7/7.2: every 32 rows
+// read the weights).
+inline bool dense_thin(int64_t rows, int64_t n, int cols, int cus) {
+  return rows <= 64 || (rows <= 512 && (rows + 31) / 32 * ((n + cols - 1) / cols) <= cus);
+}
 struct DenseShape {
   int64_t rows, cols;  // of the product (gate/up: both halves' columns)
 };
