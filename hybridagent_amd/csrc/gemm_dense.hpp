@@ -12,17 +12,25 @@
 // A workgroup of four wavefronts (2 x 2) owns a tile of 32 MI rows x 32 NI
 // columns, a wavefront 16 MI x 16 NI of it; with KG > 1 there are KG such
 // groups, each with a part of K and a ring of its own, whose sums are added in
-// LDS (a few hundred rows: a wavefront's chain of stages is what takes the time).  k advances in stages of 32
-// through a ring of dg_stages LDS slots filled by direct 16-byte global -> LDS
-// loads; the fragments of stage t + 1 are read while stage t is multiplied,
-// so that a stage has one barrier and its loads have two to three stages to
-// land.  Stages past the end are issued with an empty buffer descriptor, which
-// reads nothing, so that every wait counts the same loads.
+// LDS (a few hundred rows: a wavefront's chain of stages is what takes the
+// time).  k advances in stages of 32 through a ring of dg_slots LDS slots filled
+// by direct 16-byte global -> LDS loads; the fragments of stage t + 1 are read
+// while stage t is multiplied, so that a slot has one barrier and its loads
+// have two to three stages to land.  Slots past the end are issued with an empty
+// buffer descriptor, which reads nothing, so that every wait counts the same
+// loads.
 //
-// LDS formats of a stage's operand tile, both free of bank conflicts:
-//   rows  (k contiguous)  [rows][32 k], 64 bytes a row, the 16-byte chunks
-//         XOR-swizzled by dg_row_swz(row): a fragment is 16 rows x 64 bytes, one
-//         ds_read_b128 per lane;
+// A slot is a stage; in x W^T two, so that each row comes in whole 128-byte
+// lines: half a line per stage has left the L1 before the other half is asked
+// for, and the line comes from the L2 twice (2816 -> 2816, one / two stages a
+// slot: 1024 rows 28.4/23.9 us, 2049 38.9/34.5; 8192 rows 2816 -> 4224
+// 180.6/162.0).  dy W, one of whose operands has rows, loses by it (2049 rows
+// 38.5/42.0: longer stages take more LDS or land later).
+//
+// LDS formats of a slot's operand tile, both free of bank conflicts:
+//   rows  (k contiguous)  [rows][32 or 64 k], the 16-byte chunks of a row
+//         XOR-swizzled by bits of the row (dg_row_swz; 64 k: row / 2): a fragment
+//         is 16 rows x 64 bytes, one ds_read_b128 per lane;
 //   cols  ([k][.])        [32 k][cols], the 32-byte units of a row
 //         XOR-swizzled by bits of k (dg_swz): a fragment of 16 columns x 32 k
 //         is two transposing reads (ds_read_b64_tr_b16), which take 4 k x 16
@@ -43,8 +51,17 @@ namespace w4a16 {
 constexpr int kDgThreads = 256;
 constexpr int kDgKT = 32;     // k per stage
 
-// LDS slots of a tile: four, or three where two workgroups then share a CU
-constexpr int dg_stages(int mi, int ni) { return mi * ni >= 24 && mi * ni <= 36 ? 3 : 4; }
+// Whether a slot of the ring is two stages
+constexpr bool dg_pairs(int layout) { return layout == kDgNT; }
+constexpr int dg_slot_bytes(int layout, int mi, int ni) {
+  return 32 * (mi + ni) * kDgKT * 2 * (dg_pairs(layout) ? 2 : 1);
+}
+// LDS slots of a tile: four, or three where two workgroups then share a CU;
+// pairs: three where they fit in tiles of few MFMAs a stage, else two
+constexpr int dg_slots(int layout, int mi, int ni, int kg) {
+  if (dg_pairs(layout)) return mi * ni <= 24 && 3 * kg * dg_slot_bytes(layout, mi, ni) <= 160 * 1024 ? 3 : 2;
+  return mi * ni >= 24 && mi * ni <= 36 ? 3 : 4;
+}
 constexpr int kDgGroupM = 4;  // row tiles that run with a column tile
 constexpr int dg_bm(int mi) { return 32 * mi; }
 constexpr int dg_bn(int epi, int ni) { return epi == kDgGateUp ? 16 * ni : 32 * ni; }
@@ -90,13 +107,14 @@ __device__ __forceinline__ int dg_row_swz(int quad) { return (((quad ^ (quad >> 
 // One operand's side of a tile: W rows (or columns), F fragments of 16 per
 // wavefront.  COLS: the cols format.  GU (rows format): the first half of a
 // wavefront's fragments come from p, the second half, same rows, from p2.
-template <bool COLS, bool GU, int F>
+// PAIR: rows format of two stages.
+template <bool COLS, bool GU, int F, bool PAIR>
 struct DgOperand {
   static constexpr int W = 32 * F;
-  static constexpr int kBytes = W * kDgKT * 2;
-  static constexpr int kLoads = F / 2;  // per wavefront and stage
+  static constexpr int kBytes = W * kDgKT * (PAIR ? 4 : 2);  // of a stage, or pair of stages
+  static constexpr int kLoads = PAIR ? F : F / 2;            // per wavefront, of the same
   int voff[kLoads];                     // a lane's source bytes, per load
-  int foff[COLS ? F : 1];               // its fragment bytes in a stage
+  int foff[COLS ? F : PAIR ? 2 : 1];    // its fragment bytes in a stage
 
   // first: the tile's first row, n: rows there are (rows past it repeat the last)
   __device__ __forceinline__ void init(int first, int n, int64_t ld, int wave) {
@@ -111,8 +129,8 @@ struct DgOperand {
         const int col = min(16 * unit + 8 * (s & 1), n - first - 8);
         voff[j] = k * (int)ld * 2 + 2 * col;
       } else {
-        int r = 16 * ins + (lane >> 2);
-        const int chunk = (lane & 3) ^ dg_row_swz((lane >> 4) & 3);
+        int r = PAIR ? 8 * ins + (lane >> 3) : 16 * ins + (lane >> 2);
+        const int chunk = PAIR ? (lane & 7) ^ ((r >> 1) & 7) : (lane & 3) ^ dg_row_swz((lane >> 4) & 3);
         if constexpr (GU) {
           // tile rows 16 F w + [0, 8 F): rows 8 F w + .. of p, [8 F, 16 F): of p2
           const int w = r / (16 * F), in = r - 16 * F * w;
@@ -129,18 +147,26 @@ struct DgOperand {
       const int k = 8 * (lane >> 4) + ((lane & 15) >> 2);
 #pragma unroll
       for (int f = 0; f < F; ++f) foff[f] = k * 2 * W + 32 * ((w * F + f) ^ dg_swz<W>(k)) + 8 * (lane & 3);
+    } else if constexpr (PAIR) {
+      foff[0] = 2048 * F * w + (lane & 15) * 128 + 16 * ((lane >> 4) ^ ((lane >> 1) & 7));
+      foff[1] = foff[0] ^ 64;
     } else {
       foff[0] = 1024 * F * w + (lane & 15) * 64 + 16 * ((lane >> 4) ^ dg_row_swz((lane >> 2) & 3));
     }
   }
-  static __device__ __forceinline__ bool second(int j, int wave) { return (wave + 4 * j) % F >= F / 2; }
-  __device__ __forceinline__ u32x4_t frag(const unsigned char* st, int f) const {
+  static __device__ __forceinline__ bool second(int j, int wave) {
+    return (wave + 4 * j) / (PAIR ? 2 : 1) % F >= F / 2;
+  }
+  // h: the stage of a pair
+  __device__ __forceinline__ u32x4_t frag(const unsigned char* st, int f, int h) const {
     if constexpr (COLS) {
       const unsigned char* p = st + foff[f];
       const bf16x4_t lo = dg_tr_read((lds_bf16x4_t*)p);
       const bf16x4_t hi = dg_tr_read((lds_bf16x4_t*)(p + 8 * W));
       const bf16x8_t v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
       return __builtin_bit_cast(u32x4_t, v);
+    } else if constexpr (PAIR) {
+      return *reinterpret_cast<const u32x4_t*>(st + foff[h] + 2048 * f);
     } else {
       return *reinterpret_cast<const u32x4_t*>(st + foff[0] + 1024 * f);
     }
@@ -323,17 +349,19 @@ template <int LAYOUT, int EPI, int MI, int NI, int KG>
 __global__ __launch_bounds__(KG * kDgThreads, MI * NI > 36 ? 1 : KG > 2 ? KG : 2) void k_gemm_dense(DgArgs a) {
   constexpr bool AC = LAYOUT == kDgTN, BC = LAYOUT != kDgNT;
   constexpr bool GU = EPI == kDgGateUp;
-  using OA = DgOperand<AC, false, MI>;
-  using OB = DgOperand<BC, GU, NI>;
-  constexpr int kStage = OA::kBytes + OB::kBytes;
-  constexpr int kStages = dg_stages(MI, NI);
+  constexpr bool kPairs = dg_pairs(LAYOUT);
+  using OA = DgOperand<AC, false, MI, kPairs>;
+  using OB = DgOperand<BC, GU, NI, kPairs>;
+  constexpr int kSlot = dg_slot_bytes(LAYOUT, MI, NI);
+  static_assert(kSlot == OA::kBytes + OB::kBytes, "a slot's operands");
+  constexpr int kSlots = dg_slots(LAYOUT, MI, NI, KG);
   constexpr int kLoads = OA::kLoads + OB::kLoads;
   constexpr int BM = dg_bm(MI), BN = dg_bn(EPI, NI);
   extern __shared__ __align__(16) unsigned char smem[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
   const int group = KG > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 8) : 0;
-  unsigned char* const ring = smem + group * kStages * kStage;
+  unsigned char* const ring = smem + group * kSlots * kSlot;
 
   // the tile: kDgGroupM row tiles run with each column tile
   int item = dg_item(a.tiles * a.ksplit);
@@ -352,8 +380,9 @@ __global__ __launch_bounds__(KG * kDgThreads, MI * NI > 36 ? 1 : KG > 2 ? KG : 2
   const int m0 = (grp * kDgGroupM + rem - nt * gm) * BM, n0 = nt * BN;
   // the group's stages; every group runs as many (those past its range multiply
   // the zeros that empty descriptors give)
-  const int per = (a.nk + a.ksplit * KG - 1) / (a.ksplit * KG);
-  // what is loaded next, kStages ahead of the multiplication: stage t of the
+  constexpr int kStep = kPairs ? 2 : 1;
+  const int per = (a.nk + kStep * a.ksplit * KG - 1) / (kStep * a.ksplit * KG) * kStep;
+  // what is loaded next, kSlots ahead of the multiplication: stage t of the
   // operands (their values here: the loop reads no arguments)
   struct Feed {
     const uint16_t *A, *A2, *B, *B2;
@@ -375,7 +404,9 @@ __global__ __launch_bounds__(KG * kDgThreads, MI * NI > 36 ? 1 : KG > 2 ? KG : 2
   struct Src {
     __amdgpu_buffer_rsrc_t a, b, b2;
     int off;
+    int skip;  // pairs: a lane's chunk is past K (a last pair of one stage)
   };
+  const bool second = kPairs && (((lane >> 2) ^ wave) & 1) != 0;  // its chunk is of a pair's second stage
   auto source = [&] {
     const bool two = LAYOUT == kDgNN && f.t >= a.nk1;
     const int tt = two ? f.t - a.nk1 : f.t;
@@ -391,18 +422,20 @@ __global__ __launch_bounds__(KG * kDgThreads, MI * NI > 36 ? 1 : KG > 2 ? KG : 2
              : make_rsrc(pb + (int64_t)n0 * f.ldb, any ? bbytes : 0u);
     r.b2 = GU ? make_rsrc(f.B2 + (int64_t)n0 * f.ldb, any ? bbytes : 0u) : r.b;
     r.off = tt * (kDgKT * 2);
+    r.skip = kPairs && second && f.t + 1 >= a.nk ? kDgOut : 0;
+    f.t += kStep;
     return r;
   };
   // load j of the wavefront's kLoads into a slot
   auto issue = [&](const Src& r, unsigned char* slot, int j) {
     if (j < OA::kLoads) {
-      px_dma16(r.a, oa.voff[j], AC ? 0 : r.off, slot + (wave + 4 * j) * 1024);
+      px_dma16(r.a, oa.voff[j] + r.skip, AC ? 0 : r.off, slot + (wave + 4 * j) * 1024);
     } else {
       const int i = j - OA::kLoads;
       if (GU && OB::second(i, wave))
-        px_dma16(r.b2, ob.voff[i], r.off, slot + OA::kBytes + (wave + 4 * i) * 1024);
+        px_dma16(r.b2, ob.voff[i] + r.skip, r.off, slot + OA::kBytes + (wave + 4 * i) * 1024);
       else
-        px_dma16(r.b, ob.voff[i], BC ? 0 : r.off, slot + OA::kBytes + (wave + 4 * i) * 1024);
+        px_dma16(r.b, ob.voff[i] + r.skip, BC ? 0 : r.off, slot + OA::kBytes + (wave + 4 * i) * 1024);
     }
   };
 
@@ -428,55 +461,61 @@ __global__ __launch_bounds__(KG * kDgThreads, MI * NI > 36 ? 1 : KG > 2 ? KG : 2
   u32x4_t fa[MI], fb[kB][NI];
 
 #pragma unroll
-  for (int s = 0; s < kStages; ++s) {
+  for (int s = 0; s < kSlots; ++s) {
     const Src r = source();
 #pragma unroll
-    for (int j = 0; j < kLoads; ++j) issue(r, ring + s * kStage, j);
-    ++f.t;
+    for (int j = 0; j < kLoads; ++j) issue(r, ring + s * kSlot, j);
   }
-  dg_wait_vm<(kStages - 1) * kLoads>();
+  dg_wait_vm<(kSlots - 1) * kLoads>();
   px_barrier();
 #pragma unroll
-  for (int n = 0; n < NI; ++n) fb[0][n] = ob.frag(ring + OA::kBytes, n);
+  for (int n = 0; n < NI; ++n) fb[0][n] = ob.frag(ring + OA::kBytes, n, 0);
 #pragma unroll
-  for (int m = 0; m < MI; ++m) fa[m] = oa.frag(ring, m);
+  for (int m = 0; m < MI; ++m) fa[m] = oa.frag(ring, m, 0);
 
-  // Stage t, its fragments at hand: after the first row of fragments' MFMAs
-  // the wavefronts meet (stage t + 1 has landed, slot t is read), then slot t
-  // is refilled with stage t + kStages and every fragment register takes its
-  // fragment of stage t + 1 after its last MFMA.  Reads and loads go one by one
-  // between the MFMAs: one after every second keeps the matrix unit fed.
+  // Stage t, its fragments at hand.  Every fragment register takes its fragment
+  // of stage t + 1 after its last MFMA.  In a slot's last stage the wavefronts
+  // meet after the first row of fragments' MFMAs (the next slot has landed, this
+  // one is read), then the slot is refilled, kSlots ahead.  Reads and loads go
+  // one by one between the MFMAs: one after every second keeps the matrix unit
+  // fed.
   int slot = 0;
   auto stage = [&](auto cur_) {
     constexpr int cur = kB == 2 ? decltype(cur_)::value : 0, nxt = kB == 2 ? cur ^ 1 : 0;
-    const int ns = slot == kStages - 1 ? 0 : slot + 1;
-    unsigned char* refill = ring + slot * kStage;
-    const unsigned char* st = ring + ns * kStage;
-    const Src src = source();
+    constexpr int at = kPairs ? decltype(cur_)::value : 0;  // the stage of its slot
+    constexpr bool kMeet = at == kStep - 1;
+    constexpr int kIssue = kMeet ? kLoads : 0, kNext = kMeet ? 0 : at + 1;
+    const int ns = kMeet ? (slot == kSlots - 1 ? 0 : slot + 1) : slot;
+    unsigned char* refill = ring + slot * kSlot;
+    const unsigned char* st = ring + ns * kSlot;
+    Src src;
+    if constexpr (kMeet) src = source();
 #pragma unroll
     for (int n = 0; n < NI; ++n) acc[0][n] = mfma16(fb[cur][n], fa[0], acc[0][n]);
     __builtin_amdgcn_sched_barrier(0);
-    dg_wait_vm<(kStages - 2) * kLoads>();
-    px_barrier();
-    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (kMeet) {
+      dg_wait_vm<(kSlots - 2) * kLoads>();
+      px_barrier();
+      __builtin_amdgcn_sched_barrier(0);
+    }
     if constexpr (kB == 2) {
       // operation o of the row m: its MFMAs are done one ahead
       constexpr int R = MI - 1;
 #pragma unroll
       for (int m = 1; m < MI; ++m) {
         // this row's: fa[m - 1], then column fragments and loads by turns
-        const int b0 = (m - 1) * NI / R, b1 = m * NI / R, l0 = (m - 1) * kLoads / R, l1 = m * kLoads / R;
+        const int b0 = (m - 1) * NI / R, b1 = m * NI / R, l0 = (m - 1) * kIssue / R, l1 = m * kIssue / R;
         int done = 0;
 #pragma unroll
         for (int n = 0; n < NI; ++n) {
           acc[m][n] = mfma16(fb[cur][n], fa[m], acc[m][n]);
           if (n % 2 == 0 || NI < 6) {
             if (done == 0) {
-              fa[m - 1] = oa.frag(st, m - 1);
+              fa[m - 1] = oa.frag(st, m - 1, kNext);
             } else {
               const int k = done - 1;
               if (k < b1 - b0)
-                fb[nxt][b0 + k] = ob.frag(st + OA::kBytes, b0 + k);
+                fb[nxt][b0 + k] = ob.frag(st + OA::kBytes, b0 + k, kNext);
               else if (k - (b1 - b0) < l1 - l0)
                 issue(src, refill, l0 + k - (b1 - b0));
             }
@@ -488,28 +527,28 @@ __global__ __launch_bounds__(KG * kDgThreads, MI * NI > 36 ? 1 : KG > 2 ? KG : 2
 #pragma unroll
         for (int k = done - 1; k < (b1 - b0) + (l1 - l0); ++k) {
           if (k < b1 - b0)
-            fb[nxt][b0 + k] = ob.frag(st + OA::kBytes, b0 + k);
+            fb[nxt][b0 + k] = ob.frag(st + OA::kBytes, b0 + k, kNext);
           else
             issue(src, refill, l0 + k - (b1 - b0));
         }
         __builtin_amdgcn_sched_barrier(0);
       }
-      fa[MI - 1] = oa.frag(st, MI - 1);
+      fa[MI - 1] = oa.frag(st, MI - 1, kNext);
     } else {
-      if (MI > 2) fa[0] = oa.frag(st, 0);
+      if (MI > 2) fa[0] = oa.frag(st, 0, kNext);
 #pragma unroll
       for (int m = 1; m < MI - 2; ++m) {
 #pragma unroll
         for (int n = 0; n < NI; ++n) acc[m][n] = mfma16(fb[0][n], fa[m], acc[m][n]);
-        fa[m] = oa.frag(st, m);
+        fa[m] = oa.frag(st, m, kNext);
 #pragma unroll
-        for (int j = (m - 1) * kLoads / (MI > 3 ? MI - 3 : 1); j < m * kLoads / (MI > 3 ? MI - 3 : 1); ++j)
+        for (int j = (m - 1) * kIssue / (MI > 3 ? MI - 3 : 1); j < m * kIssue / (MI > 3 ? MI - 3 : 1); ++j)
           issue(src, refill, j);
         __builtin_amdgcn_sched_barrier(0);
       }
       if constexpr (MI <= 3) {
 #pragma unroll
-        for (int j = 0; j < kLoads; ++j) issue(src, refill, j);
+        for (int j = 0; j < kIssue; ++j) issue(src, refill, j);
       }
       // the last two rows column by column, so that a column's fragment has
       // 2 (NI - 1) MFMAs to arrive
@@ -517,14 +556,13 @@ __global__ __launch_bounds__(KG * kDgThreads, MI * NI > 36 ? 1 : KG > 2 ? KG : 2
       for (int n = 0; n < NI; ++n) {
         if (MI > 2) acc[MI - 2][n] = mfma16(fb[0][n], fa[MI - 2], acc[MI - 2][n]);
         acc[MI - 1][n] = mfma16(fb[0][n], fa[MI - 1], acc[MI - 1][n]);
-        fb[0][n] = ob.frag(st + OA::kBytes, n);
+        fb[0][n] = ob.frag(st + OA::kBytes, n, kNext);
         __builtin_amdgcn_sched_barrier(0);
       }
-      fa[MI - 2] = oa.frag(st, MI - 2);
-      fa[MI - 1] = oa.frag(st, MI - 1);
+      fa[MI - 2] = oa.frag(st, MI - 2, kNext);
+      fa[MI - 1] = oa.frag(st, MI - 1, kNext);
     }
     slot = ns;
-    ++f.t;
   };
 
 #pragma unroll
@@ -532,10 +570,10 @@ __global__ __launch_bounds__(KG * kDgThreads, MI * NI > 36 ? 1 : KG > 2 ? KG : 2
 #pragma unroll
     for (int n = 0; n < NI; ++n) acc[m][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   pin();
-  if constexpr (kB == 2) {
+  if constexpr (kB == 2 || kPairs) {
     for (int t = 0; t < per; t += 2) {
       stage(std::integral_constant<int, 0>{});
-      if (t + 1 < per) stage(std::integral_constant<int, 1>{});
+      if (kPairs || t + 1 < per) stage(std::integral_constant<int, 1>{});
     }
   } else {
     for (int t = 0; t < per; ++t) stage(std::integral_constant<int, 0>{});
@@ -569,7 +607,7 @@ __global__ __launch_bounds__(KG * kDgThreads, MI * NI > 36 ? 1 : KG > 2 ? KG : 2
   // wavefront's columns (8 bytes in 32-byte pieces took half as long again).
   constexpr int kPitch = dg_epi_pitch(NO);
   constexpr int kSums = (KG - 1) * 4 * MI * NI * 1024;
-  static_assert(kSums + 4 * kPlanes * 16 * kPitch * 4 <= KG * kStages * kStage, "the epilogue's rows fit in the ring");
+  static_assert(kSums + 4 * kPlanes * 16 * kPitch * 4 <= KG * kSlots * kSlot, "the epilogue's rows fit in the ring");
   float* const rows = reinterpret_cast<float*>(smem + kSums) + wave * kPlanes * 16 * kPitch;
   const int r0 = m0 + 16 * MI * (wave >> 1), c0 = n0 + 16 * NO * (wave & 1);
   const DgTarget g = dg_target(a, p, split, r0, 16 * MI, GU);
@@ -653,7 +691,7 @@ __global__ __launch_bounds__(256) void k_gemm_dense_join(DgArgs a) {
 
 template <int LAYOUT, int EPI, int MI, int NI, int KG>
 hipError_t dg_launch(const DgArgs& a, hipStream_t s) {
-  constexpr int lds = KG * dg_stages(MI, NI) * 32 * (MI + NI) * kDgKT * 2;
+  constexpr int lds = KG * dg_slots(LAYOUT, MI, NI, KG) * dg_slot_bytes(LAYOUT, MI, NI);
   static_assert(lds <= 160 * 1024, "LDS of a CU");
   const int64_t groups = ((int64_t)a.tiles * a.ksplit + 7) / 8;  // of eight workgroups, one per XCD
   hipLaunchKernelGGL((k_gemm_dense<LAYOUT, EPI, MI, NI, KG>), dim3((unsigned)(8 * groups)), dim3(KG * kDgThreads), lds,

@@ -100,8 +100,8 @@ inline int linear_w4_blocks(int64_t M, int64_t N, int cus, int max_blocks) {
 // Dense GEMMs (gemm_dense.hpp): the tiles that are built, 32 mi rows x 32 ni
 // operand columns by kg groups of wavefronts, with the workgroups that share a
 // CU and what a stage of 32 k takes, in ns, for a group alone on a CU and for
-// each of several (256 .. 1024 tiles of K = 512 and 2816, the three layouts'
-// mean).
+// each of several (256 .. 1024 tiles of K = 512 and 2816).  First dy W and
+// dy^T x (their mean), then x W^T.
 #define W4A16_DG_TILES(X)    \
   X(8, 8, 1, 1, 670, 670)    \
   X(8, 6, 1, 1, 560, 560)    \
@@ -118,6 +118,22 @@ inline int linear_w4_blocks(int64_t M, int64_t N, int cus, int max_blocks) {
   X(2, 4, 2, 1, 215, 185)    \
   X(2, 2, 1, 4, 155, 125)    \
   X(2, 2, 4, 1, 155, 125)
+#define W4A16_DG_TILES_NT(X) \
+  X(8, 8, 1, 1, 670, 670)    \
+  X(8, 6, 1, 1, 520, 520)    \
+  X(6, 8, 1, 1, 525, 525)    \
+  X(6, 6, 1, 1, 460, 460)    \
+  X(8, 4, 1, 1, 420, 420)    \
+  X(4, 8, 1, 1, 425, 425)    \
+  X(6, 4, 1, 1, 320, 320)    \
+  X(4, 6, 1, 1, 345, 345)    \
+  X(4, 4, 1, 1, 235, 235)    \
+  X(4, 4, 2, 1, 235, 250)    \
+  X(4, 2, 1, 2, 145, 135)    \
+  X(2, 4, 1, 2, 160, 140)    \
+  X(2, 4, 2, 1, 160, 145)    \
+  X(2, 2, 1, 3, 97, 90)      \
+  X(2, 2, 4, 1, 97, 115)
 
 // Products of few rows run as the weights' stream (gemm_thin.hpp), 32 rows x
 // `cols` columns a workgroup: up to 64 rows, and up to 512 while the workgroups
@@ -146,11 +162,9 @@ inline int dense_part_planes(int64_t plane) {
 }
 // The tile and split whose time comes out least: rounds of the workgroups that
 // fit at once, each nk stages and an epilogue of some 210 ns per 16 x 16 tiles
-// of a wavefront; a split's launch that adds its planes takes 3 us and their
-// bytes at 4 TB/s.  Two groups to a tile gain less in x W^T (`rows`: both
-// operands come in 64-byte pieces of rows): 517 rows, 2 x 4 tiles in two groups
-// / 4 x 2 in one, 2112 -> 2816 17.7 / 15.0 us there, dy W 2816 -> 2112 18.7 /
-// 22.2.  Over 27 products of 32 .. 2049 rows the plan is 2 % off the fastest.
+// of a wavefront (x W^T, `rows`: 130); a split's launch that adds its planes
+// takes 3 us and their bytes at 4 TB/s.  Over 52 products of 100 .. 8192 rows
+// the plan is 0.5 % off the fastest measured, 7 % at most.
 inline DensePlan dense_plan(const DenseShape* sh, int nprob, int nk, int max_split, int cus, bool rows) {
   DensePlan best{0, 0, 1, 1};
   int64_t least = 0, plane = 0;
@@ -164,12 +178,11 @@ inline DensePlan dense_plan(const DenseShape* sh, int nprob, int nk, int max_spl
       const int64_t stages = (nk + ks * kg - 1) / (ks * kg);
       auto round = [&](int64_t w) {
         const int64_t step = w * kg * each > alone ? w * kg * each : alone;
-        return (stages + 2) * step + w * ((ks > 1 ? 300 : 210) + 50 * (kg - 1)) * mi * ni;
+        return (stages + 2) * step + w * ((ks > 1 ? 300 : rows ? 130 : 210) + 50 * (kg - 1)) * mi * ni;
       };
       int64_t c = n / occ * round(occ);
       if (n % occ != 0) c += round(n % occ);
       if (ks > 1) c += 3000 + (2 * ks + 1) * plane / 1000;
-      if (rows && kg == 2) c += 2500;
       if (best.mi == 0 || c < least) {
         best = DensePlan{mi, ni, kg, ks};
         least = c;
@@ -177,7 +190,11 @@ inline DensePlan dense_plan(const DenseShape* sh, int nprob, int nk, int max_spl
     }
   };
 #define W4A16_DG(MI_, NI_, KG_, OCC_, ALONE_, EACH_) consider(MI_, NI_, KG_, OCC_, ALONE_, EACH_);
-  W4A16_DG_TILES(W4A16_DG)
+  if (rows) {
+    W4A16_DG_TILES_NT(W4A16_DG)
+  } else {
+    W4A16_DG_TILES(W4A16_DG)
+  }
 #undef W4A16_DG
   return best;
 }

@@ -16,6 +16,10 @@ using namespace w4a16;
 int main() {
 #define W4A16_DG(MI_, NI_, KG_, OCC_, ALONE_, EACH_) printf("%d %d %d\\n", MI_, NI_, KG_);
   W4A16_DG_TILES(W4A16_DG)
+#undef W4A16_DG
+  printf("-\\n");
+#define W4A16_DG(MI_, NI_, KG_, OCC_, ALONE_, EACH_) printf("%d %d %d\\n", MI_, NI_, KG_);
+  W4A16_DG_TILES_NT(W4A16_DG)
   printf("-\\n");
   long long n, rows, cols, nk, plane, cus, nt;
   while (scanf("%lld %lld %lld %lld %lld %lld %lld", &n, &rows, &cols, &nk, &plane, &cus, &nt) == 7) {
@@ -41,8 +45,9 @@ def plans(tmp_path_factory):
     def run(calls):
         out = subprocess.run([str(d / "plan")], input="\n".join(" ".join(map(str, c)) for c in calls), text=True,
                              capture_output=True, check=True).stdout.split("\n-\n")
-        tiles = [tuple(map(int, ln.split())) for ln in out[0].split("\n")]
-        return tiles, [tuple(map(int, ln.split())) for ln in out[1].split("\n") if ln]
+        tiles, nt, got = ([tuple(map(int, ln.split())) for ln in part.split("\n") if ln] for part in out)
+        assert tiles == nt  # one set of tiles, with costs per layout
+        return tiles, got
 
     return run
 
@@ -67,7 +72,8 @@ MEASURED = [
     ((1, 2049, 2816, 88, 2049 * 2816, 1), {"6x4x1", "4x6x1"}),
     ((1, 517, 2816, 66, 517 * 2816, 1), {"4x2x1"}),
     ((1, 517, 2112, 88, 517 * 2112, 0), {"2x4x2"}),
-    ((1, 100, 2816, 66, 100 * 2816, 1), {"2x2x4"}),
+    ((1, 100, 2816, 66, 100 * 2816, 1), {"2x2x1"}),
+    ((1, 1024, 2816, 88, 1024 * 2816, 1), {"4x4x1"}),
     ((3, 2816, 2112, 256, 3 * 2816 * 2112, 0), {"6x6x1"}),
 ]
 
