@@ -369,6 +369,39 @@ def test_hybridlink_training(dev, T, H):
     assert rel(_lib.hybridlink(h, *params), want) <= 6 * u
 
 
+@pytest.mark.parametrize("T,H,I", [(3, 4160, 96), (20, 64, 4320), (50, 4160, 96), (50, 64, 4320), (130, 96, 64),
+                                   (512, 544, 96), (513, 64, 288)])
+def test_gated_mlp_few_rows_of_wide_or_narrow_outputs(dev, T, H, I):
+    """More columns than one round of the few-rows workgroups has, and more rows of few columns."""
+    test_gated_mlp(dev, T, H, I)
+
+
+@pytest.mark.parametrize("T,H", [(20, 4160), (50, 4160), (200, 96), (512, 32)])
+def test_hybridlink_few_rows_of_wide_or_narrow_outputs(dev, T, H):
+    test_hybridlink_training(dev, T, H)
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("T", [5, 40, 64, 300, 700])
+def test_a_row_that_is_not_finite_stays_alone(dev, T, bad):
+    """Widths that end inside a stage: what lies behind a row's end is the next row."""
+    H, I, r = 96, 160, 3
+    x, wg, wu, wd, dy = _mlp_inputs(dev, T, H, I, 400 + T)
+    others = torch.arange(T, device=dev) != r
+    x2, dy2 = x.clone(), dy.clone()
+    x2[r] = bad
+    dy2[r] = bad
+    y, saved = _lib.gated_mlp(x, wg, wu, wd, return_saved=True)
+    assert torch.equal(_lib.gated_mlp(x2, wg, wu, wd)[others], y[others])
+    dx = _lib.gated_mlp_backward(dy, x, wg, wu, wd, saved)[0]
+    assert torch.equal(_lib.gated_mlp_backward(dy2, x, wg, wu, wd, saved)[0][others], dx[others])
+    wd2 = wd.clone()
+    wd2[r] = bad
+    y2 = _lib.gated_mlp(x, wg, wu, wd2)
+    columns = torch.arange(H, device=dev) != r
+    assert torch.equal(y2[:, columns], y[:, columns]) and not torch.isfinite(y2[:, r]).any()
+
+
 # ---------------------------------------------------------------- as they are used
 
 
