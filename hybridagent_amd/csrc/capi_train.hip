@@ -108,6 +108,13 @@ MlpBackWs mlp_back_ws(void* p, int64_t M, int64_t H, int64_t I) {
   return w;
 }
 
+// HybridLink's tensors between the kernels are bf16, rounded once each from
+// fp32: a, g, dr and dz are operands of the bf16 matrix instructions, and z, r
+// and da, which only an activation or a norm reads, would in fp32 be 12 more
+// bytes per element and step and take away one of some four roundings on a
+// gradient's way.  Against 64 bits (Frobenius norm, 2049 rows of 2816) out is
+// 0.0027 off and the gradients 0.0016 .. 0.0040; torch's bf16 modules under
+// autograd 0.0031 and 0.0016 .. 0.0043, one rounding alone 0.0017.
 struct LinkSaved {
   uint16_t *a, *z, *g, *r;
   float *mean1, *rstd1, *mean2, *rstd2;
