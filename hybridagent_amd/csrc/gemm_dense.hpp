@@ -27,6 +27,12 @@
 // 180.6/162.0).  dy W, one of whose operands has rows, loses by it (2049 rows
 // 38.5/42.0: longer stages take more LDS or land later).
 //
+// Bound: many rows: the matrix units at the clock that the card holds under
+// them (2816 -> 4224 of 8192 rows 162 us, 1200 TFLOP/s; dy W 2816 -> 2112 85 us,
+// 1150; dy^T x 2112 x 2816 of 8192 rows 101 us, 960); hundreds: what the CUs
+// take from the L2 (2816 -> 2816 of 1024 rows 23.9 us, 680).  The tile and the
+// split are dense_plan's (rules.hpp).
+//
 // LDS formats of a slot's operand tile, both free of bank conflicts:
 //   rows  (k contiguous)  [rows][32 or 64 k], the 16-byte chunks of a row
 //         XOR-swizzled by bits of the row (dg_row_swz; 64 k: row / 2): a fragment
@@ -56,8 +62,11 @@ constexpr bool dg_pairs(int layout) { return layout == kDgNT; }
 constexpr int dg_slot_bytes(int layout, int mi, int ni) {
   return 32 * (mi + ni) * kDgKT * 2 * (dg_pairs(layout) ? 2 : 1);
 }
-// LDS slots of a tile: four, or three where two workgroups then share a CU;
-// pairs: three where they fit in tiles of few MFMAs a stage, else two
+// LDS slots of a tile: four, or three where two workgroups then share a CU.
+// Pairs of stages: three where they fit in tiles of few MFMAs a stage, else two
+// (2049 rows 2816 -> 2816, two / three: 6 x 4 tiles 40.5/36.1 us, 6 x 6 45.9/46.6;
+// 6144 rows -> 2048, 6 x 4 tiles 59.6/65.9, two workgroups of which no longer
+// share a CU, but 6 x 8 take 53).
 constexpr int dg_slots(int layout, int mi, int ni, int kg) {
   if (dg_pairs(layout)) return mi * ni <= 24 && 3 * kg * dg_slot_bytes(layout, mi, ni) <= 160 * 1024 ? 3 : 2;
   return mi * ni >= 24 && mi * ni <= 36 ? 3 : 4;

@@ -351,7 +351,7 @@ struct LnArgs {
 constexpr int kLnMaxH = 8192;
 constexpr int kLnPartials = 256;   // one workgroup per CU
 constexpr int kLnMaxGrid = 4096;
-constexpr int64_t kLnWaveRows = 512;
+constexpr int64_t kLnWaveRows = 512;  // more: a wavefront per row
 int ln_partials(int64_t M);
 hipError_t launch_ln_forward(int dtype, const LnArgs& a, hipStream_t s);
 // dx, and the column sums' partial rows (a.part: ln_partials(M) rows of 2 H
