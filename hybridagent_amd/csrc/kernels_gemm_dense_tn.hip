@@ -8,6 +8,8 @@ namespace w4a16 {
 hipError_t launch_gemm_dense_nt(int epi, const DgArgs& a, hipStream_t s);
 hipError_t launch_gemm_dense_nn(int epi, const DgArgs& a, hipStream_t s);
 
+static_assert(kPlanNT == (int)kDgNT && kPlanNN == (int)kDgNN && kPlanTN == (int)kDgTN, "dense_plan's layouts");
+
 hipError_t launch_gemm_dense(int layout, int epi, DgArgs a, hipStream_t s) {
   if (a.nprob < 1 || a.nprob > kDgMaxProblems || a.K < 0) return hipErrorInvalidValue;
   const bool gu = epi == kDgGateUp;
@@ -32,7 +34,7 @@ hipError_t launch_gemm_dense(int layout, int epi, DgArgs a, hipStream_t s) {
   if (thin) a.ksplit = 1;
   if (a.mi == 0 && !thin) {
     const DensePlan pl = dense_plan(sh, a.nprob, a.nk, a.part != nullptr ? dense_part_planes(a.plane) : 1, device_cus(),
-                                    layout == kDgNT);
+                                    layout);
     a.mi = pl.mi;
     a.ni = pl.ni;
     a.kg = pl.kg;

@@ -100,24 +100,40 @@ inline int linear_w4_blocks(int64_t M, int64_t N, int cus, int max_blocks) {
 // Dense GEMMs (gemm_dense.hpp): the tiles that are built, 32 mi rows x 32 ni
 // operand columns by kg groups of wavefronts, with the workgroups that share a
 // CU and what a stage of 32 k takes, in ns, for a group alone on a CU and for
-// each of several (256 .. 1024 tiles of K = 512 and 2816).  First dy W and
-// dy^T x (their mean), then x W^T.
-#define W4A16_DG_TILES(X)    \
-  X(8, 8, 1, 1, 670, 670)    \
-  X(8, 6, 1, 1, 560, 560)    \
-  X(6, 8, 1, 1, 560, 560)    \
-  X(6, 6, 1, 2, 485, 430)    \
-  X(8, 4, 1, 2, 460, 420)    \
-  X(4, 8, 1, 2, 490, 415)    \
-  X(6, 4, 1, 2, 370, 325)    \
-  X(4, 6, 1, 2, 380, 315)    \
-  X(4, 4, 1, 2, 300, 250)    \
-  X(4, 4, 2, 1, 300, 250)    \
-  X(4, 2, 1, 3, 215, 190)    \
-  X(2, 4, 1, 3, 215, 185)    \
-  X(2, 4, 2, 1, 215, 185)    \
-  X(2, 2, 1, 4, 155, 125)    \
-  X(2, 2, 4, 1, 155, 125)
+// each of several (256 .. 1024 tiles of K = 64, 512 and 2816): dy W, dy^T x and
+// x W^T.
+#define W4A16_DG_TILES(X) \
+  X(8, 8, 1, 1, 750, 775) \
+  X(8, 6, 1, 1, 590, 595) \
+  X(6, 8, 1, 1, 570, 575) \
+  X(6, 6, 1, 2, 460, 435) \
+  X(8, 4, 1, 2, 410, 413) \
+  X(4, 8, 1, 2, 450, 408) \
+  X(6, 4, 1, 2, 350, 325) \
+  X(4, 6, 1, 2, 370, 319) \
+  X(4, 4, 1, 2, 290, 243) \
+  X(4, 4, 2, 1, 290, 255) \
+  X(4, 2, 1, 3, 210, 190) \
+  X(2, 4, 1, 3, 205, 178) \
+  X(2, 4, 2, 1, 205, 167) \
+  X(2, 2, 1, 4, 160, 130) \
+  X(2, 2, 4, 1, 160, 118)
+#define W4A16_DG_TILES_TN(X) \
+  X(8, 8, 1, 1, 730, 750)    \
+  X(8, 6, 1, 1, 550, 570)    \
+  X(6, 8, 1, 1, 535, 575)    \
+  X(6, 6, 1, 2, 425, 412)    \
+  X(8, 4, 1, 2, 400, 373)    \
+  X(4, 8, 1, 2, 420, 393)    \
+  X(6, 4, 1, 2, 320, 294)    \
+  X(4, 6, 1, 2, 350, 300)    \
+  X(4, 4, 1, 2, 250, 215)    \
+  X(4, 4, 2, 1, 250, 210)    \
+  X(4, 2, 1, 3, 170, 150)    \
+  X(2, 4, 1, 3, 175, 155)    \
+  X(2, 4, 2, 1, 175, 138)    \
+  X(2, 2, 1, 4, 138, 100)    \
+  X(2, 2, 4, 1, 138, 93)
 #define W4A16_DG_TILES_NT(X) \
   X(8, 8, 1, 1, 670, 670)    \
   X(8, 6, 1, 1, 520, 520)    \
@@ -161,11 +177,12 @@ inline int dense_part_planes(int64_t plane) {
   return n >= kDgMaxSplit ? kDgMaxSplit : n >= 2 ? (int)n : 1;
 }
 // The tile and split whose time comes out least: rounds of the workgroups that
-// fit at once, each nk stages and an epilogue of some 210 ns per 16 x 16 tiles
-// of a wavefront (x W^T, `rows`: 130); a split's launch that adds its planes
-// takes 3 us and their bytes at 4 TB/s.  Over 52 products of 100 .. 8192 rows
-// the plan is 0.5 % off the fastest measured, 7 % at most.
-inline DensePlan dense_plan(const DenseShape* sh, int nprob, int nk, int max_split, int cus, bool rows) {
+// fit at once, each nk stages and an epilogue of some 110 ns per 16 x 16 tiles
+// of a wavefront (x W^T 130); a split's launch that adds its planes
+// takes 3 us and their bytes at 4 TB/s.  Over 90 products of 100 .. 16384 rows
+// the plan is 0.6 % off the fastest measured, 7 % at most.
+enum { kPlanNT = 0, kPlanNN = 1, kPlanTN = 2 };  // launch.hpp's DenseLayout
+inline DensePlan dense_plan(const DenseShape* sh, int nprob, int nk, int max_split, int cus, int layout) {
   DensePlan best{0, 0, 1, 1};
   int64_t least = 0, plane = 0;
   for (int i = 0; i < nprob; ++i) plane += sh[i].rows * sh[i].cols;
@@ -178,7 +195,7 @@ inline DensePlan dense_plan(const DenseShape* sh, int nprob, int nk, int max_spl
       const int64_t stages = (nk + ks * kg - 1) / (ks * kg);
       auto round = [&](int64_t w) {
         const int64_t step = w * kg * each > alone ? w * kg * each : alone;
-        return (stages + 2) * step + w * ((ks > 1 ? 300 : rows ? 130 : 210) + 50 * (kg - 1)) * mi * ni;
+        return (stages + 2) * step + w * ((ks > 1 ? 300 : layout == kPlanNT ? 130 : 110) + 50 * (kg - 1)) * mi * ni;
       };
       int64_t c = n / occ * round(occ);
       if (n % occ != 0) c += round(n % occ);
@@ -190,10 +207,10 @@ inline DensePlan dense_plan(const DenseShape* sh, int nprob, int nk, int max_spl
     }
   };
 #define W4A16_DG(MI_, NI_, KG_, OCC_, ALONE_, EACH_) consider(MI_, NI_, KG_, OCC_, ALONE_, EACH_);
-  if (rows) {
-    W4A16_DG_TILES_NT(W4A16_DG)
-  } else {
-    W4A16_DG_TILES(W4A16_DG)
+  switch (layout) {
+    case kPlanNT: W4A16_DG_TILES_NT(W4A16_DG) break;
+    case kPlanTN: W4A16_DG_TILES_TN(W4A16_DG) break;
+    default: W4A16_DG_TILES(W4A16_DG) break;
   }
 #undef W4A16_DG
   return best;

@@ -20,13 +20,17 @@ int main() {
   printf("-\\n");
 #define W4A16_DG(MI_, NI_, KG_, OCC_, ALONE_, EACH_) printf("%d %d %d\\n", MI_, NI_, KG_);
   W4A16_DG_TILES_NT(W4A16_DG)
+#undef W4A16_DG
   printf("-\\n");
-  long long n, rows, cols, nk, plane, cus, nt;
-  while (scanf("%lld %lld %lld %lld %lld %lld %lld", &n, &rows, &cols, &nk, &plane, &cus, &nt) == 7) {
+#define W4A16_DG(MI_, NI_, KG_, OCC_, ALONE_, EACH_) printf("%d %d %d\\n", MI_, NI_, KG_);
+  W4A16_DG_TILES_TN(W4A16_DG)
+  printf("-\\n");
+  long long n, rows, cols, nk, plane, cus, layout;
+  while (scanf("%lld %lld %lld %lld %lld %lld %lld", &n, &rows, &cols, &nk, &plane, &cus, &layout) == 7) {
     DenseShape sh[3];
     for (int i = 0; i < n; ++i) sh[i] = DenseShape{rows, cols};
     const int planes = dense_part_planes(plane);
-    const DensePlan p = dense_plan(sh, (int)n, (int)nk, planes, (int)cus, nt != 0);
+    const DensePlan p = dense_plan(sh, (int)n, (int)nk, planes, (int)cus, (int)layout);
     printf("%d %d %d %d %d\\n", p.mi, p.ni, p.kg, p.ksplit, planes);
   }
 }
@@ -45,15 +49,15 @@ def plans(tmp_path_factory):
     def run(calls):
         out = subprocess.run([str(d / "plan")], input="\n".join(" ".join(map(str, c)) for c in calls), text=True,
                              capture_output=True, check=True).stdout.split("\n-\n")
-        tiles, nt, got = ([tuple(map(int, ln.split())) for ln in part.split("\n") if ln] for part in out)
-        assert tiles == nt  # one set of tiles, with costs per layout
+        tiles, nt, tn, got = ([tuple(map(int, ln.split())) for ln in part.split("\n") if ln] for part in out)
+        assert tiles == nt == tn  # one set of tiles, with costs per layout
         return tiles, got
 
     return run
 
 
 def test_every_plan_is_built_and_fits(plans):
-    calls = [(n, m, c, nk, n * m * c, cus, nk % 2) for n in (1, 2, 3) for m in (1, 33, 200, 517, 2049, 8192, 100_000)
+    calls = [(n, m, c, nk, n * m * c, cus, nk % 3) for n in (1, 2, 3) for m in (1, 33, 200, 517, 2049, 8192, 100_000)
              for c in (32, 512, 2112, 4224, 32768) for nk in (0, 1, 7, 66, 256, 5000) for cus in (32, 256, 304)]
     tiles, got = plans(calls)
     assert len(tiles) == len(set(tiles))
@@ -65,16 +69,19 @@ def test_every_plan_is_built_and_fits(plans):
 
 
 # x W^T, dy W and dy^T x at the model's shapes: the tiles (and splits) within 6 % of the fastest measured
-MEASURED = [
-    ((1, 8192, 4224, 88, 8192 * 4224, 1), {"8x6x1", "6x8x1", "6x6x1"}),
-    ((1, 8192, 2816, 66, 8192 * 2816, 1), {"8x6x1", "6x8x1"}),
-    ((1, 8192, 2112, 88, 8192 * 2112, 0), {"6x6x1"}),
-    ((1, 2049, 2816, 88, 2049 * 2816, 1), {"6x4x1", "4x6x1"}),
-    ((1, 517, 2816, 66, 517 * 2816, 1), {"4x2x1"}),
-    ((1, 517, 2112, 88, 517 * 2112, 0), {"2x4x2"}),
-    ((1, 100, 2816, 66, 100 * 2816, 1), {"2x2x1"}),
-    ((1, 1024, 2816, 88, 1024 * 2816, 1), {"4x4x1"}),
-    ((3, 2816, 2112, 256, 3 * 2816 * 2112, 0), {"6x6x1"}),
+MEASURED = [  # products, rows, columns, stages of 32 k, partial plane, layout (x W^T 0, dy W 1, dy^T x 2)
+    ((1, 8192, 4224, 88, 8192 * 4224, 0), {"8x6x1", "6x8x1"}),
+    ((1, 8192, 2816, 66, 8192 * 2816, 0), {"8x6x1", "6x8x1"}),
+    ((1, 8192, 2112, 88, 8192 * 2112, 1), {"6x6x1"}),
+    ((1, 2049, 2816, 88, 2049 * 2816, 0), {"6x4x1", "4x6x1"}),
+    ((1, 2049, 2816, 88, 2049 * 2816, 1), {"6x4x1"}),
+    ((1, 517, 2816, 66, 517 * 2816, 0), {"4x2x1"}),
+    ((1, 517, 2112, 88, 517 * 2112, 1), {"2x4x2"}),
+    ((1, 100, 2816, 66, 100 * 2816, 0), {"2x2x1"}),
+    ((1, 1024, 2816, 88, 1024 * 2816, 0), {"4x4x1"}),
+    ((3, 2816, 2112, 256, 3 * 2816 * 2112, 2), {"6x6x1"}),
+    ((2, 2816, 2816, 65, 2 * 2816 * 2816, 2), {"8x8x1", "8x4x1", "4x8x1", "6x6x1"}),
+    ((2, 2816, 2816, 1, 2 * 2816 * 2816, 2), {"8x4x1", "4x8x1", "6x6x1"}),
 ]
 
 
