@@ -119,12 +119,12 @@ inline int linear_w4_blocks(int64_t M, int64_t N, int cus, int max_blocks) {
   X(2, 2, 1, 4, 160, 130) \
   X(2, 2, 4, 1, 160, 118)
 #define W4A16_DG_TILES_TN(X) \
-  X(8, 8, 1, 1, 730, 750)    \
+  X(8, 8, 1, 1, 730, 730)    \
   X(8, 6, 1, 1, 550, 570)    \
   X(6, 8, 1, 1, 535, 575)    \
   X(6, 6, 1, 2, 425, 412)    \
-  X(8, 4, 1, 2, 400, 373)    \
-  X(4, 8, 1, 2, 420, 393)    \
+  X(8, 4, 1, 2, 400, 380)    \
+  X(4, 8, 1, 2, 420, 395)    \
   X(6, 4, 1, 2, 320, 294)    \
   X(4, 6, 1, 2, 350, 300)    \
   X(4, 4, 1, 2, 250, 215)    \
@@ -178,9 +178,9 @@ inline int dense_part_planes(int64_t plane) {
 }
 // The tile and split whose time comes out least: rounds of the workgroups that
 // fit at once, each nk stages and an epilogue of some 110 ns per 16 x 16 tiles
-// of a wavefront (x W^T 130); a split's launch that adds its planes
-// takes 3 us and their bytes at 4 TB/s.  Over 90 products of 100 .. 16384 rows
-// the plan is 0.6 % off the fastest measured, 7 % at most.
+// of a wavefront (130 where a workgroup has its CU alone); a split's launch that
+// adds its planes takes 3 us and their bytes at 4 TB/s.  Over 85 products of
+// 100 .. 16384 rows the plan is 0.5 % off the fastest measured, 6 % at most.
 enum { kPlanNT = 0, kPlanNN = 1, kPlanTN = 2 };  // launch.hpp's DenseLayout
 inline DensePlan dense_plan(const DenseShape* sh, int nprob, int nk, int max_split, int cus, int layout) {
   DensePlan best{0, 0, 1, 1};
@@ -195,7 +195,7 @@ inline DensePlan dense_plan(const DenseShape* sh, int nprob, int nk, int max_spl
       const int64_t stages = (nk + ks * kg - 1) / (ks * kg);
       auto round = [&](int64_t w) {
         const int64_t step = w * kg * each > alone ? w * kg * each : alone;
-        return (stages + 2) * step + w * ((ks > 1 ? 300 : layout == kPlanNT ? 130 : 110) + 50 * (kg - 1)) * mi * ni;
+        return (stages + 2) * step + w * ((ks > 1 ? 300 : occ == 1 ? 130 : 110) + 50 * (kg - 1)) * mi * ni;
       };
       int64_t c = n / occ * round(occ);
       if (n % occ != 0) c += round(n % occ);
