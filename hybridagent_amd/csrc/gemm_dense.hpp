@@ -620,9 +620,12 @@ __global__ __launch_bounds__(KG * kDgThreads, MI * NI > 36 ? 1 : KG > 2 ? KG : 2
   float* const rows = reinterpret_cast<float*>(smem + kSums) + wave * kPlanes * 16 * kPitch;
   const int r0 = m0 + 16 * MI * (wave >> 1), c0 = n0 + 16 * NO * (wave & 1);
   const DgTarget g = dg_target(a, p, split, r0, 16 * MI, GU);
-  // What it reads is asked for kAhead steps of 16 rows before it is needed: a
-  // step by itself would wait for memory.
-  constexpr int kAhead = EPI != kDgGateUpBack ? 3 : MI * NI > 24 && !kAccRegs ? 0 : 1;
+  // What it reads is asked for some steps of 16 rows before it is needed: a step
+  // by itself would wait for memory.  Four vectors per element (kDgGateUpBack)
+  // leave registers for one step ahead, once a step's sums are in LDS (8192 rows
+  // 2816 -> 2112 139 to 134 us), and in 4 x 8 tiles for none.
+  constexpr int kAhead = EPI != kDgGateUpBack ? 3 : kIter > 3 && !kAccRegs ? 0 : 1;
+  constexpr bool kLate = kAhead == 1;
   DgIn in[MI][kIter];
   int o[MI][kIter];
   u32x4_t bias[kIter];
@@ -641,13 +644,14 @@ __global__ __launch_bounds__(KG * kDgThreads, MI * NI > 36 ? 1 : KG > 2 ? KG : 2
   for (int m = 0; m < kAhead && m < MI; ++m) fetch(m);
 #pragma unroll
   for (int m = 0; m < MI; ++m) {
-        if (m + kAhead < MI) fetch(m + kAhead);
+    if (!kLate && m + kAhead < MI) fetch(m + kAhead);
 #pragma unroll
     for (int n = 0; n < NO; ++n) {
       float* q = rows + (lane & 15) * kPitch + 16 * n + 4 * (lane >> 4);
       *reinterpret_cast<f32x4_t*>(q) = acc[m][n];
       if (GU) *reinterpret_cast<f32x4_t*>(q + 16 * kPitch) = acc[m][GU ? n + NO : n];
     }
+    if (kLate && m + kAhead < MI) fetch(m + kAhead);
 #pragma unroll
     for (int i = 0; i < kIter; ++i) {
       const int idx = min(lane + 64 * i, 32 * NO - 1);
