@@ -10,15 +10,15 @@
 // four consecutive n of one row m.
 //
 // A workgroup of four wavefronts (2 x 2) owns a tile of 32 MI rows x 32 NI
-// columns, a wavefront 16 MI x 16 NI of it; with KG > 1 there are KG such
-// groups, each with a part of K and a ring of its own, whose sums are added in
-// LDS (a few hundred rows: a wavefront's chain of stages is what takes the
-// time).  k advances in stages of 32 through a ring of dg_slots LDS slots filled
-// by direct 16-byte global -> LDS loads; the fragments of stage t + 1 are read
-// while stage t is multiplied, so that a slot has one barrier and its loads
-// have two to three stages to land.  Slots past the end are issued with an empty
-// buffer descriptor, which reads nothing, so that every wait counts the same
-// loads.
+// columns, a wavefront 16 MI x 16 NI of it; with KG > 1 (dy W and dy^T x) there
+// are KG such groups, each with a part of K and a ring of its own, whose sums
+// are added in LDS (a few hundred rows: a wavefront's chain of stages is what
+// takes the time).  k advances in stages of 32 through a ring of dg_slots LDS
+// slots filled by direct 16-byte global -> LDS loads; the fragments of stage
+// t + 1 are read while stage t is multiplied, so that a slot has one barrier and
+// its loads have two to three stages to land.  Slots past the end are issued
+// with an empty buffer descriptor, which reads nothing, so that every wait
+// counts the same loads.
 //
 // A slot is a stage; in x W^T two, so that each row comes in whole 128-byte
 // lines: half a line per stage has left the L1 before the other half is asked
@@ -722,7 +722,13 @@ template <int LAYOUT, int EPI>
 hipError_t dg_launch_tile(const DgArgs& a, hipStream_t s) {
 #define W4A16_DG(MI_, NI_, KG_, OCC_, ALONE_, EACH_) \
   if (a.mi == MI_ && a.ni == NI_ && a.kg == KG_) return dg_launch<LAYOUT, EPI, MI_, NI_, KG_>(a, s);
-  W4A16_DG_TILES(W4A16_DG)
+  if constexpr (LAYOUT == kDgNT) {
+    W4A16_DG_TILES_NT(W4A16_DG)
+  } else if constexpr (LAYOUT == kDgNN) {
+    W4A16_DG_TILES_NN(W4A16_DG)
+  } else {
+    W4A16_DG_TILES_TN(W4A16_DG)
+  }
 #undef W4A16_DG
   return hipErrorInvalidValue;
 }

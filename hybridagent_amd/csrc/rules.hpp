@@ -101,32 +101,30 @@ inline int linear_w4_blocks(int64_t M, int64_t N, int cus, int max_blocks) {
 // operand columns by kg groups of wavefronts, with the workgroups that share a
 // CU and what a stage of 32 k takes, in ns, for a group alone on a CU and for
 // each of several (256 .. 1024 tiles of K = 64, 512 and 2816): dy W, dy^T x and
-// x W^T.
-#define W4A16_DG_TILES(X) \
-  X(8, 8, 1, 1, 750, 775) \
-  X(8, 6, 1, 1, 590, 595) \
-  X(6, 8, 1, 1, 570, 575) \
-  X(6, 6, 1, 2, 460, 435) \
-  X(8, 4, 1, 2, 410, 413) \
-  X(4, 8, 1, 2, 450, 408) \
-  X(6, 4, 1, 2, 350, 325) \
-  X(4, 6, 1, 2, 370, 319) \
-  X(4, 4, 1, 2, 290, 243) \
-  X(4, 4, 2, 1, 290, 255) \
-  X(4, 2, 1, 3, 210, 190) \
-  X(2, 4, 1, 3, 205, 178) \
-  X(2, 4, 2, 1, 205, 167) \
-  X(2, 2, 1, 4, 160, 130) \
+// x W^T.  Tiles that the rule would take for less than some 1 % of 200,000
+// random shapes are left out.
+#define W4A16_DG_TILES_NN(X) \
+  X(8, 8, 1, 1, 750, 775)    \
+  X(8, 6, 1, 1, 590, 595)    \
+  X(6, 8, 1, 1, 570, 575)    \
+  X(6, 6, 1, 2, 460, 435)    \
+  X(8, 4, 1, 2, 410, 413)    \
+  X(4, 8, 1, 2, 450, 408)    \
+  X(6, 4, 1, 2, 350, 325)    \
+  X(4, 6, 1, 2, 370, 319)    \
+  X(4, 4, 1, 2, 290, 243)    \
+  X(4, 4, 2, 1, 290, 255)    \
+  X(4, 2, 1, 3, 210, 190)    \
+  X(2, 4, 1, 3, 205, 178)    \
+  X(2, 4, 2, 1, 205, 167)    \
+  X(2, 2, 1, 4, 160, 130)    \
   X(2, 2, 4, 1, 160, 118)
 #define W4A16_DG_TILES_TN(X) \
   X(8, 8, 1, 1, 730, 730)    \
   X(8, 6, 1, 1, 550, 570)    \
-  X(6, 8, 1, 1, 535, 575)    \
   X(6, 6, 1, 2, 425, 412)    \
   X(8, 4, 1, 2, 400, 380)    \
-  X(4, 8, 1, 2, 420, 395)    \
   X(6, 4, 1, 2, 320, 294)    \
-  X(4, 6, 1, 2, 350, 300)    \
   X(4, 4, 1, 2, 250, 215)    \
   X(4, 4, 2, 1, 250, 210)    \
   X(4, 2, 1, 3, 170, 150)    \
@@ -140,16 +138,11 @@ inline int linear_w4_blocks(int64_t M, int64_t N, int cus, int max_blocks) {
   X(6, 8, 1, 1, 525, 525)    \
   X(6, 6, 1, 1, 460, 460)    \
   X(8, 4, 1, 1, 420, 420)    \
-  X(4, 8, 1, 1, 425, 425)    \
   X(6, 4, 1, 1, 320, 320)    \
-  X(4, 6, 1, 1, 345, 345)    \
   X(4, 4, 1, 1, 235, 235)    \
-  X(4, 4, 2, 1, 235, 250)    \
   X(4, 2, 1, 2, 145, 135)    \
   X(2, 4, 1, 2, 160, 140)    \
-  X(2, 4, 2, 1, 160, 145)    \
-  X(2, 2, 1, 3, 97, 90)      \
-  X(2, 2, 4, 1, 97, 115)
+  X(2, 2, 1, 3, 97, 90)
 
 // Products of few rows run as the weights' stream (gemm_thin.hpp), 32 rows x
 // `cols` columns a workgroup: up to 64 rows, and up to 512 while the workgroups
@@ -210,7 +203,7 @@ inline DensePlan dense_plan(const DenseShape* sh, int nprob, int nk, int max_spl
   switch (layout) {
     case kPlanNT: W4A16_DG_TILES_NT(W4A16_DG) break;
     case kPlanTN: W4A16_DG_TILES_TN(W4A16_DG) break;
-    default: W4A16_DG_TILES(W4A16_DG) break;
+    default: W4A16_DG_TILES_NN(W4A16_DG) break;
   }
 #undef W4A16_DG
   return best;

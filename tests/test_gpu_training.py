@@ -381,6 +381,22 @@ def test_hybridlink_few_rows_of_wide_or_narrow_outputs(dev, T, H):
     test_hybridlink_training(dev, T, H)
 
 
+# with the shapes above: every tile of every product and epilogue, and every split's join, on 256 CUs
+@pytest.mark.parametrize("T,H,I", [
+    (265, 32, 5472), (1574, 5024, 32), (1990, 64, 3616), (2053, 64, 5472), (2160, 5920, 480), (2883, 992, 4320),
+    (9592, 1184, 64), (12212, 672, 32), (12840, 768, 864), (13445, 32, 544), (16898, 544, 416), (18069, 96, 768),
+    (18484, 352, 192), (19030, 544, 128), (20342, 640, 256)])
+def test_gated_mlp_every_tile(dev, T, H, I):
+    test_gated_mlp(dev, T, H, I)
+
+
+@pytest.mark.parametrize("T,H", [
+    (1, 4128), (65, 2784), (66, 5408), (66, 5664), (5398, 352), (13124, 960), (16349, 704), (16382, 320), (16402, 480),
+    (19737, 288), (19995, 608), (21795, 352), (21846, 416), (21902, 192)])
+def test_hybridlink_every_tile(dev, T, H):
+    test_hybridlink_training(dev, T, H)
+
+
 @pytest.mark.parametrize("bad", [math.nan, math.inf])
 @pytest.mark.parametrize("T", [5, 40, 64, 300, 700])
 def test_a_row_that_is_not_finite_stays_alone(dev, T, bad):
