@@ -434,8 +434,8 @@ hipError_t ln_backward(const LnArgs& a, hipStream_t s) {
 #define W4A16_LN(EPT_, TPR_)                                                  \
   do {                                                                        \
     if (a.add != nullptr) {                                                   \
-      /* (HybridLink's rows alone) */                                         \
-      if constexpr (std::is_same<T, __bf16>::value) W4A16_LN1(EPT_, TPR_, true); \
+      /* (HybridLink's rows alone, whose H and pointers allow vectors) */       \
+      if constexpr (std::is_same<T, __bf16>::value && VEC > 1) W4A16_LN1(EPT_, TPR_, true); \
       else return hipErrorInvalidValue;                                       \
     } else {                                                                  \
       W4A16_LN1(EPT_, TPR_, false);                                           \

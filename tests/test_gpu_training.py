@@ -140,6 +140,13 @@ def test_layer_norm_rows_do_not_meet(dev):
     assert torch.equal(yz[keep], y[keep])
 
 
+@pytest.mark.parametrize("dt", [BF, HF, SF], ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("M,H", [(600, 1544), (600, 1999), (5, 3001)])
+def test_layer_norm_other_row_lengths(dev, M, H, dt):
+    """Rows that the shapes above leave out: other numbers of elements per thread."""
+    test_layer_norm(dev, M, H, dt)
+
+
 @pytest.mark.parametrize("H,dt", [(2816, BF), (1000, SF), (24, HF)])
 def test_layer_norm_layouts(dev, H, dt):
     """Leading shapes, strided rows, rows at any alignment of their type: the same bits."""
