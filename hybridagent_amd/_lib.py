@@ -976,9 +976,9 @@ def hybridlink_train(h: torch.Tensor, ln1_w: torch.Tensor, ln1_b: torch.Tensor, 
                      p1_b: torch.Tensor, p2_w: torch.Tensor, p2_b: torch.Tensor, ln2_w: torch.Tensor,
                      ln2_b: torch.Tensor, eps: float = 1e-5):
     """``hybridlink`` (hybridlink.py:17-28) for training -> (out, saved): ``saved`` is what
-    ``hybridlink_backward`` needs, one uint8 tensor of about 8 bytes per element of h.  Each
-    intermediate is rounded to bf16 once, from fp32 (``hybridlink`` rounds where the torch
-    modules do)."""
+    ``hybridlink_backward`` needs, one uint8 tensor of about 12 bytes per element of h.  Only
+    what a product takes is rounded to bf16, once, from fp32 (``hybridlink`` rounds where the
+    torch modules do)."""
     dev = _require_gpu(h, ln1_w, ln1_b, p1_w, p1_b, p2_w, p2_b, ln2_w, ln2_b)
     h = _bf16(h, "h")
     params, H = _link_params(h, (ln1_w, ln1_b, p1_w, p1_b, p2_w, p2_b, ln2_w, ln2_b))

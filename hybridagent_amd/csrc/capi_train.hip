@@ -108,15 +108,16 @@ MlpBackWs mlp_back_ws(void* p, int64_t M, int64_t H, int64_t I) {
   return w;
 }
 
-// HybridLink's tensors between the kernels are bf16, rounded once each from
-// fp32: a, g, dr and dz are operands of the bf16 matrix instructions, and z, r
-// and da, which only an activation or a norm reads, would in fp32 be 12 more
-// bytes per element and step and take away one of some four roundings on a
-// gradient's way.  Against 64 bits (Frobenius norm, 2049 rows of 2816) out is
-// 0.0027 off and the gradients 0.0016 .. 0.0040; torch's bf16 modules under
-// autograd 0.0031 and 0.0016 .. 0.0043, one rounding alone 0.0017.
+// HybridLink's tensors between the kernels: a, g, dr and dz are operands of the
+// bf16 matrix instructions and rounded once each, from fp32.  z, r and da, which
+// an activation or a norm reads, and dr where it is the residual's gradient or
+// summed, stay in fp32 (2049 rows of 2816: 17 us of a step of 280; rounded to
+// bf16, r alone would lose what proj2 adds to a row far from zero).  Against 64
+// bits (Frobenius norm, the same rows) out is 0.0021 off and the gradients
+// 0.0017 .. 0.0036, a single rounding 0.0017.
 struct LinkSaved {
-  uint16_t *a, *z, *g, *r;
+  uint16_t *a, *g;
+  float *z, *r;
   float *mean1, *rstd1, *mean2, *rstd2;
   size_t bytes;
 };
@@ -124,9 +125,9 @@ LinkSaved link_saved(void* p, int64_t B, int64_t H) {
   Carve c(p);
   LinkSaved s;
   s.a = c.take<uint16_t>(B * H);
-  s.z = c.take<uint16_t>(B * H);
   s.g = c.take<uint16_t>(B * H);
-  s.r = c.take<uint16_t>(B * H);
+  s.z = c.take<float>(B * H);
+  s.r = c.take<float>(B * H);
   s.mean1 = c.take<float>(B);
   s.rstd1 = c.take<float>(B);
   s.mean2 = c.take<float>(B);
@@ -136,7 +137,8 @@ LinkSaved link_saved(void* p, int64_t B, int64_t H) {
 }
 
 struct LinkBackWs {
-  uint16_t *dr, *dz, *da;
+  uint16_t *dr, *dz;
+  float *dr32, *da;
   float *part, *ln2, *ln1, *cols;
   size_t bytes;
 };
@@ -145,7 +147,8 @@ LinkBackWs link_back_ws(void* p, int64_t B, int64_t H) {
   LinkBackWs w;
   w.dr = c.take<uint16_t>(B * H);
   w.dz = c.take<uint16_t>(B * H);
-  w.da = c.take<uint16_t>(B * H);
+  w.dr32 = c.take<float>(B * H);
+  w.da = c.take<float>(B * H);
   w.part = c.take<float>(std::max(part_floats(B * H), part_floats(2 * H * H)));
   // partial rows of the column sums, added in one launch at the end
   w.ln2 = c.take<float>((size_t)ln_partials(B) * 2 * H);
@@ -322,12 +325,13 @@ int w4a16_hybridlink_train(const uint16_t* h, const uint16_t* ln1_w, const uint1
   hipError_t e = launch_ln_forward(W4A16_BF16, ln_args(h, ln1_w, ln1_b, sv.a, sv.mean1, sv.rstd1, B, H, eps), s);
   if (e == hipSuccess)
     e = product(kDgNT, kDgBiasGelu,
-                problem(sv.a, H, p1_w, H, B, H, DgEpilogue{sv.g, sv.z, nullptr, nullptr, nullptr, p1_b}), H, part, s);
+                problem(sv.a, H, p1_w, H, B, H, DgEpilogue{sv.g, nullptr, sv.z, nullptr, nullptr, p1_b}), H, part, s);
   if (e == hipSuccess)
     e = product(kDgNT, kDgBiasResidual,
-                problem(sv.g, H, p2_w, H, B, H, DgEpilogue{sv.r, nullptr, nullptr, nullptr, h, p2_b}), H, part, s);
-  if (e == hipSuccess)
-    e = launch_ln_forward(W4A16_BF16, ln_args(sv.r, ln2_w, ln2_b, out, sv.mean2, sv.rstd2, B, H, eps), s);
+                problem(sv.g, H, p2_w, H, B, H, DgEpilogue{nullptr, nullptr, sv.r, nullptr, h, p2_b}), H, part, s);
+  LnArgs n2 = ln_args(sv.r, ln2_w, ln2_b, out, sv.mean2, sv.rstd2, B, H, eps);
+  n2.form = kLnPost;
+  if (e == hipSuccess) e = launch_ln_forward(W4A16_BF16, n2, s);
   return launch_status(e);
 }
 
@@ -356,16 +360,20 @@ int w4a16_hybridlink_backward(const uint16_t* dout, const uint16_t* h, const uin
   const LinkBackWs ws = link_back_ws(B > 0 ? workspace : nullptr, B, H);
   // post_ln: dr, the gradient of r = h + proj2(g)
   LnArgs n2 = ln_args(sv.r, ln2_w, nullptr, ws.dr, sv.mean2, sv.rstd2, B, H, 0.f);
+  n2.form = kLnPost;
+  n2.y32 = ws.dr32;
   n2.dy = dout;
   n2.part = ws.ln2;
   hipError_t e = launch_ln_backward(W4A16_BF16, n2, s);
   // dz = (dr W2) gelu'(z), da = dz W1
   if (e == hipSuccess && B > 0)
     e = product(kDgNN, kDgGeluBack,
-                problem(ws.dr, H, p2_w, H, B, H, DgEpilogue{ws.dz, nullptr, nullptr, nullptr, sv.z, nullptr}), H,
+                problem(ws.dr, H, p2_w, H, B, H, DgEpilogue{ws.dz, nullptr, sv.z, nullptr, nullptr, nullptr}), H,
                 ws.part, s);
   if (e == hipSuccess && B > 0)
-    e = product(kDgNN, kDgPlain, problem(ws.dz, H, p1_w, H, B, H, to(ws.da)), H, ws.part, s);
+    e = product(kDgNN, kDgSums,
+                problem(ws.dz, H, p1_w, H, B, H, DgEpilogue{nullptr, nullptr, ws.da, nullptr, nullptr, nullptr}), H,
+                ws.part, s);
   if (e == hipSuccess) {
     DgArgs a{};
     a.prob[0] = problem(ws.dr, H, sv.g, H, H, H, to(dp2_w));
@@ -376,11 +384,12 @@ int w4a16_hybridlink_backward(const uint16_t* dout, const uint16_t* h, const uin
     e = launch_gemm_dense(kDgTN, kDgPlain, a, s);
   }
   const int sums = column_sum_partials(B);
-  if (e == hipSuccess && sums > 0) e = launch_column_sums(ws.dr, ws.dz, B, (int)H, ws.cols, s);
+  if (e == hipSuccess && sums > 0) e = launch_column_sums(ws.dr32, ws.dz, B, (int)H, ws.cols, s);
   // pre_ln, and the residual's dr
   LnArgs n1 = ln_args(h, ln1_w, nullptr, dh, sv.mean1, sv.rstd1, B, H, 0.f);
+  n1.form = kLnPre;
   n1.dy = ws.da;
-  n1.add = ws.dr;
+  n1.add = ws.dr32;
   n1.part = ws.ln1;
   if (e == hipSuccess) e = launch_ln_backward(W4A16_BF16, n1, s);
   LnJoin j{};
@@ -389,7 +398,7 @@ int w4a16_hybridlink_backward(const uint16_t* dout, const uint16_t* h, const uin
   if (sums > 0 || B == 0)
     j.seg[2] = {ws.cols, sums, dp2_b, dp1_b, nullptr, nullptr};
   else
-    j.seg[2] = {nullptr, (int)B, dp2_b, dp1_b, ws.dr, ws.dz};
+    j.seg[2] = {nullptr, (int)B, dp2_b, dp1_b, ws.dr32, ws.dz};
   j.n = 3;
   j.H = (int)H;
   if (e == hipSuccess) e = launch_column_join(W4A16_BF16, j, s);

@@ -284,8 +284,11 @@ __device__ __forceinline__ DgIn dg_fetch(const DgTarget& g, int o) {
       r.v[k] = buf_ld16(g.sum, 4 * o, 16 * k);
       r.v[2 + k] = buf_ld16(g.sum2, 4 * o, 16 * k);
     }
-  } else if (EPI == kDgBiasResidual || EPI == kDgGeluBack) {
+  } else if (EPI == kDgBiasResidual) {
     r.v[0] = buf_ld16(g.in, 2 * o, 0);
+  } else if (EPI == kDgGeluBack) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) r.v[k] = buf_ld16(g.sum, 4 * o, 16 * k);
   }
   return r;
 }
@@ -335,23 +338,25 @@ __device__ __forceinline__ void dg_finish(const DgTarget& g, int o, const float 
       gelu_erf_and_slope(s[i], &r[i], &slope);
     }
     dg_st8(g.out, o, r);
-    dg_st8(g.out2, o, s);
+    dg_st8_f32(g.sum, o, s);
   } else if constexpr (EPI == kDgBiasResidual) {
     float b[8];
     dg_unpack8(in.bias, b);
     dg_unpack8(in.v[0], s);
 #pragma unroll
     for (int i = 0; i < 8; ++i) r[i] = s[i] + (v[i] + b[i]);
-    dg_st8(g.out, o, r);
+    dg_st8_f32(g.sum, o, r);
   } else if constexpr (EPI == kDgGeluBack) {
-    dg_unpack8(in.v[0], s);
+    const uint32_t z[8] = {in.v[0].x, in.v[0].y, in.v[0].z, in.v[0].w, in.v[1].x, in.v[1].y, in.v[1].z, in.v[1].w};
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       float act, slope;
-      gelu_erf_and_slope(s[i], &act, &slope);
+      gelu_erf_and_slope(__uint_as_float(z[i]), &act, &slope);
       r[i] = v[i] * slope;
     }
     dg_st8(g.out, o, r);
+  } else if constexpr (EPI == kDgSums) {
+    dg_st8_f32(g.sum, o, v);
   }
 }
 
@@ -631,8 +636,10 @@ __global__ __launch_bounds__(KG * kDgThreads, MI * NI > 36 ? 1 : KG > 2 ? KG : 2
   // What it reads is asked for some steps of 16 rows before it is needed: a step
   // by itself would wait for memory.  Four vectors per element (kDgGateUpBack)
   // leave registers for one step ahead, once a step's sums are in LDS (8192 rows
-  // 2816 -> 2112 139 to 134 us), and in 4 x 8 tiles for none.
-  constexpr int kAhead = EPI != kDgGateUpBack ? 3 : kIter > 3 && !kAccRegs ? 0 : 1;
+  // 2816 -> 2112 139 to 134 us), and in 4 x 8 tiles for none.  Two (kDgGeluBack)
+  // leave them for one step in the tiles that fill the vector registers.
+  constexpr bool kFull = MI * NI > 24 && !kAccRegs;
+  constexpr int kAhead = EPI == kDgGateUpBack ? (kIter > 3 && !kAccRegs ? 0 : 1) : EPI == kDgGeluBack && kFull ? 1 : 3;
   constexpr bool kLate = kAhead == 1;
   DgIn in[MI][kIter];
   int o[MI][kIter];

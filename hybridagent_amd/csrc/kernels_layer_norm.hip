@@ -1,5 +1,6 @@
 // Layer norm and its backward pass for rows of bf16, fp16 or fp32 (weights in
-// the rows' type, everything computed in fp32):
+// the rows' type, everything computed in fp32), and for HybridLink's bf16 rows
+// beside fp32 ones (LnForm):
 //   mean = sum x / H, rstd = 1 / sqrt(sum (x - mean)^2 / H + eps)
 //   y = (x - mean) rstd w + b
 //   xh = (x - mean) rstd, g = dy w
@@ -59,16 +60,23 @@ struct LnRaw {
     for (int q = 0; q < NQ; ++q) {
       const int o = t * kChunk + TPR * q * kChunk;
       if constexpr (VEC > 1) {
-        const u32x4_t v = buf_ld16(r, o, 0);
-        w[q][0] = v.x;
-        w[q][1] = v.y;
-        w[q][2] = v.z;
-        w[q][3] = v.w;
+        load_chunk(r, q, o);
       } else if constexpr (sizeof(T) == 4) {
         w[q][0] = __builtin_amdgcn_raw_buffer_load_b32(r, o, 0, 0);
       } else {
         w[q][0] = buf_ld_u16(r, o);
       }
+    }
+  }
+  // VEC elements of 16 bytes, or of 32 beside 16-bit ones of 16
+  __device__ __forceinline__ void load_chunk(__amdgpu_buffer_rsrc_t r, int q, int o) {
+#pragma unroll
+    for (int i = 0; i + 4 <= kWords; i += 4) {
+      const u32x4_t v = buf_ld16(r, o, 4 * i);
+      w[q][i] = v.x;
+      w[q][i + 1] = v.y;
+      w[q][i + 2] = v.z;
+      w[q][i + 3] = v.w;
     }
   }
   __device__ __forceinline__ float get(int q, int e) const {
@@ -92,11 +100,15 @@ __device__ __forceinline__ void ln_store(__amdgpu_buffer_rsrc_t r, int t, int q,
   constexpr int kChunk = VEC * (int)sizeof(T);
   const int o = t * kChunk + TPR * q * kChunk;
   if constexpr (VEC > 1) {
-    typedef T vec_t __attribute__((ext_vector_type(VEC)));
-    vec_t u;
+    constexpr int N = 16 / (int)sizeof(T);
+    typedef T vec_t __attribute__((ext_vector_type(N)));
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) u[i] = (T)v[i];
-    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, u), r, o, 0, 0);
+    for (int j = 0; j < VEC; j += N) {
+      vec_t u;
+#pragma unroll
+      for (int i = 0; i < N; ++i) u[i] = (T)v[j + i];
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, u), r, o + j * (int)sizeof(T), 0, 0);
+    }
   } else if constexpr (sizeof(T) == 4) {
     __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v[0]), r, o, 0, 0);
   } else {
@@ -139,9 +151,10 @@ __device__ __forceinline__ int ln_row_of() {
 
 }  // namespace
 
-template <typename T, int VEC, int EPT, int TPR>
+template <typename T, int VEC, int EPT, int TPR, int FORM>
 __global__ __launch_bounds__(ln_threads(TPR)) void k_ln_forward(LnArgs a) {
   using Raw = LnRaw<T, VEC, EPT, TPR>;
+  using TX = std::conditional_t<FORM == kLnPost, float, T>;
   __shared__ float part[TPR > 64 ? TPR / 64 : 1];
   constexpr int RPB = ln_threads(TPR) / TPR;  // rows per workgroup
   const int t = threadIdx.x % TPR;
@@ -149,9 +162,10 @@ __global__ __launch_bounds__(ln_threads(TPR)) void k_ln_forward(LnArgs a) {
   const float fh = (float)H;
   int64_t row = (int64_t)blockIdx.x * RPB + ln_row_of<TPR>();
   if (row >= a.M) return;  // (a workgroup per row: all of it)
-  Raw x, w, b;
+  LnRaw<TX, VEC, EPT, TPR> x;
+  Raw w, b;
   // the row first: its statistics wait for nothing else
-  x.load(static_cast<const T*>(a.x) + row * H, t, H);
+  x.load(static_cast<const TX*>(a.x) + row * H, t, H);
   w.load(a.w, t, H);
   b.load(a.b != nullptr ? a.b : a.w, t, a.b != nullptr ? H : 0);
   for (;;) {
@@ -190,15 +204,20 @@ __global__ __launch_bounds__(ln_threads(TPR)) void k_ln_forward(LnArgs a) {
     }
     row += (int64_t)gridDim.x * RPB;
     if (row >= a.M) break;
-    x.load(static_cast<const T*>(a.x) + row * H, t, H);
+    x.load(static_cast<const TX*>(a.x) + row * H, t, H);
     w.forget();
     b.forget();
   }
 }
 
-template <typename T, int VEC, int EPT, int TPR, bool ADD>
+template <typename T, int VEC, int EPT, int TPR, int FORM>
 __global__ __launch_bounds__(ln_back_threads(TPR)) void k_ln_backward(LnArgs a) {
   using Raw = LnRaw<T, VEC, EPT, TPR>;
+  using TX = std::conditional_t<FORM == kLnPost, float, T>;
+  using TDY = std::conditional_t<FORM == kLnPre, float, T>;
+  using RawF = LnRaw<float, VEC, EPT, TPR>;
+  constexpr bool ADD = FORM == kLnPre;
+  constexpr bool kEarly = EPT <= 32;  // registers for all of a row's `add` at once
   constexpr int RPB = ln_back_threads(TPR) / TPR;
   extern __shared__ __align__(16) float smem[];  // TPR > 64: a row's sums; else column sums, [4][2][EPT][64]
   const int t = threadIdx.x % TPR;
@@ -210,10 +229,12 @@ __global__ __launch_bounds__(ln_back_threads(TPR)) void k_ln_backward(LnArgs a) 
 #pragma unroll
   for (int i = 0; i < EPT; ++i) dw[i] = db[i] = 0.f;
   for (int64_t row = (int64_t)blockIdx.x * RPB + ln_row_of<TPR>(); row < a.M; row += (int64_t)gridDim.x * RPB) {
-    Raw x, dy, add;
-    x.load(static_cast<const T*>(a.x) + row * H, t, H);
-    dy.load(static_cast<const T*>(a.dy) + row * H, t, H);
-    if (ADD) add.load(static_cast<const T*>(a.add) + row * H, t, H);
+    LnRaw<TX, VEC, EPT, TPR> x;
+    LnRaw<TDY, VEC, EPT, TPR> dy;
+    RawF add;
+    x.load(static_cast<const TX*>(a.x) + row * H, t, H);
+    dy.load(static_cast<const TDY*>(a.dy) + row * H, t, H);
+    if (ADD && kEarly) add.load(a.add + row * H, t, H);
     w.forget();
     const float mean = a.mean[row], rstd = a.rstd[row];
     float s[2] = {0.f, 0.f};  // sum g, sum g xh
@@ -234,8 +255,11 @@ __global__ __launch_bounds__(ln_back_threads(TPR)) void k_ln_backward(LnArgs a) 
     dy.forget();
     w.forget();
     const auto dxr = make_rsrc(static_cast<T*>(a.y) + row * H, (uint32_t)(H * (int)sizeof(T)));
+    const auto dx32 = make_rsrc(a.y32 + row * H, FORM == kLnPost ? (uint32_t)H * 4u : 0u);
+    const auto addr = make_rsrc(a.add + row * H, ADD ? (uint32_t)H * 4u : 0u);
 #pragma unroll
     for (int q = 0; q < Raw::NQ; ++q) {
+      if (ADD && !kEarly) add.load_chunk(addr, q, (t + TPR * q) * RawF::kChunk);
       float o[VEC];
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
@@ -244,6 +268,7 @@ __global__ __launch_bounds__(ln_back_threads(TPR)) void k_ln_backward(LnArgs a) 
         if (ADD) o[e] += add.get(q, e);
       }
       ln_store<T, VEC, TPR>(dxr, t, q, o);
+      if (FORM == kLnPost) ln_store<float, VEC, TPR>(dx32, t, q, o);
     }
   }
   // the wavefronts' column sums: the upper half hand theirs to the lower half,
@@ -300,10 +325,12 @@ __global__ __launch_bounds__(ln_back_threads(TPR)) void k_ln_backward(LnArgs a) 
 
 constexpr int kSumPitch = 64 + 4;
 
-// Column sums of rows r0 .. r1 of a bf16 matrix, columns 64 block ..: thread t
-// has columns 8 (t % 8) .. of every 32nd row; the 32 sums are added in order.
-// The result is that of threads t < 64, for column 64 block + t.
-__device__ __forceinline__ float column_sum(const uint16_t* __restrict__ x, int64_t r0, int64_t r1, int H, int block,
+// Column sums of rows r0 .. r1 of a matrix of fp32 or (uint16_t) bf16, columns
+// 64 block ..: thread t has columns 8 (t % 8) .. of every 32nd row; the 32 sums
+// are added in order.  The result is that of threads t < 64, for column 64
+// block + t.
+template <typename X>
+__device__ __forceinline__ float column_sum(const X* __restrict__ x, int64_t r0, int64_t r1, int H, int block,
                                             float* s) {
   const int c = threadIdx.x & 7, r = threadIdx.x >> 3;
   const int col = block * 64 + 8 * c;
@@ -313,10 +340,20 @@ __device__ __forceinline__ float column_sum(const uint16_t* __restrict__ x, int6
     for (int64_t i = r0 + r; i < r1; i += 32) {
       const u32x4_t u = ld16(x + i * H + col);
       const uint32_t w4[4] = {u.x, u.y, u.z, u.w};
+      if constexpr (sizeof(X) == 4) {
+        const u32x4_t u2 = ld16(x + i * H + col + 4);
+        const uint32_t w8[4] = {u2.x, u2.y, u2.z, u2.w};
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        v[2 * k] += bf16_bits_to_f32(w4[k] & 0xFFFFu);
-        v[2 * k + 1] += bf16_bits_to_f32(w4[k] >> 16);
+        for (int k = 0; k < 4; ++k) {
+          v[k] += __uint_as_float(w4[k]);
+          v[4 + k] += __uint_as_float(w8[k]);
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          v[2 * k] += bf16_bits_to_f32(w4[k] & 0xFFFFu);
+          v[2 * k + 1] += bf16_bits_to_f32(w4[k] >> 16);
+        }
       }
     }
   }
@@ -330,14 +367,15 @@ __device__ __forceinline__ float column_sum(const uint16_t* __restrict__ x, int6
   return t;
 }
 
-// Partial column sums of two bf16 matrices of many rows (the linears' bias
-// gradients): workgroup (x, y, z) has 64 columns of the y-th run of rows of
-// matrix z.  2 x 2049 rows of 2816: 6.0 us (3.8 TB/s).
-__global__ __launch_bounds__(256) void k_column_sum(const uint16_t* __restrict__ x0, const uint16_t* __restrict__ x1,
+// Partial column sums of two matrices of many rows (the linears' bias gradients:
+// dr's, which is there in fp32, and those of dz as the products take it): workgroup (x, y, z) has 64 columns of the y-th run of rows of
+// matrix z.  2 x 2049 rows of 2816: 7.6 us (4.6 TB/s).
+__global__ __launch_bounds__(256) void k_column_sum(const float* __restrict__ x0, const uint16_t* __restrict__ x1,
                                                     int64_t M, int H, int64_t rows, float* __restrict__ part) {
   __shared__ float s[32 * kSumPitch];
   const int64_t r0 = (int64_t)blockIdx.y * rows;
-  const float t = column_sum(blockIdx.z == 0 ? x0 : x1, r0, min(M, r0 + rows), H, blockIdx.x, s);
+  const int64_t r1 = min(M, r0 + rows);
+  const float t = blockIdx.z == 0 ? column_sum(x0, r0, r1, H, blockIdx.x, s) : column_sum(x1, r0, r1, H, blockIdx.x, s);
   const int o = blockIdx.x * 64 + (int)threadIdx.x;
   if (threadIdx.x < 64 && o < H) part[((int64_t)blockIdx.y * 2 + blockIdx.z) * H + o] = t;
 }
@@ -346,7 +384,7 @@ __global__ __launch_bounds__(256) void k_column_sum(const uint16_t* __restrict__
 // whose halves, rounded to T, are two gradients (null: not wanted).  A
 // workgroup has 32 columns, eight threads a column, each the partials i,
 // i + 8, ...; the eight sums are added in order.  A segment with x0 has no
-// partials: its gradients are the sums of two bf16 matrices of nb rows (32 rows
+// partials: its gradients are the sums of two matrices of nb rows (32 rows
 // of 2816: 4 us less than with a launch of their own).
 template <typename T>
 __global__ __launch_bounds__(256) void k_column_join(LnJoin a) {
@@ -355,7 +393,7 @@ __global__ __launch_bounds__(256) void k_column_join(LnJoin a) {
   if (std::is_same_v<T, __bf16> && g.x0 != nullptr) {
     const int blocks = (a.H + 63) / 64, z = (int)blockIdx.x >= blocks, block = blockIdx.x - z * blocks;
     if (block >= blocks) return;
-    const float t = column_sum(z ? g.x1 : g.x0, 0, g.nb, a.H, block, s);
+    const float t = z ? column_sum(g.x1, 0, g.nb, a.H, block, s) : column_sum(g.x0, 0, g.nb, a.H, block, s);
     const int o = block * 64 + (int)threadIdx.x;
     if (threadIdx.x < 64 && o < a.H) static_cast<T*>(z ? g.out1 : g.out0)[o] = (T)t;
     return;
@@ -378,10 +416,14 @@ __global__ __launch_bounds__(256) void k_column_join(LnJoin a) {
 
 namespace {
 
+// the rows that HybridLink's forms take
+template <typename T, int VEC>
+constexpr bool kLnLink = std::is_same_v<T, __bf16> && VEC > 1;
+
 inline bool ln_vector(const LnArgs& a, int size) {
   const int vec = 16 / size;
   if (a.H % vec != 0) return false;
-  const void* p[] = {a.x, a.w, a.b, a.y, a.dy, a.add};
+  const void* p[] = {a.x, a.w, a.b, a.y, a.dy};
   for (const void* q : p)
     if (reinterpret_cast<uintptr_t>(q) & 15u) return false;
   return true;
@@ -404,7 +446,17 @@ hipError_t ln_forward(const LnArgs& a, hipStream_t s) {
   const int ept = (a.H + per * VEC - 1) / (per * VEC) * VEC;
   const int64_t groups = wave ? (a.M + 3) / 4 : a.M;
   const dim3 grid((unsigned)std::min<int64_t>(groups, kLnMaxGrid));
-#define W4A16_LN(EPT_, TPR_) hipLaunchKernelGGL((k_ln_forward<T, VEC, EPT_, TPR_>), grid, dim3(ln_threads(TPR_)), 0, s, a)
+#define W4A16_LN1(EPT_, TPR_, FORM_) \
+  hipLaunchKernelGGL((k_ln_forward<T, VEC, EPT_, TPR_, FORM_>), grid, dim3(ln_threads(TPR_)), 0, s, a)
+#define W4A16_LN(EPT_, TPR_)                                                           \
+  do {                                                                                 \
+    if (a.form == kLnPost) {                                                           \
+      if constexpr (kLnLink<T, VEC>) W4A16_LN1(EPT_, TPR_, kLnPost);                    \
+      else return hipErrorInvalidValue;                                                \
+    } else {                                                                           \
+      W4A16_LN1(EPT_, TPR_, kLnRows);                                                  \
+    }                                                                                  \
+  } while (0)
   if (per == 64) {
     if (ept <= 16) W4A16_LN(16, 64);
     else if (ept <= 32) W4A16_LN(32, 64);
@@ -415,6 +467,7 @@ hipError_t ln_forward(const LnArgs& a, hipStream_t s) {
     else W4A16_LN(32, 256);
   }
 #undef W4A16_LN
+#undef W4A16_LN1
   return hipGetLastError();
 }
 
@@ -428,18 +481,18 @@ hipError_t ln_backward(const LnArgs& a, hipStream_t s) {
     const int per = wave ? 64 : 256;
     const int ept = (a.H + per * VEC - 1) / (per * VEC) * VEC;
     const int nb = ln_partials(a.M);
-#define W4A16_LN1(EPT_, TPR_, ADD_)                                                                             \
-  hipLaunchKernelGGL((k_ln_backward<T, VEC, EPT_, TPR_, ADD_>), dim3(nb), dim3(ln_back_threads(TPR_)),            \
+#define W4A16_LN1(EPT_, TPR_, FORM_)                                                                            \
+  hipLaunchKernelGGL((k_ln_backward<T, VEC, EPT_, TPR_, FORM_>), dim3(nb), dim3(ln_back_threads(TPR_)),           \
                      TPR_ == 64 ? 4 * 2 * EPT_ * 64 * 4 : 2 * 4 * 4, s, a)
-#define W4A16_LN(EPT_, TPR_)                                                  \
-  do {                                                                        \
-    if (a.add != nullptr) {                                                   \
-      /* (HybridLink's rows alone, whose H and pointers allow vectors) */       \
-      if constexpr (std::is_same<T, __bf16>::value && VEC > 1) W4A16_LN1(EPT_, TPR_, true); \
-      else return hipErrorInvalidValue;                                       \
-    } else {                                                                  \
-      W4A16_LN1(EPT_, TPR_, false);                                           \
-    }                                                                         \
+#define W4A16_LN(EPT_, TPR_)                                                           \
+  do {                                                                                 \
+    if (a.form != kLnRows) {                                                           \
+      if constexpr (!kLnLink<T, VEC>) return hipErrorInvalidValue;                     \
+      else if (a.form == kLnPost) W4A16_LN1(EPT_, TPR_, kLnPost);                       \
+      else W4A16_LN1(EPT_, TPR_, kLnPre);                                              \
+    } else {                                                                           \
+      W4A16_LN1(EPT_, TPR_, kLnRows);                                                  \
+    }                                                                                  \
   } while (0)
     if (per == 64) {
       if (ept <= 16) W4A16_LN(16, 64);
@@ -501,7 +554,7 @@ int column_sum_partials(int64_t M) {
   return M <= kColSumRows ? 0 : (int)std::min<int64_t>((M + kColSumRows - 1) / kColSumRows, kColSumPartials);
 }
 
-hipError_t launch_column_sums(const uint16_t* x0, const uint16_t* x1, int64_t M, int H, float* part, hipStream_t s) {
+hipError_t launch_column_sums(const float* x0, const uint16_t* x1, int64_t M, int H, float* part, hipStream_t s) {
   const int n = column_sum_partials(M);
   if (H <= 0 || H % 8 != 0 || n <= 0) return hipErrorInvalidValue;
   hipLaunchKernelGGL(k_column_sum, dim3((H + 63) / 64, n, 2), dim3(256), 0, s, x0, x1, M, H, (M + n - 1) / n, part);

@@ -338,15 +338,24 @@ bool gemm_bf16_supported(int64_t K, int64_t cols);
 // max_items: grouped, most m-tiles
 hipError_t launch_gemm_bf16(int epi, GemmBf16Args a, int max_items, hipStream_t s);
 // Layer norm (kernels_layer_norm.hip); dtype: 0 bf16, 1 fp16, 2 fp32
+// Tensors in fp32 beside bf16 ones, of HybridLink's norms
+enum LnForm {
+  kLnRows = 0,  // all of one type
+  kLnPost = 1,  // x fp32; backward: dx in fp32 too (y32)
+  kLnPre = 2    // backward: dy and add fp32
+};
 struct LnArgs {
   const void *x, *w, *b;    // b nullable
   void* y;                  // backward: dx
+  float* y32;               // kLnPost's backward: dx
   float *mean, *rstd;       // forward: nullable together
-  const void *dy, *add;     // backward; add nullable, [M, H]: added to dx
+  const void* dy;           // backward
+  const float* add;         // kLnPre's backward: [M, H], added to dx
   float* part;              // backward: ln_partials(M) * 2 H floats
   int64_t M;
   int H;
   float eps;
+  int form;                 // not kLnRows: bf16, H a multiple of 8, 16-byte aligned pointers
 };
 constexpr int kLnMaxH = 8192;
 constexpr int kLnPartials = 256;   // one workgroup per CU
@@ -364,27 +373,29 @@ struct LnJoin {
     const float* part;
     int nb;
     void *out0, *out1;
-    const uint16_t *x0, *x1;  // bf16 rows to sum in place of partials (nb of them, H wide; bf16 only)
+    const float* x0;     // rows to sum in place of partials (nb of them, H wide; outputs bf16)
+    const uint16_t* x1;
   } seg[3];
   int n, H;
 };
 hipError_t launch_column_join(int dtype, const LnJoin& a, hipStream_t s);
-// The column sums of two bf16 matrices of M rows as column_sum_partials(M)
+// The column sums of two matrices of M rows as column_sum_partials(M)
 // partial rows of 2 H floats, for launch_column_join; up to kColSumRows rows
 // there are none: the join sums them itself
 constexpr int kColSumPartials = 128;
 constexpr int64_t kColSumRows = 512;
 int column_sum_partials(int64_t M);
-hipError_t launch_column_sums(const uint16_t* x0, const uint16_t* x1, int64_t M, int H, float* part, hipStream_t s);
+hipError_t launch_column_sums(const float* x0, const uint16_t* x1, int64_t M, int H, float* part, hipStream_t s);
 // Dense bf16 GEMMs of the training forms (gemm_dense.hpp).
 enum DenseLayout { kDgNT = 0, kDgNN = 1, kDgTN = 2 };
 enum DenseEpilogue {
   kDgPlain = 0,        // out = C
   kDgGateUp = 1,       // NT, B gate rows, B2 up rows: out = gelu_tanh(C) C2; sum, sum2 (nullable) = C, C2
   kDgGateUpBack = 2,   // NN, sum = a, sum2 = b: out = C b gelu_tanh'(a), out2 = C gelu_tanh(a)
-  kDgBiasGelu = 3,     // NT: out2 = z = C + bias, out = gelu_erf(z)
-  kDgBiasResidual = 4, // NT: out = in + C + bias
-  kDgGeluBack = 5      // NN: out = C gelu_erf'(in)
+  kDgBiasGelu = 3,     // NT: sum = z = C + bias, out = gelu_erf(z)
+  kDgBiasResidual = 4, // NT: sum = in + C + bias
+  kDgGeluBack = 5,     // NN: out = C gelu_erf'(sum)
+  kDgSums = 6          // NN: sum = C
 };
 struct DgEpilogue {
   uint16_t *out, *out2;

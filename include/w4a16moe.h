@@ -430,9 +430,10 @@ W4A16_API int w4a16_gated_mlp_backward(const uint16_t* dy, const uint16_t* x, co
  * w4a16_hybridlink):
  *   a = LN(h; ln1), z = a p1_w^T + p1_b, g = gelu_erf(z),
  *   r = h + (g p2_w^T + p2_b), out = LN(r; ln2)
- * a, z, g, r and out are rounded to bf16 once each, from fp32
- * (w4a16_hybridlink rounds where the torch modules do, so the two differ by
- * roundings).  `saved`: w4a16_hybridlink_saved_bytes(B, H) bytes that the
+ * a, g and out are rounded to bf16 once each, from fp32, and z and r stay in
+ * fp32 (w4a16_hybridlink rounds where the torch modules do, so the two differ
+ * by roundings); in the backward pass dr and dz are rounded as operands of the
+ * products alone.  `saved`: w4a16_hybridlink_saved_bytes(B, H) bytes that the
  * forward fills and the backward of the same B, H reads.  The backward gives
  * dh and the gradients of the eight parameters.  H a multiple of 32, at most
  * 8192; every pointer 16-byte aligned.                                      */
