@@ -221,7 +221,7 @@ __global__ __launch_bounds__(ln_back_threads(TPR)) void k_ln_backward(LnArgs a) 
   constexpr int RPB = ln_back_threads(TPR) / TPR;
   extern __shared__ __align__(16) float smem[];  // TPR > 64: a row's sums; else column sums, [4][2][EPT][64]
   const int t = threadIdx.x % TPR;
-  const int H = a.H;
+  const int H = a.H, nchunks = H / VEC;
   const float fh = (float)H;
   Raw w;
   w.load(a.w, t, H);
@@ -239,16 +239,18 @@ __global__ __launch_bounds__(ln_back_threads(TPR)) void k_ln_backward(LnArgs a) 
     const float mean = a.mean[row], rstd = a.rstd[row];
     float s[2] = {0.f, 0.f};  // sum g, sum g xh
 #pragma unroll
-    for (int q = 0; q < Raw::NQ; ++q)
+    for (int q = 0; q < Raw::NQ; ++q) {
+      // past the row dy and x are zero; xh too, where -mean rstd may overflow
+      const float r = t + TPR * q < nchunks ? rstd : 0.f;
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        // elements past the row: dy is zero there
-        const float xh = (x.get(q, e) - mean) * rstd, d = dy.get(q, e), g = d * w.get(q, e);
+        const float xh = (x.get(q, e) - mean) * r, d = dy.get(q, e), g = d * w.get(q, e);
         s[0] += g;
         s[1] = __builtin_fmaf(g, xh, s[1]);
         dw[q * VEC + e] = __builtin_fmaf(d, xh, dw[q * VEC + e]);
         db[q * VEC + e] += d;
       }
+    }
     ln_sum<TPR>(s, smem);
     const float m0 = s[0] / fh, m1 = s[1] / fh;
     x.forget();
@@ -368,8 +370,8 @@ __device__ __forceinline__ float column_sum(const X* __restrict__ x, int64_t r0,
 }
 
 // Partial column sums of two matrices of many rows (the linears' bias gradients:
-// dr's, which is there in fp32, and those of dz as the products take it): workgroup (x, y, z) has 64 columns of the y-th run of rows of
-// matrix z.  2 x 2049 rows of 2816: 7.6 us (4.6 TB/s).
+// dr's, which is there in fp32, and those of dz as the products take it):
+// workgroup (x, y, z) has 64 columns of the y-th run of rows of matrix z.  2 x 2049 rows of 2816: 7.6 us (4.6 TB/s).
 __global__ __launch_bounds__(256) void k_column_sum(const float* __restrict__ x0, const uint16_t* __restrict__ x1,
                                                     int64_t M, int H, int64_t rows, float* __restrict__ part) {
   __shared__ float s[32 * kSumPitch];
