@@ -10,7 +10,7 @@ these are the same maps with hand-written backward passes:
   the module with the reference's parameter names
 
 Each is one pair of library calls (``_lib.layer_norm`` and
-``_lib.layer_norm_backward``, ...), differentiable once.  Code that captures
+``_lib.layer_norm_backward``, ...), differentiable once, in reverse mode.  Code that captures
 a training step into a graph calls those pairs itself: the functions here
 refuse to record a backward pass while the stream is capturing, because a
 gradient accumulated on another stream's graph would end the capture.
@@ -19,13 +19,18 @@ from __future__ import annotations
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
 
 
 def _wants_grad(*tensors) -> bool:
-    """Whether the call records a backward pass; refuses where it cannot."""
+    """Whether the call records a backward pass; refuses where it cannot, and forward-mode
+    derivatives, which a library call would drop (a level of them is open for any to be there)."""
+    if getattr(forward_ad, "_current_level", 0) >= 0 and any(
+            t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError("forward-mode derivatives are not supported: the gradients here are reverse-mode only")
     if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in tensors):
         return False
     if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
