@@ -109,9 +109,24 @@ def hybridlink(h: torch.Tensor, ln1_w: torch.Tensor, ln1_b: torch.Tensor, p1_w: 
     return _lib.hybridlink(h, *params, eps)
 
 
+def _check_submodule(m: nn.Module, name: str, kind: type) -> None:
+    """Only m's parameters are read: refuse what its own call would do besides."""
+    if not isinstance(m, kind) or type(m).forward is not kind.forward or "forward" in m.__dict__:
+        raise ValueError(f"{name} must be an nn.{kind.__name__} with its own forward, got {type(m).__name__}: "
+                         "HybridLink reads its weight and bias and does not call it")
+    if m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks:
+        raise ValueError(f"{name} has hooks, which would not run: HybridLink reads its weight and bias and does "
+                         "not call it")
+    if m.weight is None or m.bias is None:
+        raise ValueError(f"{name} must have a weight and a bias")
+
+
 class HybridLink(nn.Module):
     """R(h) = post_ln(h + proj2(GELU(proj1(pre_ln(h))))) with the reference module's parameter names
-    (hybridlink.py:17-28), so its state dict loads as it is."""
+    (hybridlink.py:17-28), so its state dict loads as it is.
+
+    The submodules hold the parameters and are not called: adapters in their place, hooks on them
+    and two norms of different eps are refused (a parametrization of a weight or bias works)."""
 
     def __init__(self, hidden_size: int, eps: float = 1e-5, dtype: torch.dtype = torch.bfloat16,
                  device: torch.device | str | None = None) -> None:
@@ -123,5 +138,10 @@ class HybridLink(nn.Module):
         self.post_ln = nn.LayerNorm(hidden_size, eps=eps, **kw)
 
     def forward(self, h: torch.Tensor) -> torch.Tensor:
+        for name, kind in (("pre_ln", nn.LayerNorm), ("proj1", nn.Linear), ("proj2", nn.Linear),
+                           ("post_ln", nn.LayerNorm)):
+            _check_submodule(getattr(self, name), name, kind)
+        if self.pre_ln.eps != self.post_ln.eps:
+            raise ValueError(f"pre_ln and post_ln must have one eps, got {self.pre_ln.eps} and {self.post_ln.eps}")
         return hybridlink(h, self.pre_ln.weight, self.pre_ln.bias, self.proj1.weight, self.proj1.bias,
                           self.proj2.weight, self.proj2.bias, self.post_ln.weight, self.post_ln.bias, self.pre_ln.eps)

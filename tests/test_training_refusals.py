@@ -2,6 +2,7 @@
 import pytest
 import torch
 import torch.nn.functional as F
+import torch.nn.utils.parametrize
 from torch.autograd import forward_ad
 
 from hybridagent_amd import _lib, training
@@ -49,3 +50,87 @@ def test_forward_mode_derivatives(calls, name):
                 f(*dual)
     assert calls == [name]
     assert f(*args).shape == args[0].shape
+
+
+# ---------------------------------------------------------------- the module reads its submodules' parameters
+
+
+def _link():
+    torch.manual_seed(2)
+    return training.HybridLink(H, dtype=torch.float32)
+
+
+class _Adapter(torch.nn.Linear):
+    def forward(self, x):
+        return 2 * super().forward(x)
+
+
+class _Wrapper(torch.nn.Module):
+    def __init__(self, m):
+        super().__init__()
+        self.weight, self.bias = m.weight, m.bias
+
+
+HOOKS = {"forward": lambda m: m.register_forward_hook(lambda *a: None),
+         "forward_pre": lambda m: m.register_forward_pre_hook(lambda *a: None),
+         "full_backward": lambda m: m.register_full_backward_hook(lambda *a: None),
+         "full_backward_pre": lambda m: m.register_full_backward_pre_hook(lambda *a: None)}
+
+
+@pytest.mark.parametrize("name", ["pre_ln", "proj1", "proj2", "post_ln"])
+@pytest.mark.parametrize("hook", HOOKS)
+def test_hooks_on_submodules_are_refused(calls, name, hook):
+    link = _link()
+    handle = HOOKS[hook](getattr(link, name))
+    with torch.no_grad():
+        with pytest.raises(ValueError, match=f"{name} has hooks"):
+            link(torch.zeros(3, H))
+        handle.remove()
+        link(torch.zeros(3, H))
+    assert calls == ["hybridlink"]
+
+
+@pytest.mark.parametrize("name", ["pre_ln", "proj1", "proj2", "post_ln"])
+def test_other_submodules_are_refused(calls, name):
+    for swap in (lambda m: _Adapter(H, H), _Wrapper, lambda m: torch.nn.Identity()):
+        link = _link()
+        setattr(link, name, swap(getattr(link, name)))
+        with pytest.raises(ValueError, match=f"{name} must be"):
+            link(torch.zeros(3, H))
+    link = _link()
+    getattr(link, name).forward = lambda x: x
+    with pytest.raises(ValueError, match=f"{name} must be"):
+        link(torch.zeros(3, H))
+    link = _link()
+    getattr(link, name).bias = None
+    with pytest.raises(ValueError, match="a weight and a bias"):
+        link(torch.zeros(3, H))
+    assert not calls
+
+
+def test_one_eps(calls):
+    link = _link()
+    link.post_ln.eps = 1e-6
+    with pytest.raises(ValueError, match="one eps"):
+        link(torch.zeros(3, H))
+    link.pre_ln.eps = 1e-6
+    with torch.no_grad():
+        link(torch.zeros(3, H))
+    assert calls == ["hybridlink"]
+
+
+def test_parametrized_weights_are_read(monkeypatch):
+    """A parametrization is part of the weight that is read, and the module itself may have hooks."""
+    class Twice(torch.nn.Module):
+        def forward(self, w):
+            return 2 * w
+
+    link = _link()
+    w = link.proj1.weight.detach().clone()
+    torch.nn.utils.parametrize.register_parametrization(link.proj1, "weight", Twice())
+    seen = []
+    monkeypatch.setattr(_lib, "hybridlink", lambda h, *p: seen.append(p[2]) or h)
+    link.register_forward_hook(lambda *a: seen.append("hook"))
+    with torch.no_grad():
+        link(torch.zeros(3, H))
+    assert torch.equal(seen[0], 2 * w) and seen[1] == "hook"
