@@ -829,6 +829,12 @@ def _rows_like(t: torch.Tensor, name: str, like: torch.Tensor) -> torch.Tensor:
     return _rows(t.contiguous(), t.shape[-1])
 
 
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """t at a multiple of 16 bytes.  A caller places its own tensors so; where autograd puts a
+    gradient (a slice of a concatenation's, say) it has no say in."""
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def _saved(t: torch.Tensor, nbytes: int) -> torch.Tensor:
     if t.dtype != torch.uint8 or t.dim() != 1 or not t.is_contiguous() or t.numel() != nbytes:
         raise ValueError(f"saved must be the uint8 [{nbytes}] that the forward call of this shape returned")
@@ -941,7 +947,7 @@ def gated_mlp_backward(dy: torch.Tensor, x: torch.Tensor, gate_w: torch.Tensor, 
     dev = _require_gpu(dy, x, gate_w, up_w, down_w, saved)
     x = _bf16(x, "x")
     gate_w, up_w, down_w, H, I = _mlp_weights(x, gate_w, up_w, down_w)
-    dy2 = _rows_like(dy, "dy", x)
+    dy2 = _aligned(_rows_like(dy, "dy", x))
     x2 = _rows(x, H)
     M = x2.shape[0]
     lib = load()
@@ -1003,7 +1009,7 @@ def hybridlink_backward(dout: torch.Tensor, h: torch.Tensor, ln1_w: torch.Tensor
     dev = _require_gpu(dout, h, ln1_w, ln1_b, p1_w, p1_b, p2_w, p2_b, ln2_w, ln2_b, saved)
     h = _bf16(h, "h")
     params, H = _link_params(h, (ln1_w, ln1_b, p1_w, p1_b, p2_w, p2_b, ln2_w, ln2_b))
-    d2 = _rows_like(dout, "dout", h)
+    d2 = _aligned(_rows_like(dout, "dout", h))
     h2 = _rows(h, H)
     B = h2.shape[0]
     lib = load()
