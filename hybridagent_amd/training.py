@@ -12,8 +12,10 @@ these are the same maps with hand-written backward passes:
 Each is one pair of library calls (``_lib.layer_norm`` and
 ``_lib.layer_norm_backward``, ...), differentiable once, in reverse mode.  Code that captures
 a training step into a graph calls those pairs itself: the functions here
-refuse to record a backward pass while the stream is capturing, because a
-gradient accumulated on another stream's graph would end the capture.
+refuse to record a backward pass while the stream is capturing, and to run a
+recorded one there.  Autograd adds up a leaf's gradients on the stream of the
+first graph that used it; with such a graph alive, a backward pass captured on
+another stream ends the process.
 """
 from __future__ import annotations
 
@@ -33,10 +35,14 @@ def _wants_grad(*tensors) -> bool:
         raise RuntimeError("forward-mode derivatives are not supported: the gradients here are reverse-mode only")
     if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in tensors):
         return False
+    _refuse_capture()
+    return True
+
+
+def _refuse_capture() -> None:
     if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
         raise RuntimeError("a differentiable call cannot be captured into a graph: call the forward and backward "
                            "functions of hybridagent_amd._lib in the captured code instead")
-    return True
 
 
 class _LayerNorm(torch.autograd.Function):
@@ -50,6 +56,7 @@ class _LayerNorm(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
+        _refuse_capture()
         x, weight, mean, rstd = ctx.saved_tensors
         dx, dw, db = _lib.layer_norm_backward(dy, x, weight, mean, rstd, bias=ctx.bias)
         return dx, dw, db, None
@@ -73,6 +80,7 @@ class _GatedMLP(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
+        _refuse_capture()
         return _lib.gated_mlp_backward(dy, *ctx.saved_tensors, needs=ctx.needs_input_grad)
 
 
@@ -93,6 +101,7 @@ class _HybridLink(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
+        _refuse_capture()
         h, *params, saved = ctx.saved_tensors
         dh, *grads = _lib.hybridlink_backward(dout, h, *params, saved)
         return (dh, None, *grads)

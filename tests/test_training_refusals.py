@@ -134,3 +134,42 @@ def test_parametrized_weights_are_read(monkeypatch):
     with torch.no_grad():
         link(torch.zeros(3, H))
     assert torch.equal(seen[0], 2 * w) and seen[1] == "hook"
+
+
+# ---------------------------------------------------------------- captured graphs
+
+
+@pytest.mark.parametrize("name", ["layer_norm", "gated_mlp", "hybridlink"])
+def test_no_pass_of_a_recorded_step_is_captured(monkeypatch, name):
+    """While the stream is capturing, neither a forward pass that records nor a recorded backward pass
+    reaches the library; outside a capture both do."""
+    args = [t.requires_grad_() for t in _tensors()[name]]
+    reached = []
+    forward, backward = {"layer_norm": ("layer_norm", "layer_norm_backward"),
+                         "gated_mlp": ("gated_mlp", "gated_mlp_backward"),
+                         "hybridlink": ("hybridlink_train", "hybridlink_backward")}[name]
+    kept = (torch.zeros(3), torch.zeros(3)) if name == "layer_norm" else (torch.zeros(1),)
+
+    def run_forward(x, *a, **kw):
+        reached.append("forward")
+        return (x.detach() * 1, *kept)
+
+    def run_backward(*a, **kw):
+        reached.append("backward")
+        return tuple(torch.zeros_like(t) for t in args)
+
+    monkeypatch.setattr(_lib, forward, run_forward)
+    monkeypatch.setattr(_lib, backward, run_backward)
+    capturing = [False]
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+    y = getattr(training, name)(*args)
+    capturing[0] = True
+    with pytest.raises(RuntimeError, match="cannot be captured"):
+        y.sum().backward(retain_graph=True)
+    with pytest.raises(RuntimeError, match="cannot be captured"):
+        getattr(training, name)(*args)
+    assert reached == ["forward"] and all(t.grad is None for t in args)
+    capturing[0] = False
+    y.sum().backward()
+    assert reached == ["forward", "backward"] and all(t.grad is not None for t in args)
