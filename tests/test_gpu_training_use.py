@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+import test_gpu_training as base
 from hybridagent_amd import _lib, training
 
 pytestmark = pytest.mark.gpu
@@ -53,3 +54,9 @@ def test_gradient_at_an_odd_address(dev, name, T):
             assert (e <= 2 * 2.0 ** -8 * q.double().abs() + 1e-4).all()
         else:
             assert torch.equal(p, q)
+
+
+# the tiles of the input's gradient that the shapes of the other tests leave out
+@pytest.mark.parametrize("T,H,I", [(1699, 1824, 32), (4105, 448, 32)])
+def test_gated_mlp_more_tiles(dev, T, H, I):
+    base.test_gated_mlp(dev, T, H, I)
