@@ -881,7 +881,8 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
                         rstd: torch.Tensor, bias: bool = True):
     """(dx, dweight, dbias) of ``layer_norm`` for the gradient ``dy`` of its output; ``mean`` and
     ``rstd`` are what the forward returned.  dbias is None where ``bias`` is False.  The sums
-    over the rows are taken in fp32 in an order set by the shape."""
+    over the rows are taken in fp32, in an order set by the shape, the type and the tensors'
+    alignment to 16 bytes."""
     dev = _require_gpu(dy, x, weight, mean, rstd)
     dt, H = _ln_params(x, weight, None)
     dy2 = _rows_like(dy, "dy", x)

@@ -19,8 +19,8 @@
 // forward 2.4.  The column sums of the backward pass are kept in registers
 // across the rows of a thread, added over a workgroup's wavefronts in LDS and
 // written once per workgroup (kLnPartials at most); a second launch
-// (k_column_join) adds those in order, so that a result depends on the shape
-// alone.
+// (k_column_join) adds those in order, so that a repeated call gives the same
+// bits (another alignment of the pointers takes other loads and another order).
 #include <algorithm>
 #include <type_traits>
 

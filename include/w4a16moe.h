@@ -377,8 +377,10 @@ W4A16_API int moe_ffn_block_routing_offsets(int64_t M, int64_t top_k, int64_t E,
  * backward needs, and the backward passes.  No kernel of the reference
  * matches them (it trains through torch's autograd); the maps are those of
  * the entry points above.  Gradients are sums in fp32, rounded once to the
- * tensor's type; every sum's order depends on the shapes alone, so a call
- * repeated on the same inputs gives the same bits.  Gradients of weights are
+ * tensor's type.  No sum's order changes from call to call: it depends on the
+ * shapes, the types, the pointers' alignment to 16 bytes, which gradients are
+ * asked for and the device's CU count, so a call repeated with the same of
+ * these on the same values gives the same bits.  Gradients of weights are
  * written, not accumulated, also for zero rows (as zeros).                  */
 
 /* The type of a tensor whose entry point takes several. */
