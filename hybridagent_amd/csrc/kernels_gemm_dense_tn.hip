@@ -29,10 +29,11 @@ hipError_t launch_gemm_dense(int layout, int epi, DgArgs a, hipStream_t s) {
     a.plane += (int64_t)p.M * p.N * (gu ? 2 : 1);
     sh[i] = DenseShape{p.M, gu ? 2 * (int64_t)p.N : p.N};
   }
-  const bool thin = a.mi == 0 && layout != kDgTN && a.nprob == 1 &&
-                    dense_thin(a.prob[0].M, a.prob[0].N, gu ? 16 : 32, device_cus());
-  if (thin) a.ksplit = 1;
-  if (a.mi == 0 && !thin) {
+  const bool thin =
+      layout != kDgTN && a.nprob == 1 && dense_thin(a.prob[0].M, a.prob[0].N, gu ? 16 : 32, device_cus());
+  a.mi = a.ni = 0;
+  a.kg = a.ksplit = 1;
+  if (!thin) {
     const DensePlan pl = dense_plan(sh, a.nprob, a.nk, a.part != nullptr ? dense_part_planes(a.plane) : 1, device_cus(),
                                     layout);
     a.mi = pl.mi;

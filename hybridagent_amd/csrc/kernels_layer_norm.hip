@@ -140,7 +140,7 @@ __device__ __forceinline__ void ln_sum(float (&v)[N], float* part) {
   }
 }
 
-constexpr int ln_threads(int tpr) { return 256; }
+constexpr int kLnThreads = 256;
 // backward: a wavefront's rows in workgroups of eight of them
 constexpr int ln_back_threads(int tpr) { return tpr > 64 ? tpr : 512; }
 // the thread's row of the workgroup's (wavefront-uniform)
@@ -152,11 +152,11 @@ __device__ __forceinline__ int ln_row_of() {
 }  // namespace
 
 template <typename T, int VEC, int EPT, int TPR, int FORM>
-__global__ __launch_bounds__(ln_threads(TPR)) void k_ln_forward(LnArgs a) {
+__global__ __launch_bounds__(kLnThreads) void k_ln_forward(LnArgs a) {
   using Raw = LnRaw<T, VEC, EPT, TPR>;
   using TX = std::conditional_t<FORM == kLnPost, float, T>;
   __shared__ float part[TPR > 64 ? TPR / 64 : 1];
-  constexpr int RPB = ln_threads(TPR) / TPR;  // rows per workgroup
+  constexpr int RPB = kLnThreads / TPR;  // rows per workgroup
   const int t = threadIdx.x % TPR;
   const int H = a.H, nchunks = H / VEC;
   const float fh = (float)H;
@@ -449,7 +449,7 @@ hipError_t ln_forward(const LnArgs& a, hipStream_t s) {
   const int64_t groups = wave ? (a.M + 3) / 4 : a.M;
   const dim3 grid((unsigned)std::min<int64_t>(groups, kLnMaxGrid));
 #define W4A16_LN1(EPT_, TPR_, FORM_) \
-  hipLaunchKernelGGL((k_ln_forward<T, VEC, EPT_, TPR_, FORM_>), grid, dim3(ln_threads(TPR_)), 0, s, a)
+  hipLaunchKernelGGL((k_ln_forward<T, VEC, EPT_, TPR_, FORM_>), grid, dim3(kLnThreads), 0, s, a)
 #define W4A16_LN(EPT_, TPR_)                                                           \
   do {                                                                                 \
     if (a.form == kLnPost) {                                                           \

@@ -407,7 +407,7 @@ struct DgProblem {
   int M, N;                         // of C, row-major, N a multiple of 8
   int lda, ldb;                     // elements between rows of the operands
   DgEpilogue e;
-  int tile0;                        // set by dense_gemm_args: first tile,
+  int tile0;                        // set by launch_gemm_dense: first tile,
   int64_t part0;                    // first element in a plane of partial sums
 };
 constexpr int kDgMaxProblems = 3;
@@ -415,13 +415,13 @@ struct DgArgs {
   DgProblem prob[kDgMaxProblems];
   int nprob;
   int K;        // of one pair; a multiple of 32 (TN: any)
-  int mi, ni, kg, ksplit;  // the plan
-  float* part;  // ksplit > 1: planes of partial sums
-  int64_t plane;
+  float* part;  // planes of partial sums, where ksplit > 1
+  int mi, ni, kg, ksplit;  // the plan, set by launch_gemm_dense (mi 0: the weights' stream),
+  int64_t plane;           // and elements of a plane
   int tiles, nk, nk1;
 };
 // a launch of up to three products of one layout and epilogue; a.part holds
-// dense_gemm_part_floats(plane) floats (null: no split)
+// dense_part_planes(plane) planes of all their sums (null: no split)
 hipError_t launch_gemm_dense(int layout, int epi, DgArgs a, hipStream_t s);
 // prefill grouped GEMM: one launch per stage, items = (m-tile, n-tile)
 hipError_t launch_prefill(int mode, PrefillArgs a, int max_mtiles, hipStream_t s);
