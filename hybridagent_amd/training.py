@@ -118,16 +118,18 @@ def hybridlink(h: torch.Tensor, ln1_w: torch.Tensor, ln1_b: torch.Tensor, p1_w: 
     return _lib.hybridlink(h, *params, eps)
 
 
-def _check_submodule(m: nn.Module, name: str, kind: type) -> None:
-    """Only m's parameters are read: refuse what its own call would do besides."""
+def _weight_and_bias(m: nn.Module | None, name: str, kind: type):
+    """m's parameters, all of m that is used: refuses what m's own call would do besides."""
     if not isinstance(m, kind) or type(m).forward is not kind.forward or "forward" in m.__dict__:
         raise ValueError(f"{name} must be an nn.{kind.__name__} with its own forward, got {type(m).__name__}: "
                          "HybridLink reads its weight and bias and does not call it")
     if m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks:
         raise ValueError(f"{name} has hooks, which would not run: HybridLink reads its weight and bias and does "
                          "not call it")
-    if m.weight is None or m.bias is None:
+    weight, bias = m.weight, m.bias
+    if weight is None or bias is None:
         raise ValueError(f"{name} must have a weight and a bias")
+    return weight, bias
 
 
 class HybridLink(nn.Module):
@@ -147,10 +149,12 @@ class HybridLink(nn.Module):
         self.post_ln = nn.LayerNorm(hidden_size, eps=eps, **kw)
 
     def forward(self, h: torch.Tensor) -> torch.Tensor:
-        for name, kind in (("pre_ln", nn.LayerNorm), ("proj1", nn.Linear), ("proj2", nn.Linear),
-                           ("post_ln", nn.LayerNorm)):
-            _check_submodule(getattr(self, name), name, kind)
-        if self.pre_ln.eps != self.post_ln.eps:
-            raise ValueError(f"pre_ln and post_ln must have one eps, got {self.pre_ln.eps} and {self.post_ln.eps}")
-        return hybridlink(h, self.pre_ln.weight, self.pre_ln.bias, self.proj1.weight, self.proj1.bias,
-                          self.proj2.weight, self.proj2.bias, self.post_ln.weight, self.post_ln.bias, self.pre_ln.eps)
+        mods = self._modules
+        pre_ln, post_ln = mods["pre_ln"], mods["post_ln"]
+        params = (*_weight_and_bias(pre_ln, "pre_ln", nn.LayerNorm),
+                  *_weight_and_bias(mods["proj1"], "proj1", nn.Linear),
+                  *_weight_and_bias(mods["proj2"], "proj2", nn.Linear),
+                  *_weight_and_bias(post_ln, "post_ln", nn.LayerNorm))
+        if pre_ln.eps != post_ln.eps:
+            raise ValueError(f"pre_ln and post_ln must have one eps, got {pre_ln.eps} and {post_ln.eps}")
+        return hybridlink(h, *params, pre_ln.eps)
