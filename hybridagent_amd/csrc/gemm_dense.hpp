@@ -29,8 +29,11 @@
 //
 // Bound: many rows: the matrix units at the clock that the card holds under
 // them (2816 -> 4224 of 8192 rows 162 us, 1200 TFLOP/s; dy W 2816 -> 2112 85 us,
-// 1150; dy^T x 2112 x 2816 of 8192 rows 101 us, 960); hundreds: what the CUs
-// take from the L2 (2816 -> 2816 of 1024 rows 23.9 us, 680).  The tile and the
+// 1150; dy^T x 2112 x 2816 of 8192 rows 101 us, 960); hundreds (2816 -> 2816 of
+// 1024 rows 23.9 us, 680): no unit by itself.  With a wavefront or two per SIMD,
+// LDS reads, loads and MFMAs overlap in part (of the CUs' cycles in 193 .. 2049 rows
+// the matrix units have 0.19 .. 0.47, LDS reads 0.17 .. 0.27, the wavefronts wait
+// in 0.14 .. 0.42), and 132 .. 198 workgroups leave CUs idle.  The tile and the
 // split are dense_plan's (rules.hpp).
 //
 // LDS formats of a slot's operand tile, both free of bank conflicts:

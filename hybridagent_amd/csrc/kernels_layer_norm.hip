@@ -14,9 +14,11 @@
 // rows and pointers allow it (VEC elements), else one element.  The weights
 // are loaded once per thread and kept across its rows.
 //
-// Bound: HBM; bf16 rows of 2816: 8192 forward 15.7 us (5.9 TB/s, part of it from
-// the 256 MB cache), 4099 backward 17.9 (3.9 TB/s) and the join 4.0; one row
-// forward 2.4.  The column sums of the backward pass are kept in registers
+// Bound: forward HBM: 8192 bf16 rows of 2816 15.7 us (5.9 TB/s, part of it from
+// the 256 MB cache); one row 2.4.  Backward, the same rows: 2049 13.2 us, 4099
+// 18.1 and the join 4.0: a further row comes at the memory's rate, some 9 us do
+// not depend on the rows (the first one's latency, the join of a workgroup's
+// wavefronts, the partial rows).  The column sums of the backward pass are kept in registers
 // across the rows of a thread, added over a workgroup's wavefronts in LDS and
 // written once per workgroup (kLnPartials at most); a second launch
 // (k_column_join) adds those in order, so that a repeated call gives the same
@@ -513,7 +515,9 @@ hipError_t ln_backward(const LnArgs& a, hipStream_t s) {
 }  // namespace
 
 int ln_partials(int64_t M) {
-  // a workgroup per row, or per eight rows at a time
+  // a workgroup per row, or per eight rows: the wavefront form's at a time, one
+  // after another in the workgroup form (rows wider than a wavefront keeps: 256
+  // / 257 / 1024 fp32 rows of 2816 6.1/11.2/13.2 us)
   return (int)(M <= kLnPartials ? M : std::min<int64_t>((M + 7) / 8, kLnPartials));
 }
 
