@@ -43,6 +43,7 @@ class TiledExpertsC(ctypes.Structure):
 # name -> (restype, argtypes); the exact set declared in include/w4a16moe.h
 _VP, _I64, _SZ, _F32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_size_t, ctypes.c_float
 _TP = ctypes.POINTER(TiledExpertsC)
+_HEADS = (_VP, _I64, _I64)  # [tokens, heads, D]: the pointer, elements between tokens and between heads
 SIGNATURES = {
     "w4a16moe_version": (ctypes.c_int, []),
     "w4a16moe_status_string": (ctypes.c_char_p, [ctypes.c_int]),
@@ -111,6 +112,21 @@ SIGNATURES = {
     "w4a16_hybridlink_backward_workspace_bytes": (_SZ, [_I64, _I64]),
     "w4a16_hybridlink_backward": (ctypes.c_int, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _SZ, _VP, _VP, _VP, _VP, _VP, _VP,
                                                  _VP, _VP, _VP, _I64, _I64, _VP, _SZ, _VP]),
+    "w4a16_head_norm_rope": (ctypes.c_int, [*_HEADS * 3, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, ctypes.c_int,
+                                            *[_I64] * 6, _F32, _VP]),
+    "w4a16_head_norm_rope_backward_workspace_bytes": (_SZ, [_I64] * 4),
+    "w4a16_head_norm_rope_backward": (ctypes.c_int, [_VP, _VP, _VP, *_HEADS * 3, *[_VP] * 10, ctypes.c_int,
+                                                     *[_I64] * 6, _F32, _VP, _SZ, _VP]),
+    "w4a16_append_kv": (ctypes.c_int, [*_HEADS * 3, *[_VP] * 8, _I64, _VP, _I64, ctypes.c_int, ctypes.c_int,
+                                       *[_I64] * 8, _F32, _VP]),
+    "w4a16_attention": (ctypes.c_int, [*_HEADS * 3, _VP, _VP, _VP, _VP, ctypes.c_int, *[_I64] * 6, _F32,
+                                       ctypes.c_int, _I64, _VP]),
+    "w4a16_attention_backward_workspace_bytes": (_SZ, [_I64, _I64]),
+    "w4a16_attention_backward": (ctypes.c_int, [_VP, *_HEADS * 3, *[_VP] * 7, ctypes.c_int, *[_I64] * 6, _F32,
+                                                ctypes.c_int, _I64, _VP, _SZ, _VP]),
+    "w4a16_decode_attention_workspace_bytes": (_SZ, [_I64] * 5),
+    "w4a16_decode_attention": (ctypes.c_int, [*_HEADS, _VP, _I64, _VP, _I64, _VP, _VP, _VP, ctypes.c_int,
+                                              *[_I64] * 7, _F32, _I64, _VP, _SZ, _VP]),
 }
 
 _lib = None
@@ -1024,6 +1040,264 @@ def hybridlink_backward(dout: torch.Tensor, h: torch.Tensor, ln1_w: torch.Tensor
           _ptr(params[2]), _ptr(params[4]), _ptr(params[6]), _ptr(saved), nsaved, _ptr(dh),
           *[_ptr(g) for g in grads], B, H, _ptr(ws), nbytes)
     return (_like(dh, h.shape), *grads)
+
+
+# ------------------------------------------------------------------ attention
+
+
+def _heads(t: torch.Tensor, name: str, like: torch.Tensor | None = None) -> torch.Tensor:
+    """t [tokens, heads, D] as the kernels take it: D contiguous, the other strides as they are where
+    every row starts at a multiple of 16 bytes, else a copy."""
+    if t.dim() != 3:
+        raise ValueError(f"{name} must be [tokens, heads, head size], got {list(t.shape)}")
+    if like is not None and (t.dtype != like.dtype or t.shape[0] != like.shape[0] or t.shape[2] != like.shape[2]):
+        raise ValueError(f"{name} must be {like.dtype} [{like.shape[0]}, heads, {like.shape[2]}], got {t.dtype} "
+                         f"{list(t.shape)}")
+    a, b, c = t.stride()
+    if c == 1 and t.data_ptr() % 16 == 0:
+        step = 16 // t.element_size()
+        if a % step == 0 and b % step == 0:
+            return t
+    return _aligned(t.contiguous())
+
+
+def _head_args(t: torch.Tensor | None):
+    return (None, 0, 0) if t is None else (t.data_ptr(), t.stride(0), t.stride(1))
+
+
+def _head_type(t: torch.Tensor, name: str, fp32: bool) -> int:
+    dt = _DTYPES.get(t.dtype)
+    if dt is None or (dt == 2 and not fp32):
+        raise ValueError(f"{name} must be bfloat16{', float16 or float32' if fp32 else ' or float16'}, got {t.dtype}")
+    return dt
+
+
+def _index(t: torch.Tensor, name: str, shape) -> torch.Tensor:
+    if t.dtype != torch.int32 or t.shape != shape:
+        raise ValueError(f"{name} must be int32 {list(shape)}, got {t.dtype} {list(t.shape)}")
+    return t.contiguous()
+
+
+def _rope_args(q, k, v, cos, sin, positions, q_weight, k_weight, fp32: bool):
+    """What the forms of the heads' norm check alike -> (device, type, the tensors, sizes)."""
+    dev = _require_gpu(q, k, v, cos, sin, positions, q_weight, k_weight)
+    dt = _head_type(q, "q", fp32)
+    q = _heads(q, "q")
+    k = _heads(k, "k", like=q)
+    if v is not None:
+        v = _heads(v, "v", like=q)
+        if v.shape != k.shape:
+            raise ValueError(f"v must have the shape of k, got {list(v.shape)} and {list(k.shape)}")
+    T, Hq, D = q.shape
+    P = R = 0
+    if (cos is None) != (sin is None):
+        raise ValueError("cos and sin are given together")
+    if cos is not None:
+        for t, n in ((cos, "cos"), (sin, "sin")):
+            if t.dtype != torch.float32 or t.dim() != 2 or t.shape != cos.shape:
+                raise ValueError(f"{n} must be float32 [positions, half the turned columns], got {t.dtype} "
+                                 f"{list(t.shape)}")
+        P, R = cos.shape[0], 2 * cos.shape[1]
+        cos, sin = _aligned(cos.contiguous()), _aligned(sin.contiguous())
+    positions = _index(positions, "positions", (T,))
+    if (q_weight is None) != (k_weight is None):
+        raise ValueError("q_weight and k_weight are given together")
+    if q_weight is not None:
+        for t, n in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+            if t.dtype != q.dtype or t.shape != (D,):
+                raise ValueError(f"{n} must be {q.dtype} [{D}], got {t.dtype} {list(t.shape)}")
+        q_weight, k_weight = _aligned(q_weight.contiguous()), _aligned(k_weight.contiguous())
+    return dev, dt, (q, k, v), (cos, sin, positions, q_weight, k_weight), (T, Hq, k.shape[1], D, P, R)
+
+
+def head_norm_rope(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor | None, cos: torch.Tensor | None,
+                   sin: torch.Tensor | None, positions: torch.Tensor, q_weight: torch.Tensor | None = None,
+                   k_weight: torch.Tensor | None = None, eps: float = 1e-6):
+    """RMS norm of every head and the position rotation in one pass -> (q, k, v), dense.
+
+    q [T, Hq, D], k, v [T, Hk, D] of bf16, fp16 or fp32, any strides; weights [D] (None, both: no
+    norm); cos, sin float32 [P, R / 2]: token t's columns i and i + R / 2 of q and k (i < R / 2) are
+    turned by row ``positions[t]`` (int32).  v (may be None) is normed without a weight.  A position
+    that the tables do not have makes its token's q and k NaN."""
+    dev, dt, (q, k, v), rot, sizes = _rope_args(q, k, v, cos, sin, positions, q_weight, k_weight, True)
+    out = tuple(None if t is None else torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
+    _call("w4a16_head_norm_rope", dev, load().w4a16_head_norm_rope, *_head_args(q), *_head_args(k), *_head_args(v),
+          *[_ptr(t) for t in rot], *[_ptr(t) for t in out], dt, *sizes, float(eps))
+    return out
+
+
+def head_norm_rope_backward(dq: torch.Tensor, dk: torch.Tensor, dv: torch.Tensor | None, q: torch.Tensor,
+                            k: torch.Tensor, v: torch.Tensor | None, cos: torch.Tensor | None,
+                            sin: torch.Tensor | None, positions: torch.Tensor, q_weight: torch.Tensor | None = None,
+                            k_weight: torch.Tensor | None = None, eps: float = 1e-6, weights: bool = True):
+    """(dq, dk, dv, dq_weight, dk_weight) of ``head_norm_rope`` for the gradients of its outputs.  The
+    weights' are None without weights and where ``weights`` is False; dv is None without v.  The sums
+    over the rows are taken in fp32, in an order set by the shapes."""
+    dev, dt, (q, k, v), rot, sizes = _rope_args(q, k, v, cos, sin, positions, q_weight, k_weight, True)
+    if (dv is None) != (v is None):
+        raise ValueError("dv is given with v")
+    grads = []
+    for t, x, n in ((dq, q, "dq"), (dk, k, "dk"), (dv, v, "dv")):
+        if t is not None and (t.shape != x.shape or t.dtype != x.dtype):
+            raise ValueError(f"{n} must be {x.dtype} {list(x.shape)}, got {t.dtype} {list(t.shape)}")
+        grads.append(None if t is None else _aligned(t.contiguous()))
+    _require_gpu(q, *grads)
+    out = [None if t is None else torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v)]
+    dw = [None, None]
+    nbytes, lib = 0, load()
+    if weights and q_weight is not None:
+        dw = [torch.empty_like(t) for t in rot[3:]]
+        nbytes = lib.w4a16_head_norm_rope_backward_workspace_bytes(*sizes[:4])
+    ws = _workspace(nbytes, dev)
+    _call("w4a16_head_norm_rope_backward", dev, lib.w4a16_head_norm_rope_backward, *[_ptr(t) for t in grads],
+          *_head_args(q), *_head_args(k), *_head_args(v), *[_ptr(t) for t in rot], *[_ptr(t) for t in out],
+          *[_ptr(t) for t in dw], dt, *sizes, float(eps), _ptr(ws), nbytes)
+    return (*out, *dw)
+
+
+def _cache(k_cache: torch.Tensor, v_cache: torch.Tensor, like: torch.Tensor):
+    """The sizes of a paged cache [pages, Hk, page size, D]; every page is dense."""
+    for t, n in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+        if t.dtype != like.dtype or t.dim() != 4 or t.shape != k_cache.shape or t.shape[3] != like.shape[2]:
+            raise ValueError(f"{n} must be {like.dtype} [pages, heads, page size, {like.shape[2]}], got {t.dtype} "
+                             f"{list(t.shape)}")
+        _, H, page, D = t.shape
+        if t.stride()[1:] != (page * D, D, 1) or t.data_ptr() % 16 or t.stride(0) % 8:
+            raise ValueError(f"{n} must have dense pages at multiples of 16 bytes, got strides {t.stride()}")
+    return k_cache.shape
+
+
+def append_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor | None, sin: torch.Tensor | None,
+              positions: torch.Tensor, slots: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+              q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, eps: float = 1e-6,
+              v_norm: bool = False) -> torch.Tensor:
+    """``head_norm_rope`` on the way into a paged cache -> q, dense; token t's keys and values (normed
+    without a weight where ``v_norm``) go to row ``slots[t]`` (int32; page x page size + row) of
+    k_cache, v_cache [pages, Hk, page size, D], bf16 or fp16.  A slot outside the cache (-1: a
+    padding token's) is not written; two tokens of a call must not share one."""
+    if v is None:
+        raise ValueError("v must be given")
+    dev, dt, (q, k, v), rot, sizes = _rope_args(q, k, v, cos, sin, positions, q_weight, k_weight, False)
+    _require_gpu(q, slots, k_cache, v_cache)
+    slots = _index(slots, "slots", (sizes[0],))
+    pages, H, page, _ = _cache(k_cache, v_cache, q)
+    if H != sizes[2]:
+        raise ValueError(f"the cache has {H} heads, k {sizes[2]}")
+    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    _call("w4a16_append_kv", dev, load().w4a16_append_kv, *_head_args(q), *_head_args(k), *_head_args(v),
+          _ptr(rot[0]), _ptr(rot[1]), _ptr(rot[2]), _ptr(slots), _ptr(rot[3]), _ptr(rot[4]), _ptr(out),
+          _ptr(k_cache), k_cache.stride(0), _ptr(v_cache), v_cache.stride(0), dt, int(v_norm), *sizes, pages, page,
+          float(eps))
+    return out
+
+
+def _attention_args(q, k, v, cu_q, cu_k, scale, causal, window):
+    dev = _require_gpu(q, k, v, cu_q, cu_k)
+    dt = _head_type(q, "q", False)
+    q = _heads(q, "q")
+    D = q.shape[2]
+    kv = []
+    for t, n in ((k, "k"), (v, "v")):
+        if t.dtype != q.dtype or t.dim() != 3 or t.shape[2] != D or t.shape != k.shape:
+            raise ValueError(f"{n} must be {q.dtype} [tokens, heads, {D}], got {t.dtype} {list(t.shape)}")
+        kv.append(_heads(t, n))
+    k, v = kv
+    if k.shape[1] == 0 or q.shape[1] % k.shape[1]:
+        raise ValueError(f"the query heads must be a multiple of the key-value heads, got {q.shape[1]} and "
+                         f"{k.shape[1]}")
+    if D not in (64, 128, 256, 512):
+        raise ValueError(f"the head size must be 64, 128, 256 or 512, got {D}")
+    if cu_q.dim() != 1 or cu_q.numel() == 0:
+        raise ValueError(f"cu_q must be int32 [sequences + 1], got {list(cu_q.shape)}")
+    cu_q = _index(cu_q, "cu_q", cu_q.shape)
+    if cu_k is None:
+        if k.shape[0] != q.shape[0]:
+            raise ValueError("without cu_k the queries and keys are of the same tokens")
+        cu_k = cu_q
+    cu_k = _index(cu_k, "cu_k", cu_q.shape)
+    if window and not causal:
+        raise ValueError("a window needs a causal mask")
+    sizes = (cu_q.numel() - 1, q.shape[0], k.shape[0], q.shape[1], k.shape[1], D,
+             float(D ** -0.5 if scale is None else scale), int(causal), int(window))
+    return dev, dt, (q, k, v), (cu_q, cu_k), sizes
+
+
+def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, cu_k: torch.Tensor | None = None,
+              scale: float | None = None, causal: bool = True, window: int = 0, return_lse: bool = False):
+    """Attention over packed sequences -> [Tq, Hq, D]; with ``return_lse`` also the scores' log sum of
+    exponentials, float32 [Hq, Tq], for ``attention_backward``.
+
+    q [Tq, Hq, D], k, v [Tk, Hk, D] of bf16 or fp16, any strides, D 64, 128, 256 or 512, Hq a
+    multiple of Hk.  Sequence b has the queries ``cu_q[b] .. cu_q[b + 1] - 1`` and the keys of
+    ``cu_k`` (int32, from 0 on; None: the same); its last query stands at its last key.  Causal: a
+    query sees the keys up to where it stands, with ``window`` the last so many of them.  A query
+    that sees none, and rows behind the last sequence, are zero.  ``scale`` is D^-1/2 if None."""
+    dev, dt, (q, k, v), cu, sizes = _attention_args(q, k, v, cu_q, cu_k, scale, causal, window)
+    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=dev) if return_lse else None
+    _call("w4a16_attention", dev, load().w4a16_attention, *_head_args(q), *_head_args(k), *_head_args(v),
+          *[_ptr(t) for t in cu], _ptr(out), _ptr(lse), dt, *sizes)
+    return (out, lse) if return_lse else out
+
+
+def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
+                       lse: torch.Tensor, cu_q: torch.Tensor, cu_k: torch.Tensor | None = None,
+                       scale: float | None = None, causal: bool = True, window: int = 0, needs=(True, True, True)):
+    """(dq, dk, dv) of ``attention`` for the gradient ``dout`` of its output and the ``out`` and ``lse`` of
+    that forward call.  ``needs``: which of the three are wanted; the others are None."""
+    dev, dt, (q, k, v), cu, sizes = _attention_args(q, k, v, cu_q, cu_k, scale, causal, window)
+    for t, n in ((dout, "dout"), (out, "out")):
+        if t.shape != q.shape or t.dtype != q.dtype:
+            raise ValueError(f"{n} must be {q.dtype} {list(q.shape)}, got {t.dtype} {list(t.shape)}")
+    if lse.shape != (q.shape[1], q.shape[0]) or lse.dtype != torch.float32:
+        raise ValueError(f"lse must be float32 {[q.shape[1], q.shape[0]]}, got {lse.dtype} {list(lse.shape)}")
+    _require_gpu(q, dout, out, lse)
+    if len(needs) != 3:
+        raise ValueError("needs must say for each of dq, dk and dv whether it is wanted")
+    dout, out, lse = _aligned(dout.contiguous()), _aligned(out.contiguous()), lse.contiguous()
+    dense = lambda t: torch.empty(t.shape, dtype=t.dtype, device=dev)
+    dq = dense(q) if needs[0] else None
+    dk, dv = (dense(k), dense(v)) if needs[1] or needs[2] else (None, None)
+    lib = load()
+    nbytes = lib.w4a16_attention_backward_workspace_bytes(q.shape[0], q.shape[1])
+    ws = _workspace(nbytes, dev)
+    _call("w4a16_attention_backward", dev, lib.w4a16_attention_backward, _ptr(dout), *_head_args(q), *_head_args(k),
+          *_head_args(v), _ptr(out), _ptr(lse), *[_ptr(t) for t in cu], _ptr(dq), _ptr(dk), _ptr(dv), dt, *sizes,
+          _ptr(ws), nbytes)
+    return dq, dk if needs[1] else None, dv if needs[2] else None
+
+
+def decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                     lengths: torch.Tensor, scale: float | None = None, window: int = 0) -> torch.Tensor:
+    """Attention of one new token per sequence over a paged cache -> [B, Hq, D].
+
+    q [B, Hq, D] of bf16 or fp16, any strides; k_cache, v_cache [pages, Hk, page size, D]; sequence
+    b's key j lies in row j % page size of page ``block_table[b, j / page size]``; it has
+    ``lengths[b]`` of them (both int32), of which the token sees the last ``window`` (0: all).  A
+    length of zero gives zeros; a length that the table does not cover, or a page that the cache
+    does not have, NaN."""
+    dev = _require_gpu(q, k_cache, v_cache, block_table, lengths)
+    dt = _head_type(q, "q", False)
+    q = _heads(q, "q")
+    B, Hq, D = q.shape
+    pages, Hk, page, _ = _cache(k_cache, v_cache, q)
+    if Hk == 0 or Hq % Hk:
+        raise ValueError(f"the query heads must be a multiple of the key-value heads, got {Hq} and {Hk}")
+    if D not in (64, 128, 256, 512):
+        raise ValueError(f"the head size must be 64, 128, 256 or 512, got {D}")
+    if block_table.dim() != 2:
+        raise ValueError(f"block_table must be int32 [{B}, pages of a sequence], got {list(block_table.shape)}")
+    width = block_table.shape[1]
+    block_table = _index(block_table, "block_table", (B, width))
+    lengths = _index(lengths, "lengths", (B,))
+    out = torch.empty((B, Hq, D), dtype=q.dtype, device=dev)
+    lib = load()
+    nbytes = lib.w4a16_decode_attention_workspace_bytes(B, Hq, Hk, D, width * page)
+    ws = _workspace(nbytes, dev)
+    _call("w4a16_decode_attention", dev, lib.w4a16_decode_attention, *_head_args(q), _ptr(k_cache), k_cache.stride(0),
+          _ptr(v_cache), v_cache.stride(0), _ptr(block_table), _ptr(lengths), _ptr(out), dt, B, Hq, Hk, D, pages, page,
+          width, float(D ** -0.5 if scale is None else scale), int(window), _ptr(ws), nbytes)
+    return out
 
 
 class MoEStages:

@@ -1,0 +1,347 @@
+// Attention of one new token per sequence over the paged key-value cache
+// (include/w4a16moe.h, w4a16_decode_attention): the cache read once, at the
+// memory's rate.
+//
+// The keys of a sequence that the token sees are cut into steps of 128; the
+// steps of all sequences and key-value heads (16 queries of a group at most)
+// are one row, dealt out evenly to the workgroups, whatever the lengths.  A
+// workgroup's part of a (sequence, head)'s steps is a piece: if it is all of them
+// its result is the output, else it goes to the workspace, two pieces a
+// workgroup at most, and k_decode_join adds them up in their order.  The cut
+// depends on the lengths alone.
+//
+// A wavefront takes 32 keys of a step by itself, straight from memory into the
+// operands of the matrix instructions, with no LDS between: a key's row is the
+// first operand of the scores as it lies (64 bytes of 16 rows a load), and of the
+// values a lane loads the 8 x 8 block of its eight keys and eight columns, 256
+// bytes of a row per load, which 32 byte permutations turn around in its
+// registers.
+#include <type_traits>
+
+#include "attention.hpp"
+
+namespace w4a16 {
+
+namespace {
+
+constexpr int kDaWaves = 4;
+constexpr int kDaStep = 32 * kDaWaves;  // keys
+
+// the keys first .. len - 1 that a sequence's token sees, in steps from base on
+struct DaSeq {
+  int len, first, base, steps;
+  bool over;  // longer than its row of the table
+};
+__device__ __forceinline__ DaSeq da_seq(const DecodeAttnArgs& a, int b) {
+  DaSeq s;
+  const int n = a.lengths[b], cap = a.width << a.page_log2;
+  s.over = n > cap;
+  s.len = max(min(n, cap), 0);
+  s.first = a.window > 0 ? max(s.len - a.window, 0) : 0;
+  s.base = s.first & ~31;
+  s.steps = max((s.len - s.base + kDaStep - 1) / kDaStep, 1);  // one without keys: it writes the zeros
+  return s;
+}
+
+// steps in front of sequence b (all of them: b = B), of one head
+__device__ __forceinline__ int da_before(const DecodeAttnArgs& a, int b) {
+  int sum = 0;
+  for (int i = threadIdx.x & 63; i < b; i += 64) sum += da_seq(a, i).steps;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o);
+  return sum;
+}
+
+// the first step of workgroup g's of `total`
+__device__ __forceinline__ int da_start(int g, int groups, int total) {
+  return (int)((int64_t)total * g / groups);
+}
+
+}  // namespace
+
+template <typename T, int D>
+__global__ __launch_bounds__(64 * kDaWaves, 1) void k_decode_attention(DecodeAttnArgs a) {
+  constexpr int VW = D >= 128 ? 8 : 4;    // columns of a lane's block of values
+  constexpr int NB = D / (16 * VW);       // blocks
+  constexpr int VD = VW / 2;              // dwords of a block's row
+  __shared__ float sm[kDaWaves][16], sl[kDaWaves][16];
+  extern __shared__ __align__(16) float so[];  // [kDaWaves][D * 16]
+  const int lane = threadIdx.x & 63, r = lane & 15, c = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int gt = (a.group + 15) / 16;  // tiles of a group's queries
+  const int units = a.Hk * gt;
+  const int total = da_before(a, a.B) * units;
+  const int groups = min(a.groups, total);  // each has a step at least
+  if ((int)blockIdx.x >= groups) return;
+  int pos = da_start(blockIdx.x, groups, total);
+  const int end = da_start(blockIdx.x + 1, groups, total);
+  const int begin = pos;
+
+  // the sequence of the first step
+  int b = 0, at = 0;  // at: steps in front of it
+  for (int base = 0; base < a.B; base += 64) {
+    const int n = base + lane < a.B ? da_seq(a, base + lane).steps * units : 0;
+    int sum = n;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int v = __shfl_up(sum, o);
+      if (lane >= o) sum += v;
+    }
+    const int all = __builtin_amdgcn_readlane(sum, 63);
+    if (pos < at + all) {
+      const int i = __ffsll((unsigned long long)__ballot(at + sum > pos)) - 1;
+      b = base + i;
+      at += __builtin_amdgcn_readlane(sum - n, i);
+      break;
+    }
+    at += all;
+  }
+
+  while (pos < end) {
+    const DaSeq seq = da_seq(a, b);
+    const int unit = (pos - at) / seq.steps;
+    const int s0 = pos - at - unit * seq.steps, s1 = min(seq.steps, s0 + end - pos);
+    const int hk = unit / gt, q_first = (unit - hk * gt) * 16, q_n = min(a.group - q_first, 16);
+    const int head0 = hk * a.group + q_first;
+
+    u32x4_t qf[D / 32];
+    at_load_row<D / 32>(static_cast<const unsigned char*>(a.q) + (int64_t)(head0 + min(r, q_n - 1)) * a.q_head, b,
+                   a.q_stride, qf);
+    const int64_t in_page = (int64_t)hk * (D * 2) << a.page_log2;
+    const unsigned char* kp = static_cast<const unsigned char*>(a.kc) + in_page;
+    const unsigned char* vp = static_cast<const unsigned char*>(a.vc) + in_page;
+    const int32_t* row = a.table + (int64_t)b * a.width;
+    const int mask = (1 << a.page_log2) - 1;
+
+    float m = -1e30f, l = 0.f;
+    f32x4_t acc[NB][VW];
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+      for (int e = 0; e < VW; ++e) acc[j][e] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+
+    for (int st = s0; st < s1; ++st) {
+      const int key0 = seq.base + st * kDaStep + 32 * wave;
+      if (key0 >= seq.len) break;
+      // A lane's keys are held to the ones that are seen (those beside them may lie
+      // in pages that are another's by now, and hold anything): a group of eight
+      // keys, all of one page, has its page or, with none seen, the nearest's.
+      auto hold = [&](int key) { return min(max(key, seq.first), seq.len - 1); };
+      int pk = row[hold(key0 + 8 * (r >> 2)) >> a.page_log2], pv = row[hold(key0 + 8 * c) >> a.page_log2];
+      const bool bad = seq.over || pv < 0 || pv >= a.pages;
+      pk = pk < 0 || pk >= a.pages ? 0 : pk;
+      pv = pv < 0 || pv >= a.pages ? 0 : pv;
+      u32x4_t kf[2][D / 32];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int k = hold(key0 + 8 * (r >> 2) + 4 * t + (r & 3)) & mask;
+        at_load_row<D / 32>(kp + pk * a.k_page, k, D * 2, kf[t]);
+      }
+      uint32_t vf[NB][8][VD];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const unsigned char* p = vp + pv * a.v_page + (int64_t)(hold(key0 + 8 * c + i) & mask) * (D * 2) + r * (2 * VW);
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+          if constexpr (VW == 8) {
+            const u32x4_t v = ld16(p + 256 * j);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) vf[j][i][w] = v[w];
+          } else {
+            const u32x2_t v = *reinterpret_cast<const u32x2_t*>(p);
+            vf[j][i][0] = v.x;
+            vf[j][i][1] = v.y;
+          }
+        }
+      }
+      f32x4_t s[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        s[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) s[t] = at_mfma<T>(kf[t][i], qf[i], s[t]);
+      }
+      if (key0 < seq.first || key0 + 32 > seq.len || __any(bad)) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int key = key0 + 8 * c + 4 * t + i;
+            // a page that the cache does not have, or a length that the table does not
+            // cover: not a number, and so is the output
+            s[t][i] = key < seq.first || key >= seq.len ? -INFINITY : bad ? NAN : s[t][i];
+          }
+      }
+      const float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                              fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3]))) *
+                        a.scale2;
+      if (__any(top > m + 8.f)) {
+        const float now = fmaxf(m, at_max_over_c(top));
+        const float f = __builtin_amdgcn_exp2f(m - now);
+        m = now;
+        l *= f;
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+          for (int e = 0; e < VW; ++e) acc[j][e] *= f;
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], a.scale2, -m));
+          l += s[t][i];
+        }
+      const u32x4_t p = at_pack8<T>(s[0], s[1]);
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int e = 0; e < VW; ++e) {
+          // column e of the block, its eight keys in their order
+          const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
+          u32x4_t v;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) v[w] = __builtin_amdgcn_perm(vf[j][2 * w + 1][e / 2], vf[j][2 * w][e / 2], sel);
+          acc[j][e] = at_mfma<T>(v, p, acc[j][e]);
+        }
+    }
+
+    // the wavefronts' sums, joined
+    l = at_sum_over_c(l);
+    if (c == 0) {
+      sm[wave][r] = m;
+      sl[wave][r] = l;
+    }
+    __syncthreads();
+    float top = sm[0][r];
+#pragma unroll
+    for (int w = 1; w < kDaWaves; ++w) top = fmaxf(top, sm[w][r]);
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kDaWaves; ++w) sum += sl[w][r] * __builtin_amdgcn_exp2f(sm[w][r] - top);
+    const float f = __builtin_amdgcn_exp2f(m - top);
+    if (r < q_n) {
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int e = 0; e < VW; ++e)
+          *reinterpret_cast<f32x4_t*>(so + (wave * NB + j) * VW * 256 + e * 256 + lane * 4) = acc[j][e] * f;
+    }
+    __syncthreads();
+    const bool whole = s0 == 0 && s1 == seq.steps;
+    float* part = a.part + (int64_t)(2 * blockIdx.x + (pos == begin ? 0 : 1)) * (16 * (D + 2));
+    // thread: columns 16 VW j + VW (4 c + i) .. of query r
+    if (r < q_n) {
+      const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+      for (int w = wave; w < NB * 4; w += kDaWaves) {
+        const int j = w >> 2, i = w & 3;
+        float v[VW];
+#pragma unroll
+        for (int e = 0; e < VW; ++e) {
+          v[e] = 0.f;
+#pragma unroll
+          for (int u = 0; u < kDaWaves; ++u) v[e] += so[(u * NB + j) * VW * 256 + e * 256 + lane * 4 + i];
+        }
+        const int d = 16 * VW * j + VW * (4 * c + i);
+        if (whole) {
+          unsigned char* o = static_cast<unsigned char*>(a.out) + ((int64_t)b * a.Hq + head0 + r) * (D * 2) + 2 * d;
+#pragma unroll
+          for (int e = 0; e < VW; e += 4)
+            *reinterpret_cast<u32x2_t*>(o + 2 * e) =
+                u32x2_t{at_pack2<T>(v[e] * inv, v[e + 1] * inv), at_pack2<T>(v[e + 2] * inv, v[e + 3] * inv)};
+        } else {
+#pragma unroll
+          for (int e = 0; e < VW; e += 4)
+            *reinterpret_cast<f32x4_t*>(part + r * D + d + e) = f32x4_t{v[e], v[e + 1], v[e + 2], v[e + 3]};
+        }
+      }
+      if (!whole && wave == 0 && c == 0) {
+        part[16 * D + r] = top;
+        part[16 * D + 16 + r] = sum;
+      }
+    }
+    pos += s1 - s0;
+    if (unit == units - 1 && s1 == seq.steps) {
+      at += seq.steps * units;
+      ++b;
+    }
+    __syncthreads();
+  }
+}
+
+// the pieces of a (sequence, head) added up: a workgroup for each, nothing to do
+// where one workgroup had all its steps
+template <typename T, int D>
+__global__ __launch_bounds__(256) void k_decode_join(DecodeAttnArgs a) {
+  const int gt = (a.group + 15) / 16, units = a.Hk * gt;
+  const int b = blockIdx.x / units, unit = blockIdx.x - b * units;
+  const DaSeq seq = da_seq(a, b);
+  const int total = da_before(a, a.B) * units;
+  const int first = da_before(a, b) * units + unit * seq.steps, last = first + seq.steps - 1;
+  const int groups = min(a.groups, total);
+  // the workgroup that has a step: the last whose start is not behind it
+  auto owner = [&](int step) { return (int)(((int64_t)(step + 1) * groups - 1) / total); };
+  const int g0 = owner(first), g1 = owner(last);
+  if (g0 == g1) return;
+  const int hk = unit / gt, q_first = (unit - hk * gt) * 16, q_n = min(a.group - q_first, 16);
+  // the first piece is its workgroup's second where the unit does not start with it
+  auto slot = [&](int g) {
+    const bool opens = da_start(g, groups, total) >= first;
+    return a.part + (int64_t)(2 * g + (opens ? 0 : 1)) * (16 * (D + 2));
+  };
+  for (int i = threadIdx.x; i < q_n * (D / 4); i += 256) {
+    const int q = i / (D / 4), d = 4 * (i % (D / 4));
+    float m = -1e30f, l = 0.f;
+    f32x4_t v = {0.f, 0.f, 0.f, 0.f};
+    for (int g = g0; g <= g1; ++g) {
+      const float* p = slot(g);
+      const float pm = p[16 * D + q], pl = p[16 * D + 16 + q];
+      const float now = fmaxf(m, pm);
+      const float f = __builtin_amdgcn_exp2f(m - now), h = __builtin_amdgcn_exp2f(pm - now);
+      v = v * f + *reinterpret_cast<const f32x4_t*>(p + q * D + d) * h;
+      l = l * f + pl * h;
+      m = now;
+    }
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    *reinterpret_cast<u32x2_t*>(static_cast<unsigned char*>(a.out) +
+                                ((int64_t)b * a.Hq + hk * a.group + q_first + q) * (D * 2) + 2 * d) =
+        u32x2_t{at_pack2<T>(v[0] * inv, v[1] * inv), at_pack2<T>(v[2] * inv, v[3] * inv)};
+  }
+}
+
+namespace {
+
+template <typename T, int D>
+hipError_t decode(const DecodeAttnArgs& a, hipStream_t s) {
+  hipLaunchKernelGGL((k_decode_attention<T, D>), dim3(a.groups), dim3(64 * kDaWaves), kDaWaves * D * 16 * 4, s, a);
+  // a step is never cut: with one at most there are no pieces
+  if ((a.width << a.page_log2) > kDaStep)
+    hipLaunchKernelGGL((k_decode_join<T, D>), dim3((unsigned)(a.B * a.Hk * ((a.group + 15) / 16))), dim3(256), 0, s, a);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t decode_type(const DecodeAttnArgs& a, hipStream_t s) {
+  switch (a.D) {
+    case 64: return decode<T, 64>(a, s);
+    case 128: return decode<T, 128>(a, s);
+    case 256: return decode<T, 256>(a, s);
+    case 512: return decode<T, 512>(a, s);
+  }
+  return hipErrorInvalidValue;
+}
+
+}  // namespace
+
+int decode_attn_groups(int64_t B, int64_t Hq, int64_t Hk, int64_t keys) {
+  const int64_t steps = (keys + kDaStep - 1) / kDaStep + 1;  // a window may start inside one
+  const int64_t units = B * Hk * ((Hq / Hk + 15) / 16);
+  return units * steps < kDecodeAttnGroups ? (int)(units * steps) : kDecodeAttnGroups;
+}
+size_t decode_attn_part_floats(int64_t groups, int64_t D) { return (size_t)groups * 2 * 16 * (D + 2); }
+
+hipError_t launch_decode_attention(int dtype, const DecodeAttnArgs& a, hipStream_t s) {
+  return dtype == 0 ? decode_type<__bf16>(a, s) : decode_type<_Float16>(a, s);
+}
+
+}  // namespace w4a16

@@ -435,6 +435,63 @@ hipError_t launch_prefill_x(int mode, PrefillArgs a, int max_mtiles, hipStream_t
 size_t prefill_tiled_bytes_per_expert(int mode, int64_t H, int64_t I);
 hipError_t launch_tile_prefill(int mode, const int32_t* packed, int E, int H, int I, int32_t* tiled,
                                hipStream_t s);
+// Norm of every head with the position rotation (kernels_head_norm.hip).  Strides
+// in bytes; the gradients of q, k, v and y are of their dense layout.
+struct HeadNormArgs {
+  const void *q, *k, *v;                      // v nullable
+  int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head;
+  void *yq, *yk, *yv;                         // [T][Hq][D], [T][Hk][D]; paged: yk, yv the caches
+  const void *dq, *dk, *dv;                   // backward: the gradients of yq, yk, yv
+  const float *cos, *sin;                     // [P][R / 2]
+  const int32_t *pos, *slots;                 // slots: paged
+  const void *qw, *kw;                        // nullable together: no norm
+  float* part;                                // backward: head_norm_partials() * 2 D floats
+  int64_t k_page, v_page;                     // paged: bytes between pages
+  int T, Hq, Hk, D, P, R;
+  int page, slots_n;                          // paged: tokens of a page, of the cache
+  bool v_norm;
+  float eps;
+};
+constexpr int kHeadNormMaxD = 512;
+int head_norm_partials(int64_t T, int64_t heads, int64_t D);
+hipError_t launch_head_norm(int dtype, bool paged, const HeadNormArgs& a, hipStream_t s);
+hipError_t launch_head_norm_backward(int dtype, const HeadNormArgs& a, hipStream_t s);
+
+// Attention over packed prompts (kernels_attention.hip) and its gradients
+// (kernels_attention_back.hip).  Strides in bytes.
+struct AttnArgs {
+  const void *q, *k, *v;
+  int64_t q_stride, q_head, k_stride, k_head, v_stride, v_head;
+  void* out;                   // [Tq][Hq][D]
+  float* lse;                  // [Hq][Tq], nullable in the forward pass
+  const int32_t *cu_q, *cu_k;  // [B + 1]
+  const void* dout;            // backward: [Tq][Hq][D]
+  float* delta;                // backward: [Hq][Tq]
+  void *dq, *dk, *dv;          // backward: [Tq][Hq][D], [Tk][Hk][D], nullable
+  int B, Tq, Tk, Hq, Hk, group, D;
+  float scale, scale2;         // scale2 = scale log2(e)
+  int window, tiles;
+  bool causal;
+};
+hipError_t launch_attention(int dtype, const AttnArgs& a, hipStream_t s);
+hipError_t launch_attention_backward(int dtype, const AttnArgs& a, hipStream_t s);
+
+// One new token per sequence over the paged cache (kernels_attention_decode.hip).
+struct DecodeAttnArgs {
+  const void *q, *kc, *vc;
+  int64_t q_stride, q_head, k_page, v_page;  // bytes
+  void* out;                                 // [B][Hq][D]
+  const int32_t *table, *lengths;            // [B][width], [B]
+  float* part;
+  int B, Hq, Hk, group, D;
+  int page_log2, pages, width;
+  float scale2;
+  int window, groups;                        // workgroups
+};
+constexpr int kDecodeAttnGroups = 512;       // workgroups at most
+int decode_attn_groups(int64_t B, int64_t Hq, int64_t Hk, int64_t keys);
+size_t decode_attn_part_floats(int64_t groups, int64_t D);
+hipError_t launch_decode_attention(int dtype, const DecodeAttnArgs& a, hipStream_t s);
 // CUs of the current device
 int device_cus();
 // persistent prefill grid: the workgroups that fit at once (a multiple of the

@@ -454,6 +454,98 @@ W4A16_API int w4a16_hybridlink_backward(const uint16_t* dout, const uint16_t* h,
                                         uint16_t* dp2_b, uint16_t* dln2_w, uint16_t* dln2_b, int64_t B, int64_t H,
                                         void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- The attention half of a decoder layer.  No kernel of the reference
+ * matches it (its layers call the installed model's attention, backends.py:
+ * 151-172); with moe_ffn_block_forward it is a whole layer.  Tensors of heads
+ * are [tokens][heads][D], D contiguous, with any non-negative strides (in
+ * elements) between tokens and between heads that are multiples of 16 bytes and
+ * at most 64 MiB; outputs are dense.  Sums, softmax statistics and norms are in
+ * fp32; results are rounded once to the type.  No atomics: a call repeated on
+ * the same values gives the same bits.                                      */
+
+/* RMS norm of every head with the position rotation in the same pass.  For a
+ * row x of D elements of q and k, and u = x rsqrt(mean x^2 + eps) weight:
+ *   y_i     = u_i cos[p][i] - u_{i+h} sin[p][i]       (i < h = R / 2)
+ *   y_{i+h} = u_{i+h} cos[p][i] + u_i sin[p][i],  y_i = u_i  (i >= R)
+ * p = positions[t]; rows of v (NULL: none) are normed without a weight and not
+ * turned.  q_weight, k_weight [D] (both NULL: q and k are turned alone).  cos,
+ * sin float32 [P][R / 2] (R 0: NULL).  A position outside 0 .. P - 1 makes its
+ * token's q and k rows NaN.  dtype: bf16, fp16 or fp32.  D a multiple of 8, at
+ * most 512; R a multiple of 8, at most D; 16-byte aligned pointers.
+ * backward: the gradients of the inputs (dq_in, ..: dense) for those of the
+ * outputs (dq, ..: dense), and of the weights (NULL both: not wanted), sums
+ * over all rows.                                                            */
+W4A16_API int w4a16_head_norm_rope(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token,
+                                   int64_t k_head, const void* v, int64_t v_token, int64_t v_head, const float* cos,
+                                   const float* sin, const int32_t* positions, const void* q_weight,
+                                   const void* k_weight, void* q_out, void* k_out, void* v_out, int dtype, int64_t T,
+                                   int64_t Hq, int64_t Hk, int64_t D, int64_t P, int64_t R, float eps, void* stream);
+W4A16_API size_t w4a16_head_norm_rope_backward_workspace_bytes(int64_t T, int64_t Hq, int64_t Hk, int64_t D);
+W4A16_API int w4a16_head_norm_rope_backward(const void* dq, const void* dk, const void* dv, const void* q,
+                                            int64_t q_token, int64_t q_head, const void* k, int64_t k_token,
+                                            int64_t k_head, const void* v, int64_t v_token, int64_t v_head,
+                                            const float* cos, const float* sin, const int32_t* positions,
+                                            const void* q_weight, const void* k_weight, void* dq_in, void* dk_in,
+                                            void* dv_in, void* dq_weight, void* dk_weight, int dtype, int64_t T,
+                                            int64_t Hq, int64_t Hk, int64_t D, int64_t P, int64_t R, float eps,
+                                            void* workspace, size_t workspace_bytes, void* stream);
+
+/* w4a16_head_norm_rope on the way into a paged cache: q_out dense, the rows of
+ * k and v (normed where v_norm) at slot slots[t] = page * page_size + row of
+ *   k_cache, v_cache [pages][Hk][page_size][D], k_page_stride and v_page_stride
+ * elements from page to page (multiples of 8).  A slot outside the cache (-1: a
+ * padding token's) is not written; two tokens of one call must not share a slot.
+ * page_size a power of two, 16 .. 1024; bf16 or fp16.                       */
+W4A16_API int w4a16_append_kv(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token,
+                              int64_t k_head, const void* v, int64_t v_token, int64_t v_head, const float* cos,
+                              const float* sin, const int32_t* positions, const int32_t* slots, const void* q_weight,
+                              const void* k_weight, void* q_out, void* k_cache, int64_t k_page_stride, void* v_cache,
+                              int64_t v_page_stride, int dtype, int v_norm, int64_t T, int64_t Hq, int64_t Hk,
+                              int64_t D, int64_t P, int64_t R, int64_t pages, int64_t page_size, float eps,
+                              void* stream);
+
+/* Attention over packed sequences: out_i = sum_j p_ij v_j, p the softmax of
+ * scale q_i k_j over the keys that query i sees, query head h with key-value
+ * head h / (Hq / Hk).  Sequence b has queries cu_q[b] .. cu_q[b + 1] - 1 and keys
+ * cu_k[b] .. cu_k[b + 1] - 1 (int32 [B + 1], from 0 on, never falling; values
+ * outside 0 .. Tq / Tk are held to them).  With nq queries and nk keys, query i
+ * stands at i + nk - nq; causal: it sees keys up to there, and with window > 0
+ * (causal only) the last `window` of these.  A query without keys, and every row
+ * behind the last sequence, gets zeros (lse -inf).  lse (NULL: not wanted):
+ * float32 [Hq][Tq], log sum_j exp(scale q_i k_j).  D 64, 128, 256 or 512; bf16
+ * or fp16; 16-byte aligned pointers.  The weights are rounded to the type as
+ * operands of the second product.
+ * backward: gradients of q, k and v (dq NULL, or dk and dv: not wanted) for that
+ * of out, with out and lse of the forward call; p, and ds = p (dp - delta), are
+ * rounded to the type as operands.                                          */
+W4A16_API int w4a16_attention(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token,
+                              int64_t k_head, const void* v, int64_t v_token, int64_t v_head, const int32_t* cu_q,
+                              const int32_t* cu_k, void* out, float* lse, int dtype, int64_t B, int64_t Tq, int64_t Tk,
+                              int64_t Hq, int64_t Hk, int64_t D, float scale, int causal, int64_t window, void* stream);
+W4A16_API size_t w4a16_attention_backward_workspace_bytes(int64_t Tq, int64_t Hq);
+W4A16_API int w4a16_attention_backward(const void* dout, const void* q, int64_t q_token, int64_t q_head, const void* k,
+                                       int64_t k_token, int64_t k_head, const void* v, int64_t v_token,
+                                       int64_t v_head, const void* out, const float* lse, const int32_t* cu_q,
+                                       const int32_t* cu_k, void* dq, void* dk, void* dv, int dtype, int64_t B,
+                                       int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D, float scale,
+                                       int causal, int64_t window, void* workspace, size_t workspace_bytes,
+                                       void* stream);
+
+/* Attention of one new token per sequence over the paged cache of
+ * w4a16_append_kv: q, out [B][Hq][D], keys 0 .. lengths[b] - 1 of sequence b (the
+ * last `window` of them where window > 0), key j in row j % page_size of page
+ * block_table[b][j / page_size] (int32 [B][width]).  Lengths of zero and less
+ * give zeros; a length over width * page_size, or a page outside the cache among
+ * those that the token sees, gives NaN.  Entries of pages it does not see are
+ * not read from.  `keys` of the workspace: width * page_size.               */
+W4A16_API size_t w4a16_decode_attention_workspace_bytes(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t keys);
+W4A16_API int w4a16_decode_attention(const void* q, int64_t q_token, int64_t q_head, const void* k_cache,
+                                     int64_t k_page_stride, const void* v_cache, int64_t v_page_stride,
+                                     const int32_t* block_table, const int32_t* lengths, void* out, int dtype,
+                                     int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t pages, int64_t page_size,
+                                     int64_t width, float scale, int64_t window, void* workspace,
+                                     size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

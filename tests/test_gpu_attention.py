@@ -1,0 +1,187 @@
+"""Attention over packed prompts, its gradients and decoding over the paged cache, against 64 bits:
+every element within what the kernels' roundings can move it (attention_reference.py)."""
+import math
+
+import pytest
+import torch
+
+import attention_reference as ref
+from hybridagent_amd import _lib
+
+pytestmark = pytest.mark.gpu
+
+BF, HF = torch.bfloat16, torch.float16
+
+
+@pytest.fixture(scope="module", autouse=True)
+def dev():
+    assert _lib.available(), "libw4a16moe.so must be built"
+    return torch.device("cuda:0")
+
+
+def _inputs(lens_q, lens_k, Hq, Hk, D, dtype, behind=0, std=1.5):
+    Tq, Tk = sum(lens_q) + behind, sum(lens_k) + behind
+    q = ref.normal(1, Tq, Hq, D, dtype=dtype, std=std)
+    k, v = ref.normal(2, Tk, Hk, D, dtype=dtype), ref.normal(3, Tk, Hk, D, dtype=dtype)
+    return q, k, v, ref.offsets(lens_q), ref.offsets(lens_k), ref.normal(4, Tq, Hq, D, dtype=dtype)
+
+
+def _check(q, k, v, cu_q, cu_k, dout, causal=True, window=0, scale=None, train=True):
+    sc = q.shape[2] ** -0.5 if scale is None else scale
+    kw = dict(scale=scale, causal=causal, window=window)
+    out, lse = _lib.attention(q, k, v, cu_q, cu_k, return_lse=True, **kw)
+    assert torch.equal(out, _lib.attention(q, k, v, cu_q, cu_k, **kw))
+    want = ref.packed(q, k, v, cu_q, cu_k, sc, causal, window, dout if train else None)
+    ref.check(out, want["out"], "out")
+    ref.check(lse, want["lse"], "lse")
+    if train:
+        grads = _lib.attention_backward(dout, q, k, v, out, lse, cu_q, cu_k, **kw)
+        for name, t in zip(("dq", "dk", "dv"), grads):
+            ref.check(t, want[name], name)
+        again = _lib.attention_backward(dout, q, k, v, out, lse, cu_q, cu_k, **kw)
+        assert all(torch.equal(a, b) for a, b in zip(grads, again))
+
+
+LENS = [[1], [5, 1, 64, 130, 33], [0, 33, 0, 0, 300, 0], [257], [128, 128], [31, 32, 33, 63, 65]]
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+@pytest.mark.parametrize("lens", LENS, ids=str)
+def test_prompts(D, lens, dtype):
+    _check(*_inputs(lens, lens, 4, 2, D, dtype))
+
+
+@pytest.mark.parametrize("Hq,Hk", [(1, 1), (3, 1), (8, 8), (17, 1), (24, 3)])
+@pytest.mark.parametrize("D", [64, 256])
+def test_heads(D, Hq, Hk):
+    _check(*_inputs([70, 9], [70, 9], Hq, Hk, D, BF))
+
+
+@pytest.mark.parametrize("window", [1, 2, 16, 31, 32, 33, 100, 1000])
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_windows(D, window):
+    _check(*_inputs([300, 7, 129], [300, 7, 129], 2, 1, D, BF), window=window)
+
+
+@pytest.mark.parametrize("window", [0, 40])
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_queries_and_keys_of_other_lengths(D, window):
+    """Queries at the end of their keys; more queries than keys: the first see none; none of the one,
+    none of the other."""
+    q, k, v, cu_q, cu_k, dout = _inputs([5, 100, 0, 64, 33], [205, 37, 12, 0, 33], 4, 2, D, BF)
+    _check(q, k, v, cu_q, cu_k, dout, window=window)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_all_keys_seen(D):
+    _check(*_inputs([5, 100, 1, 64], [205, 37, 12, 0], 4, 2, D, BF), causal=False)
+
+
+@pytest.mark.parametrize("scale", [1.0, 0.02])
+def test_scale(scale):
+    _check(*_inputs([90, 40], [90, 40], 2, 1, 128, BF, std=0.1 if scale == 1.0 else 3.0), scale=scale)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_long(D):
+    _check(*_inputs([1111, 389], [1111, 389], 2, 1, D, BF))
+
+
+@pytest.mark.parametrize("D", [64, 256])
+def test_long_fp16(D):
+    _check(*_inputs([1500], [1500], 2, 1, D, HF))
+
+
+def test_scores_that_grow_along_the_keys():
+    """Each key's score is above the last's, by less and by more than the running maximum's slack."""
+    for step in (0.5, 7.0, 30.0):
+        n, D = 200, 64
+        q = torch.zeros(n, 1, D, device="cuda", dtype=BF)
+        q[..., 0] = 1.0
+        k = torch.zeros(n, 1, D, device="cuda", dtype=BF)
+        k[:, 0, 0] = torch.arange(n, device="cuda") * step
+        v = ref.normal(3, n, 1, D)
+        cu = ref.offsets([n])
+        _check(q, k, v, cu, cu, ref.normal(4, n, 1, D), scale=1.0)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_rows_behind_the_last_sequence(D):
+    """Zeros there, whatever they hold, and nothing of them in the sequences."""
+    q, k, v, cu, _, dout = _inputs([50, 21], [50, 21], 2, 2, D, BF, behind=40)
+    want = _lib.attention(q[:71], k[:71], v[:71], cu, return_lse=True)
+    grads = _lib.attention_backward(dout[:71], q[:71], k[:71], v[:71], *want, cu)
+    for t in (q, k, v, dout):
+        t[71:] = math.nan
+    out, lse = _lib.attention(q, k, v, cu, return_lse=True)
+    assert torch.equal(out[:71], want[0]) and torch.equal(lse[:, :71], want[1])
+    assert not out[71:].any() and bool((lse[:, 71:] == -math.inf).all())
+    for t, w in zip(_lib.attention_backward(dout, q, k, v, out, lse, cu), grads):
+        assert torch.equal(t[:71], w) and not t[71:].any()
+
+
+# ---------------------------------------------------------------- decoding
+
+
+def _cache(lens, Hk, D, page, dtype, spare=3, width=None, seed=7):
+    """Pages in a random order, unused rows and pages not a number, unused entries -1."""
+    need = [-(-n // page) for n in lens]
+    pages = sum(need) + spare
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    order = torch.randperm(pages, generator=g, device="cuda").int()
+    table = torch.full((len(lens), max([width or 1, *need])), -1, device="cuda", dtype=torch.int32)
+    kc, vc = (torch.full((pages, Hk, page, D), math.nan, device="cuda", dtype=dtype) for _ in range(2))
+    keys, values = [], []
+    at = 0
+    for b, n in enumerate(lens):
+        table[b, :need[b]] = order[at:at + need[b]]
+        at += need[b]
+        k, v = ref.normal(10 + b, n, Hk, D, dtype=dtype), ref.normal(500 + b, n, Hk, D, dtype=dtype)
+        j = torch.arange(n, device="cuda")
+        p = table[b].long()[j // page]
+        kc[p, :, j % page], vc[p, :, j % page] = k, v
+        keys.append(k)
+        values.append(v)
+    return kc, vc, table, torch.tensor(lens, device="cuda", dtype=torch.int32), keys, values
+
+
+def _decode(lens, Hq, Hk, D, page, dtype, window=0, scale=None, **kw):
+    kc, vc, table, lengths, keys, values = _cache(lens, Hk, D, page, dtype, **kw)
+    q = ref.normal(1, len(lens), Hq, D, dtype=dtype, std=1.5)
+    out = _lib.decode_attention(q, kc, vc, table, lengths, scale=scale, window=window)
+    for b, n in enumerate(lens):
+        want = ref.attend(q[b:b + 1], keys[b], values[b], D ** -0.5 if scale is None else scale, True, window, dtype)
+        ref.check(out[b:b + 1], want["out"], f"sequence {b} of {n}")
+    assert torch.equal(out, _lib.decode_attention(q, kc, vc, table, lengths, scale=scale, window=window))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("page", [16, 64, 256])
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_decode(D, page, dtype):
+    _decode([1, 181, 0, 15, 16, 17, 129, 700, 33], 4, 2, D, page, dtype)
+
+
+@pytest.mark.parametrize("window", [1, 15, 16, 31, 128, 300])
+@pytest.mark.parametrize("D", [64, 512])
+def test_decode_windows(D, window):
+    _decode([1, 181, 0, 15, 16, 17, 129, 700, 33], 4, 2, D, 16, BF, window=window)
+
+
+@pytest.mark.parametrize("Hq,Hk", [(1, 1), (3, 1), (16, 1), (17, 1), (40, 1), (16, 8), (6, 3)])
+def test_decode_heads(Hq, Hk):
+    _decode([181, 40], Hq, Hk, 128, 32, BF)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_decode_long(D):
+    _decode([9000, 3, 2500], 8, 1, D, 64, BF)
+
+
+def test_decode_many_sequences():
+    _decode([(37 * i) % 211 for i in range(150)], 2, 1, 64, 16, BF)
+
+
+def test_decode_scale():
+    _decode([181, 40], 4, 2, 128, 32, BF, scale=0.3)
