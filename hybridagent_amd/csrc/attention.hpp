@@ -117,53 +117,51 @@ __device__ __forceinline__ uint32_t at_lds(const void* p) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const unsigned char*)p;
 }
 
-// A lane's addresses in a tile.  Its swizzle touches bits that a tile's own
-// address (a multiple of 1024) leaves zero, so a read's address is one XOR of
-// the step's base, which no register is kept for over the steps.
+// A lane's addresses in a tile: of the scores' tile 0 and of accumulate's first
+// four rows.  Four rows on the swizzle has its lowest bit turned.  It touches bits
+// that a tile's own address (a multiple of 1024) leaves zero, so a read's address
+// is an XOR of the step's base, and no register is kept for it over the steps.
 template <int D>
 struct AtLane {
-  uint32_t row[2];  // scores' tiles
-  uint32_t col[2];  // accumulate's halves
+  uint32_t row, col;
   __device__ __forceinline__ void init() {
     const int l = threadIdx.x & 63, c = l >> 4, r = l & 15;
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int k = 8 * (r >> 2) + 4 * t + (r & 3);
-      row[t] = k * D * 2 + 16 * (at_chunk(0, c) ^ at_swz<D>(k));
-      const int v = 8 * c + 4 * t + (r >> 2);
-      col[t] = v * D * 2 + 16 * (((r & 3) >> 1) ^ at_swz<D>(v)) + 8 * (r & 1);
-    }
+    const int k = 8 * (r >> 2) + (r & 3), v = 8 * c + (r >> 2);
+    row = k * D * 2 + 16 * (at_chunk(0, c) ^ at_swz<D>(k));
+    col = v * D * 2 + 16 * (((r & 3) >> 1) ^ at_swz<D>(v)) + 8 * (r & 1);
   }
   // half (0, 1) of D: scores' sum
   __device__ __forceinline__ void half_rows(int half) {
     static_assert(D >= 256, "whole windows");
-    row[0] += half * D;
-    row[1] += half * D;
+    row += half * D;
   }
   // half of D: accumulate's columns
   __device__ __forceinline__ void half_cols(int half) {
-    if constexpr (D >= 256) {
-      col[0] += half * D;
-      col[1] += half * D;
-    } else {
-      col[0] ^= half * D;
-      col[1] ^= half * D;
-    }
+    if constexpr (D >= 256)
+      col += half * D;
+    else
+      col ^= half * D;
   }
 };
 // the addresses in the tile at `base`
+template <int D>
 struct AtRows {
   uint32_t p[2];
-  template <int D>
-  __device__ __forceinline__ AtRows(const AtLane<D>& ln, uint32_t base) : p{base + ln.row[0], base + ln.row[1]} {}
+  __device__ __forceinline__ AtRows(const AtLane<D>& ln, uint32_t base) {
+    p[0] = base + ln.row;
+    p[1] = (p[0] ^ 16) + 8 * D;
+  }
   __device__ __forceinline__ u32x4_t get(int t, int i) const {
     return *(const lds_u32x4_t*)((p[t] ^ (64 * (i & 3))) + 256 * (i >> 2));
   }
 };
+template <int D>
 struct AtCols {
   uint32_t p[2];
-  template <int D>
-  __device__ __forceinline__ AtCols(const AtLane<D>& ln, uint32_t base) : p{base + ln.col[0], base + ln.col[1]} {}
+  __device__ __forceinline__ AtCols(const AtLane<D>& ln, uint32_t base) {
+    p[0] = base + ln.col;
+    p[1] = (p[0] ^ 16) + 8 * D;
+  }
   __device__ __forceinline__ u32x4_t get(int d) const {
     const u32x2_t lo = at_tr_read((lds_at4_t*)((p[0] ^ (32 * (d & 7))) + 256 * (d >> 3)));
     const u32x2_t hi = at_tr_read((lds_at4_t*)((p[1] ^ (32 * (d & 7))) + 256 * (d >> 3)));
@@ -177,10 +175,13 @@ struct AtCols {
 template <typename T, int AHEAD, int D, int NI, int N>
 __device__ __forceinline__ void at_scores(const AtLane<D>& ln, uint32_t tile, const u32x4_t (&b)[N][NI],
                                           f32x4_t (&s)[2][N]) {
-  const AtRows rows(ln, tile);
+  const AtRows<D> rows(ln, tile);
+  // the steps of one address one after the other: it is not kept for later
+  constexpr int M = NI < 4 ? 1 : NI / 4;
+  auto step = [](int j) { return NI < 4 ? j >> 1 : 4 * ((j >> 1) % M) + (j >> 1) / M; };
   u32x4_t a[AHEAD];
 #pragma unroll
-  for (int j = 0; j < AHEAD; ++j) a[j] = rows.get(j & 1, j >> 1);
+  for (int j = 0; j < AHEAD; ++j) a[j] = rows.get(j & 1, step(j));
 #pragma unroll
   for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -189,8 +190,8 @@ __device__ __forceinline__ void at_scores(const AtLane<D>& ln, uint32_t tile, co
 #pragma unroll
   for (int j = 0; j < 2 * NI; ++j) {
 #pragma unroll
-    for (int n = 0; n < N; ++n) s[j & 1][n] = at_mfma<T>(a[j % AHEAD], b[n][j >> 1], s[j & 1][n]);
-    if (j + AHEAD < 2 * NI) a[j % AHEAD] = rows.get((j + AHEAD) & 1, (j + AHEAD) >> 1);
+    for (int n = 0; n < N; ++n) s[j & 1][n] = at_mfma<T>(a[j % AHEAD], b[n][step(j)], s[j & 1][n]);
+    if (j + AHEAD < 2 * NI) a[j % AHEAD] = rows.get((j + AHEAD) & 1, step(j + AHEAD));
     __builtin_amdgcn_sched_barrier(0);
   }
 }
@@ -199,66 +200,60 @@ template <typename T, int AHEAD, int D, int ND, int N>
 __device__ __forceinline__ void at_accumulate(const AtLane<D>& ln, uint32_t tile, const u32x4_t (&p)[N],
                                               f32x4_t (&acc)[ND][N]) {
   constexpr int A = ND < AHEAD ? ND : AHEAD;
-  const AtCols cols(ln, tile);
+  const AtCols<D> cols(ln, tile);
+  constexpr int M = ND < 8 ? 1 : ND / 8;
+  auto tile_of = [](int j) { return ND < 8 ? j : 8 * (j % M) + j / M; };
   u32x4_t a[A];
 #pragma unroll
-  for (int d = 0; d < A; ++d) a[d] = cols.get(d);
+  for (int j = 0; j < A; ++j) a[j] = cols.get(tile_of(j));
   __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-  for (int d = 0; d < ND; ++d) {
+  for (int j = 0; j < ND; ++j) {
 #pragma unroll
-    for (int n = 0; n < N; ++n) acc[d][n] = at_mfma<T>(a[d % A], p[n], acc[d][n]);
-    if (d + A < ND) a[d % A] = cols.get(d + A);
+    for (int n = 0; n < N; ++n) acc[tile_of(j)][n] = at_mfma<T>(a[j % A], p[n], acc[tile_of(j)][n]);
+    if (j + A < ND) a[j % A] = cols.get(tile_of(j + A));
     __builtin_amdgcn_sched_barrier(0);
   }
 }
 
-// Two tiles of 32 rows, from matrices of D columns, into an LDS slot by direct
-// loads of NW wavefronts.
+// Tiles of 32 rows of a matrix of D columns, into LDS by direct loads of NW
+// wavefronts.
 template <int D, int NW>
 struct AtFeed {
-  static constexpr int kTileLoads = D / 16;              // 1 KB loads of a tile
-  static constexpr int kLoads = 2 * kTileLoads / NW;     // of both, per wavefront
-  static constexpr int kSlot = 2 * at_tile_bytes<D>();
-  static_assert(kLoads * NW == 2 * kTileLoads, "every wavefront as many");
-  static constexpr bool kSplit = kTileLoads < NW;        // a wavefront loads of one tile alone
-  static constexpr int kRows = 512 / D;                  // of a load
-  static constexpr int kStep = kRows * (kSplit ? kTileLoads : NW);  // rows between a wavefront's loads
-  int row, chunk;                                        // a lane's: of the first load
-  int64_t stride[2];                                     // bytes
-  const unsigned char* p[2];
+  static constexpr int kLoads = D / 16 / NW;  // 1 KB loads of a tile, per wavefront
+  static_assert(kLoads * NW * 16 == D, "every wavefront as many");
+  static constexpr int kStep = 512 / D * NW;  // rows between a wavefront's loads
+  int wave;
+  int64_t stride;  // bytes
+  const unsigned char* p;
 
-  __device__ __forceinline__ void init(const unsigned char* p0, int64_t stride0, const unsigned char* p1,
-                                       int64_t stride1, int wave) {
-    const int lane = threadIdx.x & 63;
-    row = kRows * (wave % kTileLoads) + lane / (D / 8);
-    chunk = 16 * ((lane % (D / 8)) ^ at_swz<D>(row));
-    p[0] = p0;
-    p[1] = p1;
-    stride[0] = stride0;
-    stride[1] = stride1;
+  __device__ __forceinline__ void init(const unsigned char* matrix, int64_t stride_bytes, int wave_) {
+    wave = wave_;
+    stride = stride_bytes;
+    p = matrix;
   }
   // rows first .. of `rows` in all (past the last, it again; none: nothing is
-  // read); more0, more1: bytes in front of the matrices' own first
-  __device__ __forceinline__ void issue(unsigned char* slot, int first, int rows, int wave, int64_t more0 = 0,
-                                        int64_t more1 = 0) const {
-    const int last = rows - 1 - first;
-    const bool whole = last >= 31;
+  // read); more: bytes in front of the matrix's own first
+  __device__ __forceinline__ void issue(unsigned char* tile, int first, int rows, int64_t more = 0) const {
+    const int last = rows > 0 ? rows - 1 - first : -1;
+    const auto rsrc = make_rsrc(p + first * stride + more, last < 0 ? 0u : 0x7FFFFFFFu);
+    const int one = (int)stride;
+    // a lane's row and bytes of the first load (opaque: no register is kept for them
+    // over the steps).  Rows past its are other bits of the row: so is their swizzle
+    const int lane = (int)opaque(threadIdx.x & 63);
+    const int row = 512 / D * wave + lane / (D / 8);
+    const int ch = 16 * ((lane % (D / 8)) ^ at_swz<D>(row));
+    tile += 1024 * wave;
+    if (last >= 31) {
+      const int v = row * one;
 #pragma unroll
-    for (int m = 0; m < 2; ++m) {
-      if (kSplit && m != wave / kTileLoads) continue;
-      const auto rsrc = make_rsrc(p[m] + first * stride[m] + (m ? more1 : more0), last < 0 ? 0u : 0x7FFFFFFFu);
-      unsigned char* to = slot + m * at_tile_bytes<D>() + 1024 * (wave % kTileLoads);
-      const int one = (int)stride[m];
+      for (int j = 0; j < kLoads; ++j)
+        px_dma16(rsrc, v + (ch ^ (16 * at_swz<D>(kStep * j))), kStep * j * one, tile + 1024 * NW * j);
+    } else {
 #pragma unroll
-      for (int j = 0; j < (kSplit ? 1 : kTileLoads / NW); ++j) {
-        // rows past the first load's are other bits of the row: so is their swizzle
-        const int ch = chunk ^ (16 * at_swz<D>(kStep * j));
-        if (whole)
-          px_dma16(rsrc, row * one + ch, kStep * j * one, to + 1024 * NW * j);
-        else
-          px_dma16(rsrc, min(row + kStep * j, last) * one + ch, 0, to + 1024 * NW * j);
-      }
+      for (int j = 0; j < kLoads; ++j)
+        px_dma16(rsrc, min(row + kStep * j, last) * one + (ch ^ (16 * at_swz<D>(kStep * j))), 0,
+                 tile + 1024 * NW * j);
     }
   }
 };
@@ -278,14 +273,19 @@ __device__ __forceinline__ void at_seen_keys(const AttnArgs& a, int nk, int off,
   lo = a.window > 0 ? max(0, first + off - a.window + 1) : 0;
 }
 
-// The sequence and the tile of `rows` rows in it that workgroup item idx has;
-// the tiles of all sequences in their order, then those of the rows behind the
-// last sequence (seq = n).  first, len: the sequence's rows.  Offsets are held
-// to 0 .. total, whatever the array says.
+// The tile of `rows` rows that workgroup item `rank` has.  Tiles go by level,
+// the tiles of their sequence in front of them, the highest first: with a causal
+// mask a tile's work grows with it, and what runs last should be short (more
+// sequences than lanes: one sequence after the other).  Behind the sequences the
+// rows past the last are one more (seq = n).  first, len: the sequence's rows;
+// offsets are held to 0 .. total, whatever the array says.
 struct AtItem {
-  int seq, tile, tiles, first, len;
+  int seq, level, tiles, first, len;
 };
-__device__ __forceinline__ AtItem at_find(const int32_t* __restrict__ cu, int n, int total, int rows, int idx) {
+__device__ __forceinline__ int at_wave_sum(int v) {
+  return (int)dpp_wave_reduce((uint32_t)v, [](uint32_t x, uint32_t y) { return x + y; });
+}
+__device__ __forceinline__ AtItem at_find(const int32_t* __restrict__ cu, int n, int total, int rows, int rank) {
   const int lane = threadIdx.x & 63;
   AtItem it{-1, 0, 0, 0, 0};
   for (int base = 0; base <= n; base += 64) {
@@ -294,23 +294,42 @@ __device__ __forceinline__ AtItem at_find(const int32_t* __restrict__ cu, int n,
     if (b <= n) first = min(max(cu[b], 0), total);
     if (b < n) end = min(max(cu[b + 1], first), total);
     const int len = end - first, tiles = (len + rows - 1) / rows;
-    int sum = tiles;
+    const int all = at_wave_sum(tiles);
+    if (rank >= all) {
+      rank -= all;
+      continue;
+    }
+    int at;
+    if (n < 64) {
+      // the highest level at or above which there are more than `rank` tiles
+      int low = 0, high = (int)wave_max_u32((uint32_t)tiles);
+      while (high - low > 1) {
+        const int mid = (low + high) >> 1;
+        if (at_wave_sum(max(tiles - mid, 0)) > rank)
+          low = mid;
+        else
+          high = mid;
+      }
+      it.level = low;
+      const int k = rank - at_wave_sum(max(tiles - low - 1, 0));
+      const unsigned long long has = __ballot(tiles > low);
+      const bool mine = tiles > low && __popcll(has & ((1ull << lane) - 1ull)) == k;
+      at = __ffsll((unsigned long long)__ballot(mine)) - 1;
+    } else {
+      int sum = tiles;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int v = __shfl_up(sum, o);
-      if (lane >= o) sum += v;
+      for (int o = 1; o < 64; o <<= 1) {
+        const int v = __shfl_up(sum, o);
+        if (lane >= o) sum += v;
+      }
+      at = __ffsll((unsigned long long)__ballot(sum > rank)) - 1;
+      it.level = __builtin_amdgcn_readlane(sum, at) - 1 - rank;
     }
-    const int all = __builtin_amdgcn_readlane(sum, 63);
-    if (idx < all) {
-      const int at = __ffsll((unsigned long long)__ballot(sum > idx)) - 1;
-      it.seq = base + at;
-      it.tiles = __builtin_amdgcn_readlane(tiles, at);
-      it.tile = idx - (__builtin_amdgcn_readlane(sum, at) - it.tiles);
-      it.first = __builtin_amdgcn_readlane(first, at);
-      it.len = __builtin_amdgcn_readlane(len, at);
-      return it;
-    }
-    idx -= all;
+    it.seq = base + at;
+    it.tiles = __builtin_amdgcn_readlane(tiles, at);
+    it.first = __builtin_amdgcn_readlane(first, at);
+    it.len = __builtin_amdgcn_readlane(len, at);
+    return it;
   }
   return it;
 }
@@ -324,13 +343,19 @@ __device__ __forceinline__ void at_rows(const int32_t* __restrict__ cu, int n, i
   }
 }
 
-// workgroup -> item: every XCD (workgroups go round robin) has a run of
-// consecutive ones, so that the heads that share keys and values share an L2
-__device__ __forceinline__ int at_swizzle(int total) {
-  const int per = (total + 7) >> 3;
-  const int i = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
-  return (int)(blockIdx.x >> 3) < per && i < total ? i : -1;
+// A workgroup's head and rank.  Workgroups go round robin to the eight XCDs: each
+// has heads of its own where they divide among them, so that the queries' heads
+// that share keys and values share an L2.
+struct AtPlace {
+  int head, rank;
+};
+__device__ __forceinline__ AtPlace at_place(int heads) {
+  const int b = (int)blockIdx.x;
+  if ((heads & 7) == 0) {
+    const int per = heads >> 3, i = b >> 3;
+    return {(b & 7) * per + i % per, i / per};
+  }
+  return {b % heads, b / heads};
 }
-inline unsigned at_grid(int64_t total) { return (unsigned)((total + 7) / 8 * 8); }
 
 }  // namespace w4a16

@@ -7,34 +7,55 @@
 
 namespace w4a16 {
 
+namespace {
+
+// Two groups of four wavefronts, one of each on every SIMD, take turns: while one
+// is at the matrix units (X: the last step's weights times values, then this
+// step's scores), the other turns scores into weights (Y), a barrier between the
+// phases.  Group B runs a phase behind A:
+//
+//   phase      2t             2t + 1         2t + 2
+//   A          X(t)           Y(t)           X(t + 1)
+//   B          Y(t - 1)       X(t)           Y(t)
+//
+// so keys t are read in the phases 2t and 2t + 1, values t in 2t + 2 and 2t + 3.
+// A loads the keys and B the values, each at the start of an even phase: into the
+// ring's slot that the step S before left, for S - 1 steps ahead.
+constexpr int kGroup = 4, kWaves = 2 * kGroup;
+
+template <int D>
+constexpr int fwd_slots() { return D == 512 ? 2 : 3; }
+
+}  // namespace
+
 // A workgroup has 16 NQ queries of a head per wavefront; PAIR: per pair of
-// wavefronts (of one SIMD), each with half of D: of the scores' sum, whose halves
-// they exchange through LDS, and of the output's columns.  (Heads of 512: a
-// wavefront's registers hold 16 queries' output and the queries, and every
-// operand read from LDS would feed one matrix instruction.)
-template <typename T, int D, int NQ, int NW, bool PAIR>
-__global__ __launch_bounds__(64 * NW, 2) void k_attention(AttnArgs a) {
-  constexpr int kSlots = D == 512 ? 2 : 3;
-  constexpr int NP = PAIR ? NW / 2 : NW;
-  constexpr int BQ = 16 * NQ * NP;
-  constexpr int NI = D / 32 / (PAIR ? 2 : 1), ND = D / 16 / (PAIR ? 2 : 1);
-  constexpr int kAhead = 2;
-  using Feed = AtFeed<D, NW>;
+// wavefronts of a group, each with half of D: of the scores' sum, whose halves
+// they exchange through LDS between the phases, and of the output's columns.
+// (Heads of 512: a wavefront's registers hold 16 queries' output and the queries,
+// and every operand read from LDS would feed one matrix instruction.)
+template <typename T, int D, int NQ, bool PAIR>
+__global__ __launch_bounds__(64 * kWaves, 2) void k_attention(AttnArgs a) {
+  constexpr int S = fwd_slots<D>();
+  constexpr int kHalves = PAIR ? 2 : 1;
+  constexpr int BQ = 16 * NQ * kWaves / kHalves;
+  constexpr int NI = D / 32 / kHalves, ND = D / 16 / kHalves;
+  constexpr int kTile = at_tile_bytes<D>();
+  constexpr int kAhead = 4;
+  using Feed = AtFeed<D, kGroup>;
   extern __shared__ __align__(1024) unsigned char smem[];
   const int lane = threadIdx.x & 63, r = lane & 15, c = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int half = PAIR ? wave / NP : 0, place = PAIR ? wave % NP : wave;
+  const bool second = wave >= kGroup;  // group B
+  const int half = PAIR ? wave & 1 : 0;
 
-  const int item = at_swizzle(a.tiles * a.Hq);
-  if (item < 0) return;
-  const int head = item / a.tiles;
-  const AtItem it = at_find(a.cu_q, a.B, a.Tq, BQ, item - head * a.tiles);
+  const AtPlace at = at_place(a.Hq);
+  const AtItem it = at_find(a.cu_q, a.B, a.Tq, BQ, at.rank);
   if (it.seq < 0) return;
   int k_first, nk;
   at_rows(a.cu_k, a.B, a.Tk, it.seq, k_first, nk);
   const int nq = it.len, off = nk - nq;
-  const int wg0 = (it.tiles - 1 - it.tile) * BQ;  // the longest first
-  const int q0 = wg0 + 16 * NQ * place;
+  const int wg0 = it.level * BQ;
+  const int q0 = wg0 + 16 * NQ * (wave / kHalves);
 
   int lo, hi, wlo, whi;
   at_seen_keys(a, nk, off, wg0, min(wg0 + BQ, nq) - 1, lo, hi);
@@ -43,19 +64,26 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attention(AttnArgs a) {
   lo &= ~31;
   const int steps = hi > lo ? (hi - lo + 31) / 32 : 0;
 
-  const unsigned char* kp = static_cast<const unsigned char*>(a.k) + k_first * a.k_stride + (head / a.group) * a.k_head;
-  const unsigned char* vp = static_cast<const unsigned char*>(a.v) + k_first * a.v_stride + (head / a.group) * a.v_head;
+  // its keys (A) or values (B), and their ring
   Feed feed;
-  feed.init(kp, a.k_stride, vp, a.v_stride, wave);
+  {
+    const int kvh = at.head / a.group;
+    if (second)
+      feed.init(static_cast<const unsigned char*>(a.v) + k_first * a.v_stride + kvh * a.v_head, a.v_stride,
+                wave - kGroup);
+    else
+      feed.init(static_cast<const unsigned char*>(a.k) + k_first * a.k_stride + kvh * a.k_head, a.k_stride, wave);
+  }
+  unsigned char* const ring = smem + (second ? S * kTile : 0);
 #pragma unroll
-  for (int s = 0; s < kSlots - 1; ++s) feed.issue(smem + s * Feed::kSlot, lo + 32 * s, s < steps ? hi : 0, wave);
+  for (int s = 0; s < S - 1; ++s) feed.issue(ring + s * kTile, lo + 32 * s, s < steps ? hi : 0);
 
   u32x4_t qf[NQ][NI];
   float m[NQ], l[NQ];
   f32x4_t acc[ND][NQ];
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
-    at_load_row<NI>(static_cast<const unsigned char*>(a.q) + head * a.q_head + half * D,
+    at_load_row<NI>(static_cast<const unsigned char*>(a.q) + at.head * a.q_head + half * D,
                     it.first + min(q0 + 16 * n + r, nq - 1), a.q_stride, qf[n]);
     m[n] = -1e30f;  // below every score's, so that a masked key's weight is zero
     l[n] = 0.f;
@@ -68,56 +96,59 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attention(AttnArgs a) {
     ln.half_rows(half);
     ln.half_cols(half);
   }
-  // the pairs' exchange: [half][place][tile][n][lane]
-  f32x4_t* const mine = reinterpret_cast<f32x4_t*>(smem + kSlots * Feed::kSlot) + (half * NP + place) * 2 * NQ * 64 + lane;
-  const f32x4_t* const other = mine + (half ? -1 : 1) * NP * 2 * NQ * 64;
-
+  // the pairs' exchange: [wave][tile][n][lane]
+  f32x4_t* const mine = reinterpret_cast<f32x4_t*>(smem + 2 * S * kTile) + wave * 2 * NQ * 64 + lane;
+  const f32x4_t* const other = mine + (half ? -1 : 1) * 2 * NQ * 64;
   const uint32_t base = at_lds(smem);
-  int slot = 0;
+
+  f32x4_t s[2][NQ];
+  u32x4_t p[NQ];
+  bool active = false;  // the last step had keys that the wavefront's queries see
+  if (second) px_barrier();
+  int slot = 0, last = S - 1;  // of step t, of the step before (and of the next to load)
   for (int t = 0; t < steps; ++t) {
-    __builtin_amdgcn_s_waitcnt(px_vm_wait((kSlots - 2) * Feed::kLoads));
+    if (!second) __builtin_amdgcn_s_waitcnt(px_vm_wait((S - 2) * Feed::kLoads));
     px_barrier();
-    {
-      const int ahead = t + kSlots - 1;
-      const int to = slot == 0 ? kSlots - 1 : slot - 1;
-      feed.issue(smem + to * Feed::kSlot, lo + 32 * ahead, ahead < steps ? hi : 0, wave);
-    }
-    const uint32_t tile = base + slot * Feed::kSlot;
-    slot = slot == kSlots - 1 ? 0 : slot + 1;
+    const int ahead = t + S - 1;
+    if (!second) feed.issue(ring + last * kTile, lo + 32 * ahead, ahead < steps ? hi : 0);
+    if (active) at_accumulate<T, kAhead>(ln, base + (S + last) * kTile, p, acc);
     const int key0 = lo + 32 * t;
-    const bool active = key0 < whi && key0 + 32 > wlo;
-    f32x4_t s[2][NQ];
-    if (active) at_scores<T, kAhead>(ln, tile, qf, s);
-    if constexpr (PAIR) {
-      if (active) {
+    active = key0 < whi && key0 + 32 > wlo;
+    if (active) {
+      at_scores<T, kAhead>(ln, base + slot * kTile, qf, s);
+      if constexpr (PAIR) {
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int n = 0; n < NQ; ++n) mine[(u * NQ + n) * 64] = s[u][n];
       }
-      px_barrier();
-      if (active) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int n = 0; n < NQ; ++n) s[u][n] += other[(u * NQ + n) * 64];
-      }
     }
+    if (second) __builtin_amdgcn_s_waitcnt(px_vm_wait((S - 2) * Feed::kLoads));
+    px_barrier();
+    if (second) feed.issue(ring + last * kTile, lo + 32 * ahead, ahead < steps ? hi : 0);
+    last = slot;
+    slot = slot == S - 1 ? 0 : slot + 1;
     if (!active) continue;
+    if constexpr (PAIR) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) s[u][n] += other[(u * NQ + n) * 64];
+    }
     // some query does not see some key
     if (key0 + 32 > nk || (a.causal && key0 + 31 > q0 + off) ||
         (a.window > 0 && key0 <= min(q0 + 16 * NQ, nq) - 1 + off - a.window)) {
 #pragma unroll
       for (int n = 0; n < NQ; ++n) {
         const int q = q0 + 16 * n + r + off;
-        const int last = a.causal ? min(nk - 1, q) : nk - 1;
-        const int first = a.window > 0 ? q - a.window + 1 : 0;
+        const int to = a.causal ? min(nk - 1, q) : nk - 1;
+        const int from = a.window > 0 ? q - a.window + 1 : 0;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int key = key0 + 8 * c + 4 * u + i;
-            s[u][n][i] = key <= last && key >= first ? s[u][n][i] : -INFINITY;
+            s[u][n][i] = key <= to && key >= from ? s[u][n][i] : -INFINITY;
           }
       }
     }
@@ -143,7 +174,6 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attention(AttnArgs a) {
         for (int d = 0; d < ND; ++d) acc[d][n] *= f;
       }
     }
-    u32x4_t p[NQ];
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
 #pragma unroll
@@ -155,8 +185,9 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attention(AttnArgs a) {
         }
       p[n] = at_pack8<T>(s[0][n], s[1][n]);
     }
-    at_accumulate<T, kAhead>(ln, tile + at_tile_bytes<D>(), p, acc);
   }
+  if (!second) px_barrier();
+  if (active) at_accumulate<T, kAhead>(ln, base + (S + last) * kTile, p, acc);
 
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
@@ -165,9 +196,9 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attention(AttnArgs a) {
     if (q >= nq) continue;
     const float f = sum == 0.f ? 0.f : 1.0f / sum;
     if (a.lse != nullptr && c == 0 && half == 0)
-      a.lse[(int64_t)head * a.Tq + it.first + q] = (m[n] + __builtin_amdgcn_logf(sum)) * kLn2;
+      a.lse[(int64_t)at.head * a.Tq + it.first + q] = (m[n] + __builtin_amdgcn_logf(sum)) * kLn2;
     unsigned char* o =
-        static_cast<unsigned char*>(a.out) + ((int64_t)(it.first + q) * a.Hq + head) * (D * 2) + half * D + 8 * c;
+        static_cast<unsigned char*>(a.out) + ((int64_t)(it.first + q) * a.Hq + at.head) * (D * 2) + half * D + 8 * c;
 #pragma unroll
     for (int d = 0; d < ND; ++d)
       *reinterpret_cast<u32x2_t*>(o + 32 * d) =
@@ -177,24 +208,22 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attention(AttnArgs a) {
 
 namespace {
 
-template <typename T, int D, int NQ, int NW, bool PAIR>
+template <typename T, int D, int NQ, bool PAIR>
 hipError_t fwd(AttnArgs a, hipStream_t s) {
-  constexpr int NP = PAIR ? NW / 2 : NW;
-  a.tiles = a.Tq / (16 * NQ * NP) + a.B + 1;
-  constexpr int lds = (D == 512 ? 2 : 3) * AtFeed<D, NW>::kSlot + (PAIR ? NW * 2 * NQ * 64 * 16 : 0);
+  a.tiles = a.Tq / (16 * NQ * kWaves / (PAIR ? 2 : 1)) + a.B + 1;
+  constexpr int lds = 2 * fwd_slots<D>() * at_tile_bytes<D>() + (PAIR ? kWaves * 2 * NQ * 64 * 16 : 0);
   static_assert(lds <= 160 * 1024, "a CU's LDS");
-  hipLaunchKernelGGL((k_attention<T, D, NQ, NW, PAIR>), dim3(at_grid((int64_t)a.tiles * a.Hq)), dim3(64 * NW), lds, s,
-                     a);
+  hipLaunchKernelGGL((k_attention<T, D, NQ, PAIR>), dim3((unsigned)(a.tiles * a.Hq)), dim3(64 * kWaves), lds, s, a);
   return hipGetLastError();
 }
 
 template <typename T>
 hipError_t fwd_type(const AttnArgs& a, hipStream_t s) {
   switch (a.D) {
-    case 64: return fwd<T, 64, 2, 4, false>(a, s);
-    case 128: return fwd<T, 128, 2, 4, false>(a, s);
-    case 256: return fwd<T, 256, 2, 8, false>(a, s);
-    case 512: return fwd<T, 512, 2, 8, true>(a, s);
+    case 64: return fwd<T, 64, 2, false>(a, s);
+    case 128: return fwd<T, 128, 2, false>(a, s);
+    case 256: return fwd<T, 256, 2, false>(a, s);
+    case 512: return fwd<T, 512, 2, true>(a, s);
   }
   return hipErrorInvalidValue;
 }

@@ -10,12 +10,22 @@
 // computed twice (7 products in place of 5): every sum stays in one workgroup and
 // in one order, without atomics.
 //
-// In the last two a pair of wavefronts of one SIMD shares 16 N rows: the first
-// has the scores and p, the second dout v^T and ds.  p, in fp32, and dq's ds pass
-// between them through LDS, lane to the same lane.  One wavefront would need the
-// rows of both matrices and all sums in its registers: with a quarter of the
-// matrix unit's registers for itself, that is half as many rows, and twice the
-// LDS reads per product.
+// In the last two a pair of wavefronts of one SIMD shares 16 N rows: A has the
+// scores and p, B dout v^T and ds.  p, in fp32, and dq's ds pass between them
+// through LDS, lane to the same lane.  (One wavefront would need the rows of both
+// matrices and all sums in its registers: with its half of the SIMD's that is half
+// as many rows, and twice the LDS reads per product.)  They take turns at the
+// matrix units, a barrier between the phases: X is the sums of a step before and
+// this step's scores (or dout v^T), Y turns these into p (or ds).
+//
+//   phase    2t           2t + 1       2t + 2
+//   A        X(t)         Y(t): p(t)   X(t + 1)
+//   B        Y(t - 1)     X(t)         Y(t): ds(t) from p(t)
+//
+// A step's tiles are in LDS until the last of their reads, three phases on (dk:
+// queries in X(t + 1) of B), four (dq: keys in X(t + 2) of A, which has ds from B)
+// or one.  Heads of 512 have no room for as many: there both have their scores,
+// then p, ds and the sums of one step, a barrier between.
 #include <type_traits>
 
 #include "attention.hpp"
@@ -25,14 +35,17 @@ namespace w4a16 {
 namespace {
 
 constexpr int kPairs = 4, kBackThreads = 128 * kPairs;
-constexpr int back_slots(int D) { return D == 512 ? 2 : 3; }
+constexpr bool phases(int D) { return D < 512; }
 // 16-row tiles of a pair
-constexpr int dq_rows(int D) { return D == 512 ? 1 : D == 256 ? 2 : 4; }
+constexpr int dq_rows(int D) { return D == 512 ? 1 : D == 256 ? 2 : D == 128 ? 3 : 4; }
 constexpr int dkv_rows(int D) { return D == 512 ? 1 : D == 256 ? 2 : D == 128 ? 3 : 4; }
-template <int D>
-constexpr int back_lds(int n) {
-  return back_slots(D) * AtFeed<D, 2 * kPairs>::kSlot + kPairs * n * 64 * (2 * 16 + 16);
-}
+// LDS slots of A's tiles (keys, queries) and of B's (values, dout)
+constexpr int slots_a(int D) { return phases(D) ? 4 : 2; }
+constexpr int slots_b(int D) { return phases(D) ? 3 : 2; }
+// and bytes, with the exchange
+constexpr int back_lds(int D, int n) { return (slots_a(D) + slots_b(D)) * 64 * D + kPairs * n * 64 * (2 * 16 + 16); }
+
+__device__ __forceinline__ int ring_next(int slot, int slots) { return slot == slots - 1 ? 0 : slot + 1; }
 
 }  // namespace
 
@@ -62,25 +75,27 @@ __global__ __launch_bounds__(256) void k_attention_delta(AttnArgs a) {
 // A workgroup has 16 NQ queries of a head per pair.
 template <typename T, int D, int NQ>
 __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dq(AttnArgs a) {
-  constexpr int kSlots = back_slots(D);
+  constexpr int SA = slots_a(D), SB = slots_b(D), S = SA + SB;
   constexpr int BQ = 16 * NQ * kPairs;
   constexpr int NI = D / 32, ND = D / 32;  // a wavefront sums half of dq's columns
-  constexpr int kAhead = 2;
-  using Feed = AtFeed<D, 2 * kPairs>;
+  constexpr int kTile = at_tile_bytes<D>();
+  constexpr int kAhead = 3;
+  // steps that the loads are ahead: A's in the second phase, B's in the first
+  constexpr int kAheadA = phases(D) ? SA - 2 : 1, kAheadB = SB - 1;
+  using Feed = AtFeed<D, kPairs>;
   extern __shared__ __align__(1024) unsigned char smem[];
   const int lane = threadIdx.x & 63, r = lane & 15, c = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int role = wave / kPairs, place = wave % kPairs;
 
-  const int item = at_swizzle(a.tiles * a.Hq);
-  if (item < 0) return;
-  const int head = item / a.tiles;
-  const AtItem it = at_find(a.cu_q, a.B, a.Tq, BQ, item - head * a.tiles);
+  const AtPlace wg = at_place(a.Hq);
+  const int head = wg.head;
+  const AtItem it = at_find(a.cu_q, a.B, a.Tq, BQ, wg.rank);
   if (it.seq < 0) return;
   int k_first, nk;
   at_rows(a.cu_k, a.B, a.Tk, it.seq, k_first, nk);
   const int nq = it.len, off = nk - nq;
-  const int wg0 = (it.tiles - 1 - it.tile) * BQ;
+  const int wg0 = it.level * BQ;
   const int q0 = wg0 + 16 * NQ * place;
   int lo, hi, wlo, whi;
   at_seen_keys(a, nk, off, wg0, min(wg0 + BQ, nq) - 1, lo, hi);
@@ -89,105 +104,161 @@ __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dq(AttnArgs a) {
   lo &= ~31;
   const int steps = hi > lo ? (hi - lo + 31) / 32 : 0;
 
-  const unsigned char* kp = static_cast<const unsigned char*>(a.k) + k_first * a.k_stride + (head / a.group) * a.k_head;
-  const unsigned char* vp = static_cast<const unsigned char*>(a.v) + k_first * a.v_stride + (head / a.group) * a.v_head;
   Feed feed;
-  feed.init(kp, a.k_stride, vp, a.v_stride, wave);
+  {
+    const int kvh = head / a.group;
+    if (role)
+      feed.init(static_cast<const unsigned char*>(a.v) + k_first * a.v_stride + kvh * a.v_head, a.v_stride, place);
+    else
+      feed.init(static_cast<const unsigned char*>(a.k) + k_first * a.k_stride + kvh * a.k_head, a.k_stride, place);
+  }
+  unsigned char* const ring = smem + (role ? SA * kTile : 0);
+  int load = 0, to = 0;  // the next step to load, its slot
+  auto issue = [&] {
+    feed.issue(ring + to * kTile, lo + 32 * load, load < steps ? hi : 0);
+    ++load;
+    to = ring_next(to, role ? SB : SA);
+  };
 #pragma unroll
-  for (int s = 0; s < kSlots - 1; ++s) feed.issue(smem + s * Feed::kSlot, lo + 32 * s, s < steps ? hi : 0, wave);
+  for (int s = 0; s < (kAheadA > kAheadB ? kAheadA : kAheadB); ++s)
+    if (s < (role ? kAheadB : kAheadA)) issue();
 
-  // the rows of q (first) or dout; -lse log2(e) or delta
+  // the rows of q (A) or dout; -lse log2(e) or delta
   u32x4_t rows[NQ][NI];
   float stat[NQ];
   f32x4_t acc[ND][NQ];
-  const unsigned char* rp = role ? static_cast<const unsigned char*>(a.dout) + head * (D * 2)
-                                 : static_cast<const unsigned char*>(a.q) + head * a.q_head;
-  const float* sp = (role ? a.delta : a.lse) + (int64_t)head * a.Tq;
+  {
+    const unsigned char* rp = role ? static_cast<const unsigned char*>(a.dout) + head * (D * 2)
+                                   : static_cast<const unsigned char*>(a.q) + head * a.q_head;
+    const float* sp = (role ? a.delta : a.lse) + (int64_t)head * a.Tq;
 #pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    const int64_t q = it.first + min(q0 + 16 * n + r, nq - 1);
-    at_load_row<NI>(rp, q, role ? (int64_t)a.Hq * D * 2 : a.q_stride, rows[n]);
-    const float v = sp[q];
-    // a query without keys: its scores are all masked
-    stat[n] = role ? v : v == -INFINITY ? 0.f : -v * kLog2e;
+    for (int n = 0; n < NQ; ++n) {
+      const int64_t q = it.first + min(q0 + 16 * n + r, nq - 1);
+      at_load_row<NI>(rp, q, role ? (int64_t)a.Hq * D * 2 : a.q_stride, rows[n]);
+      const float v = sp[q];
+      // a query without keys: its scores are all masked
+      stat[n] = role ? v : v == -INFINITY ? 0.f : -v * kLog2e;
 #pragma unroll
-    for (int d = 0; d < ND; ++d) acc[d][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      for (int d = 0; d < ND; ++d) acc[d][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
   }
   AtLane<D> ln;
   ln.init();
   ln.half_cols(role);
   // the exchange: p [place][tile][n][lane], then ds [place][n][lane]
-  f32x4_t* const xp = reinterpret_cast<f32x4_t*>(smem + kSlots * Feed::kSlot) + place * 2 * NQ * 64 + lane;
-  u32x4_t* const xd = reinterpret_cast<u32x4_t*>(smem + kSlots * Feed::kSlot) + (kPairs * 2 + place) * NQ * 64 + lane;
-
+  f32x4_t* const xp = reinterpret_cast<f32x4_t*>(smem + S * kTile) + place * 2 * NQ * 64 + lane;
+  u32x4_t* const xd = reinterpret_cast<u32x4_t*>(smem + S * kTile) + (kPairs * 2 + place) * NQ * 64 + lane;
   const uint32_t base = at_lds(smem);
-  int slot = 0;
-  for (int t = 0; t < steps; ++t) {
-    __builtin_amdgcn_s_waitcnt(px_vm_wait((kSlots - 2) * Feed::kLoads));
-    px_barrier();
-    {
-      const int ahead = t + kSlots - 1;
-      const int to = slot == 0 ? kSlots - 1 : slot - 1;
-      feed.issue(smem + to * Feed::kSlot, lo + 32 * ahead, ahead < steps ? hi : 0, wave);
-    }
-    const uint32_t tile = base + slot * Feed::kSlot;
-    slot = slot == kSlots - 1 ? 0 : slot + 1;
+  f32x4_t s[2][NQ];
+  u32x4_t p[NQ];
+
+  auto active_at = [&](int t) { return lo + 32 * t < whi && lo + 32 * t + 32 > wlo; };
+  // the scores, or dout v^T
+  auto scores = [&](int ka, int vb) {
+    at_scores<T, kAhead>(ln, base + (role ? SA + vb : ka) * kTile, rows, s);
+  };
+  auto weights = [&](int t) {  // A
     const int key0 = lo + 32 * t;
-    const bool active = key0 < whi && key0 + 32 > wlo;
-    f32x4_t s[2][NQ];
-    if (active) {
-      at_scores<T, kAhead>(ln, tile + (role ? at_tile_bytes<D>() : 0), rows, s);
-      if (!role) {
-        if (key0 + 32 > nk || (a.causal && key0 + 31 > q0 + off) ||
-            (a.window > 0 && key0 <= min(q0 + 16 * NQ, nq) - 1 + off - a.window)) {
+    if (key0 + 32 > nk || (a.causal && key0 + 31 > q0 + off) ||
+        (a.window > 0 && key0 <= min(q0 + 16 * NQ, nq) - 1 + off - a.window)) {
 #pragma unroll
-          for (int n = 0; n < NQ; ++n) {
-            const int q = q0 + 16 * n + r + off;
-            const int last = a.causal ? min(nk - 1, q) : nk - 1;
-            const int first = a.window > 0 ? q - a.window + 1 : 0;
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int key = key0 + 8 * c + 4 * u + i;
-                s[u][n][i] = key <= last && key >= first ? s[u][n][i] : -INFINITY;
-              }
-          }
-        }
+      for (int n = 0; n < NQ; ++n) {
+        const int q = q0 + 16 * n + r + off;
+        const int last = a.causal ? min(nk - 1, q) : nk - 1;
+        const int first = a.window > 0 ? q - a.window + 1 : 0;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int n = 0; n < NQ; ++n) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              s[u][n][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][n][i], a.scale2, stat[n]));
-            xp[(u * NQ + n) * 64] = s[u][n];
+          for (int i = 0; i < 4; ++i) {
+            const int key = key0 + 8 * c + 4 * u + i;
+            s[u][n][i] = key <= last && key >= first ? s[u][n][i] : -INFINITY;
           }
       }
     }
-    px_barrier();
-    u32x4_t p[NQ];
-    if (active && role) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int n = 0; n < NQ; ++n) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const f32x4_t w = xp[(u * NQ + n) * 64];
-          // (a masked key's dout v^T may be anything)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[u][n][i] = w[i] == 0.f ? 0.f : w[i] * (s[u][n][i] - stat[n]);
-        }
-        p[n] = at_pack8<T>(s[0][n], s[1][n]);
-        xd[n * 64] = p[n];
+        for (int i = 0; i < 4; ++i)
+          s[u][n][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][n][i], a.scale2, stat[n]));
+        xp[(u * NQ + n) * 64] = s[u][n];
       }
+  };
+  auto slopes = [&] {  // B
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const f32x4_t w = xp[(u * NQ + n) * 64];
+        // (a masked key's dout v^T may be anything)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[u][n][i] = w[i] == 0.f ? 0.f : w[i] * (s[u][n][i] - stat[n]);
+      }
+      p[n] = at_pack8<T>(s[0][n], s[1][n]);
+      xd[n * 64] = p[n];
     }
-    px_barrier();
-    if (active) {
-      if (!role) {
+  };
+  auto take = [&] {  // A: ds from B
 #pragma unroll
-        for (int n = 0; n < NQ; ++n) p[n] = xd[n * 64];
+    for (int n = 0; n < NQ; ++n) p[n] = xd[n * 64];
+  };
+  auto sum = [&](int ka) { at_accumulate<T, kAhead>(ln, base + ka * kTile, p, acc); };
+
+  if constexpr (phases(D)) {
+    // slots of the keys of step t and of the two before
+    int ka = 0, ka1 = SA - 1, ka2 = SA - 2, vb = 0;
+    bool now = false, before = false;  // whether the steps t - 1, t - 2 were active
+    if (role) px_barrier();
+    for (int t = 0; t < steps; ++t) {
+      static_assert(kAheadA == kAheadB, "one wait for both");
+      __builtin_amdgcn_s_waitcnt(px_vm_wait((kAheadA - 1) * Feed::kLoads));
+      px_barrier();
+      if (role) issue();
+      if (role ? now : before) sum(role ? ka1 : ka2);
+      before = now;
+      now = active_at(t);
+      if (now) scores(ka, vb);
+      px_barrier();
+      if (!role) {
+        issue();
+        if (now) weights(t);
+        if (before) take();
+      } else if (now) {
+        slopes();
       }
-      at_accumulate<T, kAhead>(ln, tile, p, acc);
+      ka2 = ka1;
+      ka1 = ka;
+      ka = ring_next(ka, SA);
+      vb = ring_next(vb, SB);
+    }
+    // ka1: the last step's
+    px_barrier();
+    if (!role) {
+      if (before) sum(ka2);
+      px_barrier();
+      if (now) {
+        take();
+        sum(ka1);
+      }
+    } else if (now) {
+      sum(ka1);
+    }
+  } else {
+    int slot = 0;
+    for (int t = 0; t < steps; ++t) {
+      __builtin_amdgcn_s_waitcnt(px_vm_wait(0));
+      px_barrier();
+      issue();
+      const bool now = active_at(t);
+      if (now) scores(slot, slot);
+      if (now && !role) weights(t);
+      px_barrier();
+      if (now && role) slopes();
+      px_barrier();
+      if (now && !role) take();
+      if (now) sum(slot);
+      slot = ring_next(slot, SA);
     }
   }
 
@@ -205,29 +276,29 @@ __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dq(AttnArgs a) {
   }
 }
 
-// A workgroup has 16 NK keys of a key-value head per pair; the first wavefront
-// sums dv, the second dk.
+// A workgroup has 16 NK keys of a key-value head per pair; A sums dv, B dk.
 template <typename T, int D, int NK>
 __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dkv(AttnArgs a) {
-  constexpr int kSlots = back_slots(D);
+  constexpr int SA = slots_a(D), SB = slots_b(D), S = SA + SB;
   constexpr int BK = 16 * NK * kPairs;
   constexpr int NI = D / 32, ND = D / 16;
-  constexpr int kAhead = 2;
-  using Feed = AtFeed<D, 2 * kPairs>;
+  constexpr int kTile = at_tile_bytes<D>();
+  constexpr int kAhead = 3;
+  constexpr int kAheadA = phases(D) ? SA - 2 : 1, kAheadB = SB - 1;  // both in the first phase
+  using Feed = AtFeed<D, kPairs>;
   extern __shared__ __align__(1024) unsigned char smem[];
   const int lane = threadIdx.x & 63, r = lane & 15, c = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int role = wave / kPairs, place = wave % kPairs;
 
-  const int item = at_swizzle(a.tiles * a.Hk);
-  if (item < 0) return;
-  const int kvh = item / a.tiles;
-  const AtItem it = at_find(a.cu_k, a.B, a.Tk, BK, item - kvh * a.tiles);
+  const AtPlace wg = at_place(a.Hk);
+  const int kvh = wg.head;
+  const AtItem it = at_find(a.cu_k, a.B, a.Tk, BK, wg.rank);
   if (it.seq < 0) return;
   int q_first, nq;
   at_rows(a.cu_q, a.B, a.Tq, it.seq, q_first, nq);
   const int nk = it.len, off = nk - nq;
-  const int wg0 = it.tile * BK;  // the first keys are seen by the most queries
+  const int wg0 = (it.tiles - 1 - it.level) * BK;  // the first keys are seen by the most queries
   const int k0 = wg0 + 16 * NK * place;
   // the queries lo .. hi - 1 that see a range of keys
   auto range = [&](int first, int last, int& lo, int& hi) {
@@ -241,126 +312,171 @@ __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dkv(AttnArgs a) {
   lo &= ~31;
   const int per = hi > lo ? (hi - lo + 31) / 32 : 0;  // steps of a head
   const int steps = per * a.group;
+  const int top = lo + 32 * max(per - 1, 0);
 
-  struct Next {
+  // A place in the steps: a head after the other, its queries from the last on.
+  // (So all workgroups of a sequence that run together read the same tiles.)
+  struct At {
     int head, q0;
-  } next{kvh * a.group, lo};
-  const int64_t g_stride = (int64_t)a.Hq * D * 2;
-  const unsigned char* qp = static_cast<const unsigned char*>(a.q) + q_first * a.q_stride;
-  const unsigned char* gp = static_cast<const unsigned char*>(a.dout) + q_first * g_stride;
-  Feed feed;
-  feed.init(qp, a.q_stride, gp, g_stride, wave);
-  // the next step's loads, of a head after the other
-  auto issue = [&](unsigned char* to, bool any) {
-    feed.issue(to, next.q0, any ? nq : 0, wave, next.head * a.q_head, next.head * (D * 2));
-    next.q0 += 32;
-    if (next.q0 >= hi) {
-      next.q0 = lo;
-      ++next.head;
+  };
+  auto onward = [&](At& x) {
+    x.q0 -= 32;
+    if (x.q0 < lo) {
+      x.q0 = top;
+      ++x.head;
     }
   };
+  Feed feed;
+  if (role)
+    feed.init(static_cast<const unsigned char*>(a.dout) + (int64_t)q_first * a.Hq * D * 2, (int64_t)a.Hq * D * 2, place);
+  else
+    feed.init(static_cast<const unsigned char*>(a.q) + q_first * a.q_stride, a.q_stride, place);
+  const int64_t head_bytes = role ? D * 2 : a.q_head;
+  unsigned char* const ring = smem + (role ? SA * kTile : 0);
+  At next{kvh * a.group, top};
+  int load = 0, to = 0;
+  auto issue = [&] {
+    feed.issue(ring + to * kTile, next.q0, load < steps ? nq : 0, next.head * head_bytes);
+    onward(next);
+    ++load;
+    to = ring_next(to, role ? SB : SA);
+  };
 #pragma unroll
-  for (int s = 0; s < kSlots - 1; ++s) issue(smem + s * Feed::kSlot, s < steps);
+  for (int s = 0; s < (kAheadA > kAheadB ? kAheadA : kAheadB); ++s)
+    if (s < (role ? kAheadB : kAheadA)) issue();
 
-  u32x4_t rows[NK][NI];  // of k (first) or v
+  u32x4_t rows[NK][NI];  // of k (A) or v
   f32x4_t acc[ND][NK];
-  const unsigned char* rp = role ? static_cast<const unsigned char*>(a.v) + kvh * a.v_head
-                                 : static_cast<const unsigned char*>(a.k) + kvh * a.k_head;
+  {
+    const unsigned char* rp = role ? static_cast<const unsigned char*>(a.v) + kvh * a.v_head
+                                   : static_cast<const unsigned char*>(a.k) + kvh * a.k_head;
 #pragma unroll
-  for (int n = 0; n < NK; ++n) {
-    at_load_row<NI>(rp, it.first + min(k0 + 16 * n + r, nk - 1), role ? a.v_stride : a.k_stride, rows[n]);
+    for (int n = 0; n < NK; ++n) {
+      at_load_row<NI>(rp, it.first + min(k0 + 16 * n + r, nk - 1), role ? a.v_stride : a.k_stride, rows[n]);
 #pragma unroll
-    for (int d = 0; d < ND; ++d) acc[d][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      for (int d = 0; d < ND; ++d) acc[d][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
   }
   AtLane<D> ln;
   ln.init();
-  f32x4_t* const xp = reinterpret_cast<f32x4_t*>(smem + kSlots * Feed::kSlot) + place * 2 * NK * 64 + lane;
+  f32x4_t* const xp = reinterpret_cast<f32x4_t*>(smem + S * kTile) + place * 2 * NK * 64 + lane;
+  const uint32_t base = at_lds(smem);
 
   // lse or delta of a lane's eight queries; past the last query zeros
   struct Stats {
     u32x4_t v[2];
   };
   const float* sp = (role ? a.delta : a.lse) + q_first;
-  auto fetch = [&](int head, int q0) {
+  auto fetch = [&](const At& x, bool any) {
     Stats st;
-    const auto x = make_rsrc(sp + (int64_t)head * a.Tq + q0, (uint32_t)max(nq - q0, 0) * 4u);
+    const auto rsrc = make_rsrc(sp + (int64_t)x.head * a.Tq + x.q0, any ? (uint32_t)max(nq - x.q0, 0) * 4u : 0u);
 #pragma unroll
-    for (int u = 0; u < 2; ++u) st.v[u] = buf_ld16(x, 32 * c, 16 * u);
+    for (int u = 0; u < 2; ++u) st.v[u] = buf_ld16(rsrc, 32 * c, 16 * u);
     return st;
   };
-  int head = kvh * a.group, q0 = lo;
-  Stats now = fetch(head, steps > 0 ? q0 : nq);
+  At at{kvh * a.group, top};
+  Stats st = fetch(at, steps > 0);
+  f32x4_t s[2][NK];
+  u32x4_t p[NK];
 
-  const uint32_t base = at_lds(smem);
-  int slot = 0;
-  for (int t = 0; t < steps; ++t) {
-    __builtin_amdgcn_s_waitcnt(px_vm_wait((kSlots - 2) * Feed::kLoads));
-    px_barrier();
-    const int at = q0;
-    q0 += 32;
-    if (q0 >= hi) {
-      q0 = lo;
-      ++head;
-    }
-    issue(smem + (slot == 0 ? kSlots - 1 : slot - 1) * Feed::kSlot, t + kSlots - 1 < steps);
-    const uint32_t tile = base + slot * Feed::kSlot;
-    slot = slot == kSlots - 1 ? 0 : slot + 1;
-    const bool active = at < whi && at + 32 > wlo;
-    f32x4_t s[2][NK];
-    if (active) {
-      at_scores<T, kAhead>(ln, tile + (role ? at_tile_bytes<D>() : 0), rows, s);
-      if (!role) {
+  auto active_at = [&] { return at.q0 < whi && at.q0 + 32 > wlo; };
+  auto scores = [&](int qa, int gb) {
+    at_scores<T, kAhead>(ln, base + (role ? SA + gb : qa) * kTile, rows, s);
+  };
+  auto pack = [&] {
+#pragma unroll
+    for (int n = 0; n < NK; ++n) p[n] = at_pack8<T>(s[0][n], s[1][n]);
+  };
+  auto weights = [&] {  // A
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float lse2 = __uint_as_float(st.v[u][i]) * kLog2e;
+#pragma unroll
+        for (int n = 0; n < NK; ++n)
+          s[u][n][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][n][i], a.scale2, -lse2));
+      }
+    if (at.q0 + 32 > nq || k0 + 16 * NK > nk || (a.causal && k0 + 16 * NK - 1 > at.q0 + off) ||
+        (a.window > 0 && k0 <= at.q0 + 31 + off - a.window)) {
+#pragma unroll
+      for (int n = 0; n < NK; ++n) {
+        // the queries low .. high of the step see the key
+        const int key = k0 + 16 * n + r;
+        const int low = a.causal ? key - off - at.q0 : 0;
+        const int high = key >= nk ? -1 : (a.window > 0 ? min(nq, key - off + a.window) : nq) - 1 - at.q0;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float lse2 = __uint_as_float(now.v[u][i]) * kLog2e;
-#pragma unroll
-            for (int n = 0; n < NK; ++n)
-              s[u][n][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][n][i], a.scale2, -lse2));
+            const int q = 8 * c + 4 * u + i;
+            s[u][n][i] = q >= low && q <= high ? s[u][n][i] : 0.f;
           }
-        if (at + 32 > nq || k0 + 16 * NK > nk || (a.causal && k0 + 16 * NK - 1 > at + off) ||
-            (a.window > 0 && k0 <= at + 31 + off - a.window)) {
-#pragma unroll
-          for (int n = 0; n < NK; ++n) {
-            // the queries low .. high of the step see the key
-            const int key = k0 + 16 * n + r;
-            const int low = a.causal ? key - off - at : 0;
-            const int high = key >= nk ? -1 : (a.window > 0 ? min(nq, key - off + a.window) : nq) - 1 - at;
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int q = 8 * c + 4 * u + i;
-                s[u][n][i] = q >= low && q <= high ? s[u][n][i] : 0.f;
-              }
-          }
-        }
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int n = 0; n < NK; ++n) xp[(u * NK + n) * 64] = s[u][n];
       }
     }
-    px_barrier();
-    if (active && role) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int n = 0; n < NK; ++n) {
-          const f32x4_t w = xp[(u * NK + n) * 64];
-          // (a masked query's dout v^T may be anything)
+      for (int n = 0; n < NK; ++n) xp[(u * NK + n) * 64] = s[u][n];
+    pack();
+  };
+  auto slopes = [&] {  // B
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            s[u][n][i] = w[i] == 0.f ? 0.f : w[i] * (s[u][n][i] - __uint_as_float(now.v[u][i]));
-        }
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int n = 0; n < NK; ++n) {
+        const f32x4_t w = xp[(u * NK + n) * 64];
+        // (a masked query's dout v^T may be anything)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          s[u][n][i] = w[i] == 0.f ? 0.f : w[i] * (s[u][n][i] - __uint_as_float(st.v[u][i]));
+      }
+    pack();
+  };
+  auto sum = [&](int qa, int gb) {
+    at_accumulate<T, kAhead>(ln, base + (role ? qa : SA + gb) * kTile, p, acc);
+  };
+
+  if constexpr (phases(D)) {
+    int qa = 0, qa1 = SA - 1, gb = 0, gb1 = SB - 1;
+    bool now = false;
+    if (role) px_barrier();
+    for (int t = 0; t < steps; ++t) {
+      static_assert(kAheadA == kAheadB, "one wait for both");
+      __builtin_amdgcn_s_waitcnt(px_vm_wait((kAheadA - 1) * Feed::kLoads));
+      px_barrier();
+      issue();
+      if (now) sum(qa1, gb1);
+      now = active_at();
+      if (now) scores(qa, gb);
+      px_barrier();
+      if (now && !role) weights();
+      if (now && role) slopes();
+      onward(at);
+      st = fetch(at, t + 1 < steps);
+      qa1 = qa;
+      gb1 = gb;
+      qa = ring_next(qa, SA);
+      gb = ring_next(gb, SB);
     }
-    now = fetch(t + 1 < steps ? head : kvh * a.group, t + 1 < steps ? q0 : nq);
-    if (!active) continue;
-    u32x4_t p[NK];
-#pragma unroll
-    for (int n = 0; n < NK; ++n) p[n] = at_pack8<T>(s[0][n], s[1][n]);
-    at_accumulate<T, kAhead>(ln, tile + (role ? 0 : at_tile_bytes<D>()), p, acc);
+    if (!role) px_barrier();
+    if (now) sum(qa1, gb1);
+  } else {
+    int slot = 0;
+    for (int t = 0; t < steps; ++t) {
+      __builtin_amdgcn_s_waitcnt(px_vm_wait(0));
+      px_barrier();
+      issue();
+      const bool now = active_at();
+      if (now) scores(slot, slot);
+      if (now && !role) weights();
+      px_barrier();
+      if (now && role) slopes();
+      onward(at);
+      st = fetch(at, t + 1 < steps);
+      if (now) sum(slot, slot);
+      slot = ring_next(slot, SA);
+    }
   }
 
   unsigned char* const out = static_cast<unsigned char*>(role ? a.dk : a.dv);
@@ -383,20 +499,20 @@ namespace {
 template <typename T, int D>
 hipError_t back(AttnArgs a, hipStream_t s) {
   constexpr int NQ = dq_rows(D), NK = dkv_rows(D);
-  static_assert(back_lds<D>(NQ) <= 160 * 1024 && back_lds<D>(NK) <= 160 * 1024, "a CU's LDS");
+  static_assert(back_lds(D, NQ) <= 160 * 1024 && back_lds(D, NK) <= 160 * 1024, "a CU's LDS");
   if (a.Tq > 0) {
     const int64_t rows = (int64_t)a.Tq * a.Hq, per = 256 / (D / 8);
     hipLaunchKernelGGL((k_attention_delta<T, D>), dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, s, a);
   }
   if (a.Tq > 0 && a.dq != nullptr) {
     a.tiles = a.Tq / (16 * NQ * kPairs) + a.B + 1;
-    hipLaunchKernelGGL((k_attention_dq<T, D, NQ>), dim3(at_grid((int64_t)a.tiles * a.Hq)), dim3(kBackThreads),
-                       back_lds<D>(NQ), s, a);
+    hipLaunchKernelGGL((k_attention_dq<T, D, NQ>), dim3((unsigned)(a.tiles * a.Hq)), dim3(kBackThreads), back_lds(D, NQ), s,
+                       a);
   }
   if (a.Tk > 0 && a.dk != nullptr) {
     a.tiles = a.Tk / (16 * NK * kPairs) + a.B + 1;
-    hipLaunchKernelGGL((k_attention_dkv<T, D, NK>), dim3(at_grid((int64_t)a.tiles * a.Hk)), dim3(kBackThreads),
-                       back_lds<D>(NK), s, a);
+    hipLaunchKernelGGL((k_attention_dkv<T, D, NK>), dim3((unsigned)(a.tiles * a.Hk)), dim3(kBackThreads), back_lds(D, NK),
+                       s, a);
   }
   return hipGetLastError();
 }

@@ -60,7 +60,7 @@ __device__ __forceinline__ int da_start(int g, int groups, int total) {
 }  // namespace
 
 template <typename T, int D>
-__global__ __launch_bounds__(64 * kDaWaves, 1) void k_decode_attention(DecodeAttnArgs a) {
+__global__ __launch_bounds__(64 * kDaWaves, D == 512 ? 1 : 2) void k_decode_attention(DecodeAttnArgs a) {
   constexpr int VW = D >= 128 ? 8 : 4;    // columns of a lane's block of values
   constexpr int NB = D / (16 * VW);       // blocks
   constexpr int VD = VW / 2;              // dwords of a block's row
@@ -269,12 +269,19 @@ __global__ __launch_bounds__(64 * kDaWaves, 1) void k_decode_attention(DecodeAtt
   }
 }
 
-// the pieces of a (sequence, head) added up: a workgroup for each, nothing to do
-// where one workgroup had all its steps
+// The pieces of a query added up, in an order set by their number: a workgroup
+// for each query of each (sequence, head), nothing to do where one workgroup had
+// all its steps.  256 / (D / 4) groups of threads take a part of the pieces each.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void k_decode_join(DecodeAttnArgs a) {
+  constexpr int L = D / 4, P = 256 / L;
+  __shared__ __align__(16) float sv[P][D];
+  __shared__ float sl[P];
+  const int lane = threadIdx.x & 63;
   const int gt = (a.group + 15) / 16, units = a.Hk * gt;
-  const int b = blockIdx.x / units, unit = blockIdx.x - b * units;
+  const int b = blockIdx.x / units, unit = blockIdx.x - b * units, q = blockIdx.y;
+  const int hk = unit / gt, q_first = (unit - hk * gt) * 16;
+  if (q_first + q >= a.group) return;
   const DaSeq seq = da_seq(a, b);
   const int total = da_before(a, a.B) * units;
   const int first = da_before(a, b) * units + unit * seq.steps, last = first + seq.steps - 1;
@@ -283,30 +290,35 @@ __global__ __launch_bounds__(256) void k_decode_join(DecodeAttnArgs a) {
   auto owner = [&](int step) { return (int)(((int64_t)(step + 1) * groups - 1) / total); };
   const int g0 = owner(first), g1 = owner(last);
   if (g0 == g1) return;
-  const int hk = unit / gt, q_first = (unit - hk * gt) * 16, q_n = min(a.group - q_first, 16);
   // the first piece is its workgroup's second where the unit does not start with it
-  auto slot = [&](int g) {
-    const bool opens = da_start(g, groups, total) >= first;
-    return a.part + (int64_t)(2 * g + (opens ? 0 : 1)) * (16 * (D + 2));
-  };
-  for (int i = threadIdx.x; i < q_n * (D / 4); i += 256) {
-    const int q = i / (D / 4), d = 4 * (i % (D / 4));
-    float m = -1e30f, l = 0.f;
-    f32x4_t v = {0.f, 0.f, 0.f, 0.f};
-    for (int g = g0; g <= g1; ++g) {
-      const float* p = slot(g);
-      const float pm = p[16 * D + q], pl = p[16 * D + 16 + q];
-      const float now = fmaxf(m, pm);
-      const float f = __builtin_amdgcn_exp2f(m - now), h = __builtin_amdgcn_exp2f(pm - now);
-      v = v * f + *reinterpret_cast<const f32x4_t*>(p + q * D + d) * h;
-      l = l * f + pl * h;
-      m = now;
-    }
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
-    *reinterpret_cast<u32x2_t*>(static_cast<unsigned char*>(a.out) +
-                                ((int64_t)b * a.Hq + hk * a.group + q_first + q) * (D * 2) + 2 * d) =
-        u32x2_t{at_pack2<T>(v[0] * inv, v[1] * inv), at_pack2<T>(v[2] * inv, v[3] * inv)};
+  const bool opens = da_start(g0, groups, total) >= first;
+  auto piece = [&](int g) { return a.part + (int64_t)(2 * g + (g == g0 && !opens ? 1 : 0)) * (16 * (D + 2)); };
+  float top = -1e30f;
+  for (int g = g0 + lane; g <= g1; g += 64) top = fmaxf(top, piece(g)[16 * D + q]);
+  top = wave_max_f32(top);
+  const int at = threadIdx.x / L, d = 4 * (threadIdx.x % L);
+  f32x4_t v = {0.f, 0.f, 0.f, 0.f};
+  float l = 0.f;
+#pragma unroll 4
+  for (int g = g0 + at; g <= g1; g += P) {
+    const float* p = piece(g);
+    const float f = __builtin_amdgcn_exp2f(p[16 * D + q] - top);
+    v += *reinterpret_cast<const f32x4_t*>(p + q * D + d) * f;
+    l += p[16 * D + 16 + q] * f;
   }
+  *reinterpret_cast<f32x4_t*>(&sv[at][d]) = v;
+  if (d == 0) sl[at] = l;
+  __syncthreads();
+  if (at != 0) return;
+#pragma unroll
+  for (int i = 1; i < P; ++i) {
+    v += *reinterpret_cast<const f32x4_t*>(&sv[i][d]);
+    l += sl[i];
+  }
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  *reinterpret_cast<u32x2_t*>(static_cast<unsigned char*>(a.out) +
+                              ((int64_t)b * a.Hq + hk * a.group + q_first + q) * (D * 2) + 2 * d) =
+      u32x2_t{at_pack2<T>(v[0] * inv, v[1] * inv), at_pack2<T>(v[2] * inv, v[3] * inv)};
 }
 
 namespace {
@@ -316,7 +328,9 @@ hipError_t decode(const DecodeAttnArgs& a, hipStream_t s) {
   hipLaunchKernelGGL((k_decode_attention<T, D>), dim3(a.groups), dim3(64 * kDaWaves), kDaWaves * D * 16 * 4, s, a);
   // a step is never cut: with one at most there are no pieces
   if ((a.width << a.page_log2) > kDaStep)
-    hipLaunchKernelGGL((k_decode_join<T, D>), dim3((unsigned)(a.B * a.Hk * ((a.group + 15) / 16))), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((k_decode_join<T, D>), dim3((unsigned)(a.B * a.Hk * ((a.group + 15) / 16)),
+                                                    (unsigned)(a.group < 16 ? a.group : 16)),
+                       dim3(256), 0, s, a);
   return hipGetLastError();
 }
 
