@@ -97,12 +97,8 @@ __device__ __forceinline__ int at_chunk(int i, int c) { return 4 * i + (((c & 1)
 //   neighbouring c, two neighbouring chunks.
 // Rows are a multiple of the 256-byte window apart, or (D 64) half of one.
 template <int D>
-__device__ __forceinline__ int at_swz(int row) {
-  const int low = ((row >> 2) ^ (row >> 4)) & 1;
-  if constexpr (D >= 128)
-    return low | ((row & 3) << 1) | (row & 8);
-  else
-    return low | (row & 2) | ((row >> 1) & 4);
+__host__ __device__ constexpr int at_swz(int row) {
+  return (((row >> 2) ^ (row >> 4)) & 1) | (D >= 128 ? ((row & 3) << 1) | (row & 8) : (row & 2) | ((row >> 1) & 4));
 }
 template <int D>
 constexpr int at_tile_bytes() { return 32 * D * 2; }
@@ -169,19 +165,30 @@ struct AtCols {
   }
 };
 
+// The products' fragments are read AHEAD of their instructions (the scheduling
+// barriers keep them so: a fragment's N instructions take 16 N cycles, its read
+// about 130), over the border between the two: `next` is the scores' first.
+// Steps of one address come one after the other: it is not kept for later.
+template <int NI>
+__device__ __forceinline__ constexpr int at_row_step(int j) {
+  return NI < 4 ? j >> 1 : 4 * ((j >> 1) % (NI / 4)) + (j >> 1) / (NI / 4);
+}
+template <int ND>
+__device__ __forceinline__ constexpr int at_col_step(int j) {
+  return ND < 8 ? j : 8 * (j % (ND / 8)) + j / (ND / 8);
+}
 // s[t][n] = rows of the tile . columns b[n], over 32 NI columns of D from the one
-// that the lane's addresses stand at.  AHEAD: fragments read ahead of their
-// matrix instructions (the scheduling barriers keep them so)
+// that the lane's addresses stand at
+template <int NI, int AHEAD, int D>
+__device__ __forceinline__ void at_scores_first(const AtLane<D>& ln, uint32_t tile, u32x4_t (&next)[AHEAD]) {
+  const AtRows<D> rows(ln, tile);
+#pragma unroll
+  for (int j = 0; j < AHEAD; ++j) next[j] = rows.get(j & 1, at_row_step<NI>(j));
+}
 template <typename T, int AHEAD, int D, int NI, int N>
 __device__ __forceinline__ void at_scores(const AtLane<D>& ln, uint32_t tile, const u32x4_t (&b)[N][NI],
-                                          f32x4_t (&s)[2][N]) {
+                                          f32x4_t (&s)[2][N], u32x4_t (&a)[AHEAD]) {
   const AtRows<D> rows(ln, tile);
-  // the steps of one address one after the other: it is not kept for later
-  constexpr int M = NI < 4 ? 1 : NI / 4;
-  auto step = [](int j) { return NI < 4 ? j >> 1 : 4 * ((j >> 1) % M) + (j >> 1) / M; };
-  u32x4_t a[AHEAD];
-#pragma unroll
-  for (int j = 0; j < AHEAD; ++j) a[j] = rows.get(j & 1, step(j));
 #pragma unroll
   for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -190,28 +197,33 @@ __device__ __forceinline__ void at_scores(const AtLane<D>& ln, uint32_t tile, co
 #pragma unroll
   for (int j = 0; j < 2 * NI; ++j) {
 #pragma unroll
-    for (int n = 0; n < N; ++n) s[j & 1][n] = at_mfma<T>(a[j % AHEAD], b[n][step(j)], s[j & 1][n]);
-    if (j + AHEAD < 2 * NI) a[j % AHEAD] = rows.get((j + AHEAD) & 1, step(j + AHEAD));
+    for (int n = 0; n < N; ++n) s[j & 1][n] = at_mfma<T>(a[j % AHEAD], b[n][at_row_step<NI>(j)], s[j & 1][n]);
+    if (j + AHEAD < 2 * NI) a[j % AHEAD] = rows.get((j + AHEAD) & 1, at_row_step<NI>(j + AHEAD));
     __builtin_amdgcn_sched_barrier(0);
   }
 }
-// acc[d][n] += (tile's columns 16 d ..)^T . p[n], as many of D
-template <typename T, int AHEAD, int D, int ND, int N>
+// acc[d][n] += (tile's columns 16 d ..)^T . p[n], ND of D / 16; then the first
+// fragments of the tile `of`
+template <typename T, int NI, int AHEAD, int D, int ND, int N>
 __device__ __forceinline__ void at_accumulate(const AtLane<D>& ln, uint32_t tile, const u32x4_t (&p)[N],
-                                              f32x4_t (&acc)[ND][N]) {
-  constexpr int A = ND < AHEAD ? ND : AHEAD;
+                                              f32x4_t (&acc)[ND][N], uint32_t of, u32x4_t (&next)[AHEAD]) {
+  static_assert(ND >= AHEAD, "fragments ahead");
   const AtCols<D> cols(ln, tile);
-  constexpr int M = ND < 8 ? 1 : ND / 8;
-  auto tile_of = [](int j) { return ND < 8 ? j : 8 * (j % M) + j / M; };
-  u32x4_t a[A];
+  const AtRows<D> rows(ln, of);
+  u32x4_t a[AHEAD];
 #pragma unroll
-  for (int j = 0; j < A; ++j) a[j] = cols.get(tile_of(j));
+  for (int j = 0; j < AHEAD; ++j) a[j] = cols.get(at_col_step<ND>(j));
   __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
   for (int j = 0; j < ND; ++j) {
+    const int d = at_col_step<ND>(j);
 #pragma unroll
-    for (int n = 0; n < N; ++n) acc[tile_of(j)][n] = at_mfma<T>(a[j % A], p[n], acc[tile_of(j)][n]);
-    if (j + A < ND) a[j % A] = cols.get(tile_of(j + A));
+    for (int n = 0; n < N; ++n) acc[d][n] = at_mfma<T>(a[j % AHEAD], p[n], acc[d][n]);
+    const int k = j + AHEAD - ND;
+    if (k < 0)
+      a[j % AHEAD] = cols.get(at_col_step<ND>(j + AHEAD));
+    else
+      next[k] = rows.get(k & 1, at_row_step<NI>(k));
     __builtin_amdgcn_sched_barrier(0);
   }
 }
@@ -226,34 +238,35 @@ struct AtFeed {
   int wave;
   int64_t stride;  // bytes
   const unsigned char* p;
+  int off, ch;  // a lane's of the first load: bytes to its row, in the row
 
   __device__ __forceinline__ void init(const unsigned char* matrix, int64_t stride_bytes, int wave_) {
     wave = wave_;
     stride = stride_bytes;
     p = matrix;
+    const int lane = threadIdx.x & 63, row = 512 / D * wave + lane / (D / 8);
+    off = row * (int)stride;
+    ch = 16 * ((lane % (D / 8)) ^ at_swz<D>(row));
   }
   // rows first .. of `rows` in all (past the last, it again; none: nothing is
   // read); more: bytes in front of the matrix's own first
   __device__ __forceinline__ void issue(unsigned char* tile, int first, int rows, int64_t more = 0) const {
     const int last = rows > 0 ? rows - 1 - first : -1;
     const auto rsrc = make_rsrc(p + first * stride + more, last < 0 ? 0u : 0x7FFFFFFFu);
-    const int one = (int)stride;
-    // a lane's row and bytes of the first load (opaque: no register is kept for them
-    // over the steps).  Rows past its are other bits of the row: so is their swizzle
-    const int lane = (int)opaque(threadIdx.x & 63);
-    const int row = 512 / D * wave + lane / (D / 8);
-    const int ch = 16 * ((lane % (D / 8)) ^ at_swz<D>(row));
+    const int one = __builtin_amdgcn_readfirstlane((int)stride);
     tile += 1024 * wave;
+    // rows past the first load's are other bits of the row: so is their swizzle
+    // (opaque: no register is kept for each load over the steps)
+    const int c0 = (int)opaque((uint32_t)ch);
     if (last >= 31) {
-      const int v = row * one;
 #pragma unroll
       for (int j = 0; j < kLoads; ++j)
-        px_dma16(rsrc, v + (ch ^ (16 * at_swz<D>(kStep * j))), kStep * j * one, tile + 1024 * NW * j);
+        px_dma16(rsrc, off + (c0 ^ (16 * at_swz<D>(kStep * j))), kStep * j * one, tile + 1024 * NW * j);
     } else {
+      const int row = 512 / D * wave + (int)opaque(threadIdx.x & 63) / (D / 8);
 #pragma unroll
       for (int j = 0; j < kLoads; ++j)
-        px_dma16(rsrc, min(row + kStep * j, last) * one + (ch ^ (16 * at_swz<D>(kStep * j))), 0,
-                 tile + 1024 * NW * j);
+        px_dma16(rsrc, min(row + kStep * j, last) * one + (c0 ^ (16 * at_swz<D>(kStep * j))), 0, tile + 1024 * NW * j);
     }
   }
 };

@@ -19,12 +19,12 @@ namespace {
 //   B          Y(t - 1)       X(t)           Y(t)
 //
 // so keys t are read in the phases 2t and 2t + 1, values t in 2t + 2 and 2t + 3.
-// A loads the keys and B the values, each at the start of an even phase: into the
-// ring's slot that the step S before left, for S - 1 steps ahead.
+// A loads the keys and B the values, each at the start of its Y, for S - 1 steps
+// ahead: into the ring's slot that the step S before left.
 constexpr int kGroup = 4, kWaves = 2 * kGroup;
 
-template <int D>
-constexpr int fwd_slots() { return D == 512 ? 2 : 3; }
+// LDS slots of a ring, of steps of 32 KT keys
+constexpr int fwd_slots(int D, int KT) { return D * KT == 256 ? 3 : 2; }
 
 }  // namespace
 
@@ -33,14 +33,14 @@ constexpr int fwd_slots() { return D == 512 ? 2 : 3; }
 // they exchange through LDS between the phases, and of the output's columns.
 // (Heads of 512: a wavefront's registers hold 16 queries' output and the queries,
 // and every operand read from LDS would feed one matrix instruction.)
-template <typename T, int D, int NQ, bool PAIR>
+template <typename T, int D, int NQ, int KT, bool PAIR>
 __global__ __launch_bounds__(64 * kWaves, 2) void k_attention(AttnArgs a) {
-  constexpr int S = fwd_slots<D>();
+  constexpr int S = fwd_slots(D, KT);
   constexpr int kHalves = PAIR ? 2 : 1;
   constexpr int BQ = 16 * NQ * kWaves / kHalves;
   constexpr int NI = D / 32 / kHalves, ND = D / 16 / kHalves;
-  constexpr int kTile = at_tile_bytes<D>();
-  constexpr int kAhead = 4;
+  constexpr int kTile = at_tile_bytes<D>(), kStepBytes = KT * kTile, kKeys = 32 * KT;
+  constexpr int kAhead = 2;
   using Feed = AtFeed<D, kGroup>;
   extern __shared__ __align__(1024) unsigned char smem[];
   const int lane = threadIdx.x & 63, r = lane & 15, c = lane >> 4;
@@ -61,8 +61,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_attention(AttnArgs a) {
   at_seen_keys(a, nk, off, wg0, min(wg0 + BQ, nq) - 1, lo, hi);
   at_seen_keys(a, nk, off, q0, min(q0 + 16 * NQ, nq) - 1, wlo, whi);
   if (q0 >= nq) whi = 0;
-  lo &= ~31;
-  const int steps = hi > lo ? (hi - lo + 31) / 32 : 0;
+  lo &= -kKeys;
+  const int steps = hi > lo ? (hi - lo + kKeys - 1) / kKeys : 0;
 
   // its keys (A) or values (B), and their ring
   Feed feed;
@@ -74,9 +74,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_attention(AttnArgs a) {
     else
       feed.init(static_cast<const unsigned char*>(a.k) + k_first * a.k_stride + kvh * a.k_head, a.k_stride, wave);
   }
-  unsigned char* const ring = smem + (second ? S * kTile : 0);
+  unsigned char* const ring = smem + (second ? S * kStepBytes : 0);
+  auto issue = [&](int slot, int t) {
 #pragma unroll
-  for (int s = 0; s < S - 1; ++s) feed.issue(ring + s * kTile, lo + 32 * s, s < steps ? hi : 0);
+    for (int k = 0; k < KT; ++k)
+      feed.issue(ring + slot * kStepBytes + k * kTile, lo + kKeys * t + 32 * k, t < steps ? hi : 0);
+  };
+#pragma unroll
+  for (int s = 0; s < S - 1; ++s) issue(s, s);
 
   u32x4_t qf[NQ][NI];
   float m[NQ], l[NQ];
@@ -85,7 +90,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_attention(AttnArgs a) {
   for (int n = 0; n < NQ; ++n) {
     at_load_row<NI>(static_cast<const unsigned char*>(a.q) + at.head * a.q_head + half * D,
                     it.first + min(q0 + 16 * n + r, nq - 1), a.q_stride, qf[n]);
-    m[n] = -1e30f;  // below every score's, so that a masked key's weight is zero
+    m[n] = 0.f;
     l[n] = 0.f;
 #pragma unroll
     for (int d = 0; d < ND; ++d) acc[d][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -97,46 +102,64 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_attention(AttnArgs a) {
     ln.half_cols(half);
   }
   // the pairs' exchange: [wave][tile][n][lane]
-  f32x4_t* const mine = reinterpret_cast<f32x4_t*>(smem + 2 * S * kTile) + wave * 2 * NQ * 64 + lane;
-  const f32x4_t* const other = mine + (half ? -1 : 1) * 2 * NQ * 64;
+  f32x4_t* const mine = reinterpret_cast<f32x4_t*>(smem + 2 * S * kStepBytes) + wave * 2 * KT * NQ * 64 + lane;
+  const f32x4_t* const other = mine + (half ? -1 : 1) * 2 * KT * NQ * 64;
   const uint32_t base = at_lds(smem);
 
-  f32x4_t s[2][NQ];
-  u32x4_t p[NQ];
+  f32x4_t s[KT][2][NQ];
+  u32x4_t p[KT][NQ];
+  // X: the weights of a step times its values, in slot `from`, and the scores of one
+  // whose keys are in slot `of`
+  auto products = [&](bool sum, bool scores, int from, int of) {
+    u32x4_t next[kAhead];
+#pragma unroll
+    for (int k = 0; k < KT; ++k) {
+      const uint32_t v = base + (S + from) * kStepBytes + k * kTile, w = base + of * kStepBytes + k * kTile;
+      if (sum)
+        at_accumulate<T, NI>(ln, v, p[k], acc, w, next);
+      else
+        at_scores_first<NI>(ln, w, next);
+      if (scores) at_scores<T>(ln, w, qf, s[k], next);
+    }
+  };
   bool active = false;  // the last step had keys that the wavefront's queries see
   if (second) px_barrier();
   int slot = 0, last = S - 1;  // of step t, of the step before (and of the next to load)
   for (int t = 0; t < steps; ++t) {
-    if (!second) __builtin_amdgcn_s_waitcnt(px_vm_wait((S - 2) * Feed::kLoads));
+    if (!second) __builtin_amdgcn_s_waitcnt(px_vm_wait((S - 2) * KT * Feed::kLoads));
     px_barrier();
-    const int ahead = t + S - 1;
-    if (!second) feed.issue(ring + last * kTile, lo + 32 * ahead, ahead < steps ? hi : 0);
-    if (active) at_accumulate<T, kAhead>(ln, base + (S + last) * kTile, p, acc);
-    const int key0 = lo + 32 * t;
-    active = key0 < whi && key0 + 32 > wlo;
+    const int key0 = lo + kKeys * t;
+    const bool before = active;
+    active = key0 < whi && key0 + kKeys > wlo;
+    __builtin_amdgcn_s_setprio(1);
+    products(before, active, last, slot);
+    __builtin_amdgcn_s_setprio(0);
     if (active) {
-      at_scores<T, kAhead>(ln, base + slot * kTile, qf, s);
       if constexpr (PAIR) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int k = 0; k < KT; ++k)
 #pragma unroll
-          for (int n = 0; n < NQ; ++n) mine[(u * NQ + n) * 64] = s[u][n];
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) mine[((k * 2 + u) * NQ + n) * 64] = s[k][u][n];
       }
     }
-    if (second) __builtin_amdgcn_s_waitcnt(px_vm_wait((S - 2) * Feed::kLoads));
+    if (second) __builtin_amdgcn_s_waitcnt(px_vm_wait((S - 2) * KT * Feed::kLoads));
     px_barrier();
-    if (second) feed.issue(ring + last * kTile, lo + 32 * ahead, ahead < steps ? hi : 0);
+    issue(last, t + S - 1);
     last = slot;
     slot = slot == S - 1 ? 0 : slot + 1;
     if (!active) continue;
     if constexpr (PAIR) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int k = 0; k < KT; ++k)
 #pragma unroll
-        for (int n = 0; n < NQ; ++n) s[u][n] += other[(u * NQ + n) * 64];
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) s[k][u][n] += other[((k * 2 + u) * NQ + n) * 64];
     }
     // some query does not see some key
-    if (key0 + 32 > nk || (a.causal && key0 + 31 > q0 + off) ||
+    if (key0 + kKeys > nk || (a.causal && key0 + kKeys - 1 > q0 + off) ||
         (a.window > 0 && key0 <= min(q0 + 16 * NQ, nq) - 1 + off - a.window)) {
 #pragma unroll
       for (int n = 0; n < NQ; ++n) {
@@ -144,50 +167,68 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_attention(AttnArgs a) {
         const int to = a.causal ? min(nk - 1, q) : nk - 1;
         const int from = a.window > 0 ? q - a.window + 1 : 0;
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int k = 0; k < KT; ++k)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int key = key0 + 8 * c + 4 * u + i;
-            s[u][n][i] = key <= to && key >= from ? s[u][n][i] : -INFINITY;
-          }
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int key = key0 + 32 * k + 8 * c + 4 * u + i;
+              s[k][u][n][i] = key <= to && key >= from ? s[k][u][n][i] : -INFINITY;
+            }
       }
     }
-    // the running maximum moves where a score is 2^8 above it: the weights stay
-    // below 2^8 of the sum's first
+    // The exponents, from the running maximum as it is.  It moves where one is
+    // above 8, so that the weights stay below 2^8 of the first; and to the first
+    // that a query sees (a lane without a weight so far asks).
     float top[NQ];
     bool over = false;
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
-      top[n] = fmaxf(fmaxf(fmaxf(s[0][n][0], s[0][n][1]), fmaxf(s[0][n][2], s[0][n][3])),
-                     fmaxf(fmaxf(s[1][n][0], s[1][n][1]), fmaxf(s[1][n][2], s[1][n][3]))) *
-               a.scale2;
-      over |= top[n] > m[n] + 8.f;
+      top[n] = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < KT; ++k)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            s[k][u][n][i] = __builtin_fmaf(s[k][u][n][i], a.scale2, -m[n]);
+            top[n] = fmaxf(top[n], s[k][u][n][i]);
+          }
+      over |= top[n] > (l[n] == 0.f ? -INFINITY : 8.f);
     }
     if (__any(over)) {
 #pragma unroll
       for (int n = 0; n < NQ; ++n) {
-        const float now = fmaxf(m[n], at_max_over_c(top[n]));
-        const float f = __builtin_amdgcn_exp2f(m[n] - now);
-        m[n] = now;
+        const float t = at_max_over_c(top[n]);
+        const bool first = at_sum_over_c(l[n]) == 0.f;
+        const float up = t > (first ? -INFINITY : 0.f) ? t : 0.f;
+        const float f = __builtin_amdgcn_exp2f(-up);
+        m[n] += up;
         l[n] *= f;
+#pragma unroll
+        for (int k = 0; k < KT; ++k)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) s[k][u][n] -= up;
 #pragma unroll
         for (int d = 0; d < ND; ++d) acc[d][n] *= f;
       }
     }
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
+    for (int k = 0; k < KT; ++k)
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int n = 0; n < NQ; ++n) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          s[u][n][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][n][i], a.scale2, -m[n]));
-          l[n] += s[u][n][i];
-        }
-      p[n] = at_pack8<T>(s[0][n], s[1][n]);
-    }
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            s[k][u][n][i] = __builtin_amdgcn_exp2f(s[k][u][n][i]);
+            l[n] += s[k][u][n][i];
+          }
+        p[k][n] = at_pack8<T>(s[k][0][n], s[k][1][n]);
+      }
   }
   if (!second) px_barrier();
-  if (active) at_accumulate<T, kAhead>(ln, base + (S + last) * kTile, p, acc);
+  products(active, false, last, slot);
 
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
@@ -208,22 +249,22 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_attention(AttnArgs a) {
 
 namespace {
 
-template <typename T, int D, int NQ, bool PAIR>
+template <typename T, int D, int NQ, int KT, bool PAIR>
 hipError_t fwd(AttnArgs a, hipStream_t s) {
   a.tiles = a.Tq / (16 * NQ * kWaves / (PAIR ? 2 : 1)) + a.B + 1;
-  constexpr int lds = 2 * fwd_slots<D>() * at_tile_bytes<D>() + (PAIR ? kWaves * 2 * NQ * 64 * 16 : 0);
+  constexpr int lds = 2 * fwd_slots(D, KT) * KT * at_tile_bytes<D>() + (PAIR ? kWaves * 2 * KT * NQ * 64 * 16 : 0);
   static_assert(lds <= 160 * 1024, "a CU's LDS");
-  hipLaunchKernelGGL((k_attention<T, D, NQ, PAIR>), dim3((unsigned)(a.tiles * a.Hq)), dim3(64 * kWaves), lds, s, a);
+  hipLaunchKernelGGL((k_attention<T, D, NQ, KT, PAIR>), dim3((unsigned)(a.tiles * a.Hq)), dim3(64 * kWaves), lds, s, a);
   return hipGetLastError();
 }
 
 template <typename T>
 hipError_t fwd_type(const AttnArgs& a, hipStream_t s) {
   switch (a.D) {
-    case 64: return fwd<T, 64, 2, false>(a, s);
-    case 128: return fwd<T, 128, 2, false>(a, s);
-    case 256: return fwd<T, 256, 2, false>(a, s);
-    case 512: return fwd<T, 512, 2, true>(a, s);
+    case 64: return fwd<T, 64, 2, 2, false>(a, s);
+    case 128: return fwd<T, 128, 2, 2, false>(a, s);
+    case 256: return fwd<T, 256, 2, 1, false>(a, s);
+    case 512: return fwd<T, 512, 2, 1, true>(a, s);
   }
   return hipErrorInvalidValue;
 }

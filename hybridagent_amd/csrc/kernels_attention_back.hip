@@ -79,7 +79,7 @@ __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dq(AttnArgs a) {
   constexpr int BQ = 16 * NQ * kPairs;
   constexpr int NI = D / 32, ND = D / 32;  // a wavefront sums half of dq's columns
   constexpr int kTile = at_tile_bytes<D>();
-  constexpr int kAhead = 3;
+  constexpr int kAhead = 2;
   // steps that the loads are ahead: A's in the second phase, B's in the first
   constexpr int kAheadA = phases(D) ? SA - 2 : 1, kAheadB = SB - 1;
   using Feed = AtFeed<D, kPairs>;
@@ -153,9 +153,16 @@ __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dq(AttnArgs a) {
   u32x4_t p[NQ];
 
   auto active_at = [&](int t) { return lo + 32 * t < whi && lo + 32 * t + 32 > wlo; };
-  // the scores, or dout v^T
-  auto scores = [&](int ka, int vb) {
-    at_scores<T, kAhead>(ln, base + (role ? SA + vb : ka) * kTile, rows, s);
+  // X: ds times the keys in slot `from`, and the scores, or dout v^T, of the step
+  // whose tiles are in ka, vb
+  auto products = [&](bool sum, bool scores, int from, int ka, int vb) {
+    const uint32_t v = base + from * kTile, w = base + (role ? SA + vb : ka) * kTile;
+    u32x4_t next[kAhead];
+    if (sum)
+      at_accumulate<T, NI>(ln, v, p, acc, w, next);
+    else
+      at_scores_first<NI>(ln, w, next);
+    if (scores) at_scores<T>(ln, w, rows, s, next);
   };
   auto weights = [&](int t) {  // A
     const int key0 = lo + 32 * t;
@@ -203,7 +210,6 @@ __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dq(AttnArgs a) {
 #pragma unroll
     for (int n = 0; n < NQ; ++n) p[n] = xd[n * 64];
   };
-  auto sum = [&](int ka) { at_accumulate<T, kAhead>(ln, base + ka * kTile, p, acc); };
 
   if constexpr (phases(D)) {
     // slots of the keys of step t and of the two before
@@ -215,10 +221,12 @@ __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dq(AttnArgs a) {
       __builtin_amdgcn_s_waitcnt(px_vm_wait((kAheadA - 1) * Feed::kLoads));
       px_barrier();
       if (role) issue();
-      if (role ? now : before) sum(role ? ka1 : ka2);
+      const bool sum = role ? now : before;
       before = now;
       now = active_at(t);
-      if (now) scores(ka, vb);
+      __builtin_amdgcn_s_setprio(1);
+      products(sum, now, role ? ka1 : ka2, ka, vb);
+      __builtin_amdgcn_s_setprio(0);
       px_barrier();
       if (!role) {
         issue();
@@ -235,15 +243,11 @@ __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dq(AttnArgs a) {
     // ka1: the last step's
     px_barrier();
     if (!role) {
-      if (before) sum(ka2);
+      products(before, false, ka2, ka, vb);
       px_barrier();
-      if (now) {
-        take();
-        sum(ka1);
-      }
-    } else if (now) {
-      sum(ka1);
+      if (now) take();
     }
+    products(now, false, ka1, ka, vb);
   } else {
     int slot = 0;
     for (int t = 0; t < steps; ++t) {
@@ -251,13 +255,13 @@ __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dq(AttnArgs a) {
       px_barrier();
       issue();
       const bool now = active_at(t);
-      if (now) scores(slot, slot);
+      products(false, now, slot, slot, slot);
       if (now && !role) weights(t);
       px_barrier();
       if (now && role) slopes();
       px_barrier();
       if (now && !role) take();
-      if (now) sum(slot);
+      products(now, false, slot, slot, slot);
       slot = ring_next(slot, SA);
     }
   }
@@ -283,8 +287,9 @@ __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dkv(AttnArgs a) {
   constexpr int BK = 16 * NK * kPairs;
   constexpr int NI = D / 32, ND = D / 16;
   constexpr int kTile = at_tile_bytes<D>();
-  constexpr int kAhead = 3;
-  constexpr int kAheadA = phases(D) ? SA - 2 : 1, kAheadB = SB - 1;  // both in the first phase
+  constexpr int kAhead = 2;
+  // steps that the loads are ahead, in the second phase
+  constexpr int kAheadA = phases(D) ? SA - 2 : 1, kAheadB = SB - 1;
   using Feed = AtFeed<D, kPairs>;
   extern __shared__ __align__(1024) unsigned char smem[];
   const int lane = threadIdx.x & 63, r = lane & 15, c = lane >> 4;
@@ -380,8 +385,16 @@ __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dkv(AttnArgs a) {
   u32x4_t p[NK];
 
   auto active_at = [&] { return at.q0 < whi && at.q0 + 32 > wlo; };
-  auto scores = [&](int qa, int gb) {
-    at_scores<T, kAhead>(ln, base + (role ? SA + gb : qa) * kTile, rows, s);
+  // X: p times dout, or ds times the queries, of the step in qa1, gb1, and the
+  // scores, or dout v^T, of that in qa, gb
+  auto products = [&](bool sum, bool scores, int qa1, int gb1, int qa, int gb) {
+    const uint32_t v = base + (role ? qa1 : SA + gb1) * kTile, w = base + (role ? SA + gb : qa) * kTile;
+    u32x4_t next[kAhead];
+    if (sum)
+      at_accumulate<T, NI>(ln, v, p, acc, w, next);
+    else
+      at_scores_first<NI>(ln, w, next);
+    if (scores) at_scores<T>(ln, w, rows, s, next);
   };
   auto pack = [&] {
 #pragma unroll
@@ -433,9 +446,6 @@ __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dkv(AttnArgs a) {
       }
     pack();
   };
-  auto sum = [&](int qa, int gb) {
-    at_accumulate<T, kAhead>(ln, base + (role ? qa : SA + gb) * kTile, p, acc);
-  };
 
   if constexpr (phases(D)) {
     int qa = 0, qa1 = SA - 1, gb = 0, gb1 = SB - 1;
@@ -445,13 +455,15 @@ __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dkv(AttnArgs a) {
       static_assert(kAheadA == kAheadB, "one wait for both");
       __builtin_amdgcn_s_waitcnt(px_vm_wait((kAheadA - 1) * Feed::kLoads));
       px_barrier();
-      issue();
-      if (now) sum(qa1, gb1);
+      const bool before = now;
       now = active_at();
-      if (now) scores(qa, gb);
+      __builtin_amdgcn_s_setprio(1);
+      products(before, now, qa1, gb1, qa, gb);
+      __builtin_amdgcn_s_setprio(0);
       px_barrier();
       if (now && !role) weights();
       if (now && role) slopes();
+      issue();
       onward(at);
       st = fetch(at, t + 1 < steps);
       qa1 = qa;
@@ -460,7 +472,7 @@ __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dkv(AttnArgs a) {
       gb = ring_next(gb, SB);
     }
     if (!role) px_barrier();
-    if (now) sum(qa1, gb1);
+    products(now, false, qa1, gb1, qa, gb);
   } else {
     int slot = 0;
     for (int t = 0; t < steps; ++t) {
@@ -468,13 +480,13 @@ __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dkv(AttnArgs a) {
       px_barrier();
       issue();
       const bool now = active_at();
-      if (now) scores(slot, slot);
+      products(false, now, slot, slot, slot, slot);
       if (now && !role) weights();
       px_barrier();
       if (now && role) slopes();
       onward(at);
       st = fetch(at, t + 1 < steps);
-      if (now) sum(slot, slot);
+      products(now, false, slot, slot, slot, slot);
       slot = ring_next(slot, SA);
     }
   }
