@@ -280,6 +280,21 @@ __device__ __forceinline__ void at_load_row(const void* p, int64_t row, int64_t 
   for (int i = 0; i < NI; ++i) b[i] = ld16(q + 16 * at_chunk(i, c));
 }
 
+// Registers that loads in flight will fill, waited for here: in a loop the compiler
+// would wait in every step, and with them for the steps' loads issued since.
+template <int M, int N>
+__device__ __forceinline__ void at_settle(u32x4_t (&x)[M][N]) {
+#pragma unroll
+  for (int m = 0; m < M; ++m)
+#pragma unroll
+    for (int n = 0; n < N; ++n) asm volatile("" : "+v"(x[m][n]));
+}
+template <int N>
+__device__ __forceinline__ void at_settle(float (&x)[N]) {
+#pragma unroll
+  for (int n = 0; n < N; ++n) asm volatile("" : "+v"(x[n]));
+}
+
 // The keys lo .. hi - 1 that the queries first .. last of a sequence see, one at least
 __device__ __forceinline__ void at_seen_keys(const AttnArgs& a, int nk, int off, int first, int last, int& lo, int& hi) {
   hi = a.causal ? min(nk, last + off + 1) : nk;

@@ -95,6 +95,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_attention(AttnArgs a) {
 #pragma unroll
     for (int d = 0; d < ND; ++d) acc[d][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
+  at_settle(qf);
   AtLane<D> ln;
   ln.init();
   if constexpr (PAIR) {

@@ -142,6 +142,8 @@ __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dq(AttnArgs a) {
       for (int d = 0; d < ND; ++d) acc[d][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
   }
+  at_settle(rows);
+  at_settle(stat);
   AtLane<D> ln;
   ln.init();
   ln.half_cols(role);
@@ -362,6 +364,7 @@ __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dkv(AttnArgs a) {
       for (int d = 0; d < ND; ++d) acc[d][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
   }
+  at_settle(rows);
   AtLane<D> ln;
   ln.init();
   f32x4_t* const xp = reinterpret_cast<f32x4_t*>(smem + S * kTile) + place * 2 * NK * 64 + lane;
@@ -381,6 +384,8 @@ __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dkv(AttnArgs a) {
   };
   At at{kvh * a.group, top};
   Stats st = fetch(at, steps > 0);
+#pragma unroll
+  for (int u = 0; u < 2; ++u) asm volatile("" : "+v"(st.v[u]));
   f32x4_t s[2][NK];
   u32x4_t p[NK];
 
@@ -463,9 +468,9 @@ __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dkv(AttnArgs a) {
       px_barrier();
       if (now && !role) weights();
       if (now && role) slopes();
-      issue();
       onward(at);
-      st = fetch(at, t + 1 < steps);
+      st = fetch(at, t + 1 < steps);  // in front of the loads, which then need not be waited for with it
+      issue();
       qa1 = qa;
       gb1 = gb;
       qa = ring_next(qa, SA);
