@@ -1044,25 +1044,61 @@ def hybridlink_backward(dout: torch.Tensor, h: torch.Tensor, ln1_w: torch.Tensor
 
 # ------------------------------------------------------------------ attention
 
+# The calls of a decoded token take 5 to 15 us on the GPU: what the host does in front of them is
+# kept to one pass over the arguments (devices by number, strides and sizes read once).
 
-def _heads(t: torch.Tensor, name: str, like: torch.Tensor | None = None) -> torch.Tensor:
+
+def _gpu_of(*tensors: torch.Tensor | None) -> int:
+    """The number of the GPU that all tensors are on (``_require_gpu``'s errors)."""
+    index = -1
+    for t in tensors:
+        if t is not None:
+            i = t.get_device()
+            if i != index:
+                if i < 0 or index >= 0:
+                    _require_gpu(*tensors)
+                    raise RuntimeError("tensors on different devices")
+                index = i
+    return index
+
+
+def _launch(what: str, index: int, fn, *args) -> None:
+    """fn(*args, the current stream of GPU ``index``), run with it current."""
+    if _get_device() == index:
+        status = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, _raw_stream(index))
+    if status != W4A16_OK:
+        _check(status, what)
+
+
+def _dense_like(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
+def _dense(t: torch.Tensor) -> torch.Tensor:
+    """t contiguous, at a multiple of 16 bytes."""
+    return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else _aligned(t.contiguous())
+
+
+def _heads(t: torch.Tensor, name: str) -> torch.Tensor:
     """t [tokens, heads, D] as the kernels take it: D contiguous, the other strides as they are where
     every row starts at a multiple of 16 bytes, else a copy."""
     if t.dim() != 3:
         raise ValueError(f"{name} must be [tokens, heads, head size], got {list(t.shape)}")
-    if like is not None and (t.dtype != like.dtype or t.shape[0] != like.shape[0] or t.shape[2] != like.shape[2]):
-        raise ValueError(f"{name} must be {like.dtype} [{like.shape[0]}, heads, {like.shape[2]}], got {t.dtype} "
-                         f"{list(t.shape)}")
     a, b, c = t.stride()
-    if c == 1 and t.data_ptr() % 16 == 0:
-        step = 16 // t.element_size()
-        if a % step == 0 and b % step == 0:
-            return t
+    size = t.element_size()
+    if c == 1 and (a * size | b * size | t.data_ptr()) & 15 == 0:
+        return t
     return _aligned(t.contiguous())
 
 
 def _head_args(t: torch.Tensor | None):
-    return (None, 0, 0) if t is None else (t.data_ptr(), t.stride(0), t.stride(1))
+    if t is None:
+        return None, 0, 0
+    a, b, _ = t.stride()
+    return t.data_ptr(), a, b
 
 
 def _head_type(t: torch.Tensor, name: str, fp32: bool) -> int:
@@ -1072,42 +1108,46 @@ def _head_type(t: torch.Tensor, name: str, fp32: bool) -> int:
     return dt
 
 
-def _index(t: torch.Tensor, name: str, shape) -> torch.Tensor:
+def _index(t: torch.Tensor, name: str, *shape: int) -> torch.Tensor:
     if t.dtype != torch.int32 or t.shape != shape:
         raise ValueError(f"{name} must be int32 {list(shape)}, got {t.dtype} {list(t.shape)}")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _rope_args(q, k, v, cos, sin, positions, q_weight, k_weight, fp32: bool):
-    """What the forms of the heads' norm check alike -> (device, type, the tensors, sizes)."""
-    dev = _require_gpu(q, k, v, cos, sin, positions, q_weight, k_weight)
+    """What the forms of the heads' norm check alike -> (type, q, k, v, (cos, sin, positions, weights),
+    sizes)."""
+    dtype = q.dtype
     dt = _head_type(q, "q", fp32)
     q = _heads(q, "q")
-    k = _heads(k, "k", like=q)
-    if v is not None:
-        v = _heads(v, "v", like=q)
-        if v.shape != k.shape:
-            raise ValueError(f"v must have the shape of k, got {list(v.shape)} and {list(k.shape)}")
     T, Hq, D = q.shape
+    k = _heads(k, "k")
+    shape = k.shape
+    if k.dtype != dtype or shape[0] != T or shape[2] != D:
+        raise ValueError(f"k must be {dtype} [{T}, heads, {D}], got {k.dtype} {list(shape)}")
+    if v is not None:
+        v = _heads(v, "v")
+        if v.dtype != dtype or v.shape != shape:
+            raise ValueError(f"v must be {dtype} {list(shape)}, got {v.dtype} {list(v.shape)}")
     P = R = 0
-    if (cos is None) != (sin is None):
+    if cos is not None and sin is not None:
+        table = cos.shape
+        if cos.dtype != torch.float32 or sin.dtype != torch.float32 or len(table) != 2 or sin.shape != table:
+            raise ValueError("cos and sin must be float32 [positions, half the turned columns], got "
+                             f"{cos.dtype} {list(table)} and {sin.dtype} {list(sin.shape)}")
+        P, R = table[0], 2 * table[1]
+        cos, sin = _dense(cos), _dense(sin)
+    elif cos is not None or sin is not None:
         raise ValueError("cos and sin are given together")
-    if cos is not None:
-        for t, n in ((cos, "cos"), (sin, "sin")):
-            if t.dtype != torch.float32 or t.dim() != 2 or t.shape != cos.shape:
-                raise ValueError(f"{n} must be float32 [positions, half the turned columns], got {t.dtype} "
-                                 f"{list(t.shape)}")
-        P, R = cos.shape[0], 2 * cos.shape[1]
-        cos, sin = _aligned(cos.contiguous()), _aligned(sin.contiguous())
-    positions = _index(positions, "positions", (T,))
-    if (q_weight is None) != (k_weight is None):
-        raise ValueError("q_weight and k_weight are given together")
-    if q_weight is not None:
+    positions = _index(positions, "positions", T)
+    if q_weight is not None and k_weight is not None:
         for t, n in ((q_weight, "q_weight"), (k_weight, "k_weight")):
-            if t.dtype != q.dtype or t.shape != (D,):
-                raise ValueError(f"{n} must be {q.dtype} [{D}], got {t.dtype} {list(t.shape)}")
-        q_weight, k_weight = _aligned(q_weight.contiguous()), _aligned(k_weight.contiguous())
-    return dev, dt, (q, k, v), (cos, sin, positions, q_weight, k_weight), (T, Hq, k.shape[1], D, P, R)
+            if t.dtype != dtype or t.shape != (D,):
+                raise ValueError(f"{n} must be {dtype} [{D}], got {t.dtype} {list(t.shape)}")
+        q_weight, k_weight = _dense(q_weight), _dense(k_weight)
+    elif q_weight is not None or k_weight is not None:
+        raise ValueError("q_weight and k_weight are given together")
+    return dt, q, k, v, (cos, sin, positions, q_weight, k_weight), (T, Hq, shape[1], D, P, R)
 
 
 def head_norm_rope(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor | None, cos: torch.Tensor | None,
@@ -1119,11 +1159,13 @@ def head_norm_rope(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor | None, cos
     norm); cos, sin float32 [P, R / 2]: token t's columns i and i + R / 2 of q and k (i < R / 2) are
     turned by row ``positions[t]`` (int32).  v (may be None) is normed without a weight.  A position
     that the tables do not have makes its token's q and k NaN."""
-    dev, dt, (q, k, v), rot, sizes = _rope_args(q, k, v, cos, sin, positions, q_weight, k_weight, True)
-    out = tuple(None if t is None else torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
-    _call("w4a16_head_norm_rope", dev, load().w4a16_head_norm_rope, *_head_args(q), *_head_args(k), *_head_args(v),
-          *[_ptr(t) for t in rot], *[_ptr(t) for t in out], dt, *sizes, float(eps))
-    return out
+    index = _gpu_of(q, k, v, cos, sin, positions, q_weight, k_weight)
+    dt, q, k, v, rot, sizes = _rope_args(q, k, v, cos, sin, positions, q_weight, k_weight, True)
+    yq, yk = _dense_like(q), _dense_like(k)
+    yv = None if v is None else _dense_like(v)
+    _launch("w4a16_head_norm_rope", index, load().w4a16_head_norm_rope, *_head_args(q), *_head_args(k),
+            *_head_args(v), *map(_ptr, rot), yq.data_ptr(), yk.data_ptr(), _ptr(yv), dt, *sizes, eps)
+    return yq, yk, yv
 
 
 def head_norm_rope_backward(dq: torch.Tensor, dk: torch.Tensor, dv: torch.Tensor | None, q: torch.Tensor,
@@ -1133,38 +1175,44 @@ def head_norm_rope_backward(dq: torch.Tensor, dk: torch.Tensor, dv: torch.Tensor
     """(dq, dk, dv, dq_weight, dk_weight) of ``head_norm_rope`` for the gradients of its outputs.  The
     weights' are None without weights and where ``weights`` is False; dv is None without v.  The sums
     over the rows are taken in fp32, in an order set by the shapes."""
-    dev, dt, (q, k, v), rot, sizes = _rope_args(q, k, v, cos, sin, positions, q_weight, k_weight, True)
+    index = _gpu_of(q, k, v, cos, sin, positions, q_weight, k_weight, dq, dk, dv)
+    dt, q, k, v, rot, sizes = _rope_args(q, k, v, cos, sin, positions, q_weight, k_weight, True)
     if (dv is None) != (v is None):
         raise ValueError("dv is given with v")
-    grads = []
     for t, x, n in ((dq, q, "dq"), (dk, k, "dk"), (dv, v, "dv")):
         if t is not None and (t.shape != x.shape or t.dtype != x.dtype):
             raise ValueError(f"{n} must be {x.dtype} {list(x.shape)}, got {t.dtype} {list(t.shape)}")
-        grads.append(None if t is None else _aligned(t.contiguous()))
-    _require_gpu(q, *grads)
-    out = [None if t is None else torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v)]
-    dw = [None, None]
+    dq, dk, dv = _dense(dq), _dense(dk), None if dv is None else _dense(dv)
+    xq, xk = torch.empty_like(dq), torch.empty_like(dk)
+    xv = None if dv is None else torch.empty_like(dv)
+    wq = wk = ws = None
     nbytes, lib = 0, load()
     if weights and q_weight is not None:
-        dw = [torch.empty_like(t) for t in rot[3:]]
+        wq, wk = torch.empty_like(rot[3]), torch.empty_like(rot[4])
         nbytes = lib.w4a16_head_norm_rope_backward_workspace_bytes(*sizes[:4])
-    ws = _workspace(nbytes, dev)
-    _call("w4a16_head_norm_rope_backward", dev, lib.w4a16_head_norm_rope_backward, *[_ptr(t) for t in grads],
-          *_head_args(q), *_head_args(k), *_head_args(v), *[_ptr(t) for t in rot], *[_ptr(t) for t in out],
-          *[_ptr(t) for t in dw], dt, *sizes, float(eps), _ptr(ws), nbytes)
-    return (*out, *dw)
+        ws = q.new_empty(nbytes, dtype=torch.uint8)
+    _launch("w4a16_head_norm_rope_backward", index, lib.w4a16_head_norm_rope_backward, dq.data_ptr(), dk.data_ptr(),
+            _ptr(dv), *_head_args(q), *_head_args(k), *_head_args(v), *map(_ptr, rot), xq.data_ptr(), xk.data_ptr(),
+            _ptr(xv), _ptr(wq), _ptr(wk), dt, *sizes, eps, _ptr(ws), nbytes)
+    return xq, xk, xv, wq, wk
 
 
-def _cache(k_cache: torch.Tensor, v_cache: torch.Tensor, like: torch.Tensor):
-    """The sizes of a paged cache [pages, Hk, page size, D]; every page is dense."""
+def _cache_args(k_cache: torch.Tensor, v_cache: torch.Tensor, dtype: torch.dtype, D: int):
+    """(the pointers and bytes between pages of a paged cache [pages, Hk, page size, D], its sizes);
+    every page is dense."""
+    shape = k_cache.shape
+    if len(shape) != 4 or shape[3] != D or v_cache.shape != shape or k_cache.dtype != dtype or v_cache.dtype != dtype:
+        raise ValueError(f"k_cache and v_cache must be {dtype} [pages, heads, page size, {D}], got {k_cache.dtype} "
+                         f"{list(shape)} and {v_cache.dtype} {list(v_cache.shape)}")
+    pages, H, page, _ = shape
+    args = []
     for t, n in ((k_cache, "k_cache"), (v_cache, "v_cache")):
-        if t.dtype != like.dtype or t.dim() != 4 or t.shape != k_cache.shape or t.shape[3] != like.shape[2]:
-            raise ValueError(f"{n} must be {like.dtype} [pages, heads, page size, {like.shape[2]}], got {t.dtype} "
-                             f"{list(t.shape)}")
-        _, H, page, D = t.shape
-        if t.stride()[1:] != (page * D, D, 1) or t.data_ptr() % 16 or t.stride(0) % 8:
+        a, b, c, d = t.stride()
+        p = t.data_ptr()
+        if b != page * D or c != D or d != 1 or (p | 2 * a) & 15:
             raise ValueError(f"{n} must have dense pages at multiples of 16 bytes, got strides {t.stride()}")
-    return k_cache.shape
+        args += (p, a)
+    return args, pages, H, page
 
 
 def append_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor | None, sin: torch.Tensor | None,
@@ -1177,49 +1225,50 @@ def append_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tens
     padding token's) is not written; two tokens of a call must not share one."""
     if v is None:
         raise ValueError("v must be given")
-    dev, dt, (q, k, v), rot, sizes = _rope_args(q, k, v, cos, sin, positions, q_weight, k_weight, False)
-    _require_gpu(q, slots, k_cache, v_cache)
-    slots = _index(slots, "slots", (sizes[0],))
-    pages, H, page, _ = _cache(k_cache, v_cache, q)
+    index = _gpu_of(q, k, v, cos, sin, positions, q_weight, k_weight, slots, k_cache, v_cache)
+    dt, q, k, v, rot, sizes = _rope_args(q, k, v, cos, sin, positions, q_weight, k_weight, False)
+    slots = _index(slots, "slots", sizes[0])
+    cache, pages, H, page = _cache_args(k_cache, v_cache, q.dtype, sizes[3])
     if H != sizes[2]:
         raise ValueError(f"the cache has {H} heads, k {sizes[2]}")
-    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    _call("w4a16_append_kv", dev, load().w4a16_append_kv, *_head_args(q), *_head_args(k), *_head_args(v),
-          _ptr(rot[0]), _ptr(rot[1]), _ptr(rot[2]), _ptr(slots), _ptr(rot[3]), _ptr(rot[4]), _ptr(out),
-          _ptr(k_cache), k_cache.stride(0), _ptr(v_cache), v_cache.stride(0), dt, int(v_norm), *sizes, pages, page,
-          float(eps))
+    out = _dense_like(q)
+    cos, sin, positions, q_weight, k_weight = rot
+    _launch("w4a16_append_kv", index, load().w4a16_append_kv, *_head_args(q), *_head_args(k), *_head_args(v),
+            _ptr(cos), _ptr(sin), positions.data_ptr(), slots.data_ptr(), _ptr(q_weight), _ptr(k_weight),
+            out.data_ptr(), *cache, dt, bool(v_norm), *sizes, pages, page, eps)
     return out
 
 
-def _attention_args(q, k, v, cu_q, cu_k, scale, causal, window):
-    dev = _require_gpu(q, k, v, cu_q, cu_k)
-    dt = _head_type(q, "q", False)
-    q = _heads(q, "q")
-    D = q.shape[2]
-    kv = []
-    for t, n in ((k, "k"), (v, "v")):
-        if t.dtype != q.dtype or t.dim() != 3 or t.shape[2] != D or t.shape != k.shape:
-            raise ValueError(f"{n} must be {q.dtype} [tokens, heads, {D}], got {t.dtype} {list(t.shape)}")
-        kv.append(_heads(t, n))
-    k, v = kv
-    if k.shape[1] == 0 or q.shape[1] % k.shape[1]:
-        raise ValueError(f"the query heads must be a multiple of the key-value heads, got {q.shape[1]} and "
-                         f"{k.shape[1]}")
+def _group(Hq: int, Hk: int, D: int) -> None:
+    if Hk == 0 or Hq == 0 or Hq % Hk:
+        raise ValueError(f"the query heads must be a multiple of the key-value heads, got {Hq} and {Hk}")
     if D not in (64, 128, 256, 512):
         raise ValueError(f"the head size must be 64, 128, 256 or 512, got {D}")
+
+
+def _attention_args(q, k, v, cu_q, cu_k, scale, causal, window):
+    dt = _head_type(q, "q", False)
+    q, k, v = _heads(q, "q"), _heads(k, "k"), _heads(v, "v")
+    Tq, Hq, D = q.shape
+    Tk, Hk, _ = shape = k.shape
+    if k.dtype != q.dtype or v.dtype != q.dtype or shape[2] != D or v.shape != shape:
+        raise ValueError(f"k and v must be {q.dtype} [tokens, heads, {D}], got {k.dtype} {list(shape)} and {v.dtype} "
+                         f"{list(v.shape)}")
+    _group(Hq, Hk, D)
     if cu_q.dim() != 1 or cu_q.numel() == 0:
         raise ValueError(f"cu_q must be int32 [sequences + 1], got {list(cu_q.shape)}")
-    cu_q = _index(cu_q, "cu_q", cu_q.shape)
+    n = cu_q.shape[0]
+    cu_q = _index(cu_q, "cu_q", n)
     if cu_k is None:
-        if k.shape[0] != q.shape[0]:
+        if Tk != Tq:
             raise ValueError("without cu_k the queries and keys are of the same tokens")
         cu_k = cu_q
-    cu_k = _index(cu_k, "cu_k", cu_q.shape)
+    else:
+        cu_k = _index(cu_k, "cu_k", n)
     if window and not causal:
         raise ValueError("a window needs a causal mask")
-    sizes = (cu_q.numel() - 1, q.shape[0], k.shape[0], q.shape[1], k.shape[1], D,
-             float(D ** -0.5 if scale is None else scale), int(causal), int(window))
-    return dev, dt, (q, k, v), (cu_q, cu_k), sizes
+    sizes = (n - 1, Tq, Tk, Hq, Hk, D, D ** -0.5 if scale is None else scale, bool(causal), window)
+    return dt, q, k, v, cu_q, cu_k, sizes
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, cu_k: torch.Tensor | None = None,
@@ -1232,11 +1281,12 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Ten
     ``cu_k`` (int32, from 0 on; None: the same); its last query stands at its last key.  Causal: a
     query sees the keys up to where it stands, with ``window`` the last so many of them.  A query
     that sees none, and rows behind the last sequence, are zero.  ``scale`` is D^-1/2 if None."""
-    dev, dt, (q, k, v), cu, sizes = _attention_args(q, k, v, cu_q, cu_k, scale, causal, window)
-    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=dev) if return_lse else None
-    _call("w4a16_attention", dev, load().w4a16_attention, *_head_args(q), *_head_args(k), *_head_args(v),
-          *[_ptr(t) for t in cu], _ptr(out), _ptr(lse), dt, *sizes)
+    index = _gpu_of(q, k, v, cu_q, cu_k)
+    dt, q, k, v, cu_q, cu_k, sizes = _attention_args(q, k, v, cu_q, cu_k, scale, causal, window)
+    out = _dense_like(q)
+    lse = q.new_empty((sizes[3], sizes[1]), dtype=torch.float32) if return_lse else None
+    _launch("w4a16_attention", index, load().w4a16_attention, *_head_args(q), *_head_args(k), *_head_args(v),
+            cu_q.data_ptr(), cu_k.data_ptr(), out.data_ptr(), _ptr(lse), dt, *sizes)
     return (out, lse) if return_lse else out
 
 
@@ -1245,25 +1295,25 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
                        scale: float | None = None, causal: bool = True, window: int = 0, needs=(True, True, True)):
     """(dq, dk, dv) of ``attention`` for the gradient ``dout`` of its output and the ``out`` and ``lse`` of
     that forward call.  ``needs``: which of the three are wanted; the others are None."""
-    dev, dt, (q, k, v), cu, sizes = _attention_args(q, k, v, cu_q, cu_k, scale, causal, window)
+    index = _gpu_of(q, k, v, cu_q, cu_k, dout, out, lse)
+    dt, q, k, v, cu_q, cu_k, sizes = _attention_args(q, k, v, cu_q, cu_k, scale, causal, window)
     for t, n in ((dout, "dout"), (out, "out")):
         if t.shape != q.shape or t.dtype != q.dtype:
             raise ValueError(f"{n} must be {q.dtype} {list(q.shape)}, got {t.dtype} {list(t.shape)}")
-    if lse.shape != (q.shape[1], q.shape[0]) or lse.dtype != torch.float32:
-        raise ValueError(f"lse must be float32 {[q.shape[1], q.shape[0]]}, got {lse.dtype} {list(lse.shape)}")
-    _require_gpu(q, dout, out, lse)
+    Tq, Hq = sizes[1], sizes[3]
+    if lse.shape != (Hq, Tq) or lse.dtype != torch.float32:
+        raise ValueError(f"lse must be float32 {[Hq, Tq]}, got {lse.dtype} {list(lse.shape)}")
     if len(needs) != 3:
         raise ValueError("needs must say for each of dq, dk and dv whether it is wanted")
-    dout, out, lse = _aligned(dout.contiguous()), _aligned(out.contiguous()), lse.contiguous()
-    dense = lambda t: torch.empty(t.shape, dtype=t.dtype, device=dev)
-    dq = dense(q) if needs[0] else None
-    dk, dv = (dense(k), dense(v)) if needs[1] or needs[2] else (None, None)
+    dout, out, lse = _dense(dout), _dense(out), lse.contiguous()
+    dq = torch.empty_like(dout) if needs[0] else None
+    dk, dv = (_dense_like(k), _dense_like(v)) if needs[1] or needs[2] else (None, None)
     lib = load()
-    nbytes = lib.w4a16_attention_backward_workspace_bytes(q.shape[0], q.shape[1])
-    ws = _workspace(nbytes, dev)
-    _call("w4a16_attention_backward", dev, lib.w4a16_attention_backward, _ptr(dout), *_head_args(q), *_head_args(k),
-          *_head_args(v), _ptr(out), _ptr(lse), *[_ptr(t) for t in cu], _ptr(dq), _ptr(dk), _ptr(dv), dt, *sizes,
-          _ptr(ws), nbytes)
+    nbytes = lib.w4a16_attention_backward_workspace_bytes(Tq, Hq)
+    ws = q.new_empty(nbytes, dtype=torch.uint8)
+    _launch("w4a16_attention_backward", index, lib.w4a16_attention_backward, dout.data_ptr(), *_head_args(q),
+            *_head_args(k), *_head_args(v), out.data_ptr(), lse.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(),
+            _ptr(dq), _ptr(dk), _ptr(dv), dt, *sizes, ws.data_ptr(), nbytes)
     return dq, dk if needs[1] else None, dv if needs[2] else None
 
 
@@ -1276,27 +1326,24 @@ def decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     ``lengths[b]`` of them (both int32), of which the token sees the last ``window`` (0: all).  A
     length of zero gives zeros; a length that the table does not cover, or a page that the cache
     does not have, NaN."""
-    dev = _require_gpu(q, k_cache, v_cache, block_table, lengths)
+    index = _gpu_of(q, k_cache, v_cache, block_table, lengths)
     dt = _head_type(q, "q", False)
     q = _heads(q, "q")
     B, Hq, D = q.shape
-    pages, Hk, page, _ = _cache(k_cache, v_cache, q)
-    if Hk == 0 or Hq % Hk:
-        raise ValueError(f"the query heads must be a multiple of the key-value heads, got {Hq} and {Hk}")
-    if D not in (64, 128, 256, 512):
-        raise ValueError(f"the head size must be 64, 128, 256 or 512, got {D}")
+    cache, pages, Hk, page = _cache_args(k_cache, v_cache, q.dtype, D)
+    _group(Hq, Hk, D)
     if block_table.dim() != 2:
         raise ValueError(f"block_table must be int32 [{B}, pages of a sequence], got {list(block_table.shape)}")
     width = block_table.shape[1]
-    block_table = _index(block_table, "block_table", (B, width))
-    lengths = _index(lengths, "lengths", (B,))
-    out = torch.empty((B, Hq, D), dtype=q.dtype, device=dev)
+    block_table = _index(block_table, "block_table", B, width)
+    lengths = _index(lengths, "lengths", B)
+    out = _dense_like(q)
     lib = load()
     nbytes = lib.w4a16_decode_attention_workspace_bytes(B, Hq, Hk, D, width * page)
-    ws = _workspace(nbytes, dev)
-    _call("w4a16_decode_attention", dev, lib.w4a16_decode_attention, *_head_args(q), _ptr(k_cache), k_cache.stride(0),
-          _ptr(v_cache), v_cache.stride(0), _ptr(block_table), _ptr(lengths), _ptr(out), dt, B, Hq, Hk, D, pages, page,
-          width, float(D ** -0.5 if scale is None else scale), int(window), _ptr(ws), nbytes)
+    ws = q.new_empty(nbytes, dtype=torch.uint8)
+    _launch("w4a16_decode_attention", index, lib.w4a16_decode_attention, *_head_args(q), *cache,
+            block_table.data_ptr(), lengths.data_ptr(), out.data_ptr(), dt, B, Hq, Hk, D, pages, page, width,
+            D ** -0.5 if scale is None else scale, window, ws.data_ptr(), nbytes)
     return out
 
 

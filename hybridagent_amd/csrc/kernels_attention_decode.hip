@@ -64,21 +64,25 @@ __global__ __launch_bounds__(64 * kDaWaves, D == 512 ? 1 : 2) void k_decode_atte
   constexpr int VW = D >= 128 ? 8 : 4;    // columns of a lane's block of values
   constexpr int NB = D / (16 * VW);       // blocks
   constexpr int VD = VW / 2;              // dwords of a block's row
+  constexpr bool kEarly = D < 256;
   __shared__ float sm[kDaWaves][16], sl[kDaWaves][16];
   extern __shared__ __align__(16) float so[];  // [kDaWaves][D * 16]
   const int lane = threadIdx.x & 63, r = lane & 15, c = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int gt = (a.group + 15) / 16;  // tiles of a group's queries
   const int units = a.Hk * gt;
-  const int total = da_before(a, a.B) * units;
-  const int groups = min(a.groups, total);  // each has a step at least
-  if ((int)blockIdx.x >= groups) return;
-  int pos = da_start(blockIdx.x, groups, total);
-  const int end = da_start(blockIdx.x + 1, groups, total);
-  const int begin = pos;
 
-  // the sequence of the first step
-  int b = 0, at = 0;  // at: steps in front of it
+  // the workgroup's steps pos .. end - 1, the sequence of the first, and the steps
+  // `at` in front of that
+  int pos, end, b = 0, at = 0;
+  auto deal = [&](int total) {
+    const int groups = min(a.groups, total);  // each has a step at least
+    if ((int)blockIdx.x >= groups) return false;
+    pos = da_start(blockIdx.x, groups, total);
+    end = da_start(blockIdx.x + 1, groups, total);
+    return true;
+  };
+  if (a.B > 64 && !deal(da_before(a, a.B) * units)) return;
   for (int base = 0; base < a.B; base += 64) {
     const int n = base + lane < a.B ? da_seq(a, base + lane).steps * units : 0;
     int sum = n;
@@ -88,6 +92,7 @@ __global__ __launch_bounds__(64 * kDaWaves, D == 512 ? 1 : 2) void k_decode_atte
       if (lane >= o) sum += v;
     }
     const int all = __builtin_amdgcn_readlane(sum, 63);
+    if (a.B <= 64 && !deal(all)) return;
     if (pos < at + all) {
       const int i = __ffsll((unsigned long long)__ballot(at + sum > pos)) - 1;
       b = base + i;
@@ -96,6 +101,7 @@ __global__ __launch_bounds__(64 * kDaWaves, D == 512 ? 1 : 2) void k_decode_atte
     }
     at += all;
   }
+  const int begin = pos;
 
   while (pos < end) {
     const DaSeq seq = da_seq(a, b);
@@ -104,53 +110,71 @@ __global__ __launch_bounds__(64 * kDaWaves, D == 512 ? 1 : 2) void k_decode_atte
     const int hk = unit / gt, q_first = (unit - hk * gt) * 16, q_n = min(a.group - q_first, 16);
     const int head0 = hk * a.group + q_first;
 
-    u32x4_t qf[D / 32];
-    at_load_row<D / 32>(static_cast<const unsigned char*>(a.q) + (int64_t)(head0 + min(r, q_n - 1)) * a.q_head, b,
-                   a.q_stride, qf);
     const int64_t in_page = (int64_t)hk * (D * 2) << a.page_log2;
     const unsigned char* kp = static_cast<const unsigned char*>(a.kc) + in_page;
     const unsigned char* vp = static_cast<const unsigned char*>(a.vc) + in_page;
     const int32_t* row = a.table + (int64_t)b * a.width;
     const int mask = (1 << a.page_log2) - 1;
+    // A lane's keys are held to the ones that are seen (those beside them may lie
+    // in pages that are another's by now, and hold anything): a group of eight
+    // keys, all of one page, has its page or, with none seen, the nearest's.
+    auto hold = [&](int key) { return min(max(key, seq.first), seq.len - 1); };
+    // the pages of a lane's eight keys as rows of the scores (k) and of the values (v)
+    struct Pages {
+      int k, v;
+    };
+    auto pages = [&](int key0) {
+      return Pages{row[hold(key0 + 8 * (r >> 2)) >> a.page_log2], row[hold(key0 + 8 * c) >> a.page_log2]};
+    };
+    u32x4_t kf[2][D / 32];
+    auto keys = [&](int key0, int page) {
+      const unsigned char* p = kp + (page < 0 || page >= a.pages ? 0 : page) * a.k_page;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) at_load_row<D / 32>(p, hold(key0 + 8 * (r >> 2) + 4 * t + (r & 3)) & mask, D * 2, kf[t]);
+    };
 
-    float m = -1e30f, l = 0.f;
+    // The wavefront's keys of a step are key0 ..; the next ones' pages are read a step
+    // ahead.  kEarly: their rows too, once the scores are done with these (heads of
+    // 256: two wavefronts of a SIMD cover for each other instead, without the room).
+    int key0 = seq.base + s0 * kDaStep + 32 * wave;
+    const int stop = min(seq.len, seq.base + s1 * kDaStep);
+    Pages now{0, 0}, next{0, 0};
+    if (key0 < stop) {
+      now = pages(key0);
+      if (key0 + kDaStep < stop) next = pages(key0 + kDaStep);
+      if (kEarly) keys(key0, now.k);
+    }
+    u32x4_t qf[D / 32];
+    at_load_row<D / 32>(static_cast<const unsigned char*>(a.q) + (int64_t)(head0 + min(r, q_n - 1)) * a.q_head, b,
+                        a.q_stride, qf);
+
+    float m = 0.f, l = 0.f;
     f32x4_t acc[NB][VW];
 #pragma unroll
     for (int j = 0; j < NB; ++j)
 #pragma unroll
       for (int e = 0; e < VW; ++e) acc[j][e] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
-    for (int st = s0; st < s1; ++st) {
-      const int key0 = seq.base + st * kDaStep + 32 * wave;
-      if (key0 >= seq.len) break;
-      // A lane's keys are held to the ones that are seen (those beside them may lie
-      // in pages that are another's by now, and hold anything): a group of eight
-      // keys, all of one page, has its page or, with none seen, the nearest's.
-      auto hold = [&](int key) { return min(max(key, seq.first), seq.len - 1); };
-      int pk = row[hold(key0 + 8 * (r >> 2)) >> a.page_log2], pv = row[hold(key0 + 8 * c) >> a.page_log2];
-      const bool bad = seq.over || pv < 0 || pv >= a.pages;
-      pk = pk < 0 || pk >= a.pages ? 0 : pk;
-      pv = pv < 0 || pv >= a.pages ? 0 : pv;
-      u32x4_t kf[2][D / 32];
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int k = hold(key0 + 8 * (r >> 2) + 4 * t + (r & 3)) & mask;
-        at_load_row<D / 32>(kp + pk * a.k_page, k, D * 2, kf[t]);
-      }
+    for (; key0 < stop; key0 += kDaStep) {
+      if (!kEarly) keys(key0, now.k);
+      const bool bad = seq.over || now.v < 0 || now.v >= a.pages;
       uint32_t vf[NB][8][VD];
+      {
+        const unsigned char* q = vp + (bad ? 0 : now.v) * a.v_page + r * (2 * VW);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const unsigned char* p = vp + pv * a.v_page + (int64_t)(hold(key0 + 8 * c + i) & mask) * (D * 2) + r * (2 * VW);
+        for (int i = 0; i < 8; ++i) {
+          const unsigned char* p = q + (int64_t)(hold(key0 + 8 * c + i) & mask) * (D * 2);
 #pragma unroll
-        for (int j = 0; j < NB; ++j) {
-          if constexpr (VW == 8) {
-            const u32x4_t v = ld16(p + 256 * j);
+          for (int j = 0; j < NB; ++j) {
+            if constexpr (VW == 8) {
+              const u32x4_t v = ld16(p + 256 * j);
 #pragma unroll
-            for (int w = 0; w < 4; ++w) vf[j][i][w] = v[w];
-          } else {
-            const u32x2_t v = *reinterpret_cast<const u32x2_t*>(p);
-            vf[j][i][0] = v.x;
-            vf[j][i][1] = v.y;
+              for (int w = 0; w < 4; ++w) vf[j][i][w] = v[w];
+            } else {
+              const u32x2_t v = *reinterpret_cast<const u32x2_t*>(p);
+              vf[j][i][0] = v.x;
+              vf[j][i][1] = v.y;
+            }
           }
         }
       }
@@ -160,6 +184,13 @@ __global__ __launch_bounds__(64 * kDaWaves, D == 512 ? 1 : 2) void k_decode_atte
         s[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) s[t] = at_mfma<T>(kf[t][i], qf[i], s[t]);
+      }
+      Pages after{0, 0};
+      if (key0 + kDaStep < stop) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (key0 + 2 * kDaStep < stop) after = pages(key0 + 2 * kDaStep);
+        if (kEarly) keys(key0 + kDaStep, next.k);
+        __builtin_amdgcn_sched_barrier(0);
       }
       if (key0 < seq.first || key0 + 32 > seq.len || __any(bad)) {
 #pragma unroll
@@ -172,14 +203,23 @@ __global__ __launch_bounds__(64 * kDaWaves, D == 512 ? 1 : 2) void k_decode_atte
             s[t][i] = key < seq.first || key >= seq.len ? -INFINITY : bad ? NAN : s[t][i];
           }
       }
-      const float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
-                              fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3]))) *
-                        a.scale2;
-      if (__any(top > m + 8.f)) {
-        const float now = fmaxf(m, at_max_over_c(top));
-        const float f = __builtin_amdgcn_exp2f(m - now);
-        m = now;
+      // exponents from the running maximum as it is (as k_attention's)
+      float top = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s[t][i] = __builtin_fmaf(s[t][i], a.scale2, -m);
+          top = fmaxf(top, s[t][i]);
+        }
+      if (__any(top > (l == 0.f ? -INFINITY : 8.f))) {
+        const float t = at_max_over_c(top);
+        const float up = t > (at_sum_over_c(l) == 0.f ? -INFINITY : 0.f) ? t : 0.f;
+        const float f = __builtin_amdgcn_exp2f(-up);
+        m += up;
         l *= f;
+        s[0] -= up;
+        s[1] -= up;
 #pragma unroll
         for (int j = 0; j < NB; ++j)
 #pragma unroll
@@ -189,7 +229,7 @@ __global__ __launch_bounds__(64 * kDaWaves, D == 512 ? 1 : 2) void k_decode_atte
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          s[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], a.scale2, -m));
+          s[t][i] = __builtin_amdgcn_exp2f(s[t][i]);
           l += s[t][i];
         }
       const u32x4_t p = at_pack8<T>(s[0], s[1]);
@@ -204,10 +244,13 @@ __global__ __launch_bounds__(64 * kDaWaves, D == 512 ? 1 : 2) void k_decode_atte
           for (int w = 0; w < 4; ++w) v[w] = __builtin_amdgcn_perm(vf[j][2 * w + 1][e / 2], vf[j][2 * w][e / 2], sel);
           acc[j][e] = at_mfma<T>(v, p, acc[j][e]);
         }
+      now = next;
+      next = after;
     }
 
-    // the wavefronts' sums, joined
+    // the wavefronts' sums, joined (a wavefront without keys has no maximum)
     l = at_sum_over_c(l);
+    if (l == 0.f) m = -INFINITY;
     if (c == 0) {
       sm[wave][r] = m;
       sl[wave][r] = l;
@@ -216,6 +259,7 @@ __global__ __launch_bounds__(64 * kDaWaves, D == 512 ? 1 : 2) void k_decode_atte
     float top = sm[0][r];
 #pragma unroll
     for (int w = 1; w < kDaWaves; ++w) top = fmaxf(top, sm[w][r]);
+    if (top == -INFINITY) top = 0.f;
     float sum = 0.f;
 #pragma unroll
     for (int w = 0; w < kDaWaves; ++w) sum += sl[w][r] * __builtin_amdgcn_exp2f(sm[w][r] - top);
@@ -293,9 +337,10 @@ __global__ __launch_bounds__(256) void k_decode_join(DecodeAttnArgs a) {
   // the first piece is its workgroup's second where the unit does not start with it
   const bool opens = da_start(g0, groups, total) >= first;
   auto piece = [&](int g) { return a.part + (int64_t)(2 * g + (g == g0 && !opens ? 1 : 0)) * (16 * (D + 2)); };
-  float top = -1e30f;
+  float top = -INFINITY;
   for (int g = g0 + lane; g <= g1; g += 64) top = fmaxf(top, piece(g)[16 * D + q]);
   top = wave_max_f32(top);
+  if (top == -INFINITY) top = 0.f;
   const int at = threadIdx.x / L, d = 4 * (threadIdx.x % L);
   f32x4_t v = {0.f, 0.f, 0.f, 0.f};
   float l = 0.f;

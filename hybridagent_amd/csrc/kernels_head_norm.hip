@@ -9,11 +9,11 @@
 // backward, with g = dy turned back by the same angles and t = g w:
 //   dx = r (t - x r mean(t x r)),  dw = sum over rows of g x r
 //
-// Bound: memory (one read and one write of each row).  L lanes have a row, 8
-// elements each, so that every load is 16 bytes a lane and whole lines; a
-// wavefront takes kHnRows groups of 64 / L rows of one token, loaded together,
-// and reads its token's angles once for them.  The two halves of a rotated pair
-// meet through the wavefront's own LDS rows.
+// Bound: memory (one read and one write of each row).  L lanes have a row, each
+// two pieces of four elements: of the turned columns piece i and its partner R / 2
+// further, of the others neighbours, so that a pair never leaves its lane and an
+// angle is read once.  A wavefront takes kHnRows groups of 64 / L rows of one
+// token, loaded together, and its token's angles once for them.
 #include <type_traits>
 
 #include "attention.hpp"
@@ -23,7 +23,7 @@ namespace w4a16 {
 namespace {
 
 constexpr int kHnRows = 4;
-constexpr int kHnBackBlocks = 512;
+constexpr int kHnBackBlocks = 1024;
 
 // the number of lanes of a row
 inline int hn_lanes(int64_t D) { return D <= 64 ? 8 : D <= 128 ? 16 : D <= 256 ? 32 : 64; }
@@ -32,97 +32,100 @@ inline int64_t hn_tasks(int64_t T, int64_t heads, int64_t D) {
   return T * ((heads + per - 1) / per);
 }
 
-// eight elements
+// a lane's elements of a row: pieces at a and b
+struct HnPlace {
+  int a, b;
+  bool in, turned;
+};
+__device__ __forceinline__ HnPlace hn_place(const HeadNormArgs& g, int j) {
+  HnPlace p;
+  p.turned = 8 * j < g.R;
+  p.a = p.turned ? 4 * j : 8 * j;
+  p.b = p.turned ? 4 * j + (g.R >> 1) : 8 * j + 4;
+  p.in = 8 * j < g.D;
+  return p;
+}
 template <typename T>
 struct Hn8 {
-  static constexpr int kWords = 2 * sizeof(T);
-  uint32_t w[kWords];
-  __device__ __forceinline__ void load(const void* p) {
-#pragma unroll
-    for (int i = 0; i < kWords; i += 4) {
-      const u32x4_t v = ld16(static_cast<const uint32_t*>(p) + i);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) w[i + j] = v[j];
-    }
+  static constexpr int kWords = sizeof(T);  // of a piece
+  typedef __attribute__((ext_vector_type(kWords))) uint32_t piece_t;
+  piece_t w[2];
+  __device__ __forceinline__ void load(const void* row, const HnPlace& p) {
+    w[0] = *reinterpret_cast<const piece_t*>(static_cast<const T*>(row) + p.a);
+    w[1] = *reinterpret_cast<const piece_t*>(static_cast<const T*>(row) + p.b);
   }
   __device__ __forceinline__ void zero() {
 #pragma unroll
-    for (int i = 0; i < kWords; ++i) w[i] = 0;
+    for (int i = 0; i < kWords; ++i) w[0][i] = w[1][i] = 0;
   }
   __device__ __forceinline__ float get(int i) const {
     if constexpr (sizeof(T) == 4)
-      return __uint_as_float(w[i]);
+      return __uint_as_float(w[i >> 2][i & 3]);
     else
-      return i & 1 ? at_hi<T>(w[i / 2]) : at_lo<T>(w[i / 2]);
+      return i & 1 ? at_hi<T>(w[i >> 2][(i & 3) >> 1]) : at_lo<T>(w[i >> 2][(i & 3) >> 1]);
   }
 };
 template <typename T>
-__device__ __forceinline__ void hn_store(void* p, const float (&v)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    st16(p, u32x4_t{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])});
-    st16(static_cast<char*>(p) + 16,
-         u32x4_t{__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7])});
-  } else {
-    st16(p, u32x4_t{at_pack2<T>(v[0], v[1]), at_pack2<T>(v[2], v[3]), at_pack2<T>(v[4], v[5]), at_pack2<T>(v[6], v[7])});
+__device__ __forceinline__ void hn_store(void* row, const HnPlace& p, const float (&v)[8]) {
+  typedef typename Hn8<T>::piece_t piece_t;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const float* x = v + 4 * h;
+    piece_t w;
+    if constexpr (sizeof(T) == 4)
+      w = piece_t{__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])};
+    else
+      w = piece_t{at_pack2<T>(x[0], x[1]), at_pack2<T>(x[2], x[3])};
+    *reinterpret_cast<piece_t*>(static_cast<T*>(row) + (h ? p.b : p.a)) = w;
   }
 }
 
+// over the L lanes of a row, each gets the sum
 template <int L>
 __device__ __forceinline__ float hn_sum(float v) {
-#pragma unroll
-  for (int o = 1; o < L; o <<= 1) v += __shfl_xor(v, o);
+  auto add = [](float x, int y) { return x + __int_as_float(y); };
+  auto bits = [](float x) { return __float_as_int(x); };
+  v = add(v, __builtin_amdgcn_update_dpp(0, bits(v), 0xB1, 0xF, 0xF, false));   // quad [1,0,3,2]
+  v = add(v, __builtin_amdgcn_update_dpp(0, bits(v), 0x4E, 0xF, 0xF, false));   // quad [2,3,0,1]
+  v = add(v, __builtin_amdgcn_update_dpp(0, bits(v), 0x141, 0xF, 0xF, false));  // row_half_mirror
+  if constexpr (L >= 16) v = add(v, __builtin_amdgcn_update_dpp(0, bits(v), 0x140, 0xF, 0xF, false));  // row_mirror
+  if constexpr (L >= 32) {
+    const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+  }
+  if constexpr (L >= 64) {
+    const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+  }
   return v;
 }
 
-// A lane's angles for elements 8 j .. 8 j + 7 of a rotated row, in two groups of
-// four: y = cos u + sin u', u' the element `to` further (sin with its sign)
+// a lane's angles; not turned: cos 1, sin 0
 struct HnTurn {
-  float cos[8], sin[8];
-  int to[2];
+  f32x4_t cos, sin;
 };
-// dir: 1, or -1 to turn back.  h = R / 2, a multiple of four.
-__device__ __forceinline__ HnTurn hn_turn(const HeadNormArgs& a, int t, int j, float dir) {
+// dir: 1, or -1 to turn back.  A position that the tables do not have: not a number.
+__device__ __forceinline__ HnTurn hn_turn(const HeadNormArgs& g, int t, const HnPlace& p, float dir) {
+  const int pos = g.pos[t];
+  const bool bad = pos < 0 || pos >= g.P;
   HnTurn n;
-  const int h = a.R >> 1, p = a.pos[t];
-  const bool bad = p < 0 || p >= a.P;
-#pragma unroll
-  for (int g = 0; g < 2; ++g) {
-    const int e = 8 * j + 4 * g;
-    const bool low = e < h, turned = e < a.R;
-    n.to[g] = low && turned ? h : turned ? -h : 0;
-    f32x4_t c = {1.f, 1.f, 1.f, 1.f}, s = {0.f, 0.f, 0.f, 0.f};
-    if (turned && !bad) {
-      const int64_t at = (int64_t)p * h + (low ? e : e - h);
-      c = *reinterpret_cast<const f32x4_t*>(a.cos + at);
-      s = *reinterpret_cast<const f32x4_t*>(a.sin + at) * (low ? -dir : dir);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      // a position that the tables do not have: not a number
-      n.cos[4 * g + i] = bad ? NAN : c[i];
-      n.sin[4 * g + i] = s[i];
-    }
+  n.cos = f32x4_t{1.f, 1.f, 1.f, 1.f};
+  n.sin = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  if (p.turned && !bad) {
+    const int64_t at = (int64_t)pos * (g.R >> 1) + p.a;
+    n.cos = *reinterpret_cast<const f32x4_t*>(g.cos + at);
+    n.sin = *reinterpret_cast<const f32x4_t*>(g.sin + at) * dir;
   }
+  if (bad) n.cos = n.sin = f32x4_t{NAN, NAN, NAN, NAN};
   return n;
 }
-// u turned, through the row's LDS place (of this wavefront alone)
-__device__ __forceinline__ void hn_rotate(const HnTurn& n, float* row, int j, float (&u)[8]) {
-  float* p = row + 8 * j;
+__device__ __forceinline__ void hn_rotate(const HnTurn& n, float (&u)[8]) {
 #pragma unroll
-  for (int g = 0; g < 2; ++g)
-    *reinterpret_cast<f32x4_t*>(p + 4 * g) = f32x4_t{u[4 * g], u[4 * g + 1], u[4 * g + 2], u[4 * g + 3]};
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-#pragma unroll
-  for (int g = 0; g < 2; ++g) {
-    const f32x4_t v = *reinterpret_cast<const f32x4_t*>(p + 4 * g + n.to[g]);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) u[4 * g + i] = u[4 * g + i] * n.cos[4 * g + i] + v[i] * n.sin[4 * g + i];
+  for (int i = 0; i < 4; ++i) {
+    const float x = u[i], y = u[4 + i];
+    u[i] = x * n.cos[i] - y * n.sin[i];
+    u[4 + i] = y * n.cos[i] + x * n.sin[i];
   }
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
 // head h of token t: its row in the inputs, what it is (0: query, 1: key, 2:
@@ -147,14 +150,14 @@ __device__ __forceinline__ HnRow hn_row(const HeadNormArgs& a, int t, int h) {
 template <typename T, int L, bool PAGED>
 __global__ __launch_bounds__(256) void k_head_norm(HeadNormArgs a, int chunks) {
   constexpr int RP = 64 / L;
-  __shared__ __align__(16) float rows[4][64 * 8];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane % L, sub = lane / L;
+  const int lane = threadIdx.x & 63, j = lane % L, sub = lane / L;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t task = (int64_t)blockIdx.x * 4 + wave;
   const int t = (int)(task / chunks);
   if (t >= a.T) return;
   const int heads = a.Hq + a.Hk + (a.v != nullptr ? a.Hk : 0);
   const int h0 = (int)(task - (int64_t)t * chunks) * (kHnRows * RP) + sub;
-  const bool in = 8 * j < a.D;
+  const HnPlace at = hn_place(a, j);
 
   HnRow row[kHnRows];
   Hn8<T> x[kHnRows];
@@ -162,16 +165,15 @@ __global__ __launch_bounds__(256) void k_head_norm(HeadNormArgs a, int chunks) {
   for (int i = 0; i < kHnRows; ++i) {
     const int h = h0 + RP * i;
     row[i] = hn_row(a, t, min(h, heads - 1));
-    if (in && h < heads)
-      x[i].load(row[i].x + 8 * j * sizeof(T));
+    if (at.in && h < heads)
+      x[i].load(row[i].x, at);
     else
       x[i].zero();
   }
-  const HnTurn turn = hn_turn(a, t, j, 1.f);
+  const HnTurn turn = hn_turn(a, t, at, 1.f);
   const int slot = PAGED ? a.slots[t] : 0;
   const int page = PAGED ? slot / a.page : 0;
   const bool kept = PAGED ? slot >= 0 && slot < a.slots_n : true;
-  float* place = rows[wave] + sub * (L * 8);
 #pragma unroll
   for (int i = 0; i < kHnRows; ++i) {
     const int h = h0 + RP * i, kind = row[i].kind;
@@ -185,27 +187,23 @@ __global__ __launch_bounds__(256) void k_head_norm(HeadNormArgs a, int chunks) {
     sum = hn_sum<L>(sum);
     const bool norm = kind == 2 ? a.v_norm : w != nullptr;
     const float f = norm ? __frsqrt_rn(sum / (float)a.D + a.eps) : 1.f;
-    Hn8<T> wv;
-    if (w != nullptr && in) wv.load(static_cast<const unsigned char*>(w) + 8 * j * sizeof(T));
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      u[e] *= f;
-      if (w != nullptr && in) u[e] *= wv.get(e);
+    for (int e = 0; e < 8; ++e) u[e] *= f;
+    if (w != nullptr && at.in) {
+      Hn8<T> wv;
+      wv.load(w, at);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) u[e] *= wv.get(e);
     }
-    float y[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = u[e];
-    hn_rotate(turn, place, j, y);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = kind == 2 ? u[e] : y[e];
-    if (!in || h >= heads) continue;
+    if (kind != 2) hn_rotate(turn, u);
+    if (!at.in || h >= heads) continue;
     const int n = row[i].head;
     if (!PAGED || kind == 0) {
       void* o = kind == 0 ? a.yq : kind == 1 ? a.yk : a.yv;
-      hn_store<T>(static_cast<T*>(o) + ((int64_t)t * (kind == 0 ? a.Hq : a.Hk) + n) * a.D + 8 * j, y);
+      hn_store<T>(static_cast<T*>(o) + ((int64_t)t * (kind == 0 ? a.Hq : a.Hk) + n) * a.D, at, u);
     } else if (kept) {
       unsigned char* o = static_cast<unsigned char*>(kind == 1 ? a.yk : a.yv) + page * (kind == 1 ? a.k_page : a.v_page);
-      hn_store<T>(o + (((int64_t)n * a.page + (slot - page * a.page)) * a.D + 8 * j) * sizeof(T), y);
+      hn_store<T>(o + ((int64_t)n * a.page + (slot - page * a.page)) * a.D * sizeof(T), at, u);
     }
   }
 }
@@ -213,21 +211,20 @@ __global__ __launch_bounds__(256) void k_head_norm(HeadNormArgs a, int chunks) {
 template <typename T, int L>
 __global__ __launch_bounds__(256) void k_head_norm_backward(HeadNormArgs a, int chunks, int64_t tasks) {
   constexpr int RP = 64 / L;
-  __shared__ __align__(16) float rows[4][64 * 8];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane % L, sub = lane / L;
+  const int lane = threadIdx.x & 63, j = lane % L, sub = lane / L;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int heads = a.Hq + a.Hk + (a.v != nullptr ? a.Hk : 0);
-  const bool in = 8 * j < a.D;
+  const HnPlace at = hn_place(a, j);
   const float over = 1.0f / (float)a.D;
-  float* place = rows[wave] + sub * (L * 8);
   float dw[2][8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) dw[0][e] = dw[1][e] = 0.f;
   Hn8<T> wq, wk;
   wq.zero();
   wk.zero();
-  if (a.qw != nullptr && in) {
-    wq.load(static_cast<const T*>(a.qw) + 8 * j);
-    wk.load(static_cast<const T*>(a.kw) + 8 * j);
+  if (a.qw != nullptr && at.in) {
+    wq.load(a.qw, at);
+    wk.load(a.kw, at);
   }
 
   for (int64_t task = (int64_t)blockIdx.x * 4 + wave; task < tasks; task += (int64_t)gridDim.x * 4) {
@@ -239,51 +236,49 @@ __global__ __launch_bounds__(256) void k_head_norm_backward(HeadNormArgs a, int 
       const int h = h0 + RP * i;
       const HnRow row = hn_row(a, t, min(h, heads - 1));
       const void* d = row.kind == 0 ? a.dq : row.kind == 1 ? a.dk : a.dv;
-      const int64_t at = ((int64_t)t * (row.kind == 0 ? a.Hq : a.Hk) + row.head) * a.D + 8 * j;
-      if (in && h < heads) {
-        x[i].load(row.x + 8 * j * sizeof(T));
-        dy[i].load(static_cast<const T*>(d) + at);
+      if (at.in && h < heads) {
+        x[i].load(row.x, at);
+        dy[i].load(static_cast<const T*>(d) + ((int64_t)t * (row.kind == 0 ? a.Hq : a.Hk) + row.head) * a.D, at);
       } else {
         x[i].zero();
         dy[i].zero();
       }
     }
-    const HnTurn turn = hn_turn(a, t, j, -1.f);
+    const HnTurn turn = hn_turn(a, t, at, -1.f);
 #pragma unroll
     for (int i = 0; i < kHnRows; ++i) {
       const int h = h0 + RP * i;
       const HnRow row = hn_row(a, t, min(h, heads - 1));
       const int kind = row.kind;
       const bool norm = kind == 2 || a.qw != nullptr;
-      float g[8], u[8], sum = 0.f;
+      float g[8], xh[8], sum = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float v = x[i].get(e);
-        sum = __builtin_fmaf(v, v, sum);
-        u[e] = g[e] = dy[i].get(e);
+        xh[e] = x[i].get(e);
+        sum = __builtin_fmaf(xh[e], xh[e], sum);
+        g[e] = dy[i].get(e);
       }
-      sum = hn_sum<L>(sum);
-      hn_rotate(turn, place, j, u);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) g[e] = kind == 2 ? g[e] : u[e];
-      const float f = __frsqrt_rn(sum * over + a.eps);
+      const float f = __frsqrt_rn(hn_sum<L>(sum) * over + a.eps);
+      if (kind != 2) hn_rotate(turn, g);
       float dot = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float xh = x[i].get(e) * f;
-        if (h < heads && in) {
-          dw[0][e] += kind == 0 ? g[e] * xh : 0.f;
-          dw[1][e] += kind == 1 ? g[e] * xh : 0.f;
+        xh[e] *= f;
+        if (h < heads && at.in) {
+          dw[0][e] += kind == 0 ? g[e] * xh[e] : 0.f;
+          dw[1][e] += kind == 1 ? g[e] * xh[e] : 0.f;
         }
-        u[e] = kind == 2 ? g[e] : g[e] * (kind == 0 ? wq.get(e) : wk.get(e));
-        dot = __builtin_fmaf(u[e], xh, dot);
+        if (norm && kind != 2) g[e] *= kind == 0 ? wq.get(e) : wk.get(e);
+        dot = __builtin_fmaf(g[e], xh[e], dot);
       }
       dot = hn_sum<L>(dot) * over;
+      if (norm) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) u[e] = norm ? f * (u[e] - x[i].get(e) * f * dot) : g[e];
-      if (!in || h >= heads) continue;
+        for (int e = 0; e < 8; ++e) g[e] = f * (g[e] - xh[e] * dot);
+      }
+      if (!at.in || h >= heads) continue;
       void* o = kind == 0 ? a.yq : kind == 1 ? a.yk : a.yv;
-      hn_store<T>(static_cast<T*>(o) + ((int64_t)t * (kind == 0 ? a.Hq : a.Hk) + row.head) * a.D + 8 * j, u);
+      hn_store<T>(static_cast<T*>(o) + ((int64_t)t * (kind == 0 ? a.Hq : a.Hk) + row.head) * a.D, at, g);
     }
   }
   if (a.part == nullptr) return;
@@ -296,7 +291,7 @@ __global__ __launch_bounds__(256) void k_head_norm_backward(HeadNormArgs a, int 
       float v = dw[k][e];
 #pragma unroll
       for (int o = L; o < 64; o <<= 1) v += __shfl_xor(v, o);
-      if (sub == 0) all[wave][k][8 * j + e] = v;
+      if (sub == 0 && at.in) all[wave][k][(e < 4 ? at.a : at.b - 4) + e] = v;
     }
   __syncthreads();
   for (int i = threadIdx.x; i < 2 * a.D; i += 256) {

@@ -488,7 +488,7 @@ struct DecodeAttnArgs {
   float scale2;
   int window, groups;                        // workgroups
 };
-constexpr int kDecodeAttnGroups = 512;       // workgroups at most
+constexpr int kDecodeAttnGroups = 256;       // workgroups at most: one per CU
 int decode_attn_groups(int64_t B, int64_t Hq, int64_t Hk, int64_t keys);
 size_t decode_attn_part_floats(int64_t groups, int64_t D);
 hipError_t launch_decode_attention(int dtype, const DecodeAttnArgs& a, hipStream_t s);
