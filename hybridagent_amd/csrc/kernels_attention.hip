@@ -28,6 +28,41 @@ constexpr int fwd_slots(int D, int KT) { return D * KT == 256 ? 3 : 2; }
 
 }  // namespace
 
+// A query's output (E columns from `at` on) once more, one key after the other: zero
+// times a value that is not finite is not a number, so in a matrix product a key's
+// value reaches the queries of its step that do not see it.  Rows that came out not
+// finite go through here (causal masks alone have such steps); a wavefront has a
+// row, lane l of it D / 64 columns.  Ends where every column is not a number.
+template <typename T, int D, int E>
+__device__ __forceinline__ void attention_again(const AttnArgs& a, const unsigned char* q, const unsigned char* k,
+                                             const unsigned char* v, int from, int to, float m, float sum, int at,
+                                             unsigned char* out) {
+  const int lane = threadIdx.x & 63;
+  constexpr int QE = D / 64, VE = E / 64;
+  auto load = [](const unsigned char* p) { return at_lo<T>(*reinterpret_cast<const uint16_t*>(p)); };
+  float x[QE], acc[VE];
+#pragma unroll
+  for (int i = 0; i < QE; ++i) x[i] = load(q + 2 * (64 * i + lane));
+#pragma unroll
+  for (int i = 0; i < VE; ++i) acc[i] = 0.f;
+  for (int key = from; key <= to; ++key) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < QE; ++i) s = __builtin_fmaf(x[i], load(k + key * a.k_stride + 2 * (64 * i + lane)), s);
+    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(wave_sum_f32(s), a.scale2, -m));
+#pragma unroll
+    for (int i = 0; i < VE; ++i)
+      acc[i] = __builtin_fmaf(p, load(v + key * a.v_stride + 2 * (at + 64 * i + lane)), acc[i]);
+    bool more = false;
+#pragma unroll
+    for (int i = 0; i < VE; ++i) more |= acc[i] == acc[i];
+    if (__ballot(more) == 0) break;
+  }
+#pragma unroll
+  for (int i = 0; i < VE; ++i)
+    *reinterpret_cast<uint16_t*>(out + 2 * (at + 64 * i + lane)) = (uint16_t)at_pack2<T>(acc[i] / sum, 0.f);
+}
+
 // A workgroup has 16 NQ queries of a head per wavefront; PAIR: per pair of
 // wavefronts of a group, each with half of D: of the scores' sum, whose halves
 // they exchange through LDS between the phases, and of the output's columns.
@@ -231,20 +266,43 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_attention(AttnArgs a) {
   if (!second) px_barrier();
   products(active, false, last, slot);
 
+  unsigned char* const out = static_cast<unsigned char*>(a.out) + ((int64_t)it.first * a.Hq + at.head) * (D * 2);
+  const int64_t out_row = (int64_t)a.Hq * D * 2;
+  unsigned long long odd[NQ];  // lanes with a result that is not finite
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     const int q = q0 + 16 * n + r;
-    const float sum = at_sum_over_c(l[n]);
-    if (q >= nq) continue;
-    const float f = sum == 0.f ? 0.f : 1.0f / sum;
-    if (a.lse != nullptr && c == 0 && half == 0)
-      a.lse[(int64_t)at.head * a.Tq + it.first + q] = (m[n] + __builtin_amdgcn_logf(sum)) * kLn2;
-    unsigned char* o =
-        static_cast<unsigned char*>(a.out) + ((int64_t)(it.first + q) * a.Hq + at.head) * (D * 2) + half * D + 8 * c;
+    l[n] = at_sum_over_c(l[n]);
+    const float f = l[n] == 0.f ? 0.f : 1.0f / l[n];
+    if (a.lse != nullptr && c == 0 && half == 0 && q < nq)
+      a.lse[(int64_t)at.head * a.Tq + it.first + q] = (m[n] + __builtin_amdgcn_logf(l[n])) * kLn2;
+    float zero = 0.f;
+    unsigned char* o = out + q * out_row + half * D + 8 * c;
 #pragma unroll
-    for (int d = 0; d < ND; ++d)
-      *reinterpret_cast<u32x2_t*>(o + 32 * d) =
-          u32x2_t{at_pack2<T>(acc[d][n][0] * f, acc[d][n][1] * f), at_pack2<T>(acc[d][n][2] * f, acc[d][n][3] * f)};
+    for (int d = 0; d < ND; ++d) {
+      const f32x4_t v = acc[d][n] * f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) zero = __builtin_fmaf(v[i], 0.f, zero);
+      if (q < nq) *reinterpret_cast<u32x2_t*>(o + 32 * d) = u32x2_t{at_pack2<T>(v[0], v[1]), at_pack2<T>(v[2], v[3])};
+    }
+    odd[n] = __ballot(q < nq && zero != 0.f && l[n] == l[n]);  // a sum that is not: a seen key's score
+  }
+  if (!a.causal) return;
+  __builtin_amdgcn_s_waitcnt(px_vm_wait(0));  // the rows' first stores are done
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    unsigned long long rows = (odd[n] | odd[n] >> 16 | odd[n] >> 32 | odd[n] >> 48) & 0xFFFFull;
+    while (rows != 0) {
+      const int i = __ffsll(rows) - 1, q = q0 + 16 * n + i, kvh = at.head / a.group;
+      rows &= rows - 1;
+      attention_again<T, D, D / kHalves>(
+          a, static_cast<const unsigned char*>(a.q) + at.head * a.q_head + (it.first + q) * a.q_stride,
+          static_cast<const unsigned char*>(a.k) + k_first * a.k_stride + kvh * a.k_head,
+          static_cast<const unsigned char*>(a.v) + k_first * a.v_stride + kvh * a.v_head,
+          a.window > 0 ? max(0, q + off - a.window + 1) : 0, min(nk - 1, q + off),
+          __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(m[n]), i)),
+          __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(l[n]), i)), half * (D / 2), out + q * out_row);
+    }
   }
 }
 

@@ -121,6 +121,53 @@ def test_rows_behind_the_last_sequence(D):
         assert torch.equal(t[:71], w) and not t[71:].any()
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("window", [0, 40])
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_values_that_are_not_finite_reach_those_who_see_them(D, window, bad, dtype):
+    """A value column that is not finite: the queries in front of it and behind its window keep their
+    outputs, the others get it in that column alone."""
+    lens, at = [150, 90], (77, 150 + 31)
+    q, k, v, cu, _, _ = _inputs(lens, lens, 4, 2, D, dtype)
+    clean = ref.packed(q, k, v, cu, cu, D ** -0.5, True, window)
+    for t in at:
+        v[t, 1, D // 2] = bad
+    out, lse = _lib.attention(q, k, v, cu, window=window, return_lse=True)
+    ref.check(lse, clean["lse"], "lse")
+    hit = torch.zeros(240, 4, D, dtype=torch.bool, device="cuda")
+    for t, end in zip(at, (150, 240)):
+        hit[t:min(end, t + window) if window else end, 2:, D // 2] = True
+    assert not out[hit].isfinite().any()
+    want, bound = clean["out"]
+    ref.check(out.double().masked_fill(hit, 0.0), (want.masked_fill(hit, 0.0), bound), "out")
+
+
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_keys_that_are_not_finite_reach_those_who_see_them(D):
+    q, k, v, cu, _, _ = _inputs([150, 90], [150, 90], 4, 2, D, BF)
+    clean = ref.packed(q, k, v, cu, cu, D ** -0.5, True, 0)["out"]
+    k[77], q[200] = math.nan, math.nan
+    out = _lib.attention(q, k, v, cu)
+    hit = torch.zeros(240, 4, D, dtype=torch.bool, device="cuda")
+    hit[77:150] = hit[200] = True
+    assert not out[hit].isfinite().any()
+    ref.check(out.double().masked_fill(hit, 0.0), (clean[0].masked_fill(hit, 0.0), clean[1]), "out")
+
+
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_gradients_of_other_sequences_stay_finite(D):
+    """What is not finite stays in its sequence."""
+    q, k, v, cu, _, dout = _inputs([50, 21, 60], [50, 21, 60], 2, 1, D, BF)
+    k[60], v[55], q[52], dout[65] = math.nan, math.inf, -math.inf, math.nan
+    want = ref.packed(q.nan_to_num(0, 0, 0), k.nan_to_num(0, 0, 0), v.nan_to_num(0, 0, 0), cu, cu, D ** -0.5, True, 0,
+                      dout.nan_to_num(0, 0, 0))
+    out, lse = _lib.attention(q, k, v, cu, return_lse=True)
+    fine = [*range(50), *range(71, 131)]
+    for name, t in zip(("out", "dq", "dk", "dv"), (out, *_lib.attention_backward(dout, q, k, v, out, lse, cu))):
+        ref.check(t[fine], tuple(x[fine] for x in want[name]), name)
+
+
 # ---------------------------------------------------------------- decoding
 
 
