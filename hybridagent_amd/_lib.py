@@ -117,7 +117,7 @@ SIGNATURES = {
     "w4a16_head_norm_rope_backward_workspace_bytes": (_SZ, [_I64] * 4),
     "w4a16_head_norm_rope_backward": (ctypes.c_int, [_VP, _VP, _VP, *_HEADS * 3, *[_VP] * 10, ctypes.c_int,
                                                      *[_I64] * 6, _F32, _VP, _SZ, _VP]),
-    "w4a16_append_kv": (ctypes.c_int, [*_HEADS * 3, *[_VP] * 8, _I64, _VP, _I64, ctypes.c_int, ctypes.c_int,
+    "w4a16_append_kv": (ctypes.c_int, [*_HEADS * 3, *[_VP] * 10, _I64, _VP, _I64, ctypes.c_int, ctypes.c_int,
                                        *[_I64] * 8, _F32, _VP]),
     "w4a16_attention": (ctypes.c_int, [*_HEADS * 3, _VP, _VP, _VP, _VP, ctypes.c_int, *[_I64] * 6, _F32,
                                        ctypes.c_int, _I64, _VP]),
@@ -1050,7 +1050,7 @@ def hybridlink_backward(dout: torch.Tensor, h: torch.Tensor, ln1_w: torch.Tensor
 
 def _gpu_of(*tensors: torch.Tensor | None) -> int:
     """The number of the GPU that all tensors are on (``_require_gpu``'s errors)."""
-    index = -1
+    index = -2  # -1: the host
     for t in tensors:
         if t is not None:
             i = t.get_device()
@@ -1084,14 +1084,14 @@ def _dense(t: torch.Tensor) -> torch.Tensor:
 
 def _heads(t: torch.Tensor, name: str) -> torch.Tensor:
     """t [tokens, heads, D] as the kernels take it: D contiguous, the other strides as they are where
-    every row starts at a multiple of 16 bytes, else a copy."""
+    every row starts at a multiple of 16 bytes and they are 64 MiB at most, else a copy."""
     if t.dim() != 3:
         raise ValueError(f"{name} must be [tokens, heads, head size], got {list(t.shape)}")
     a, b, c = t.stride()
     size = t.element_size()
-    if c == 1 and (a * size | b * size | t.data_ptr()) & 15 == 0:
+    if c == 1 and (a * size | b * size | t.data_ptr()) & 15 == 0 and max(a, b) * size <= 1 << 26:
         return t
-    return _aligned(t.contiguous())
+    return t.clone(memory_format=torch.contiguous_format)  # a size of one leaves contiguous()'s strides open
 
 
 def _head_args(t: torch.Tensor | None):
@@ -1209,7 +1209,9 @@ def _cache_args(k_cache: torch.Tensor, v_cache: torch.Tensor, dtype: torch.dtype
     for t, n in ((k_cache, "k_cache"), (v_cache, "v_cache")):
         a, b, c, d = t.stride()
         p = t.data_ptr()
-        if b != page * D or c != D or d != 1 or (p | 2 * a) & 15:
+        if pages == 1:  # the strides of a size of one are any
+            a = H * page * D
+        if (b != page * D and H != 1) or c != D or d != 1 or (p | 2 * a) & 15:
             raise ValueError(f"{n} must have dense pages at multiples of 16 bytes, got strides {t.stride()}")
         args += (p, a)
     return args, pages, H, page
@@ -1218,11 +1220,12 @@ def _cache_args(k_cache: torch.Tensor, v_cache: torch.Tensor, dtype: torch.dtype
 def append_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor | None, sin: torch.Tensor | None,
               positions: torch.Tensor, slots: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
               q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, eps: float = 1e-6,
-              v_norm: bool = False) -> torch.Tensor:
+              v_norm: bool = False, return_kv: bool = False):
     """``head_norm_rope`` on the way into a paged cache -> q, dense; token t's keys and values (normed
     without a weight where ``v_norm``) go to row ``slots[t]`` (int32; page x page size + row) of
     k_cache, v_cache [pages, Hk, page size, D], bf16 or fp16.  A slot outside the cache (-1: a
-    padding token's) is not written; two tokens of a call must not share one."""
+    padding token's) is not written; two tokens of a call must not share one.  With ``return_kv``
+    (q, k, v), dense, for ``attention`` over the same prompt."""
     if v is None:
         raise ValueError("v must be given")
     index = _gpu_of(q, k, v, cos, sin, positions, q_weight, k_weight, slots, k_cache, v_cache)
@@ -1232,11 +1235,12 @@ def append_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tens
     if H != sizes[2]:
         raise ValueError(f"the cache has {H} heads, k {sizes[2]}")
     out = _dense_like(q)
+    yk, yv = (_dense_like(k), _dense_like(v)) if return_kv else (None, None)
     cos, sin, positions, q_weight, k_weight = rot
     _launch("w4a16_append_kv", index, load().w4a16_append_kv, *_head_args(q), *_head_args(k), *_head_args(v),
             _ptr(cos), _ptr(sin), positions.data_ptr(), slots.data_ptr(), _ptr(q_weight), _ptr(k_weight),
-            out.data_ptr(), *cache, dt, bool(v_norm), *sizes, pages, page, eps)
-    return out
+            out.data_ptr(), _ptr(yk), _ptr(yv), *cache, dt, bool(v_norm), *sizes, pages, page, eps)
+    return (out, yk, yv) if return_kv else out
 
 
 def _group(Hq: int, Hk: int, D: int) -> None:

@@ -88,8 +88,9 @@ int attn_args(AttnArgs& a, const Heads& q, const Heads& k, const Heads& v, const
       Tk < 0 || Tk > kMaxTokens || bad_group(Hq, Hk) || bad_attn_dim(D) || bad_scale(scale) || window < 0 ||
       (window > 0 && !causal) || bad_stride(q, 2) || bad_stride(k, 2) || bad_stride(v, 2))
     return W4A16_ERR_SHAPE;
-  // workgroups of 64 rows at least
-  if ((std::max(Tq, Tk) / 64 + B + 9) * Hq > kMaxBlocks) return W4A16_ERR_SHAPE;
+  // workgroups of 64 rows at least and 512 threads; delta has a thread for eight elements
+  if ((std::max(Tq, Tk) / 64 + B + 9) * Hq > kMaxBlocks / 2 || Tq * Hq > (kMaxBlocks << 8) / (D / 8))
+    return W4A16_ERR_SHAPE;
   if ((Tq > 0 && !q.p) || (Tk > 0 && (!k.p || !v.p)) || !cu_q || !cu_k) return W4A16_ERR_NULL;
   if (odd(q, 2) || odd(k, 2) || odd(v, 2)) return W4A16_ERR_ALIGN;
   a = AttnArgs{};
@@ -196,9 +197,9 @@ int w4a16_head_norm_rope_backward(const void* dq, const void* dk, const void* dv
 int w4a16_append_kv(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token, int64_t k_head,
                     const void* v, int64_t v_token, int64_t v_head, const float* cos, const float* sin,
                     const int32_t* positions, const int32_t* slots, const void* q_weight, const void* k_weight,
-                    void* q_out, void* k_cache, int64_t k_page_stride, void* v_cache, int64_t v_page_stride, int dtype,
-                    int v_norm, int64_t T, int64_t Hq, int64_t Hk, int64_t D, int64_t P, int64_t R, int64_t pages,
-                    int64_t page_size, float eps, void* stream) {
+                    void* q_out, void* k_out, void* v_out, void* k_cache, int64_t k_page_stride, void* v_cache,
+                    int64_t v_page_stride, int dtype, int v_norm, int64_t T, int64_t Hq, int64_t Hk, int64_t D,
+                    int64_t P, int64_t R, int64_t pages, int64_t page_size, float eps, void* stream) {
   if (dtype != W4A16_BF16 && dtype != W4A16_F16) return W4A16_ERR_SHAPE;
   HeadNormArgs a;
   const int st = head_norm_args(a, {q, q_token, q_head}, {k, k_token, k_head}, {v, v_token, v_head}, cos, sin,
@@ -208,13 +209,15 @@ int w4a16_append_kv(const void* q, int64_t q_token, int64_t q_head, const void* 
       v_page_stride < Hk * page_size * D)
     return W4A16_ERR_SHAPE;
   if (T == 0) return W4A16_OK;
-  if (!v || !slots || !q_out || !k_cache || !v_cache) return W4A16_ERR_NULL;
-  if (!aligned16(q_out) || !aligned16(k_cache) || !aligned16(v_cache) || k_page_stride % 8 != 0 ||
-      v_page_stride % 8 != 0)
+  if (!v || !slots || !q_out || !k_cache || !v_cache || (k_out == nullptr) != (v_out == nullptr)) return W4A16_ERR_NULL;
+  if (!aligned16(q_out) || !aligned16(k_out) || !aligned16(v_out) || !aligned16(k_cache) || !aligned16(v_cache) ||
+      k_page_stride % 8 != 0 || v_page_stride % 8 != 0)
     return W4A16_ERR_ALIGN;
   a.yq = q_out;
-  a.yk = k_cache;
-  a.yv = v_cache;
+  a.yk = k_out;
+  a.yv = v_out;
+  a.kc = k_cache;
+  a.vc = v_cache;
   a.k_page = 2 * k_page_stride;
   a.v_page = 2 * v_page_stride;
   a.slots = slots;

@@ -198,12 +198,12 @@ __global__ __launch_bounds__(256) void k_head_norm(HeadNormArgs a, int chunks) {
     if (kind != 2) hn_rotate(turn, u);
     if (!at.in || h >= heads) continue;
     const int n = row[i].head;
-    if (!PAGED || kind == 0) {
-      void* o = kind == 0 ? a.yq : kind == 1 ? a.yk : a.yv;
+    void* o = kind == 0 ? a.yq : kind == 1 ? a.yk : a.yv;
+    if (!PAGED || o != nullptr)
       hn_store<T>(static_cast<T*>(o) + ((int64_t)t * (kind == 0 ? a.Hq : a.Hk) + n) * a.D, at, u);
-    } else if (kept) {
-      unsigned char* o = static_cast<unsigned char*>(kind == 1 ? a.yk : a.yv) + page * (kind == 1 ? a.k_page : a.v_page);
-      hn_store<T>(o + ((int64_t)n * a.page + (slot - page * a.page)) * a.D * sizeof(T), at, u);
+    if (PAGED && kept && kind != 0) {
+      unsigned char* to = static_cast<unsigned char*>(kind == 1 ? a.kc : a.vc) + page * (kind == 1 ? a.k_page : a.v_page);
+      hn_store<T>(to + ((int64_t)n * a.page + (slot - page * a.page)) * a.D * sizeof(T), at, u);
     }
   }
 }

@@ -440,7 +440,8 @@ hipError_t launch_tile_prefill(int mode, const int32_t* packed, int E, int H, in
 struct HeadNormArgs {
   const void *q, *k, *v;                      // v nullable
   int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head;
-  void *yq, *yk, *yv;                         // [T][Hq][D], [T][Hk][D]; paged: yk, yv the caches
+  void *yq, *yk, *yv;                         // [T][Hq][D], [T][Hk][D]
+  void *kc, *vc;                              // paged: the caches (yk, yv nullable then)
   const void *dq, *dk, *dv;                   // backward: the gradients of yq, yk, yv
   const float *cos, *sin;                     // [P][R / 2]
   const int32_t *pos, *slots;                 // slots: paged

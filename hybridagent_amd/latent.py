@@ -14,6 +14,12 @@ front of the first layer one w4a16_add_rms_norm launch), and so does the
 HybridLink map
 (w4a16_hybridlink: two LayerNorm launches and two bf16 weight-streaming
 linear launches with the bias, GELU and residual fused).
+
+With ``attention``, a layer has its attention half too, ``h <- h +
+Attention(RMSNorm(h))`` in front of the MoE, over a paged key-value cache:
+``prompt`` takes whole prompts in and ``decode`` one token per sequence (or a
+latent step's state, fed back as it is), where the reference calls the
+installed model's layers (backends.py:173-196).
 """
 from __future__ import annotations
 
@@ -23,6 +29,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib, synth
+from .attention import Attention, PagedKVCache, rope_tables
 
 
 @dataclass
@@ -31,11 +38,24 @@ class _Layer:
     experts: synth.MoEWeights
     pre_norm: torch.Tensor  # RMSNorm weight of the MoE input (bf16 [H])
     tiles: _lib.TiledWeights | None = None  # the decode streamers' tiled weight copies
+    attn_norm: torch.Tensor | None = None  # RMSNorm weight of the attention's input (bf16 [H])
+    attn: Attention | None = None
+
+
+@dataclass
+class AttentionSizes:
+    """The attention half of every layer of a LatentStack."""
+    heads: int
+    kv_heads: int
+    head_size: int
+    window: int = 0  # tokens that a query sees, 0: all before it
+    longest: int = 8192  # tokens of a sequence at most
+    theta: float = 10000.0
 
 
 class LatentStack:
     def __init__(self, n_layers: int, E: int, H: int, I: int, top_k: int, group_size: int, seed: int,
-                 device, eps: float = 1e-6, tiled: bool = True):
+                 device, eps: float = 1e-6, tiled: bool = True, attention: AttentionSizes | None = None):
         self.H, self.top_k, self.G, self.eps = H, top_k, group_size, eps
         dev = torch.device(device)
         g = torch.Generator(device=dev).manual_seed(seed)
@@ -59,6 +79,17 @@ class LatentStack:
             "ln2w": (1.0 + 0.05 * torch.randn(H, generator=g, device=dev)).to(torch.bfloat16),
             "ln2b": mk(H, sc=0.02),
         }
+        self.attention = attention
+        if attention is not None:  # after all the rest: the other weights are those of a stack without
+            self.cos, self.sin = rope_tables(attention.longest, attention.head_size, attention.theta, dev)
+            for ly in self.layers:
+                ly.attn_norm = (1.0 + 0.05 * torch.randn(H, generator=g, device=dev)).to(torch.bfloat16)
+                ly.attn = Attention(H, attention.heads, attention.kv_heads, attention.head_size, attention.window,
+                                    eps=eps, device=dev).requires_grad_(False)
+                for p in (ly.attn.qkv_proj.weight, ly.attn.o_proj.weight):
+                    p.copy_(mk(*p.shape, sc=1.0 / math.sqrt(p.shape[1])))
+                for p in (ly.attn.q_norm, ly.attn.k_norm):
+                    p.copy_(1.0 + 0.05 * torch.randn(p.shape, generator=g, device=dev))
 
     def rms_norm(self, h: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
         """fp32 x * rsqrt(mean(x^2) + eps) * w, back to bf16 (TF:modeling_gemma4.py:197-215)."""
@@ -110,3 +141,58 @@ class LatentStack:
             ew.gate_up_packed, ew.gate_up_scale, ew.down_packed, ew.down_scale, next_norm, self.eps,
             group_size=self.G, tiles=ly.tiles)
         return h_out, y
+
+    def cache(self, pages: int, sequences: int, page_size: int = 64) -> PagedKVCache:
+        """An empty key-value cache for ``sequences`` sequences of this stack."""
+        a = self._sizes()
+        return PagedKVCache(len(self.layers), a.kv_heads, a.head_size, pages, sequences, a.longest, page_size,
+                            device=self.cos.device)
+
+    def prompt(self, h: torch.Tensor, cache: PagedKVCache, counts: dict[int, int]) -> torch.Tensor:
+        """The layers on whole prompts h [tokens, H] of new sequences (counts[s] tokens of sequence s, one
+        after another) -> the residuals [tokens, H]; the cache holds their keys and values."""
+        self._sizes()
+        self._check(h, sum(counts.values()))
+        for s in counts:
+            if cache.length(s):
+                raise ValueError(f"sequence {s} has tokens already: a prompt starts a sequence")
+        positions, slots = cache.append(counts)
+        ends = torch.tensor([0, *counts.values()]).cumsum(0).to(h.device, torch.int32)
+        return self._attended(h, lambda x, i: self.layers[i].attn.prompt(
+            x, positions, slots, ends, self.cos, self.sin, cache.k[i], cache.v[i]))
+
+    def decode(self, h: torch.Tensor, cache: PagedKVCache, sequences: list[int]) -> torch.Tensor:
+        """The layers on one new token of each named sequence, h [sequences, H] -> the residuals."""
+        self._sizes()
+        self._check(h, len(sequences))
+        if len(set(sequences)) != len(sequences):
+            raise ValueError("a sequence is named twice")
+        positions, slots = cache.append({s: 1 for s in sequences})
+        table, lengths = cache.rows(sequences)
+        return self._attended(h, lambda x, i: self.layers[i].attn.decode(
+            x, positions, slots, table, lengths, self.cos, self.sin, cache.k[i], cache.v[i]))
+
+    def latent(self, h: torch.Tensor, cache: PagedKVCache, sequences: list[int]) -> torch.Tensor:
+        """``decode``, then HybridLink x sqrt(H): a latent step whose result is the next one's input."""
+        return self.hybridlink(self.decode(h, cache, sequences)) * math.sqrt(self.H)
+
+    def _sizes(self) -> AttentionSizes:
+        if self.attention is None:
+            raise ValueError("this stack has no attention: build it with attention=AttentionSizes(...)")
+        return self.attention
+
+    def _check(self, h: torch.Tensor, tokens: int) -> None:
+        if h.shape != (tokens, self.H):
+            raise ValueError(f"h must be [{tokens}, {self.H}], got {list(h.shape)}")
+
+    def _attended(self, h: torch.Tensor, attend) -> torch.Tensor:
+        n = len(self.layers)
+        if n == 0 or h.shape[0] == 0:
+            return h
+        h, x = _lib.add_rms_norm(h, self.layers[0].attn_norm, self.eps)
+        for i, ly in enumerate(self.layers):
+            h, x = _lib.add_rms_norm(h, ly.pre_norm, self.eps, attend(x, i))
+            if i + 1 < n:
+                h, x = self.moe_add_norm(h, x, i, self.layers[i + 1].attn_norm)
+        out, _, _ = self.moe_on(h, x, n - 1)
+        return h + out

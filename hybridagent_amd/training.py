@@ -8,6 +8,9 @@ these are the same maps with hand-written backward passes:
 * ``gated_mlp``   the shared MLP of a decoder layer (backends.py:105-108)
 * ``hybridlink``  HybridLink.forward (hybridlink.py:17-28), and ``HybridLink``,
   the module with the reference's parameter names
+* ``head_norm_rope``, ``attention``  the attention half of a decoder layer
+  (the installed model's attention, backends.py:173-196): the heads' norms with
+  the position rotation, and attention over packed sequences
 
 Each is one pair of library calls (``_lib.layer_norm`` and
 ``_lib.layer_norm_backward``, ...), differentiable once, in reverse mode.  Code that captures
@@ -116,6 +119,65 @@ def hybridlink(h: torch.Tensor, ln1_w: torch.Tensor, ln1_b: torch.Tensor, p1_w: 
     if _wants_grad(h, *params):
         return _HybridLink.apply(h, eps, *params)
     return _lib.hybridlink(h, *params, eps)
+
+
+def _constants(**tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{name} has no gradient here: detach it")
+
+
+class _HeadNormRope(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, q_weight, k_weight, cos, sin, positions, eps):
+        out = _lib.head_norm_rope(q, k, v, cos, sin, positions, q_weight, k_weight, eps)
+        ctx.save_for_backward(q, k, v, cos, sin, positions, q_weight, k_weight)
+        ctx.eps = eps
+        return out if v is not None else out[:2]
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dq, dk, dv=None):
+        _refuse_capture()
+        weights = ctx.needs_input_grad[3] or ctx.needs_input_grad[4]
+        grads = _lib.head_norm_rope_backward(dq, dk, dv, *ctx.saved_tensors, ctx.eps, weights=weights)
+        return (*grads, None, None, None, None)
+
+
+def head_norm_rope(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor | None, cos: torch.Tensor | None,
+                   sin: torch.Tensor | None, positions: torch.Tensor, q_weight: torch.Tensor | None = None,
+                   k_weight: torch.Tensor | None = None, eps: float = 1e-6):
+    """(q, k, v) with every head normed and q and k turned (``_lib.head_norm_rope``); cos and sin are
+    constants."""
+    if _wants_grad(q, k, v, q_weight, k_weight, cos, sin):
+        _constants(cos=cos, sin=sin)
+        out = _HeadNormRope.apply(q, k, v, q_weight, k_weight, cos, sin, positions, eps)
+        return out if v is not None else (*out, None)
+    return _lib.head_norm_rope(q, k, v, cos, sin, positions, q_weight, k_weight, eps)
+
+
+class _Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, cu_q, cu_k, scale, causal, window):
+        out, lse = _lib.attention(q, k, v, cu_q, cu_k, scale, causal, window, return_lse=True)
+        ctx.save_for_backward(q, k, v, out, lse, cu_q, cu_k)
+        ctx.mask = scale, causal, window
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        _refuse_capture()
+        grads = _lib.attention_backward(dout, *ctx.saved_tensors, *ctx.mask, needs=ctx.needs_input_grad[:3])
+        return (*grads, None, None, None, None, None)
+
+
+def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, cu_k: torch.Tensor | None = None,
+              scale: float | None = None, causal: bool = True, window: int = 0) -> torch.Tensor:
+    """Attention over packed sequences (``_lib.attention``)."""
+    if _wants_grad(q, k, v):
+        return _Attention.apply(q, k, v, cu_q, cu_k, scale, causal, window)
+    return _lib.attention(q, k, v, cu_q, cu_k, scale, causal, window)
 
 
 def _weight_and_bias(m: nn.Module | None, name: str, kind: type):

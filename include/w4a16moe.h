@@ -456,7 +456,7 @@ W4A16_API int w4a16_hybridlink_backward(const uint16_t* dout, const uint16_t* h,
 
 /* ---- The attention half of a decoder layer.  No kernel of the reference
  * matches it (its layers call the installed model's attention, backends.py:
- * 151-172); with moe_ffn_block_forward it is a whole layer.  Tensors of heads
+ * 173-196); with moe_ffn_block_forward it is a whole layer.  Tensors of heads
  * are [tokens][heads][D], D contiguous, with any non-negative strides (in
  * elements) between tokens and between heads that are multiples of 16 bytes and
  * at most 64 MiB; outputs are dense.  Sums, softmax statistics and norms are in
@@ -493,16 +493,18 @@ W4A16_API int w4a16_head_norm_rope_backward(const void* dq, const void* dk, cons
 /* w4a16_head_norm_rope on the way into a paged cache: q_out dense, the rows of
  * k and v (normed where v_norm) at slot slots[t] = page * page_size + row of
  *   k_cache, v_cache [pages][Hk][page_size][D], k_page_stride and v_page_stride
- * elements from page to page (multiples of 8).  A slot outside the cache (-1: a
- * padding token's) is not written; two tokens of one call must not share a slot.
- * page_size a power of two, 16 .. 1024; bf16 or fp16.                       */
+ * elements from page to page (multiples of 8), and dense in k_out and v_out (both
+ * NULL: not wanted) for attention over the same prompt.  A slot outside the cache
+ * (-1: a padding token's) is not written; two tokens of one call must not share a
+ * slot (which of them it would hold, piece by piece, is not set).  page_size a
+ * power of two, 16 .. 1024; bf16 or fp16.                                   */
 W4A16_API int w4a16_append_kv(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token,
                               int64_t k_head, const void* v, int64_t v_token, int64_t v_head, const float* cos,
                               const float* sin, const int32_t* positions, const int32_t* slots, const void* q_weight,
-                              const void* k_weight, void* q_out, void* k_cache, int64_t k_page_stride, void* v_cache,
-                              int64_t v_page_stride, int dtype, int v_norm, int64_t T, int64_t Hq, int64_t Hk,
-                              int64_t D, int64_t P, int64_t R, int64_t pages, int64_t page_size, float eps,
-                              void* stream);
+                              const void* k_weight, void* q_out, void* k_out, void* v_out, void* k_cache,
+                              int64_t k_page_stride, void* v_cache, int64_t v_page_stride, int dtype, int v_norm,
+                              int64_t T, int64_t Hq, int64_t Hk, int64_t D, int64_t P, int64_t R, int64_t pages,
+                              int64_t page_size, float eps, void* stream);
 
 /* Attention over packed sequences: out_i = sum_j p_ij v_j, p the softmax of
  * scale q_i k_j over the keys that query i sees, query head h with key-value
@@ -514,10 +516,12 @@ W4A16_API int w4a16_append_kv(const void* q, int64_t q_token, int64_t q_head, co
  * behind the last sequence, gets zeros (lse -inf).  lse (NULL: not wanted):
  * float32 [Hq][Tq], log sum_j exp(scale q_i k_j).  D 64, 128, 256 or 512; bf16
  * or fp16; 16-byte aligned pointers.  The weights are rounded to the type as
- * operands of the second product.
+ * operands of the second product.  What is not finite in a key or value that a
+ * query does not see does not reach it.
  * backward: gradients of q, k and v (dq NULL, or dk and dv: not wanted) for that
  * of out, with out and lse of the forward call; p, and ds = p (dp - delta), are
- * rounded to the type as operands.                                          */
+ * rounded to the type as operands.  What is not finite in a sequence may make any
+ * of its gradients NaN, of no other sequence.                               */
 W4A16_API int w4a16_attention(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token,
                               int64_t k_head, const void* v, int64_t v_token, int64_t v_head, const int32_t* cu_q,
                               const int32_t* cu_k, void* out, float* lse, int dtype, int64_t B, int64_t Tq, int64_t Tk,

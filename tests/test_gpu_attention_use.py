@@ -1,0 +1,603 @@
+"""The attention half of a decoder layer as a program uses it: strides, streams, graphs, long caches,
+bad pages, the differentiable forms, the module over a paged cache and the latent stack."""
+import math
+
+import pytest
+import torch
+
+import attention_reference as ref
+from hybridagent_amd import _lib, training
+from hybridagent_amd.attention import Attention, PagedKVCache, rope_tables
+from hybridagent_amd.latent import AttentionSizes, LatentStack
+
+pytestmark = pytest.mark.gpu
+
+BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+@pytest.fixture(scope="module", autouse=True)
+def dev():
+    assert _lib.available(), "libw4a16moe.so must be built"
+    return torch.device("cuda:0")
+
+
+def _qkv(lens, Hq, Hk, D, dtype=BF):
+    T = sum(lens)
+    return (ref.normal(1, T, Hq, D, dtype=dtype, std=1.5), ref.normal(2, T, Hk, D, dtype=dtype),
+            ref.normal(3, T, Hk, D, dtype=dtype), ref.offsets(lens))
+
+
+def _same(a, b):
+    a, b = ([t] if torch.is_tensor(t) else t for t in (a, b))
+    assert len(a) == len(b)
+    for x, y in zip(a, b):
+        assert (x is None) == (y is None) and (x is None or torch.equal(x, y))
+
+
+# ---------------------------------------------------------------- strides
+
+
+def _layouts(t):
+    """t [T, H, D] in other layouts."""
+    T, H, D = t.shape
+    row = torch.full((T, 2 * H + 1, D), math.nan, device=t.device, dtype=t.dtype)
+    row[:, 1:H + 1] = t
+    far = torch.full((3 * T, H, D), math.nan, device=t.device, dtype=t.dtype)
+    far[::3] = t
+    odd = torch.empty(T * H * D + 1, device=t.device, dtype=t.dtype)[1:].view(T, H, D)
+    odd.copy_(t)
+    wide = torch.full((T, H, D + 4), math.nan, device=t.device, dtype=t.dtype)  # rows of no multiple of 16 bytes
+    wide[..., :D] = t
+    return [row[:, 1:H + 1], far[::3], t.transpose(0, 1).contiguous().transpose(0, 1), odd, wide[..., :D],
+            t.transpose(1, 2).contiguous().transpose(1, 2)]
+
+
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_strides(D):
+    q, k, v, cu = _qkv([45, 0, 1, 20], 4, 2, D)
+    dout = ref.normal(4, *q.shape)
+    out, lse = _lib.attention(q, k, v, cu, return_lse=True)
+    grads = _lib.attention_backward(dout, q, k, v, out, lse, cu)
+    for a, b, c, d in zip(*map(_layouts, (q, k, v, dout))):
+        _same(_lib.attention(a, b, c, cu, return_lse=True), (out, lse))
+        _same(_lib.attention_backward(d, a, b, c, out, lse, cu), grads)
+    two = torch.stack((torch.full_like(cu, 7), cu), 1)[:, 1]
+    _same(_lib.attention(q, k, v, two), out)
+
+
+def test_heads_that_share_memory():
+    """One key-value head expanded to all: read as it lies; the gradients are of the expanded tensor."""
+    q, k, v, cu = _qkv([45, 20], 6, 1, 64)
+    wide = [t.expand(-1, 3, -1) for t in (k, v)]
+    dense = [t.contiguous() for t in wide]
+    out, lse = _lib.attention(q, *wide, cu, return_lse=True)
+    _same((out, lse), _lib.attention(q, *dense, cu, return_lse=True))
+    dout = ref.normal(4, *q.shape)
+    _same(_lib.attention_backward(dout, q, *wide, out, lse, cu), _lib.attention_backward(dout, q, *dense, out, lse, cu))
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    got = torch.autograd.grad(training.attention(leaves[0], *(t.expand(-1, 3, -1) for t in leaves[1:]), cu), leaves, dout)
+    want = _lib.attention_backward(dout, q, *dense, out, lse, cu)
+    _same(got[0], want[0])
+    for g, w in zip(got[1:], want[1:]):
+        _same(g, w.sum(1, keepdim=True))
+
+
+def test_cache_in_strides():
+    """Keys and values of a page side by side, a layer of many, one page, one head."""
+    Hk, D, page = 2, 64, 16
+    lens = [40, 3]
+    both = ref.normal(1, 5, 3, 2, Hk, page, D)
+    kc, vc = both[:, 1, 0], both[:, 1, 1]
+    table = torch.tensor([[4, 0, 2], [3, -1, -1]], device="cuda", dtype=torch.int32)
+    lengths = torch.tensor(lens, device="cuda", dtype=torch.int32)
+    q = ref.normal(2, 2, 4, D)
+    want = _lib.decode_attention(q, kc.contiguous(), vc.contiguous(), table, lengths)
+    for x in _layouts(q):
+        _same(_lib.decode_attention(x, kc, vc, table, lengths), want)
+    wide = torch.full((2, 7), 99, device="cuda", dtype=torch.int32)
+    wide[:, 2:5] = table
+    _same(_lib.decode_attention(q, kc, vc, wide[:, 2:5], lengths), want)
+    one = _lib.decode_attention(q, kc[:1], vc[:1], table[:, 1:2].clamp(min=0), lengths.clamp(max=16))
+    ref.check(one[:1], ref.attend(q[:1], kc[0].transpose(0, 1), vc[0].transpose(0, 1), D ** -0.5, True, 0, BF)["out"], "one page")
+    kv = ref.normal(5, 2, 43, Hk, D)
+    pos = torch.tensor([*range(40), *range(3)], device="cuda", dtype=torch.int32)
+    slots = torch.cat([table[b, torch.arange(n, device="cuda") // page] * page + torch.arange(n, device="cuda") % page
+                       for b, n in enumerate(lens)]).int()
+    dense = [kc.contiguous(), vc.contiguous()]
+    before = both.clone()
+    qs = ref.normal(6, 43, 4, D)
+    yq = _lib.append_kv(qs, kv[0], kv[1], None, None, pos, slots, *dense)
+    _same(_lib.append_kv(qs, kv[0], kv[1], None, None, pos, slots, kc, vc), yq)
+    _same([kc, vc], dense)
+    before[:, 1, 0], before[:, 1, 1] = dense
+    assert torch.equal(both, before)
+
+
+def test_append_returns_the_rows_too():
+    T, Hq, Hk, D = 37, 4, 2, 128
+    q, k, v, _ = _qkv([T], Hq, Hk, D)
+    cos, sin = rope_tables(50, D, device="cuda")
+    pos = torch.arange(T, device="cuda", dtype=torch.int32)
+    w = [ref.normal(8 + i, D, std=0.1, mean=1.0) for i in range(2)]
+    slots = torch.randperm(48, device="cuda")[:T].int()
+    slots[5] = -1  # written to the dense rows all the same
+    for norm in (True, False):
+        caches = [[torch.zeros(3, Hk, 16, D, device="cuda", dtype=BF) for _ in range(2)] for _ in range(2)]
+        yq, yk, yv = _lib.append_kv(q, k, v, cos, sin, pos, slots, *caches[0], *w, v_norm=norm, return_kv=True)
+        _same(yq, _lib.append_kv(q, k, v, cos, sin, pos, slots, *caches[1], *w, v_norm=norm))
+        _same(caches[0], caches[1])
+        hq, hk, hv = _lib.head_norm_rope(q, k, v, cos, sin, pos, *w)
+        _same((yq, yk, yv), (hq, hk, hv if norm else v))
+
+
+# ---------------------------------------------------------------- sizes at their ends
+
+
+@pytest.mark.parametrize("D", [64, 512])
+def test_nothing(D):
+    e = lambda *s, dtype=BF: torch.empty(*s, device="cuda", dtype=dtype)
+    i = lambda *s: torch.zeros(*s, device="cuda", dtype=torch.int32)
+    out, lse = _lib.attention(e(0, 4, D), e(0, 2, D), e(0, 2, D), i(1), return_lse=True)
+    assert out.shape == (0, 4, D) and lse.shape == (4, 0)
+    q, k, v, _ = _qkv([9], 4, 2, D)
+    for cu_q, cu_k in ((i(1), i(1)), (i(3), i(3))):  # rows, but in no sequence
+        out, lse = _lib.attention(q, k, v, cu_q, cu_k, return_lse=True)
+        assert not out.any() and bool((lse == -math.inf).all())
+        for g in _lib.attention_backward(q, q, k, v, out, lse, cu_q, cu_k):
+            assert not g.any()
+    # keys without queries, queries without keys
+    _, dk, dv = _lib.attention_backward(e(0, 4, D), e(0, 4, D), k, v, e(0, 4, D), e(4, 0, dtype=F32), i(2), ref.offsets([9]))
+    assert not dk.any() and not dv.any()
+    out, lse = _lib.attention(q, e(0, 2, D), e(0, 2, D), ref.offsets([9]), i(2), return_lse=True)
+    assert not out.any()
+    dq, _, _ = _lib.attention_backward(q, q, e(0, 2, D), e(0, 2, D), out, lse, ref.offsets([9]), i(2))
+    assert not dq.any()
+    assert _lib.decode_attention(e(0, 4, D), e(2, 2, 16, D), e(2, 2, 16, D), i(0, 3), i(0)).shape == (0, 4, D)
+    w = ref.normal(5, D)
+    got = _lib.head_norm_rope(e(0, 4, D), e(0, 2, D), e(0, 2, D), None, None, i(0), w, w)
+    assert [t.shape[0] for t in got] == [0, 0, 0]
+    *_, wq, wk = _lib.head_norm_rope_backward(e(0, 4, D), e(0, 2, D), None, e(0, 4, D), e(0, 2, D), None, None, None, i(0), w, w)
+    assert not wq.any() and not wk.any()
+    assert _lib.append_kv(e(0, 4, D), e(0, 2, D), e(0, 2, D), None, None, i(0), i(0), e(2, 2, 16, D), e(2, 2, 16, D)).shape[0] == 0
+
+
+def test_parts_of_the_gradients():
+    q, k, v, cu = _qkv([70, 9], 4, 2, 64)
+    dout = ref.normal(4, *q.shape)
+    out, lse = _lib.attention(q, k, v, cu, return_lse=True)
+    want = _lib.attention_backward(dout, q, k, v, out, lse, cu)
+    for needs in ((True, False, False), (False, True, False), (False, False, True), (False, False, False)):
+        got = _lib.attention_backward(dout, q, k, v, out, lse, cu, needs=needs)
+        _same(got, [w if n else None for w, n in zip(want, needs)])
+
+
+def test_many_sequences():
+    lens = [(29 * i) % 71 for i in range(150)]
+    q, k, v, cu = _qkv(lens, 2, 1, 64)
+    dout = ref.normal(4, *q.shape)
+    out, lse = _lib.attention(q, k, v, cu, window=50, return_lse=True)
+    want = ref.packed(q, k, v, cu, cu, 0.125, True, 50, dout)
+    ref.check(out, want["out"], "out")
+    for name, t in zip(("dq", "dk", "dv"), _lib.attention_backward(dout, q, k, v, out, lse, cu, window=50)):
+        ref.check(t, want[name], name)
+
+
+def test_offsets_outside_the_tensors():
+    """They are held to them: nothing outside is read or written."""
+    q, k, v, cu = _qkv([40, 30, 20], 4, 2, 64)
+    dout = ref.normal(4, *q.shape)
+    for wrong, right in (([-5, 40, 70, 10 ** 9], [0, 40, 70, 90]), ([0, 40, 2 ** 31 - 1, 2 ** 31 - 1], [0, 40, 90, 90])):
+        wrong, right = (torch.tensor(t, device="cuda", dtype=torch.int32) for t in (wrong, right))
+        out, lse = _lib.attention(q, k, v, right, return_lse=True)
+        _same(_lib.attention(q, k, v, wrong, return_lse=True), (out, lse))
+        _same(_lib.attention_backward(dout, q, k, v, out, lse, wrong), _lib.attention_backward(dout, q, k, v, out, lse, right))
+
+
+def _paged(lens, Hk, D, page, pages, first, dtype=BF, seed=3):
+    """A cache whose sequences lie in its pages from ``first`` on, in falling order."""
+    kc, vc = (torch.empty(pages, Hk, page, D, device="cuda", dtype=dtype) for _ in range(2))
+    need = [-(-n // page) for n in lens]
+    table = torch.full((len(lens), max(need)), -1, device="cuda", dtype=torch.int32)
+    at, slots = first + sum(need) - 1, []
+    for b, n in enumerate(need):
+        table[b, :n] = torch.arange(at, at - n, -1, device="cuda")
+        at -= n
+        j = torch.arange(lens[b], device="cuda")
+        slots.append(table[b, j // page] * page + j % page)
+    return kc, vc, table, torch.cat(slots).int(), torch.tensor(lens, device="cuda", dtype=torch.int32)
+
+
+def test_cache_longer_than_32_bits():
+    """Pages 10 GiB behind the cache's start, in bytes and, of a page of 512 rows, in elements."""
+    lens, Hk, D, page = [700, 30], 4, 512, 512
+    pages = 5200
+    kc, vc, table, slots, lengths = _paged(lens, Hk, D, page, pages, pages - 3)
+    assert kc[:-3].numel() > 2 ** 32
+    q, k, v, _ = _qkv(lens, 8, Hk, D)
+    pos = torch.arange(730, device="cuda", dtype=torch.int32)
+    _lib.append_kv(q, k, v, None, None, pos, slots, kc, vc)
+    one = ref.normal(7, 2, 8, D, std=1.5)
+    out = _lib.decode_attention(one, kc, vc, table, lengths)
+    for b, (at, n) in enumerate(((0, 700), (700, 30))):
+        want = ref.attend(one[b:b + 1], k[at:at + n], v[at:at + n], D ** -0.5, True, 0, BF)
+        ref.check(out[b:b + 1], want["out"], f"sequence {b}")
+
+
+def test_rows_far_apart():
+    """Tokens 32 MiB apart: offsets past 32 bits in every operand."""
+    T, D = 200, 64
+    step = 1 << 24
+    far = [torch.empty(T * step, device="cuda", dtype=BF).as_strided((T, 2, D), (step, D, 1)) for _ in range(3)]
+    near = [ref.normal(i, T, 2, D) for i in range(3)]
+    for f, n in zip(far, near):
+        f.copy_(n)
+    cu = ref.offsets([150, 50])
+    out, lse = _lib.attention(*near, cu, return_lse=True)
+    _same(_lib.attention(*far, cu, return_lse=True), (out, lse))
+    dout = ref.normal(4, T, 2, D)
+    _same(_lib.attention_backward(dout, *far, out, lse, cu), _lib.attention_backward(dout, *near, out, lse, cu))
+    pos = torch.arange(T, device="cuda", dtype=torch.int32)
+    _same(_lib.head_norm_rope(*far, None, None, pos), _lib.head_norm_rope(*near, None, None, pos))
+
+
+# ---------------------------------------------------------------- bad pages
+
+
+@pytest.mark.parametrize("window", [0, 20])
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_bad_pages(D, window):
+    """A page among the seen that the cache does not have, or a length over the table's: NaN in that sequence;
+    a wrong entry that no seen key lies in, and a negative length, do no harm."""
+    lens = [100, 100, 100, 64, 100, 33]
+    kc, vc, table, slots, lengths = _paged(lens, 2, D, 16, 60, 5)
+    q, k, v, _ = _qkv(lens, 4, 2, D)
+    _lib.append_kv(q, k, v, None, None, torch.zeros_like(slots), slots, kc, vc)
+    one = ref.normal(7, 6, 4, D, std=1.5)
+    want = _lib.decode_attention(one, kc, vc, table, lengths, window=window)
+    table[0, 6], table[1, 6] = 60, -1              # seen with any window
+    table[2, 0] = 2 ** 31 - 1                      # seen without one
+    table[3, 4:] = torch.tensor([-2 ** 31, 10 ** 6, -7], device="cuda", dtype=torch.int32)  # behind the length
+    lengths[4], lengths[5] = 7 * 16 + 1, -3
+    got = _lib.decode_attention(one, kc, vc, table, lengths, window=window)
+    assert bool(got[[0, 1, 4]].isnan().all())
+    assert bool(got[2].isnan().all()) if not window else torch.equal(got[2], want[2])
+    assert torch.equal(got[3], want[3]) and not got[5].any()
+
+
+# ---------------------------------------------------------------- streams and graphs
+
+
+def _chain(q, k, v, cos, sin, pos, slots, kc, vc, w, cu, table, lengths, dout):
+    """Every operator once, each on the last one's results."""
+    yq, yk, yv = _lib.append_kv(q, k, v, cos, sin, pos, slots, kc, vc, *w, v_norm=True, return_kv=True)
+    out, lse = _lib.attention(yq, yk, yv, cu, return_lse=True)
+    one = _lib.decode_attention(out[:2], kc, vc, table, lengths)
+    grads = _lib.attention_backward(dout, yq, yk, yv, out, lse, cu)
+    back = _lib.head_norm_rope_backward(*grads, q, k, v, cos, sin, pos, *w)
+    return [yq, out, one, *back]
+
+
+def _chain_inputs(seed=0, D=128):
+    lens = [150, 61]
+    T = sum(lens)
+    q, k, v = (ref.normal(seed + 1 + i, T, 4 if i == 0 else 2, D) for i in range(3))
+    cos, sin = rope_tables(160, D, device="cuda")
+    kc, vc, table, slots, lengths = _paged(lens, 2, D, 16, 20, 2)
+    kc.zero_(), vc.zero_()
+    pos = torch.cat([torch.arange(n, device="cuda") for n in lens]).int()
+    w = [ref.normal(8 + i, D, std=0.1, mean=1.0) for i in range(2)]
+    return [q, k, v, cos, sin, pos, slots, kc, vc, w, ref.offsets(lens), table, lengths, ref.normal(seed + 20, T, 4, D)]
+
+
+def test_streams():
+    """On a stream of its own behind work that makes the inputs, two such at once."""
+    args = [_chain_inputs(), _chain_inputs(50)]
+    want = [[t.clone() for t in _chain(*a)] for a in args]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in args]
+    for _ in range(3):
+        got = []
+        for s, a in zip(streams, args):
+            with torch.cuda.stream(s):
+                fresh = [(t.float() * 1).to(t.dtype) for t in a[:3]]
+                got.append(_chain(*fresh, *a[3:]))
+        torch.cuda.synchronize()
+        for g, w in zip(got, want):
+            _same(g, w)
+
+
+def test_captured_graphs():
+    """Two graphs of the whole chain from one pool, replayed in turn with new inputs and eager work between."""
+    pool = torch.cuda.graph_pool_handle()
+    args = [_chain_inputs(), _chain_inputs(50)]
+    for a in args:
+        _chain(*a)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for a in args:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, pool=pool):
+            outs.append(_chain(*a))
+        graphs.append(g)
+    for turn in range(4):
+        for i, a in enumerate(args):
+            for j in (0, 1, 2, 13):
+                a[j].copy_(ref.normal(100 * turn + 10 * i + j, *a[j].shape))
+            a[12].sub_(3)  # the lengths too
+            want = [t.clone() for t in _chain(*a)]
+            caches = a[7].clone(), a[8].clone()
+            a[7].zero_(), a[8].zero_()
+            torch.cuda.synchronize()
+            graphs[i].replay()
+            got = [t.clone() for t in outs[i]]
+            torch.cuda.synchronize()
+            _same(got, want)
+            _same((a[7], a[8]), caches)
+
+
+def test_recording_calls_are_not_captured():
+    """They are refused while the stream captures; the same calls without gradients are captured.  (That a
+    recorded backward pass is refused there too is tested without a GPU.)"""
+    q, k, v, cu = _qkv([20], 2, 1, 64)
+    leaf = q.clone().requires_grad_()
+    want = training.attention(q, k, v, cu)
+    pos = torch.zeros(20, device="cuda", dtype=torch.int32)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        for f in (lambda: training.attention(leaf, k, v, cu), lambda: training.head_norm_rope(leaf, k, v, None, None, pos)):
+            with pytest.raises(RuntimeError, match="captured"):
+                f()
+        out = training.attention(q, k, v, cu)
+    g.replay()
+    _same(out, want)
+
+
+# ---------------------------------------------------------------- the differentiable forms
+
+
+def test_autograd_is_the_library():
+    q, k, v, cu = _qkv([45, 20], 4, 2, 64)
+    T, D = 65, 64
+    cos, sin = rope_tables(T, 32, device="cuda")
+    pos = torch.arange(T, device="cuda", dtype=torch.int32)
+    w = [ref.normal(8 + i, D, std=0.1, mean=1.0) for i in range(2)]
+    leaves = [t.clone().requires_grad_() for t in (q, k, v, *w)]
+    dout = ref.normal(4, *q.shape)
+    n = training.head_norm_rope(*leaves[:3], cos, sin, pos, *leaves[3:])
+    y = training.attention(*n, cu, window=30, scale=0.2)
+    got = torch.autograd.grad(y, leaves, dout)
+    m = _lib.head_norm_rope(q, k, v, cos, sin, pos, *w)
+    out, lse = _lib.attention(*m, cu, window=30, scale=0.2, return_lse=True)
+    _same(y, out)
+    dn = _lib.attention_backward(dout, *m, out, lse, cu, window=30, scale=0.2)
+    _same(got, _lib.head_norm_rope_backward(*dn, q, k, v, cos, sin, pos, *w))
+    # without v, without weights, weights as constants
+    a, b = training.head_norm_rope(leaves[0], leaves[1], None, cos, sin, pos)[:2]
+    got = torch.autograd.grad((a, b), leaves[:2], dn[:2])
+    _same(got, _lib.head_norm_rope_backward(*dn[:2], None, q, k, None, cos, sin, pos)[:2])
+    n = training.head_norm_rope(*leaves[:3], cos, sin, pos, *w)
+    _same(torch.autograd.grad(n, leaves[:3], dn), _lib.head_norm_rope_backward(*dn, q, k, v, cos, sin, pos, *w)[:3])
+    # an output that nothing is asked of
+    got = torch.autograd.grad(training.head_norm_rope(*leaves[:3], cos, sin, pos)[0], leaves[:3], dn[0])
+    zero = [torch.zeros_like(t) for t in (k, v)]
+    _same(got, _lib.head_norm_rope_backward(dn[0], *zero, q, k, v, cos, sin, pos)[:3])
+
+
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+@pytest.mark.parametrize("causal,window", [(True, 0), (True, 9), (False, 0)])
+def test_attention_gradients_against_differences(D, causal, window):
+    """Along a direction d the gradients' sum g d is (f(x + h d) - f(x - h d)) / 2 h of the plain forward in
+    64 bits, up to h^2 f''' / 6 (nothing at h = 1e-5 beside the roundings), within the sum of bound |d|."""
+    lens = [40, 25]
+    q, k, v, cu = _qkv(lens, 4, 2, D)
+    dout = ref.normal(4, *q.shape)
+    out, lse = _lib.attention(q, k, v, cu, causal=causal, window=window, return_lse=True)
+    grads = _lib.attention_backward(dout, q, k, v, out, lse, cu, causal=causal, window=window)
+    want = ref.packed(q, k, v, cu, cu, D ** -0.5, causal, window, dout)
+
+    def f(*x):
+        total = 0.0
+        for a, n in ((0, 40), (40, 25)):
+            Q, K, V = (t[a:a + n].transpose(0, 1) for t in x)
+            s = (Q @ K.repeat_interleave(2, 0).transpose(1, 2)) * D ** -0.5
+            p = s.masked_fill(~ref.seen_keys(n, n, causal, window, q.device), -math.inf).softmax(-1)
+            total = total + ((p @ V.repeat_interleave(2, 0)).transpose(0, 1) * dout[a:a + n].double()).sum()
+        return float(total)
+
+    h, base = 1e-5, [t.double() for t in (q, k, v)]
+    for i, name in enumerate(("dq", "dk", "dv")):
+        d = ref.normal(30 + i, *base[i].shape, dtype=torch.float64)
+        up, down = ([t + s * d if j == i else t for j, t in enumerate(base)] for s in (h, -h))
+        slope = (f(*up) - f(*down)) / (2 * h)
+        got = float((grads[i].double() * d).sum())
+        room = float((want[name][1] * d.abs()).sum()) + 1e-6 * abs(slope)
+        assert abs(got - slope) <= room, (name, got, slope, room)
+
+
+@pytest.mark.parametrize("R", [0, 32, 64])
+def test_head_norm_gradients_against_differences(R):
+    """As above; fp32, whose results are off by (D + 20) 2^-24 of the magnitudes that enter them: the gradient
+    of a row is at most rstd |w| (|g| + |n| mean|g w n|) an element, n the normed row."""
+    T, D, eps = 9, 64, 1e-6
+    x = [ref.normal(1 + i, T, 4 if i == 0 else 2, D, dtype=F32) for i in range(3)]
+    w = [ref.normal(8 + i, D, dtype=F32, std=0.2, mean=1.0) for i in range(2)]
+    g = [ref.normal(20 + i, *t.shape, dtype=F32) for i, t in enumerate(x)]
+    pos = torch.arange(T, device="cuda", dtype=torch.int32) * 3
+    cos, sin = rope_tables(30, R, device="cuda") if R else (None, None)
+    got = _lib.head_norm_rope_backward(*g, *x, cos, sin, pos, *w, eps)
+
+    def turn(t):
+        if not R:
+            return t
+        c, s = (m.double()[pos.long()][:, None] for m in (cos, sin))
+        a, b, rest = t.split([R // 2, R // 2, D - R], -1)
+        return torch.cat([a * c - b * s, b * c + a * s, rest], -1)
+
+    def f(q, k, v, qw, kw):
+        n = lambda t: t * (t.pow(2).mean(-1, keepdim=True) + eps).rsqrt()
+        return float(sum((y * z.double()).sum() for y, z in zip((turn(n(q) * qw), turn(n(k) * kw), n(v)), g)))
+
+    base = [t.double() for t in (*x, *w)]
+    h = 1e-6
+    for i in range(5):
+        d = ref.normal(40 + i, *base[i].shape, dtype=torch.float64)
+        up, down = ([t + s * d if j == i else t for j, t in enumerate(base)] for s in (h, -h))
+        slope = (f(*up) - f(*down)) / (2 * h)
+        t = base[i] if i < 3 else base[i - 3]
+        G = g[i if i < 3 else i - 3].double()
+        n = t / t.pow(2).mean(-1, keepdim=True).sqrt()
+        wt = base[3 + i].abs() if i < 2 else torch.ones(D, dtype=torch.float64, device="cuda")
+        G = turn(G).abs() + G.abs() if R else G.abs()  # the turned back gradient is at most the two columns' sum
+        G = G + G.roll(R // 2, -1) + G.roll(-(R // 2), -1) if R else G
+        if i < 3:
+            big = (G * wt + n.abs() * (G * wt * n.abs()).mean(-1, keepdim=True)) / t.pow(2).mean(-1, keepdim=True).sqrt()
+            room = float((big * d.abs()).sum())
+        else:
+            room = float((G * n.abs() * d.abs()).sum()) * 2
+        # the differences themselves: 64 bits' rounding of f over h
+        noise = 2.0 ** -50 * sum(float(z.double().abs().sum()) for z in g) * 4 / h
+        assert abs(float((got[i].double() * d).sum()) - slope) <= (D + 20) * 2.0 ** -24 * room + noise, i
+
+
+# ---------------------------------------------------------------- the module and the stack
+
+
+def _module(D=64, window=0, Hq=4, Hk=2, H=256, v_norm=True):
+    torch.manual_seed(3)
+    m = Attention(H, Hq, Hk, D, window, v_norm=v_norm, device="cuda")
+    with torch.no_grad():
+        for p in (m.q_norm, m.k_norm):
+            p.add_(0.1 * torch.randn_like(p))
+    return m
+
+
+def _project(w, pair):
+    """o_proj in 64 bits of (value, bound): the bound through the weights, fp32 sums, one rounding."""
+    W, (x, e) = w.double(), (t.flatten(1) for t in pair)
+    y = x @ W.t()
+    return y, (e + w.shape[1] * ref.F32 * x.abs()) @ W.abs().t() + ref.half_step(w.dtype) * y.abs()
+
+
+@pytest.mark.parametrize("v_norm", [True, False])
+@pytest.mark.parametrize("D,window", [(64, 0), (128, 40), (256, 0), (512, 17)])
+def test_prompt_then_tokens(D, window, v_norm):
+    """Prompts into the cache, then a token at a time beside a new prompt: each output against attention in
+    64 bits over all that the sequence has had."""
+    m = _module(D, window, v_norm=v_norm)
+    cos, sin = rope_tables(200, D, device="cuda")
+    cache = PagedKVCache(1, 2, D, 40, 3, 200, page_size=16, device="cuda")
+    seen = {0: [], 1: [], 2: []}  # the projections of every token
+
+    def check(y, counts, raw):
+        at = 0
+        for s, n in counts.items():
+            seen[s].append([t[at:at + n] for t in raw])
+            q, k, v = (torch.cat(t) for t in zip(*seen[s]))
+            pos = torch.arange(q.shape[0], device="cuda", dtype=torch.int32)
+            with torch.no_grad():
+                q, k, u = _lib.head_norm_rope(q, k, v, cos, sin, pos, m.q_norm, m.k_norm, m.eps)
+            want = ref.attend(q[-n:], k, u if v_norm else v, D ** -0.5, True, window, BF)["out"]
+            ref.check(y[at:at + n], _project(m.o_proj.weight, want), f"sequence {s}, {q.shape[0]} tokens")
+            at += n
+
+    def prompt(counts, seed):
+        x = ref.normal(seed, sum(counts.values()), 256)
+        pos, slots = cache.append(counts)
+        y = m.prompt(x, pos, slots, ref.offsets(list(counts.values())), cos, sin, cache.k[0], cache.v[0])
+        check(y, counts, m._qkv(x))
+
+    def tokens(sequences, seed):
+        x = ref.normal(seed, len(sequences), 256)
+        pos, slots = cache.append({s: 1 for s in sequences})
+        y = m.decode(x, pos, slots, *cache.rows(sequences), cos, sin, cache.k[0], cache.v[0])
+        check(y, {s: 1 for s in sequences}, m._qkv(x))
+
+    with torch.no_grad():
+        prompt({0: 31, 2: 70}, 1)
+        for i in range(3):
+            tokens([2, 0], 10 + i)
+        prompt({1: 5}, 2)
+        for i in range(3):
+            tokens([0, 1, 2], 20 + i)
+        cache.free(2)
+        seen[2] = []
+        prompt({2: 18}, 3)
+        tokens([0, 1, 2], 30)
+
+
+def test_module_gradients():
+    """The module's backward pass is the library calls' one after the other; a step of it and the prompt form
+    of the same sequences agree."""
+    m, lens = _module(window=30), [45, 20]
+    x = ref.normal(1, 65, 256).requires_grad_()
+    cos, sin = rope_tables(65, 64, device="cuda")
+    pos = torch.cat([torch.arange(n, device="cuda") for n in lens]).int()
+    cu, dy = ref.offsets(lens), ref.normal(2, 65, 256)
+    y = m(x, pos, cu, cos, sin)
+    params = [x, m.qkv_proj.weight, m.q_norm, m.k_norm, m.o_proj.weight]
+    got = torch.autograd.grad(y, params, dy)
+    with torch.no_grad():
+        raw = m._qkv(x)
+        n = _lib.head_norm_rope(*raw, cos, sin, pos, m.q_norm, m.k_norm, m.eps)
+        o, lse = _lib.attention(*n, cu, window=30, return_lse=True)
+        do = (dy @ m.o_proj.weight).view_as(o)
+        back = _lib.head_norm_rope_backward(*_lib.attention_backward(do, *n, o, lse, cu, window=30), *raw, cos, sin, pos,
+                                            m.q_norm, m.k_norm, m.eps)
+        draw = torch.cat([t.flatten(1) for t in back[:3]], 1)
+        want = [draw @ m.qkv_proj.weight, draw.t() @ x, back[3], back[4], dy.t() @ o.flatten(1)]
+    _same(got, want)
+    cache = PagedKVCache(1, 2, 64, 10, 2, 65, page_size=16, device="cuda")
+    p, slots = cache.append({0: 45, 1: 20})
+    assert torch.equal(p, pos)
+    _same(m.prompt(x.detach(), p, slots, cu, cos, sin, cache.k[0], cache.v[0]), y.detach())
+
+
+def test_latent_stack_with_attention():
+    """The stack's prompt, decode and latent steps are its layers called one after the other; without attention
+    its weights and steps are what they were."""
+    sizes = AttentionSizes(heads=4, kv_heads=2, head_size=64, window=40, longest=128)
+    E, H, I, G = 8, 256, 128, 32
+    st = LatentStack(3, E, H, I, 2, G, seed=5, device="cuda", attention=sizes)
+    plain = LatentStack(3, E, H, I, 2, G, seed=5, device="cuda")
+    x = ref.normal(1, 6, H)
+    _same(st.step(x), plain.step(x))
+    with pytest.raises(ValueError, match="no attention"):
+        plain.cache(4, 1)
+    caches = [st.cache(30, 3, page_size=16) for _ in range(2)]
+
+    def layers(h, attend):
+        for i, ly in enumerate(st.layers):
+            h = h + attend(st.rms_norm(h, ly.attn_norm), ly.attn, i)
+            h = h + st.moe(h, i)[0]
+        return h
+
+    def both(h, counts, prompt):
+        got = st.prompt(h, caches[0], counts) if prompt else st.decode(h, caches[0], list(counts))
+        c = caches[1]
+        pos, slots = c.append(counts)
+        if prompt:
+            cu = ref.offsets(list(counts.values()))
+            want = layers(h, lambda x, m, i: m.prompt(x, pos, slots, cu, st.cos, st.sin, c.k[i], c.v[i]))
+        else:
+            rows = c.rows(list(counts))
+            want = layers(h, lambda x, m, i: m.decode(x, pos, slots, *rows, st.cos, st.sin, c.k[i], c.v[i]))
+        assert torch.equal(got, want) and bool(got.isfinite().all())
+        return got
+
+    both(ref.normal(2, 50, H), {0: 30, 2: 20}, True)
+    h = both(ref.normal(3, 2, H), {2: 1, 0: 1}, False)
+    both(ref.normal(4, 9, H), {1: 9}, True)
+    both(ref.normal(5, 3, H), {0: 1, 1: 1, 2: 1}, False)
+    for c in caches[1:]:
+        c.append({0: 1, 1: 1})
+    h = h[:2]
+    out = st.latent(h, caches[0], [0, 1])
+    assert out.shape == (2, H) and bool(out.isfinite().all()) and caches[0].length(0) == caches[1].length(0) == 33
+    with pytest.raises(ValueError, match="already"):
+        st.prompt(ref.normal(6, 4, H), caches[0], {0: 4})
+    with pytest.raises(ValueError, match="twice"):
+        st.decode(h, caches[0], [0, 0])
+    with pytest.raises(ValueError):
+        st.decode(h, caches[0], [0])
+    assert caches[0].length(0) == 33
