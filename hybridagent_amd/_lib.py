@@ -119,9 +119,10 @@ SIGNATURES = {
                                                      *[_I64] * 6, _F32, _VP, _SZ, _VP]),
     "w4a16_append_kv": (ctypes.c_int, [*_HEADS * 3, *[_VP] * 10, _I64, _VP, _I64, ctypes.c_int, ctypes.c_int,
                                        *[_I64] * 8, _F32, _VP]),
+    "w4a16_attention_workspace_bytes": (_SZ, [_I64] * 7),
     "w4a16_attention": (ctypes.c_int, [*_HEADS * 3, _VP, _VP, _VP, _VP, ctypes.c_int, *[_I64] * 6, _F32,
-                                       ctypes.c_int, _I64, _VP]),
-    "w4a16_attention_backward_workspace_bytes": (_SZ, [_I64, _I64]),
+                                       ctypes.c_int, _I64, _VP, _SZ, _VP]),
+    "w4a16_attention_backward_workspace_bytes": (_SZ, [_I64] * 7),
     "w4a16_attention_backward": (ctypes.c_int, [_VP, *_HEADS * 3, *[_VP] * 7, ctypes.c_int, *[_I64] * 6, _F32,
                                                 ctypes.c_int, _I64, _VP, _SZ, _VP]),
     "w4a16_decode_attention_workspace_bytes": (_SZ, [_I64] * 5),
@@ -1289,8 +1290,11 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Ten
     dt, q, k, v, cu_q, cu_k, sizes = _attention_args(q, k, v, cu_q, cu_k, scale, causal, window)
     out = _dense_like(q)
     lse = q.new_empty((sizes[3], sizes[1]), dtype=torch.float32) if return_lse else None
-    _launch("w4a16_attention", index, load().w4a16_attention, *_head_args(q), *_head_args(k), *_head_args(v),
-            cu_q.data_ptr(), cu_k.data_ptr(), out.data_ptr(), _ptr(lse), dt, *sizes)
+    lib = load()
+    nbytes = lib.w4a16_attention_workspace_bytes(*sizes[:6], window)
+    ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    _launch("w4a16_attention", index, lib.w4a16_attention, *_head_args(q), *_head_args(k), *_head_args(v),
+            cu_q.data_ptr(), cu_k.data_ptr(), out.data_ptr(), _ptr(lse), dt, *sizes, _ptr(ws), nbytes)
     return (out, lse) if return_lse else out
 
 
@@ -1313,7 +1317,7 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
     dq = torch.empty_like(dout) if needs[0] else None
     dk, dv = (_dense_like(k), _dense_like(v)) if needs[1] or needs[2] else (None, None)
     lib = load()
-    nbytes = lib.w4a16_attention_backward_workspace_bytes(Tq, Hq)
+    nbytes = lib.w4a16_attention_backward_workspace_bytes(*sizes[:6], window)
     ws = q.new_empty(nbytes, dtype=torch.uint8)
     _launch("w4a16_attention_backward", index, lib.w4a16_attention_backward, dout.data_ptr(), *_head_args(q),
             *_head_args(k), *_head_args(v), out.data_ptr(), lse.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(),

@@ -84,6 +84,17 @@ __device__ __forceinline__ float at_sum_over_c(float v) {
   return at_over_c(v, [](float x, float y) { return x + y; });
 }
 
+// Two tiles side by side of a product's sums (lane: columns 4 c .. of row r), rounded,
+// as lane c's eight columns from at_pair_column(c) on: stores of 16 bytes, 64 of a row
+// together, take half the time of 8 as they lie.
+template <typename T>
+__device__ __forceinline__ u32x4_t at_pair(f32x4_t a, f32x4_t b) {
+  const auto lo = __builtin_amdgcn_permlane16_swap(at_pack2<T>(a[0], a[1]), at_pack2<T>(b[0], b[1]), false, false);
+  const auto hi = __builtin_amdgcn_permlane16_swap(at_pack2<T>(a[2], a[3]), at_pack2<T>(b[2], b[3]), false, false);
+  return u32x4_t{lo[0], hi[0], lo[1], hi[1]};
+}
+__device__ __forceinline__ int at_pair_column(int c) { return 16 * (c & 1) + 8 * (c >> 1); }
+
 // The 16-byte chunk of D that lane group c takes in step i of a score's sum
 // (32 columns of D a step, in an order of its own: both operands use it)
 __device__ __forceinline__ int at_chunk(int i, int c) { return 4 * i + (((c & 1) << 1) | (c >> 1)); }
@@ -369,6 +380,44 @@ __device__ __forceinline__ void at_rows(const int32_t* __restrict__ cu, int n, i
     first = min(max(cu[seq], 0), total);
     len = min(max(cu[seq + 1], first), total) - first;
   }
+}
+
+// The rows of a workgroup's tile, and of the other axis' steps.
+constexpr int attn_rows(int kernel, int D, bool low = false) {
+  return kernel == kAttnForward ? (D == 512 ? 128 : 256) >> (low ? 1 : 0) : D == 512 ? 64 : D == 256 ? 128 : D == 128 ? 192 : 256;
+}
+constexpr int attn_keys(int kernel, int D) { return kernel == kAttnForward && D < 256 ? 64 : 32; }
+constexpr int64_t kAttnParts = 512, kAttnChunk = 12, kAttnMostParts = 32, kAttnLow = 256;
+
+// How many workgroups share a tile of `steps` steps over the other axis, and what
+// one of them has.  The first parts of all tiles go first: what has no part is last.
+// (Quotients come from the vector unit: what loops go by is brought back to scalars.)
+__device__ __forceinline__ int at_parts(const AttnArgs& a, int steps) {
+  return __builtin_amdgcn_readfirstlane(max(min((steps + a.chunk - 1) / a.chunk, a.split), 1));
+}
+struct AtPart {
+  int index, of, first, steps;
+};
+__device__ __forceinline__ AtPart at_part(const AttnArgs& a, int steps, int index) {
+  AtPart p{index, at_parts(a, steps), 0, 0};
+  // its share, and the first steps % of parts one more
+  const int each = __builtin_amdgcn_readfirstlane(steps / p.of), more = steps - each * p.of;
+  p.first = index * each + min(index, more);
+  p.steps = each + (index < more ? 1 : 0);
+  return p;
+}
+
+// The steps of `keys` keys that a tile of `rows` queries from wg0 on takes: all keys
+// that some query of it sees.
+struct AtSpan {
+  int lo, hi, steps;
+};
+__device__ __forceinline__ AtSpan at_key_span(const AttnArgs& a, int nk, int off, int wg0, int rows, int nq, int keys) {
+  AtSpan s;
+  at_seen_keys(a, nk, off, wg0, min(wg0 + rows, nq) - 1, s.lo, s.hi);
+  s.lo &= -keys;
+  s.steps = s.hi > s.lo ? (s.hi - s.lo + keys - 1) / keys : 0;
+  return s;
 }
 
 // A workgroup's head and rank.  Workgroups go round robin to the eight XCDs: each

@@ -119,6 +119,9 @@ int attn_args(AttnArgs& a, const Heads& q, const Heads& k, const Heads& v, const
   return W4A16_OK;
 }
 
+// bytes of the backward pass' workspace: delta, then the parts of one split kernel
+inline size_t delta_floats(int64_t Tq, int64_t Hq) { return ((size_t)Tq * Hq + 3) & ~size_t(3); }
+
 inline int log2_of(int64_t n) {
   int i = 0;
   while ((int64_t(1) << i) < n) ++i;
@@ -227,25 +230,40 @@ int w4a16_append_kv(const void* q, int64_t q_token, int64_t q_head, const void* 
   return launch_status(launch_head_norm(dtype, true, a, static_cast<hipStream_t>(stream)));
 }
 
+size_t w4a16_attention_workspace_bytes(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D,
+                                       int64_t window) {
+  if (B <= 0 || Tq <= 0 || Tk <= 0 || bad_group(Hq, Hk) || bad_attn_dim(D) || window < 0) return 0;
+  return attn_split(kAttnForward, B, Tq, Tk, Hq, Hk, D, window).floats * sizeof(float);
+}
+
 int w4a16_attention(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token, int64_t k_head,
                     const void* v, int64_t v_token, int64_t v_head, const int32_t* cu_q, const int32_t* cu_k, void* out,
                     float* lse, int dtype, int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D,
-                    float scale, int causal, int64_t window, void* stream) {
+                    float scale, int causal, int64_t window, void* workspace, size_t workspace_bytes, void* stream) {
   AttnArgs a;
   const int st = attn_args(a, {q, q_token, q_head}, {k, k_token, k_head}, {v, v_token, v_head}, cu_q, cu_k, dtype, B,
                            Tq, Tk, Hq, Hk, D, scale, causal, window);
   if (st != W4A16_OK) return st;
   if (Tq == 0) return W4A16_OK;
   if (!out) return W4A16_ERR_NULL;
-  if (!aligned16(out)) return W4A16_ERR_ALIGN;
+  if (!aligned16(out) || !aligned16(workspace)) return W4A16_ERR_ALIGN;
+  const AttnSplit p = attn_split(kAttnForward, B, Tq, Tk, Hq, Hk, D, window);
+  if (p.floats > 0 && (workspace == nullptr || workspace_bytes < p.floats * sizeof(float))) return W4A16_ERR_WORKSPACE;
   a.out = out;
   a.lse = lse;
+  a.low = p.low;
+  a.split = p.split;
+  a.chunk = p.chunk;
+  a.part = static_cast<float*>(workspace);
   return launch_status(launch_attention(dtype, a, static_cast<hipStream_t>(stream)));
 }
 
-size_t w4a16_attention_backward_workspace_bytes(int64_t Tq, int64_t Hq) {
-  if (Tq <= 0 || Hq <= 0) return 0;
-  return (size_t)Tq * Hq * sizeof(float);
+size_t w4a16_attention_backward_workspace_bytes(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D,
+                                                int64_t window) {
+  if (Tq <= 0 || bad_group(Hq, Hk) || bad_attn_dim(D) || window < 0) return 0;
+  const size_t part = std::max(attn_split(kAttnDq, B, Tq, Tk, Hq, Hk, D, window).floats,
+                               attn_split(kAttnDkv, B, Tq, Tk, Hq, Hk, D, window).floats);
+  return (delta_floats(Tq, Hq) + part) * sizeof(float);
 }
 
 int w4a16_attention_backward(const void* dout, const void* q, int64_t q_token, int64_t q_head, const void* k,
@@ -263,12 +281,14 @@ int w4a16_attention_backward(const void* dout, const void* q, int64_t q_token, i
   const void* p[] = {dout, out, dq, dk, dv, workspace};
   for (const void* x : p)
     if (!aligned16(x)) return W4A16_ERR_ALIGN;
-  if (Tq > 0 && (workspace == nullptr || workspace_bytes < w4a16_attention_backward_workspace_bytes(Tq, Hq)))
+  if (Tq > 0 && (workspace == nullptr ||
+                 workspace_bytes < w4a16_attention_backward_workspace_bytes(B, Tq, Tk, Hq, Hk, D, window)))
     return W4A16_ERR_WORKSPACE;
   a.dout = dout;
   a.out = const_cast<void*>(out);
   a.lse = const_cast<float*>(lse);
   a.delta = static_cast<float*>(workspace);
+  a.part = Tq > 0 ? a.delta + delta_floats(Tq, Hq) : nullptr;
   a.dq = dq;
   a.dk = dk;
   a.dv = dv;

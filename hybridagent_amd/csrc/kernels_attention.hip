@@ -1,6 +1,7 @@
 // Attention over packed prompts: out = softmax(scale q k^T) v over the keys that
 // a query sees, with grouped heads, sequences of any lengths packed one behind
 // the other, causal masks and windows (include/w4a16moe.h, w4a16_attention).
+#include <algorithm>
 #include <type_traits>
 
 #include "attention.hpp"
@@ -24,7 +25,7 @@ namespace {
 constexpr int kGroup = 4, kWaves = 2 * kGroup;
 
 // LDS slots of a ring, of steps of 32 KT keys
-constexpr int fwd_slots(int D, int KT) { return D * KT == 256 ? 3 : 2; }
+constexpr int fwd_slots(int D, int KT, int NQ) { return D == 256 || (D == 128 && NQ == 2) ? 3 : 2; }
 
 }  // namespace
 
@@ -33,10 +34,10 @@ constexpr int fwd_slots(int D, int KT) { return D * KT == 256 ? 3 : 2; }
 // value reaches the queries of its step that do not see it.  Rows that came out not
 // finite go through here (causal masks alone have such steps); a wavefront has a
 // row, lane l of it D / 64 columns.  Ends where every column is not a number.
-template <typename T, int D, int E>
+template <typename T, int D, int E, typename Store>
 __device__ __forceinline__ void attention_again(const AttnArgs& a, const unsigned char* q, const unsigned char* k,
-                                             const unsigned char* v, int from, int to, float m, float sum, int at,
-                                             unsigned char* out) {
+                                                const unsigned char* v, int from, int to, float m, int at,
+                                                const Store& store) {
   const int lane = threadIdx.x & 63;
   constexpr int QE = D / 64, VE = E / 64;
   auto load = [](const unsigned char* p) { return at_lo<T>(*reinterpret_cast<const uint16_t*>(p)); };
@@ -59,8 +60,17 @@ __device__ __forceinline__ void attention_again(const AttnArgs& a, const unsigne
     if (__ballot(more) == 0) break;
   }
 #pragma unroll
-  for (int i = 0; i < VE; ++i)
-    *reinterpret_cast<uint16_t*>(out + 2 * (at + 64 * i + lane)) = (uint16_t)at_pack2<T>(acc[i] / sum, 0.f);
+  for (int i = 0; i < VE; ++i) store(at + 64 * i + lane, acc[i]);
+}
+
+// Where a part of a split tile leaves a query's sums and (m, l), and the query's
+// place in out and lse: [split][Tq][Hq][D], then [split][Hq][Tq].
+__device__ __forceinline__ float* fwd_part(const AttnArgs& a, int part, int64_t token, int head) {
+  return a.part + (((int64_t)part * a.Tq + token) * a.Hq + head) * a.D;
+}
+__device__ __forceinline__ float2* fwd_stats(const AttnArgs& a, int part, int64_t token, int head) {
+  return reinterpret_cast<float2*>(a.part + (int64_t)a.split * a.Tq * a.Hq * a.D) +
+         ((int64_t)part * a.Hq + head) * a.Tq + token;
 }
 
 // A workgroup has 16 NQ queries of a head per wavefront; PAIR: per pair of
@@ -68,9 +78,10 @@ __device__ __forceinline__ void attention_again(const AttnArgs& a, const unsigne
 // they exchange through LDS between the phases, and of the output's columns.
 // (Heads of 512: a wavefront's registers hold 16 queries' output and the queries,
 // and every operand read from LDS would feed one matrix instruction.)
-template <typename T, int D, int NQ, int KT, bool PAIR>
-__global__ __launch_bounds__(64 * kWaves, 2) void k_attention(AttnArgs a) {
-  constexpr int S = fwd_slots(D, KT);
+// SPLIT: a tile's steps may have several parts.
+template <typename T, int D, int NQ, int KT, bool PAIR, bool SPLIT>
+__global__ __launch_bounds__(64 * kWaves, NQ == 1 && D <= 128 ? 4 : 2) void k_attention(AttnArgs a) {
+  constexpr int S = fwd_slots(D, KT, NQ);
   constexpr int kHalves = PAIR ? 2 : 1;
   constexpr int BQ = 16 * NQ * kWaves / kHalves;
   constexpr int NI = D / 32 / kHalves, ND = D / 16 / kHalves;
@@ -84,7 +95,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_attention(AttnArgs a) {
   const int half = PAIR ? wave & 1 : 0;
 
   const AtPlace at = at_place(a.Hq);
-  const AtItem it = at_find(a.cu_q, a.B, a.Tq, BQ, at.rank);
+  const int index = SPLIT ? __builtin_amdgcn_readfirstlane(at.rank / a.tiles) : 0, tile = at.rank - index * a.tiles;
+  const AtItem it = at_find(a.cu_q, a.B, a.Tq, BQ, tile);
   if (it.seq < 0) return;
   int k_first, nk;
   at_rows(a.cu_k, a.B, a.Tk, it.seq, k_first, nk);
@@ -92,12 +104,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_attention(AttnArgs a) {
   const int wg0 = it.level * BQ;
   const int q0 = wg0 + 16 * NQ * (wave / kHalves);
 
-  int lo, hi, wlo, whi;
-  at_seen_keys(a, nk, off, wg0, min(wg0 + BQ, nq) - 1, lo, hi);
+  int wlo, whi;
   at_seen_keys(a, nk, off, q0, min(q0 + 16 * NQ, nq) - 1, wlo, whi);
   if (q0 >= nq) whi = 0;
-  lo &= -kKeys;
-  const int steps = hi > lo ? (hi - lo + kKeys - 1) / kKeys : 0;
+  const AtSpan span = at_key_span(a, nk, off, wg0, BQ, nq, kKeys);
+  const AtPart part = SPLIT ? at_part(a, span.steps, index) : AtPart{0, 1, 0, span.steps};
+  if (part.index >= part.of) return;
+  const int lo = span.lo + kKeys * part.first, hi = span.hi, steps = part.steps;
 
   // its keys (A) or values (B), and their ring
   Feed feed;
@@ -268,22 +281,37 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_attention(AttnArgs a) {
 
   unsigned char* const out = static_cast<unsigned char*>(a.out) + ((int64_t)it.first * a.Hq + at.head) * (D * 2);
   const int64_t out_row = (int64_t)a.Hq * D * 2;
+  const bool whole = !SPLIT || part.of == 1;
   unsigned long long odd[NQ];  // lanes with a result that is not finite
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     const int q = q0 + 16 * n + r;
     l[n] = at_sum_over_c(l[n]);
-    const float f = l[n] == 0.f ? 0.f : 1.0f / l[n];
-    if (a.lse != nullptr && c == 0 && half == 0 && q < nq)
-      a.lse[(int64_t)at.head * a.Tq + it.first + q] = (m[n] + __builtin_amdgcn_logf(l[n])) * kLn2;
+    const float f = !whole ? 1.f : l[n] == 0.f ? 0.f : 1.0f / l[n];
+    if (c == 0 && half == 0 && q < nq) {
+      if (!whole)
+        *fwd_stats(a, part.index, it.first + q, at.head) = float2{l[n] == 0.f ? -INFINITY : m[n], l[n]};
+      else if (a.lse != nullptr)
+        a.lse[(int64_t)at.head * a.Tq + it.first + q] = (m[n] + __builtin_amdgcn_logf(l[n])) * kLn2;
+    }
     float zero = 0.f;
-    unsigned char* o = out + q * out_row + half * D + 8 * c;
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
-      const f32x4_t v = acc[d][n] * f;
+      acc[d][n] *= f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) zero = __builtin_fmaf(v[i], 0.f, zero);
-      if (q < nq) *reinterpret_cast<u32x2_t*>(o + 32 * d) = u32x2_t{at_pack2<T>(v[0], v[1]), at_pack2<T>(v[2], v[3])};
+      for (int i = 0; i < 4; ++i) zero = __builtin_fmaf(acc[d][n][i], 0.f, zero);
+    }
+    if (whole) {
+      unsigned char* o = out + q * out_row + half * D + 2 * at_pair_column(c);
+#pragma unroll
+      for (int d = 0; d < ND; d += 2) {
+        const u32x4_t v = at_pair<T>(acc[d][n], acc[d + 1][n]);
+        if (q < nq) *reinterpret_cast<u32x4_t*>(o + 32 * d) = v;
+      }
+    } else if (q < nq) {
+      float* o = fwd_part(a, part.index, it.first + q, at.head) + half * (D / 2) + 4 * c;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) *reinterpret_cast<f32x4_t*>(o + 16 * d) = acc[d][n];
     }
     odd[n] = __ballot(q < nq && zero != 0.f && l[n] == l[n]);  // a sum that is not: a seen key's score
   }
@@ -295,14 +323,73 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_attention(AttnArgs a) {
     while (rows != 0) {
       const int i = __ffsll(rows) - 1, q = q0 + 16 * n + i, kvh = at.head / a.group;
       rows &= rows - 1;
+      const float sum = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(l[n]), i));
       attention_again<T, D, D / kHalves>(
           a, static_cast<const unsigned char*>(a.q) + at.head * a.q_head + (it.first + q) * a.q_stride,
           static_cast<const unsigned char*>(a.k) + k_first * a.k_stride + kvh * a.k_head,
           static_cast<const unsigned char*>(a.v) + k_first * a.v_stride + kvh * a.v_head,
-          a.window > 0 ? max(0, q + off - a.window + 1) : 0, min(nk - 1, q + off),
-          __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(m[n]), i)),
-          __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(l[n]), i)), half * (D / 2), out + q * out_row);
+          max(lo, a.window > 0 ? q + off - a.window + 1 : 0), min(lo + kKeys * steps, min(nk, q + off + 1)) - 1,
+          __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(m[n]), i)), half * (D / 2), [&](int d, float v) {
+            if (whole)
+              *reinterpret_cast<uint16_t*>(out + q * out_row + 2 * d) = (uint16_t)at_pack2<T>(sum == 0.f ? 0.f : v / sum, 0.f);
+            else
+              fwd_part(a, part.index, it.first + q, at.head)[d] = v;
+          });
     }
+  }
+}
+
+constexpr int kAttnJoin = 4;
+
+// The parts of the split tiles put together: a workgroup has kAttnJoin 1024 / D
+// queries of a tile, whose loads are under way together.
+template <typename T, int D, int BQ, int kKeys>
+__global__ __launch_bounds__(256) void k_attention_join(AttnArgs a) {
+  constexpr int L = D / 4;
+  const AtPlace at = at_place(a.Hq);
+  const AtItem it = at_find(a.cu_q, a.B, a.Tq, BQ, at.rank);
+  if (it.seq < 0) return;
+  int k_first, nk;
+  at_rows(a.cu_k, a.B, a.Tk, it.seq, k_first, nk);
+  const int nq = it.len, wg0 = it.level * BQ;
+  const int parts = at_parts(a, at_key_span(a, nk, nk - nq, wg0, BQ, nq, kKeys).steps);
+  if (parts == 1) return;
+  constexpr int R = kAttnJoin;
+  const int d = 4 * (threadIdx.x % L), q0 = wg0 + R * (256 / L) * blockIdx.y + threadIdx.x / L;
+  if (q0 >= nq) return;
+  int64_t token[R];
+  float top[R], l[R];
+  f32x4_t v[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    token[i] = it.first + min(q0 + 256 / L * i, nq - 1);
+    top[i] = -INFINITY;
+    l[i] = 0.f;
+    v[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+#pragma unroll 4
+  for (int p = 0; p < parts; ++p)
+#pragma unroll
+    for (int i = 0; i < R; ++i) top[i] = fmaxf(top[i], fwd_stats(a, p, token[i], at.head)->x);
+#pragma unroll 2
+  for (int p = 0; p < parts; ++p)
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const float2 s = *fwd_stats(a, p, token[i], at.head);
+      const float f = __builtin_amdgcn_exp2f(s.x - (top[i] == -INFINITY ? 0.f : top[i]));
+      l[i] += s.y * f;
+      v[i] += *reinterpret_cast<const f32x4_t*>(fwd_part(a, p, token[i], at.head) + d) * f;
+    }
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    if (q0 + 256 / L * i >= nq) break;
+    const float f = l[i] == 0.f ? 0.f : 1.0f / l[i];
+    *reinterpret_cast<u32x2_t*>(static_cast<unsigned char*>(a.out) + ((token[i] * a.Hq + at.head) * D + d) * 2) =
+        u32x2_t{at_pack2<T>(v[i][0] * f, v[i][1] * f), at_pack2<T>(v[i][2] * f, v[i][3] * f)};
+    // (no key at all: log2 0 is the least)
+    if (a.lse != nullptr && d == 0)
+      a.lse[(int64_t)at.head * a.Tq + token[i]] =
+          ((top[i] == -INFINITY ? 0.f : top[i]) + __builtin_amdgcn_logf(l[i])) * kLn2;
   }
 }
 
@@ -311,27 +398,61 @@ namespace {
 template <typename T, int D, int NQ, int KT, bool PAIR>
 hipError_t fwd(AttnArgs a, hipStream_t s) {
   a.tiles = a.Tq / (16 * NQ * kWaves / (PAIR ? 2 : 1)) + a.B + 1;
-  constexpr int lds = 2 * fwd_slots(D, KT) * KT * at_tile_bytes<D>() + (PAIR ? kWaves * 2 * KT * NQ * 64 * 16 : 0);
+  constexpr int lds = 2 * fwd_slots(D, KT, NQ) * KT * at_tile_bytes<D>() + (PAIR ? kWaves * 2 * KT * NQ * 64 * 16 : 0);
   static_assert(lds <= 160 * 1024, "a CU's LDS");
-  hipLaunchKernelGGL((k_attention<T, D, NQ, KT, PAIR>), dim3((unsigned)(a.tiles * a.Hq)), dim3(64 * kWaves), lds, s, a);
+  constexpr int BQ = 16 * NQ * kWaves / (PAIR ? 2 : 1);
+  static_assert(BQ == attn_rows(kAttnForward, D, NQ == 1) && 32 * KT == attn_keys(kAttnForward, D), "attn_split's tiles");
+  const dim3 grid((unsigned)(a.tiles * a.Hq * a.split));
+  if (a.split == 1) {
+    hipLaunchKernelGGL((k_attention<T, D, NQ, KT, PAIR, false>), grid, dim3(64 * kWaves), lds, s, a);
+  } else {
+    hipLaunchKernelGGL((k_attention<T, D, NQ, KT, PAIR, true>), grid, dim3(64 * kWaves), lds, s, a);
+    hipLaunchKernelGGL((k_attention_join<T, D, BQ, 32 * KT>), dim3((unsigned)(a.tiles * a.Hq), BQ * D / 1024 / kAttnJoin), dim3(256), 0,
+                       s, a);
+  }
   return hipGetLastError();
 }
 
 template <typename T>
-hipError_t fwd_type(const AttnArgs& a, hipStream_t s) {
+hipError_t fwd_type(const AttnArgs& a, bool low, hipStream_t s) {
   switch (a.D) {
-    case 64: return fwd<T, 64, 2, 2, false>(a, s);
-    case 128: return fwd<T, 128, 2, 2, false>(a, s);
-    case 256: return fwd<T, 256, 2, 1, false>(a, s);
-    case 512: return fwd<T, 512, 2, 1, true>(a, s);
+    case 64: return low ? fwd<T, 64, 1, 2, false>(a, s) : fwd<T, 64, 2, 2, false>(a, s);
+    case 128: return low ? fwd<T, 128, 1, 2, false>(a, s) : fwd<T, 128, 2, 2, false>(a, s);
+    case 256: return low ? fwd<T, 256, 1, 1, false>(a, s) : fwd<T, 256, 2, 1, false>(a, s);
+    case 512: return low ? fwd<T, 512, 1, 1, true>(a, s) : fwd<T, 512, 2, 1, true>(a, s);
   }
   return hipErrorInvalidValue;
 }
 
 }  // namespace
 
+// Tiles with few heads or tokens leave most CUs idle, and a tile's steps follow one
+// another: they are cut so that there are about two workgroups per CU.
+AttnSplit attn_split(int kernel, int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D, int64_t window) {
+  AttnSplit r{false, 1, 1, 0};
+  const bool dkv = kernel == kAttnDkv;
+  const int64_t heads = dkv ? Hk : Hq, each = dkv ? Hq / Hk : 1;
+  const int64_t T = dkv ? Tk : Tq, other = dkv ? Tq : Tk;
+  r.low = kernel == kAttnForward && (T / attn_rows(kernel, (int)D) + B + 1) * heads <= kAttnLow;
+  const int64_t rows = attn_rows(kernel, (int)D, r.low), keys = attn_keys(kernel, (int)D);
+  if (B <= 0 || B > 64 || T <= 0 || other <= 0) return r;
+  const int64_t tiles = T / rows + B + 1;
+  // sequences of one length: their tiles, and a tile's steps
+  const int64_t like = ((T / B + rows - 1) / rows) * B;
+  auto steps = [&](int64_t n) { return (((window > 0 && window < n ? std::min(n, window + rows) : n) + keys - 1) / keys + 1) * each; };
+  const int64_t work = like * heads * steps(other / B);
+  const int64_t chunk = std::max<int64_t>(kAttnChunk, work / kAttnParts);
+  const int64_t split =
+      std::min<int64_t>({kAttnMostParts, steps(other) / chunk, 2 * kAttnParts / (tiles * heads)});
+  if (split < 2) return r;
+  r.split = (int)split;
+  r.chunk = (int)chunk;
+  r.floats = dkv ? (size_t)(2 * split * Tk * Hk * D) : (size_t)(split * Tq * Hq * (D + (kernel == kAttnForward ? 2 : 0)));
+  return r;
+}
+
 hipError_t launch_attention(int dtype, const AttnArgs& a, hipStream_t s) {
-  return dtype == 0 ? fwd_type<__bf16>(a, s) : fwd_type<_Float16>(a, s);
+  return dtype == 0 ? fwd_type<__bf16>(a, a.low, s) : fwd_type<_Float16>(a, a.low, s);
 }
 
 }  // namespace w4a16

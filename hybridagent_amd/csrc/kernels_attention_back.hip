@@ -72,6 +72,43 @@ __global__ __launch_bounds__(256) void k_attention_delta(AttnArgs a) {
   }
 }
 
+// A lane's columns of a row's gradient: the output's `ok` row at `at`, or a part's of
+// it, which lie `plane` floats apart.
+template <typename T, int ND, int N>
+__device__ __forceinline__ void back_store(const f32x4_t (&acc)[ND][N], int n, bool ok, void* out, float* parts,
+                                           int64_t plane, const AtPart& part, int64_t at, int c, float scale) {
+  if (part.of == 1) {
+    unsigned char* o = static_cast<unsigned char*>(out) + 2 * (at + at_pair_column(c));
+#pragma unroll
+    for (int d = 0; d < ND; d += 2) {
+      const u32x4_t v = at_pair<T>(acc[d][n] * scale, acc[d + 1][n] * scale);
+      if (ok) *reinterpret_cast<u32x4_t*>(o + 32 * d) = v;
+    }
+  } else if (ok) {
+    float* o = parts + part.index * plane + at + 4 * c;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) *reinterpret_cast<f32x4_t*>(o + 16 * d) = acc[d][n];
+  }
+}
+
+// join_rows rows of a sequence, from `row` on, joined (several rows a thread, as in the
+// forward pass, are slower here: more parts, fewer tiles)
+constexpr int join_rows(int D) { return 1024 / D; }
+template <typename T, int D>
+__device__ __forceinline__ void back_join(const float* parts, int64_t plane, int n, int first, int row, int len, int heads,
+                                          int head, float scale, void* out) {
+  constexpr int L = D / 4;
+  const int i = row + threadIdx.x / L;
+  if (i >= len) return;
+  const int64_t at = ((int64_t)(first + i) * heads + head) * D + 4 * (threadIdx.x % L);
+  f32x4_t v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+  for (int p = 0; p < n; ++p) v += *reinterpret_cast<const f32x4_t*>(parts + p * plane + at);
+  v *= scale;
+  *reinterpret_cast<u32x2_t*>(static_cast<unsigned char*>(out) + 2 * at) =
+      u32x2_t{at_pack2<T>(v[0], v[1]), at_pack2<T>(v[2], v[3])};
+}
+
 // A workgroup has 16 NQ queries of a head per pair.
 template <typename T, int D, int NQ>
 __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dq(AttnArgs a) {
@@ -90,19 +127,21 @@ __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dq(AttnArgs a) {
 
   const AtPlace wg = at_place(a.Hq);
   const int head = wg.head;
-  const AtItem it = at_find(a.cu_q, a.B, a.Tq, BQ, wg.rank);
+  const int index = __builtin_amdgcn_readfirstlane(wg.rank / a.tiles), tile = wg.rank - index * a.tiles;
+  const AtItem it = at_find(a.cu_q, a.B, a.Tq, BQ, tile);
   if (it.seq < 0) return;
   int k_first, nk;
   at_rows(a.cu_k, a.B, a.Tk, it.seq, k_first, nk);
   const int nq = it.len, off = nk - nq;
   const int wg0 = it.level * BQ;
   const int q0 = wg0 + 16 * NQ * place;
-  int lo, hi, wlo, whi;
-  at_seen_keys(a, nk, off, wg0, min(wg0 + BQ, nq) - 1, lo, hi);
+  int wlo, whi;
   at_seen_keys(a, nk, off, q0, min(q0 + 16 * NQ, nq) - 1, wlo, whi);
   if (q0 >= nq) whi = 0;
-  lo &= ~31;
-  const int steps = hi > lo ? (hi - lo + 31) / 32 : 0;
+  const AtSpan span = at_key_span(a, nk, off, wg0, BQ, nq, 32);
+  const AtPart part = at_part(a, span.steps, index);
+  if (part.index >= part.of) return;
+  const int lo = span.lo + 32 * part.first, hi = span.hi, steps = part.steps;
 
   Feed feed;
   {
@@ -271,15 +310,40 @@ __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dq(AttnArgs a) {
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     const int q = q0 + 16 * n + r;
-    if (q >= nq) continue;
-    unsigned char* o =
-        static_cast<unsigned char*>(a.dq) + ((int64_t)(it.first + q) * a.Hq + head) * (D * 2) + role * D + 8 * c;
-#pragma unroll
-    for (int d = 0; d < ND; ++d) {
-      const f32x4_t v = acc[d][n] * a.scale;
-      *reinterpret_cast<u32x2_t*>(o + 32 * d) = u32x2_t{at_pack2<T>(v[0], v[1]), at_pack2<T>(v[2], v[3])};
-    }
+    back_store<T>(acc, n, q < nq, a.dq, a.part, (int64_t)a.Tq * a.Hq * D, part,
+                  ((int64_t)(it.first + q) * a.Hq + head) * D + role * (D / 2), c, a.scale);
   }
+}
+
+// The parts of the split tiles added up, in their order: a workgroup has
+// join_rows queries of a tile.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void k_attention_dq_join(AttnArgs a) {
+  constexpr int BQ = 16 * kPairs * dq_rows(D);
+  const AtPlace wg = at_place(a.Hq);
+  const AtItem it = at_find(a.cu_q, a.B, a.Tq, BQ, wg.rank);
+  if (it.seq < 0) return;
+  int k_first, nk;
+  at_rows(a.cu_k, a.B, a.Tk, it.seq, k_first, nk);
+  const int wg0 = it.level * BQ;
+  const int parts = at_parts(a, at_key_span(a, nk, nk - it.len, wg0, BQ, it.len, 32).steps);
+  if (parts > 1)
+    back_join<T, D>(a.part, (int64_t)a.Tq * a.Hq * D, parts, it.first, wg0 + join_rows(D) * (int)blockIdx.y, it.len, a.Hq, wg.head,
+                    a.scale, a.dq);
+}
+
+// The queries that some key of a tile of `rows` from wg0 on sees, in steps of 32 of
+// every head of the group.
+__device__ __forceinline__ void query_range(const AttnArgs& a, int nq, int off, int first, int last, int& lo, int& hi) {
+  lo = a.causal ? max(0, first - off) : 0;
+  hi = a.window > 0 ? min(nq, last - off + a.window) : nq;
+}
+__device__ __forceinline__ AtSpan query_span(const AttnArgs& a, int nq, int nk, int wg0, int rows) {
+  AtSpan s;
+  query_range(a, nq, nk - nq, wg0, min(wg0 + rows, nk) - 1, s.lo, s.hi);
+  s.lo &= ~31;
+  s.steps = s.hi > s.lo ? (s.hi - s.lo + 31) / 32 : 0;
+  return s;
 }
 
 // A workgroup has 16 NK keys of a key-value head per pair; A sums dv, B dk.
@@ -300,26 +364,23 @@ __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dkv(AttnArgs a) {
 
   const AtPlace wg = at_place(a.Hk);
   const int kvh = wg.head;
-  const AtItem it = at_find(a.cu_k, a.B, a.Tk, BK, wg.rank);
+  const int index = __builtin_amdgcn_readfirstlane(wg.rank / a.tiles), tile = wg.rank - index * a.tiles;
+  const AtItem it = at_find(a.cu_k, a.B, a.Tk, BK, tile);
   if (it.seq < 0) return;
   int q_first, nq;
   at_rows(a.cu_q, a.B, a.Tq, it.seq, q_first, nq);
   const int nk = it.len, off = nk - nq;
   const int wg0 = (it.tiles - 1 - it.level) * BK;  // the first keys are seen by the most queries
   const int k0 = wg0 + 16 * NK * place;
-  // the queries lo .. hi - 1 that see a range of keys
-  auto range = [&](int first, int last, int& lo, int& hi) {
-    lo = a.causal ? max(0, first - off) : 0;
-    hi = a.window > 0 ? min(nq, last - off + a.window) : nq;
-  };
-  int lo, hi, wlo, whi;
-  range(wg0, min(wg0 + BK, nk) - 1, lo, hi);
-  range(k0, min(k0 + 16 * NK, nk) - 1, wlo, whi);
+  int wlo, whi;
+  query_range(a, nq, off, k0, min(k0 + 16 * NK, nk) - 1, wlo, whi);
   if (k0 >= nk) whi = 0;
-  lo &= ~31;
-  const int per = hi > lo ? (hi - lo + 31) / 32 : 0;  // steps of a head
-  const int steps = per * a.group;
-  const int top = lo + 32 * max(per - 1, 0);
+  const AtSpan span = query_span(a, nq, nk, wg0, BK);
+  const int per = max(span.steps, 1), lo = span.lo;  // steps of a head
+  const AtPart part = at_part(a, span.steps * a.group, index);
+  if (part.index >= part.of) return;
+  const int steps = part.steps;
+  const int top = lo + 32 * (per - 1);
 
   // A place in the steps: a head after the other, its queries from the last on.
   // (So all workgroups of a sequence that run together read the same tiles.)
@@ -340,7 +401,9 @@ __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dkv(AttnArgs a) {
     feed.init(static_cast<const unsigned char*>(a.q) + q_first * a.q_stride, a.q_stride, place);
   const int64_t head_bytes = role ? D * 2 : a.q_head;
   unsigned char* const ring = smem + (role ? SA * kTile : 0);
-  At next{kvh * a.group, top};
+  const int heads = __builtin_amdgcn_readfirstlane(part.first / per);  // in front of the part
+  const At begin{kvh * a.group + heads, top - 32 * (part.first - heads * per)};
+  At next = begin;
   int load = 0, to = 0;
   auto issue = [&] {
     feed.issue(ring + to * kTile, next.q0, load < steps ? nq : 0, next.head * head_bytes);
@@ -382,7 +445,7 @@ __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dkv(AttnArgs a) {
     for (int u = 0; u < 2; ++u) st.v[u] = buf_ld16(rsrc, 32 * c, 16 * u);
     return st;
   };
-  At at{kvh * a.group, top};
+  At at = begin;
   Stats st = fetch(at, steps > 0);
 #pragma unroll
   for (int u = 0; u < 2; ++u) asm volatile("" : "+v"(st.v[u]));
@@ -496,19 +559,32 @@ __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dkv(AttnArgs a) {
     }
   }
 
-  unsigned char* const out = static_cast<unsigned char*>(role ? a.dk : a.dv);
-  const float scale = role ? a.scale : 1.f;
+  const int64_t plane = (int64_t)a.Tk * a.Hk * D;
+  float* const parts = a.part + (role ? a.split * plane : 0);
 #pragma unroll
   for (int n = 0; n < NK; ++n) {
     const int k = k0 + 16 * n + r;
-    if (k >= nk) continue;
-    unsigned char* o = out + ((int64_t)(it.first + k) * a.Hk + kvh) * (D * 2) + 8 * c;
-#pragma unroll
-    for (int d = 0; d < ND; ++d) {
-      const f32x4_t v = acc[d][n] * scale;
-      *reinterpret_cast<u32x2_t*>(o + 32 * d) = u32x2_t{at_pack2<T>(v[0], v[1]), at_pack2<T>(v[2], v[3])};
-    }
+    back_store<T>(acc, n, k < nk, role ? a.dk : a.dv, parts, plane, part, ((int64_t)(it.first + k) * a.Hk + kvh) * D, c,
+                  role ? a.scale : 1.f);
   }
+}
+
+// As k_attention_dq_join: blockIdx.z 0 dv, 1 dk.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void k_attention_dkv_join(AttnArgs a) {
+  constexpr int BK = 16 * kPairs * dkv_rows(D);
+  const AtPlace wg = at_place(a.Hk);
+  const AtItem it = at_find(a.cu_k, a.B, a.Tk, BK, wg.rank);
+  if (it.seq < 0) return;
+  int q_first, nq;
+  at_rows(a.cu_q, a.B, a.Tq, it.seq, q_first, nq);
+  const int wg0 = (it.tiles - 1 - it.level) * BK;
+  const int parts = at_parts(a, query_span(a, nq, it.len, wg0, BK).steps * a.group);
+  const int64_t plane = (int64_t)a.Tk * a.Hk * D;
+  const bool keys = blockIdx.z != 0;
+  if (parts > 1)
+    back_join<T, D>(a.part + (keys ? a.split * plane : 0), plane, parts, it.first, wg0 + join_rows(D) * (int)blockIdx.y, it.len, a.Hk,
+                    wg.head, keys ? a.scale : 1.f, keys ? a.dk : a.dv);
 }
 
 namespace {
@@ -521,15 +597,29 @@ hipError_t back(AttnArgs a, hipStream_t s) {
     const int64_t rows = (int64_t)a.Tq * a.Hq, per = 256 / (D / 8);
     hipLaunchKernelGGL((k_attention_delta<T, D>), dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, s, a);
   }
+  constexpr int BQ = 16 * NQ * kPairs, BK = 16 * NK * kPairs;
+  static_assert(BQ == attn_rows(kAttnDq, D) && BK == attn_rows(kAttnDkv, D), "attn_split's tiles");
+  auto split = [&](int kernel) {
+    const AttnSplit p = attn_split(kernel, a.B, a.Tq, a.Tk, a.Hq, a.Hk, a.D, a.window);
+    a.split = p.split;
+    a.chunk = p.chunk;
+  };
   if (a.Tq > 0 && a.dq != nullptr) {
-    a.tiles = a.Tq / (16 * NQ * kPairs) + a.B + 1;
-    hipLaunchKernelGGL((k_attention_dq<T, D, NQ>), dim3((unsigned)(a.tiles * a.Hq)), dim3(kBackThreads), back_lds(D, NQ), s,
-                       a);
+    a.tiles = a.Tq / BQ + a.B + 1;
+    split(kAttnDq);
+    hipLaunchKernelGGL((k_attention_dq<T, D, NQ>), dim3((unsigned)(a.tiles * a.Hq * a.split)), dim3(kBackThreads),
+                       back_lds(D, NQ), s, a);
+    if (a.split > 1)
+      hipLaunchKernelGGL((k_attention_dq_join<T, D>), dim3((unsigned)(a.tiles * a.Hq), BQ / join_rows(D)), dim3(256), 0, s, a);
   }
   if (a.Tk > 0 && a.dk != nullptr) {
-    a.tiles = a.Tk / (16 * NK * kPairs) + a.B + 1;
-    hipLaunchKernelGGL((k_attention_dkv<T, D, NK>), dim3((unsigned)(a.tiles * a.Hk)), dim3(kBackThreads), back_lds(D, NK),
-                       s, a);
+    a.tiles = a.Tk / BK + a.B + 1;
+    split(kAttnDkv);
+    hipLaunchKernelGGL((k_attention_dkv<T, D, NK>), dim3((unsigned)(a.tiles * a.Hk * a.split)), dim3(kBackThreads),
+                       back_lds(D, NK), s, a);
+    if (a.split > 1)
+      hipLaunchKernelGGL((k_attention_dkv_join<T, D>), dim3((unsigned)(a.tiles * a.Hk), BK / join_rows(D), 2), dim3(256), 0, s,
+                         a);
   }
   return hipGetLastError();
 }

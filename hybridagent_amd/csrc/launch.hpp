@@ -473,7 +473,21 @@ struct AttnArgs {
   float scale, scale2;         // scale2 = scale log2(e)
   int window, tiles;
   bool causal;
+  // a tile's steps over the other axis go to up to `split` workgroups, `chunk` of
+  // them each at least (attn_split); part: what these leave for the join
+  int split, chunk;
+  bool low;
+  float* part;
 };
+// The split of each kernel's tiles (forward, dq, dk and dv), and the floats that
+// its parts take.
+enum { kAttnForward, kAttnDq, kAttnDkv };
+struct AttnSplit {
+  bool low;  // forward: tiles of half as many queries
+  int split, chunk;
+  size_t floats;
+};
+AttnSplit attn_split(int kernel, int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D, int64_t window);
 hipError_t launch_attention(int dtype, const AttnArgs& a, hipStream_t s);
 hipError_t launch_attention_backward(int dtype, const AttnArgs& a, hipStream_t s);
 

@@ -516,17 +516,22 @@ W4A16_API int w4a16_append_kv(const void* q, int64_t q_token, int64_t q_head, co
  * behind the last sequence, gets zeros (lse -inf).  lse (NULL: not wanted):
  * float32 [Hq][Tq], log sum_j exp(scale q_i k_j).  D 64, 128, 256 or 512; bf16
  * or fp16; 16-byte aligned pointers.  The weights are rounded to the type as
- * operands of the second product.  What is not finite in a key or value that a
- * query does not see does not reach it.
+ * operands of the second product.  The workspace (0 bytes where there are many
+ * tokens and heads) holds the parts of long sums that workgroups share.  What is
+ * not finite in a key or value that a query does not see does not reach it.
  * backward: gradients of q, k and v (dq NULL, or dk and dv: not wanted) for that
  * of out, with out and lse of the forward call; p, and ds = p (dp - delta), are
  * rounded to the type as operands.  What is not finite in a sequence may make any
  * of its gradients NaN, of no other sequence.                               */
+W4A16_API size_t w4a16_attention_workspace_bytes(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D,
+                                                 int64_t window);
 W4A16_API int w4a16_attention(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token,
                               int64_t k_head, const void* v, int64_t v_token, int64_t v_head, const int32_t* cu_q,
                               const int32_t* cu_k, void* out, float* lse, int dtype, int64_t B, int64_t Tq, int64_t Tk,
-                              int64_t Hq, int64_t Hk, int64_t D, float scale, int causal, int64_t window, void* stream);
-W4A16_API size_t w4a16_attention_backward_workspace_bytes(int64_t Tq, int64_t Hq);
+                              int64_t Hq, int64_t Hk, int64_t D, float scale, int causal, int64_t window,
+                              void* workspace, size_t workspace_bytes, void* stream);
+W4A16_API size_t w4a16_attention_backward_workspace_bytes(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk,
+                                                          int64_t D, int64_t window);
 W4A16_API int w4a16_attention_backward(const void* dout, const void* q, int64_t q_token, int64_t q_head, const void* k,
                                        int64_t k_token, int64_t k_head, const void* v, int64_t v_token,
                                        int64_t v_head, const void* out, const float* lse, const int32_t* cu_q,

@@ -81,9 +81,9 @@ def _attn(lib, back=False, **kw):
     sizes = dict(dtype=0, B=2, Tq=50, Tk=60, Hq=4, Hk=2, D=64, scale=0.125, causal=1, window=0)
     if back:
         a = {"dout": FAKE, **heads, "out": FAKE, "lse": FAKE, "cu_q": FAKE, "cu_k": FAKE, "dq": FAKE, "dk": FAKE,
-             "dv": FAKE, **sizes, "ws": FAKE, "bytes": 4 * 4 * 50}
+             "dv": FAKE, **sizes, "ws": FAKE, "bytes": 1 << 30}
     else:
-        a = {**heads, "cu_q": FAKE, "cu_k": FAKE, "out": FAKE, "lse": FAKE, **sizes}
+        a = {**heads, "cu_q": FAKE, "cu_k": FAKE, "out": FAKE, "lse": FAKE, **sizes, "ws": FAKE, "bytes": 1 << 30}
     assert set(kw) <= set(a)
     return (lib.w4a16_attention_backward if back else lib.w4a16_attention)(*{**a, **kw}.values(), NULL)
 
@@ -102,12 +102,18 @@ def test_attention_host_validation(lib, kw, status, back):
 
 
 def test_attention_backward_host_validation(lib):
-    assert lib.w4a16_attention_backward_workspace_bytes(50, 4) == 4 * 4 * 50
+    need = lib.w4a16_attention_backward_workspace_bytes(2, 50, 60, 4, 2, 64, 0)
+    assert need >= 4 * 4 * 50
     for kw in (dict(dk=NULL), dict(dv=NULL), dict(dout=NULL), dict(lse=NULL)):
         assert _attn(lib, True, **kw) == ERR_NULL, kw
     for kw in (dict(dq=ODD), dict(dv=ODD), dict(ws=ODD), dict(dout=ODD)):
         assert _attn(lib, True, **kw) == ALIGN, kw
-    assert _attn(lib, True, bytes=799) == _attn(lib, True, ws=NULL) == WORKSPACE
+    assert _attn(lib, True, bytes=need - 1) == _attn(lib, True, ws=NULL) == WORKSPACE
+    # one long sequence of few heads: its workgroups share the sums
+    need, sizes = lib.w4a16_attention_workspace_bytes(1, 5000, 5000, 4, 2, 64, 0), dict(B=1, Tq=5000, Tk=5000)
+    assert need > 0 and lib.w4a16_attention_workspace_bytes(1, 50000, 50000, 64, 2, 64, 0) == 0
+    assert _attn(lib, False, bytes=need - 1, **sizes) == _attn(lib, False, ws=NULL, **sizes) == WORKSPACE
+    assert _attn(lib, False, ws=ODD, **sizes) == ALIGN
     assert _attn(lib, False, Tq=0, q=NULL, out=NULL) == OK
 
 

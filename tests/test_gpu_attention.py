@@ -168,6 +168,50 @@ def test_gradients_of_other_sequences_stay_finite(D):
         ref.check(t[fine], tuple(x[fine] for x in want[name]), name)
 
 
+# ---------------------------------------------------------------- sums that workgroups share
+
+
+def _split(lens_q, lens_k, Hq, Hk, D, window=0):
+    """Whether the forward and the backward call share sums: beside them the latter has delta alone."""
+    n = (len(lens_q), sum(lens_q), sum(lens_k), Hq, Hk, D, window)
+    lib = _lib.load()
+    return lib.w4a16_attention_workspace_bytes(*n) > 0, lib.w4a16_attention_backward_workspace_bytes(*n) > 4 * n[1] * Hq + 16
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+@pytest.mark.parametrize("Hq,Hk", [(4, 1), (3, 3), (8, 2)])
+def test_shared_sums(D, Hq, Hk, dtype):
+    lens = [1500, 3, 900]
+    assert _split(lens, lens, Hq, Hk, D) == (True, True)
+    _check(*_inputs(lens, lens, Hq, Hk, D, dtype))
+
+
+@pytest.mark.parametrize("causal,window", [(True, 700), (False, 0)])
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_shared_sums_masks(D, causal, window):
+    """Other lengths too: queries without keys, tiles that no query sees, more keys than queries."""
+    lens_q, lens_k = [1300, 40, 700], [1000, 1500, 700]
+    assert _split(lens_q, lens_k, 4, 1, D, window)[1]
+    _check(*_inputs(lens_q, lens_k, 4, 1, D, BF), causal=causal, window=window)
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_shared_sums_values_that_are_not_finite(D, bad):
+    """As above; the first 100 queries see no key."""
+    lens_q, lens_k = [1600, 900], [1500, 900]
+    assert _split(lens_q, lens_k, 4, 2, D)[0]
+    q, k, v, cu_q, cu_k, _ = _inputs(lens_q, lens_k, 4, 2, D, BF)
+    clean = ref.packed(q, k, v, cu_q, cu_k, D ** -0.5, True, 0)["out"]
+    v[20, 1, 5] = v[700, 1, 5] = v[1500 + 450, 1, D - 1] = bad
+    out = _lib.attention(q, k, v, cu_q, cu_k)
+    hit = torch.zeros(2500, 4, D, dtype=torch.bool, device="cuda")
+    hit[120:1600, 2:, 5] = hit[1600 + 450:, 2:, D - 1] = True
+    assert not out[hit].isfinite().any()
+    ref.check(out.double().masked_fill(hit, 0.0), (clean[0].masked_fill(hit, 0.0), clean[1]), "out")
+
+
 # ---------------------------------------------------------------- decoding
 
 
