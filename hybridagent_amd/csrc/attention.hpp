@@ -382,9 +382,11 @@ __device__ __forceinline__ void at_rows(const int32_t* __restrict__ cu, int n, i
   }
 }
 
-// The rows of a workgroup's tile, and of the other axis' steps.
+// The rows of a workgroup's tile (low: where there are few of them), and of the other
+// axis' steps.
 constexpr int attn_rows(int kernel, int D, bool low = false) {
-  return kernel == kAttnForward ? (D == 512 ? 128 : 256) >> (low ? 1 : 0) : D == 512 ? 64 : D == 256 ? 128 : D == 128 ? 192 : 256;
+  if (kernel == kAttnForward) return (D == 512 ? 128 : 256) >> (low ? 1 : 0);
+  return D == 512 || (low && D > 64) ? 64 : D == 128 ? 192 : 128;
 }
 constexpr int attn_keys(int kernel, int D) { return kernel == kAttnForward && D < 256 ? 64 : 32; }
 constexpr int64_t kAttnParts = 512, kAttnChunk = 12, kAttnMostParts = 32, kAttnLow = 256;

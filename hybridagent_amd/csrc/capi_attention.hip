@@ -88,9 +88,8 @@ int attn_args(AttnArgs& a, const Heads& q, const Heads& k, const Heads& v, const
       Tk < 0 || Tk > kMaxTokens || bad_group(Hq, Hk) || bad_attn_dim(D) || bad_scale(scale) || window < 0 ||
       (window > 0 && !causal) || bad_stride(q, 2) || bad_stride(k, 2) || bad_stride(v, 2))
     return W4A16_ERR_SHAPE;
-  // workgroups of 64 rows at least and 512 threads; delta has a thread for eight elements
-  if ((std::max(Tq, Tk) / 64 + B + 9) * Hq > kMaxBlocks / 2 || Tq * Hq > (kMaxBlocks << 8) / (D / 8))
-    return W4A16_ERR_SHAPE;
+  // workgroups of 64 rows at least and 512 threads
+  if ((std::max(Tq, Tk) / 64 + B + 9) * Hq > kMaxBlocks / 2) return W4A16_ERR_SHAPE;
   if ((Tq > 0 && !q.p) || (Tk > 0 && (!k.p || !v.p)) || !cu_q || !cu_k) return W4A16_ERR_NULL;
   if (odd(q, 2) || odd(k, 2) || odd(v, 2)) return W4A16_ERR_ALIGN;
   a = AttnArgs{};

@@ -427,13 +427,25 @@ hipError_t fwd_type(const AttnArgs& a, bool low, hipStream_t s) {
 }  // namespace
 
 // Tiles with few heads or tokens leave most CUs idle, and a tile's steps follow one
-// another: they are cut so that there are about two workgroups per CU.
+// another: they are cut so that there are about two workgroups per CU, of kAttnChunk
+// steps at least (a part costs some 10 us of its own: its start, its sums to memory and
+// back).  4096 tokens, 8 heads and one key-value head of 128: dk and dv 1600 -> 217 us,
+// dq 182 -> 130, forward 116 -> 82; 2000 tokens, 4 heads of 256, a training step 581 ->
+// 131 us, with 8 steps at least 172, with 16 138.
 AttnSplit attn_split(int kernel, int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D, int64_t window) {
   AttnSplit r{false, 1, 1, 0};
   const bool dkv = kernel == kAttnDkv;
   const int64_t heads = dkv ? Hk : Hq, each = dkv ? Hq / Hk : 1;
   const int64_t T = dkv ? Tk : Tq, other = dkv ? Tq : Tk;
-  r.low = kernel == kAttnForward && (T / attn_rows(kernel, (int)D) + B + 1) * heads <= kAttnLow;
+  // Smaller tiles where the others leave CUs idle (forward: 180 tokens of 16 heads of
+  // 256 19 -> 14 us).  Backward, by the sequences' length: of 128, in 64 rows two
+  // workgroups share a CU, which up to 2048 tokens outweighs the operands they read
+  // twice (8 x 1024 tokens, 8 heads, dq 90 -> 56 us, dk and dv 112 -> 72; 4096 tokens
+  // 108 -> 121 and 143 -> 142); of 256 they do not fit, and a step's latency alone
+  // speaks for it (8 x 256 tokens 31 -> 27 and 44 -> 37; 2 x 1024 44 -> 54 and 59 -> 64).
+  const int64_t even = other / std::max<int64_t>(B, 1), length = window > 0 ? std::min(even, window) : even;
+  r.low = kernel == kAttnForward ? (T / attn_rows(kernel, (int)D) + B + 1) * heads <= kAttnLow
+                                 : length <= (D == 128 ? 2048 : D == 256 ? 256 : 0);
   const int64_t rows = attn_rows(kernel, (int)D, r.low), keys = attn_keys(kernel, (int)D);
   if (B <= 0 || B > 64 || T <= 0 || other <= 0) return r;
   const int64_t tiles = T / rows + B + 1;

@@ -4,7 +4,7 @@
 //   delta = sum over d of dout out      (a query's)
 //   dv = p^T dout, ds = p (dout v^T - delta), dq = scale ds k, dk = scale ds^T q
 //
-// in three launches: delta; dq, with a workgroup's queries in registers and the
+// in two launches: delta and dq, with a workgroup's queries in registers and the
 // keys and values in tiles; dk and dv, with its keys and values in registers and
 // the queries and gradients of all heads of its group in tiles.  The scores are
 // computed twice (7 products in place of 5): every sum stays in one workgroup and
@@ -37,8 +37,7 @@ namespace {
 constexpr int kPairs = 4, kBackThreads = 128 * kPairs;
 constexpr bool phases(int D) { return D < 512; }
 // 16-row tiles of a pair
-constexpr int dq_rows(int D) { return D == 512 ? 1 : D == 256 ? 2 : D == 128 ? 3 : 4; }
-constexpr int dkv_rows(int D) { return D == 512 ? 1 : D == 256 ? 2 : D == 128 ? 3 : 4; }
+constexpr int back_rows(int D, bool low) { return attn_rows(kAttnDq, D, low) / (16 * kPairs); }
 // LDS slots of A's tiles (keys, queries) and of B's (values, dout)
 constexpr int slots_a(int D) { return phases(D) ? 4 : 2; }
 constexpr int slots_b(int D) { return phases(D) ? 3 : 2; }
@@ -49,24 +48,30 @@ __device__ __forceinline__ int ring_next(int slot, int slots) { return slot == s
 
 }  // namespace
 
-// delta[h][t]: D / 8 lanes per row
-template <typename T, int D>
-__global__ __launch_bounds__(256) void k_attention_delta(AttnArgs a) {
-  constexpr int L = D / 8;
-  const int64_t row = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
-  if (row >= (int64_t)a.Tq * a.Hq) return;
-  const int64_t at = row * (D * 2) + 16 * (threadIdx.x % L);
-  const u32x4_t x = ld16(static_cast<const unsigned char*>(a.dout) + at);
-  const u32x4_t y = ld16(static_cast<const unsigned char*>(a.out) + at);
+// delta of row r, in lane c's chunks of dout's row and out's
+template <typename T, int NI>
+__device__ __forceinline__ float row_delta(const u32x4_t (&x)[NI], const u32x4_t (&y)[NI]) {
   float v = 0.f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v = __builtin_fmaf(at_lo<T>(x[i]), at_lo<T>(y[i]), v);
-    v = __builtin_fmaf(at_hi<T>(x[i]), at_hi<T>(y[i]), v);
-  }
+  for (int i = 0; i < NI; ++i)
 #pragma unroll
-  for (int o = 1; o < L; o <<= 1) v += __shfl_xor(v, o);
-  if (threadIdx.x % L == 0) {
+    for (int w = 0; w < 4; ++w) {
+      v = __builtin_fmaf(at_lo<T>(x[i][w]), at_lo<T>(y[i][w]), v);
+      v = __builtin_fmaf(at_hi<T>(x[i][w]), at_hi<T>(y[i][w]), v);
+    }
+  return at_sum_over_c(v);
+}
+
+// delta[h][t], where dq is not wanted: a wavefront has 16 rows
+template <typename T, int D>
+__global__ __launch_bounds__(256) void k_attention_delta(AttnArgs a) {
+  const int lane = threadIdx.x & 63, r = lane & 15, c = lane >> 4;
+  const int64_t rows = (int64_t)a.Tq * a.Hq, row = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 16 + r;
+  u32x4_t x[D / 32], y[D / 32];
+  at_load_row<D / 32>(static_cast<const unsigned char*>(a.dout), min(row, rows - 1), D * 2, x);
+  at_load_row<D / 32>(static_cast<const unsigned char*>(a.out), min(row, rows - 1), D * 2, y);
+  const float v = row_delta<T>(x, y);
+  if (c == 0 && row < rows) {
     const int64_t t = row / a.Hq;
     a.delta[(row - t * a.Hq) * a.Tq + t] = v;
   }
@@ -169,14 +174,20 @@ __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dq(AttnArgs a) {
   {
     const unsigned char* rp = role ? static_cast<const unsigned char*>(a.dout) + head * (D * 2)
                                    : static_cast<const unsigned char*>(a.q) + head * a.q_head;
-    const float* sp = (role ? a.delta : a.lse) + (int64_t)head * a.Tq;
+    const float* lse = a.lse + (int64_t)head * a.Tq;
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
       const int64_t q = it.first + min(q0 + 16 * n + r, nq - 1);
       at_load_row<NI>(rp, q, role ? (int64_t)a.Hq * D * 2 : a.q_stride, rows[n]);
-      const float v = sp[q];
-      // a query without keys: its scores are all masked
-      stat[n] = role ? v : v == -INFINITY ? 0.f : -v * kLog2e;
+      if (role) {
+        u32x4_t out[NI];
+        at_load_row<NI>(static_cast<const unsigned char*>(a.out) + head * (D * 2), q, (int64_t)a.Hq * D * 2, out);
+        stat[n] = row_delta<T>(rows[n], out);
+        if (part.index == 0 && c == 0 && q0 + 16 * n + r < nq) a.delta[(int64_t)head * a.Tq + q] = stat[n];
+      } else {
+        // a query without keys: its scores are all masked
+        stat[n] = lse[q] == -INFINITY ? 0.f : -lse[q] * kLog2e;
+      }
 #pragma unroll
       for (int d = 0; d < ND; ++d) acc[d][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
@@ -317,9 +328,8 @@ __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dq(AttnArgs a) {
 
 // The parts of the split tiles added up, in their order: a workgroup has
 // join_rows queries of a tile.
-template <typename T, int D>
+template <typename T, int D, int BQ>
 __global__ __launch_bounds__(256) void k_attention_dq_join(AttnArgs a) {
-  constexpr int BQ = 16 * kPairs * dq_rows(D);
   const AtPlace wg = at_place(a.Hq);
   const AtItem it = at_find(a.cu_q, a.B, a.Tq, BQ, wg.rank);
   if (it.seq < 0) return;
@@ -570,9 +580,8 @@ __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dkv(AttnArgs a) {
 }
 
 // As k_attention_dq_join: blockIdx.z 0 dv, 1 dk.
-template <typename T, int D>
+template <typename T, int D, int BK>
 __global__ __launch_bounds__(256) void k_attention_dkv_join(AttnArgs a) {
-  constexpr int BK = 16 * kPairs * dkv_rows(D);
   const AtPlace wg = at_place(a.Hk);
   const AtItem it = at_find(a.cu_k, a.B, a.Tk, BK, wg.rank);
   if (it.seq < 0) return;
@@ -589,37 +598,45 @@ __global__ __launch_bounds__(256) void k_attention_dkv_join(AttnArgs a) {
 
 namespace {
 
+template <typename T, int D, int N>
+void launch_dq(const AttnArgs& a, hipStream_t s) {
+  constexpr int BQ = 16 * N * kPairs;
+  hipLaunchKernelGGL((k_attention_dq<T, D, N>), dim3((unsigned)(a.tiles * a.Hq * a.split)), dim3(kBackThreads),
+                     back_lds(D, N), s, a);
+  if (a.split > 1)
+    hipLaunchKernelGGL((k_attention_dq_join<T, D, BQ>), dim3((unsigned)(a.tiles * a.Hq), BQ / join_rows(D)), dim3(256), 0,
+                       s, a);
+}
+template <typename T, int D, int N>
+void launch_dkv(const AttnArgs& a, hipStream_t s) {
+  constexpr int BK = 16 * N * kPairs;
+  hipLaunchKernelGGL((k_attention_dkv<T, D, N>), dim3((unsigned)(a.tiles * a.Hk * a.split)), dim3(kBackThreads),
+                     back_lds(D, N), s, a);
+  if (a.split > 1)
+    hipLaunchKernelGGL((k_attention_dkv_join<T, D, BK>), dim3((unsigned)(a.tiles * a.Hk), BK / join_rows(D), 2), dim3(256),
+                       0, s, a);
+}
+
 template <typename T, int D>
 hipError_t back(AttnArgs a, hipStream_t s) {
-  constexpr int NQ = dq_rows(D), NK = dkv_rows(D);
-  static_assert(back_lds(D, NQ) <= 160 * 1024 && back_lds(D, NK) <= 160 * 1024, "a CU's LDS");
-  if (a.Tq > 0) {
-    const int64_t rows = (int64_t)a.Tq * a.Hq, per = 256 / (D / 8);
-    hipLaunchKernelGGL((k_attention_delta<T, D>), dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, s, a);
-  }
-  constexpr int BQ = 16 * NQ * kPairs, BK = 16 * NK * kPairs;
-  static_assert(BQ == attn_rows(kAttnDq, D) && BK == attn_rows(kAttnDkv, D), "attn_split's tiles");
-  auto split = [&](int kernel) {
+  constexpr int N = back_rows(D, false), L = back_rows(D, true);
+  static_assert(back_lds(D, N) <= 160 * 1024 && attn_rows(kAttnDq, D) == attn_rows(kAttnDkv, D), "a CU's LDS");
+  auto plan = [&](int kernel, int tokens) {
     const AttnSplit p = attn_split(kernel, a.B, a.Tq, a.Tk, a.Hq, a.Hk, a.D, a.window);
     a.split = p.split;
     a.chunk = p.chunk;
+    a.low = p.low;
+    a.tiles = tokens / attn_rows(kernel, D, p.low) + a.B + 1;
   };
+  if (a.Tq > 0 && a.dq == nullptr)
+    hipLaunchKernelGGL((k_attention_delta<T, D>), dim3((unsigned)(((int64_t)a.Tq * a.Hq + 63) / 64)), dim3(256), 0, s, a);
   if (a.Tq > 0 && a.dq != nullptr) {
-    a.tiles = a.Tq / BQ + a.B + 1;
-    split(kAttnDq);
-    hipLaunchKernelGGL((k_attention_dq<T, D, NQ>), dim3((unsigned)(a.tiles * a.Hq * a.split)), dim3(kBackThreads),
-                       back_lds(D, NQ), s, a);
-    if (a.split > 1)
-      hipLaunchKernelGGL((k_attention_dq_join<T, D>), dim3((unsigned)(a.tiles * a.Hq), BQ / join_rows(D)), dim3(256), 0, s, a);
+    plan(kAttnDq, a.Tq);
+    a.low ? launch_dq<T, D, L>(a, s) : launch_dq<T, D, N>(a, s);
   }
   if (a.Tk > 0 && a.dk != nullptr) {
-    a.tiles = a.Tk / BK + a.B + 1;
-    split(kAttnDkv);
-    hipLaunchKernelGGL((k_attention_dkv<T, D, NK>), dim3((unsigned)(a.tiles * a.Hk * a.split)), dim3(kBackThreads),
-                       back_lds(D, NK), s, a);
-    if (a.split > 1)
-      hipLaunchKernelGGL((k_attention_dkv_join<T, D>), dim3((unsigned)(a.tiles * a.Hk), BK / join_rows(D), 2), dim3(256), 0, s,
-                         a);
+    plan(kAttnDkv, a.Tk);
+    a.low ? launch_dkv<T, D, L>(a, s) : launch_dkv<T, D, N>(a, s);
   }
   return hipGetLastError();
 }

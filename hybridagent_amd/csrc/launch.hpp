@@ -483,7 +483,7 @@ struct AttnArgs {
 // its parts take.
 enum { kAttnForward, kAttnDq, kAttnDkv };
 struct AttnSplit {
-  bool low;  // forward: tiles of half as many queries
+  bool low;  // tiles of fewer rows
   int split, chunk;
   size_t floats;
 };

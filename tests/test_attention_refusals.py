@@ -104,6 +104,9 @@ def test_attention_host_validation(lib, kw, status, back):
 def test_attention_backward_host_validation(lib):
     need = lib.w4a16_attention_backward_workspace_bytes(2, 50, 60, 4, 2, 64, 0)
     assert need >= 4 * 4 * 50
+    for B, Tq, Tk in ((0, 50, 60), (0, 50, 0), (5, 50, 0), (65, 50, 60), (1 << 20, 1, 1)):
+        assert lib.w4a16_attention_backward_workspace_bytes(B, Tq, Tk, 4, 2, 128, 0) == 4 * 4 * Tq
+        assert lib.w4a16_attention_workspace_bytes(B, Tq, Tk, 4, 2, 128, 0) == 0
     for kw in (dict(dk=NULL), dict(dv=NULL), dict(dout=NULL), dict(lse=NULL)):
         assert _attn(lib, True, **kw) == ERR_NULL, kw
     for kw in (dict(dq=ODD), dict(dv=ODD), dict(ws=ODD), dict(dout=ODD)):
