@@ -1348,10 +1348,10 @@ def decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     out = _dense_like(q)
     lib = load()
     nbytes = lib.w4a16_decode_attention_workspace_bytes(B, Hq, Hk, D, width * page)
-    ws = q.new_empty(nbytes, dtype=torch.uint8)
+    ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     _launch("w4a16_decode_attention", index, lib.w4a16_decode_attention, *_head_args(q), *cache,
             block_table.data_ptr(), lengths.data_ptr(), out.data_ptr(), dt, B, Hq, Hk, D, pages, page, width,
-            D ** -0.5 if scale is None else scale, window, ws.data_ptr(), nbytes)
+            D ** -0.5 if scale is None else scale, window, _ptr(ws), nbytes)
     return out
 
 

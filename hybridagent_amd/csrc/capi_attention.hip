@@ -295,8 +295,8 @@ int w4a16_attention_backward(const void* dout, const void* q, int64_t q_token, i
 }
 
 size_t w4a16_decode_attention_workspace_bytes(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t keys) {
-  if (B <= 0 || bad_group(Hq, Hk) || D <= 0 || keys <= 0) return 0;
-  return decode_attn_part_floats(decode_attn_groups(B, Hq, Hk, keys), D) * sizeof(float);
+  if (B <= 0 || bad_group(Hq, Hk) || bad_attn_dim(D) || keys <= 0) return 0;
+  return decode_attn_whole(D, keys) ? 0 : decode_attn_part_floats(decode_attn_groups(B, Hq, Hk, D, keys), D) * sizeof(float);
 }
 
 int w4a16_decode_attention(const void* q, int64_t q_token, int64_t q_head, const void* k_cache, int64_t k_page_stride,
@@ -317,8 +317,8 @@ int w4a16_decode_attention(const void* q, int64_t q_token, int64_t q_head, const
   if (odd(h, 2) || !aligned16(k_cache) || !aligned16(v_cache) || k_page_stride % 8 != 0 || v_page_stride % 8 != 0 ||
       !aligned16(out) || !aligned16(workspace))
     return W4A16_ERR_ALIGN;
-  if (workspace == nullptr || workspace_bytes < w4a16_decode_attention_workspace_bytes(B, Hq, Hk, D, keys))
-    return W4A16_ERR_WORKSPACE;
+  const size_t need = w4a16_decode_attention_workspace_bytes(B, Hq, Hk, D, keys);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return W4A16_ERR_WORKSPACE;
   DecodeAttnArgs a{};
   a.q = q;
   a.q_stride = 2 * q_token;
@@ -341,7 +341,8 @@ int w4a16_decode_attention(const void* q, int64_t q_token, int64_t q_head, const
   a.width = (int)width;
   a.scale2 = scale * 1.4426950408889634f;
   a.window = (int)std::min<int64_t>(window, INT32_MAX);
-  a.groups = decode_attn_groups(B, Hq, Hk, keys);
+  a.groups = decode_attn_groups(B, Hq, Hk, D, keys);
+  a.whole = decode_attn_whole(D, keys);
   return launch_status(launch_decode_attention(dtype, a, static_cast<hipStream_t>(stream)));
 }
 

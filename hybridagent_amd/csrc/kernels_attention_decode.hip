@@ -2,7 +2,8 @@
 // (include/w4a16moe.h, w4a16_decode_attention): the cache read once, at the
 // memory's rate.
 //
-// The keys of a sequence that the token sees are cut into steps of 128; the
+// The keys of a sequence that the token sees are cut into steps of 128.  Where there
+// are few by the table's width, a workgroup has all of a (sequence, head).  Else the
 // steps of all sequences and key-value heads (16 queries of a group at most)
 // are one row, dealt out evenly to the workgroups, whatever the lengths.  A
 // workgroup's part of a (sequence, head)'s steps is a piece: if it is all of them
@@ -16,6 +17,7 @@
 // values a lane loads the 8 x 8 block of its eight keys and eight columns, 256
 // bytes of a row per load, which 32 byte permutations turn around in its
 // registers.
+#include <algorithm>
 #include <type_traits>
 
 #include "attention.hpp"
@@ -82,8 +84,15 @@ __global__ __launch_bounds__(64 * kDaWaves, D == 512 ? 1 : 2) void k_decode_atte
     end = da_start(blockIdx.x + 1, groups, total);
     return true;
   };
-  if (a.B > 64 && !deal(da_before(a, a.B) * units)) return;
-  for (int base = 0; base < a.B; base += 64) {
+  if (a.whole) {
+    b = (int)blockIdx.x / units;
+    const int steps = da_seq(a, b).steps;
+    pos = ((int)blockIdx.x - b * units) * steps;
+    end = pos + steps;
+  } else if (a.B > 64 && !deal(da_before(a, a.B) * units)) {
+    return;
+  }
+  for (int base = 0; !a.whole && base < a.B; base += 64) {
     const int n = base + lane < a.B ? da_seq(a, base + lane).steps * units : 0;
     int sum = n;
 #pragma unroll
@@ -371,8 +380,7 @@ namespace {
 template <typename T, int D>
 hipError_t decode(const DecodeAttnArgs& a, hipStream_t s) {
   hipLaunchKernelGGL((k_decode_attention<T, D>), dim3(a.groups), dim3(64 * kDaWaves), kDaWaves * D * 16 * 4, s, a);
-  // a step is never cut: with one at most there are no pieces
-  if ((a.width << a.page_log2) > kDaStep)
+  if (!a.whole)
     hipLaunchKernelGGL((k_decode_join<T, D>), dim3((unsigned)(a.B * a.Hk * ((a.group + 15) / 16)),
                                                     (unsigned)(a.group < 16 ? a.group : 16)),
                        dim3(256), 0, s, a);
@@ -392,7 +400,13 @@ hipError_t decode_type(const DecodeAttnArgs& a, hipStream_t s) {
 
 }  // namespace
 
-int decode_attn_groups(int64_t B, int64_t Hq, int64_t Hk, int64_t keys) {
+// Few steps: a workgroup has all of a (sequence, head)'s, without pieces and their join,
+// which cost about 4 us of both sides (181 keys, heads of 256: 16.7 -> 12.3 us a call;
+// 4 x 1000 keys of 128 16.2 -> 14.4; too many, 1000 keys of 256 16.6 -> 25.8, 512 of 512
+// 20.3 -> 29.1).
+bool decode_attn_whole(int64_t D, int64_t keys) { return keys <= kDaStep * std::min<int64_t>(8, 1024 / D); }
+int decode_attn_groups(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t keys) {
+  if (decode_attn_whole(D, keys)) return (int)(B * Hk * ((Hq / Hk + 15) / 16));
   const int64_t steps = (keys + kDaStep - 1) / kDaStep + 1;  // a window may start inside one
   const int64_t units = B * Hk * ((Hq / Hk + 15) / 16);
   return units * steps < kDecodeAttnGroups ? (int)(units * steps) : kDecodeAttnGroups;

@@ -502,9 +502,11 @@ struct DecodeAttnArgs {
   int page_log2, pages, width;
   float scale2;
   int window, groups;                        // workgroups
+  bool whole;                                // each has all of a (sequence, head)
 };
-constexpr int kDecodeAttnGroups = 256;       // workgroups at most: one per CU
-int decode_attn_groups(int64_t B, int64_t Hq, int64_t Hk, int64_t keys);
+constexpr int kDecodeAttnGroups = 256;       // workgroups at most, where they share: one per CU
+bool decode_attn_whole(int64_t D, int64_t keys);
+int decode_attn_groups(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t keys);
 size_t decode_attn_part_floats(int64_t groups, int64_t D);
 hipError_t launch_decode_attention(int dtype, const DecodeAttnArgs& a, hipStream_t s);
 // CUs of the current device

@@ -546,7 +546,7 @@ W4A16_API int w4a16_attention_backward(const void* dout, const void* q, int64_t 
  * block_table[b][j / page_size] (int32 [B][width]).  Lengths of zero and less
  * give zeros; a length over width * page_size, or a page outside the cache among
  * those that the token sees, gives NaN.  Entries of pages it does not see are
- * not read from.  `keys` of the workspace: width * page_size.               */
+ * not read from.  `keys` of the workspace: width * page_size (few need none: 0 bytes). */
 W4A16_API size_t w4a16_decode_attention_workspace_bytes(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t keys);
 W4A16_API int w4a16_decode_attention(const void* q, int64_t q_token, int64_t q_head, const void* k_cache,
                                      int64_t k_page_stride, const void* v_cache, int64_t v_page_stride,

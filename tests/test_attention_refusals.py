@@ -121,11 +121,12 @@ def test_attention_backward_host_validation(lib):
 
 
 def test_decode_host_validation(lib):
-    need = lib.w4a16_decode_attention_workspace_bytes(3, 4, 2, 64, 128)
+    need = lib.w4a16_decode_attention_workspace_bytes(3, 4, 2, 64, 2048)
+    assert need > 0 and lib.w4a16_decode_attention_workspace_bytes(3, 4, 2, 64, 128) == 0
 
     def call(**kw):
         a = dict(q=FAKE, qt=256, qh=64, kc=FAKE, kp=2 * 16 * 64, vc=FAKE, vp=2 * 16 * 64, table=FAKE, lengths=FAKE,
-                 out=FAKE, dtype=0, B=3, Hq=4, Hk=2, D=64, pages=9, page=16, width=8, scale=0.125, window=0, ws=FAKE,
+                 out=FAKE, dtype=0, B=3, Hq=4, Hk=2, D=64, pages=9, page=16, width=128, scale=0.125, window=0, ws=FAKE,
                  bytes=need)
         return lib.w4a16_decode_attention(*{**a, **kw}.values(), NULL)
 
@@ -139,7 +140,7 @@ def test_decode_host_validation(lib):
         assert call(**kw) == ALIGN, kw
     assert call(bytes=need - 1) == call(ws=NULL) == WORKSPACE
     assert call(B=0) == OK
-    assert lib.w4a16_decode_attention_workspace_bytes(0, 4, 2, 64, 128) == 0
+    assert lib.w4a16_decode_attention_workspace_bytes(0, 4, 2, 64, 2048) == 0
 
 
 # ---------------------------------------------------------------- the Python functions

@@ -270,6 +270,16 @@ def test_decode_long(D):
     _decode([9000, 3, 2500], 8, 1, D, 64, BF)
 
 
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_decode_around_a_workgroup_of_its_own(D):
+    """Tables on both sides of the width up to which a workgroup has all of a sequence's keys."""
+    limit = 128 * min(8, 1024 // D)
+    lib = _lib.load()
+    for width, whole in ((limit // 16, True), (limit // 16 + 1, False)):
+        assert (lib.w4a16_decode_attention_workspace_bytes(3, 6, 2, D, width * 16) == 0) == whole
+        _decode([limit, 1, limit - 37, 0, 130], 6, 2, D, 16, BF, width=width)
+
+
 def test_decode_many_sequences():
     _decode([(37 * i) % 211 for i in range(150)], 2, 1, 64, 16, BF)
 
