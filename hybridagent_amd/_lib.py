@@ -1078,28 +1078,32 @@ def _dense_like(t: torch.Tensor) -> torch.Tensor:
     return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
 
 
-def _dense(t: torch.Tensor) -> torch.Tensor:
-    """t contiguous, at a multiple of 16 bytes."""
-    return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else _aligned(t.contiguous())
+def _dense(t: torch.Tensor):
+    """t contiguous, at a multiple of 16 bytes, and its address."""
+    p = t.data_ptr()
+    if p & 15 or not t.is_contiguous():
+        t = _aligned(t.contiguous())
+        p = t.data_ptr()
+    return t, p
 
 
-def _heads(t: torch.Tensor, name: str) -> torch.Tensor:
-    """t [tokens, heads, D] as the kernels take it: D contiguous, the other strides as they are where
-    every row starts at a multiple of 16 bytes and they are 64 MiB at most, else a copy."""
+_NO_HEADS = (None, 0, 0)
+_LANES = {torch.bfloat16: 8, torch.float16: 8, torch.float32: 4}  # elements of 16 bytes
+
+
+def _heads(t: torch.Tensor, name: str):
+    """t [tokens, heads, D] as the kernels take it, and its pointer and strides for them: D contiguous, the
+    other strides as they are where every row starts at a multiple of 16 bytes and they are 64 MiB at
+    most, else a copy."""
     if t.dim() != 3:
         raise ValueError(f"{name} must be [tokens, heads, head size], got {list(t.shape)}")
     a, b, c = t.stride()
-    size = t.element_size()
-    if c == 1 and (a * size | b * size | t.data_ptr()) & 15 == 0 and max(a, b) * size <= 1 << 26:
-        return t
-    return t.clone(memory_format=torch.contiguous_format)  # a size of one leaves contiguous()'s strides open
-
-
-def _head_args(t: torch.Tensor | None):
-    if t is None:
-        return None, 0, 0
-    a, b, _ = t.stride()
-    return t.data_ptr(), a, b
+    p = t.data_ptr()
+    lanes = _LANES.get(t.dtype, 8)
+    if c != 1 or (a | b) % lanes or p & 15 or a > lanes << 22 or b > lanes << 22:
+        t = t.clone(memory_format=torch.contiguous_format)  # a size of one leaves contiguous()'s strides open
+        p, (a, b, c) = t.data_ptr(), t.stride()
+    return t, (p, a, b)
 
 
 def _head_type(t: torch.Tensor, name: str, fp32: bool) -> int:
@@ -1116,28 +1120,34 @@ def _index(t: torch.Tensor, name: str, *shape: int) -> torch.Tensor:
 
 
 def _rope_args(q, k, v, cos, sin, positions, q_weight, k_weight, fp32: bool):
-    """What the forms of the heads' norm check alike -> (type, q, k, v, (cos, sin, positions, weights),
-    sizes)."""
+    """What the forms of the heads' norm check alike -> (type, q, k, v, the pointers and strides of these,
+    (cos, sin, positions, weights), the pointers of these, sizes)."""
     dtype = q.dtype
     dt = _head_type(q, "q", fp32)
-    q = _heads(q, "q")
+    q, args = _heads(q, "q")
     T, Hq, D = q.shape
-    k = _heads(k, "k")
+    k, more = _heads(k, "k")
+    args += more
     shape = k.shape
     if k.dtype != dtype or shape[0] != T or shape[2] != D:
         raise ValueError(f"k must be {dtype} [{T}, heads, {D}], got {k.dtype} {list(shape)}")
     if v is not None:
-        v = _heads(v, "v")
+        v, more = _heads(v, "v")
+        args += more
         if v.dtype != dtype or v.shape != shape:
             raise ValueError(f"v must be {dtype} {list(shape)}, got {v.dtype} {list(v.shape)}")
+    else:
+        args += _NO_HEADS
     P = R = 0
+    pc = ps = pq = pk = None
     if cos is not None and sin is not None:
         table = cos.shape
         if cos.dtype != torch.float32 or sin.dtype != torch.float32 or len(table) != 2 or sin.shape != table:
             raise ValueError("cos and sin must be float32 [positions, half the turned columns], got "
                              f"{cos.dtype} {list(table)} and {sin.dtype} {list(sin.shape)}")
         P, R = table[0], 2 * table[1]
-        cos, sin = _dense(cos), _dense(sin)
+        cos, pc = _dense(cos)
+        sin, ps = _dense(sin)
     elif cos is not None or sin is not None:
         raise ValueError("cos and sin are given together")
     positions = _index(positions, "positions", T)
@@ -1145,10 +1155,12 @@ def _rope_args(q, k, v, cos, sin, positions, q_weight, k_weight, fp32: bool):
         for t, n in ((q_weight, "q_weight"), (k_weight, "k_weight")):
             if t.dtype != dtype or t.shape != (D,):
                 raise ValueError(f"{n} must be {dtype} [{D}], got {t.dtype} {list(t.shape)}")
-        q_weight, k_weight = _dense(q_weight), _dense(k_weight)
+        q_weight, pq = _dense(q_weight)
+        k_weight, pk = _dense(k_weight)
     elif q_weight is not None or k_weight is not None:
         raise ValueError("q_weight and k_weight are given together")
-    return dt, q, k, v, (cos, sin, positions, q_weight, k_weight), (T, Hq, shape[1], D, P, R)
+    return (dt, q, k, v, args, (cos, sin, positions, q_weight, k_weight), (pc, ps, positions.data_ptr(), pq, pk),
+            (T, Hq, shape[1], D, P, R))
 
 
 def head_norm_rope(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor | None, cos: torch.Tensor | None,
@@ -1161,11 +1173,11 @@ def head_norm_rope(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor | None, cos
     turned by row ``positions[t]`` (int32).  v (may be None) is normed without a weight.  A position
     that the tables do not have makes its token's q and k NaN."""
     index = _gpu_of(q, k, v, cos, sin, positions, q_weight, k_weight)
-    dt, q, k, v, rot, sizes = _rope_args(q, k, v, cos, sin, positions, q_weight, k_weight, True)
+    dt, q, k, v, heads, rot, at, sizes = _rope_args(q, k, v, cos, sin, positions, q_weight, k_weight, True)
     yq, yk = _dense_like(q), _dense_like(k)
     yv = None if v is None else _dense_like(v)
-    _launch("w4a16_head_norm_rope", index, load().w4a16_head_norm_rope, *_head_args(q), *_head_args(k),
-            *_head_args(v), *map(_ptr, rot), yq.data_ptr(), yk.data_ptr(), _ptr(yv), dt, *sizes, eps)
+    _launch("w4a16_head_norm_rope", index, load().w4a16_head_norm_rope, *heads, *at, yq.data_ptr(), yk.data_ptr(),
+            _ptr(yv), dt, *sizes, eps)
     return yq, yk, yv
 
 
@@ -1177,13 +1189,15 @@ def head_norm_rope_backward(dq: torch.Tensor, dk: torch.Tensor, dv: torch.Tensor
     weights' are None without weights and where ``weights`` is False; dv is None without v.  The sums
     over the rows are taken in fp32, in an order set by the shapes."""
     index = _gpu_of(q, k, v, cos, sin, positions, q_weight, k_weight, dq, dk, dv)
-    dt, q, k, v, rot, sizes = _rope_args(q, k, v, cos, sin, positions, q_weight, k_weight, True)
+    dt, q, k, v, heads, rot, at, sizes = _rope_args(q, k, v, cos, sin, positions, q_weight, k_weight, True)
     if (dv is None) != (v is None):
         raise ValueError("dv is given with v")
     for t, x, n in ((dq, q, "dq"), (dk, k, "dk"), (dv, v, "dv")):
         if t is not None and (t.shape != x.shape or t.dtype != x.dtype):
             raise ValueError(f"{n} must be {x.dtype} {list(x.shape)}, got {t.dtype} {list(t.shape)}")
-    dq, dk, dv = _dense(dq), _dense(dk), None if dv is None else _dense(dv)
+    dq, pq = _dense(dq)
+    dk, pk = _dense(dk)
+    dv, pv = (None, None) if dv is None else _dense(dv)
     xq, xk = torch.empty_like(dq), torch.empty_like(dk)
     xv = None if dv is None else torch.empty_like(dv)
     wq = wk = ws = None
@@ -1192,9 +1206,8 @@ def head_norm_rope_backward(dq: torch.Tensor, dk: torch.Tensor, dv: torch.Tensor
         wq, wk = torch.empty_like(rot[3]), torch.empty_like(rot[4])
         nbytes = lib.w4a16_head_norm_rope_backward_workspace_bytes(*sizes[:4])
         ws = q.new_empty(nbytes, dtype=torch.uint8)
-    _launch("w4a16_head_norm_rope_backward", index, lib.w4a16_head_norm_rope_backward, dq.data_ptr(), dk.data_ptr(),
-            _ptr(dv), *_head_args(q), *_head_args(k), *_head_args(v), *map(_ptr, rot), xq.data_ptr(), xk.data_ptr(),
-            _ptr(xv), _ptr(wq), _ptr(wk), dt, *sizes, eps, _ptr(ws), nbytes)
+    _launch("w4a16_head_norm_rope_backward", index, lib.w4a16_head_norm_rope_backward, pq, pk, pv, *heads, *at,
+            xq.data_ptr(), xk.data_ptr(), _ptr(xv), _ptr(wq), _ptr(wk), dt, *sizes, eps, _ptr(ws), nbytes)
     return xq, xk, xv, wq, wk
 
 
@@ -1230,17 +1243,16 @@ def append_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tens
     if v is None:
         raise ValueError("v must be given")
     index = _gpu_of(q, k, v, cos, sin, positions, q_weight, k_weight, slots, k_cache, v_cache)
-    dt, q, k, v, rot, sizes = _rope_args(q, k, v, cos, sin, positions, q_weight, k_weight, False)
+    dt, q, k, v, heads, rot, at, sizes = _rope_args(q, k, v, cos, sin, positions, q_weight, k_weight, False)
     slots = _index(slots, "slots", sizes[0])
     cache, pages, H, page = _cache_args(k_cache, v_cache, q.dtype, sizes[3])
     if H != sizes[2]:
         raise ValueError(f"the cache has {H} heads, k {sizes[2]}")
     out = _dense_like(q)
     yk, yv = (_dense_like(k), _dense_like(v)) if return_kv else (None, None)
-    cos, sin, positions, q_weight, k_weight = rot
-    _launch("w4a16_append_kv", index, load().w4a16_append_kv, *_head_args(q), *_head_args(k), *_head_args(v),
-            _ptr(cos), _ptr(sin), positions.data_ptr(), slots.data_ptr(), _ptr(q_weight), _ptr(k_weight),
-            out.data_ptr(), _ptr(yk), _ptr(yv), *cache, dt, bool(v_norm), *sizes, pages, page, eps)
+    pc, ps, pp, pq, pk = at
+    _launch("w4a16_append_kv", index, load().w4a16_append_kv, *heads, pc, ps, pp, slots.data_ptr(), pq, pk, out.data_ptr(),
+            _ptr(yk), _ptr(yv), *cache, dt, bool(v_norm), *sizes, pages, page, eps)
     return (out, yk, yv) if return_kv else out
 
 
@@ -1253,7 +1265,9 @@ def _group(Hq: int, Hk: int, D: int) -> None:
 
 def _attention_args(q, k, v, cu_q, cu_k, scale, causal, window):
     dt = _head_type(q, "q", False)
-    q, k, v = _heads(q, "q"), _heads(k, "k"), _heads(v, "v")
+    q, args = _heads(q, "q")
+    k, more = _heads(k, "k")
+    v, last = _heads(v, "v")
     Tq, Hq, D = q.shape
     Tk, Hk, _ = shape = k.shape
     if k.dtype != q.dtype or v.dtype != q.dtype or shape[2] != D or v.shape != shape:
@@ -1273,7 +1287,7 @@ def _attention_args(q, k, v, cu_q, cu_k, scale, causal, window):
     if window and not causal:
         raise ValueError("a window needs a causal mask")
     sizes = (n - 1, Tq, Tk, Hq, Hk, D, D ** -0.5 if scale is None else scale, bool(causal), window)
-    return dt, q, k, v, cu_q, cu_k, sizes
+    return dt, q, k, v, args + more + last, cu_q, cu_k, sizes
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, cu_k: torch.Tensor | None = None,
@@ -1287,14 +1301,13 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Ten
     query sees the keys up to where it stands, with ``window`` the last so many of them.  A query
     that sees none, and rows behind the last sequence, are zero.  ``scale`` is D^-1/2 if None."""
     index = _gpu_of(q, k, v, cu_q, cu_k)
-    dt, q, k, v, cu_q, cu_k, sizes = _attention_args(q, k, v, cu_q, cu_k, scale, causal, window)
+    dt, q, k, v, heads, cu_q, cu_k, sizes = _attention_args(q, k, v, cu_q, cu_k, scale, causal, window)
     out = _dense_like(q)
     lse = q.new_empty((sizes[3], sizes[1]), dtype=torch.float32) if return_lse else None
     lib = load()
     nbytes = lib.w4a16_attention_workspace_bytes(*sizes[:6], window)
     ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-    _launch("w4a16_attention", index, lib.w4a16_attention, *_head_args(q), *_head_args(k), *_head_args(v),
-            cu_q.data_ptr(), cu_k.data_ptr(), out.data_ptr(), _ptr(lse), dt, *sizes, _ptr(ws), nbytes)
+    _launch("w4a16_attention", index, lib.w4a16_attention, *heads, cu_q.data_ptr(), cu_k.data_ptr(), out.data_ptr(), _ptr(lse), dt, *sizes, _ptr(ws), nbytes)
     return (out, lse) if return_lse else out
 
 
@@ -1304,7 +1317,7 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
     """(dq, dk, dv) of ``attention`` for the gradient ``dout`` of its output and the ``out`` and ``lse`` of
     that forward call.  ``needs``: which of the three are wanted; the others are None."""
     index = _gpu_of(q, k, v, cu_q, cu_k, dout, out, lse)
-    dt, q, k, v, cu_q, cu_k, sizes = _attention_args(q, k, v, cu_q, cu_k, scale, causal, window)
+    dt, q, k, v, heads, cu_q, cu_k, sizes = _attention_args(q, k, v, cu_q, cu_k, scale, causal, window)
     for t, n in ((dout, "dout"), (out, "out")):
         if t.shape != q.shape or t.dtype != q.dtype:
             raise ValueError(f"{n} must be {q.dtype} {list(q.shape)}, got {t.dtype} {list(t.shape)}")
@@ -1313,15 +1326,16 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
         raise ValueError(f"lse must be float32 {[Hq, Tq]}, got {lse.dtype} {list(lse.shape)}")
     if len(needs) != 3:
         raise ValueError("needs must say for each of dq, dk and dv whether it is wanted")
-    dout, out, lse = _dense(dout), _dense(out), lse.contiguous()
+    dout, pd = _dense(dout)
+    out, po = _dense(out)
+    lse = lse.contiguous()
     dq = torch.empty_like(dout) if needs[0] else None
     dk, dv = (_dense_like(k), _dense_like(v)) if needs[1] or needs[2] else (None, None)
     lib = load()
     nbytes = lib.w4a16_attention_backward_workspace_bytes(*sizes[:6], window)
     ws = q.new_empty(nbytes, dtype=torch.uint8)
-    _launch("w4a16_attention_backward", index, lib.w4a16_attention_backward, dout.data_ptr(), *_head_args(q),
-            *_head_args(k), *_head_args(v), out.data_ptr(), lse.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(),
-            _ptr(dq), _ptr(dk), _ptr(dv), dt, *sizes, ws.data_ptr(), nbytes)
+    _launch("w4a16_attention_backward", index, lib.w4a16_attention_backward, pd, *heads, po, lse.data_ptr(),
+            cu_q.data_ptr(), cu_k.data_ptr(), _ptr(dq), _ptr(dk), _ptr(dv), dt, *sizes, ws.data_ptr(), nbytes)
     return dq, dk if needs[1] else None, dv if needs[2] else None
 
 
@@ -1336,7 +1350,7 @@ def decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     does not have, NaN."""
     index = _gpu_of(q, k_cache, v_cache, block_table, lengths)
     dt = _head_type(q, "q", False)
-    q = _heads(q, "q")
+    q, heads = _heads(q, "q")
     B, Hq, D = q.shape
     cache, pages, Hk, page = _cache_args(k_cache, v_cache, q.dtype, D)
     _group(Hq, Hk, D)
@@ -1349,7 +1363,7 @@ def decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     lib = load()
     nbytes = lib.w4a16_decode_attention_workspace_bytes(B, Hq, Hk, D, width * page)
     ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-    _launch("w4a16_decode_attention", index, lib.w4a16_decode_attention, *_head_args(q), *cache,
+    _launch("w4a16_decode_attention", index, lib.w4a16_decode_attention, *heads, *cache,
             block_table.data_ptr(), lengths.data_ptr(), out.data_ptr(), dt, B, Hq, Hk, D, pages, page, width,
             D ** -0.5 if scale is None else scale, window, _ptr(ws), nbytes)
     return out
