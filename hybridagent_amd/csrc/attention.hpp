@@ -182,11 +182,13 @@ struct AtCols {
 // Steps of one address come one after the other: it is not kept for later.
 template <int NI>
 __device__ __forceinline__ constexpr int at_row_step(int j) {
-  return NI < 4 ? j >> 1 : 4 * ((j >> 1) % (NI / 4)) + (j >> 1) / (NI / 4);
+  constexpr int n = NI < 4 ? 1 : NI / 4;
+  return NI < 4 ? j >> 1 : 4 * ((j >> 1) % n) + (j >> 1) / n;
 }
 template <int ND>
 __device__ __forceinline__ constexpr int at_col_step(int j) {
-  return ND < 8 ? j : 8 * (j % (ND / 8)) + j / (ND / 8);
+  constexpr int n = ND < 8 ? 1 : ND / 8;
+  return ND < 8 ? j : 8 * (j % n) + j / n;
 }
 // s[t][n] = rows of the tile . columns b[n], over 32 NI columns of D from the one
 // that the lane's addresses stand at

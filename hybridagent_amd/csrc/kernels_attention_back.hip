@@ -7,8 +7,9 @@
 // in two launches: delta and dq, with a workgroup's queries in registers and the
 // keys and values in tiles; dk and dv, with its keys and values in registers and
 // the queries and gradients of all heads of its group in tiles.  The scores are
-// computed twice (7 products in place of 5): every sum stays in one workgroup and
-// in one order, without atomics.
+// computed twice (7 products in place of 5): every sum stays in one workgroup, or in
+// the few that share a tile's steps (attn_split) and a join of theirs, and in one
+// order, without atomics.
 //
 // In the last two a pair of wavefronts of one SIMD shares 16 N rows: A has the
 // scores and p, B dout v^T and ds.  p, in fp32, and dq's ds pass between them
@@ -121,7 +122,7 @@ __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dq(AttnArgs a) {
   constexpr int BQ = 16 * NQ * kPairs;
   constexpr int NI = D / 32, ND = D / 32;  // a wavefront sums half of dq's columns
   constexpr int kTile = at_tile_bytes<D>();
-  constexpr int kAhead = 2;
+  constexpr int kAhead = D == 256 ? 4 : 2;  // (2: 384 us where 4 take 375; dk and dv have no room)
   // steps that the loads are ahead: A's in the second phase, B's in the first
   constexpr int kAheadA = phases(D) ? SA - 2 : 1, kAheadB = SB - 1;
   using Feed = AtFeed<D, kPairs>;
