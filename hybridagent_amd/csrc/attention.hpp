@@ -242,31 +242,41 @@ __device__ __forceinline__ void at_accumulate(const AtLane<D>& ln, uint32_t tile
 }
 
 // Tiles of 32 rows of a matrix of D columns, into LDS by direct loads of NW
-// wavefronts.
+// wavefronts.  A cursor goes over the rows in scalar registers: an address from the
+// row's number took 300 cycles of a step.
 template <int D, int NW>
 struct AtFeed {
   static constexpr int kLoads = D / 16 / NW;  // 1 KB loads of a tile, per wavefront
   static_assert(kLoads * NW * 16 == D, "every wavefront as many");
   static constexpr int kStep = 512 / D * NW;  // rows between a wavefront's loads
-  int wave;
-  int64_t stride;  // bytes
-  const unsigned char* p;
+  int wave, one;                              // one: bytes from row to row
+  const unsigned char *matrix, *p;            // p: the next tile's first row
+  int left;                                   // rows from there on
   int off, ch;  // a lane's of the first load: bytes to its row, in the row
 
-  __device__ __forceinline__ void init(const unsigned char* matrix, int64_t stride_bytes, int wave_) {
+  __device__ __forceinline__ void init(const unsigned char* m, int64_t stride_bytes, int wave_) {
     wave = wave_;
-    stride = stride_bytes;
-    p = matrix;
+    one = __builtin_amdgcn_readfirstlane((int)stride_bytes);
+    matrix = p = m;
+    left = 0;
     const int lane = threadIdx.x & 63, row = 512 / D * wave + lane / (D / 8);
-    off = row * (int)stride;
+    off = row * one;
     ch = 16 * ((lane % (D / 8)) ^ at_swz<D>(row));
   }
-  // rows first .. of `rows` in all (past the last, it again; none: nothing is
-  // read); more: bytes in front of the matrix's own first
-  __device__ __forceinline__ void issue(unsigned char* tile, int first, int rows, int64_t more = 0) const {
-    const int last = rows > 0 ? rows - 1 - first : -1;
-    const auto rsrc = make_rsrc(p + first * stride + more, last < 0 ? 0u : 0x7FFFFFFFu);
-    const int one = __builtin_amdgcn_readfirstlane((int)stride);
+  // to row `first` of `rows`, `more` bytes further
+  __device__ __forceinline__ void seek(int first, int rows, int64_t more = 0) {
+    p = matrix + (int64_t)first * one + more;
+    left = rows - first;
+  }
+  // tiles on (n may be negative)
+  __device__ __forceinline__ void skip(int n) {
+    p += (int64_t)(32 * n) * one;
+    left -= 32 * n;
+  }
+  // The next tile's rows (past the last, it again; none, or !any: nothing is read).
+  __device__ __forceinline__ void issue(unsigned char* tile, bool any) const {
+    const int last = any ? left - 1 : -1;
+    const auto rsrc = make_rsrc(p, last < 0 ? 0u : 0x7FFFFFFFu);
     tile += 1024 * wave;
     // rows past the first load's are other bits of the row: so is their swizzle
     // (opaque: no register is kept for each load over the steps)

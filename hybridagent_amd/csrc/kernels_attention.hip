@@ -122,11 +122,14 @@ __global__ __launch_bounds__(64 * kWaves, NQ == 1 && D <= 128 ? 4 : 2) void k_at
     else
       feed.init(static_cast<const unsigned char*>(a.k) + k_first * a.k_stride + kvh * a.k_head, a.k_stride, wave);
   }
+  feed.seek(lo, hi);
   unsigned char* const ring = smem + (second ? S * kStepBytes : 0);
   auto issue = [&](int slot, int t) {
 #pragma unroll
-    for (int k = 0; k < KT; ++k)
-      feed.issue(ring + slot * kStepBytes + k * kTile, lo + kKeys * t + 32 * k, t < steps ? hi : 0);
+    for (int k = 0; k < KT; ++k) {
+      feed.issue(ring + slot * kStepBytes + k * kTile, t < steps);
+      feed.skip(1);
+    }
   };
 #pragma unroll
   for (int s = 0; s < S - 1; ++s) issue(s, s);

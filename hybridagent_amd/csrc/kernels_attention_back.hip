@@ -157,10 +157,12 @@ __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dq(AttnArgs a) {
     else
       feed.init(static_cast<const unsigned char*>(a.k) + k_first * a.k_stride + kvh * a.k_head, a.k_stride, place);
   }
+  feed.seek(lo, hi);
   unsigned char* const ring = smem + (role ? SA * kTile : 0);
   int load = 0, to = 0;  // the next step to load, its slot
   auto issue = [&] {
-    feed.issue(ring + to * kTile, lo + 32 * load, load < steps ? hi : 0);
+    feed.issue(ring + to * kTile, load < steps);
+    feed.skip(1);
     ++load;
     to = ring_next(to, role ? SB : SA);
   };
@@ -208,7 +210,7 @@ __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dq(AttnArgs a) {
   auto active_at = [&](int t) { return lo + 32 * t < whi && lo + 32 * t + 32 > wlo; };
   // X: ds times the keys in slot `from`, and the scores, or dout v^T, of the step
   // whose tiles are in ka, vb
-  auto products = [&](bool sum, bool scores, int from, int ka, int vb) {
+  auto products = [&](auto role, bool sum, bool scores, int from, int ka, int vb) {
     const uint32_t v = base + from * kTile, w = base + (role ? SA + vb : ka) * kTile;
     u32x4_t next[kAhead];
     if (sum)
@@ -251,9 +253,9 @@ __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dq(AttnArgs a) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const f32x4_t w = xp[(u * NQ + n) * 64];
-        // (a masked key's dout v^T may be anything)
+        // (a masked key's weight is zero, and its row one of the sequence's own)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[u][n][i] = w[i] == 0.f ? 0.f : w[i] * (s[u][n][i] - stat[n]);
+        for (int i = 0; i < 4; ++i) s[u][n][i] = w[i] * (s[u][n][i] - stat[n]);
       }
       p[n] = at_pack8<T>(s[0][n], s[1][n]);
       xd[n * 64] = p[n];
@@ -264,60 +266,67 @@ __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dq(AttnArgs a) {
     for (int n = 0; n < NQ; ++n) p[n] = xd[n * 64];
   };
 
-  if constexpr (phases(D)) {
-    // slots of the keys of step t and of the two before
-    int ka = 0, ka1 = SA - 1, ka2 = SA - 2, vb = 0;
-    bool now = false, before = false;  // whether the steps t - 1, t - 2 were active
-    if (role) px_barrier();
-    for (int t = 0; t < steps; ++t) {
-      static_assert(kAheadA == kAheadB, "one wait for both");
-      __builtin_amdgcn_s_waitcnt(px_vm_wait((kAheadA - 1) * Feed::kLoads));
-      px_barrier();
-      if (role) issue();
-      const bool sum = role ? now : before;
-      before = now;
-      now = active_at(t);
-      __builtin_amdgcn_s_setprio(1);
-      products(sum, now, role ? ka1 : ka2, ka, vb);
-      __builtin_amdgcn_s_setprio(0);
+  // (each role's loop by itself: in one the compiler copies registers where they meet)
+  auto run = [&](auto role) {
+    if constexpr (phases(D)) {
+      // slots of the keys of step t and of the two before
+      int ka = 0, ka1 = SA - 1, ka2 = SA - 2, vb = 0;
+      bool now = false, before = false;  // whether the steps t - 1, t - 2 were active
+      if (role) px_barrier();
+      for (int t = 0; t < steps; ++t) {
+        static_assert(kAheadA == kAheadB, "one wait for both");
+        __builtin_amdgcn_s_waitcnt(px_vm_wait((kAheadA - 1) * Feed::kLoads));
+        px_barrier();
+        if (role) issue();
+        const bool sum = role ? now : before;
+        before = now;
+        now = active_at(t);
+        __builtin_amdgcn_s_setprio(1);
+        products(role, sum, now, role ? ka1 : ka2, ka, vb);
+        __builtin_amdgcn_s_setprio(0);
+        px_barrier();
+        if (!role) {
+          issue();
+          if (now) weights(t);
+          if (before) take();
+        } else if (now) {
+          slopes();
+        }
+        ka2 = ka1;
+        ka1 = ka;
+        ka = ring_next(ka, SA);
+        vb = ring_next(vb, SB);
+      }
+      // ka1: the last step's
       px_barrier();
       if (!role) {
-        issue();
-        if (now) weights(t);
-        if (before) take();
-      } else if (now) {
-        slopes();
+        products(role, before, false, ka2, ka, vb);
+        px_barrier();
+        if (now) take();
       }
-      ka2 = ka1;
-      ka1 = ka;
-      ka = ring_next(ka, SA);
-      vb = ring_next(vb, SB);
+      products(role, now, false, ka1, ka, vb);
+    } else {
+      int slot = 0;
+      for (int t = 0; t < steps; ++t) {
+        __builtin_amdgcn_s_waitcnt(px_vm_wait(0));
+        px_barrier();
+        issue();
+        const bool now = active_at(t);
+        products(role, false, now, slot, slot, slot);
+        if (now && !role) weights(t);
+        px_barrier();
+        if (now && role) slopes();
+        px_barrier();
+        if (now && !role) take();
+        products(role, now, false, slot, slot, slot);
+        slot = ring_next(slot, SA);
+      }
     }
-    // ka1: the last step's
-    px_barrier();
-    if (!role) {
-      products(before, false, ka2, ka, vb);
-      px_barrier();
-      if (now) take();
-    }
-    products(now, false, ka1, ka, vb);
-  } else {
-    int slot = 0;
-    for (int t = 0; t < steps; ++t) {
-      __builtin_amdgcn_s_waitcnt(px_vm_wait(0));
-      px_barrier();
-      issue();
-      const bool now = active_at(t);
-      products(false, now, slot, slot, slot);
-      if (now && !role) weights(t);
-      px_barrier();
-      if (now && role) slopes();
-      px_barrier();
-      if (now && !role) take();
-      products(now, false, slot, slot, slot);
-      slot = ring_next(slot, SA);
-    }
-  }
+  };
+  if (role)
+    run(std::true_type{});
+  else
+    run(std::false_type{});
 
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
@@ -415,10 +424,15 @@ __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dkv(AttnArgs a) {
   const int heads = __builtin_amdgcn_readfirstlane(part.first / per);  // in front of the part
   const At begin{kvh * a.group + heads, top - 32 * (part.first - heads * per)};
   At next = begin;
+  feed.seek(next.q0, nq, next.head * head_bytes);
   int load = 0, to = 0;
   auto issue = [&] {
-    feed.issue(ring + to * kTile, next.q0, load < steps ? nq : 0, next.head * head_bytes);
+    feed.issue(ring + to * kTile, load < steps);
     onward(next);
+    if (next.q0 == top)
+      feed.seek(top, nq, next.head * head_bytes);
+    else
+      feed.skip(-1);
     ++load;
     to = ring_next(to, role ? SB : SA);
   };
@@ -466,7 +480,7 @@ __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dkv(AttnArgs a) {
   auto active_at = [&] { return at.q0 < whi && at.q0 + 32 > wlo; };
   // X: p times dout, or ds times the queries, of the step in qa1, gb1, and the
   // scores, or dout v^T, of that in qa, gb
-  auto products = [&](bool sum, bool scores, int qa1, int gb1, int qa, int gb) {
+  auto products = [&](auto role, bool sum, bool scores, int qa1, int gb1, int qa, int gb) {
     const uint32_t v = base + (role ? qa1 : SA + gb1) * kTile, w = base + (role ? SA + gb : qa) * kTile;
     u32x4_t next[kAhead];
     if (sum)
@@ -518,57 +532,61 @@ __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dkv(AttnArgs a) {
 #pragma unroll
       for (int n = 0; n < NK; ++n) {
         const f32x4_t w = xp[(u * NK + n) * 64];
-        // (a masked query's dout v^T may be anything)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          s[u][n][i] = w[i] == 0.f ? 0.f : w[i] * (s[u][n][i] - __uint_as_float(st.v[u][i]));
+        for (int i = 0; i < 4; ++i) s[u][n][i] = w[i] * (s[u][n][i] - __uint_as_float(st.v[u][i]));
       }
     pack();
   };
 
-  if constexpr (phases(D)) {
-    int qa = 0, qa1 = SA - 1, gb = 0, gb1 = SB - 1;
-    bool now = false;
-    if (role) px_barrier();
-    for (int t = 0; t < steps; ++t) {
-      static_assert(kAheadA == kAheadB, "one wait for both");
-      __builtin_amdgcn_s_waitcnt(px_vm_wait((kAheadA - 1) * Feed::kLoads));
-      px_barrier();
-      const bool before = now;
-      now = active_at();
-      __builtin_amdgcn_s_setprio(1);
-      products(before, now, qa1, gb1, qa, gb);
-      __builtin_amdgcn_s_setprio(0);
-      px_barrier();
-      if (now && !role) weights();
-      if (now && role) slopes();
-      onward(at);
-      st = fetch(at, t + 1 < steps);  // in front of the loads, which then need not be waited for with it
-      issue();
-      qa1 = qa;
-      gb1 = gb;
-      qa = ring_next(qa, SA);
-      gb = ring_next(gb, SB);
+  auto run = [&](auto role) {
+    if constexpr (phases(D)) {
+      int qa = 0, qa1 = SA - 1, gb = 0, gb1 = SB - 1;
+      bool now = false;
+      if (role) px_barrier();
+      for (int t = 0; t < steps; ++t) {
+        static_assert(kAheadA == kAheadB, "one wait for both");
+        __builtin_amdgcn_s_waitcnt(px_vm_wait((kAheadA - 1) * Feed::kLoads));
+        px_barrier();
+        const bool before = now;
+        now = active_at();
+        __builtin_amdgcn_s_setprio(1);
+        products(role, before, now, qa1, gb1, qa, gb);
+        __builtin_amdgcn_s_setprio(0);
+        px_barrier();
+        if (now && !role) weights();
+        if (now && role) slopes();
+        onward(at);
+        st = fetch(at, t + 1 < steps);  // in front of the loads, which then need not be waited for with it
+        issue();
+        qa1 = qa;
+        gb1 = gb;
+        qa = ring_next(qa, SA);
+        gb = ring_next(gb, SB);
+      }
+      if (!role) px_barrier();
+      products(role, now, false, qa1, gb1, qa, gb);
+    } else {
+      int slot = 0;
+      for (int t = 0; t < steps; ++t) {
+        __builtin_amdgcn_s_waitcnt(px_vm_wait(0));
+        px_barrier();
+        issue();
+        const bool now = active_at();
+        products(role, false, now, slot, slot, slot, slot);
+        if (now && !role) weights();
+        px_barrier();
+        if (now && role) slopes();
+        onward(at);
+        st = fetch(at, t + 1 < steps);
+        products(role, now, false, slot, slot, slot, slot);
+        slot = ring_next(slot, SA);
+      }
     }
-    if (!role) px_barrier();
-    products(now, false, qa1, gb1, qa, gb);
-  } else {
-    int slot = 0;
-    for (int t = 0; t < steps; ++t) {
-      __builtin_amdgcn_s_waitcnt(px_vm_wait(0));
-      px_barrier();
-      issue();
-      const bool now = active_at();
-      products(false, now, slot, slot, slot, slot);
-      if (now && !role) weights();
-      px_barrier();
-      if (now && role) slopes();
-      onward(at);
-      st = fetch(at, t + 1 < steps);
-      products(now, false, slot, slot, slot, slot);
-      slot = ring_next(slot, SA);
-    }
-  }
+  };
+  if (role)
+    run(std::true_type{});
+  else
+    run(std::false_type{});
 
   const int64_t plane = (int64_t)a.Tk * a.Hk * D;
   float* const parts = a.part + (role ? a.split * plane : 0);
