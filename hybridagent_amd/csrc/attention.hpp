@@ -401,7 +401,10 @@ constexpr int attn_rows(int kernel, int D, bool low = false) {
   return D == 512 || (low && D > 64) ? 64 : D == 128 ? 192 : 128;
 }
 constexpr int attn_keys(int kernel, int D) { return kernel == kAttnForward && D < 256 ? 64 : 32; }
-constexpr int64_t kAttnParts = 512, kAttnChunk = 12, kAttnMostParts = 32, kAttnLow = 256;
+constexpr int64_t kAttnParts = 512, kAttnChunk = 12, kAttnMostParts = 32;
+// Forward: smaller tiles up to so many of the others and their heads (of 512 as many as
+// are ever split: the others' kernel has no registers left for that).
+constexpr int64_t attn_low(int64_t D) { return D == 512 ? kAttnParts : kAttnParts / 2; }
 
 // How many workgroups share a tile of `steps` steps over the other axis, and what
 // one of them has.  The first parts of all tiles go first: what has no part is last.

@@ -408,10 +408,12 @@ hipError_t fwd(AttnArgs a, hipStream_t s) {
   const dim3 grid((unsigned)(a.tiles * a.Hq * a.split));
   if (a.split == 1) {
     hipLaunchKernelGGL((k_attention<T, D, NQ, KT, PAIR, false>), grid, dim3(64 * kWaves), lds, s, a);
-  } else {
+  } else if constexpr (!PAIR || NQ == 1) {
     hipLaunchKernelGGL((k_attention<T, D, NQ, KT, PAIR, true>), grid, dim3(64 * kWaves), lds, s, a);
-    hipLaunchKernelGGL((k_attention_join<T, D, BQ, 32 * KT>), dim3((unsigned)(a.tiles * a.Hq), BQ * D / 1024 / kAttnJoin), dim3(256), 0,
-                       s, a);
+    hipLaunchKernelGGL((k_attention_join<T, D, BQ, 32 * KT>),
+                       dim3((unsigned)(a.tiles * a.Hq), BQ * D / 1024 / kAttnJoin), dim3(256), 0, s, a);
+  } else {
+    return hipErrorInvalidValue;
   }
   return hipGetLastError();
 }
@@ -447,7 +449,7 @@ AttnSplit attn_split(int kernel, int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, 
   // 108 -> 121 and 143 -> 142); of 256 they do not fit, and a step's latency alone
   // speaks for it (8 x 256 tokens 31 -> 27 and 44 -> 37; 2 x 1024 44 -> 54 and 59 -> 64).
   const int64_t even = other / std::max<int64_t>(B, 1), length = window > 0 ? std::min(even, window) : even;
-  r.low = kernel == kAttnForward ? (T / attn_rows(kernel, (int)D) + B + 1) * heads <= kAttnLow
+  r.low = kernel == kAttnForward ? (T / attn_rows(kernel, (int)D) + B + 1) * heads <= attn_low(D)
                                  : length <= (D == 128 ? 2048 : D == 256 ? 256 : 0);
   const int64_t rows = attn_rows(kernel, (int)D, r.low), keys = attn_keys(kernel, (int)D);
   if (B <= 0 || B > 64 || T <= 0 || other <= 0) return r;
