@@ -73,6 +73,13 @@ __device__ __forceinline__ float2* fwd_stats(const AttnArgs& a, int part, int64_
          ((int64_t)part * a.Hq + head) * a.Tq + token;
 }
 
+// Bound: the matrix units between the barriers.  A phase X of heads of 256 takes
+// 1450 cycles, of which 1024 are its 64 matrix instructions (its LDS reads as many,
+// free of bank conflicts; wider than two tiles of queries a wavefront there are no
+// registers); Y hides behind the other group's X.  2 x 4096 tokens, 16 heads, 8
+// key-value heads: heads of 64 110 us (626 TFLOP/s of the pairs seen), 128 138
+// (999), 256 235 (1171), 512 524 (1049); a product of 8192^3 reaches 1373.
+//
 // A workgroup has 16 NQ queries of a head per wavefront; PAIR: per pair of
 // wavefronts of a group, each with half of D: of the scores' sum, whose halves
 // they exchange through LDS between the phases, and of the output's columns.

@@ -17,6 +17,11 @@
 // values a lane loads the 8 x 8 block of its eight keys and eight columns, 256
 // bytes of a row per load, which 32 byte permutations turn around in its
 // registers.
+//
+// Bound: the cache's bytes.  64 sequences of 4000 keys, 8 key-value heads of 128: 183
+// us, 5.7 TB/s; of 2000 keys of 256 180 us, 5.8 (reads alone; a copy reaches 4.95); of
+// 64 x 4000 keys of 64 98 us, 5.4.  A few sequences: the first loads, one after the
+// other (length, page, keys), 5 us, and the join's launch.
 #include <algorithm>
 #include <type_traits>
 

@@ -9,7 +9,10 @@
 // backward, with g = dy turned back by the same angles and t = g w:
 //   dx = r (t - x r mean(t x r)),  dw = sum over rows of g x r
 //
-// Bound: memory (one read and one write of each row).  L lanes have a row, each
+// Bound: memory (one read and one write of each row; 8191 tokens of 32 heads of 256:
+// forward 58 us, 4.6 TB/s, where a copy reaches 4.95; backward 91 us, two reads and a
+// write, 4.4, and 8 for the join of the weights' partial rows; into the cache 4097
+// tokens of 16 + 2 + 2 heads of 512 35 us, 4.8).  L lanes have a row, each
 // two pieces of four elements: of the turned columns piece i and its partner R / 2
 // further, of the others neighbours, so that a pair never leaves its lane and an
 // angle is read once.  A wavefront takes kHnRows groups of 64 / L rows of one
