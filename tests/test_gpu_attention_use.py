@@ -277,21 +277,21 @@ def _chain(q, k, v, cos, sin, pos, slots, kc, vc, w, cu, table, lengths, dout):
     return [yq, out, one, *back]
 
 
-def _chain_inputs(seed=0, D=128):
-    lens = [150, 61]
+def _chain_inputs(seed=0, D=128, lens=(150, 61)):
     T = sum(lens)
     q, k, v = (ref.normal(seed + 1 + i, T, 4 if i == 0 else 2, D) for i in range(3))
-    cos, sin = rope_tables(160, D, device="cuda")
-    kc, vc, table, slots, lengths = _paged(lens, 2, D, 16, 20, 2)
+    cos, sin = rope_tables(max(lens) + 10, D, device="cuda")
+    kc, vc, table, slots, lengths = _paged(lens, 2, D, 16, T // 16 + 7, 2)
     kc.zero_(), vc.zero_()
     pos = torch.cat([torch.arange(n, device="cuda") for n in lens]).int()
     w = [ref.normal(8 + i, D, std=0.1, mean=1.0) for i in range(2)]
     return [q, k, v, cos, sin, pos, slots, kc, vc, w, ref.offsets(lens), table, lengths, ref.normal(seed + 20, T, 4, D)]
 
 
-def test_streams():
+@pytest.mark.parametrize("lens", [(150, 61), (1500, 700)])
+def test_streams(lens):
     """On a stream of its own behind work that makes the inputs, two such at once."""
-    args = [_chain_inputs(), _chain_inputs(50)]
+    args = [_chain_inputs(lens=lens), _chain_inputs(50, lens=lens)]
     want = [[t.clone() for t in _chain(*a)] for a in args]
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream() for _ in args]
@@ -306,10 +306,14 @@ def test_streams():
             _same(g, w)
 
 
-def test_captured_graphs():
-    """Two graphs of the whole chain from one pool, replayed in turn with new inputs and eager work between."""
+@pytest.mark.parametrize("lens", [(150, 61), (1500, 700)])
+def test_captured_graphs(lens):
+    """Two graphs of the whole chain from one pool, replayed in turn with new inputs and eager work between;
+    the longer ones' sums are shared by workgroups, through a workspace."""
+    lib, T = _lib.load(), sum(lens)
+    assert (lib.w4a16_attention_workspace_bytes(2, T, T, 4, 2, 128, 0) > 0) == (lens[0] == 1500)
     pool = torch.cuda.graph_pool_handle()
-    args = [_chain_inputs(), _chain_inputs(50)]
+    args = [_chain_inputs(lens=lens), _chain_inputs(50, lens=lens)]
     for a in args:
         _chain(*a)
     torch.cuda.synchronize()
