@@ -79,15 +79,18 @@ class PagedKVCache:
             raise RuntimeError(f"{need} pages are needed, {len(self._free)} are free")
         positions = [torch.empty(0, dtype=torch.int64)]
         slots = [torch.empty(0, dtype=torch.int64)]
+        grown = []
         for s, n in counts.items():
             at, pages = self._lengths[s], self._pages[s]
+            if len(pages) * size < at + n:
+                grown.append(s)
             while len(pages) * size < at + n:
                 pages.append(self._free.pop())
             new = torch.arange(at, at + n)
             positions.append(new)
             slots.append(torch.tensor(pages, dtype=torch.int64)[new // size] * size + new % size)
             self._lengths[s] = at + n
-        self._copy(counts)
+        self._copy(list(counts), grown)
         both = torch.stack((torch.cat(positions), torch.cat(slots))).to(self.lengths.device, torch.int32)
         return both[0], both[1]
 
@@ -109,18 +112,17 @@ class PagedKVCache:
             self._free.extend(reversed(self._pages[s]))
             self._pages[s] = []
             self._lengths[s] = 0
-        self._copy(sequences)
+        self._copy(list(sequences), list(sequences))
 
-    def _copy(self, sequences) -> None:
-        which = list(sequences)
-        if not which:
-            return
+    def _copy(self, lengths: list[int], tables: list[int]) -> None:
+        """The lengths and the rows of the table of these sequences, to the device."""
+        def rows(into: torch.Tensor, which: list[int], values: list) -> None:
+            if which:
+                into[torch.tensor(which).to(into.device)] = torch.tensor(values, dtype=torch.int32).to(into.device)
+
         width = self.block_table.shape[1]
-        rows = [self._pages[s] + [-1] * (width - len(self._pages[s])) for s in which]
-        device = self.lengths.device
-        at = torch.tensor(which).to(device)
-        self.block_table[at] = torch.tensor(rows, dtype=torch.int32).to(device)
-        self.lengths[at] = torch.tensor([self._lengths[s] for s in which], dtype=torch.int32).to(device)
+        rows(self.lengths, lengths, [self._lengths[s] for s in lengths])
+        rows(self.block_table, tables, [self._pages[s] + [-1] * (width - len(self._pages[s])) for s in tables])
 
 
 class Attention(nn.Module):
