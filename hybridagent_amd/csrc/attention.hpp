@@ -329,7 +329,9 @@ __device__ __forceinline__ void at_seen_keys(const AttnArgs& a, int nk, int off,
 // mask a tile's work grows with it, and what runs last should be short (more
 // sequences than lanes: one sequence after the other).  Behind the sequences the
 // rows past the last are one more (seq = n).  first, len: the sequence's rows;
-// offsets are held to 0 .. total, whatever the array says.
+// offsets are held to 0 .. total, whatever the array says.  The search takes 2000
+// cycles, which a sequence alone need not wait for (4096 tokens, 16 heads of 512: 273
+// -> 265 us).
 struct AtItem {
   int seq, level, tiles, first, len;
 };
@@ -351,7 +353,11 @@ __device__ __forceinline__ AtItem at_find(const int32_t* __restrict__ cu, int n,
       continue;
     }
     int at;
-    if (n < 64) {
+    if (n == 1) {
+      const int own = __builtin_amdgcn_readlane(tiles, 0);
+      at = rank < own ? 0 : 1;
+      it.level = at == 0 ? own - 1 - rank : rank - own;
+    } else if (n < 64) {
       // the highest level at or above which there are more than `rank` tiles
       int low = 0, high = (int)wave_max_u32((uint32_t)tiles);
       while (high - low > 1) {
