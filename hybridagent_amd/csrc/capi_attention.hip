@@ -17,7 +17,7 @@ inline int launch_status(hipError_t e) { return e == hipSuccess ? W4A16_OK : W4A
 
 constexpr int64_t kMaxTokens = (int64_t(1) << 24) - 1;
 constexpr int64_t kMaxHeads = 1024;
-constexpr int64_t kMaxSequences = 1 << 20;
+constexpr int64_t kMaxSequences = 1 << 14;  // every workgroup goes through their lengths
 constexpr int64_t kMaxBlocks = (int64_t(1) << 24) - 1;  // 256 threads each: a launch has 2^32 at most
 // bytes between two tokens, between two heads: a tile of 32 rows is addressed in 32 bits
 constexpr int64_t kMaxStride = int64_t(1) << 26;

@@ -510,10 +510,10 @@ W4A16_API int w4a16_append_kv(const void* q, int64_t q_token, int64_t q_head, co
  * scale q_i k_j over the keys that query i sees, query head h with key-value
  * head h / (Hq / Hk).  Sequence b has queries cu_q[b] .. cu_q[b + 1] - 1 and keys
  * cu_k[b] .. cu_k[b + 1] - 1 (int32 [B + 1], from 0 on, never falling; values
- * outside 0 .. Tq / Tk are held to them).  With nq queries and nk keys, query i
- * stands at i + nk - nq; causal: it sees keys up to there, and with window > 0
- * (causal only) the last `window` of these.  A query without keys, and every row
- * behind the last sequence, gets zeros (lse -inf).  lse (NULL: not wanted):
+ * outside 0 .. Tq / Tk are held to them; at most 16384 sequences).  With nq
+ * queries and nk keys, query i stands at i + nk - nq; causal: it sees keys up to
+ * there, and with window > 0 (causal only) the last `window` of these.  A query
+ * without keys, and every row behind the last sequence, gets zeros (lse -inf).  lse (NULL: not wanted):
  * float32 [Hq][Tq], log sum_j exp(scale q_i k_j).  D 64, 128, 256 or 512; bf16
  * or fp16; 16-byte aligned pointers.  The weights are rounded to the type as
  * operands of the second product.  The workspace (0 bytes where there are many
@@ -541,12 +541,12 @@ W4A16_API int w4a16_attention_backward(const void* dout, const void* q, int64_t 
                                        void* stream);
 
 /* Attention of one new token per sequence over the paged cache of
- * w4a16_append_kv: q, out [B][Hq][D], keys 0 .. lengths[b] - 1 of sequence b (the
- * last `window` of them where window > 0), key j in row j % page_size of page
- * block_table[b][j / page_size] (int32 [B][width]).  Lengths of zero and less
+ * w4a16_append_kv: q, out [B][Hq][D] (B at most 16384), keys 0 .. lengths[b] - 1
+ * of sequence b (the last `window` of them where window > 0), key j in row
+ * j % page_size of page block_table[b][j / page_size] (int32 [B][width]).  Lengths of zero and less
  * give zeros; a length over width * page_size, or a page outside the cache among
  * those that the token sees, gives NaN.  Entries of pages it does not see are
- * not read from.  `keys` of the workspace: width * page_size (few need none: 0 bytes). */
+ * not read from.  `keys` of the workspace: width * page_size (few: 0 bytes).  */
 W4A16_API size_t w4a16_decode_attention_workspace_bytes(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t keys);
 W4A16_API int w4a16_decode_attention(const void* q, int64_t q_token, int64_t q_head, const void* k_cache,
                                      int64_t k_page_stride, const void* v_cache, int64_t v_page_stride,

@@ -90,7 +90,7 @@ def _attn(lib, back=False, **kw):
 
 @pytest.mark.parametrize("back", [False, True])
 @pytest.mark.parametrize("kw,status", [
-    (dict(dtype=2), SHAPE), (dict(B=-1), SHAPE), (dict(B=(1 << 20) + 1), SHAPE), (dict(Tq=1 << 24), SHAPE),
+    (dict(dtype=2), SHAPE), (dict(B=-1), SHAPE), (dict(B=(1 << 14) + 1), SHAPE), (dict(Tq=1 << 24), SHAPE),
     (dict(Tk=-1), SHAPE), (dict(Hq=3), SHAPE), (dict(Hk=0), SHAPE), (dict(Hq=2048), SHAPE), (dict(D=96), SHAPE),
     (dict(D=1024), SHAPE), (dict(scale=0.0), SHAPE), (dict(scale=-1.0), SHAPE), (dict(scale=float("inf")), SHAPE),
     (dict(scale=float("nan")), SHAPE), (dict(window=-1), SHAPE), (dict(window=5, causal=0), SHAPE),
@@ -130,9 +130,9 @@ def test_decode_host_validation(lib):
                  bytes=need)
         return lib.w4a16_decode_attention(*{**a, **kw}.values(), NULL)
 
-    for kw in (dict(dtype=2), dict(B=-1), dict(B=BIG), dict(Hq=5), dict(D=80), dict(page=8), dict(page=48),
+    for kw in (dict(dtype=2), dict(B=-1), dict(B=(1 << 14) + 1), dict(B=BIG), dict(Hq=5), dict(D=80), dict(page=8), dict(page=48),
                dict(pages=0), dict(pages=1 << 28), dict(width=0), dict(width=1 << 28), dict(scale=0.0), dict(window=-1),
-               dict(kp=0), dict(vp=2 * 16 * 64 - 8), dict(qt=-8), dict(B=1 << 20, width=1 << 16)):
+               dict(kp=0), dict(vp=2 * 16 * 64 - 8), dict(qt=-8), dict(B=1 << 14, Hq=1024, Hk=1024, width=1 << 20, kp=1024 * 16 * 64, vp=1024 * 16 * 64)):
         assert call(**kw) == SHAPE, kw
     for name in ("q", "kc", "vc", "table", "lengths", "out"):
         assert call(**{name: NULL}) == ERR_NULL, name

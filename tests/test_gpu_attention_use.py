@@ -182,6 +182,21 @@ def test_many_sequences():
         ref.check(t, want[name], name)
 
 
+def test_the_most_sequences():
+    """16384 of one token each: its own value, and the gradient back."""
+    B, H, D = 1 << 14, 2, 64
+    q, k, v, dout = (ref.normal(i, B, H, D) for i in range(4))
+    cu = torch.arange(B + 1, device="cuda", dtype=torch.int32)
+    out, lse = _lib.attention(q, k, v, cu, return_lse=True)
+    assert torch.equal(out, v)
+    assert torch.equal(_lib.attention_backward(dout, q, k, v, out, lse, cu)[2], dout)
+    table = torch.arange(B, device="cuda", dtype=torch.int32)[:, None].repeat(1, 70)  # one sees only the first
+    caches = [t[:, :, None].expand(-1, -1, 16, -1).contiguous() for t in (k, v)]
+    ones = torch.ones(B, device="cuda", dtype=torch.int32)
+    for width in (1, 70):  # a workgroup of its own, and dealt
+        assert torch.equal(_lib.decode_attention(q, *caches, table[:, :width], ones), v)
+
+
 def test_offsets_outside_the_tensors():
     """They are held to them: nothing outside is read or written."""
     q, k, v, cu = _qkv([40, 30, 20], 4, 2, 64)
