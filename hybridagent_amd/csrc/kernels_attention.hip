@@ -261,7 +261,8 @@ __global__ __launch_bounds__(64 * kWaves, NQ == 1 && D <= 128 ? 4 : 2) void k_at
         const float t = at_max_over_c(top[n]);
         const bool first = at_sum_over_c(l[n]) == 0.f;
         const float up = t > (first ? -INFINITY : 0.f) ? t : 0.f;
-        const float f = __builtin_amdgcn_exp2f(-up);
+        // the first seen may lie far below zero: nothing is summed yet, and 0 x 2^-up would not be a number
+        const float f = first ? 1.f : __builtin_amdgcn_exp2f(-up);
         m[n] += up;
         l[n] *= f;
 #pragma unroll

@@ -1,0 +1,91 @@
+"""Attention at the ends of its numbers' ranges: scores far below zero, infinite keys and values, and
+fp16 where weights and slopes lie below its normal numbers; against 64 bits, as test_gpu_attention.py."""
+import pytest
+import torch
+
+import attention_reference as ref
+from hybridagent_amd import _lib
+from test_gpu_attention import _check, _inputs, _split
+
+pytestmark = pytest.mark.gpu
+
+BF, HF = torch.bfloat16, torch.float16
+
+
+@pytest.fixture(scope="module", autouse=True)
+def dev():
+    assert _lib.available(), "libw4a16moe.so must be built"
+    return torch.device("cuda:0")
+
+
+@pytest.fixture(autouse=True)
+def underflow(monkeypatch):
+    """The bounds know no end of fp32, and 64 bits keep a weight of e^-200.  fp32's normal numbers end at
+    2^-126 and what is below may be zero: a weight is off by 2^-126, and a slope, weight x (dout v - delta)
+    with magnitudes below 2^16 here, by 2^-110.  bf16 ends there too."""
+    fp16 = ref.least(HF)
+    monkeypatch.setattr(ref, "least", lambda dtype: fp16 if dtype == HF else 2.0 ** -110)
+
+
+# ---------------------------------------------------------------- scores far below zero
+
+# the score of key j beside a few units of noise: all low; the first steps low; falling; low blocks
+SHAPES = {
+    "all": lambda j, low: torch.full_like(j, low),
+    "first": lambda j, low: torch.where(j < 70, low, 4.0),
+    "falling": lambda j, low: low / 16 * j.clamp(max=64),
+    "blocks": lambda j, low: torch.where(j // 96 % 2 == 0, low, 2.0),
+}
+
+
+def _scored(lens_q, lens_k, Hq, Hk, D, dtype, shape, low):
+    """Inputs whose scores, at a scale of one, go by the key's place in its sequence."""
+    q, k, v, cu_q, cu_k, dout = _inputs(lens_q, lens_k, Hq, Hk, D, dtype, std=0.1)
+    j = torch.cat([torch.arange(n, device="cuda", dtype=torch.float64) for n in lens_k])
+    q[..., 0] = 1.0
+    k[..., 0] = SHAPES[shape](j, low).to(dtype)[:, None]
+    return q, k, v, cu_q, cu_k, dout
+
+
+@pytest.mark.parametrize("low", [-90.0, -200.0, -1000.0])
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_low_scores(D, shape, low):
+    lens = [1, 300, 33]
+    _check(*_scored(lens, lens, 4, 2, D, BF, shape, low), scale=1.0)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_low_scores_fp16(D):
+    lens = [1, 300, 33]
+    _check(*_scored(lens, lens, 4, 2, D, HF, "first", -200.0), scale=1.0)
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_low_scores_of_many_heads(D, shape):
+    """The larger tiles, which many heads take."""
+    lens = [300, 33]
+    _check(*_scored(lens, lens, 128, 2, D, BF, shape, -200.0), scale=1.0)
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_low_scores_of_shared_sums(D, shape):
+    """Every part of a tile begins with a maximum of its own."""
+    lens = [1500, 3, 900]
+    assert _split(lens, lens, 4, 1, D) == (True, True)
+    _check(*_scored(lens, lens, 4, 1, D, BF, shape, -200.0), scale=1.0)
+
+
+@pytest.mark.parametrize("window", [1, 16, 90])
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("D", [64, 256, 512])
+def test_low_scores_in_windows(D, shape, window):
+    lens = [300, 33]
+    _check(*_scored(lens, lens, 4, 2, D, BF, shape, -200.0), scale=1.0, window=window)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_low_scores_all_keys_seen(D):
+    _check(*_scored([5, 100], [205, 37], 4, 2, D, BF, "first", -200.0), scale=1.0, causal=False)
