@@ -228,8 +228,9 @@ __global__ __launch_bounds__(64 * kDaWaves, D == 512 ? 1 : 2) void k_decode_atte
         }
       if (__any(top > (l == 0.f ? -INFINITY : 8.f))) {
         const float t = at_max_over_c(top);
-        const float up = t > (at_sum_over_c(l) == 0.f ? -INFINITY : 0.f) ? t : 0.f;
-        const float f = __builtin_amdgcn_exp2f(-up);
+        const bool first = at_sum_over_c(l) == 0.f;
+        const float up = t > (first ? -INFINITY : 0.f) ? t : 0.f;
+        const float f = first ? 1.f : __builtin_amdgcn_exp2f(-up);  // (0 x 2^-up need not be a number)
         m += up;
         l *= f;
         s[0] -= up;

@@ -5,7 +5,7 @@ import torch
 
 import attention_reference as ref
 from hybridagent_amd import _lib
-from test_gpu_attention import _check, _inputs, _split
+from test_gpu_attention import _cache, _check, _inputs, _split
 
 pytestmark = pytest.mark.gpu
 
@@ -89,3 +89,37 @@ def test_low_scores_in_windows(D, shape, window):
 @pytest.mark.parametrize("D", [64, 128, 256, 512])
 def test_low_scores_all_keys_seen(D):
     _check(*_scored([5, 100], [205, 37], 4, 2, D, BF, "first", -200.0), scale=1.0, causal=False)
+
+
+def _decode_scored(lens, D, dtype, low_of, window=0, width=None, Hq=4, Hk=2, page=16):
+    """Decoding with keys whose scores, at a scale of one, are low_of(place, length)."""
+    kc, vc, table, lengths, keys, values = _cache(lens, Hk, D, page, dtype, width=width)
+    q = ref.normal(1, len(lens), Hq, D, dtype=dtype, std=0.1)
+    q[..., 0] = 1.0
+    for b, n in enumerate(lens):
+        j = torch.arange(n, device="cuda")
+        keys[b][..., 0] = low_of(j.double(), n).to(dtype)[:, None]
+        kc[table[b].long()[j // page], :, j % page] = keys[b]
+    out = _lib.decode_attention(q, kc, vc, table, lengths, scale=1.0, window=window)
+    for b, n in enumerate(lens):
+        want = ref.attend(q[b:b + 1], keys[b], values[b], 1.0, True, window, dtype)
+        ref.check(out[b:b + 1], want["out"], f"sequence {b} of {n}")
+
+
+@pytest.mark.parametrize("low", [-90.0, -200.0, -1000.0])
+@pytest.mark.parametrize("shape", [*SHAPES, "last"])
+@pytest.mark.parametrize("window", [0, 20])
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_decode_low_scores(D, window, shape, low):
+    """Tables on both sides of the width up to which a workgroup has all of a sequence's keys; "last":
+    the last key alone is low, in a wavefront of its own where the length is one more than 32."""
+    of = (lambda j, n: torch.where(j == n - 1, low, 10.0)) if shape == "last" else lambda j, n: SHAPES[shape](j, low)
+    limit = 128 * min(8, 1024 // D)
+    for width in (limit // 16, limit // 16 + 1):
+        _decode_scored([1, 33, 129, 181, 0, 32], D, BF, of, window=window, width=width)
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("D", [64, 512])
+def test_decode_low_scores_long(D, shape):
+    _decode_scored([9000, 3, 2500], D, HF, lambda j, n: SHAPES[shape](j, -200.0), Hq=8, Hk=1, page=64)
