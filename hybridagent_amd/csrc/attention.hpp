@@ -324,6 +324,12 @@ __device__ __forceinline__ void at_seen_keys(const AttnArgs& a, int nk, int off,
   lo = a.window > 0 ? max(0, first + off - a.window + 1) : 0;
 }
 
+// Whether query `q` sees a key at all.  One that does and has a sum of zero saw scores of
+// -infinity alone: its softmax is not a number.
+__device__ __forceinline__ bool at_sees(const AttnArgs& a, int nk, int off, int q) {
+  return nk > 0 && (!a.causal || q + off >= 0);
+}
+
 // The tile of `rows` rows that workgroup item `rank` has.  Tiles go by level,
 // the tiles of their sequence in front of them, the highest first: with a causal
 // mask a tile's work grows with it, and what runs last should be short (more

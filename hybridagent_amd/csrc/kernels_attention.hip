@@ -298,7 +298,7 @@ __global__ __launch_bounds__(64 * kWaves, NQ == 1 && D <= 128 ? 4 : 2) void k_at
   for (int n = 0; n < NQ; ++n) {
     const int q = q0 + 16 * n + r;
     l[n] = at_sum_over_c(l[n]);
-    const float f = !whole ? 1.f : l[n] == 0.f ? 0.f : 1.0f / l[n];
+    const float f = !whole ? 1.f : l[n] != 0.f ? 1.0f / l[n] : at_sees(a, nk, off, q) ? NAN : 0.f;
     if (c == 0 && half == 0 && q < nq) {
       if (!whole)
         *fwd_stats(a, part.index, it.first + q, at.head) = float2{l[n] == 0.f ? -INFINITY : m[n], l[n]};
@@ -342,7 +342,8 @@ __global__ __launch_bounds__(64 * kWaves, NQ == 1 && D <= 128 ? 4 : 2) void k_at
           max(lo, a.window > 0 ? q + off - a.window + 1 : 0), min(lo + kKeys * steps, min(nk, q + off + 1)) - 1,
           __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(m[n]), i)), half * (D / 2), [&](int d, float v) {
             if (whole)
-              *reinterpret_cast<uint16_t*>(out + q * out_row + 2 * d) = (uint16_t)at_pack2<T>(sum == 0.f ? 0.f : v / sum, 0.f);
+              *reinterpret_cast<uint16_t*>(out + q * out_row + 2 * d) =
+                  (uint16_t)at_pack2<T>(sum == 0.f && !at_sees(a, nk, off, q) ? 0.f : v / sum, 0.f);
             else
               fwd_part(a, part.index, it.first + q, at.head)[d] = v;
           });
@@ -394,7 +395,7 @@ __global__ __launch_bounds__(256) void k_attention_join(AttnArgs a) {
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     if (q0 + 256 / L * i >= nq) break;
-    const float f = l[i] == 0.f ? 0.f : 1.0f / l[i];
+    const float f = l[i] != 0.f ? 1.0f / l[i] : at_sees(a, nk, nk - nq, q0 + 256 / L * i) ? NAN : 0.f;
     *reinterpret_cast<u32x2_t*>(static_cast<unsigned char*>(a.out) + ((token[i] * a.Hq + at.head) * D + d) * 2) =
         u32x2_t{at_pack2<T>(v[i][0] * f, v[i][1] * f), at_pack2<T>(v[i][2] * f, v[i][3] * f)};
     // (no key at all: log2 0 is the least)

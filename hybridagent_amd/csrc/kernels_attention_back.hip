@@ -196,8 +196,9 @@ __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dq(AttnArgs a) {
         stat[n] = row_delta<T>(rows[n], out);
         if (part.index == 0 && c == 0 && q0 + 16 * n + r < nq) a.delta[(int64_t)head * a.Tq + q] = stat[n];
       } else {
-        // a query without keys: its scores are all masked
-        stat[n] = lse[q] == -INFINITY ? 0.f : -lse[q] * kLog2e;
+        // a query without keys: its scores are all masked (one whose scores are all -infinity
+        // has p not a number here, as in dk and dv)
+        stat[n] = lse[q] == -INFINITY && !at_sees(a, nk, off, (int)q - it.first) ? 0.f : -lse[q] * kLog2e;
       }
 #pragma unroll
       for (int d = 0; d < ND; ++d) acc[d][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};

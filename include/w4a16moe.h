@@ -513,7 +513,8 @@ W4A16_API int w4a16_append_kv(const void* q, int64_t q_token, int64_t q_head, co
  * outside 0 .. Tq / Tk are held to them; at most 16384 sequences).  With nq
  * queries and nk keys, query i stands at i + nk - nq; causal: it sees keys up to
  * there, and with window > 0 (causal only) the last `window` of these.  A query
- * without keys, and every row behind the last sequence, gets zeros (lse -inf).  lse (NULL: not wanted):
+ * without keys, and every row behind the last sequence, gets zeros (lse -inf); one
+ * whose scores are all -inf NaN (lse -inf).  lse (NULL: not wanted):
  * float32 [Hq][Tq], log sum_j exp(scale q_i k_j).  D 64, 128, 256 or 512; bf16
  * or fp16; 16-byte aligned pointers.  The weights are rounded to the type as
  * operands of the second product.  The workspace (0 bytes where there are many

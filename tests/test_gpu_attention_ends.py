@@ -1,5 +1,7 @@
 """Attention at the ends of its numbers' ranges: scores far below zero, infinite keys and values, and
 fp16 where weights and slopes lie below its normal numbers; against 64 bits, as test_gpu_attention.py."""
+import math
+
 import pytest
 import torch
 
@@ -123,3 +125,51 @@ def test_decode_low_scores(D, window, shape, low):
 @pytest.mark.parametrize("D", [64, 512])
 def test_decode_low_scores_long(D, shape):
     _decode_scored([9000, 3, 2500], D, HF, lambda j, n: SHAPES[shape](j, -200.0), Hq=8, Hk=1, page=64)
+
+
+# ---------------------------------------------------------------- scores that are minus infinity
+
+
+def _without_first(q, k, v, lens, scale, window):
+    """Each sequence's queries but the first over its keys but the first, in 64 bits: (rows, bounds)."""
+    cu = ref.offsets([n - 1 for n in lens])
+    kept = torch.cat([torch.arange(n - 1, device="cuda") + 1 + at for n, at in zip(lens, ref.offsets(lens).tolist())])
+    return kept, ref.packed(q[kept], k[kept], v[kept], cu, cu, scale, True, window)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("Hq,window", [(4, 0), (4, 1), (4, 40), (128, 0)])
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_infinite_key(D, Hq, window, dtype):
+    """The first key of a sequence is infinite and every query's score of it minus infinity: the query
+    that sees nothing else has no softmax, the others give it no weight."""
+    lens = [150, 1, 90]
+    q, k, v, cu, _, dout = _inputs(lens, lens, Hq, 2, D, dtype)
+    first = cu[:-1].long()
+    q[..., 0], k[first, :, 0] = -1.0, math.inf
+    out, lse = _lib.attention(q, k, v, cu, window=window, return_lse=True)
+    assert bool(out[first].isnan().all()) and bool((lse[:, first] == -math.inf).all())
+    kept, want = _without_first(q, k, v, lens, D ** -0.5, window)
+    ref.check(out[kept], want["out"], "out")
+    ref.check(lse[:, kept], want["lse"], "lse")
+    dq, dk, dv = _lib.attention_backward(dout, q, k, v, out, lse, cu, window=window)
+    for name, t in (("dq", dq), ("dk", dk), ("dv", dv)):
+        assert bool(t[first].isnan().all()), name
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_infinite_keys_of_shared_sums(D, causal):
+    """A sequence without one finite score, in parts; the others, and queries without keys, are as they were."""
+    lens_q, lens_k = [1500, 30, 900], [1500, 20, 900]
+    assert _split(lens_q, lens_k, 4, 1, D) == (True, True)
+    q, k, v, cu_q, cu_k, dout = _inputs(lens_q, lens_k, 4, 1, D, BF)
+    q[..., 0] = -1.0
+    want = ref.packed(q, k, v, cu_q, cu_k, D ** -0.5, causal, 0, dout)
+    k[:1500, :, 0] = math.inf
+    out, lse = _lib.attention(q, k, v, cu_q, cu_k, causal=causal, return_lse=True)
+    assert bool(out[:1500].isnan().all()) and bool((lse[:, :1500] == -math.inf).all())
+    grads = _lib.attention_backward(dout, q, k, v, out, lse, cu_q, cu_k, causal=causal)
+    for name, t, at in (("out", out, 1500), *zip(("dq", "dk", "dv"), grads, (1500, 1500, 1500))):
+        assert bool(t[:at].isnan().all()), name
+        ref.check(t[at:], tuple(x[at:] for x in want[name]), name)
