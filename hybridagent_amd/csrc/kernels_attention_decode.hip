@@ -291,7 +291,8 @@ __global__ __launch_bounds__(64 * kDaWaves, D == 512 ? 1 : 2) void k_decode_atte
     float* part = a.part + (int64_t)(2 * blockIdx.x + (pos == begin ? 0 : 1)) * (16 * (D + 2));
     // thread: columns 16 VW j + VW (4 c + i) .. of query r
     if (r < q_n) {
-      const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+      // a sum of zero: no keys, or scores of -infinity alone, whose softmax is not a number
+      const float inv = sum != 0.f ? 1.0f / sum : seq.len > 0 ? NAN : 0.f;
       for (int w = wave; w < NB * 4; w += kDaWaves) {
         const int j = w >> 2, i = w & 3;
         float v[VW];
@@ -315,7 +316,7 @@ __global__ __launch_bounds__(64 * kDaWaves, D == 512 ? 1 : 2) void k_decode_atte
         }
       }
       if (!whole && wave == 0 && c == 0) {
-        part[16 * D + r] = top;
+        part[16 * D + r] = sum == 0.f ? -INFINITY : top;  // (no maximum: it must not outweigh a lower one)
         part[16 * D + 16 + r] = sum;
       }
     }
@@ -375,7 +376,7 @@ __global__ __launch_bounds__(256) void k_decode_join(DecodeAttnArgs a) {
     v += *reinterpret_cast<const f32x4_t*>(&sv[i][d]);
     l += sl[i];
   }
-  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  const float inv = l != 0.f ? 1.0f / l : seq.len > 0 ? NAN : 0.f;
   *reinterpret_cast<u32x2_t*>(static_cast<unsigned char*>(a.out) +
                               ((int64_t)b * a.Hq + hk * a.group + q_first + q) * (D * 2) + 2 * d) =
       u32x2_t{at_pack2<T>(v[0] * inv, v[1] * inv), at_pack2<T>(v[2] * inv, v[3] * inv)};

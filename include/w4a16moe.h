@@ -545,8 +545,8 @@ W4A16_API int w4a16_attention_backward(const void* dout, const void* q, int64_t 
  * w4a16_append_kv: q, out [B][Hq][D] (B at most 16384), keys 0 .. lengths[b] - 1
  * of sequence b (the last `window` of them where window > 0), key j in row
  * j % page_size of page block_table[b][j / page_size] (int32 [B][width]).  Lengths of zero and less
- * give zeros; a length over width * page_size, or a page outside the cache among
- * those that the token sees, gives NaN.  Entries of pages it does not see are
+ * give zeros; a length over width * page_size, a page outside the cache among
+ * those that the token sees, or scores that are all -inf give NaN.  Entries of pages it does not see are
  * not read from.  `keys` of the workspace: width * page_size (few: 0 bytes).  */
 W4A16_API size_t w4a16_decode_attention_workspace_bytes(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t keys);
 W4A16_API int w4a16_decode_attention(const void* q, int64_t q_token, int64_t q_head, const void* k_cache,

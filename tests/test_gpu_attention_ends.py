@@ -173,3 +173,28 @@ def test_infinite_keys_of_shared_sums(D, causal):
     for name, t, at in (("out", out, 1500), *zip(("dq", "dk", "dv"), grads, (1500, 1500, 1500))):
         assert bool(t[:at].isnan().all()), name
         ref.check(t[at:], tuple(x[at:] for x in want[name]), name)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("window", [0, 20])
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_decode_infinite_keys(D, window, dtype):
+    """Keys whose scores are minus infinity have no weight: some of a wavefront's, all of one's, all of a
+    piece's; a token that sees no others has no softmax.  The finite scores are low: e^-200."""
+    lens, spoilt = [1, 33, 181, 300, 0, 9000, 2500], [1, 32, 181, 7, 0, 5000, 2500]
+    limit = 128 * min(8, 1024 // D)
+    for few, width in ((5, limit // 16), (5, limit // 16 + 1), (7, None)):
+        kc, vc, table, lengths, keys, values = _cache(lens[:few], 2, D, 16, dtype, width=width)
+        q = ref.normal(1, few, 4, D, dtype=dtype, std=0.1)
+        q[..., 0] = -1.0
+        for b, n in enumerate(lens[:few]):
+            j = torch.arange(n, device="cuda")
+            keys[b][..., 0] = torch.where(j < spoilt[b], math.inf, 200.0).to(dtype)[:, None]
+            kc[table[b].long()[j // 16], :, j % 16] = keys[b]
+        out = _lib.decode_attention(q, kc, vc, table, lengths, scale=1.0, window=window)
+        for b, n in enumerate(lens[:few]):
+            if n and spoilt[b] == n:
+                assert bool(out[b].isnan().all()), n
+                continue
+            rest = [t[b][spoilt[b]:] for t in (keys, values)]
+            ref.check(out[b:b + 1], ref.attend(q[b:b + 1], *rest, 1.0, True, window, dtype)["out"], f"sequence {b} of {n}")
