@@ -122,12 +122,14 @@ __device__ __forceinline__ HnTurn hn_turn(const HeadNormArgs& g, int t, const Hn
   if (bad) n.cos = n.sin = f32x4_t{NAN, NAN, NAN, NAN};
   return n;
 }
-__device__ __forceinline__ void hn_rotate(const HnTurn& n, float (&u)[8]) {
+// (Columns that are not turned are neighbours in u, not a pair: with a sine of zero one that is
+// not finite would make a finite one not a number.)
+__device__ __forceinline__ void hn_rotate(const HnTurn& n, bool turned, float (&u)[8]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float x = u[i], y = u[4 + i];
-    u[i] = x * n.cos[i] - y * n.sin[i];
-    u[4 + i] = y * n.cos[i] + x * n.sin[i];
+    u[i] = x * n.cos[i] - (turned ? y : 0.f) * n.sin[i];
+    u[4 + i] = y * n.cos[i] + (turned ? x : 0.f) * n.sin[i];
   }
 }
 
@@ -198,7 +200,7 @@ __global__ __launch_bounds__(256) void k_head_norm(HeadNormArgs a, int chunks) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) u[e] *= wv.get(e);
     }
-    if (kind != 2) hn_rotate(turn, u);
+    if (kind != 2) hn_rotate(turn, at.turned, u);
     if (!at.in || h >= heads) continue;
     const int n = row[i].head;
     void* o = kind == 0 ? a.yq : kind == 1 ? a.yk : a.yv;
@@ -262,7 +264,7 @@ __global__ __launch_bounds__(256) void k_head_norm_backward(HeadNormArgs a, int 
         g[e] = dy[i].get(e);
       }
       const float f = __frsqrt_rn(hn_sum<L>(sum) * over + a.eps);
-      if (kind != 2) hn_rotate(turn, g);
+      if (kind != 2) hn_rotate(turn, at.turned, g);
       float dot = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {

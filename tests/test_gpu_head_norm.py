@@ -165,3 +165,45 @@ def test_strides():
         got = _lib.head_norm_rope(*args, cos, sin, pos, qw, kw)
         assert all(torch.equal(a, b) for a, b in zip(got, want))
     assert math.isfinite(float(want[0].float().sum()))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, FF])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("D,R", [(64, 16), (96, 24), (512, 128), (512, 0), (8, 0)])
+def test_columns_behind_the_turned_ones(D, R, bad, dtype):
+    """A column that is not finite reaches its norm and its turned partner, no column beside it."""
+    q, k, v, cos, sin, pos, _, _ = _inputs(7, 3, 2, D, R, dtype, weights=False)
+    want = _lib.head_norm_rope(q, k, v, cos, sin, pos)
+    dys = [ref.normal(20 + i, *t.shape, dtype=dtype) for i, t in enumerate((q, k, v))]
+    back = _lib.head_norm_rope_backward(*dys, q, k, v, cos, sin, pos)
+    for at in sorted({R, R + 3, R + 4, D - 1}):
+        x, d = [t.clone() for t in (q, k)], [t.clone() for t in dys]
+        for t in (*x, *d[:2]):
+            t[2, 1, at] = bad
+        got = _lib.head_norm_rope(*x, v, cos, sin, pos)
+        grads = _lib.head_norm_rope_backward(*d, q, k, v, cos, sin, pos)
+        for a, b in (*zip(got[:2], want), *zip(grads[:2], back)):
+            b = b.clone()
+            b[2, 1, at] = bad
+            assert torch.equal(a.nan_to_num(nan=7.0), b.nan_to_num(nan=7.0)), at
+
+
+@pytest.mark.parametrize("dtype", [BF, FF])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_normed_columns_behind_the_turned_ones(dtype, bad):
+    """With weights: infinity over itself is not a number, a finite column over infinity zero; of the weights'
+    gradients the column alone."""
+    D, R, at = 64, 16, 33
+    q, k, v, cos, sin, pos, qw, kw = _inputs(7, 3, 2, D, R, dtype)
+    dys = [ref.normal(20 + i, *t.shape, dtype=dtype) for i, t in enumerate((q, k, v))]
+    *_, wq, wk = _lib.head_norm_rope_backward(*dys, q, k, v, cos, sin, pos, qw, kw)
+    d = [t.clone() for t in dys]
+    d[0][2, 1, at] = d[1][2, 1, at] = bad
+    *_, gq, gk = _lib.head_norm_rope_backward(*d, q, k, v, cos, sin, pos, qw, kw)
+    other = torch.arange(D, device="cuda") != at
+    for g, w in ((gq, wq), (gk, wk)):
+        assert not g[at].isfinite() and torch.equal(g[other], w[other])
+    x = q.clone()
+    x[2, 1, at] = bad
+    y = _lib.head_norm_rope(x, k, v, cos, sin, pos, qw, kw)[0][2, 1]
+    assert bool(y[at].isnan()) and bool((y[other].isnan() if bad != bad else y[other] == 0).all())
