@@ -50,11 +50,61 @@ constexpr int back_rows(int D, bool low) { return attn_rows(kAttnDq, D, low) / (
 constexpr int slots_a(int D) { return phases(D) ? 4 : 2; }
 constexpr int slots_b(int D) { return phases(D) ? 3 : 2; }
 // and bytes, with the exchange
-constexpr int back_lds(int D, int n) { return (slots_a(D) + slots_b(D)) * 64 * D + kPairs * n * 64 * (2 * 16 + 16); }
+constexpr int back_lds(int D, int n) { return (slots_a(D) + slots_b(D)) * 64 * D + kPairs * n * 64 * (2 * 16 + 16 + 4); }
 
 __device__ __forceinline__ int ring_next(int slot, int slots) { return slot == slots - 1 ? 0 : slot + 1; }
 
 }  // namespace
+
+// ds as an operand.  fp16 has numbers of 2^-24 .. 2^16 and ds follows dout's size, whatever that
+// is: rounded as it is, with dout of 3e-5 over 1500 keys elements of dq and dk were off by up to
+// 300 times their rounding, and above 65504 infinite.  So a column's ds carry a power of two, as a
+// softmax its maximum: the largest so far makes 2^7 or more of it, and when one exceeds 2^15 the
+// column's sums take a lower power.  What is then below fp16's numbers is 2^-32 of the largest.
+// (bf16 has fp32's range.)  The first power leaves fp32 room for any ds of fp16 numbers.
+template <typename T>
+constexpr bool kLift = std::is_same_v<T, _Float16>;
+constexpr float kFirstLift = 0x1p64f;
+// the power of two that takes `top` to 2^7 .. 2^8
+__device__ __forceinline__ float lift_for(float top) {
+  return __uint_as_float((uint32_t)(261 - max((int)(__float_as_uint(top) >> 23), 8)) << 23);
+}
+// Columns N0 .. N1 - 1 of ds at their powers: where one exceeds the bound all take lower
+// ones, the sums too.  True: powers changed.
+template <int N0, int N1, int ND, int N>
+__device__ __forceinline__ bool fit_slopes(f32x4_t (&s)[2][N], f32x4_t (&acc)[ND][N], float (&lift)[N]) {
+  float top[N];
+  bool over = false;
+#pragma unroll
+  for (int n = N0; n < N1; ++n) {
+    top[n] = 0.f;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top[n] = fmaxf(top[n], fabsf(s[u][n][i]));
+    over |= top[n] > 0x1p15f;
+  }
+  if (!__any(over)) return false;
+#pragma unroll
+  for (int n = N0; n < N1; ++n) {
+    const float t = at_max_over_c(top[n]), f = t > 0x1p15f ? lift_for(t) : 1.f;
+    lift[n] *= f;
+    s[0][n] *= f;
+    s[1][n] *= f;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) acc[d][n] *= f;
+  }
+  return true;
+}
+// the sums as they are, of sums with a power
+template <typename T, int ND, int N>
+__device__ __forceinline__ void unlift(f32x4_t (&acc)[ND][N], const float (&lift)[N]) {
+  if constexpr (kLift<T>)
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int d = 0; d < ND; ++d) acc[d][n] *= 1.0f / lift[n];
+}
 
 // delta of row r, in lane c's chunks of dout's row and out's
 template <typename T, int NI>
@@ -209,9 +259,19 @@ __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dq(AttnArgs a) {
   AtLane<D> ln;
   ln.init();
   ln.half_cols(role);
-  // the exchange: p [place][tile][n][lane], then ds [place][n][lane]
+  // the exchange: p [place][tile][n][lane], then ds [place][n][lane] and (fp16) its powers
   f32x4_t* const xp = reinterpret_cast<f32x4_t*>(smem + S * kTile) + place * 2 * NQ * 64 + lane;
   u32x4_t* const xd = reinterpret_cast<u32x4_t*>(smem + S * kTile) + (kPairs * 2 + place) * NQ * 64 + lane;
+  float* const xl = reinterpret_cast<float*>(smem + S * kTile + kPairs * 3 * NQ * 64 * 16) + place * NQ * 64 + lane;
+  float lift[NQ];
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    lift[n] = kFirstLift;
+    if (kLift<T> && role) {
+      stat[n] *= kFirstLift;
+      xl[n * 64] = kFirstLift;
+    }
+  }
   const uint32_t base = at_lds(smem);
   f32x4_t s[2][NQ];
   u32x4_t p[NQ];
@@ -258,19 +318,53 @@ __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dq(AttnArgs a) {
   };
   auto slopes = [&] {  // B
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
+    for (int n = 0; n < NQ; ++n)
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const f32x4_t w = xp[(u * NQ + n) * 64];
-        // (a masked key's weight is zero, and its row one of the sequence's own)
+        // (a masked key's weight is zero, and its row one of the sequence's own; delta
+        // has the column's power already)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[u][n][i] = w[i] * (s[u][n][i] - stat[n]);
+        for (int i = 0; i < 4; ++i)
+          s[u][n][i] = w[i] * (kLift<T> ? __builtin_fmaf(s[u][n][i], lift[n], -stat[n]) : s[u][n][i] - stat[n]);
       }
+    if constexpr (kLift<T>) {
+      float last[NQ];
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) last[n] = lift[n];
+      if (fit_slopes<0, NQ>(s, acc, lift)) {
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+          stat[n] *= lift[n] / last[n];
+          xl[n * 64] = lift[n];
+        }
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
       p[n] = at_pack8<T>(s[0][n], s[1][n]);
       xd[n * 64] = p[n];
     }
   };
   auto take = [&] {  // A: ds from B
+    if constexpr (kLift<T>) {
+      float now[NQ];
+      bool other = false;
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+        now[n] = xl[n * 64];
+        other |= now[n] != lift[n];
+      }
+      if (__any(other)) {
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+          const float f = now[n] / lift[n];
+          lift[n] = now[n];
+#pragma unroll
+          for (int d = 0; d < ND; ++d) acc[d][n] *= f;
+        }
+      }
+    }
 #pragma unroll
     for (int n = 0; n < NQ; ++n) p[n] = xd[n * 64];
   };
@@ -336,6 +430,7 @@ __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dq(AttnArgs a) {
   else
     run(std::false_type{});
 
+  unlift<T>(acc, lift);
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     const int q = q0 + 16 * n + r;
@@ -463,7 +558,18 @@ __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dkv(AttnArgs a) {
   at_settle(rows);
   AtLane<D> ln;
   ln.init();
-  f32x4_t* const xp = reinterpret_cast<f32x4_t*>(smem + S * kTile) + place * 2 * NK * 64 + lane;
+  // the exchange [place][lane]: p [tile][n], then (fp16) the powers of B's columns, for which
+  // heads of 256 have no registers over the steps
+  f32x4_t* const xp = reinterpret_cast<f32x4_t*>(smem + S * kTile) + place * 3 * NK * 64 + lane;
+  float* const xl = reinterpret_cast<float*>(xp + 2 * NK * 64);
+  constexpr bool kAway = kLift<T> && D == 256;
+  static_assert(NK <= 4, "in a lane's 16 bytes");
+  float lift[NK];
+#pragma unroll
+  for (int n = 0; n < NK; ++n) {
+    lift[n] = kFirstLift;
+    if (kAway && role) xl[n] = kFirstLift;
+  }
   const uint32_t base = at_lds(smem);
 
   // lse or delta of a lane's eight queries; past the last query zeros
@@ -534,16 +640,35 @@ __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dkv(AttnArgs a) {
       for (int n = 0; n < NK; ++n) xp[(u * NK + n) * 64] = s[u][n];
     pack();
   };
-  auto slopes = [&] {  // B
+  auto slope = [&](int n) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int u = 0; u < 2; ++u) {
+      const f32x4_t w = xp[(u * NK + n) * 64];
 #pragma unroll
-      for (int n = 0; n < NK; ++n) {
-        const f32x4_t w = xp[(u * NK + n) * 64];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[u][n][i] = w[i] * (s[u][n][i] - __uint_as_float(st.v[u][i]));
+      for (int i = 0; i < 4; ++i) {
+        s[u][n][i] = w[i] * (s[u][n][i] - __uint_as_float(st.v[u][i]));
+        if (kLift<T>) s[u][n][i] *= lift[n];
       }
-    pack();
+    }
+  };
+  auto slopes = [&] {  // B
+    if constexpr (kAway) {
+      auto away = [&](auto N0) {
+        constexpr int n = decltype(N0)::value;
+        lift[n] = xl[n];
+        slope(n);
+        if (fit_slopes<n, n + 1>(s, acc, lift)) xl[n] = lift[n];
+        p[n] = at_pack8<T>(s[0][n], s[1][n]);
+      };
+      away(std::integral_constant<int, 0>{});
+      if constexpr (NK > 1) away(std::integral_constant<int, 1>{});
+      static_assert(NK <= 2, "heads of 256");
+    } else {
+#pragma unroll
+      for (int n = 0; n < NK; ++n) slope(n);
+      if constexpr (kLift<T>) fit_slopes<0, NK>(s, acc, lift);
+      pack();
+    }
   };
 
   auto run = [&](auto role) {
@@ -596,6 +721,12 @@ __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dkv(AttnArgs a) {
   else
     run(std::false_type{});
 
+  if (role) {
+#pragma unroll
+    for (int n = 0; n < NK; ++n)
+      if (kAway) lift[n] = xl[n];
+    unlift<T>(acc, lift);
+  }
   const int64_t plane = (int64_t)a.Tk * a.Hk * D;
   float* const parts = a.part + (role ? a.split * plane : 0);
 #pragma unroll

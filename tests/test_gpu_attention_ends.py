@@ -198,3 +198,53 @@ def test_decode_infinite_keys(D, window, dtype):
                 continue
             rest = [t[b][spoilt[b]:] for t in (keys, values)]
             ref.check(out[b:b + 1], ref.attend(q[b:b + 1], *rest, 1.0, True, window, dtype)["out"], f"sequence {b} of {n}")
+
+
+# ---------------------------------------------------------------- fp16 below its normal numbers
+
+# fp16's normal numbers end at 2^-14 and all at 2^-24.  The bounds of these tests have every weight and slope
+# rounded by half a step of itself (``least`` zero), and the results' last rounding by 2^-25 besides.
+
+
+@pytest.fixture
+def relative(monkeypatch):
+    monkeypatch.setattr(ref, "least", lambda dtype: 0.0)
+
+
+@pytest.mark.parametrize("size", [3e-5, 1e-4, 1e-3, 1.0])
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_small_gradients_fp16(relative, D, size):
+    """dout of any size: the slopes' smallest are a weight of 1 / 1500 of it."""
+    lens = [1500, 40]
+    q, k, v, cu, _, dout = _inputs(lens, lens, 2, 1, D, HF)
+    dout = (dout.float() * size).half()
+    out, lse = _lib.attention(q, k, v, cu, return_lse=True)
+    want = ref.packed(q, k, v, cu, cu, D ** -0.5, True, 0, dout)
+    for name, t in zip(("dq", "dk", "dv"), _lib.attention_backward(dout, q, k, v, out, lse, cu)):
+        ref.check(t, want[name], name, slack=2.0 ** -25)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_large_gradients_fp16(relative, D):
+    """Slopes beyond fp16's 65504 whose sums it holds."""
+    lens = [70, 9]
+    q, k, v, cu, _, dout = _inputs(lens, lens, 4, 2, D, HF, std=0.2)
+    k, v, dout = k * 0.2, v * 8.0, dout * 2500.0
+    want = ref.packed(q, k, v, cu, cu, D ** -0.5, True, 0, dout)
+    assert max(float(want[n][0].abs().max()) for n in ("dq", "dk", "dv")) < 50000
+    out, lse = _lib.attention(q, k, v, cu, return_lse=True)
+    for name, t in zip(("dq", "dk", "dv"), _lib.attention_backward(dout, q, k, v, out, lse, cu)):
+        ref.check(t, want[name], name, slack=2.0 ** -25)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_gradients_of_unequal_rows_fp16(relative, D):
+    """Each query's gradient a size of its own, growing and falling along the sequence."""
+    lens = [700, 300]
+    q, k, v, cu, _, dout = _inputs(lens, lens, 4, 2, D, HF)
+    e = torch.cat([torch.linspace(-12, 6, 700, device="cuda"), torch.linspace(6, -12, 300, device="cuda")])
+    dout = (dout.float() * 2.0 ** e[:, None, None]).half()
+    out, lse = _lib.attention(q, k, v, cu, return_lse=True)
+    want = ref.packed(q, k, v, cu, cu, D ** -0.5, True, 0, dout)
+    for name, t in zip(("dq", "dk", "dv"), _lib.attention_backward(dout, q, k, v, out, lse, cu)):
+        ref.check(t, want[name], name, slack=2.0 ** -25)
