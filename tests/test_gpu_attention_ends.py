@@ -248,3 +248,19 @@ def test_gradients_of_unequal_rows_fp16(relative, D):
     want = ref.packed(q, k, v, cu, cu, D ** -0.5, True, 0, dout)
     for name, t in zip(("dq", "dk", "dv"), _lib.attention_backward(dout, q, k, v, out, lse, cu)):
         ref.check(t, want[name], name, slack=2.0 ** -25)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_gradient_of_values_of_many_keys_fp16(D):
+    """n equal weights: 1 / n is 20.5 of fp16's least steps.  dv is the gradients' sum over n, off by the roundings
+    of p and of itself; lse and the exponential add 2^-17 at most (log n is 13.6 and rounded to 2^-20)."""
+    n, m = 818400, 33
+    q = torch.zeros(m, 1, D, device="cuda", dtype=HF)
+    k, v = ref.normal(2, n, 1, D, dtype=HF), ref.normal(3, n, 1, D, dtype=HF)
+    dout = ref.normal(4, m, 1, D, dtype=HF, std=5.0, mean=60.0)
+    cu_q, cu_k = ref.offsets([m]), ref.offsets([n])
+    out, lse = _lib.attention(q, k, v, cu_q, cu_k, causal=False, return_lse=True)
+    _, _, dv = _lib.attention_backward(dout, q, k, v, out, lse, cu_q, cu_k, causal=False, needs=(False, False, True))
+    want = (dout.double().sum(0) / n)[None]
+    off = float(((dv.double() - want) / want).abs().max())
+    assert off <= 2 * ref.half_step(HF) + 2.0 ** -17, off
