@@ -69,6 +69,17 @@ __device__ __forceinline__ u32x4_t at_pack8(f32x4_t a, f32x4_t b) {
   return u32x4_t{at_pack2<T>(a[0], a[1]), at_pack2<T>(a[2], a[3]), at_pack2<T>(b[0], b[1]), at_pack2<T>(b[2], b[3])};
 }
 
+// The weights of a softmax as operands, by their exponents over a running maximum that moves
+// where one exceeds kOver, and then makes kTop of the largest.  bf16 has fp32's range.  fp16's
+// normal numbers are 2^-14 .. 2^15, the least steps 2^-24: the largest weight lies 2^11 high and
+// may grow to 2^15, so that one is off by 2^-36 of it at most, n keys' by n 2^-36 (2^24 keys:
+// half a rounding).  With 0 and 8, as in bf16, weights of 2^-25 were lost: a quarter of 2^16
+// such keys' in decoding, where one wavefront of four had the key above them.
+template <typename T>
+struct AtWeight {
+  static constexpr float kTop = std::is_same_v<T, __bf16> ? 0.f : 11.f, kOver = std::is_same_v<T, __bf16> ? 8.f : 15.f;
+};
+
 // over the four lanes of a column (c = 0 .. 3), each gets the result
 template <typename Op>
 __device__ __forceinline__ float at_over_c(float v, Op op) {

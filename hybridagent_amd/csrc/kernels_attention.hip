@@ -237,7 +237,7 @@ __global__ __launch_bounds__(64 * kWaves, NQ == 1 && D <= 128 ? 4 : 2) void k_at
       }
     }
     // The exponents, from the running maximum as it is.  It moves where one is
-    // above 8, so that the weights stay below 2^8 of the first; and to the first
+    // above kOver, so that the weights stay below 2^kOver; and to the first
     // that a query sees (a lane without a weight so far asks).
     float top[NQ];
     bool over = false;
@@ -253,12 +253,12 @@ __global__ __launch_bounds__(64 * kWaves, NQ == 1 && D <= 128 ? 4 : 2) void k_at
             s[k][u][n][i] = __builtin_fmaf(s[k][u][n][i], a.scale2, -m[n]);
             top[n] = fmaxf(top[n], s[k][u][n][i]);
           }
-      over |= top[n] > (l[n] == 0.f ? -INFINITY : 8.f);
+      over |= top[n] > (l[n] == 0.f ? -INFINITY : AtWeight<T>::kOver);
     }
     if (__any(over)) {
 #pragma unroll
       for (int n = 0; n < NQ; ++n) {
-        const float t = at_max_over_c(top[n]);
+        const float t = at_max_over_c(top[n]) - AtWeight<T>::kTop;
         const bool first = at_sum_over_c(l[n]) == 0.f;
         const float up = t > (first ? -INFINITY : 0.f) ? t : 0.f;
         // the first seen may lie far below zero: nothing is summed yet, and 0 x 2^-up would not be a number

@@ -264,3 +264,30 @@ def test_gradient_of_values_of_many_keys_fp16(D):
     want = (dout.double().sum(0) / n)[None]
     off = float(((dv.double() - want) / want).abs().max())
     assert off <= 2 * ref.half_step(HF) + 2.0 ** -17, off
+
+
+def _faint(n, D):
+    """One key with a score of 0 and n with one whose weight is 2^-25: as much as 1/128 together where n is
+    2^18.  (key, value, the result's first column): the one key's value is zero, the others' one."""
+    k = torch.zeros(n + 1, 1, D, device="cuda", dtype=HF)
+    k[1:, 0, 0] = 1.0
+    v = torch.ones(n + 1, 1, D, device="cuda", dtype=HF)
+    v[0] = 0.0
+    return k, v, n * 2.0 ** -25 / (1 + n * 2.0 ** -25)
+
+
+# the scale: 25 ln 2 is off by 2^-21 in fp32 at most, as are the products with log2 e, and so each weight by
+# 2^-19 of itself; their sum of n terms by n 2^-24 in the worst order, in tiles by far less: 2^-10 is allowed
+# for all and half a step of the result
+FAINT = 2.0 ** -10 + 2.0 ** -11
+
+
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_faint_weights_fp16(D):
+    n = 1 << 18
+    k, v, want = _faint(n, D)
+    q = torch.zeros(1, 1, D, device="cuda", dtype=HF)
+    q[..., 0] = -1.0
+    out = _lib.attention(q, k, v, ref.offsets([1]), ref.offsets([n + 1]), scale=25 * math.log(2.0))
+    off = float((out.double() / want - 1).abs().max())
+    assert off <= FAINT, off
