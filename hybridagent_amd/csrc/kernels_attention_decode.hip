@@ -217,7 +217,8 @@ __global__ __launch_bounds__(64 * kDaWaves, D == 512 ? 1 : 2) void k_decode_atte
             s[t][i] = key < seq.first || key >= seq.len ? -INFINITY : bad ? NAN : s[t][i];
           }
       }
-      // exponents from the running maximum as it is (as k_attention's)
+      // exponents from the running maximum as it is (as k_attention's, but for kTop, which
+      // is added last: heads of 512 have no register for it in the branch)
       float top = -INFINITY;
 #pragma unroll
       for (int t = 0; t < 2; ++t)
@@ -226,7 +227,7 @@ __global__ __launch_bounds__(64 * kDaWaves, D == 512 ? 1 : 2) void k_decode_atte
           s[t][i] = __builtin_fmaf(s[t][i], a.scale2, -m);
           top = fmaxf(top, s[t][i]);
         }
-      if (__any(top > (l == 0.f ? -INFINITY : 8.f))) {
+      if (__any(top > (l == 0.f ? -INFINITY : AtWeight<T>::kOver - AtWeight<T>::kTop))) {
         const float t = at_max_over_c(top);
         const bool first = at_sum_over_c(l) == 0.f;
         const float up = t > (first ? -INFINITY : 0.f) ? t : 0.f;
@@ -244,7 +245,7 @@ __global__ __launch_bounds__(64 * kDaWaves, D == 512 ? 1 : 2) void k_decode_atte
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          s[t][i] = __builtin_amdgcn_exp2f(s[t][i]);
+          s[t][i] = __builtin_amdgcn_exp2f(AtWeight<T>::kTop == 0.f ? s[t][i] : s[t][i] + AtWeight<T>::kTop);
           l += s[t][i];
         }
       const u32x4_t p = at_pack8<T>(s[0], s[1]);

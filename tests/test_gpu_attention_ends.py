@@ -291,3 +291,18 @@ def test_faint_weights_fp16(D):
     out = _lib.attention(q, k, v, ref.offsets([1]), ref.offsets([n + 1]), scale=25 * math.log(2.0))
     off = float((out.double() / want - 1).abs().max())
     assert off <= FAINT, off
+
+
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_decode_faint_weights_fp16(D):
+    """256 sequences of the same pages: a workgroup has all of one, and a wavefront of it the first key."""
+    n, page, B = (1 << 16) - 1, 1024, 256
+    k, v, want = _faint(n, D)
+    kc, vc = (t.view(-1, page, 1, D).transpose(1, 2).contiguous() for t in (k, v))
+    q = torch.zeros(B, 1, D, device="cuda", dtype=HF)
+    q[..., 0] = -1.0
+    table = torch.arange(kc.shape[0], device="cuda", dtype=torch.int32).expand(B, -1)
+    out = _lib.decode_attention(q, kc, vc, table, torch.full((B,), n + 1, device="cuda", dtype=torch.int32),
+                                scale=25 * math.log(2.0))
+    off = float((out.double() / want - 1).abs().max())
+    assert off <= FAINT, off
