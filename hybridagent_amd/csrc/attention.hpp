@@ -95,6 +95,26 @@ __device__ __forceinline__ float at_sum_over_c(float v) {
   return at_over_c(v, [](float x, float y) { return x + y; });
 }
 
+// over L lanes side by side, each gets the sum
+template <int L>
+__device__ __forceinline__ float at_sum_over(float v) {
+  auto add = [](float x, int y) { return x + __int_as_float(y); };
+  auto bits = [](float x) { return __float_as_int(x); };
+  v = add(v, __builtin_amdgcn_update_dpp(0, bits(v), 0xB1, 0xF, 0xF, false));   // quad [1,0,3,2]
+  v = add(v, __builtin_amdgcn_update_dpp(0, bits(v), 0x4E, 0xF, 0xF, false));   // quad [2,3,0,1]
+  v = add(v, __builtin_amdgcn_update_dpp(0, bits(v), 0x141, 0xF, 0xF, false));  // row_half_mirror
+  if constexpr (L >= 16) v = add(v, __builtin_amdgcn_update_dpp(0, bits(v), 0x140, 0xF, 0xF, false));  // row_mirror
+  if constexpr (L >= 32) {
+    const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+  }
+  if constexpr (L >= 64) {
+    const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+  }
+  return v;
+}
+
 // Two tiles side by side of a product's sums (lane: columns 4 c .. of row r), rounded,
 // as lane c's eight columns from at_pair_column(c) on: stores of 16 bytes, 64 of a row
 // together, take half the time of 8 as they lie.

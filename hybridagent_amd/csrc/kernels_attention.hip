@@ -2,6 +2,7 @@
 // a query sees, with grouped heads, sequences of any lengths packed one behind
 // the other, causal masks and windows (include/w4a16moe.h, w4a16_attention).
 #include <algorithm>
+#include <climits>
 #include <type_traits>
 
 #include "attention.hpp"
@@ -29,38 +30,161 @@ constexpr int fwd_slots(int D, int KT, int NQ) { return D == 256 || (D == 128 &&
 
 }  // namespace
 
-// A query's output (E columns from `at` on) once more, one key after the other: zero
-// times a value that is not finite is not a number, so in a matrix product a key's
-// value reaches the queries of its step that do not see it.  Rows that came out not
-// finite go through here (causal masks alone have such steps); a wavefront has a
-// row, lane l of it D / 64 columns.  Ends where every column is not a number.
+// Zero times a value that is not finite is not a number, so in a matrix product a key's value
+// reaches the queries of its step that do not see it.  Only steps with hidden keys do that, so a
+// column of a row can be wrong where one of the few hidden keys beside the row's own has such a
+// value in it: these are looked for once per wavefront whose rows did not come out finite, and
+// the columns summed again over the keys that the row sees.  A wavefront has a row, a lane of it
+// E / 64 columns.
+template <typename T>
+__device__ __forceinline__ bool not_finite(uint16_t x) {
+  constexpr uint16_t kExponent = std::is_same_v<T, __bf16> ? 0x7F80 : 0x7C00;
+  return (x & kExponent) == kExponent;
+}
+// a lane's E / 64 columns of a row of values
+template <int E>
+struct LaneValues {
+  static constexpr int kWords = E / 128 > 0 ? E / 128 : 1;
+  typedef __attribute__((ext_vector_type(kWords))) uint32_t words_t;
+  words_t w;
+  __device__ __forceinline__ void load(const unsigned char* p) {
+    if constexpr (E == 64)
+      w[0] = *reinterpret_cast<const uint16_t*>(p);
+    else
+      w = *reinterpret_cast<const words_t*>(p);
+  }
+  __device__ __forceinline__ uint16_t bits(int i) const { return (uint16_t)(w[i >> 1] >> (16 * (i & 1))); }
+};
+template <int E>
+struct HiddenValues {
+  int least[E / 64], most[E / 64];  // keys with such a value below the rows' keys, and above
+};
+// of the keys below .. below_end - 1 and above .. above_end - 1
+template <typename T, int E>
+__device__ __forceinline__ HiddenValues<E> hidden_values(const unsigned char* v, int64_t stride, int below, int below_end,
+                                                         int above, int above_end, int at) {
+  constexpr int VE = E / 64;
+  const unsigned char* const p = v + 2 * (at + VE * (int)opaque(threadIdx.x & 63));
+  HiddenValues<E> h;
+#pragma unroll
+  for (int i = 0; i < VE; ++i) {
+    h.least[i] = INT_MAX;
+    h.most[i] = -1;
+  }
+  LaneValues<E> x;
+#pragma unroll 4
+  for (int key = below; key < below_end; ++key) {
+    x.load(p + key * stride);
+#pragma unroll
+    for (int i = 0; i < VE; ++i) h.least[i] = not_finite<T>(x.bits(i)) ? min(h.least[i], key) : h.least[i];
+  }
+#pragma unroll 4
+  for (int key = above; key < above_end; ++key) {
+    x.load(p + key * stride);
+#pragma unroll
+    for (int i = 0; i < VE; ++i) h.most[i] = not_finite<T>(x.bits(i)) ? max(h.most[i], key) : h.most[i];
+  }
+  return h;
+}
+// A row to sum again: the keys from .. to that it sees, its maximum.
+struct AgainRow {
+  const unsigned char* q;
+  int from, to;
+  float m;
+};
+template <int E>
+__device__ __forceinline__ bool hidden_hits(const HiddenValues<E>& h, const AgainRow& r, int i) {
+  return h.least[i] < r.from || h.most[i] > r.to;
+}
+constexpr int kAgainRows = 4;
+// The columns of kAgainRows rows with a hidden value, over the keys that each sees, from the last
+// on in blocks of 64.  Ends where all of them are not finite by keys that their rows see, so
+// that values that are not finite throughout cost a block.  A block costs the latency of its
+// loads, 6 to 8 us for heads of 512, which is why rows go together.  store(row, column, sum).
 template <typename T, int D, int E, typename Store>
-__device__ __forceinline__ void attention_again(const AttnArgs& a, const unsigned char* q, const unsigned char* k,
-                                                const unsigned char* v, int from, int to, float m, int at,
-                                                const Store& store) {
-  const int lane = threadIdx.x & 63;
-  constexpr int QE = D / 64, VE = E / 64;
-  auto load = [](const unsigned char* p) { return at_lo<T>(*reinterpret_cast<const uint16_t*>(p)); };
-  float x[QE], acc[VE];
+__device__ __forceinline__ void attention_again(const AttnArgs& a, const HiddenValues<E>& hidden,
+                                                const AgainRow (&rows)[kAgainRows], const unsigned char* k,
+                                                const unsigned char* v, int at, const Store& store) {
+  const int lane = (int)opaque(threadIdx.x & 63);  // (no register is kept for what comes of it over the steps)
+  // L lanes have a key's row in turn, and lane i + L j of a block the key 64 / L i + j in the end;
+  // C, U: loads of keys, of values together
+  constexpr int VE = E / 64, L = D / 8, C = 8, U = 16, R = kAgainRows;
+  float acc[R][VE];
+  u32x4_t x[R];
+  int from = INT_MAX, to = -1;
 #pragma unroll
-  for (int i = 0; i < QE; ++i) x[i] = load(q + 2 * (64 * i + lane));
+  for (int r = 0; r < R; ++r) {
 #pragma unroll
-  for (int i = 0; i < VE; ++i) acc[i] = 0.f;
-  for (int key = from; key <= to; ++key) {
-    float s = 0.f;
+    for (int i = 0; i < VE; ++i) acc[r][i] = 0.f;
+    x[r] = ld16(rows[r].q + 16 * (lane % L));
+    if (rows[r].from <= rows[r].to) {
+      from = min(from, rows[r].from);
+      to = max(to, rows[r].to);
+    }
+  }
+  const unsigned char* const lowest = k + (to < 0 ? 0 : from) * a.k_stride + 16 * (lane % L);
+  const int64_t step = 64 / L * a.k_stride;
+  for (int last = to; last >= from; last -= 64) {
+    const int n = min(last - from + 1, 64);
+    float p[R];
 #pragma unroll
-    for (int i = 0; i < QE; ++i) s = __builtin_fmaf(x[i], load(k + key * a.k_stride + 2 * (64 * i + lane)), s);
-    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(wave_sum_f32(s), a.scale2, -m));
+    for (int r = 0; r < R; ++r) p[r] = 0.f;
+    const unsigned char* const first = lowest + (last - from - lane / L) * a.k_stride;
+    for (int i0 = 0; i0 < L; i0 += C) {
+      u32x4_t y[C];
 #pragma unroll
-    for (int i = 0; i < VE; ++i)
-      acc[i] = __builtin_fmaf(p, load(v + key * a.v_stride + 2 * (at + 64 * i + lane)), acc[i]);
+      for (int i = 0; i < C; ++i) {
+        const unsigned char* const key = first - (i0 + i) * step;
+        y[i] = ld16(key < lowest ? lowest : key);
+      }
+#pragma unroll
+      for (int i = 0; i < C; ++i)
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          float s = 0.f;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            s = __builtin_fmaf(at_lo<T>(x[r][w]), at_lo<T>(y[i][w]), s);
+            s = __builtin_fmaf(at_hi<T>(x[r][w]), at_hi<T>(y[i][w]), s);
+          }
+          s = at_sum_over<L>(s);
+          p[r] = lane % L == i0 + i ? s : p[r];
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[r], a.scale2, -rows[r].m));
+    const unsigned char* const columns = v + 2 * (at + VE * lane);
+    for (int j0 = 0; j0 < n; j0 += U) {
+      LaneValues<E> y[U];
+#pragma unroll
+      for (int j = 0; j < U; ++j) y[j].load(columns + max(last - j0 - j, from) * a.v_stride);
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const int of = j0 + j, key = last - of, owner = of % (64 / L) * L + of / (64 / L);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(p[r]), owner));
+          const bool seen = key >= rows[r].from && key <= rows[r].to;
+#pragma unroll
+          for (int i = 0; i < VE; ++i) {
+            const float sum = __builtin_fmaf(w, at_lo<T>(y[j].bits(i)), acc[r][i]);
+            acc[r][i] = seen ? sum : acc[r][i];
+          }
+        }
+      }
+    }
     bool more = false;
 #pragma unroll
-    for (int i = 0; i < VE; ++i) more |= acc[i] == acc[i];
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int i = 0; i < VE; ++i) more |= hidden_hits(hidden, rows[r], i) && __builtin_fabsf(acc[r][i]) < INFINITY;
     if (__ballot(more) == 0) break;
   }
 #pragma unroll
-  for (int i = 0; i < VE; ++i) store(at + 64 * i + lane, acc[i]);
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int i = 0; i < VE; ++i)
+      if (hidden_hits(hidden, rows[r], i)) store(r, at + VE * lane + i, acc[r][i]);
 }
 
 // Where a part of a split tile leaves a query's sums and (m, l), and the query's
@@ -327,26 +451,58 @@ __global__ __launch_bounds__(64 * kWaves, NQ == 1 && D <= 128 ? 4 : 2) void k_at
     odd[n] = __ballot(q < nq && zero != 0.f && l[n] == l[n]);  // a sum that is not: a seen key's score
   }
   if (!a.causal) return;
+  bool again = false;
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) again |= odd[n] != 0;
+  if (!again) return;
   __builtin_amdgcn_s_waitcnt(px_vm_wait(0));  // the rows' first stores are done
+  const int kvh = at.head / a.group;
+  const unsigned char* const kp = static_cast<const unsigned char*>(a.k) + k_first * a.k_stride + kvh * a.k_head;
+  const unsigned char* const vp = static_cast<const unsigned char*>(a.v) + k_first * a.v_stride + kvh * a.v_head;
+  // the keys that the rows' last and first see, and of the steps that the wavefront took
+  const int begin = max(lo, wlo - kKeys + 1), end = min(min(lo + kKeys * steps, hi), whi + kKeys - 1);
+  const int q_last = min(q0 + 16 * NQ, nq) - 1;
+  const HiddenValues<D / kHalves> hidden = hidden_values<T, D / kHalves>(
+      vp, a.v_stride, begin, a.window > 0 ? min(end, q_last + off - a.window + 1) : begin, max(begin, q0 + off + 1), end,
+      half * (D / 2));
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
-    unsigned long long rows = (odd[n] | odd[n] >> 16 | odd[n] >> 32 | odd[n] >> 48) & 0xFFFFull;
-    while (rows != 0) {
-      const int i = __ffsll(rows) - 1, q = q0 + 16 * n + i, kvh = at.head / a.group;
-      rows &= rows - 1;
-      const float sum = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(l[n]), i));
-      attention_again<T, D, D / kHalves>(
-          a, static_cast<const unsigned char*>(a.q) + at.head * a.q_head + (it.first + q) * a.q_stride,
-          static_cast<const unsigned char*>(a.k) + k_first * a.k_stride + kvh * a.k_head,
-          static_cast<const unsigned char*>(a.v) + k_first * a.v_stride + kvh * a.v_head,
-          max(lo, a.window > 0 ? q + off - a.window + 1 : 0), min(lo + kKeys * steps, min(nk, q + off + 1)) - 1,
-          __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(m[n]), i)), half * (D / 2), [&](int d, float v) {
-            if (whole)
-              *reinterpret_cast<uint16_t*>(out + q * out_row + 2 * d) =
-                  (uint16_t)at_pack2<T>(sum == 0.f && !at_sees(a, nk, off, q) ? 0.f : v / sum, 0.f);
-            else
-              fwd_part(a, part.index, it.first + q, at.head)[d] = v;
-          });
+    unsigned long long left = (odd[n] | odd[n] >> 16 | odd[n] >> 32 | odd[n] >> 48) & 0xFFFFull;
+    while (left != 0) {
+      AgainRow rows[kAgainRows];
+      int q[kAgainRows], r = 0;
+      float sum[kAgainRows];
+      while (left != 0 && r < kAgainRows) {
+        const int i = __ffsll(left) - 1;
+        left &= left - 1;
+        const int query = q0 + 16 * n + i;
+        const AgainRow row{static_cast<const unsigned char*>(a.q) + at.head * a.q_head + (it.first + query) * a.q_stride,
+                           max(lo, a.window > 0 ? query + off - a.window + 1 : 0),
+                           min(lo + kKeys * steps, min(nk, query + off + 1)) - 1,
+                           __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(m[n]), i))};
+        bool hit = false;
+#pragma unroll
+        for (int j = 0; j < D / kHalves / 64; ++j) hit |= hidden_hits(hidden, row, j);
+        if (__ballot(hit) == 0) continue;
+        // (the rest of the places: this one once more)
+        const float l1 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(l[n]), i));
+#pragma unroll
+        for (int j = 0; j < kAgainRows; ++j)
+          if (j >= r) {
+            rows[j] = row;
+            q[j] = query;
+            sum[j] = l1;
+          }
+        ++r;
+      }
+      if (r == 0) break;
+      attention_again<T, D, D / kHalves>(a, hidden, rows, kp, vp, half * (D / 2), [&](int j, int d, float v) {
+        if (whole)
+          *reinterpret_cast<uint16_t*>(out + q[j] * out_row + 2 * d) =
+              (uint16_t)at_pack2<T>(sum[j] == 0.f && !at_sees(a, nk, off, q[j]) ? 0.f : v / sum[j], 0.f);
+        else
+          fwd_part(a, part.index, it.first + q[j], at.head)[d] = v;
+      });
     }
   }
 }

@@ -83,26 +83,6 @@ __device__ __forceinline__ void hn_store(void* row, const HnPlace& p, const floa
   }
 }
 
-// over the L lanes of a row, each gets the sum
-template <int L>
-__device__ __forceinline__ float hn_sum(float v) {
-  auto add = [](float x, int y) { return x + __int_as_float(y); };
-  auto bits = [](float x) { return __float_as_int(x); };
-  v = add(v, __builtin_amdgcn_update_dpp(0, bits(v), 0xB1, 0xF, 0xF, false));   // quad [1,0,3,2]
-  v = add(v, __builtin_amdgcn_update_dpp(0, bits(v), 0x4E, 0xF, 0xF, false));   // quad [2,3,0,1]
-  v = add(v, __builtin_amdgcn_update_dpp(0, bits(v), 0x141, 0xF, 0xF, false));  // row_half_mirror
-  if constexpr (L >= 16) v = add(v, __builtin_amdgcn_update_dpp(0, bits(v), 0x140, 0xF, 0xF, false));  // row_mirror
-  if constexpr (L >= 32) {
-    const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = __uint_as_float(p[0]) + __uint_as_float(p[1]);
-  }
-  if constexpr (L >= 64) {
-    const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = __uint_as_float(p[0]) + __uint_as_float(p[1]);
-  }
-  return v;
-}
-
 // a lane's angles; not turned: cos 1, sin 0
 struct HnTurn {
   f32x4_t cos, sin;
@@ -189,7 +169,7 @@ __global__ __launch_bounds__(256) void k_head_norm(HeadNormArgs a, int chunks) {
       u[e] = x[i].get(e);
       sum = __builtin_fmaf(u[e], u[e], sum);
     }
-    sum = hn_sum<L>(sum);
+    sum = at_sum_over<L>(sum);
     const bool norm = kind == 2 ? a.v_norm : w != nullptr;
     const float f = norm ? __frsqrt_rn(sum / (float)a.D + a.eps) : 1.f;
 #pragma unroll
@@ -263,7 +243,7 @@ __global__ __launch_bounds__(256) void k_head_norm_backward(HeadNormArgs a, int 
         sum = __builtin_fmaf(xh[e], xh[e], sum);
         g[e] = dy[i].get(e);
       }
-      const float f = __frsqrt_rn(hn_sum<L>(sum) * over + a.eps);
+      const float f = __frsqrt_rn(at_sum_over<L>(sum) * over + a.eps);
       if (kind != 2) hn_rotate(turn, at.turned, g);
       float dot = 0.f;
 #pragma unroll
@@ -276,7 +256,7 @@ __global__ __launch_bounds__(256) void k_head_norm_backward(HeadNormArgs a, int 
         if (norm && kind != 2) g[e] *= kind == 0 ? wq.get(e) : wk.get(e);
         dot = __builtin_fmaf(g[e], xh[e], dot);
       }
-      dot = hn_sum<L>(dot) * over;
+      dot = at_sum_over<L>(dot) * over;
       if (norm) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) g[e] = f * (g[e] - xh[e] * dot);

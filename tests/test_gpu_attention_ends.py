@@ -1,6 +1,7 @@
 """Attention at the ends of its numbers' ranges: scores far below zero, infinite keys and values, and
 fp16 where weights and slopes lie below its normal numbers; against 64 bits, as test_gpu_attention.py."""
 import math
+import time
 
 import pytest
 import torch
@@ -306,3 +307,80 @@ def test_decode_faint_weights_fp16(D):
                                 scale=25 * math.log(2.0))
     off = float((out.double() / want - 1).abs().max())
     assert off <= FAINT, off
+
+
+# ---------------------------------------------------------------- values that are not finite, in number
+
+
+def _sprinkled(v, share, seed=9):
+    """v with a share of its elements not finite: the clean v, the spoilt one, where."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    bad = torch.rand(v.shape, generator=g, device="cuda") < share
+    kind = torch.randint(0, 3, v.shape, generator=g, device="cuda")
+    values = torch.tensor([math.nan, math.inf, -math.inf], device="cuda", dtype=v.dtype)[kind]
+    return v.masked_fill(bad, 0.0), torch.where(bad, values, v), bad
+
+
+def _hit(bad, lens_q, lens_k, g, window):
+    """Where a query sees such a value: [Tq, Hq, D]."""
+    res, k0 = [], 0
+    for n, m in zip(lens_q, lens_k):
+        seen = ref.seen_keys(n, m, True, window, "cuda").double()
+        res.append((seen @ bad[k0:k0 + m].double().flatten(1)).view(n, *bad.shape[1:]) > 0)
+        k0 += m
+    return torch.cat(res).repeat_interleave(g, 1)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("share", [0.0003, 0.05])
+@pytest.mark.parametrize("Hq,window", [(4, 0), (4, 1), (4, 40), (4, 130), (128, 0), (128, 40)])
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_many_values_that_are_not_finite(D, Hq, window, share, dtype):
+    lens_q, lens_k = [400, 33], [350, 90]
+    q, k, v, cu_q, cu_k, _ = _inputs(lens_q, lens_k, Hq, 2, D, dtype)
+    clean, v, bad = _sprinkled(v, share)
+    hit = _hit(bad, lens_q, lens_k, Hq // 2, window)
+    want, bound = ref.packed(q, k, clean, cu_q, cu_k, D ** -0.5, True, window)["out"]
+    out = _lib.attention(q, k, v, cu_q, cu_k, window=window)
+    assert not out[hit].isfinite().any()
+    ref.check(out.double().masked_fill(hit, 0.0), (want.masked_fill(hit, 0.0), bound), "out")
+
+
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_many_values_that_are_not_finite_in_shared_sums(D):
+    lens = [1500, 900]
+    assert _split(lens, lens, 4, 2, D)[0]
+    q, k, v, cu, _, _ = _inputs(lens, lens, 4, 2, D, BF)
+    clean, v, bad = _sprinkled(v, 0.0005)
+    hit = _hit(bad, lens, lens, 2, 0)
+    want, bound = ref.packed(q, k, clean, cu, cu, D ** -0.5, True, 0)["out"]
+    out = _lib.attention(q, k, v, cu)
+    assert not out[hit].isfinite().any()
+    ref.check(out.double().masked_fill(hit, 0.0), (want.masked_fill(hit, 0.0), bound), "out")
+
+
+@pytest.mark.parametrize("what", ["first", "all", "last", "one", "sparse"])
+@pytest.mark.parametrize("D", [64, 512])
+def test_values_that_are_not_finite_take_no_square_time(D, what):
+    """One key after the other for every query took 75 to 115 times as long: 30 times is allowed here."""
+    n = 8192
+    q, k, v, cu, _, _ = _inputs([n], [n], 2, 1, D, HF)
+    bad = v.clone()
+    at = {"first": slice(0, 1), "all": slice(None), "last": slice(-1, None), "one": slice(5000, 5001),
+          "sparse": slice(150, None, 301)}[what]
+    bad[at, 0, 7] = math.inf
+
+    def took(v):
+        best = math.inf
+        for _ in range(3):
+            torch.cuda.synchronize()
+            start = time.perf_counter()
+            _lib.attention(q, k, v, cu)
+            torch.cuda.synchronize()
+            best = min(best, time.perf_counter() - start)
+        return best
+
+    took(v)
+    fine, spoilt = took(v), took(bad)
+    print(f"{1e6 * fine:.0f} us, {1e6 * spoilt:.0f} us", flush=True)
+    assert spoilt < 30 * fine
