@@ -62,37 +62,57 @@ class PagedKVCache:
         return len(self._free)
 
     def length(self, sequence: int) -> int:
+        self._check(sequence)
         return self._lengths[sequence]
 
     def append(self, counts: dict[int, int]) -> tuple[torch.Tensor, torch.Tensor]:
         """Room for counts[s] new tokens of each sequence s -> (positions, slots), int32 on the device, of
         all new tokens, sequence after sequence in the order of ``counts``.  Raises, and takes nothing,
-        where the pages or the table do not suffice."""
-        size, need = self.page_size, 0
+        where the pages or the table do not suffice or a copy to the device fails."""
+        size, left = self.page_size, len(self._free)
+        self._check(*counts)
         for s, n in counts.items():
-            if not 0 <= s < len(self._lengths):
-                raise ValueError(f"no sequence {s}")
             if n < 0 or self._lengths[s] + n > self.longest:
                 raise ValueError(f"sequence {s} has {self._lengths[s]} tokens of {self.longest}: no room for {n}")
-            need += -(-(self._lengths[s] + n) // size) - len(self._pages[s])
-        if need > len(self._free):
-            raise RuntimeError(f"{need} pages are needed, {len(self._free)} are free")
+        grown: dict[int, list[int]] = {}
         positions = [torch.empty(0, dtype=torch.int64)]
         slots = [torch.empty(0, dtype=torch.int64)]
-        grown = []
         for s, n in counts.items():
             at, pages = self._lengths[s], self._pages[s]
-            if len(pages) * size < at + n:
-                grown.append(s)
-            while len(pages) * size < at + n:
-                pages.append(self._free.pop())
+            more = -(-(at + n) // size) - len(pages)
+            if more > 0:
+                left -= more
+                if left < 0:
+                    continue
+                pages = grown[s] = pages + self._free[left:left + more][::-1]
             new = torch.arange(at, at + n)
             positions.append(new)
             slots.append(torch.tensor(pages, dtype=torch.int64)[new // size] * size + new % size)
-            self._lengths[s] = at + n
-        self._copy(list(counts), grown)
+        if left < 0:
+            raise RuntimeError(f"{len(self._free) - left} pages are needed, {len(self._free)} are free")
         both = torch.stack((torch.cat(positions), torch.cat(slots))).to(self.lengths.device, torch.int32)
+        lengths = {s: self._lengths[s] + n for s, n in counts.items()}
+        self._copy(lengths, grown)
+        self._keep(lengths, grown)
+        del self._free[left:]
         return both[0], both[1]
+
+    def take_back(self, counts: dict[int, int]) -> None:
+        """The last counts[s] tokens of each sequence s off again, and the pages that held nothing else free:
+        what undoes an ``append`` whose keys and values were not written."""
+        self._check(*counts)
+        for s, n in counts.items():
+            if not 0 <= n <= self._lengths[s]:
+                raise ValueError(f"sequence {s} has {self._lengths[s]} tokens: {n} cannot be taken back")
+        shrunk: dict[int, list[int]] = {}
+        lengths = {s: self._lengths[s] - n for s, n in counts.items()}
+        for s in reversed(lengths):
+            pages, kept = self._pages[s], -(-lengths[s] // self.page_size)
+            if kept < len(pages):
+                self._free.extend(reversed(pages[kept:]))
+                shrunk[s] = pages[:kept]
+        self._keep(lengths, shrunk)
+        self._copy(lengths, shrunk)
 
     def rows(self, sequences) -> tuple[torch.Tensor, torch.Tensor]:
         """(block table, lengths) of the named sequences: the cache's own tensors where they are all, in
@@ -105,24 +125,31 @@ class PagedKVCache:
 
     def free(self, *sequences: int) -> None:
         """Gives the sequences' pages back; they start anew."""
+        self._check(*sequences)
+        self.take_back({s: self._lengths[s] for s in reversed(sequences)})
+
+    def _check(self, *sequences: int) -> None:
         for s in sequences:
             if not 0 <= s < len(self._lengths):
                 raise ValueError(f"no sequence {s}")
-        for s in sequences:
-            self._free.extend(reversed(self._pages[s]))
-            self._pages[s] = []
-            self._lengths[s] = 0
-        self._copy(list(sequences), list(sequences))
 
-    def _copy(self, lengths: list[int], tables: list[int]) -> None:
-        """The lengths and the rows of the table of these sequences, to the device."""
-        def rows(into: torch.Tensor, which: list[int], values: list) -> None:
-            if which:
-                into[torch.tensor(which).to(into.device)] = torch.tensor(values, dtype=torch.int32).to(into.device)
+    def _keep(self, lengths: dict[int, int], pages: dict[int, list[int]]) -> None:
+        for s, n in lengths.items():
+            self._lengths[s] = n
+        for s, p in pages.items():
+            self._pages[s] = p
+
+    def _copy(self, lengths: dict[int, int], pages: dict[int, list[int]]) -> None:
+        """These sequences' rows of the table and lengths, to the device: the lengths last, so that a
+        failure between the two leaves no length without its pages."""
+        def rows(into: torch.Tensor, values: dict) -> None:
+            if values:
+                at = torch.tensor(list(values)).to(into.device)
+                into[at] = torch.tensor(list(values.values()), dtype=torch.int32).to(into.device)
 
         width = self.block_table.shape[1]
-        rows(self.lengths, lengths, [self._lengths[s] for s in lengths])
-        rows(self.block_table, tables, [self._pages[s] + [-1] * (width - len(self._pages[s])) for s in tables])
+        rows(self.block_table, {s: p + [-1] * (width - len(p)) for s, p in pages.items()})
+        rows(self.lengths, lengths)
 
 
 class Attention(nn.Module):

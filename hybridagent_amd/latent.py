@@ -156,10 +156,13 @@ class LatentStack:
         for s in counts:
             if cache.length(s):
                 raise ValueError(f"sequence {s} has tokens already: a prompt starts a sequence")
+        def run():
+            ends = torch.tensor([0, *counts.values()]).cumsum(0).to(h.device, torch.int32)
+            return self._attended(h, lambda x, i: self.layers[i].attn.prompt(
+                x, positions, slots, ends, self.cos, self.sin, cache.k[i], cache.v[i]))
+
         positions, slots = cache.append(counts)
-        ends = torch.tensor([0, *counts.values()]).cumsum(0).to(h.device, torch.int32)
-        return self._attended(h, lambda x, i: self.layers[i].attn.prompt(
-            x, positions, slots, ends, self.cos, self.sin, cache.k[i], cache.v[i]))
+        return self._or_undone(cache, counts, run)
 
     def decode(self, h: torch.Tensor, cache: PagedKVCache, sequences: list[int]) -> torch.Tensor:
         """The layers on one new token of each named sequence, h [sequences, H] -> the residuals."""
@@ -167,10 +170,14 @@ class LatentStack:
         self._check(h, len(sequences))
         if len(set(sequences)) != len(sequences):
             raise ValueError("a sequence is named twice")
-        positions, slots = cache.append({s: 1 for s in sequences})
-        table, lengths = cache.rows(sequences)
-        return self._attended(h, lambda x, i: self.layers[i].attn.decode(
-            x, positions, slots, table, lengths, self.cos, self.sin, cache.k[i], cache.v[i]))
+        def run():
+            table, lengths = cache.rows(sequences)
+            return self._attended(h, lambda x, i: self.layers[i].attn.decode(
+                x, positions, slots, table, lengths, self.cos, self.sin, cache.k[i], cache.v[i]))
+
+        counts = {s: 1 for s in sequences}
+        positions, slots = cache.append(counts)
+        return self._or_undone(cache, counts, run)
 
     def latent(self, h: torch.Tensor, cache: PagedKVCache, sequences: list[int]) -> torch.Tensor:
         """``decode``, then HybridLink x sqrt(H): a latent step whose result is the next one's input."""
@@ -184,6 +191,17 @@ class LatentStack:
     def _check(self, h: torch.Tensor, tokens: int) -> None:
         if h.shape != (tokens, self.H):
             raise ValueError(f"h must be [{tokens}, {self.H}], got {list(h.shape)}")
+        if h.dtype != torch.bfloat16 or h.device != self.cos.device:
+            raise ValueError(f"h must be bfloat16 on {self.cos.device}, got {h.dtype} on {h.device}")
+
+    @staticmethod
+    def _or_undone(cache: PagedKVCache, counts: dict[int, int], run) -> torch.Tensor:
+        """run() on the tokens that the cache was given room for; where it raises they are none of its."""
+        try:
+            return run()
+        except BaseException:
+            cache.take_back(counts)
+            raise
 
     def _attended(self, h: torch.Tensor, attend) -> torch.Tensor:
         n = len(self.layers)
