@@ -118,6 +118,7 @@ class PagedKVCache:
         """(block table, lengths) of the named sequences: the cache's own tensors where they are all, in
         order, else copies."""
         which = list(sequences)
+        self._check(*which)  # (an index outside would end the process on the device)
         if which == list(range(len(self._lengths))):
             return self.block_table, self.lengths
         at = torch.tensor(which, dtype=torch.int64).to(self.lengths.device)

@@ -94,3 +94,16 @@ def test_residuals_of_another_kind(wrong):
         with pytest.raises(ValueError, match="bfloat16"):
             call()
         assert c.length(0) == 0 and c.free_pages == 8
+
+
+@pytest.mark.parametrize("which", [[-1], [3], [0, 3], [1, -4]])
+def test_rows_of_no_sequence(which):
+    c = _cache()
+    c.append({0: 3, 2: 5})
+    with pytest.raises(ValueError, match="no sequence"):
+        c.rows(which)
+    for s in which:
+        if not 0 <= s < 3:
+            with pytest.raises(ValueError, match="no sequence"):
+                c.length(s)
+    assert c.rows([2, 0])[1].tolist() == [5, 3]
