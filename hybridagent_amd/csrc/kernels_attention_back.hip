@@ -65,10 +65,12 @@ __device__ __forceinline__ int ring_next(int slot, int slots) { return slot == s
 template <typename T>
 constexpr bool kLift = std::is_same_v<T, _Float16>;
 constexpr float kFirstLift = 0x1p64f;
-// p as the operand of dv in fp16, at most 1, lies 2^15 higher: 1 / n of n equal weights is below
-// fp16's normal numbers from 16385 on (818400 of them: dv off by 2.5 %).  ds, made of it, too.
+// p as the operand of dv in fp16 lies 2^12 higher: 1 / n of n equal weights is below fp16's normal
+// numbers from 16385 on (818400 of them: dv off by 2.5 %), with 2^12 of no number of keys.  Not
+// higher: of scores of 10^7 fp32's roundings leave a p of one up to a few times as large, which must
+// stay below 65504.  ds, made of it, has the 2^12 too.
 template <typename T>
-constexpr float kWeightLift = kLift<T> ? 15.f : 0.f;
+constexpr float kWeightLift = kLift<T> ? 12.f : 0.f;
 // the power of two that takes `top` to 2^7 .. 2^8
 __device__ __forceinline__ float lift_for(float top) {
   return __uint_as_float((uint32_t)(261 - max((int)(__float_as_uint(top) >> 23), 8)) << 23);
@@ -730,7 +732,7 @@ __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dkv(AttnArgs a) {
 
 #pragma unroll
   for (int n = 0; n < NK; ++n) lift[n] = !role ? 1.f : kAway ? xl[n] : lift[n];
-  unlift<T>(acc, lift, 0x1p-15f);  // (kWeightLift)
+  unlift<T>(acc, lift, 0x1p-12f);  // (kWeightLift)
   const int64_t plane = (int64_t)a.Tk * a.Hk * D;
   float* const parts = a.part + (role ? a.split * plane : 0);
 #pragma unroll

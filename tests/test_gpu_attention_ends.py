@@ -384,3 +384,18 @@ def test_values_that_are_not_finite_take_no_square_time(D, what):
     fine, spoilt = took(v), took(bad)
     print(f"{1e6 * fine:.0f} us, {1e6 * spoilt:.0f} us", flush=True)
     assert spoilt < 30 * fine
+
+
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_gradients_of_huge_scores_fp16(D):
+    """Scores of 10^7, where fp32 leaves a weight of one a factor of 2^2: log2 e times them has a last place
+    of 2, and three such roundings of half a place lie between the forward pass' maximum and p.  dv, p dout
+    of one key, is that much and no infinity."""
+    q = torch.zeros(1, 1, D, device="cuda", dtype=HF)
+    q[..., 0] = 3600.0
+    for k0 in (2600.0, 2801.0, 3003.0, 3301.0, 3333.0):
+        k, v, dout = q * (k0 / 3600.0), torch.ones_like(q), torch.full_like(q, 100.0)
+        cu = ref.offsets([1])
+        out, lse = _lib.attention(q, k, v, cu, scale=1.0, return_lse=True)
+        dv = _lib.attention_backward(dout, q, k, v, out, lse, cu, scale=1.0)[2]
+        assert bool((out == 1).all()) and bool(((dv >= 12.5) & (dv <= 800.0)).all()), (k0, dv)
