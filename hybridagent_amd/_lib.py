@@ -1251,8 +1251,8 @@ def append_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tens
     out = _dense_like(q)
     yk, yv = (_dense_like(k), _dense_like(v)) if return_kv else (None, None)
     pc, ps, pp, pq, pk = at
-    _launch("w4a16_append_kv", index, load().w4a16_append_kv, *heads, pc, ps, pp, slots.data_ptr(), pq, pk, out.data_ptr(),
-            _ptr(yk), _ptr(yv), *cache, dt, bool(v_norm), *sizes, pages, page, eps)
+    _launch("w4a16_append_kv", index, load().w4a16_append_kv, *heads, pc, ps, pp, slots.data_ptr(), pq, pk,
+            out.data_ptr(), _ptr(yk), _ptr(yv), *cache, dt, bool(v_norm), *sizes, pages, page, eps)
     return (out, yk, yv) if return_kv else out
 
 
@@ -1299,7 +1299,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Ten
     multiple of Hk.  Sequence b has the queries ``cu_q[b] .. cu_q[b + 1] - 1`` and the keys of
     ``cu_k`` (int32, from 0 on; None: the same); its last query stands at its last key.  Causal: a
     query sees the keys up to where it stands, with ``window`` the last so many of them.  A query
-    that sees none, and rows behind the last sequence, are zero.  ``scale`` is D^-1/2 if None."""
+    that sees none, and rows behind the last sequence, are zero; one whose scores are all minus
+    infinity is NaN.  ``scale`` is D^-1/2 if None."""
     index = _gpu_of(q, k, v, cu_q, cu_k)
     dt, q, k, v, heads, cu_q, cu_k, sizes = _attention_args(q, k, v, cu_q, cu_k, scale, causal, window)
     out = _dense_like(q)
@@ -1307,7 +1308,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Ten
     lib = load()
     nbytes = lib.w4a16_attention_workspace_bytes(*sizes[:6], window)
     ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-    _launch("w4a16_attention", index, lib.w4a16_attention, *heads, cu_q.data_ptr(), cu_k.data_ptr(), out.data_ptr(), _ptr(lse), dt, *sizes, _ptr(ws), nbytes)
+    _launch("w4a16_attention", index, lib.w4a16_attention, *heads, cu_q.data_ptr(), cu_k.data_ptr(), out.data_ptr(),
+            _ptr(lse), dt, *sizes, _ptr(ws), nbytes)
     return (out, lse) if return_lse else out
 
 
@@ -1346,8 +1348,9 @@ def decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     q [B, Hq, D] of bf16 or fp16, any strides; k_cache, v_cache [pages, Hk, page size, D]; sequence
     b's key j lies in row j % page size of page ``block_table[b, j / page size]``; it has
     ``lengths[b]`` of them (both int32), of which the token sees the last ``window`` (0: all).  A
-    length of zero gives zeros; a length that the table does not cover, or a page that the cache
-    does not have, NaN."""
+    length of zero gives zeros; a length that the table does not cover, a page that the cache does
+    not have, or scores that are all minus infinity NaN.  Tables of few pages (heads of 128 and
+    less 1024 keys, 256 512, 512 256) take one launch and no workspace, whatever the lengths."""
     index = _gpu_of(q, k_cache, v_cache, block_table, lengths)
     dt = _head_type(q, "q", False)
     q, heads = _heads(q, "q")

@@ -160,7 +160,8 @@ class Attention(nn.Module):
         ``v_norm``);  ``o_proj`` of softmax(scale q k^T) v over the last ``window`` (0: all) tokens
 
     ``scale`` is head_size^-1/2 if None.  The tables ``cos`` and ``sin`` (``rope_tables``) are the caller's:
-    layers share them."""
+    layers share them.  The projections are torch's products: the library has no call of a product alone
+    (its own are part of the MLP's, HybridLink's and the experts' calls), and these must be differentiable."""
 
     def __init__(self, hidden_size: int, heads: int, kv_heads: int, head_size: int, window: int = 0,
                  scale: float | None = None, eps: float = 1e-6, v_norm: bool = True,

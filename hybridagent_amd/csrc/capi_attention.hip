@@ -296,7 +296,8 @@ int w4a16_attention_backward(const void* dout, const void* q, int64_t q_token, i
 
 size_t w4a16_decode_attention_workspace_bytes(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t keys) {
   if (B <= 0 || bad_group(Hq, Hk) || bad_attn_dim(D) || keys <= 0) return 0;
-  return decode_attn_whole(D, keys) ? 0 : decode_attn_part_floats(decode_attn_groups(B, Hq, Hk, D, keys), D) * sizeof(float);
+  if (decode_attn_whole(D, keys)) return 0;
+  return decode_attn_part_floats(decode_attn_groups(B, Hq, Hk, D, keys), D) * sizeof(float);
 }
 
 int w4a16_decode_attention(const void* q, int64_t q_token, int64_t q_head, const void* k_cache, int64_t k_page_stride,

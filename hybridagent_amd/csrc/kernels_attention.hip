@@ -61,8 +61,8 @@ struct HiddenValues {
 };
 // of the keys below .. below_end - 1 and above .. above_end - 1
 template <typename T, int E>
-__device__ __forceinline__ HiddenValues<E> hidden_values(const unsigned char* v, int64_t stride, int below, int below_end,
-                                                         int above, int above_end, int at) {
+__device__ __forceinline__ HiddenValues<E> hidden_values(const unsigned char* v, int64_t stride, int below,
+                                                         int below_end, int above, int above_end, int at) {
   constexpr int VE = E / 64;
   const unsigned char* const p = v + 2 * (at + VE * (int)opaque(threadIdx.x & 63));
   HiddenValues<E> h;
@@ -197,12 +197,16 @@ __device__ __forceinline__ float2* fwd_stats(const AttnArgs& a, int part, int64_
          ((int64_t)part * a.Hq + head) * a.Tq + token;
 }
 
-// Bound: the matrix units between the barriers.  A phase X of heads of 256 takes
+// Bound, heads of 256 and 512: the matrix units between the barriers.  A phase X of heads of 256 takes
 // 1450 cycles, of which 1024 are its 64 matrix instructions (its LDS reads as many,
 // free of bank conflicts; wider than two tiles of queries a wavefront there are no
-// registers); Y hides behind the other group's X.  2 x 4096 tokens, 16 heads, 8
-// key-value heads: heads of 64 110 us (626 TFLOP/s of the pairs seen), 128 138
-// (999), 256 235 (1171), 512 524 (1049); a product of 8192^3 reaches 1373.
+// registers); Y hides behind the other group's X.  Of 64 and 128 Y is the longer: a score
+// costs an fma, a maximum, an exponential, a sum and half a packing there, whatever D is,
+// and the matrix units are busy 0.30 and 0.45 of the CUs' cycles (256: 0.52).
+// 2 x 4096 tokens, 16 heads, 8 key-value heads: heads of 64 97-102 us (680 TFLOP/s of the
+// pairs seen), 128 132-138 (1030), 256 225-235 (1190), 512 502-524 (1070); a product of
+// 8192^3 reaches 1373.  A window of 1024 keys: 67, 88, 148, 288 us; all keys seen: 168,
+// 242, 412, 940.  fp16: 110, 145, 248, 530.
 //
 // A workgroup has 16 NQ queries of a head per wavefront; PAIR: per pair of
 // wavefronts of a group, each with half of D: of the scores' sum, whose halves
@@ -457,14 +461,15 @@ __global__ __launch_bounds__(64 * kWaves, NQ == 1 && D <= 128 ? 4 : 2) void k_at
   if (!again) return;
   __builtin_amdgcn_s_waitcnt(px_vm_wait(0));  // the rows' first stores are done
   const int kvh = at.head / a.group;
+  const unsigned char* const qp = static_cast<const unsigned char*>(a.q) + at.head * a.q_head;
   const unsigned char* const kp = static_cast<const unsigned char*>(a.k) + k_first * a.k_stride + kvh * a.k_head;
   const unsigned char* const vp = static_cast<const unsigned char*>(a.v) + k_first * a.v_stride + kvh * a.v_head;
   // the keys that the rows' last and first see, and of the steps that the wavefront took
   const int begin = max(lo, wlo - kKeys + 1), end = min(min(lo + kKeys * steps, hi), whi + kKeys - 1);
   const int q_last = min(q0 + 16 * NQ, nq) - 1;
-  const HiddenValues<D / kHalves> hidden = hidden_values<T, D / kHalves>(
-      vp, a.v_stride, begin, a.window > 0 ? min(end, q_last + off - a.window + 1) : begin, max(begin, q0 + off + 1), end,
-      half * (D / 2));
+  const int below = a.window > 0 ? min(end, q_last + off - a.window + 1) : begin, above = max(begin, q0 + off + 1);
+  const HiddenValues<D / kHalves> hidden =
+      hidden_values<T, D / kHalves>(vp, a.v_stride, begin, below, above, end, half * (D / 2));
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     unsigned long long left = (odd[n] | odd[n] >> 16 | odd[n] >> 32 | odd[n] >> 48) & 0xFFFFull;
@@ -476,8 +481,7 @@ __global__ __launch_bounds__(64 * kWaves, NQ == 1 && D <= 128 ? 4 : 2) void k_at
         const int i = __ffsll(left) - 1;
         left &= left - 1;
         const int query = q0 + 16 * n + i;
-        const AgainRow row{static_cast<const unsigned char*>(a.q) + at.head * a.q_head + (it.first + query) * a.q_stride,
-                           max(lo, a.window > 0 ? query + off - a.window + 1 : 0),
+        const AgainRow row{qp + (it.first + query) * a.q_stride, max(lo, a.window > 0 ? query + off - a.window + 1 : 0),
                            min(lo + kKeys * steps, min(nk, query + off + 1)) - 1,
                            __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(m[n]), i))};
         bool hit = false;
@@ -569,7 +573,8 @@ hipError_t fwd(AttnArgs a, hipStream_t s) {
   constexpr int lds = 2 * fwd_slots(D, KT, NQ) * KT * at_tile_bytes<D>() + (PAIR ? kWaves * 2 * KT * NQ * 64 * 16 : 0);
   static_assert(lds <= 160 * 1024, "a CU's LDS");
   constexpr int BQ = 16 * NQ * kWaves / (PAIR ? 2 : 1);
-  static_assert(BQ == attn_rows(kAttnForward, D, NQ == 1) && 32 * KT == attn_keys(kAttnForward, D), "attn_split's tiles");
+  static_assert(BQ == attn_rows(kAttnForward, D, NQ == 1), "attn_split's tiles");
+  static_assert(32 * KT == attn_keys(kAttnForward, D), "attn_split's steps");
   const dim3 grid((unsigned)(a.tiles * a.Hq * a.split));
   if (a.split == 1) {
     hipLaunchKernelGGL((k_attention<T, D, NQ, KT, PAIR, false>), grid, dim3(64 * kWaves), lds, s, a);
@@ -601,7 +606,10 @@ hipError_t fwd_type(const AttnArgs& a, bool low, hipStream_t s) {
 // steps at least (a part costs some 10 us of its own: its start, its sums to memory and
 // back).  4096 tokens, 8 heads and one key-value head of 128: dk and dv 1600 -> 217 us,
 // dq 182 -> 130, forward 116 -> 82; 2000 tokens, 4 heads of 256, a training step 581 ->
-// 131 us, with 8 steps at least 172, with 16 138.
+// 131 us, with 8 steps at least 172, with 16 138.  The host knows the sequences' number and
+// sum, not their lengths: tiles and chunks go by the mean, and a long sequence among short
+// ones has theirs.  Above 64 sequences, where at_find goes round the offsets, none are cut:
+// that was not tried.
 AttnSplit attn_split(int kernel, int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D, int64_t window) {
   AttnSplit r{false, 1, 1, 0};
   const bool dkv = kernel == kAttnDkv;
@@ -621,7 +629,10 @@ AttnSplit attn_split(int kernel, int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, 
   const int64_t tiles = T / rows + B + 1;
   // sequences of one length: their tiles, and a tile's steps
   const int64_t like = ((T / B + rows - 1) / rows) * B;
-  auto steps = [&](int64_t n) { return (((window > 0 && window < n ? std::min(n, window + rows) : n) + keys - 1) / keys + 1) * each; };
+  auto steps = [&](int64_t n) {
+    const int64_t seen = window > 0 && window < n ? std::min(n, window + rows) : n;
+    return ((seen + keys - 1) / keys + 1) * each;
+  };
   const int64_t work = like * heads * steps(other / B);
   const int64_t chunk = std::max<int64_t>(kAttnChunk, work / kAttnParts);
   const int64_t split =
@@ -629,7 +640,8 @@ AttnSplit attn_split(int kernel, int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, 
   if (split < 2) return r;
   r.split = (int)split;
   r.chunk = (int)chunk;
-  r.floats = dkv ? (size_t)(2 * split * Tk * Hk * D) : (size_t)(split * Tq * Hq * (D + (kernel == kAttnForward ? 2 : 0)));
+  r.floats = dkv ? (size_t)(2 * split * Tk * Hk * D)
+                 : (size_t)(split * Tq * Hq * (D + (kernel == kAttnForward ? 2 : 0)));
   return r;
 }
 

@@ -1,7 +1,8 @@
 // Gradients of the attention over packed prompts (include/w4a16moe.h,
 // w4a16_attention_backward).  With p = exp(scale q k^T - lse) over the seen keys:
 //
-//   delta = sum over d of dout out      (a query's)
+//   delta = sum over d of dout out      (a query's; of out as it was rounded: the forward
+//                                        pass keeps no other)
 //   dv = p^T dout, ds = p (dout v^T - delta), dq = scale ds k, dk = scale ds^T q
 //
 // in two launches: delta and dq, with a workgroup's queries in registers and the
@@ -30,10 +31,12 @@
 //
 // Bound: the phases.  Of heads of 256 dq's X takes 1500 cycles for 768 of matrix
 // instructions, dkv's as forward; of 64 and 128 Y, the exponentials and the exchange,
-// is the longer.  2 x 4096 tokens, 16 heads, 8 key-value heads, TFLOP/s of the three
-// products of dq, and of the four of dk and dv: heads of 64 161 us (639) and 266
-// (517), 128 243 (849) and 394 (698), 256 391 (1056) and 478 (1149), 512 947 (871)
-// and 1171 (939).
+// is the longer (matrix units busy 0.32 and 0.39 of the CUs' cycles in dq, 0.29 and 0.43 in
+// dkv).  2 x 4096 tokens, 16 heads, 8 key-value heads, TFLOP/s of the three products
+// of dq, and of the four of dk and dv: heads of 64 148 us (696) and 260 (528), 128 240
+// (859) and 395 (696), 256 383-396 (1060) and 475-490 (1140), 512 925-960 (875) and
+// 1130-1183 (950).  Of the five that the gradients cannot do without: 430, 550, 790 and
+// 660.  fp16 with its powers (below): 176 and 283, 261 and 411, 408 and 512, 970 and 1215.
 #include <type_traits>
 
 #include "attention.hpp"
@@ -50,7 +53,9 @@ constexpr int back_rows(int D, bool low) { return attn_rows(kAttnDq, D, low) / (
 constexpr int slots_a(int D) { return phases(D) ? 4 : 2; }
 constexpr int slots_b(int D) { return phases(D) ? 3 : 2; }
 // and bytes, with the exchange
-constexpr int back_lds(int D, int n) { return (slots_a(D) + slots_b(D)) * 64 * D + kPairs * n * 64 * (2 * 16 + 16 + 4); }
+constexpr int back_lds(int D, int n) {
+  return (slots_a(D) + slots_b(D)) * 64 * D + kPairs * n * 64 * (2 * 16 + 16 + 4);
+}
 
 __device__ __forceinline__ int ring_next(int slot, int slots) { return slot == slots - 1 ? 0 : slot + 1; }
 
@@ -166,8 +171,8 @@ __device__ __forceinline__ void back_store(const f32x4_t (&acc)[ND][N], int n, b
 // forward pass, are slower here: more parts, fewer tiles)
 constexpr int join_rows(int D) { return 1024 / D; }
 template <typename T, int D>
-__device__ __forceinline__ void back_join(const float* parts, int64_t plane, int n, int first, int row, int len, int heads,
-                                          int head, float scale, void* out) {
+__device__ __forceinline__ void back_join(const float* parts, int64_t plane, int n, int first, int row, int len,
+                                          int heads, int head, float scale, void* out) {
   constexpr int L = D / 4;
   const int i = row + threadIdx.x / L;
   if (i >= len) return;
@@ -459,8 +464,8 @@ __global__ __launch_bounds__(256) void k_attention_dq_join(AttnArgs a) {
   const int wg0 = it.level * BQ;
   const int parts = at_parts(a, at_key_span(a, nk, nk - it.len, wg0, BQ, it.len, 32).steps);
   if (parts > 1)
-    back_join<T, D>(a.part, (int64_t)a.Tq * a.Hq * D, parts, it.first, wg0 + join_rows(D) * (int)blockIdx.y, it.len, a.Hq, wg.head,
-                    a.scale, a.dq);
+    back_join<T, D>(a.part, (int64_t)a.Tq * a.Hq * D, parts, it.first, wg0 + join_rows(D) * (int)blockIdx.y, it.len,
+                    a.Hq, wg.head, a.scale, a.dq);
 }
 
 // The queries that some key of a tile of `rows` from wg0 on sees, in steps of 32 of
@@ -527,7 +532,8 @@ __global__ __launch_bounds__(kBackThreads, 2) void k_attention_dkv(AttnArgs a) {
   };
   Feed feed;
   if (role)
-    feed.init(static_cast<const unsigned char*>(a.dout) + (int64_t)q_first * a.Hq * D * 2, (int64_t)a.Hq * D * 2, place);
+    feed.init(static_cast<const unsigned char*>(a.dout) + (int64_t)q_first * a.Hq * D * 2, (int64_t)a.Hq * D * 2,
+              place);
   else
     feed.init(static_cast<const unsigned char*>(a.q) + q_first * a.q_stride, a.q_stride, place);
   const int64_t head_bytes = role ? D * 2 : a.q_head;
@@ -756,8 +762,9 @@ __global__ __launch_bounds__(256) void k_attention_dkv_join(AttnArgs a) {
   const int64_t plane = (int64_t)a.Tk * a.Hk * D;
   const bool keys = blockIdx.z != 0;
   if (parts > 1)
-    back_join<T, D>(a.part + (keys ? a.split * plane : 0), plane, parts, it.first, wg0 + join_rows(D) * (int)blockIdx.y, it.len, a.Hk,
-                    wg.head, keys ? a.scale : 1.f, keys ? a.dk : a.dv);
+    back_join<T, D>(a.part + (keys ? a.split * plane : 0), plane, parts, it.first,
+                    wg0 + join_rows(D) * (int)blockIdx.y, it.len, a.Hk, wg.head, keys ? a.scale : 1.f,
+                    keys ? a.dk : a.dv);
 }
 
 namespace {
@@ -768,8 +775,8 @@ void launch_dq(const AttnArgs& a, hipStream_t s) {
   hipLaunchKernelGGL((k_attention_dq<T, D, N>), dim3((unsigned)(a.tiles * a.Hq * a.split)), dim3(kBackThreads),
                      back_lds(D, N), s, a);
   if (a.split > 1)
-    hipLaunchKernelGGL((k_attention_dq_join<T, D, BQ>), dim3((unsigned)(a.tiles * a.Hq), BQ / join_rows(D)), dim3(256), 0,
-                       s, a);
+    hipLaunchKernelGGL((k_attention_dq_join<T, D, BQ>), dim3((unsigned)(a.tiles * a.Hq), BQ / join_rows(D)),
+                       dim3(256), 0, s, a);
 }
 template <typename T, int D, int N>
 void launch_dkv(const AttnArgs& a, hipStream_t s) {
@@ -777,8 +784,8 @@ void launch_dkv(const AttnArgs& a, hipStream_t s) {
   hipLaunchKernelGGL((k_attention_dkv<T, D, N>), dim3((unsigned)(a.tiles * a.Hk * a.split)), dim3(kBackThreads),
                      back_lds(D, N), s, a);
   if (a.split > 1)
-    hipLaunchKernelGGL((k_attention_dkv_join<T, D, BK>), dim3((unsigned)(a.tiles * a.Hk), BK / join_rows(D), 2), dim3(256),
-                       0, s, a);
+    hipLaunchKernelGGL((k_attention_dkv_join<T, D, BK>), dim3((unsigned)(a.tiles * a.Hk), BK / join_rows(D), 2),
+                       dim3(256), 0, s, a);
 }
 
 template <typename T, int D>
@@ -793,7 +800,8 @@ hipError_t back(AttnArgs a, hipStream_t s) {
     a.tiles = tokens / attn_rows(kernel, D, p.low) + a.B + 1;
   };
   if (a.Tq > 0 && a.dq == nullptr)
-    hipLaunchKernelGGL((k_attention_delta<T, D>), dim3((unsigned)(((int64_t)a.Tq * a.Hq + 63) / 64)), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((k_attention_delta<T, D>), dim3((unsigned)(((int64_t)a.Tq * a.Hq + 63) / 64)), dim3(256), 0, s,
+                       a);
   if (a.Tq > 0 && a.dq != nullptr) {
     plan(kAttnDq, a.Tq);
     a.low ? launch_dq<T, D, L>(a, s) : launch_dq<T, D, N>(a, s);

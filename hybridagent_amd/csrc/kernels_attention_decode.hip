@@ -144,7 +144,8 @@ __global__ __launch_bounds__(64 * kDaWaves, D == 512 ? 1 : 2) void k_decode_atte
     auto keys = [&](int key0, int page) {
       const unsigned char* p = kp + (page < 0 || page >= a.pages ? 0 : page) * a.k_page;
 #pragma unroll
-      for (int t = 0; t < 2; ++t) at_load_row<D / 32>(p, hold(key0 + 8 * (r >> 2) + 4 * t + (r & 3)) & mask, D * 2, kf[t]);
+      for (int t = 0; t < 2; ++t)
+        at_load_row<D / 32>(p, hold(key0 + 8 * (r >> 2) + 4 * t + (r & 3)) & mask, D * 2, kf[t]);
     };
 
     // The wavefront's keys of a step are key0 ..; the next ones' pages are read a step
@@ -411,7 +412,9 @@ hipError_t decode_type(const DecodeAttnArgs& a, hipStream_t s) {
 // Few steps: a workgroup has all of a (sequence, head)'s, without pieces and their join,
 // which cost about 4 us of both sides (181 keys, heads of 256: 16.7 -> 12.3 us a call;
 // 4 x 1000 keys of 128 16.2 -> 14.4; too many, 1000 keys of 256 16.6 -> 25.8, 512 of 512
-// 20.3 -> 29.1).
+// 20.3 -> 29.1).  "Few" is said of the table's width, which the host knows: a short sequence
+// in a wide table, or a window, is dealt out all the same (181 keys in a table for 8192: 14.0 us
+// where one of three pages takes 10.1).
 bool decode_attn_whole(int64_t D, int64_t keys) { return keys <= kDaStep * std::min<int64_t>(8, 1024 / D); }
 int decode_attn_groups(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t keys) {
   if (decode_attn_whole(D, keys)) return (int)(B * Hk * ((Hq / Hk + 15) / 16));

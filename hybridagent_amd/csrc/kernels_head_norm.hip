@@ -11,8 +11,9 @@
 //
 // Bound: memory (one read and one write of each row; 8191 tokens of 32 heads of 256:
 // forward 58 us, 4.6 TB/s, where a copy reaches 4.95; backward 91 us, two reads and a
-// write, 4.4, and 8 for the join of the weights' partial rows; into the cache 4097
-// tokens of 16 + 2 + 2 heads of 512 35 us, 4.8).  L lanes have a row, each
+// write, 4.4, and 8 for the join of the weights' partial rows; fp32, twice the bytes,
+// 102 and 181 with the join; into the cache 4097 tokens of 16 + 2 + 2 heads of 512 35 us,
+// 4.8, and 2 more with dense keys and values for the prompt).  L lanes have a row, each
 // two pieces of four elements: of the turned columns piece i and its partner R / 2
 // further, of the others neighbours, so that a pair never leaves its lane and an
 // angle is read once.  A wavefront takes kHnRows groups of 64 / L rows of one
@@ -187,7 +188,8 @@ __global__ __launch_bounds__(256) void k_head_norm(HeadNormArgs a, int chunks) {
     if (!PAGED || o != nullptr)
       hn_store<T>(static_cast<T*>(o) + ((int64_t)t * (kind == 0 ? a.Hq : a.Hk) + n) * a.D, at, u);
     if (PAGED && kept && kind != 0) {
-      unsigned char* to = static_cast<unsigned char*>(kind == 1 ? a.kc : a.vc) + page * (kind == 1 ? a.k_page : a.v_page);
+      unsigned char* to =
+          static_cast<unsigned char*>(kind == 1 ? a.kc : a.vc) + page * (kind == 1 ? a.k_page : a.v_page);
       hn_store<T>(to + ((int64_t)n * a.page + (slot - page * a.page)) * a.D * sizeof(T), at, u);
     }
   }

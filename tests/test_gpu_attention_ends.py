@@ -198,7 +198,8 @@ def test_decode_infinite_keys(D, window, dtype):
                 assert bool(out[b].isnan().all()), n
                 continue
             rest = [t[b][spoilt[b]:] for t in (keys, values)]
-            ref.check(out[b:b + 1], ref.attend(q[b:b + 1], *rest, 1.0, True, window, dtype)["out"], f"sequence {b} of {n}")
+            want = ref.attend(q[b:b + 1], *rest, 1.0, True, window, dtype)
+            ref.check(out[b:b + 1], want["out"], f"sequence {b} of {n}")
 
 
 # ---------------------------------------------------------------- fp16 below its normal numbers
