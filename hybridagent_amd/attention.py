@@ -19,13 +19,15 @@ def rope_tables(positions: int, columns: int, theta: float = 10000.0, device: to
                 frequencies: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """(cos, sin) float32 [positions, columns / 2] of position x frequency, ``frequencies`` (a vector of
     columns / 2; zero: the pair stays as it is) theta^(-2 i / columns) if None.  The angles are taken in
-    64 bits: in 32, one near 100,000 is off by 0.004."""
+    64 bits: in 32, one near 100,000 is off by 0.004.  ``device`` is the frequencies' if None."""
     if columns % 2 or columns < 0:
         raise ValueError(f"columns must be even, got {columns}")
     if frequencies is None:
         frequencies = theta ** (-torch.arange(0, columns, 2, dtype=torch.float64, device=device) / max(columns, 1))
     elif frequencies.shape != (columns // 2,):
         raise ValueError(f"frequencies must be [{columns // 2}], got {list(frequencies.shape)}")
+    elif device is None:
+        device = frequencies.device
     angle = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * frequencies.to(device, torch.float64)
     return angle.cos().float(), angle.sin().float()
 

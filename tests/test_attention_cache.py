@@ -107,3 +107,11 @@ def test_rows_of_no_sequence(which):
             with pytest.raises(ValueError, match="no sequence"):
                 c.length(s)
     assert c.rows([2, 0])[1].tolist() == [5, 3]
+
+
+def test_rope_tables_of_frequencies_elsewhere():
+    """Without a device the tables are where the frequencies are."""
+    f = torch.ones(4, device="meta")
+    assert all(t.device == f.device and t.shape == (7, 4) for t in attention.rope_tables(7, 8, frequencies=f))
+    assert attention.rope_tables(7, 8, frequencies=torch.ones(4))[0].device.type == "cpu"
+    assert attention.rope_tables(7, 8, device="cpu", frequencies=torch.ones(4, dtype=torch.float64))[1].shape == (7, 4)
