@@ -34,14 +34,13 @@ constexpr int fwd_slots(int D, int KT, int NQ) { return D == 256 || (D == 128 &&
 // reaches the queries of its step that do not see it.  Only steps with hidden keys do that, so a
 // column of a row can be wrong where one of the few hidden keys beside the row's own has such a
 // value in it: these are looked for once per wavefront whose rows did not come out finite, and
-// the columns summed again over the keys that the row sees.  A wavefront has a row, a lane of it
-// E / 64 columns.
+// the columns summed again over the keys that the row sees.
 template <typename T>
 __device__ __forceinline__ bool not_finite(uint16_t x) {
   constexpr uint16_t kExponent = std::is_same_v<T, __bf16> ? 0x7F80 : 0x7C00;
   return (x & kExponent) == kExponent;
 }
-// a lane's E / 64 columns of a row of values
+// a lane's E / 64 columns, side by side, of a row of values
 template <int E>
 struct LaneValues {
   static constexpr int kWords = E / 128 > 0 ? E / 128 : 1;
@@ -99,8 +98,8 @@ __device__ __forceinline__ bool hidden_hits(const HiddenValues<E>& h, const Agai
 constexpr int kAgainRows = 4;
 // The columns of kAgainRows rows with a hidden value, over the keys that each sees, from the last
 // on in blocks of 64.  Ends where all of them are not finite by keys that their rows see, so
-// that values that are not finite throughout cost a block.  A block costs the latency of its
-// loads, 6 to 8 us for heads of 512, which is why rows go together.  store(row, column, sum).
+// that values that are not finite throughout cost a block.  Rows go together for the loads'
+// sake (8192 keys of heads of 512, a block: one row 8.4 us, four 23).  store(row, column, sum).
 template <typename T, int D, int E, typename Store>
 __device__ __forceinline__ void attention_again(const AttnArgs& a, const HiddenValues<E>& hidden,
                                                 const AgainRow (&rows)[kAgainRows], const unsigned char* k,
